@@ -22,7 +22,8 @@ SOURCES = ["qgemm_gemv.hip", "qgemm_mlp.hip", "qgemm_tile_q4k.hip", "qgemm_tile_
            "qgemm_skinny_q6k.hip", "qgemm_skinny_q80.hip", "qgemm_skinny_q5k.hip", "qgemm_skinny_q4k.hip",
            "qgemm_skinny_q41.hip", "qgemm_skinny_q40.hip", "qgemm_tile_q40.hip", "qgemm_tile_q41.hip",
            "qgemm_tile_q80.hip", "qgemm_skinny.hip", "qgemm_tile.hip", "qgemm_api.hip", "qgemm_pack.hip", "qgemm_noalloc.hip",
-           "q_gemm_dequant_primitive.cpp", "synth.cpp", "gguf.cpp", "act.hip", "linear.cpp"]
+           "paged_attn_bf16.hip", "paged_attn_f16.hip", "paged_attn_bf16_e4m3.hip", "paged_attn_f16_e4m3.hip", "paged_attn.hip",
+           "paged_table.hip", "lora.hip", "q_gemm_dequant_primitive.cpp", "synth.cpp", "gguf.cpp", "act.hip", "linear.cpp"]
 BENCH_SOURCES = ["bench_probe.hip"]
 COMMON = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-Wall",
           # packed fp32 VALU ops are kept out of the device code

@@ -1,0 +1,413 @@
+// Decode attention over a paged key-value cache: one new token per row.
+//
+//   o[h] = sum_t p_t v[t] / sum_t p_t,   p_t = exp(scale q[h] . k[t] - m),   m the running maximum
+//
+// in one pass over keys and values.  The heads that share a kv head (up to 16 of them) are the
+// columns of the matrix instructions, so a key or value is read once for all of them:
+//   S^T[32 tokens, 16 heads] = K Q^T        rows of K from memory straight into A operands
+//   O^T[dim, 16 heads]      += V^T P^T      V^T by exchanging 16-bit halves between registers
+// Which token a row of the first product stands for is free: row 4 b + i of its half hh is token
+// 8 b + 4 hh + i, so the scores that a lane holds (heads across lanes, rows 4 g .. 4 g + 3 for lane
+// group g) are those of tokens 8 g .. 8 g + 7, which is what the second product wants in that lane
+// as its operand: P never leaves the registers, and the softmax's factors are one value per lane.
+// P is split in two 16-bit parts, hi + lo: with one part its rounding (2^-9 in bf16) would be as
+// large as the output's own.  A second product costs matrix cycles that the kernel, bound by
+// memory, has to spare.
+//
+// The work is cut evenly: the tiles (32 tokens) of all rows and kv heads, in one sequence, are
+// dealt to the wavefronts of the launch in equal contiguous runs.  A run that covers a row's
+// whole (row, kv head) writes the output; others leave (m, sum, unnormalized o) in the workspace,
+// at most two per wavefront, for the join kernel.  Lengths are read on the device, nothing of the
+// launch depends on them.
+#pragma once
+#include "mfma16.h"
+#include "paged_internal.h"
+
+namespace mlxr {
+namespace paged {
+
+constexpr int kTile = 32;     // tokens
+constexpr int kWaves = 4;     // of a workgroup
+constexpr int kHeads = 16;    // columns of the products
+
+struct AttnArgs {
+  const uint8_t *k, *v;  // element addresses in bytes
+  const float *k_scale, *v_scale;
+  int64_t k_page, k_head, k_token, v_page, v_head, v_token;  // strides, bytes
+  const uint16_t* q;
+  int64_t q_row, q_head;  // elements
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  void* out;
+  float* lse;
+  float* ws;        // partials
+  int32_t* prefix;  // [rows + 1] tiles before each row, for the join
+  int rows, heads, kv_heads, group, groups;  // groups: of 16 heads, of a kv head
+  int dim, page, page_shift, pages, width, window, out_dtype;
+  int part_rows, workers;
+  float scale;  // times log2(e)
+};
+
+// Tokens [first, len) of row r; the first tile starts at base.
+struct Span {
+  int first, base, len, tiles;
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int r) {
+  Span s;
+  const int64_t most = (int64_t)a.width * a.page;
+  const int n = a.lens[r];
+  s.len = n < 0 ? 0 : n > most ? (int)most : n;
+  s.first = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
+  s.base = s.first & ~7;  // a block of eight tokens lies in one page where page % 8 == 0
+  s.tiles = (s.len - s.base + kTile - 1) / kTile;
+  return s;
+}
+
+// Partial of slot `slot` of worker w: part_rows rows of dim floats, then m and sum of each.
+__host__ __device__ constexpr int partial_floats(int part_rows, int dim) { return part_rows * dim + (2 * part_rows + 3) / 4 * 4; }
+__device__ __forceinline__ float* partial(const AttnArgs& a, int w, int slot) {
+  return a.ws + ((int64_t)w * 2 + slot) * partial_floats(a.part_rows, a.dim);
+}
+__device__ __forceinline__ int64_t tiles_per_worker(const AttnArgs& a, int64_t total) {
+  return (total + a.workers - 1) / a.workers;
+}
+
+// Two e4m3 values (half `h` of w) as two 16-bit floats: exact in either type.
+template <bool F16, bool H>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+  if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, H));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, H));
+}
+
+// F16: the products' type (else bf16).  F8: the cache is e4m3.  DT: 64, 128 or 256, at least dim (DIM:
+// equal).  P8: page_size % 8 == 0.
+template <bool F16, bool F8, int DT, bool DIM, bool P8>
+struct Attn {
+  static constexpr int KS = DT / 32;               // steps of the first product
+  static constexpr int VE = DT == 64 ? 4 : 8;      // neighbouring values of a token that a lane loads
+  static constexpr int VH = DT / (16 * VE);        // times that
+  static constexpr int NC = DT / 16;               // accumulators
+  // p times 2^14 in f16: weights down to 2^-28 of the largest stay normal numbers (bf16 has the range)
+  static constexpr float SHIFT = F16 ? 14.f : 0.f;
+  static constexpr float UNSHIFT = F16 ? 0x1p-14f : 1.f;
+  static constexpr int KL = F8 ? KS / 2 : KS;      // 16-byte loads of a key row by a lane
+
+  const AttnArgs& a;
+  const int lane, col, g;
+  u32x4_t q[KS];
+  u32x4_t kr[2][KL];
+  uint32_t vr[VH][8][F8 ? VE / 4 : VE / 2];
+  f32x4_t o[NC];
+  float m, l, sc;
+  const uint8_t *kh, *vh;
+  const int32_t* trow;
+
+  __device__ Attn(const AttnArgs& a_) : a(a_), lane(threadIdx.x & 63), col(lane & 15), g(lane >> 4) {}
+
+  // First element of the k-th operand of step j that lane group g holds, as in the keys' loads.
+  __device__ __forceinline__ int dim_of(int j) const {
+    return F8 ? (j >> 1) * 64 + g * 16 + (j & 1) * 8 : j * 32 + g * 8;
+  }
+
+  __device__ __forceinline__ void start(int r, int kvh, int grp) {
+    const int h = grp * kHeads + col;
+    const bool ok = h < a.group;
+    const uint16_t* p = a.q + (int64_t)r * a.q_row + (int64_t)(kvh * a.group + (ok ? h : 0)) * a.q_head;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      const int d = dim_of(j);
+      q[j] = ok && (DIM || d < a.dim) ? *(const u32x4_t*)(p + d) : u32x4_t{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[c] = f32x4_t{0, 0, 0, 0};
+    m = -INFINITY;
+    l = 0.f;
+    sc = a.scale * (a.k_scale ? a.k_scale[kvh] : 1.f);
+    kh = a.k + (int64_t)kvh * a.k_head;
+    vh = a.v + (int64_t)kvh * a.v_head;
+    trow = a.table + (int64_t)r * a.table_stride;
+  }
+
+  // Page and place within it of position pos.
+  __device__ __forceinline__ int page_of(int pos) const {
+    return a.page_shift >= 0 ? pos >> a.page_shift : (int)((unsigned)pos / (unsigned)a.page);
+  }
+  // Page id of a position of the row, -1 past its tokens and for entries outside the cache.
+  __device__ __forceinline__ int id_of(int pos, const Span& s) const {
+    if (pos >= s.len) return -1;
+    const int id = trow[page_of(pos)];
+    return id >= 0 && id < a.pages ? id : -1;
+  }
+
+  __device__ __forceinline__ void load_k(int hh, int id, int pos) {
+    const uint8_t* p = kh + (int64_t)id * a.k_page + (int64_t)(pos - page_of(pos) * a.page) * a.k_token;
+#pragma unroll
+    for (int j = 0; j < KL; ++j) {
+      const int d = F8 ? j * 64 + g * 16 : j * 32 + g * 8;
+      kr[hh][j] = id >= 0 && (DIM || d < a.dim) ? *(const u32x4_t*)(p + d * (F8 ? 1 : 2)) : u32x4_t{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ void load_v(int j, bool ok, const uint8_t* p) {
+#pragma unroll
+    for (int x = 0; x < VH; ++x) {
+      const int d = x * 128 + VE * col;
+      constexpr int W = F8 ? VE / 4 : VE / 2;
+      const uint8_t* at = p + d * (F8 ? 1 : 2);
+      const bool in = ok && (DIM || d < a.dim);
+      if constexpr (W == 4) {
+        const u32x4_t w = in ? *(const u32x4_t*)at : u32x4_t{0, 0, 0, 0};
+        vr[x][j][0] = w.x, vr[x][j][1] = w.y, vr[x][j][2] = w.z, vr[x][j][3] = w.w;
+      } else if constexpr (W == 2) {
+        const u32x2_t w = in ? *(const u32x2_t*)at : u32x2_t{0, 0};
+        vr[x][j][0] = w.x, vr[x][j][1] = w.y;
+      } else {
+        vr[x][j][0] = in ? *(const uint32_t*)at : 0u;
+      }
+    }
+  }
+
+  // Bits of this lane's eight tokens (t0 + 8 g + j) that count.
+  __device__ __forceinline__ uint32_t load_tile(int t0, const Span& s) {
+    uint32_t live = 0;
+    if constexpr (P8) {
+      const int pos = t0 + 8 * g, id = id_of(pos, s);
+      const int kb = col >> 2;  // block of this lane's key rows
+      const int kid = __shfl(id, kb * 16);
+      const int kpos = t0 + 8 * kb + (col & 3);
+      load_k(0, kid, kpos);
+      load_k(1, kid, kpos + 4);
+      const uint8_t* p = vh + (int64_t)id * a.v_page + (int64_t)(pos - page_of(pos) * a.page) * a.v_token;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool ok = id >= 0 && pos + j >= s.first && pos + j < s.len;
+        load_v(j, ok, p + j * a.v_token);
+        live |= (uint32_t)ok << j;
+      }
+    } else {
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const int pos = t0 + 8 * (col >> 2) + 4 * hh + (col & 3);
+        load_k(hh, id_of(pos, s), pos);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int pos = t0 + 8 * g + j, id = id_of(pos, s);
+        const bool ok = id >= 0 && pos >= s.first;
+        load_v(j, ok, vh + (int64_t)id * a.v_page + (int64_t)(pos - page_of(pos) * a.page) * a.v_token);
+        live |= (uint32_t)ok << j;
+      }
+    }
+    return live;
+  }
+
+  // Word w (dims 2 w, 2 w + 1 of the lane's VE) of token j, as a pair of 16-bit floats.
+  template <int W>
+  __device__ __forceinline__ uint32_t v_word(int x, int j) const {
+    if constexpr (F8) return widen<F16, (W & 1) != 0>(vr[x][j][W >> 1]);
+    else return vr[x][j][W];
+  }
+  template <int W>
+  __device__ __forceinline__ void add_v(int x, u32x4_t hi, u32x4_t lo) {
+    if constexpr (W < VE / 2) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = v_word<W>(x, j);
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        u32x4_t f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = __builtin_amdgcn_perm(w[2 * k + 1], w[2 * k], odd ? 0x07060302u : 0x05040100u);
+        const int c = x * VE + 2 * W + odd;
+        o[c] = mfma16<F16>(f, lo, o[c]);
+        o[c] = mfma16<F16>(f, hi, o[c]);
+      }
+      add_v<W + 1>(x, hi, lo);
+    }
+  }
+
+  __device__ __forceinline__ void tile(uint32_t live) {
+    f32x4_t s[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      s[hh] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        u32x4_t kf;
+        if constexpr (F8) {
+          const uint32_t w0 = kr[hh][j >> 1][2 * (j & 1)], w1 = kr[hh][j >> 1][2 * (j & 1) + 1];
+          kf = u32x4_t{widen<F16, false>(w0), widen<F16, true>(w0), widen<F16, false>(w1), widen<F16, true>(w1)};
+        } else {
+          kf = kr[hh][j];
+        }
+        s[hh] = mfma16<F16>(kf, q[j], s[hh]);
+      }
+    }
+    float x[8], top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = live >> j & 1 ? s[j >> 2][j & 3] * sc : -INFINITY;
+      top = fmaxf(top, x[j]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float m_new = fmaxf(m, top);
+    const float ref = m_new == -INFINITY ? 0.f : m_new;  // nothing but -inf so far: p = 0, not NaN
+    const float alpha = __builtin_amdgcn_exp2f(m - ref);
+    m = m_new;
+    const float off = SHIFT - ref;
+    float sum = 0.f;
+    u32x4_t hi, lo;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float p0 = __builtin_amdgcn_exp2f(x[2 * k] + off), p1 = __builtin_amdgcn_exp2f(x[2 * k + 1] + off);
+      sum += p0 + p1;
+      hi[k] = pack2<F16>(p0, p1);
+      lo[k] = pack2<F16>(p0 - unpack<F16>(hi[k], 0), p1 - unpack<F16>(hi[k], 1));
+    }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[c] *= alpha;
+#pragma unroll
+    for (int xh = 0; xh < VH; ++xh) add_v<0>(xh, hi, lo);
+  }
+
+  // First of the VE neighbouring dims that this lane holds of row i of the accumulators of half x.
+  __device__ __forceinline__ int out_dim(int x, int i) const { return x * 128 + VE * (4 * g + i); }
+
+  __device__ __forceinline__ void finish(int r, int kvh, int grp, float* part) {
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const int h = grp * kHeads + col;
+    if (h >= a.group) return;
+    if (part) {
+      float* row = part + (int64_t)col * a.dim;
+#pragma unroll
+      for (int x = 0; x < VH; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = out_dim(x, i);
+          if (DIM || d < a.dim)
+#pragma unroll
+            for (int c = 0; c < VE; c += 4)
+              *(f32x4_t*)(row + d + c) = f32x4_t{o[x * VE + c][i], o[x * VE + c + 1][i], o[x * VE + c + 2][i], o[x * VE + c + 3][i]} * UNSHIFT;
+        }
+      if (g == 0) {
+        float* st = part + (int64_t)a.part_rows * a.dim + 2 * col;
+        st[0] = m;
+        st[1] = l * UNSHIFT;
+      }
+      return;
+    }
+    const int64_t head = (int64_t)r * a.heads + kvh * a.group + h;
+    const float f = (a.v_scale ? a.v_scale[kvh] : 1.f) / l;
+#pragma unroll
+    for (int x = 0; x < VH; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = out_dim(x, i);
+        if (DIM || d < a.dim)
+#pragma unroll
+          for (int c = 0; c < VE; ++c) store_scalar(a.out, a.out_dtype, head * a.dim + d + c, o[x * VE + c][i] * f);
+      }
+    if (a.lse && g == 0) a.lse[head] = (m + __builtin_amdgcn_logf(l * UNSHIFT)) * 0.69314718055994531f;
+  }
+};
+
+template <bool F16, bool F8, int DT, bool DIM, bool P8>
+__global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(AttnArgs a) {
+  extern __shared__ int pre[];  // [rows + 1] tiles before each row
+  __shared__ int part[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per_thread = (a.rows + 64 * kWaves - 1) / (64 * kWaves);
+  const int r0 = min(tid * per_thread, a.rows), r1 = min(r0 + per_thread, a.rows);
+  int n = 0;
+  for (int r = r0; r < r1; ++r) n += span_of(a, r).tiles;
+  int sum = n;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int v = __shfl_up(sum, d);
+    if (lane >= d) sum += v;
+  }
+  if (lane == 63) part[wave] = sum;
+  __syncthreads();
+  int at = sum - n;
+  for (int w = 0; w < wave; ++w) at += part[w];
+  for (int r = r0; r < r1; ++r) {
+    pre[r] = at;
+    at += span_of(a, r).tiles;
+  }
+  if (tid == 64 * kWaves - 1) pre[a.rows] = at;  // the last thread's sum is the total
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int r = tid; r <= a.rows; r += 64 * kWaves) a.prefix[r] = pre[r];
+
+  const int per_row = a.kv_heads * a.groups;  // sequences of tiles of one row
+  const int64_t total = (int64_t)pre[a.rows] * per_row;
+  const int64_t per = tiles_per_worker(a, total);
+  const int w = __builtin_amdgcn_readfirstlane(wave) * (int)gridDim.x + (int)blockIdx.x;
+  int64_t pos = (int64_t)w * per;
+  const int64_t end = pos + per < total ? pos + per : total;
+  if (pos >= end) return;
+  int lo = 0, hi = a.rows;  // the row of pos
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((int64_t)pre[mid] * per_row <= pos) lo = mid;
+    else hi = mid;
+  }
+  int r = __builtin_amdgcn_readfirstlane(lo);
+  Attn<F16, F8, DT, DIM, P8> t(a);
+  int slot = 0;
+  while (pos < end) {
+    const Span s = span_of(a, r);
+    if (s.tiles == 0) {
+      ++r;
+      continue;
+    }
+    const int64_t in_row = pos - (int64_t)pre[r] * per_row;
+    const int hg = (int)(in_row / s.tiles), first = (int)(in_row - (int64_t)hg * s.tiles);
+    const int count = (int)min((int64_t)(s.tiles - first), end - pos);
+    const int kvh = hg / a.groups, grp = hg - kvh * a.groups;
+    t.start(r, kvh, grp);
+    for (int i = 0; i < count; ++i) {
+      const uint32_t live = t.load_tile(s.base + (first + i) * kTile, s);
+      t.tile(live);
+    }
+    const bool whole = first == 0 && count == s.tiles;
+    t.finish(r, kvh, grp, whole ? nullptr : partial(a, w, slot));
+    slot = 1;
+    pos += count;
+    if (first + count == s.tiles && hg + 1 == per_row) ++r;
+  }
+}
+
+struct AttnKern {
+  const void* fn;
+  std::atomic<int> residents[64];  // workgroups of a CU, by device; 0: not asked yet
+};
+// The kernel for head_dim at a page size; F16/F8 as above.
+AttnKern& kern_bf16(int dim, bool p8);
+AttnKern& kern_f16(int dim, bool p8);
+AttnKern& kern_bf16_e4m3(int dim, bool p8);
+AttnKern& kern_f16_e4m3(int dim, bool p8);
+
+template <bool F16, bool F8>
+AttnKern& kern_of(int dim, bool p8) {
+#define MLXR_ATTN(DT, DIM, P8) \
+  { static AttnKern k{(const void*)attn_kernel<F16, F8, DT, DIM, P8>, {}}; return k; }
+  if (dim == 64 && p8) MLXR_ATTN(64, true, true)
+  if (dim == 128 && p8) MLXR_ATTN(128, true, true)
+  if (dim == 256 && p8) MLXR_ATTN(256, true, true)
+  if (p8) {
+    if (dim < 64) MLXR_ATTN(64, false, true)
+    if (dim < 128) MLXR_ATTN(128, false, true)
+    MLXR_ATTN(256, false, true)
+  }
+  if (dim <= 64) MLXR_ATTN(64, false, false)
+  if (dim <= 128) MLXR_ATTN(128, false, false)
+  MLXR_ATTN(256, false, false)
+#undef MLXR_ATTN
+}
+
+}  // namespace paged
+}  // namespace mlxr

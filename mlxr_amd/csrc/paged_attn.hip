@@ -1,0 +1,174 @@
+// Decode attention over a paged cache: the C entry, and the join of the pieces that the kernel
+// (paged_attn.h) leaves of rows dealt to several wavefronts.
+#include "paged_attn.h"
+
+namespace mlxr {
+namespace paged {
+
+namespace {
+
+constexpr int kJoinThreads = 256;
+
+// One workgroup per (row, head): o = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w over the wavefronts w
+// that had a piece of the row, M the maximum of their m.  Rows without tokens get zeros; rows that one
+// wavefront covered are done.
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
+  __shared__ float sh[kJoinThreads * 4];
+  __shared__ float sh_m[4], sh_l[kJoinThreads];
+  const int r = blockIdx.x / a.heads, h = blockIdx.x - r * a.heads, tid = threadIdx.x;
+  const int kvh = h / a.group, hk = h - kvh * a.group, grp = hk / kHeads, row = hk - grp * kHeads;
+  const int per_row = a.kv_heads * a.groups, tiles = a.prefix[r + 1] - a.prefix[r];
+  const int64_t head = (int64_t)r * a.heads + h;
+  if (tiles == 0) {
+    for (int d = tid; d < a.dim; d += kJoinThreads) store_scalar(a.out, a.out_dtype, head * a.dim + d, 0.f);
+    if (a.lse && tid == 0) a.lse[head] = -INFINITY;
+    return;
+  }
+  const int64_t per = tiles_per_worker(a, (int64_t)a.prefix[a.rows] * per_row);
+  const int64_t s = (int64_t)a.prefix[r] * per_row + (int64_t)(kvh * a.groups + grp) * tiles;
+  const int w0 = (int)(s / per), w1 = (int)((s + tiles - 1) / per);
+  if (w0 == w1) return;
+  const int count = w1 - w0 + 1;
+  // the first of them may have had another row before this one
+  auto part = [&](int i) { return partial(a, w0 + i, i == 0 && (int64_t)w0 * per < s ? 1 : 0); };
+  const int64_t st = (int64_t)a.part_rows * a.dim + 2 * row;
+  float m = -INFINITY;
+  for (int i = tid; i < count; i += kJoinThreads) m = fmaxf(m, part(i)[st]);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  if ((tid & 63) == 0) sh_m[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
+  const float ref = m == -INFINITY ? 0.f : m;
+  // threads: `lanes` of a piece's row (four dims each) by `across` pieces
+  const int lanes = a.dim / 4, across = kJoinThreads / lanes, x = tid % lanes, y = tid / lanes;
+  f32x4_t o = {0, 0, 0, 0};
+  float l = 0.f;
+  if (y < across)
+    for (int i = y; i < count; i += across) {
+      const float* p = part(i);
+      const float f = __builtin_amdgcn_exp2f(p[st] - ref);
+      const f32x4_t v = *(const f32x4_t*)(p + (int64_t)row * a.dim + 4 * x);
+      l += f * p[st + 1];
+      o += f * v;
+    }
+  *(f32x4_t*)(sh + 4 * tid) = o;
+  sh_l[tid] = l;
+  __syncthreads();
+  if (y) return;
+  for (int i = 1; i < across; ++i) {
+    o += *(const f32x4_t*)(sh + 4 * (i * lanes + x));
+    l += sh_l[i * lanes + x];
+  }
+  const float f = (a.v_scale ? a.v_scale[kvh] : 1.f) / l;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) store_scalar(a.out, a.out_dtype, head * a.dim + 4 * x + c, o[c] * f);
+  if (a.lse && x == 0) a.lse[head] = (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+}
+
+// Workgroups of the launch: as many as the device holds at once.
+int grid_of(AttnKern& k, int rows, hipError_t* e) {
+  int dev = 0;
+  *e = hipGetDevice(&dev);
+  if (*e != hipSuccess) return 0;
+  const int d = dev >= 0 && dev < 64 ? dev : 0;
+  int occ = k.residents[d].load(std::memory_order_acquire);
+  if (!occ) {
+    *e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k.fn, 64 * kWaves, 0);
+    if (*e != hipSuccess) return 0;
+    if (occ < 1) occ = 1;
+    if (occ > 4) occ = 4;
+    k.residents[d].store(occ, std::memory_order_release);
+  }
+  return occ * device_cu_count();
+}
+
+AttnKern& kern(const mlxr_paged_cache* c, int q_dtype) {
+  const bool f16 = q_dtype == MLXR_F16, p8 = c->page_size % 8 == 0;
+  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, p8) : kern_bf16_e4m3(c->head_dim, p8);
+  return f16 ? kern_f16(c->head_dim, p8) : kern_bf16(c->head_dim, p8);
+}
+
+constexpr size_t kPrefixBytes = (MLXR_PAGED_MAX_ROWS + 1 + 3) / 4 * 4 * sizeof(int32_t);
+constexpr int kMaxGridPerCu = 4;
+
+size_t workspace(const mlxr_paged_cache* c, int heads) {
+  const int group = heads / c->kv_heads, part_rows = group < kHeads ? group : kHeads;
+  return kPrefixBytes + (size_t)device_cu_count() * kMaxGridPerCu * kWaves * 2 * partial_floats(part_rows, c->head_dim) * sizeof(float);
+}
+
+int check_attn(const mlxr_paged_cache* c, int rows, int heads) {
+  if (const int rc = check_cache(c)) return rc;
+  if (rows < 0 || heads <= 0) return set_error(MLXR_E_INVALID, "paged_attention: bad sizes");
+  if (rows > MLXR_PAGED_MAX_ROWS)
+    return set_error(MLXR_E_SHAPE, "paged_attention: at most %d rows", MLXR_PAGED_MAX_ROWS);
+  if (heads % c->kv_heads) return set_error(MLXR_E_SHAPE, "heads must be a multiple of kv_heads");
+  return MLXR_OK;
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace mlxr
+
+using namespace mlxr;
+using namespace mlxr::paged;
+
+extern "C" int mlxr_paged_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int heads, size_t* bytes) {
+  if (!bytes) return set_error(MLXR_E_INVALID, "null bytes");
+  if (const int rc = check_attn(cache, rows, heads)) return rc;
+  *bytes = workspace(cache, heads);
+  return MLXR_OK;
+}
+
+extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int heads, const void* q_dev, int q_dtype,
+                                    int64_t q_row_stride, int64_t q_head_stride, const int32_t* table_dev,
+                                    int64_t table_stride, int table_width, const int32_t* lens_dev, float scale,
+                                    int window, void* out_dev, int out_dtype, float* lse_dev, void* workspace_dev,
+                                    size_t workspace_bytes, void* stream) {
+  if (const int rc = check_attn(cache, rows, heads)) return rc;
+  if (q_dtype != MLXR_F16 && q_dtype != MLXR_BF16) return set_error(MLXR_E_INVALID, "invalid query dtype %d", q_dtype);
+  if (cache->dtype != MLXR_E4M3 && cache->dtype != q_dtype)
+    return set_error(MLXR_E_INVALID, "queries must have the cache's type");
+  if (out_dtype != MLXR_F32 && out_dtype != MLXR_F16 && out_dtype != MLXR_BF16)
+    return set_error(MLXR_E_INVALID, "invalid output dtype %d", out_dtype);
+  if (window < 0) return set_error(MLXR_E_INVALID, "paged_attention: window must not be negative");
+  if (rows == 0) return MLXR_OK;
+  if (!q_dev || !table_dev || !lens_dev || !out_dev || !workspace_dev) return set_error(MLXR_E_INVALID, "null buffer");
+  if (table_width <= 0) return set_error(MLXR_E_INVALID, "paged_attention: table_width must be positive");
+  if (q_row_stride % 8 || q_head_stride % 8 || ((uintptr_t)q_dev & 15) || ((uintptr_t)out_dev & 15) || ((uintptr_t)workspace_dev & 15))
+    return set_error(MLXR_E_SHAPE, "paged_attention: query rows, output and workspace must start at multiples of 16 bytes");
+  const int64_t most = (int64_t)table_width * cache->page_size;
+  if (most > INT32_MAX || (most / kTile + 1) * rows > INT32_MAX || (int64_t)rows * heads > INT32_MAX)
+    return set_error(MLXR_E_SHAPE, "paged_attention: the table covers too many tokens");
+  if (workspace_bytes < workspace(cache, heads))
+    return set_error(MLXR_E_INVALID, "paged_attention: the workspace is smaller than mlxr_paged_attention_workspace_size");
+  AttnKern& k = kern(cache, q_dtype);
+  hipError_t e = hipSuccess;
+  const int grid = grid_of(k, rows, &e);
+  if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_attention: %s", hipGetErrorString(e));
+  const int es = cache->dtype == MLXR_E4M3 ? 1 : 2;
+  AttnArgs a;
+  a.k = (const uint8_t*)cache->k_dev, a.v = (const uint8_t*)cache->v_dev;
+  a.k_scale = cache->k_scale_dev, a.v_scale = cache->v_scale_dev;
+  a.k_page = cache->k_stride[0] * es, a.k_head = cache->k_stride[1] * es, a.k_token = cache->k_stride[2] * es;
+  a.v_page = cache->v_stride[0] * es, a.v_head = cache->v_stride[1] * es, a.v_token = cache->v_stride[2] * es;
+  a.q = (const uint16_t*)q_dev, a.q_row = q_row_stride, a.q_head = q_head_stride;
+  a.table = table_dev, a.table_stride = table_stride, a.lens = lens_dev;
+  a.out = out_dev, a.lse = lse_dev;
+  a.prefix = (int32_t*)workspace_dev, a.ws = (float*)((uint8_t*)workspace_dev + kPrefixBytes);
+  a.rows = rows, a.heads = heads, a.kv_heads = cache->kv_heads, a.group = heads / cache->kv_heads;
+  a.groups = (a.group + kHeads - 1) / kHeads;
+  a.part_rows = a.group < kHeads ? a.group : kHeads;
+  a.dim = cache->head_dim, a.page = cache->page_size, a.pages = cache->num_pages, a.width = table_width;
+  a.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
+  a.window = window, a.out_dtype = out_dtype, a.workers = grid * kWaves;
+  a.scale = scale * 1.44269504088896341f;
+  void* args[] = {&a};
+  e = hipLaunchKernel(k.fn, dim3(grid), dim3(64 * kWaves), args, (size_t)(rows + 1) * 4, (hipStream_t)stream);
+  if (e == hipSuccess) {
+    join_kernel<<<rows * heads, kJoinThreads, 0, (hipStream_t)stream>>>(a);
+    e = hipGetLastError();
+  }
+  if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_attention launch: %s", hipGetErrorString(e));
+  return MLXR_OK;
+}

@@ -1,0 +1,8 @@
+// Decode attention instantiated for one pair of query and cache types (paged_attn.h).
+#include "paged_attn.h"
+
+namespace mlxr {
+namespace paged {
+AttnKern& kern_bf16(int dim, bool p8) { return kern_of<false, false>(dim, p8); }
+}  // namespace paged
+}  // namespace mlxr

@@ -1,0 +1,330 @@
+// Page tables and slot maps of a paged key-value cache, and the writes of new keys and values
+// (include/mlxr_paged.h).
+#include <hip/hip_runtime.h>
+
+#include "../../include/mlxr_paged.h"
+#include "paged_internal.h"
+
+namespace mlxr {
+
+namespace {
+
+struct ResizeArgs {
+  int32_t* table;
+  int64_t stride;
+  const int32_t *lens, *want, *free_count;
+  int32_t* free;
+  int32_t *lens_out, *count_out, *starts, *slots, *positions, *refused;
+  int rows, page, pages, width, tokens;
+};
+
+constexpr int kResizeThreads = 1024;
+
+struct Sum3 {
+  int a, b, c;
+};
+// Exclusive sums over the threads of a workgroup, and the totals.
+__device__ Sum3 block_scan(Sum3 v, Sum3* total, int* part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Sum3 s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int a = __shfl_up(s.a, d), b = __shfl_up(s.b, d), c = __shfl_up(s.c, d);
+    if (lane >= d) s.a += a, s.b += b, s.c += c;
+  }
+  __syncthreads();  // part may still be read from the call before
+  if (lane == 63) part[3 * wave] = s.a, part[3 * wave + 1] = s.b, part[3 * wave + 2] = s.c;
+  __syncthreads();
+  Sum3 before = {0, 0, 0}, all = {0, 0, 0};
+  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+    const Sum3 p = {part[3 * w], part[3 * w + 1], part[3 * w + 2]};
+    if (w < wave) before.a += p.a, before.b += p.b, before.c += p.c;
+    all.a += p.a, all.b += p.b, all.c += p.c;
+  }
+  *total = all;
+  return {before.a + s.a - v.a, before.b + s.b - v.b, before.c + s.c - v.c};
+}
+
+// Largest r in [0, n) with first[r] <= k (first is nondecreasing, first[0] = 0).
+__device__ __forceinline__ int row_of(const int* first, int n, int k) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= k) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((unsigned)tokens + page - 1) / (unsigned)page); }
+
+// With P(n) = ceil(n / page): row r takes need = P(want) - P(lens) pages or gives back as many, and the
+// exclusive sums of both over the rows say which place of the stack each page goes to or comes
+// from: the i-th page given back by r lands at count + G_r + i, the i-th page that r takes lies
+// at c1 - 1 - (N_r + i), c1 = count + all that is given back.  Every output element follows from
+// the sums alone (a page taken from a place at or above `count` is read from the table of the row
+// that gives it back), so nothing in the launch waits for anything else in it: each workgroup
+// makes the sums for itself and fills its share of the outputs.
+__global__ __launch_bounds__(kResizeThreads) void resize_kernel(ResizeArgs a) {
+  extern __shared__ int sh[];
+  int* first_need = sh;               // N_r
+  int* first_give = sh + a.rows;      // G_r
+  int* first_new = sh + 2 * a.rows;   // new tokens before row r
+  __shared__ int part[3 * (kResizeThreads / 64)];
+  const int tid = threadIdx.x, nt = blockDim.x, page = a.page;
+  const int most = a.width * page;
+  const int per = (a.rows + nt - 1) / nt, r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
+  auto have_of = [&](int r) { return min(max(a.lens[r], 0), most); };
+
+  Sum3 mine = {0, 0, 0}, total;
+  for (int r = r0; r < r1; ++r) {
+    const int have = have_of(r), want = a.want[r];
+    if (want < 0 || want > most) continue;
+    const int d = pages_of(want, page) - pages_of(have, page);
+    mine.a += max(d, 0);
+    mine.b += max(-d, 0);
+  }
+  Sum3 before = block_scan(mine, &total, part);
+  const int count = min(max(a.free_count[0], 0), a.pages);
+  const int given = total.b;
+  const int stack = min(count + given, a.pages);
+  int taken = 0, refused = 0;
+  mine = {0, 0, 0};
+  for (int r = r0; r < r1; ++r) {
+    const int have = have_of(r), want = a.want[r];
+    first_need[r] = before.a;
+    first_give[r] = before.b;
+    bool ok = want >= 0 && want <= most;
+    if (ok) {
+      const int d = pages_of(want, page) - pages_of(have, page);
+      if (d > 0) {
+        before.a += d;
+        ok = before.a <= stack;
+        if (ok) taken = before.a;
+      } else {
+        before.b -= d;
+      }
+    }
+    if (!ok) ++refused;
+    const int len = ok ? want : have;
+    mine.c += max(len - have, 0);
+    if (blockIdx.x == 0) a.lens_out[r] = len;
+  }
+  mine.b = refused;
+  // the sums grow with r: the rows that get pages are a prefix of those that ask
+  before = block_scan(mine, &total, part);
+  const int new_tokens = total.c, all_refused = total.b;
+  __shared__ int most_taken;
+  if (tid == 0) most_taken = 0;
+  __syncthreads();
+  if (taken) atomicMax(&most_taken, taken);
+  int at = before.c;
+  for (int r = r0; r < r1; ++r) {
+    first_new[r] = at;
+    if (blockIdx.x == 0) a.starts[r] = at;
+    const int have = have_of(r), want = a.want[r];
+    bool ok = want >= 0 && want <= most;
+    if (ok) {
+      const int d = pages_of(want, page) - pages_of(have, page);
+      ok = d <= 0 || first_need[r] + d <= stack;
+    }
+    at += ok ? max(want - have, 0) : 0;
+  }
+  __syncthreads();
+  const int all_taken = most_taken;
+  if (blockIdx.x == 0 && tid == 0) {
+    a.starts[a.rows] = new_tokens;
+    a.count_out[0] = stack - all_taken;
+    a.refused[0] = all_refused;
+  }
+
+  const int gid = blockIdx.x * nt + tid, gn = gridDim.x * nt;
+  auto given_page = [&](int k) {  // the k-th page given back
+    const int r = row_of(first_give, a.rows, k);
+    return a.table[r * a.stride + pages_of(a.want[r], page) + (k - first_give[r])];
+  };
+  auto taken_page = [&](int k) {  // the k-th page taken
+    const int p = stack - 1 - k;
+    return p < count ? a.free[p] : given_page(p - count);
+  };
+  for (int k = gid; k < all_taken; k += gn) {
+    const int r = row_of(first_need, a.rows, k);
+    a.table[r * a.stride + pages_of(have_of(r), page) + (k - first_need[r])] = taken_page(k);
+  }
+  for (int k = gid; k < given && count + k < a.pages; k += gn) a.free[count + k] = given_page(k);
+  for (int t = gid; t < a.tokens; t += gn) {
+    int slot = -1, pos = -1;
+    if (t < new_tokens) {
+      const int r = row_of(first_new, a.rows, t);
+      const int have = have_of(r), held = pages_of(have, page);
+      pos = have + (t - first_new[r]);
+      const int j = (int)((unsigned)pos / (unsigned)page);
+      const int id = j < held ? a.table[r * a.stride + j] : taken_page(first_need[r] + j - held);
+      slot = id < 0 || id >= a.pages ? -1 : id * page + (pos - j * page);
+    }
+    a.slots[t] = slot;
+    a.positions[t] = pos;
+  }
+}
+
+struct AppendSide {
+  const void* x;
+  int64_t token, head;          // strides of x
+  uint8_t* store;
+  int64_t s_page, s_head, s_token;  // strides of the store
+  const float* scale;
+};
+struct AppendArgs {
+  AppendSide side[2];  // keys, values
+  const int32_t* slots;
+  int tokens, heads, dim8, page;
+  int64_t slots_end;
+};
+
+// One thread moves eight elements of one head's row of one token: 16 bytes of a 16-bit input, and
+// 16 or 8 bytes of the store.
+template <int XT, int CT>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+  const AppendSide& s = a.side[blockIdx.y];
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = a.heads * a.dim8;
+  if (i >= (int64_t)a.tokens * per) return;
+  const int t = (int)(i / per), e = (int)(i - (int64_t)t * per), h = e / a.dim8, c = e - h * a.dim8;
+  const int slot = a.slots[t];
+  if (slot < 0 || slot >= a.slots_end) return;
+  const int64_t from = (int64_t)t * s.token + (int64_t)h * s.head + 8 * c;
+  const int pg = slot / a.page;
+  const int64_t to = (int64_t)pg * s.s_page + (int64_t)h * s.s_head + (int64_t)(slot - pg * a.page) * s.s_token + 8 * c;
+  if constexpr (XT == CT) {
+    if (!s.scale) {  // same type: the bits
+      *(uint4*)(s.store + 2 * to) = *(const uint4*)((const uint16_t*)s.x + from);
+      return;
+    }
+  }
+  float v[8];
+  if constexpr (XT == DT_F32) {
+    const float4 lo = *(const float4*)((const float*)s.x + from), hi = *(const float4*)((const float*)s.x + from + 4);
+    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+  } else {
+    const uint4 b = *(const uint4*)((const uint16_t*)s.x + from);
+    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t u = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
+      v[k] = XT == DT_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
+    }
+  }
+  if (s.scale) {
+    const float d = s.scale[h];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] /= d;
+  }
+  if constexpr (CT == MLXR_E4M3) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = v[k] > 448.f ? 448.f : v[k] < -448.f ? -448.f : v[k];  // NaN stays
+    uint2 o;
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    o.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+    o.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], w, true);
+    *(uint2*)(s.store + to) = o;
+  } else {
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      o[k] = CT == DT_BF16 ? pack_bf16x2(v[2 * k], v[2 * k + 1])
+                           : (f32_to_f16_bits(v[2 * k]) | ((uint32_t)f32_to_f16_bits(v[2 * k + 1]) << 16));
+    *(uint4*)(s.store + 2 * to) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+template <int XT>
+void launch_append(const AppendArgs& a, int ct, dim3 grid, hipStream_t s) {
+  if (ct == MLXR_F16) append_kernel<XT, DT_F16><<<grid, 256, 0, s>>>(a);
+  else if (ct == MLXR_BF16) append_kernel<XT, DT_BF16><<<grid, 256, 0, s>>>(a);
+  else append_kernel<XT, MLXR_E4M3><<<grid, 256, 0, s>>>(a);
+}
+
+}  // namespace
+
+int check_cache(const mlxr_paged_cache* c) {
+  if (!c) return set_error(MLXR_E_INVALID, "null cache");
+  if (!c->k_dev || !c->v_dev) return set_error(MLXR_E_INVALID, "null buffer");
+  if (c->dtype != MLXR_F16 && c->dtype != MLXR_BF16 && c->dtype != MLXR_E4M3)
+    return set_error(MLXR_E_INVALID, "invalid cache dtype %d", c->dtype);
+  if (c->num_pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0 || c->head_dim <= 0)
+    return set_error(MLXR_E_INVALID, "cache sizes must be positive");
+  if ((int64_t)c->num_pages * c->page_size > INT32_MAX)
+    return set_error(MLXR_E_SHAPE, "a cache holds at most %d tokens", INT32_MAX);
+  const int unit = c->dtype == MLXR_E4M3 ? 16 : 8;
+  if (c->head_dim % unit || c->head_dim > 256)
+    return set_error(MLXR_E_SHAPE, "head_dim must be a multiple of %d and at most 256 (got %d)", unit, c->head_dim);
+  for (int i = 0; i < 3; ++i)
+    if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_stride[i] % unit || c->v_stride[i] % unit)
+      return set_error(MLXR_E_SHAPE, "cache strides must be multiples of 16 bytes");
+  if (((uintptr_t)c->k_dev | (uintptr_t)c->v_dev) & 15)
+    return set_error(MLXR_E_INVALID, "cache addresses must be multiples of 16 bytes");
+  return MLXR_OK;
+}
+
+}  // namespace mlxr
+
+using namespace mlxr;
+
+extern "C" int mlxr_page_resize(int rows, int page_size, int num_pages, int32_t* table_dev, int64_t table_stride,
+                                int table_width, const int32_t* lens_dev, const int32_t* want_dev, int32_t* free_dev,
+                                const int32_t* free_count_dev, int32_t* lens_out_dev, int32_t* free_count_out_dev,
+                                int32_t* starts_dev, int32_t* slots_dev, int32_t* positions_dev, int tokens,
+                                int32_t* refused_dev, void* stream) {
+  if (rows < 0 || tokens < 0 || page_size <= 0 || num_pages <= 0 || table_width <= 0)
+    return set_error(MLXR_E_INVALID, "page_resize: bad sizes");
+  if (!free_count_dev || !free_count_out_dev || !starts_dev || !refused_dev || !free_dev ||
+      (rows && (!table_dev || !lens_dev || !want_dev || !lens_out_dev)) || (tokens && (!slots_dev || !positions_dev)))
+    return set_error(MLXR_E_INVALID, "null buffer");
+  if (rows > MLXR_PAGED_MAX_ROWS)
+    return set_error(MLXR_E_SHAPE, "page_resize: at most %d rows", MLXR_PAGED_MAX_ROWS);
+  if (table_stride < table_width) return set_error(MLXR_E_SHAPE, "page_resize: table rows overlap");
+  if ((int64_t)num_pages * page_size > INT32_MAX ||
+      (__int128)(rows ? rows : 1) * table_width * page_size > INT32_MAX)
+    return set_error(MLXR_E_SHAPE, "page_resize: a pool and a table cover at most %d tokens", INT32_MAX);
+  if (lens_out_dev == lens_dev || free_count_out_dev == free_count_dev)
+    return set_error(MLXR_E_INVALID, "page_resize: outputs must not be the inputs");
+  ResizeArgs a{table_dev, table_stride, lens_dev, want_dev, free_count_dev, free_dev, lens_out_dev, free_count_out_dev,
+               starts_dev, slots_dev, positions_dev, refused_dev, rows, page_size, num_pages, table_width, tokens};
+  const int grid = tokens <= 4096 ? 1 : tokens >= 128 * 4096 ? 128 : (tokens + 4095) / 4096;
+  resize_kernel<<<grid, kResizeThreads, (size_t)rows * 12, (hipStream_t)stream>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return set_error(MLXR_E_HIP, "page_resize launch: %s", hipGetErrorString(e));
+  return MLXR_OK;
+}
+
+extern "C" int mlxr_paged_append(const mlxr_paged_cache* cache, int tokens, const void* k_dev, int64_t k_token_stride,
+                                 int64_t k_head_stride, const void* v_dev, int64_t v_token_stride, int64_t v_head_stride,
+                                 int x_dtype, const int32_t* slots_dev, void* stream) {
+  if (const int rc = check_cache(cache)) return rc;
+  if (tokens < 0) return set_error(MLXR_E_INVALID, "paged_append: tokens must not be negative");
+  if (tokens == 0) return MLXR_OK;
+  if (!k_dev || !v_dev || !slots_dev) return set_error(MLXR_E_INVALID, "null buffer");
+  if (x_dtype != MLXR_F32 && x_dtype != MLXR_F16 && x_dtype != MLXR_BF16)
+    return set_error(MLXR_E_INVALID, "invalid dtype %d", x_dtype);
+  const int unit = x_dtype == MLXR_F32 ? 4 : 8;
+  if (k_token_stride % unit || k_head_stride % unit || v_token_stride % unit || v_head_stride % unit ||
+      (((uintptr_t)k_dev | (uintptr_t)v_dev) & 15))
+    return set_error(MLXR_E_SHAPE, "paged_append: rows must start at multiples of 16 bytes");
+  AppendArgs a{{{k_dev, k_token_stride, k_head_stride, (uint8_t*)cache->k_dev, cache->k_stride[0], cache->k_stride[1],
+                 cache->k_stride[2], cache->k_scale_dev},
+                {v_dev, v_token_stride, v_head_stride, (uint8_t*)cache->v_dev, cache->v_stride[0], cache->v_stride[1],
+                 cache->v_stride[2], cache->v_scale_dev}},
+               slots_dev, tokens, cache->kv_heads, cache->head_dim / 8, cache->page_size,
+               (int64_t)cache->num_pages * cache->page_size};
+  const int64_t blocks = ((int64_t)tokens * a.heads * a.dim8 + 255) / 256;
+  if (blocks > INT32_MAX) return set_error(MLXR_E_SHAPE, "paged_append: too many elements");
+  const dim3 grid((unsigned)blocks, 2);
+  const hipStream_t s = (hipStream_t)stream;
+  if (x_dtype == MLXR_F32) launch_append<DT_F32>(a, cache->dtype, grid, s);
+  else if (x_dtype == MLXR_F16) launch_append<DT_F16>(a, cache->dtype, grid, s);
+  else launch_append<DT_BF16>(a, cache->dtype, grid, s);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_append launch: %s", hipGetErrorString(e));
+  return MLXR_OK;
+}

@@ -1,0 +1,129 @@
+"""Low-rank adapters of many requests beside shared (quantized) projections.
+
+``lora_apply`` adds each token's own adapter to the outputs of projections that read the same
+input (include/mlxr_lora.h): ``out[t] = y[t] + scale * (x[t] A^T) B^T`` with the A, B and scale of
+adapter ``ids[t]``.  ``LoraBank`` keeps a projection's adapters in the layout that it takes.
+"""
+import ctypes
+
+from . import qgemm
+from .paged import _code, _empty, _i32, _on
+from .qgemm import QGemmError
+
+MAX_ADAPTERS, MAX_RANK = 4096, 128
+_P, _I = ctypes.c_void_p, ctypes.c_int
+
+
+class Item(ctypes.Structure):
+    """mlxr_lora_item."""
+    _fields_ = [("a_dev", _P), ("b_dev", _P), ("y_dev", _P), ("out_dev", _P), ("N", _I), ("y_dtype", _I)]
+
+
+_SIGS = {
+    "mlxr_lora_workspace_size": (_I, [_I] * 5 + [ctypes.POINTER(ctypes.c_size_t)]),
+    "mlxr_lora_apply": (_I, [_I, _P] + [_I] * 4 + [_P, _I, ctypes.c_int64, _P, _P, _P, _P, ctypes.c_size_t, _P]),
+}
+_bound = None
+
+
+def _lib():
+    global _bound
+    if _bound is None:
+        l = qgemm.lib()
+        for name, (res, args) in _SIGS.items():
+            f = getattr(l, name)
+            f.restype, f.argtypes = res, args
+        _bound = l
+    return _bound
+
+
+def lora_apply(x, ids, a, b, y, scales=None, ranks=None, outs=None, stream=None):
+    """For each projection i that reads x [tokens, K]: y[i] + scale * (x A^T) B^T with the adapter
+    ``ids`` [tokens] (int32; outside [0, adapters): none) of each token (mlxr_lora_apply).
+
+    a[i] [adapters, rank, K] and b[i] [adapters, N_i, rank] have x's dtype (float16 / bfloat16), one
+    rank (a multiple of 8, up to 128) for all; ``ranks`` [adapters] (int32) says how much of it each
+    adapter uses.  ``scales`` [adapters] float32.  outs[i] may be y[i].  Returns the outputs."""
+    torch = qgemm._torch()
+    d = x.device
+    n = len(a)
+    if x.dim() != 2 or d.type != "cuda":
+        raise QGemmError(-3, "Input shape must be [tokens, K] on a GPU")
+    tokens, K = x.shape
+    if len(b) != n or len(y) != n or (outs is not None and len(outs) != n):
+        raise QGemmError(-1, "one A, one B, one y (and one output) per projection")
+    _i32(ids, "ids", d)
+    if ids.shape[0] != tokens:
+        raise QGemmError(-3, "ids must be [tokens]")
+    if n == 0:
+        return []
+    adapters, rank = a[0].shape[0], a[0].shape[1]
+    if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (adapters,) or
+                               not scales.is_contiguous() or scales.device != d):
+        raise QGemmError(-1, f"scales must be a contiguous float32 [{adapters}] tensor on {d}")
+    if ranks is not None and _i32(ranks, "ranks", d).shape[0] != adapters:
+        raise QGemmError(-3, f"ranks must be [{adapters}]")
+    dt = _code(x.dtype, "x")
+    ptr, ctx = _on(stream, d)
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < 0 or x.data_ptr() % 16:
+        if ctx is None:
+            x = x.clone(memory_format=torch.contiguous_format)
+        else:
+            with ctx:
+                x = x.clone(memory_format=torch.contiguous_format)
+    if outs is None:
+        outs = [_empty(ctx, t.shape, t.dtype, d) for t in y]
+    items = (Item * n)()
+    for i, (A, B, t, o) in enumerate(zip(a, b, y, outs)):
+        if A.dim() != 3 or tuple(A.shape) != (adapters, rank, K):
+            raise QGemmError(-3, f"a[{i}] must be [{adapters}, {rank}, {K}]")
+        if B.dim() != 3 or B.shape[0] != adapters or B.shape[2] != rank:
+            raise QGemmError(-3, f"b[{i}] must be [{adapters}, N, {rank}]")
+        if A.dtype != x.dtype or B.dtype != x.dtype or A.device != d or B.device != d or \
+                not A.is_contiguous() or not B.is_contiguous():
+            raise QGemmError(-1, f"a[{i}] and b[{i}] must be contiguous, of x's dtype and device")
+        N = B.shape[1]
+        if tuple(t.shape) != (tokens, N) or o.shape != t.shape or t.dtype != o.dtype or t.device != d or o.device != d or \
+                not t.is_contiguous() or not o.is_contiguous():
+            raise QGemmError(-1, f"y[{i}] and its output must be contiguous [{tokens}, {N}] tensors of one dtype on {d}")
+        items[i] = Item(A.data_ptr(), B.data_ptr(), t.data_ptr(), o.data_ptr(), N, _code(t.dtype, f"y[{i}]"))
+    lib = _lib()
+    nb = ctypes.c_size_t()
+    qgemm._check(lib.mlxr_lora_workspace_size(n, tokens, K, adapters, rank, ctypes.byref(nb)))
+    ws = _empty(ctx, nb.value, torch.uint8, d)
+    qgemm._check(lib.mlxr_lora_apply(n, items, tokens, K, adapters, rank, x.data_ptr(), dt, x.stride(0), ids.data_ptr(),
+                                     scales.data_ptr() if scales is not None else None,
+                                     ranks.data_ptr() if ranks is not None else None, ws.data_ptr(), nb.value, ptr))
+    return outs
+
+
+class LoraBank:
+    """The adapters of one projection [N, K]: A [adapters, rank, K], B [adapters, N, rank], a scale and a
+    rank for each, filled by ``load``."""
+
+    def __init__(self, adapters, rank, N, K, dtype=None, device="cuda"):
+        torch = qgemm._torch()
+        if not 0 < adapters <= MAX_ADAPTERS or not 0 < rank <= MAX_RANK or N <= 0 or K <= 0 or K % 8:
+            raise QGemmError(-1, f"LoraBank: up to {MAX_ADAPTERS} adapters of rank up to {MAX_RANK}, K a multiple of 8")
+        dtype = dtype or torch.bfloat16
+        room = -(-rank // 8) * 8
+        self.N, self.K, self.rank = N, K, rank
+        self.a = torch.zeros((adapters, room, K), dtype=dtype, device=device)
+        self.b = torch.zeros((adapters, N, room), dtype=dtype, device=device)
+        self.scales = torch.zeros(adapters, dtype=torch.float32, device=device)
+        self.ranks = torch.zeros(adapters, dtype=torch.int32, device=device)
+
+    def load(self, i, a, b, scale=1.0):
+        """Adapter i: a [r, K], b [N, r] with r up to the bank's rank, and its scale."""
+        r = a.shape[0]
+        if a.dim() != 2 or b.dim() != 2 or r > self.rank or a.shape[1] != self.K or tuple(b.shape) != (self.N, r):
+            raise QGemmError(-3, f"LoraBank: an adapter is [r, {self.K}] and [{self.N}, r], r up to {self.rank}")
+        self.a[i, :r].copy_(a)
+        self.b[i, :, :r].copy_(b)
+        self.scales[i] = scale
+        self.ranks[i] = r
+        return self
+
+    def apply(self, x, ids, y, out=None, stream=None):
+        """y + the tokens' adapters (out may be y)."""
+        return lora_apply(x, ids, [self.a], [self.b], [y], self.scales, self.ranks, None if out is None else [out], stream)[0]

@@ -1,0 +1,208 @@
+"""Low-rank adapters beside shared projections (lora_apply) against the formula in float64."""
+import ctypes
+
+import pytest
+
+import mlxr_amd as mx
+from mlxr_amd import lora
+
+P = ctypes.c_void_p
+
+
+# ------------------------------------------------------------------------------ refusals (no GPU)
+
+def test_refusals():
+    L = lora._lib()
+
+    def call(count=1, tokens=4, K=256, adapters=3, rank=16, x=64, dt=mx.BF16, xs=256, ids=64, ws=64, nb=1 << 40, a=64, b=64,
+             y=64, out=64, N=32, ydt=mx.BF16):
+        items = (lora.Item * max(1, count))(*[lora.Item(a, b, y, out, N, ydt)] * max(1, count))
+        return L.mlxr_lora_apply(count, items, tokens, K, adapters, rank, P(x), dt, xs, P(ids), None, None, P(ws), nb, None)
+    assert call(count=0) == 0 and call(tokens=0) == 0
+    assert call(count=-1) == -1 and call(tokens=-1) == -1 and call(K=0) == -1 and call(adapters=0) == -1 and call(rank=0) == -1
+    assert call(adapters=4097) == -3 and call(rank=12) == -3 and call(rank=136) == -3 and call(K=252) == -3
+    assert call(tokens=(1 << 24) + 1) == -3
+    assert call(dt=mx.F32) == -1 and call(dt=3) == -1
+    for name in ("x", "ids", "ws", "a", "b", "y", "out"):
+        assert call(**{name: 0 if name in ("x", "ids", "ws") else None}) == -1, name
+    assert call(xs=252) == -3 and call(x=72) == -3 and call(ws=72) == -3 and call(a=72) == -3 and call(b=72) == -3
+    assert call(N=0) == -1 and call(ydt=3) == -1
+    assert call(nb=16) == -1 and "workspace" in L.mlxr_qgemm_last_error().decode()
+    n = ctypes.c_size_t()
+    assert L.mlxr_lora_workspace_size(1, 4, 256, 3, 16, None) == -1
+    assert L.mlxr_lora_workspace_size(1, 4, 256, 3, 17, ctypes.byref(n)) == -3
+    assert L.mlxr_lora_workspace_size(0, 4, 256, 3, 16, ctypes.byref(n)) == 0 and n.value == 0
+
+
+def test_wrapper_refusals():
+    import torch
+    x = torch.zeros((4, 256), dtype=torch.bfloat16)
+    with pytest.raises(mx.QGemmError, match="on a GPU"):
+        mx.lora_apply(x, torch.zeros(4, dtype=torch.int32), [], [], [])
+    with pytest.raises(mx.QGemmError, match="multiple of 8"):
+        mx.LoraBank(4, 16, 32, 100, device="cpu")
+    bank = mx.LoraBank(4, 12, 32, 64, device="cpu")
+    assert bank.a.shape == (4, 16, 64) and bank.b.shape == (4, 32, 16)
+    with pytest.raises(mx.QGemmError, match="up to 12"):
+        bank.load(0, torch.zeros(13, 64), torch.zeros(32, 13))
+    bank.load(2, torch.ones(5, 64), torch.ones(32, 5), 0.5)
+    assert bank.ranks.tolist() == [0, 0, 5, 0] and bank.scales.tolist() == [0, 0, 0.5, 0]
+
+
+# ------------------------------------------------------------------------------ values
+
+def _dt(name):
+    import torch
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def _make(cuda, tokens, K, adapters, rank, widths, dtype, ydt, seed, ids=None, ranks=None):
+    """Inputs whose A and B hold NaN past each adapter's rank."""
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(tokens, K, generator=g).to(_dt(dtype))
+    if ids is None:
+        ids = torch.randint(-1, adapters, (tokens,), generator=g)
+    ids = torch.as_tensor(ids).to(torch.int32)
+    ranks = torch.randint(0, rank + 1, (adapters,), generator=g) if ranks is None else torch.as_tensor(ranks)
+    a, b, y = [], [], []
+    for n in widths:
+        A, B = torch.randn(adapters, rank, K, generator=g) * K ** -0.5, torch.randn(adapters, n, rank, generator=g) * 0.3
+        for i, r in enumerate(ranks.tolist()):
+            A[i, r:] = float("nan")
+            B[i, :, r:] = float("nan")
+        a.append(A.to(_dt(dtype))), b.append(B.to(_dt(dtype))), y.append(torch.randn(tokens, n, generator=g).to(_dt(ydt)))
+    scales = torch.rand(adapters, generator=g) + 0.5
+    return x, ids, a, b, y, scales, ranks.to(torch.int32)
+
+
+def _formula(x, ids, A, B, y, scales, ranks):
+    """(result, what the error of the products is measured by) in float64."""
+    import torch
+    x, y = x.double(), y.double()
+    out, size = y.clone(), torch.zeros_like(y)
+    for i in set(ids.tolist()):
+        if 0 <= i < A.shape[0]:
+            r, rows = int(ranks[i]), torch.nonzero(ids == i)[:, 0]
+            a, b, s = A[i, :r].double(), B[i, :, :r].double(), float(scales[i])
+            out[rows] += s * (x[rows] @ a.t() @ b.t())
+            size[rows] = s * (x[rows].abs() @ a.abs().t() @ b.abs().t())
+    return out, size
+
+
+def _check(got, x, ids, A, B, y, scales, ranks, ydt):
+    """The products' fp32 sums of K and of rank terms are off by at most (K + rank + 64) 2^-24 of the sum of
+    magnitudes (64: joins of partial sums), h enters the second product with 2^-16; then one sum with y and one
+    rounding to y's type."""
+    import torch
+    ref, size = _formula(x, ids, A, B, y, scales, ranks)
+    got = got.double().cpu()
+    half = {"f32": 2.0 ** -23, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[ydt]
+    tol = ((A.shape[2] + A.shape[1] + 64) * 2.0 ** -24 + 2.0 ** -16) * size * 1.01 + half * ref.abs() + 2.0 ** -25
+    assert torch.isfinite(got).all()
+    bad = ((got - ref).abs() / tol).max()
+    assert float(bad) <= 1.0, float(bad)
+
+
+def _run(cuda, tokens, K, adapters, rank, widths, dtype="bf16", ydt=None, seed=0, **kw):
+    ydt = ydt or dtype
+    x, ids, a, b, y, scales, ranks = _make(cuda, tokens, K, adapters, rank, widths, dtype, ydt, seed, **kw)
+    got = mx.lora_apply(x.to(cuda), ids.to(cuda), [t.to(cuda) for t in a], [t.to(cuda) for t in b], [t.to(cuda) for t in y],
+                        scales.to(cuda), ranks.to(cuda))
+    for o, A, B, t in zip(got, a, b, y):
+        _check(o, x, ids, A, B, t, scales, ranks, ydt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,K,adapters,rank,widths", [
+    (1, 8, 1, 8, [1]), (1, 4096, 3, 16, [64]), (2, 264, 2, 8, [65, 3]), (8, 2048, 16, 16, [2048, 256, 256]),
+    (15, 520, 4, 24, [100]), (16, 1024, 1, 32, [257]), (17, 1024, 2, 40, [130, 64, 7, 12, 33]), (61, 2048, 24, 64, [500, 500]),
+    (100, 1000, 5, 128, [300]), (333, 256, 300, 8, [72]), (700, 512, 6, 16, [640]), (2048, 256, 3, 32, [96, 1024]),
+])
+def test_lora(cuda, dtype, tokens, K, adapters, rank, widths):
+    _run(cuda, tokens, K, adapters, rank, widths, dtype, seed=tokens)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ydt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_lora_output_types(cuda, dtype, ydt):
+    _run(cuda, 37, 512, 4, 16, [130, 64], dtype, ydt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ids", [[-1] * 40, [2] * 40, [3, 4, -5, 1 << 30] * 10, list(range(40)), [0] * 16 + [1] * 24, [0] * 17 + [-1] * 23])
+def test_lora_ids(cuda, ids):
+    _run(cuda, 40, 320, 41 if max(ids) == 39 else 3, 16, [96], ids=ids, ranks=[16] * (41 if max(ids) == 39 else 3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ranks", [[0, 0, 0], [1, 7, 9], [16, 15, 3], [2, 0, 16]])
+def test_lora_ranks(cuda, ranks):
+    _run(cuda, 30, 256, 3, 16, [64], ranks=ranks)
+
+
+@pytest.mark.gpu
+def test_lora_of_many_adapters(cuda):
+    _run(cuda, 500, 64, 4096, 8, [40], seed=1)
+
+
+@pytest.mark.gpu
+def test_lora_f16_products_outside_its_range(cuda):
+    """x . A^T far above 65504 and far below 2^-24 in f16: the products between are held in fp32."""
+    import torch
+    for size_a, size_b in ((3e4, 1e-4), (1e-7, 60.0)):
+        x, ids, a, b, y, scales, ranks = _make(cuda, 9, 2048, 2, 16, [80], "f16", "f32", 3, ranks=[16, 16])
+        a[0], b[0] = (a[0].float() * size_a).to(torch.float16), (b[0].float() * size_b).to(torch.float16)
+        x = (x.float() * (8 if size_a > 1 else 0.5)).to(torch.float16)
+        got = mx.lora_apply(x.to(cuda), ids.to(cuda), [a[0].to(cuda)], [b[0].to(cuda)], [y[0].to(cuda)], scales.to(cuda),
+                            ranks.to(cuda))
+        _check(got[0], x, ids, a[0], b[0], y[0], scales, ranks, "f32")
+
+
+@pytest.mark.gpu
+def test_lora_in_place_strided_and_on_another_stream(cuda):
+    import torch
+    x, ids, a, b, y, scales, ranks = _make(cuda, 50, 256, 4, 16, [72, 64], "bf16", "bf16", 5)
+    dev = lambda t: t.to(cuda)  # noqa: E731
+    ids, a, b, y, scales, ranks = dev(ids), list(map(dev, a)), list(map(dev, b)), list(map(dev, y)), dev(scales), dev(ranks)
+    want = mx.lora_apply(dev(x), ids, a, b, y, scales, ranks)
+    wide = torch.zeros(50, 400, dtype=torch.bfloat16, device=cuda)
+    wide[:, 64:320] = dev(x)
+    odd = torch.zeros(50, 401, dtype=torch.bfloat16, device=cuda)
+    odd[:, 3:259] = dev(x)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    for xs in (wide[:, 64:320], odd[:, 3:259]):
+        for stream in (None, s):
+            got = mx.lora_apply(xs, ids, a, b, y, scales, ranks, stream=stream)
+            torch.cuda.current_stream().wait_stream(s)
+            assert all(torch.equal(g, w) for g, w in zip(got, want))
+            s.wait_stream(torch.cuda.current_stream())
+    mine = [t.clone() for t in y]
+    assert mx.lora_apply(dev(x), ids, a, b, mine, scales, ranks, outs=mine)[0] is mine[0]
+    assert all(torch.equal(g, w) for g, w in zip(mine, want))
+    with pytest.raises(mx.QGemmError, match="x's dtype"):
+        mx.lora_apply(dev(x), ids, [t.half() for t in a], b, y, scales, ranks)
+
+
+@pytest.mark.gpu
+def test_lora_bank(cuda):
+    import torch
+    bank = mx.LoraBank(3, 20, 96, 256, device=cuda)
+    torch.manual_seed(4)
+    parts = []
+    for i, r in enumerate((4, 20, 9)):
+        A, B = torch.randn(r, 256) / 16, torch.randn(96, r) / 4
+        bank.load(i, A, B, 0.5 * i + 1)
+        parts.append((A.to(torch.bfloat16).double(), B.to(torch.bfloat16).double(), 0.5 * i + 1))
+    x, y = torch.randn(7, 256).to(torch.bfloat16), torch.randn(7, 96)
+    ids = torch.tensor([2, 0, -1, 1, 1, 2, 0], dtype=torch.int32)
+    got = bank.apply(x.to(cuda), ids.to(cuda), y.to(cuda))
+    for t, i in enumerate(ids.tolist()):
+        ref = y[t].double()
+        if i >= 0:
+            A, B, s = parts[i]
+            ref = ref + s * (x[t].double() @ A.t() @ B.t())
+        assert float((got[t].double().cpu() - ref).abs().max()) < 1e-3

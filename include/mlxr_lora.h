@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-enum { MLXR_LORA_MAX_ADAPTERS = 4096, MLXR_LORA_MAX_RANK = 128 };
+enum { MLXR_LORA_MAX_ADAPTERS = 4096, MLXR_LORA_MAX_RANK = 128, MLXR_LORA_MAX_TOKENS = 1 << 20 };
 
 typedef struct mlxr_lora_item {
   const void* a_dev; /* [adapters, rank, K] of x's type, contiguous */

@@ -2,11 +2,14 @@
 //
 //   out[t] = y[t] + s_a h_t B_a^T,   h_t = x_t A_a^T,   a = ids[t]
 //
-// Three launches: the tokens are sorted by adapter into tiles of up to 16 tokens of one adapter;
-// h for each tile, K split over workgroups (fp32 partial sums in the workspace); the second
-// product with the partial sums added up, and y.  Both products take the adapter's rows as the
-// A operand and the tile's tokens as columns of the matrix instructions.
+// Tokens of one adapter are brought together in tiles, the columns of the matrix instructions; the
+// adapter's rows of A and B are their other operand, read once for a tile.  The first launch
+// computes h, K split over workgroups (fp32 partial sums in the workspace); the second adds the
+// partial sums up, multiplies with B and adds y.  Up to kInline tokens, each workgroup finds its
+// tile among the ids by itself; above, a launch before sorts the tokens.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "../../include/mlxr_lora.h"
 #include "mfma16.h"
@@ -16,8 +19,15 @@ namespace mlxr {
 
 namespace {
 
-constexpr int kTokens = 16;  // of a tile
-constexpr int kItems = 4;    // projections of one launch
+constexpr int kItems = 4;      // projections of one launch
+constexpr int kThreads = 256;  // of shrink and expand
+constexpr int kWaves = kThreads / 64;
+constexpr int kInline = kThreads;  // tokens
+// Groups of 16 tokens in a tile of the sorted tokens: the accumulators of a wavefront, sub * rank / 16 of
+// four registers, and what the wavefronts of a workgroup add up in LDS, stay at 16.
+constexpr int sub_of(int rank_groups) { return rank_groups > 4 ? 2 : 4; }
+constexpr int rank_groups_of(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
+constexpr int kMaxSplits = 8;  // of K
 constexpr int kPlanThreads = 1024;
 
 struct Tile {
@@ -33,7 +43,7 @@ struct LoraArgs {
   int32_t* counts;  // tiles with an adapter, all tiles
   Tile* tiles;
   float* h;  // [count][splits][tokens][rank]
-  int count, tokens, K, adapters, rank, splits, chunk;
+  int count, tokens, K, adapters, rank, splits, chunk, columns;
 };
 
 __device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
@@ -43,7 +53,7 @@ __device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
 // Tokens sorted by adapter, and the tiles; the last bucket holds the tokens without one.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   extern __shared__ int sh[];
-  const int nb = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int TM = 16 * sub_of(rank_groups_of(a.rank)), nb = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int *count = sh, *next = sh + nb;
   __shared__ int part[2 * kPlanThreads / 64];
   for (int b = tid; b < nb; b += kPlanThreads) count[b] = 0;
@@ -56,7 +66,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   __syncthreads();
   const int per = (nb + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, nb), b1 = min(b0 + per, nb);
   int n = 0, m = 0;
-  for (int b = b0; b < b1; ++b) n += count[b], m += (count[b] + kTokens - 1) / kTokens;
+  for (int b = b0; b < b1; ++b) n += count[b], m += (count[b] + TM - 1) / TM;
   int sn = n, sm = m;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -72,136 +82,277 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
     next[b] = at;
     if (b == a.adapters) {
       a.counts[0] = tile;
-      a.counts[1] = tile + (c + kTokens - 1) / kTokens;
+      a.counts[1] = tile + (c + TM - 1) / TM;
     }
-    for (int i = 0; i < c; i += kTokens) a.tiles[tile++] = {b, at + i, min(kTokens, c - i)};
+    for (int i = 0; i < c; i += TM) a.tiles[tile++] = {b, at + i, min(TM, c - i)};
     at += c;
   }
   __syncthreads();
+  // which place of its adapter a token gets depends on the order of the atomics; no value does
   for (int t = tid; t < a.tokens; t += kPlanThreads) a.order[atomicAdd(&next[bucket(t)], 1)] = t;
 }
 
-// h of one tile over one chunk of K: four wavefronts take a quarter each and add up in LDS.
-// RT: tiles of 16 ranks.
-template <bool F16, int RT>
-__global__ __launch_bounds__(256) void shrink_kernel(LoraArgs a) {
-  if ((int)blockIdx.x >= a.counts[0]) return;
-  __shared__ float sh[3][RT][64][4];
-  const Tile t = a.tiles[blockIdx.x];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int split = blockIdx.y, item = blockIdx.z, rank = rank_of(a, t.adapter);
-  const int k_end = min((split + 1) * a.chunk, a.K);
-  const bool tok = col < t.count;
-  const uint16_t* x = a.x + (int64_t)a.order[t.first + (tok ? col : 0)] * a.x_stride;
-  const uint16_t* A = (const uint16_t*)a.item[item].a_dev + (int64_t)t.adapter * a.rank * a.K;
-  f32x4_t acc[RT] = {};
-  for (int k = split * a.chunk + wave * 32; k < k_end; k += 4 * 32) {
-    const int kk = k + 8 * g;
-    const bool in = kk < k_end;
-    const u32x4_t xf = tok && in ? *(const u32x4_t*)(x + kk) : u32x4_t{0, 0, 0, 0};
+// Tile `index`: its adapter (a.adapters: none), its tokens in token[0 .. count).  count 0: there is no such
+// tile.  INLINE: tile t exists if token t is the 1st, 17th, 33rd .. of its adapter, and holds it and the next 15.
+template <bool INLINE>
+__device__ __forceinline__ int tile_tokens(const LoraArgs& a, int index, int* adapter, int* token) {
+  const int tid = threadIdx.x;
+  if constexpr (INLINE) {
+    __shared__ uint64_t same[kWaves];
+    const int lane = tid & 63, wave = tid >> 6;
+    auto bucket = [&](int id) { return id >= 0 && id < a.adapters ? id : a.adapters; };
+    const int mine = bucket(a.ids[index]);
+    const bool eq = tid < a.tokens && bucket(a.ids[min(tid, a.tokens - 1)]) == mine;
+    const uint64_t vote = __ballot(eq);
+    if (lane == 0) same[wave] = vote;
+    __syncthreads();
+    int before = 0, at = 0, all = 0;  // of the adapter: tokens before `index`, before this thread's, all
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      const int row = 16 * r + col;
-      const u32x4_t af = in && row < rank ? *(const u32x4_t*)(A + (int64_t)row * a.K + kk) : u32x4_t{0, 0, 0, 0};
-      acc[r] = mfma16<F16>(af, xf, acc[r]);
+    for (int w = 0; w < kWaves; ++w) {
+      const uint64_t v = same[w];
+      const int n = __popcll(v);
+      before += w < (index >> 6) ? n : w == (index >> 6) ? __popcll(v & ((1ull << (index & 63)) - 1)) : 0;
+      at += w < wave ? n : w == wave ? __popcll(v & ((1ull << lane) - 1)) : 0;
+      all += n;
     }
-  }
-  if (wave)
-#pragma unroll
-    for (int r = 0; r < RT; ++r) *(f32x4_t*)sh[wave - 1][r][lane] = acc[r];
-  __syncthreads();
-  if (wave || !tok) return;
-  float* h = a.h + (((int64_t)item * a.splits + split) * a.tokens + t.first + col) * a.rank;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-#pragma unroll
-    for (int w = 0; w < 3; ++w) acc[r] += *(const f32x4_t*)sh[w][r][lane];
-    if (16 * r + 4 * g < a.rank) *(f32x4_t*)(h + 16 * r + 4 * g) = acc[r];
+    if (before & 15) return 0;
+    if (eq && at >= before && at < before + 16) token[at - before] = tid;
+    *adapter = mine;
+    __syncthreads();
+    return min(16, all - before);
+  } else {
+    if (index >= a.counts[1]) return 0;
+    const Tile t = a.tiles[index];
+    if (tid < t.count) token[tid] = a.order[t.first + tid];
+    *adapter = t.adapter;
+    __syncthreads();
+    return t.count;
   }
 }
 
-// 64 columns of one tile for each wavefront.  Row 4 g + i of the c-th product is column 16 g + 4 c + i
-// of the 64, so a lane ends with 16 neighbouring columns of its token.
-template <bool F16, int RT>
-__global__ __launch_bounds__(256) void expand_kernel(LoraArgs a) {
-  if ((int)blockIdx.x >= a.counts[1]) return;
-  constexpr int KT = (RT + 1) / 2;
-  const Tile t = a.tiles[blockIdx.x];
+// h of one tile over one chunk of K: the wavefronts take turns over it in steps of 64 and add up in LDS.
+// RT: groups of 16 ranks; SUB: of 16 tokens.  A lane reads 32 neighbouring bytes of a row of x or A,
+// the four lane groups 128: which k an operand's place stands for is free, alike for both.
+template <bool F16, int RT, int SUB, bool INLINE>
+__global__ __launch_bounds__(kThreads) void shrink_kernel(LoraArgs a) {
+  __shared__ int token[16 * SUB];
+  __shared__ f32x4_t sh[kWaves - 1][SUB * RT][64];
+  int adapter = 0;
+  const int count = tile_tokens<INLINE>(a, blockIdx.x, &adapter, token);
+  if (count == 0 || adapter == a.adapters) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const mlxr_lora_item& it = a.item[blockIdx.z];
-  const int n0 = (blockIdx.y * 4 + wave) * 64;
-  if (n0 >= it.N) return;
-  f32x4_t acc[4] = {};
-  float back = 1.f;
-  if (t.adapter < a.adapters) {
-    const int rank = rank_of(a, t.adapter);
-    const float scale = a.scales ? a.scales[t.adapter] : 1.f;
-    float h[KT][8];
-    float top = 0.f;
+  const int split = blockIdx.y, item = blockIdx.z, rank = rank_of(a, adapter);
+  const int k_end = min((split + 1) * a.chunk, a.K);
+  const uint16_t* A = (const uint16_t*)a.item[item].a_dev + (int64_t)adapter * a.rank * a.K + (int64_t)col * a.K;
+  const uint16_t* x[SUB];
 #pragma unroll
-    for (int k = 0; k < KT; ++k) {
-      const int at = 32 * k + 8 * g;
+  for (int s = 0; s < SUB; ++s) x[s] = a.x + (int64_t)token[16 * s + col < count ? 16 * s + col : 0] * a.x_stride;
+  f32x4_t acc[SUB][RT] = {};
+  u32x4_t xf[SUB][2], af[RT][2];
+  auto load = [&](int k) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[k][e] = 0.f;
-      if (col < t.count && at < rank)
-        for (int s = 0; s < a.splits; ++s) {
-          const float* p = a.h + (((int64_t)blockIdx.z * a.splits + s) * a.tokens + t.first + col) * a.rank + at;
-          const f32x4_t lo = *(const f32x4_t*)p, hi = *(const f32x4_t*)(p + 4);
+    for (int e = 0; e < 2; ++e) {
+      const int kk = k + 16 * g + 8 * e;
+      const bool in = kk < k_end;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) h[k][e] += lo[e], h[k][4 + e] += hi[e];
-        }
+      for (int s = 0; s < SUB; ++s) xf[s][e] = in ? *(const u32x4_t*)(x[s] + kk) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        h[k][e] *= scale;
-        top = fmaxf(top, fabsf(h[k][e]));
+      for (int r = 0; r < RT; ++r)
+        af[r][e] = in && 16 * r + col < rank ? *(const u32x4_t*)(A + (int64_t)(16 * r) * a.K + kk) : u32x4_t{0, 0, 0, 0};
+    }
+  };
+  int k = split * a.chunk + wave * 64;
+  load(k);
+  while (k < k_end) {
+    u32x4_t xc[SUB][2], ac[RT][2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) xc[s][e] = xf[s][e];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) ac[r][e] = af[r][e];
+    }
+    k += kWaves * 64;
+    load(k);  // nothing past k_end is read
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[s][r] = mfma16<F16>(ac[r][e], xc[s][e], acc[s][r]);
+  }
+  if (wave)
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) sh[wave - 1][s * RT + r][lane] = acc[s][r];
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int s = 0; s < SUB; ++s) {
+    if (16 * s + col >= count) continue;
+    float* h = a.h + (((int64_t)item * a.splits + split) * a.tokens + token[16 * s + col]) * a.rank + 4 * g;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      f32x4_t v = acc[s][r];
+#pragma unroll
+      for (int w = 0; w < kWaves - 1; ++w) v += sh[w][s * RT + r][lane];
+      if (16 * r + 4 * g < a.rank) *(f32x4_t*)(h + 16 * r) = v;
+    }
+  }
+}
+
+// 16 neighbouring columns n .. of a token's row: out = y + v.  Rows start at multiples of 16 bytes where vec.
+template <int YT>
+__device__ __forceinline__ void add_row(const mlxr_lora_item& it, int64_t row, int n, const f32x4_t* v, float back, bool vec) {
+  if (vec && n + 16 <= it.N) {
+    if constexpr (YT == DT_F32) {
+      const f32x4_t* y = (const f32x4_t*)((const float*)it.y_dev + row + n);
+      f32x4_t* o = (f32x4_t*)((float*)it.out_dev + row + n);
+      f32x4_t in[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) in[c] = y[c];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[c] = in[c] + v[c] * back;
+    } else {
+      constexpr bool F = YT == DT_F16;
+      const u32x4_t* y = (const u32x4_t*)((const uint16_t*)it.y_dev + row + n);
+      u32x4_t* o = (u32x4_t*)((uint16_t*)it.out_dev + row + n);
+      const u32x4_t in[2] = {y[0], y[1]};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        u32x4_t w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = pack2<F>(unpack<F>(in[c][e], 0) + v[2 * c + (e >> 1)][2 * (e & 1)] * back,
+                          unpack<F>(in[c][e], 1) + v[2 * c + (e >> 1)][2 * (e & 1) + 1] * back);
+        o[c] = w;
       }
     }
-    if constexpr (F16) {  // h may lie outside f16: a power of two brings the token's largest to [1/2, 1)
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (top > 0.f && top < INFINITY) {
-        const int e = __builtin_amdgcn_frexp_expf(top);
-        back = __builtin_amdgcn_ldexpf(1.f, e);
-#pragma unroll
-        for (int k = 0; k < KT; ++k)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) h[k][i] = __builtin_amdgcn_ldexpf(h[k][i], -e);
-      }
-    }
-    const uint16_t* B = (const uint16_t*)it.b_dev + (int64_t)t.adapter * it.N * a.rank;
-#pragma unroll
-    for (int k = 0; k < KT; ++k) {
-      u32x4_t hi, lo;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        hi[e] = pack2<F16>(h[k][2 * e], h[k][2 * e + 1]);
-        const float d0 = h[k][2 * e] - unpack<F16>(hi[e], 0), d1 = h[k][2 * e + 1] - unpack<F16>(hi[e], 1);
-        lo[e] = pack2<F16>(d0 == d0 ? d0 : 0.f, d1 == d1 ? d1 : 0.f);  // an infinite h stays infinite
-      }
-      const int at = 32 * k + 8 * g, left = rank - at;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int n = n0 + 16 * (col >> 2) + 4 * c + (col & 3);
-        u32x4_t bf = n < it.N && left > 0 ? *(const u32x4_t*)(B + (int64_t)n * a.rank + at) : u32x4_t{0, 0, 0, 0};
-        if (left < 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) bf[e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
-        acc[c] = mfma16<F16>(bf, lo, acc[c]);
-        acc[c] = mfma16<F16>(bf, hi, acc[c]);
-      }
-    }
-  } else if (it.out_dev == it.y_dev) {
     return;
   }
-  if (col >= t.count) return;
-  const int64_t row = (int64_t)a.order[t.first + col] * it.N;
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = n0 + 16 * g + 4 * c + i;
-      if (n < it.N) store_scalar(it.out_dev, it.y_dtype, row + n, load_scalar(it.y_dev, it.y_dtype, row + n) + acc[c][i] * back);
+    for (int i = 0; i < 4; ++i)
+      if (n + 4 * c + i < it.N)
+        store_scalar(it.out_dev, YT, row + n + 4 * c + i, load_scalar(it.y_dev, YT, row + n + 4 * c + i) + v[c][i] * back);
+}
+
+// One tile and `columns` columns of an item, in steps of 64 for each wavefront.  Row 4 g + i of the c-th
+// product of a step is column 16 g + 4 c + i, so a lane ends with 16 neighbouring columns of its token.  h enters
+// as the sum of two 16-bit parts: rounded to one it would lose what the fp32 sums kept.
+template <bool F16, int RT, int SUB, bool INLINE>
+__global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
+  constexpr int R = 16 * RT, KT = RT == 1 ? 1 : RT / 2;
+  constexpr int ROW = 2 * R + 8;  // of LDS: R high parts, R low parts; padded against bank conflicts
+  __shared__ int token[16 * SUB];
+  __shared__ float back[16 * SUB];
+  __shared__ __attribute__((aligned(16))) uint16_t hs[16 * SUB * ROW];
+  const mlxr_lora_item& it = a.item[blockIdx.z];
+  const int begin = blockIdx.x * a.columns;
+  if (begin >= it.N) return;
+  int adapter = 0;
+  const int count = tile_tokens<INLINE>(a, blockIdx.y, &adapter, token);
+  if (count == 0) return;
+  const bool none = adapter == a.adapters;
+  if (none && it.out_dev == it.y_dev) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int rank = none ? 0 : rank_of(a, adapter);
+  if (!none) {
+    const float scale = a.scales ? a.scales[adapter] : 1.f;
+    // 8 ranks of a token for each thread, a token's threads side by side
+    for (int u = threadIdx.x; u < 16 * SUB * 2 * RT; u += kThreads) {
+      const int t = u / (2 * RT), at = 8 * (u % (2 * RT));
+      f32x4_t v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      if (t < count && at < rank) {
+        const float* p = a.h + ((int64_t)blockIdx.z * a.splits * a.tokens + token[t]) * a.rank + at;
+        const int64_t step = (int64_t)a.tokens * a.rank;
+        f32x4_t in[kMaxSplits][2];
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) in[s][e] = s < a.splits ? *(const f32x4_t*)(p + s * step + 4 * e) : f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) v[e] += in[s][e];
+      }
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        v[e] *= scale;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[e][i]));
+      }
+      if constexpr (F16) {  // h may lie outside f16: a power of two brings the token's largest to [1/2, 1)
+#pragma unroll
+        for (int d = 1; d < 2 * RT; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+        const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+        if (at == 0) back[t] = __builtin_amdgcn_ldexpf(1.f, e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = __builtin_amdgcn_ldexpf(v[i >> 2][i & 3], -e);
+      }
+      u32x4_t hi, lo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v0 = v[e >> 1][2 * (e & 1)], v1 = v[e >> 1][2 * (e & 1) + 1];
+        hi[e] = pack2<F16>(v0, v1);
+        const float d0 = v0 - unpack<F16>(hi[e], 0), d1 = v1 - unpack<F16>(hi[e], 1);
+        lo[e] = pack2<F16>(d0 == d0 ? d0 : 0.f, d1 == d1 ? d1 : 0.f);  // an infinite h stays infinite
+      }
+      *(u32x4_t*)(hs + t * ROW + at) = hi;
+      *(u32x4_t*)(hs + t * ROW + R + at) = lo;
     }
+    __syncthreads();
+  }
+  const bool vec = (it.N * (it.y_dtype == DT_F32 ? 4 : 2)) % 16 == 0 && (((uintptr_t)it.y_dev | (uintptr_t)it.out_dev) & 15) == 0;
+  const uint16_t* B = (const uint16_t*)it.b_dev + (int64_t)(none ? 0 : adapter) * it.N * a.rank;
+  const int end = min(begin + a.columns, it.N);
+  for (int n0 = begin + wave * 64; n0 < end; n0 += kWaves * 64) {
+    // operands of B: RT 1 multiplies the high and the low parts in one step, ranks 8 (g & 1) ..
+    u32x4_t bf[KT][4];
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int n = n0 + 16 * (col >> 2) + 4 * c + (col & 3), at = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g, left = rank - at;
+        bf[k][c] = n < it.N && left > 0 ? *(const u32x4_t*)(B + (int64_t)n * a.rank + at) : u32x4_t{0, 0, 0, 0};
+        if (left < 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bf[k][c][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
+      }
+#pragma unroll 1
+    for (int s = 0; s < SUB; ++s) {
+      if (16 * s >= count) break;
+      f32x4_t acc[4] = {};
+      if (!none) {
+        const uint16_t* h = hs + (16 * s + col) * ROW;
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+          if constexpr (RT == 1) {
+            const u32x4_t f = *(const u32x4_t*)(h + 8 * g);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[c] = mfma16<F16>(bf[k][c], f, acc[c]);
+          } else {
+            const u32x4_t hi = *(const u32x4_t*)(h + 32 * k + 8 * g), lo = *(const u32x4_t*)(h + R + 32 * k + 8 * g);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              acc[c] = mfma16<F16>(bf[k][c], lo, acc[c]);
+              acc[c] = mfma16<F16>(bf[k][c], hi, acc[c]);
+            }
+          }
+        }
+      }
+      if (16 * s + col < count) {
+        const int64_t row = (int64_t)token[16 * s + col] * it.N;
+        const float f = F16 && !none ? back[16 * s + col] : 1.f;
+        if (it.y_dtype == DT_BF16) add_row<DT_BF16>(it, row, n0 + 16 * g, acc, f, vec);
+        else if (it.y_dtype == DT_F16) add_row<DT_F16>(it, row, n0 + 16 * g, acc, f, vec);
+        else add_row<DT_F32>(it, row, n0 + 16 * g, acc, f, vec);
+      }
+    }
+  }
 }
 
 struct Layout {
@@ -210,15 +361,14 @@ struct Layout {
 };
 Layout layout_of(int count, int tokens, int K, int adapters, int rank) {
   Layout l;
-  const int items = count < kItems ? count : kItems;
+  const int items = count < kItems ? count : kItems, tm = 16 * sub_of(rank_groups_of(rank));
   const int buckets = tokens < adapters + 1 ? tokens : adapters + 1;
-  l.tiles = tokens / kTokens + buckets;
-  if (l.tiles > tokens) l.tiles = tokens;
-  // enough workgroups for the device; a wavefront takes at least two steps of 32
+  l.tiles = tokens <= kInline ? tokens : (tokens / tm + buckets < tokens ? tokens / tm + buckets : tokens);
+  // enough workgroups for the device; a wavefront takes two steps of K or more
   const long want = 512 / ((long)l.tiles * items) + 1;
-  const int most = (K + 255) / 256;
+  const int most = std::min(kMaxSplits, (K + 511) / 512);
   int splits = (int)(want < most ? want : most);
-  l.chunk = ((K + splits - 1) / splits + 31) / 32 * 32;
+  l.chunk = ((K + splits - 1) / splits + 63) / 64 * 64;
   l.splits = (K + l.chunk - 1) / l.chunk;
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   l.order = 0;
@@ -229,19 +379,25 @@ Layout layout_of(int count, int tokens, int K, int adapters, int rank) {
   return l;
 }
 
-template <bool F16, int RT>
+template <bool F16, int RT, int SUB, bool INLINE>
 void launch(const LoraArgs& a, int tiles, hipStream_t s) {
   int wide = 0;
   for (int i = 0; i < a.count; ++i) wide = wide > a.item[i].N ? wide : a.item[i].N;
-  shrink_kernel<F16, RT><<<dim3(tiles, a.splits, a.count), 256, 0, s>>>(a);
-  expand_kernel<F16, RT><<<dim3(tiles, (wide + 255) / 256, a.count), 256, 0, s>>>(a);
+  shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles, a.splits, a.count), kThreads, 0, s>>>(a);
+  expand_kernel<F16, RT, SUB, INLINE><<<dim3((wide + a.columns - 1) / a.columns, tiles, a.count), kThreads, 0, s>>>(a);
+}
+template <bool F16, int RT>
+void launch_tokens(const LoraArgs& a, int tiles, hipStream_t s) {
+  if (a.tokens <= kInline) launch<F16, RT, 1, true>(a, tiles, s);
+  else launch<F16, RT, sub_of(RT), false>(a, tiles, s);
 }
 template <bool F16>
 void launch_rank(const LoraArgs& a, int tiles, hipStream_t s) {
-  if (a.rank <= 16) launch<F16, 1>(a, tiles, s);
-  else if (a.rank <= 32) launch<F16, 2>(a, tiles, s);
-  else if (a.rank <= 64) launch<F16, 4>(a, tiles, s);
-  else launch<F16, 8>(a, tiles, s);
+  const int n = rank_groups_of(a.rank);
+  if (n == 1) launch_tokens<F16, 1>(a, tiles, s);
+  else if (n == 2) launch_tokens<F16, 2>(a, tiles, s);
+  else if (n == 4) launch_tokens<F16, 4>(a, tiles, s);
+  else launch_tokens<F16, 8>(a, tiles, s);
 }
 
 int check_lora(int count, int tokens, int K, int adapters, int rank) {
@@ -251,7 +407,7 @@ int check_lora(int count, int tokens, int K, int adapters, int rank) {
   if (rank % 8 || rank > MLXR_LORA_MAX_RANK)
     return set_error(MLXR_E_SHAPE, "lora: rank must be a multiple of 8 and at most %d", MLXR_LORA_MAX_RANK);
   if (K % 8) return set_error(MLXR_E_SHAPE, "lora: K must be a multiple of 8");
-  if (tokens > (1 << 24)) return set_error(MLXR_E_SHAPE, "lora: at most %d tokens", 1 << 24);
+  if (tokens > MLXR_LORA_MAX_TOKENS) return set_error(MLXR_E_SHAPE, "lora: at most %d tokens", MLXR_LORA_MAX_TOKENS);
   return MLXR_OK;
 }
 
@@ -298,10 +454,11 @@ extern "C" int mlxr_lora_apply(int count, const mlxr_lora_item* items, int token
   a.order = (int32_t*)(ws + l.order), a.counts = (int32_t*)(ws + l.counts), a.tiles = (Tile*)(ws + l.tile);
   a.h = (float*)(ws + l.h);
   a.tokens = tokens, a.K = K, a.adapters = adapters, a.rank = rank, a.splits = l.splits, a.chunk = l.chunk;
+  a.columns = 64 * kWaves;
   for (int i = 0; i < count; i += kItems) {
     a.count = count - i < kItems ? count - i : kItems;
     for (int j = 0; j < a.count; ++j) a.item[j] = items[i + j];
-    if (i == 0) plan_kernel<<<1, kPlanThreads, (size_t)(adapters + 1) * 8, s>>>(a);
+    if (i == 0 && tokens > kInline) plan_kernel<<<1, kPlanThreads, (size_t)(adapters + 1) * 8, s>>>(a);
     if (x_dtype == MLXR_F16) launch_rank<true>(a, l.tiles, s);
     else launch_rank<false>(a, l.tiles, s);
   }

@@ -10,6 +10,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/mlxr_lora.h"
 #include "mfma16.h"
@@ -20,8 +21,9 @@ namespace mlxr {
 namespace {
 
 constexpr int kItems = 4;      // projections of one launch
-constexpr int kThreads = 256;  // of shrink and expand
+constexpr int kThreads = 256;  // of expand, and of shrink over 64-token tiles
 constexpr int kWaves = kThreads / 64;
+constexpr int kShrinkWide = 512;  // threads of shrink over 16-token tiles
 constexpr int kInline = kThreads;  // tokens
 // Groups of 16 tokens in a tile of the sorted tokens: the accumulators of a wavefront, sub * rank / 16 of
 // four registers, and what the wavefronts of a workgroup add up in LDS, stay at 16.
@@ -29,6 +31,7 @@ constexpr int sub_of(int rank_groups) { return rank_groups > 4 ? 2 : 4; }
 constexpr int rank_groups_of(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 constexpr int kMaxSplits = 8;  // of K
 constexpr int kPlanThreads = 1024;
+constexpr int kExpandGroups = 2048;  // workgroups of expand: eight for each CU
 
 struct Tile {
   int adapter, first, count;  // tokens order[first .. first + count)
@@ -50,6 +53,25 @@ __device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
   return a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
 }
 
+// counter[b] + 1 for each active lane with its own b; returns a place of its own, as atomicAdd would.
+__device__ __forceinline__ int wave_add(int* counter, int b) {
+  const int lane = threadIdx.x & 63;
+  int at = 0;
+  bool done = false;
+  while (!done) {
+    const int first = __builtin_amdgcn_readfirstlane(b);
+    const uint64_t same = __ballot(b == first);
+    if (b == first) {
+      const int leader = __builtin_ctzll(same);
+      int base = 0;
+      if (lane == leader) base = atomicAdd(&counter[b], __popcll(same));
+      at = __shfl(base, leader) + __popcll(same & ((1ull << lane) - 1));
+      done = true;
+    }
+  }
+  return at;
+}
+
 // Tokens sorted by adapter, and the tiles; the last bucket holds the tokens without one.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   extern __shared__ int sh[];
@@ -62,7 +84,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
     const int id = a.ids[t];
     return id >= 0 && id < a.adapters ? id : a.adapters;
   };
-  for (int t = tid; t < a.tokens; t += kPlanThreads) atomicAdd(&count[bucket(t)], 1);
+  // one atomic for the lanes of a wavefront that share a bucket: neighbouring tokens often do
+  for (int t = tid; t < a.tokens; t += kPlanThreads) {
+    const int b = bucket(t);
+    wave_add(count, b);
+  }
   __syncthreads();
   const int per = (nb + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, nb), b1 = min(b0 + per, nb);
   int n = 0, m = 0;
@@ -89,16 +115,16 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   }
   __syncthreads();
   // which place of its adapter a token gets depends on the order of the atomics; no value does
-  for (int t = tid; t < a.tokens; t += kPlanThreads) a.order[atomicAdd(&next[bucket(t)], 1)] = t;
+  for (int t = tid; t < a.tokens; t += kPlanThreads) a.order[wave_add(next, bucket(t))] = t;
 }
 
 // Tile `index`: its adapter (a.adapters: none), its tokens in token[0 .. count).  count 0: there is no such
 // tile.  INLINE: tile t exists if token t is the 1st, 17th, 33rd .. of its adapter, and holds it and the next 15.
-template <bool INLINE>
+template <bool INLINE, int WAVES>
 __device__ __forceinline__ int tile_tokens(const LoraArgs& a, int index, int* adapter, int* token) {
   const int tid = threadIdx.x;
   if constexpr (INLINE) {
-    __shared__ uint64_t same[kWaves];
+    __shared__ uint64_t same[WAVES];
     const int lane = tid & 63, wave = tid >> 6;
     auto bucket = [&](int id) { return id >= 0 && id < a.adapters ? id : a.adapters; };
     const int mine = bucket(a.ids[index]);
@@ -108,7 +134,7 @@ __device__ __forceinline__ int tile_tokens(const LoraArgs& a, int index, int* ad
     __syncthreads();
     int before = 0, at = 0, all = 0;  // of the adapter: tokens before `index`, before this thread's, all
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const uint64_t v = same[w];
       const int n = __popcll(v);
       before += w < (index >> 6) ? n : w == (index >> 6) ? __popcll(v & ((1ull << (index & 63)) - 1)) : 0;
@@ -134,11 +160,12 @@ __device__ __forceinline__ int tile_tokens(const LoraArgs& a, int index, int* ad
 // RT: groups of 16 ranks; SUB: of 16 tokens.  A lane reads 32 neighbouring bytes of a row of x or A,
 // the four lane groups 128: which k an operand's place stands for is free, alike for both.
 template <bool F16, int RT, int SUB, bool INLINE>
-__global__ __launch_bounds__(kThreads) void shrink_kernel(LoraArgs a) {
+__global__ __launch_bounds__(SUB == 1 ? kShrinkWide : kThreads) void shrink_kernel(LoraArgs a) {
+  constexpr int kWaves = (SUB == 1 ? kShrinkWide : kThreads) / 64;
   __shared__ int token[16 * SUB];
   __shared__ f32x4_t sh[kWaves - 1][SUB * RT][64];
   int adapter = 0;
-  const int count = tile_tokens<INLINE>(a, blockIdx.x, &adapter, token);
+  const int count = tile_tokens<INLINE, kWaves>(a, blockIdx.x, &adapter, token);
   if (count == 0 || adapter == a.adapters) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int split = blockIdx.y, item = blockIdx.z, rank = rank_of(a, adapter);
@@ -202,42 +229,46 @@ __global__ __launch_bounds__(kThreads) void shrink_kernel(LoraArgs a) {
   }
 }
 
-// 16 neighbouring columns n .. of a token's row: out = y + v.  Rows start at multiples of 16 bytes where vec.
+// 16 neighbouring columns n .. of a token's row of y, as they lie in memory (YT: the type); rows start at
+// multiples of 16 bytes where vec.
 template <int YT>
-__device__ __forceinline__ void add_row(const mlxr_lora_item& it, int64_t row, int n, const f32x4_t* v, float back, bool vec) {
-  if (vec && n + 16 <= it.N) {
-    if constexpr (YT == DT_F32) {
-      const f32x4_t* y = (const f32x4_t*)((const float*)it.y_dev + row + n);
-      f32x4_t* o = (f32x4_t*)((float*)it.out_dev + row + n);
-      f32x4_t in[4];
+struct Cols {
+  static constexpr int W = YT == DT_F32 ? 4 : 2;
+  u32x4_t w[W];
+  __device__ __forceinline__ void load(const mlxr_lora_item& it, int64_t row, int n, bool vec) {
+    if (!vec || n + 16 > it.N) return;
+    const u32x4_t* y = (const u32x4_t*)((const uint8_t*)it.y_dev + (row + n) * (YT == DT_F32 ? 4 : 2));
 #pragma unroll
-      for (int c = 0; c < 4; ++c) in[c] = y[c];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] = in[c] + v[c] * back;
-    } else {
-      constexpr bool F = YT == DT_F16;
-      const u32x4_t* y = (const u32x4_t*)((const uint16_t*)it.y_dev + row + n);
-      u32x4_t* o = (u32x4_t*)((uint16_t*)it.out_dev + row + n);
-      const u32x4_t in[2] = {y[0], y[1]};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        u32x4_t w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          w[e] = pack2<F>(unpack<F>(in[c][e], 0) + v[2 * c + (e >> 1)][2 * (e & 1)] * back,
-                          unpack<F>(in[c][e], 1) + v[2 * c + (e >> 1)][2 * (e & 1) + 1] * back);
-        o[c] = w;
-      }
-    }
-    return;
+    for (int c = 0; c < W; ++c) w[c] = y[c];
   }
+  // out = y + v * back
+  __device__ __forceinline__ void store(const mlxr_lora_item& it, int64_t row, int n, bool vec, const f32x4_t* v, float back) {
+    if (vec && n + 16 <= it.N) {
+      u32x4_t* o = (u32x4_t*)((uint8_t*)it.out_dev + (row + n) * (YT == DT_F32 ? 4 : 2));
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < W; ++c) {
+        if constexpr (YT == DT_F32) {
+          o[c] = __builtin_bit_cast(u32x4_t, __builtin_bit_cast(f32x4_t, w[c]) + v[c] * back);
+        } else {
+          constexpr bool F = YT == DT_F16;
+          u32x4_t p;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + 4 * c + i < it.N)
-        store_scalar(it.out_dev, YT, row + n + 4 * c + i, load_scalar(it.y_dev, YT, row + n + 4 * c + i) + v[c][i] * back);
-}
+          for (int e = 0; e < 4; ++e)
+            p[e] = pack2<F>(unpack<F>(w[c][e], 0) + v[2 * c + (e >> 1)][2 * (e & 1)] * back,
+                            unpack<F>(w[c][e], 1) + v[2 * c + (e >> 1)][2 * (e & 1) + 1] * back);
+          o[c] = p;
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + 4 * c + i < it.N)
+          store_scalar(it.out_dev, YT, row + n + 4 * c + i, load_scalar(it.y_dev, YT, row + n + 4 * c + i) + v[c][i] * back);
+  }
+};
 
 // One tile and `columns` columns of an item, in steps of 64 for each wavefront.  Row 4 g + i of the c-th
 // product of a step is column 16 g + 4 c + i, so a lane ends with 16 neighbouring columns of its token.  h enters
@@ -253,12 +284,31 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
   const int begin = blockIdx.x * a.columns;
   if (begin >= it.N) return;
   int adapter = 0;
-  const int count = tile_tokens<INLINE>(a, blockIdx.y, &adapter, token);
+  const int count = tile_tokens<INLINE, kWaves>(a, blockIdx.y, &adapter, token);
   if (count == 0) return;
   const bool none = adapter == a.adapters;
   if (none && it.out_dev == it.y_dev) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int rank = none ? 0 : rank_of(a, adapter);
+  // operands of B for 64 columns, on their way while h is summed up or the columns before are computed; RT 1
+  // multiplies the high and the low parts in one step, ranks 8 (g & 1) ..
+  const uint16_t* B = (const uint16_t*)it.b_dev + (int64_t)(none ? 0 : adapter) * it.N * a.rank;
+  const int end = min(begin + a.columns, it.N);
+  int n0 = begin + wave * 64;
+  u32x4_t next[KT][4];
+  auto load_b = [&](int n0) {
+#pragma unroll
+    for (int k = 0; k < KT; ++k)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int n = n0 + 16 * (col >> 2) + 4 * c + (col & 3), at = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g, left = rank - at;
+        next[k][c] = n < it.N && left > 0 ? *(const u32x4_t*)(B + (int64_t)n * a.rank + at) : u32x4_t{0, 0, 0, 0};
+        if (left < 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) next[k][c][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
+      }
+  };
+  load_b(n0);
   if (!none) {
     const float scale = a.scales ? a.scales[adapter] : 1.f;
     // 8 ranks of a token for each thread, a token's threads side by side
@@ -307,65 +357,65 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
     __syncthreads();
   }
   const bool vec = (it.N * (it.y_dtype == DT_F32 ? 4 : 2)) % 16 == 0 && (((uintptr_t)it.y_dev | (uintptr_t)it.out_dev) & 15) == 0;
-  const uint16_t* B = (const uint16_t*)it.b_dev + (int64_t)(none ? 0 : adapter) * it.N * a.rank;
-  const int end = min(begin + a.columns, it.N);
-  for (int n0 = begin + wave * 64; n0 < end; n0 += kWaves * 64) {
-    // operands of B: RT 1 multiplies the high and the low parts in one step, ranks 8 (g & 1) ..
-    u32x4_t bf[KT][4];
+  auto columns = [&](auto yt) {
+    constexpr int YT = decltype(yt)::value;
+    for (; n0 < end; n0 += kWaves * 64) {
+      u32x4_t bf[KT][4];
 #pragma unroll
-    for (int k = 0; k < KT; ++k)
+      for (int k = 0; k < KT; ++k)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int n = n0 + 16 * (col >> 2) + 4 * c + (col & 3), at = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g, left = rank - at;
-        bf[k][c] = n < it.N && left > 0 ? *(const u32x4_t*)(B + (int64_t)n * a.rank + at) : u32x4_t{0, 0, 0, 0};
-        if (left < 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) bf[k][c][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
-      }
+        for (int c = 0; c < 4; ++c) bf[k][c] = next[k][c];
+      Cols<YT> y;
+      const int n = n0 + 16 * g;
+      auto row_of = [&](int s) { return (int64_t)token[16 * s + col] * it.N; };
+      if (col < count) y.load(it, row_of(0), n, vec);
+      if (n0 + kWaves * 64 < end) load_b(n0 + kWaves * 64);
 #pragma unroll 1
-    for (int s = 0; s < SUB; ++s) {
-      if (16 * s >= count) break;
-      f32x4_t acc[4] = {};
-      if (!none) {
-        const uint16_t* h = hs + (16 * s + col) * ROW;
+      for (int s = 0; s < SUB; ++s) {
+        if (16 * s >= count) break;
+        Cols<YT> y_next;
+        if (SUB > 1 && 16 * (s + 1) + col < count) y_next.load(it, row_of(s + 1), n, vec);
+        f32x4_t acc[4] = {};
+        if (!none) {
+          const uint16_t* h = hs + (16 * s + col) * ROW;
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-          if constexpr (RT == 1) {
-            const u32x4_t f = *(const u32x4_t*)(h + 8 * g);
+          for (int k = 0; k < KT; ++k) {
+            if constexpr (RT == 1) {
+              const u32x4_t f = *(const u32x4_t*)(h + 8 * g);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) acc[c] = mfma16<F16>(bf[k][c], f, acc[c]);
-          } else {
-            const u32x4_t hi = *(const u32x4_t*)(h + 32 * k + 8 * g), lo = *(const u32x4_t*)(h + R + 32 * k + 8 * g);
+              for (int c = 0; c < 4; ++c) acc[c] = mfma16<F16>(bf[k][c], f, acc[c]);
+            } else {
+              const u32x4_t hi = *(const u32x4_t*)(h + 32 * k + 8 * g), lo = *(const u32x4_t*)(h + R + 32 * k + 8 * g);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              acc[c] = mfma16<F16>(bf[k][c], lo, acc[c]);
-              acc[c] = mfma16<F16>(bf[k][c], hi, acc[c]);
+              for (int c = 0; c < 4; ++c) {
+                acc[c] = mfma16<F16>(bf[k][c], lo, acc[c]);
+                acc[c] = mfma16<F16>(bf[k][c], hi, acc[c]);
+              }
             }
           }
         }
-      }
-      if (16 * s + col < count) {
-        const int64_t row = (int64_t)token[16 * s + col] * it.N;
-        const float f = F16 && !none ? back[16 * s + col] : 1.f;
-        if (it.y_dtype == DT_BF16) add_row<DT_BF16>(it, row, n0 + 16 * g, acc, f, vec);
-        else if (it.y_dtype == DT_F16) add_row<DT_F16>(it, row, n0 + 16 * g, acc, f, vec);
-        else add_row<DT_F32>(it, row, n0 + 16 * g, acc, f, vec);
+        if (16 * s + col < count) y.store(it, row_of(s), n, vec, acc, F16 && !none ? back[16 * s + col] : 1.f);
+        if constexpr (SUB > 1) y = y_next;
       }
     }
-  }
+  };
+  if (it.y_dtype == DT_BF16) columns(std::integral_constant<int, DT_BF16>());
+  else if (it.y_dtype == DT_F16) columns(std::integral_constant<int, DT_F16>());
+  else columns(std::integral_constant<int, DT_F32>());
 }
 
 struct Layout {
-  int tiles, splits, chunk;  // most tiles a call may have; splits of K
+  int tiles, live, splits, chunk;  // workgroups for tiles, tiles as far as known; splits of K
   size_t order, counts, tile, h, bytes;
 };
 Layout layout_of(int count, int tokens, int K, int adapters, int rank) {
   Layout l;
-  const int items = count < kItems ? count : kItems, tm = 16 * sub_of(rank_groups_of(rank));
+  const int items = count < kItems ? count : kItems, tm = tokens <= kInline ? 16 : 16 * sub_of(rank_groups_of(rank));
   const int buckets = tokens < adapters + 1 ? tokens : adapters + 1;
-  l.tiles = tokens <= kInline ? tokens : (tokens / tm + buckets < tokens ? tokens / tm + buckets : tokens);
+  l.tiles = tokens <= kInline ? tokens : std::min(tokens, tokens / tm + buckets);
   // enough workgroups for the device; a wavefront takes two steps of K or more
-  const long want = 512 / ((long)l.tiles * items) + 1;
+  l.live = std::min(tokens, tokens / tm + buckets);
+  const long want = 512 / ((long)l.live * items) + 1;
   const int most = std::min(kMaxSplits, (K + 511) / 512);
   int splits = (int)(want < most ? want : most);
   l.chunk = ((K + splits - 1) / splits + 63) / 64 * 64;
@@ -383,7 +433,7 @@ template <bool F16, int RT, int SUB, bool INLINE>
 void launch(const LoraArgs& a, int tiles, hipStream_t s) {
   int wide = 0;
   for (int i = 0; i < a.count; ++i) wide = wide > a.item[i].N ? wide : a.item[i].N;
-  shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles, a.splits, a.count), kThreads, 0, s>>>(a);
+  shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles, a.splits, a.count), SUB == 1 ? kShrinkWide : kThreads, 0, s>>>(a);
   expand_kernel<F16, RT, SUB, INLINE><<<dim3((wide + a.columns - 1) / a.columns, tiles, a.count), kThreads, 0, s>>>(a);
 }
 template <bool F16, int RT>
@@ -454,7 +504,12 @@ extern "C" int mlxr_lora_apply(int count, const mlxr_lora_item* items, int token
   a.order = (int32_t*)(ws + l.order), a.counts = (int32_t*)(ws + l.counts), a.tiles = (Tile*)(ws + l.tile);
   a.h = (float*)(ws + l.h);
   a.tokens = tokens, a.K = K, a.adapters = adapters, a.rank = rank, a.splits = l.splits, a.chunk = l.chunk;
-  a.columns = 64 * kWaves;
+  // columns of a workgroup of expand: several steps where that leaves enough workgroups, so that what a
+  // workgroup does first (its tile, h) is paid less often
+  long wide = 0;
+  for (int i = 0; i < count; ++i) wide += items[i].N;
+  const long steps = (wide / count + 255) / 256 * std::min(count, kItems) * l.live / kExpandGroups;
+  a.columns = 64 * kWaves * (int)std::max(1L, std::min(16L, steps));
   for (int i = 0; i < count; i += kItems) {
     a.count = count - i < kItems ? count - i : kItems;
     for (int j = 0; j < a.count; ++j) a.item[j] = items[i + j];

@@ -5,9 +5,10 @@ input (include/mlxr_lora.h): ``out[t] = y[t] + scale * (x[t] A^T) B^T`` with the
 adapter ``ids[t]``.  ``LoraBank`` keeps a projection's adapters in the layout that it takes.
 """
 import ctypes
+import struct
 
-from . import qgemm
-from .paged import _code, _empty, _i32, _on
+from . import paged, qgemm
+from .paged import _code, _i32, _on, _stream
 from .qgemm import QGemmError
 
 MAX_ADAPTERS, MAX_RANK = 4096, 128
@@ -19,6 +20,8 @@ class Item(ctypes.Structure):
     _fields_ = [("a_dev", _P), ("b_dev", _P), ("y_dev", _P), ("out_dev", _P), ("N", _I), ("y_dtype", _I)]
 
 
+_pack_item = struct.Struct("@4P2i").pack  # the same as bytes
+
 _SIGS = {
     "mlxr_lora_workspace_size": (_I, [_I] * 5 + [ctypes.POINTER(ctypes.c_size_t)]),
     "mlxr_lora_apply": (_I, [_I, _P] + [_I] * 4 + [_P, _I, ctypes.c_int64, _P, _P, _P, _P, ctypes.c_size_t, _P]),
@@ -29,7 +32,7 @@ _bound = None
 def _lib():
     global _bound
     if _bound is None:
-        l = qgemm.lib()
+        l = paged._lib()
         for name, (res, args) in _SIGS.items():
             f = getattr(l, name)
             f.restype, f.argtypes = res, args
@@ -44,56 +47,54 @@ def lora_apply(x, ids, a, b, y, scales=None, ranks=None, outs=None, stream=None)
     a[i] [adapters, rank, K] and b[i] [adapters, N_i, rank] have x's dtype (float16 / bfloat16), one
     rank (a multiple of 8, up to 128) for all; ``ranks`` [adapters] (int32) says how much of it each
     adapter uses.  ``scales`` [adapters] float32.  outs[i] may be y[i].  Returns the outputs."""
-    torch = qgemm._torch()
-    d = x.device
-    n = len(a)
-    if x.dim() != 2 or d.type != "cuda":
+    lib, d, n, torch = _lib(), x.device, len(a), paged._torch
+    if x.dim() != 2 or not x.is_cuda:
         raise QGemmError(-3, "Input shape must be [tokens, K] on a GPU")
     tokens, K = x.shape
     if len(b) != n or len(y) != n or (outs is not None and len(outs) != n):
         raise QGemmError(-1, "one A, one B, one y (and one output) per projection")
-    _i32(ids, "ids", d)
+    pi = _i32(ids, "ids", d)
     if ids.shape[0] != tokens:
         raise QGemmError(-3, "ids must be [tokens]")
     if n == 0:
         return []
-    adapters, rank = a[0].shape[0], a[0].shape[1]
-    if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (adapters,) or
-                               not scales.is_contiguous() or scales.device != d):
-        raise QGemmError(-1, f"scales must be a contiguous float32 [{adapters}] tensor on {d}")
-    if ranks is not None and _i32(ranks, "ranks", d).shape[0] != adapters:
+    if a[0].dim() != 3:
+        raise QGemmError(-3, "a[0] must be [adapters, rank, K]")
+    adapters, rank, _ = shape = a[0].shape
+    ps = paged._per_head(scales, adapters, "scales", d) if scales is not None else None
+    pr = _i32(ranks, "ranks", d) if ranks is not None else None
+    if ranks is not None and ranks.shape[0] != adapters:
         raise QGemmError(-3, f"ranks must be [{adapters}]")
-    dt = _code(x.dtype, "x")
-    ptr, ctx = _on(stream, d)
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < 0 or x.data_ptr() % 16:
-        if ctx is None:
-            x = x.clone(memory_format=torch.contiguous_format)
-        else:
-            with ctx:
-                x = x.clone(memory_format=torch.contiguous_format)
+    xt = x.dtype
+    dt = _code(paged._x_codes, xt, "x")
+    xs = x.stride()
+    if xs[1] != 1 or xs[0] % 8 or xs[0] < 0 or x.data_ptr() % 16:
+        x = _on(stream, x.clone, memory_format=torch.contiguous_format)
+        xs = x.stride()
+        if xs[0] % 8:
+            raise QGemmError(-3, "lora: K must be a multiple of 8")
     if outs is None:
-        outs = [_empty(ctx, t.shape, t.dtype, d) for t in y]
-    items = (Item * n)()
-    for i, (A, B, t, o) in enumerate(zip(a, b, y, outs)):
-        if A.dim() != 3 or tuple(A.shape) != (adapters, rank, K):
+        outs = [_on(stream, torch.empty_like, t, memory_format=torch.contiguous_format) for t in y]
+    items = b""
+    for i in range(n):
+        A, B, t, o = a[i], b[i], y[i], outs[i]
+        if A.shape != shape or shape[2] != K:
             raise QGemmError(-3, f"a[{i}] must be [{adapters}, {rank}, {K}]")
-        if B.dim() != 3 or B.shape[0] != adapters or B.shape[2] != rank:
+        N = B.shape[1] if B.dim() == 3 else 0
+        if B.shape != (adapters, N, rank):
             raise QGemmError(-3, f"b[{i}] must be [{adapters}, N, {rank}]")
-        if A.dtype != x.dtype or B.dtype != x.dtype or A.device != d or B.device != d or \
-                not A.is_contiguous() or not B.is_contiguous():
+        if A.dtype != xt or B.dtype != xt or A.device != d or B.device != d or not A.is_contiguous() or not B.is_contiguous():
             raise QGemmError(-1, f"a[{i}] and b[{i}] must be contiguous, of x's dtype and device")
-        N = B.shape[1]
-        if tuple(t.shape) != (tokens, N) or o.shape != t.shape or t.dtype != o.dtype or t.device != d or o.device != d or \
+        if t.shape != (tokens, N) or o.shape != t.shape or t.dtype != o.dtype or t.device != d or o.device != d or \
                 not t.is_contiguous() or not o.is_contiguous():
             raise QGemmError(-1, f"y[{i}] and its output must be contiguous [{tokens}, {N}] tensors of one dtype on {d}")
-        items[i] = Item(A.data_ptr(), B.data_ptr(), t.data_ptr(), o.data_ptr(), N, _code(t.dtype, f"y[{i}]"))
-    lib = _lib()
+        items += _pack_item(A.data_ptr(), B.data_ptr(), t.data_ptr(), o.data_ptr(), N, _code(paged._x_codes, t.dtype, "y"))
     nb = ctypes.c_size_t()
     qgemm._check(lib.mlxr_lora_workspace_size(n, tokens, K, adapters, rank, ctypes.byref(nb)))
-    ws = _empty(ctx, nb.value, torch.uint8, d)
-    qgemm._check(lib.mlxr_lora_apply(n, items, tokens, K, adapters, rank, x.data_ptr(), dt, x.stride(0), ids.data_ptr(),
-                                     scales.data_ptr() if scales is not None else None,
-                                     ranks.data_ptr() if ranks is not None else None, ws.data_ptr(), nb.value, ptr))
+    nb = nb.value
+    ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=d)
+    qgemm._check(lib.mlxr_lora_apply(n, items, tokens, K, adapters, rank, x.data_ptr(), dt, xs[0], pi, ps, pr, ws.data_ptr(), nb,
+                                     _stream(stream, d.index)))
     return outs
 
 

@@ -14,9 +14,10 @@ dimension is contiguous (a ``[pages, page_size, heads, dim]`` tensor is passed a
 """
 import collections
 import ctypes
+import struct
 
 from . import qgemm
-from .qgemm import QGemmError
+from .qgemm import BF16, F16, F32, QGemmError
 
 E4M3 = 3
 MAX_ROWS = 4096
@@ -31,6 +32,9 @@ class Cache(ctypes.Structure):
                 ("dtype", _I), ("num_pages", _I), ("page_size", _I), ("kv_heads", _I), ("head_dim", _I)]
 
 
+# the same structure as bytes, which a call takes for its address: a third of the time of a Structure
+_pack_cache = struct.Struct("@4P6q5i4x").pack
+
 _SIGS = {
     "mlxr_page_resize": (_I, [_I] * 3 + [_P, _I64, _I] + [_P] * 9 + [_I, _P, _P]),
     "mlxr_paged_append": (_I, [_P, _I, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _P]),
@@ -40,84 +44,80 @@ _SIGS = {
 }
 
 _bound = None
+_torch = None
+_x_codes, _cache_codes = {}, {}
 
 
 def _lib():
-    global _bound
+    """The library with this module's entries declared."""
+    global _bound, _torch
     if _bound is None:
         l = qgemm.lib()
         for name, (res, args) in _SIGS.items():
             f = getattr(l, name)
             f.restype, f.argtypes = res, args
+        import torch
+        _torch = torch
+        _x_codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _cache_codes.update({torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3})
         _bound = l
     return _bound
 
 
-_codes = {}
-
-
-def _code(dtype, what, cache=False):
-    if not _codes:
-        torch = qgemm._torch()
-        _codes.update({torch.float32: qgemm.F32, torch.float16: qgemm.F16, torch.bfloat16: qgemm.BF16,
-                       torch.float8_e4m3fn: E4M3})
-    c = _codes.get(dtype)
-    if c is None or (c == qgemm.F32 if cache else c == E4M3):
+def _code(codes, dtype, what):
+    c = codes.get(dtype)
+    if c is None:
         raise QGemmError(-1, f"{what} has an unsupported dtype {dtype}")
     return c
 
 
-def _on(stream, device):
-    """The torch stream a call runs on, its handle, and the context that makes new tensors belong to it."""
-    torch = qgemm._torch()
+def _stream(stream, index):
+    """Handle of the torch stream a call runs on: the given one, or the device's current one."""
+    return _torch._C._cuda_getCurrentRawStream(index) if stream is None else stream.cuda_stream
+
+
+def _on(stream, make, *args, **kw):
+    """A tensor that belongs to the call's stream."""
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream, None
-    return stream.cuda_stream, torch.cuda.stream(stream)
-
-
-def _empty(ctx, shape, dtype, device):
-    torch = qgemm._torch()
-    if ctx is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with ctx:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return make(*args, **kw)
+    with _torch.cuda.stream(stream):
+        return make(*args, **kw)
 
 
 def _i32(t, what, device, dims=1):
-    torch = qgemm._torch()
-    if t.dtype != torch.int32 or t.dim() != dims or t.device != device or (t.shape[-1] > 1 and t.stride(-1) != 1):
+    if t.dtype != _torch.int32 or t.dim() != dims or t.device != device or (t.stride()[-1] != 1 and t.shape[-1] > 1):
         raise QGemmError(-1, f"{what} must be a{' contiguous' if dims == 1 else ''} {dims}-dimensional int32 tensor on {device}")
-    return t
+    return t.data_ptr()
 
 
-def _scale(t, heads, what, device):
-    if t is None:
-        return None
-    if t.dtype != qgemm._torch().float32 or tuple(t.shape) != (heads,) or not t.is_contiguous() or t.device != device:
+def _per_head(t, heads, what, device):
+    if t.dtype != _torch.float32 or t.shape != (heads,) or not t.is_contiguous() or t.device != device:
         raise QGemmError(-1, f"{what} must be a contiguous float32 [{heads}] tensor on {device}")
     return t.data_ptr()
 
 
 def _cache(k, v, k_scale, v_scale):
-    if k.dim() != 4 or v.shape != k.shape:
+    """mlxr_paged_cache of two stores, its dtype code and the stores' shape."""
+    shape, ks, vs, d = k.shape, k.stride(), v.stride(), k.device
+    if len(shape) != 4 or v.shape != shape:
         raise QGemmError(-3, "key and value stores must be [num_pages, kv_heads, page_size, head_dim] of one shape")
-    if v.dtype != k.dtype or v.device != k.device or k.device.type != "cuda":
+    if v.dtype != k.dtype or v.device != d or not k.is_cuda:
         raise QGemmError(-1, "key and value stores must have one dtype and be on one GPU")
-    pages, heads, page, dim = k.shape
-    ks, vs = k.stride(), v.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise QGemmError(-3, "the last dimension of a store must be contiguous")
-    d = k.device
-    return Cache(k.data_ptr(), v.data_ptr(), _scale(k_scale, heads, "k_scale", d), _scale(v_scale, heads, "v_scale", d),
-                 ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], _code(k.dtype, "the cache", True), pages, page, heads, dim)
+    pages, heads, page, dim = shape
+    code = _code(_cache_codes, k.dtype, "the cache")
+    return _pack_cache(k.data_ptr(), v.data_ptr(), _per_head(k_scale, heads, "k_scale", d) if k_scale is not None else 0,
+                       _per_head(v_scale, heads, "v_scale", d) if v_scale is not None else 0, ks[0], ks[1], ks[2], vs[0], vs[1],
+                       vs[2], code, pages, page, heads, dim), code, shape
 
 
-def _rows16(t):
+def _rows16(t, stream):
     """t [n, heads, dim] with rows that start at multiples of 16 bytes: t itself, or a copy."""
-    s, unit = t.stride(), 16 // t.element_size()
-    if s[2] == 1 and s[0] % unit == 0 and s[1] % unit == 0 and s[0] >= 0 and t.data_ptr() % 16 == 0:
+    s, size = t.stride(), t.element_size()
+    if s[2] == 1 and s[0] * size % 16 == 0 and s[1] * size % 16 == 0 and s[0] >= 0 and t.data_ptr() % 16 == 0:
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    return _on(stream, t.clone, memory_format=_torch.contiguous_format)
 
 
 Resized = collections.namedtuple("Resized", "lens free_count starts slots positions refused")
@@ -131,54 +131,57 @@ def page_resize(table, lens, want, free, free_count, page_size, tokens, stream=N
     ``free`` [num_pages] is the pool's stack of free pages, its first ``free_count`` [1] entries; both
     it and the table are changed in place.  ``tokens``: places for the new tokens' slots.  All
     tensors int32.  Returns ``Resized``; nothing is copied to the host."""
-    torch = qgemm._torch()
-    d = table.device
-    _i32(table, "table", d, 2)
-    for t, what in ((lens, "lens"), (want, "want"), (free, "free"), (free_count, "free_count")):
-        _i32(t, what, d)
+    lib, d = _lib(), table.device
+    pt, pl, pw = _i32(table, "table", d, 2), _i32(lens, "lens", d), _i32(want, "want", d)
+    pf, pc = _i32(free, "free", d), _i32(free_count, "free_count", d)
     rows, width = table.shape
-    if d.type != "cuda" or lens.shape[0] != rows or want.shape[0] != rows or free_count.shape[0] != 1:
+    if not table.is_cuda or lens.shape != (rows,) or want.shape != (rows,) or free_count.shape != (1,):
         raise QGemmError(-3, "page_resize: lens and want must be [rows], free_count [1], on the table's GPU")
     if tokens < 0:
         raise QGemmError(-1, "page_resize: tokens must not be negative")
-    ptr, ctx = _on(stream, d)
-    # one allocation, each part at a multiple of 16 bytes
-    parts = [rows, 1, rows + 1, tokens, tokens, 1]
-    at = [0]
-    for n in parts:
-        at.append(at[-1] + (n + 3) // 4 * 4)
-    buf = _empty(ctx, at[-1], torch.int32, d)
-    base = buf.data_ptr()
-    p = [base + 4 * x for x in at]
-    qgemm._check(_lib().mlxr_page_resize(rows, int(page_size), free.shape[0], table.data_ptr(), table.stride(0), width,
-                                              lens.data_ptr(), want.data_ptr(), free.data_ptr(), free_count.data_ptr(),
-                                              p[0], p[1], p[2], p[3], p[4], tokens, p[5], ptr))
-    return Resized(*[buf[x:x + n] for x, n in zip(at, parts)])
+    buf = _on(stream, _torch.empty, 2 * (rows + tokens) + 3, dtype=_torch.int32, device=d)
+    p0 = buf.data_ptr()
+    p1 = p0 + 4 * rows
+    p2 = p1 + 4
+    p3 = p2 + 4 * (rows + 1)
+    p4 = p3 + 4 * tokens
+    qgemm._check(lib.mlxr_page_resize(rows, page_size, free.shape[0], pt, table.stride()[0], width, pl, pw, pf, pc, p0, p1, p2,
+                                      p3, p4, tokens, p4 + 4 * tokens, _stream(stream, d.index)))
+    return Resized._make(buf.split((rows, 1, rows + 1, tokens, tokens, 1)))
 
 
 def paged_append(k, v, k_store, v_store, slots, k_scale=None, v_scale=None, stream=None):
     """Writes keys and values [tokens, kv_heads, head_dim] into the slots [tokens] (int32; tokens whose
     slot is -1 are left out) of the stores, divided by their head's scale (mlxr_paged_append)."""
-    c = _cache(k_store, v_store, k_scale, v_scale)
-    d = k_store.device
-    if k.dim() != 3 or k.shape[1] != c.kv_heads or k.shape[2] != c.head_dim or v.shape != k.shape:
+    lib = _lib()
+    c, _, (_, heads, _, dim) = _cache(k_store, v_store, k_scale, v_scale)
+    d, shape = k_store.device, k.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape:
         raise QGemmError(-3, "keys and values must be [tokens, kv_heads, head_dim]")
     if k.device != d or v.device != d or v.dtype != k.dtype:
         raise QGemmError(-1, "keys and values must have one dtype and be on the cache's GPU")
-    _i32(slots, "slots", d)
-    n = k.shape[0]
-    if slots.shape[0] != n:
+    n, ps = shape[0], _i32(slots, "slots", d)
+    if slots.shape != (n,):
         raise QGemmError(-3, "slots must be [tokens]")
-    dt = _code(k.dtype, "keys")
-    ptr, ctx = _on(stream, d)
-    if ctx is None:
-        k, v = _rows16(k), _rows16(v)
-    else:
-        with ctx:
-            k, v = _rows16(k), _rows16(v)
+    dt = _code(_x_codes, k.dtype, "keys")
+    k, v = _rows16(k, stream), _rows16(v, stream)
     ks, vs = k.stride(), v.stride()
-    qgemm._check(_lib().mlxr_paged_append(ctypes.byref(c), n, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt,
-                                               slots.data_ptr(), ptr))
+    qgemm._check(lib.mlxr_paged_append(c, n, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, ps,
+                                       _stream(stream, d.index)))
+
+
+_ws_bytes = {}
+
+
+def _attention_workspace(lib, c, device, rows, heads, kv_heads, dim):
+    """Workspace bytes of a call; they depend on the device and the heads alone."""
+    key = (device, heads, kv_heads, dim)
+    got = _ws_bytes.get(key)
+    if got is None:
+        n = ctypes.c_size_t()
+        qgemm._check(lib.mlxr_paged_attention_workspace_size(c, rows, heads, ctypes.byref(n)))
+        got = _ws_bytes[key] = n.value
+    return got
 
 
 def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_scale=None, v_scale=None, out=None,
@@ -188,40 +191,32 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
     names their pages.  ``scale`` defaults to head_dim ** -0.5; ``window`` keeps the last tokens only
     (0: all).  Rows of length 0 give zeros.  Returns out [rows, heads, head_dim] (q's dtype or
     ``out_dtype``), with ``return_lse`` also the log of the softmax's sum, float32 [rows, heads]."""
-    torch = qgemm._torch()
-    c = _cache(k_store, v_store, k_scale, v_scale)
-    d = k_store.device
-    if q.dim() != 3 or q.shape[2] != c.head_dim:
+    lib = _lib()
+    c, _, (_, kv_heads, _, dim) = _cache(k_store, v_store, k_scale, v_scale)
+    d, shape = k_store.device, q.shape
+    if len(shape) != 3 or shape[2] != dim:
         raise QGemmError(-3, "queries must be [rows, heads, head_dim]")
     if q.device != d:
         raise QGemmError(-1, "queries must be on the cache's GPU")
-    rows, heads, dim = q.shape
-    _i32(table, "table", d, 2)
-    _i32(lens, "lens", d)
+    rows, heads, _ = shape
+    pt, pl = _i32(table, "table", d, 2), _i32(lens, "lens", d)
+    width = table.shape[1]
     if table.shape[0] != rows or lens.shape[0] != rows:
         raise QGemmError(-3, "table and lens must have one row per query")
-    dt = _code(q.dtype, "queries")
-    ptr, ctx = _on(stream, d)
+    dt = _code(_x_codes, q.dtype, "queries")
     if out is None:
-        out = _empty(ctx, (rows, heads, dim), out_dtype or q.dtype, d)
-    elif tuple(out.shape) != (rows, heads, dim) or not out.is_contiguous() or out.device != d:
+        out = _on(stream, _torch.empty, shape, dtype=out_dtype or q.dtype, device=d)
+    elif out.shape != shape or not out.is_contiguous() or out.device != d:
         raise QGemmError(-1, f"out must be a contiguous [{rows}, {heads}, {dim}] tensor on {d}")
-    odt = _code(out.dtype, "out")
-    if ctx is None:
-        q = _rows16(q)
-    else:
-        with ctx:
-            q = _rows16(q)
-    lse = _empty(ctx, (rows, heads), torch.float32, d) if return_lse else None
-    lib, cp = _lib(), ctypes.byref(c)
-    n = ctypes.c_size_t()
-    qgemm._check(lib.mlxr_paged_attention_workspace_size(cp, rows, heads, ctypes.byref(n)))
-    ws = _empty(ctx, n.value, torch.uint8, d)
+    odt = _code(_x_codes, out.dtype, "out")
+    q = _rows16(q, stream)
+    lse = _on(stream, _torch.empty, (rows, heads), dtype=_torch.float32, device=d) if return_lse else None
+    nb = _attention_workspace(lib, c, d.index, rows, heads, kv_heads, dim)
+    ws = _on(stream, _torch.empty, nb, dtype=_torch.uint8, device=d)
     qs = q.stride()
-    qgemm._check(lib.mlxr_paged_attention(cp, rows, heads, q.data_ptr(), dt, qs[0], qs[1], table.data_ptr(), table.stride(0),
-                                          table.shape[1], lens.data_ptr(), dim ** -0.5 if scale is None else float(scale),
-                                          int(window), out.data_ptr(), odt, lse.data_ptr() if lse is not None else None,
-                                          ws.data_ptr(), n.value, ptr))
+    qgemm._check(lib.mlxr_paged_attention(c, rows, heads, q.data_ptr(), dt, qs[0], qs[1], pt, table.stride()[0], width, pl,
+                                          dim ** -0.5 if scale is None else scale, window, out.data_ptr(), odt,
+                                          lse.data_ptr() if return_lse else None, ws.data_ptr(), nb, _stream(stream, d.index)))
     return (out, lse) if return_lse else out
 
 

@@ -85,7 +85,8 @@ int mlxr_paged_append(const mlxr_paged_cache* cache, int tokens, const void* k_d
  *                  an empty row
  * Tokens of pages whose table entry lies outside the cache are left out.  What lies in the cache
  * past a row's tokens is not used, whatever its bits.  head_dim: a multiple of 8 (e4m3: 16), at
- * most 256; keys' and values' strides and addresses are multiples of 16 bytes.  Sums, maxima and
+ * most 256; keys' and values' strides and addresses are multiples of 16 bytes, the pages and tokens
+ * of a store at most 2^31 elements apart.  Sums, maxima and
  * the output before its rounding are fp32. */
 int mlxr_paged_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int heads, size_t* bytes);
 int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int heads, const void* q_dev, int q_dtype,

@@ -33,7 +33,8 @@ constexpr int kHeads = 16;    // columns of the products
 struct AttnArgs {
   const uint8_t *k, *v;  // element addresses in bytes
   const float *k_scale, *v_scale;
-  int64_t k_page, k_head, k_token, v_page, v_head, v_token;  // strides, bytes
+  int64_t k_head, v_head;  // strides, bytes
+  uint32_t k_page, k_token, v_page, v_token;
   const uint16_t* q;
   int64_t q_row, q_head;  // elements
   const int32_t* table;
@@ -44,7 +45,8 @@ struct AttnArgs {
   float* ws;        // partials
   int32_t* prefix;  // [rows + 1] tiles before each row, for the join
   int rows, heads, kv_heads, group, groups;  // groups: of 16 heads, of a kv head
-  int dim, page, page_shift, pages, width, window, out_dtype;
+  int dim, page, pages, width, window, out_dtype;
+  uint32_t page_mul, page_shift;  // n / page = (mulhi(n, page_mul) + n) >> page_shift for n < 2^31
   int part_rows, workers;
   float scale;  // times log2(e)
 };
@@ -129,76 +131,99 @@ struct Attn {
     trow = a.table + (int64_t)r * a.table_stride;
   }
 
-  // Page and place within it of position pos.
+  // Keys and values are read once: past the caches (64 rows of Llama-3-8B heads 180 -> 170 us), unless a row
+  // of a head is not whole 128-byte lines and so shares them with rows that other wavefronts read (32 heads
+  // of 80 in [token, head] order 53 -> 66 us).
+  template <class T>
+  static __device__ __forceinline__ T stream_load(const T* p) {
+    if constexpr (DIM && DT * (F8 ? 1 : 2) >= 128) return __builtin_nontemporal_load(p);
+    else return *p;
+  }
+  // Index of a position's page among its row's.
   __device__ __forceinline__ int page_of(int pos) const {
-    return a.page_shift >= 0 ? pos >> a.page_shift : (int)((unsigned)pos / (unsigned)a.page);
+    return (int)((__umulhi((uint32_t)pos, a.page_mul) + (uint32_t)pos) >> a.page_shift);
   }
-  // Page id of a position of the row, -1 past its tokens and for entries outside the cache.
-  __device__ __forceinline__ int id_of(int pos, const Span& s) const {
-    if (pos >= s.len) return -1;
-    const int id = trow[page_of(pos)];
-    return id >= 0 && id < a.pages ? id : -1;
-  }
-
-  __device__ __forceinline__ void load_k(int hh, int id, int pos) {
-    const uint8_t* p = kh + (int64_t)id * a.k_page + (int64_t)(pos - page_of(pos) * a.page) * a.k_token;
-#pragma unroll
-    for (int j = 0; j < KL; ++j) {
-      const int d = F8 ? j * 64 + g * 16 : j * 32 + g * 8;
-      kr[hh][j] = id >= 0 && (DIM || d < a.dim) ? *(const u32x4_t*)(p + d * (F8 ? 1 : 2)) : u32x4_t{0, 0, 0, 0};
-    }
-  }
-  __device__ __forceinline__ void load_v(int j, bool ok, const uint8_t* p) {
-#pragma unroll
-    for (int x = 0; x < VH; ++x) {
-      const int d = x * 128 + VE * col;
-      constexpr int W = F8 ? VE / 4 : VE / 2;
-      const uint8_t* at = p + d * (F8 ? 1 : 2);
-      const bool in = ok && (DIM || d < a.dim);
-      if constexpr (W == 4) {
-        const u32x4_t w = in ? *(const u32x4_t*)at : u32x4_t{0, 0, 0, 0};
-        vr[x][j][0] = w.x, vr[x][j][1] = w.y, vr[x][j][2] = w.z, vr[x][j][3] = w.w;
-      } else if constexpr (W == 2) {
-        const u32x2_t w = in ? *(const u32x2_t*)at : u32x2_t{0, 0};
-        vr[x][j][0] = w.x, vr[x][j][1] = w.y;
-      } else {
-        vr[x][j][0] = in ? *(const uint32_t*)at : 0u;
-      }
-    }
+  // Table entry of a position of the row (of the row's last token, past it).
+  __device__ __forceinline__ int entry_of(int pos, const Span& s) const { return trow[page_of(min(pos, s.len - 1))]; }
+  // Byte offset of a position in a store whose page is `id` (page 0 for one outside the cache: read, not used).
+  __device__ __forceinline__ uint64_t offset(int id, int pos, uint32_t page, uint32_t token) const {
+    return (uint64_t)((uint32_t)id < (uint32_t)a.pages ? id : 0) * page + (uint64_t)(uint32_t)(pos - page_of(pos) * a.page) * token;
   }
 
-  // Bits of this lane's eight tokens (t0 + 8 g + j) that count.
-  __device__ __forceinline__ uint32_t load_tile(int t0, const Span& s) {
-    uint32_t live = 0;
+  // Table entries of a tile's tokens: one for each block of eight where a block lies in one page, else one for
+  // each token of the lane's values and keys.
+  struct Ids {
+    int id[P8 ? 1 : 10];
+  };
+  __device__ __forceinline__ Ids ids_of(int t0, const Span& s) const {
+    Ids n;
     if constexpr (P8) {
-      const int pos = t0 + 8 * g, id = id_of(pos, s);
-      const int kb = col >> 2;  // block of this lane's key rows
-      const int kid = __shfl(id, kb * 16);
-      const int kpos = t0 + 8 * kb + (col & 3);
-      load_k(0, kid, kpos);
-      load_k(1, kid, kpos + 4);
-      const uint8_t* p = vh + (int64_t)id * a.v_page + (int64_t)(pos - page_of(pos) * a.page) * a.v_token;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool ok = id >= 0 && pos + j >= s.first && pos + j < s.len;
-        load_v(j, ok, p + j * a.v_token);
-        live |= (uint32_t)ok << j;
-      }
+      n.id[0] = entry_of(t0 + 8 * g, s);
     } else {
 #pragma unroll
-      for (int hh = 0; hh < 2; ++hh) {
-        const int pos = t0 + 8 * (col >> 2) + 4 * hh + (col & 3);
-        load_k(hh, id_of(pos, s), pos);
-      }
+      for (int j = 0; j < 8; ++j) n.id[j] = entry_of(t0 + 8 * g + j, s);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int pos = t0 + 8 * g + j, id = id_of(pos, s);
-        const bool ok = id >= 0 && pos >= s.first;
-        load_v(j, ok, vh + (int64_t)id * a.v_page + (int64_t)(pos - page_of(pos) * a.page) * a.v_token);
-        live |= (uint32_t)ok << j;
-      }
+      for (int hh = 0; hh < 2; ++hh) n.id[8 + hh] = entry_of(t0 + key_token(hh), s);
+    }
+    return n;
+  }
+  // Token of the tile that is row `col` of half hh of the keys.
+  __device__ __forceinline__ int key_token(int hh) const { return 8 * (col >> 2) + 4 * hh + (col & 3); }
+  // Bits of this lane's eight tokens (t0 + 8 g + j) that count.
+  __device__ __forceinline__ uint32_t live_of(const Ids& n, int t0, const Span& s) const {
+    const int pos = t0 + 8 * g, from = min(max(s.first - pos, 0), 8), to = min(max(s.len - pos, 0), 8);
+    uint32_t live = (1u << to) - (1u << from);  // from <= to: a window is no later than the row's end
+    if constexpr (P8) {
+      if ((uint32_t)n.id[0] >= (uint32_t)a.pages) live = 0;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if ((uint32_t)n.id[j] >= (uint32_t)a.pages) live &= ~(1u << j);
     }
     return live;
+  }
+
+  // The loads of a tile are unconditional, from an address within the stores for whatever does not count, so
+  // that they stay in flight over the branches: what they bring for tokens that do not count is left out later.
+  // more: false where there is no further tile; all lanes then read the first page's first rows again.
+  __device__ __forceinline__ void load_k(const Ids& n, int t0, bool more) {
+    const uint8_t* block = nullptr;
+    if constexpr (P8) block = kh + (more ? offset(__shfl(n.id[0], (col & 12) * 4), t0 + key_token(0), a.k_page, a.k_token) : 0);
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const uint8_t* p = P8 ? block + (uint64_t)a.k_token * (4 * hh)
+                            : kh + (more ? offset(n.id[P8 ? 0 : 8 + hh], t0 + key_token(hh), a.k_page, a.k_token) : 0);
+#pragma unroll
+      for (int j = 0; j < KL; ++j) {
+        int d = F8 ? j * 64 + g * 16 : j * 32 + g * 8;
+        if (!DIM && d >= a.dim) d = 0;
+        kr[hh][j] = stream_load((const u32x4_t*)(p + d * (F8 ? 1 : 2)));
+      }
+    }
+  }
+  __device__ __forceinline__ void load_v(const Ids& n, int t0, bool more) {
+    constexpr int W = F8 ? VE / 4 : VE / 2;
+    const uint8_t* block = vh + (P8 && more ? offset(n.id[0], t0 + 8 * g, a.v_page, a.v_token) : 0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* p = P8 ? block + (uint64_t)a.v_token * j
+                            : vh + (more ? offset(n.id[P8 ? 0 : j], t0 + 8 * g + j, a.v_page, a.v_token) : 0);
+#pragma unroll
+      for (int x = 0; x < VH; ++x) {
+        int d = x * 128 + VE * col;
+        if (!DIM && d >= a.dim) d = 0;  // its sums are not stored
+        const uint8_t* at = p + d * (F8 ? 1 : 2);
+        if constexpr (W == 4) {
+          const u32x4_t w = stream_load((const u32x4_t*)at);
+          vr[x][j][0] = w.x, vr[x][j][1] = w.y, vr[x][j][2] = w.z, vr[x][j][3] = w.w;
+        } else if constexpr (W == 2) {
+          const u32x2_t w = stream_load((const u32x2_t*)at);
+          vr[x][j][0] = w.x, vr[x][j][1] = w.y;
+        } else {
+          vr[x][j][0] = stream_load((const uint32_t*)at);
+        }
+      }
+    }
   }
 
   // Word w (dims 2 w, 2 w + 1 of the lane's VE) of token j, as a pair of 16-bit floats.
@@ -226,29 +251,76 @@ struct Attn {
     }
   }
 
-  __device__ __forceinline__ void tile(uint32_t live) {
-    f32x4_t s[2];
+  // Tiles first .. first + count of the row: while a tile's weights are computed its values and the next
+  // tile's keys are on their way, while its values are added up the next tile's keys and values.  Table
+  // entries are read a tile before they are needed: loads return in order, waiting for one that was
+  // asked for last would wait for all.
+  __device__ __forceinline__ void run(const Span& s, int first, int count) {
+    int t0 = s.base + first * kTile;
+    const int last = s.base + (first + count - 1) * kTile;
+    int t1 = t0 + kTile;
+    Ids ids = ids_of(t0, s), next = ids_of(t1, s);
+    load_k(ids, t0, true);
+    __builtin_amdgcn_sched_barrier(0);  // the order of the loop's loads, which its waits count
+    load_v(ids, t0, true);
+    uint32_t live = live_of(ids, t0, s);
+    while (true) {
+      const bool more = t0 != last;
+      ids = next;
+      next = ids_of(t1 + kTile, s);
+      f32x4_t x[2];
+      scores(x);
+      load_k(ids, t1, more);
+      const bool full = __ballot(live != 0xff) == 0;
+      u32x4_t hi, lo;
+      weights(x, live, full, &hi, &lo);
+      if (!full) drop(live);
+#pragma unroll
+      for (int xh = 0; xh < VH; ++xh) add_v<0>(xh, hi, lo);
+      load_v(ids, t1, more);
+      if (!more) break;
+      live = live_of(ids, t1, s);
+      t0 = t1;
+      t1 += kTile;
+    }
+  }
+
+  // Zeros for the values of tokens that do not count: their weight is 0, their bits may be NaN.
+  __device__ __forceinline__ void drop(uint32_t live) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int x = 0; x < VH; ++x)
+#pragma unroll
+        for (int w = 0; w < (F8 ? VE / 4 : VE / 2); ++w) vr[x][j][w] = live >> j & 1 ? vr[x][j][w] : 0u;
+  }
+
+  __device__ __forceinline__ void scores(f32x4_t (&s)[2]) {
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       s[hh] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
-        u32x4_t kf;
+        u32x4_t kf = kr[hh][F8 ? j >> 1 : j];
         if constexpr (F8) {
-          const uint32_t w0 = kr[hh][j >> 1][2 * (j & 1)], w1 = kr[hh][j >> 1][2 * (j & 1) + 1];
+          const uint32_t w0 = kf[2 * (j & 1)], w1 = kf[2 * (j & 1) + 1];
           kf = u32x4_t{widen<F16, false>(w0), widen<F16, true>(w0), widen<F16, false>(w1), widen<F16, true>(w1)};
-        } else {
-          kf = kr[hh][j];
         }
+        if (!DIM && dim_of(j) >= a.dim) kf = u32x4_t{0, 0, 0, 0};
         s[hh] = mfma16<F16>(kf, q[j], s[hh]);
       }
     }
+  }
+
+  __device__ __forceinline__ void weights(const f32x4_t (&s)[2], uint32_t live, bool full, u32x4_t* hi, u32x4_t* lo) {
     float x[8], top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = live >> j & 1 ? s[j >> 2][j & 3] * sc : -INFINITY;
-      top = fmaxf(top, x[j]);
-    }
+    for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * sc;
+    if (!full)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = live >> j & 1 ? x[j] : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, x[j]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     const float m_new = fmaxf(m, top);
@@ -257,19 +329,16 @@ struct Attn {
     m = m_new;
     const float off = SHIFT - ref;
     float sum = 0.f;
-    u32x4_t hi, lo;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float p0 = __builtin_amdgcn_exp2f(x[2 * k] + off), p1 = __builtin_amdgcn_exp2f(x[2 * k + 1] + off);
       sum += p0 + p1;
-      hi[k] = pack2<F16>(p0, p1);
-      lo[k] = pack2<F16>(p0 - unpack<F16>(hi[k], 0), p1 - unpack<F16>(hi[k], 1));
+      (*hi)[k] = pack2<F16>(p0, p1);
+      (*lo)[k] = pack2<F16>(p0 - unpack<F16>((*hi)[k], 0), p1 - unpack<F16>((*hi)[k], 1));
     }
     l = l * alpha + sum;
 #pragma unroll
     for (int c = 0; c < NC; ++c) o[c] *= alpha;
-#pragma unroll
-    for (int xh = 0; xh < VH; ++xh) add_v<0>(xh, hi, lo);
   }
 
   // First of the VE neighbouring dims that this lane holds of row i of the accumulators of half x.
@@ -315,7 +384,7 @@ struct Attn {
 };
 
 template <bool F16, bool F8, int DT, bool DIM, bool P8>
-__global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_kernel(AttnArgs a) {
   extern __shared__ int pre[];  // [rows + 1] tiles before each row
   __shared__ int part[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -369,10 +438,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attn_kernel(AttnArgs a) {
     const int count = (int)min((int64_t)(s.tiles - first), end - pos);
     const int kvh = hg / a.groups, grp = hg - kvh * a.groups;
     t.start(r, kvh, grp);
-    for (int i = 0; i < count; ++i) {
-      const uint32_t live = t.load_tile(s.base + (first + i) * kTile, s);
-      t.tile(live);
-    }
+    t.run(s, first, count);
     const bool whole = first == 0 && count == s.tiles;
     t.finish(r, kvh, grp, whole ? nullptr : partial(a, w, slot));
     slot = 1;

@@ -140,6 +140,9 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   const int64_t most = (int64_t)table_width * cache->page_size;
   if (most > INT32_MAX || (most / kTile + 1) * rows > INT32_MAX || (int64_t)rows * heads > INT32_MAX)
     return set_error(MLXR_E_SHAPE, "paged_attention: the table covers too many tokens");
+  for (int i = 0; i < 3; i += 2)
+    if (cache->k_stride[i] > UINT32_MAX / 2 || cache->v_stride[i] > UINT32_MAX / 2)
+      return set_error(MLXR_E_SHAPE, "paged_attention: pages and tokens must lie less than 4 GiB apart");
   if (workspace_bytes < workspace(cache, heads))
     return set_error(MLXR_E_INVALID, "paged_attention: the workspace is smaller than mlxr_paged_attention_workspace_size");
   AttnKern& k = kern(cache, q_dtype);
@@ -150,8 +153,9 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   AttnArgs a;
   a.k = (const uint8_t*)cache->k_dev, a.v = (const uint8_t*)cache->v_dev;
   a.k_scale = cache->k_scale_dev, a.v_scale = cache->v_scale_dev;
-  a.k_page = cache->k_stride[0] * es, a.k_head = cache->k_stride[1] * es, a.k_token = cache->k_stride[2] * es;
-  a.v_page = cache->v_stride[0] * es, a.v_head = cache->v_stride[1] * es, a.v_token = cache->v_stride[2] * es;
+  a.k_head = cache->k_stride[1] * es, a.v_head = cache->v_stride[1] * es;
+  a.k_page = (uint32_t)(cache->k_stride[0] * es), a.k_token = (uint32_t)(cache->k_stride[2] * es);
+  a.v_page = (uint32_t)(cache->v_stride[0] * es), a.v_token = (uint32_t)(cache->v_stride[2] * es);
   a.q = (const uint16_t*)q_dev, a.q_row = q_row_stride, a.q_head = q_head_stride;
   a.table = table_dev, a.table_stride = table_stride, a.lens = lens_dev;
   a.out = out_dev, a.lse = lse_dev;
@@ -160,7 +164,8 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   a.groups = (a.group + kHeads - 1) / kHeads;
   a.part_rows = a.group < kHeads ? a.group : kHeads;
   a.dim = cache->head_dim, a.page = cache->page_size, a.pages = cache->num_pages, a.width = table_width;
-  a.page_shift = (a.page & (a.page - 1)) == 0 ? __builtin_ctz(a.page) : -1;
+  a.page_shift = a.page > 1 ? 32 - __builtin_clz(a.page - 1) : 0;
+  a.page_mul = (uint32_t)((((1ull << a.page_shift) - a.page) << 32) / a.page + 1);
   a.window = window, a.out_dtype = out_dtype, a.workers = grid * kWaves;
   a.scale = scale * 1.44269504088896341f;
   void* args[] = {&a};

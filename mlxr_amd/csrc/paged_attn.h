@@ -43,7 +43,7 @@ struct AttnArgs {
   void* out;
   float* lse;
   float* ws;        // partials
-  int32_t* prefix;  // [rows + 1] tiles before each row, for the join
+  int32_t* prefix;  // [rows + 1] tiles before each row, then tiles of a wavefront, for the join
   int rows, heads, kv_heads, group, groups;  // groups: of 16 heads, of a kv head
   int dim, page, pages, width, window, out_dtype;
   uint32_t page_mul, page_shift;  // n / page = (mulhi(n, page_mul) + n) >> page_shift for n < 2^31
@@ -71,8 +71,9 @@ __host__ __device__ constexpr int partial_floats(int part_rows, int dim) { retur
 __device__ __forceinline__ float* partial(const AttnArgs& a, int w, int slot) {
   return a.ws + ((int64_t)w * 2 + slot) * partial_floats(a.part_rows, a.dim);
 }
-__device__ __forceinline__ int64_t tiles_per_worker(const AttnArgs& a, int64_t total) {
-  return (total + a.workers - 1) / a.workers;
+// n / d, d > 0; most calls stay within 32 bits, whose division takes a tenth of the instructions.
+__device__ __forceinline__ int quotient(int64_t n, int d) {
+  return n < (1ll << 31) ? (int)((uint32_t)n / (uint32_t)d) : (int)(n / d);
 }
 
 // Two e4m3 values (half `h` of w) as two 16-bit floats: exact in either type.
@@ -278,6 +279,7 @@ struct Attn {
 #pragma unroll
       for (int xh = 0; xh < VH; ++xh) add_v<0>(xh, hi, lo);
       load_v(ids, t1, more);
+      asm volatile("" ::: "memory");  // the loads stay here, or what waits for the keys would wait for the values too
       if (!more) break;
       live = live_of(ids, t1, s);
       t0 = t1;
@@ -408,12 +410,13 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_kernel(At
   }
   if (tid == 64 * kWaves - 1) pre[a.rows] = at;  // the last thread's sum is the total
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int r = tid; r <= a.rows; r += 64 * kWaves) a.prefix[r] = pre[r];
-
   const int per_row = a.kv_heads * a.groups;  // sequences of tiles of one row
   const int64_t total = (int64_t)pre[a.rows] * per_row;
-  const int64_t per = tiles_per_worker(a, total);
+  const int per = quotient(total + a.workers - 1, a.workers);
+  if (blockIdx.x == 0) {  // for the join
+    for (int r = tid; r <= a.rows; r += 64 * kWaves) a.prefix[r] = pre[r];
+    if (tid == 0) a.prefix[a.rows + 1] = per;
+  }
   const int w = __builtin_amdgcn_readfirstlane(wave) * (int)gridDim.x + (int)blockIdx.x;
   int64_t pos = (int64_t)w * per;
   const int64_t end = pos + per < total ? pos + per : total;
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_kernel(At
       continue;
     }
     const int64_t in_row = pos - (int64_t)pre[r] * per_row;
-    const int hg = (int)(in_row / s.tiles), first = (int)(in_row - (int64_t)hg * s.tiles);
+    const int hg = quotient(in_row, s.tiles), first = (int)(in_row - (int64_t)hg * s.tiles);
     const int count = (int)min((int64_t)(s.tiles - first), end - pos);
     const int kvh = hg / a.groups, grp = hg - kvh * a.groups;
     t.start(r, kvh, grp);

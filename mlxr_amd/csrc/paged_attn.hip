@@ -7,63 +7,75 @@ namespace paged {
 
 namespace {
 
-constexpr int kJoinThreads = 256;
+// A part of a softmax average: sum of weights relative to 2^m, and the weighted values.
+struct Part {
+  float m, l;
+  f32x4_t o;
+};
+__device__ __forceinline__ void add(Part& a, const Part& b) {
+  const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
+  const float fa = __builtin_amdgcn_exp2f(a.m - ref), fb = __builtin_amdgcn_exp2f(b.m - ref);
+  a.m = m;
+  a.l = a.l * fa + b.l * fb;
+  a.o = a.o * fa + b.o * fb;
+}
 
 // One workgroup per (row, head): o = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w over the wavefronts w
 // that had a piece of the row, M the maximum of their m.  Rows without tokens get zeros; rows that one
-// wavefront covered are done.
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(AttnArgs a) {
-  __shared__ float sh[kJoinThreads * 4];
-  __shared__ float sh_m[4], sh_l[kJoinThreads];
+// wavefront covered are done.  Threads: four dims each (LANES, a power of two that covers head_dim), several
+// pieces side by side, four of them on their way at once.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void join_kernel(AttnArgs a, int lanes) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ Part sh[WAVES][64];
   const int r = blockIdx.x / a.heads, h = blockIdx.x - r * a.heads, tid = threadIdx.x;
   const int kvh = h / a.group, hk = h - kvh * a.group, grp = hk / kHeads, row = hk - grp * kHeads;
-  const int per_row = a.kv_heads * a.groups, tiles = a.prefix[r + 1] - a.prefix[r];
+  const int per_row = a.kv_heads * a.groups, before = a.prefix[r], tiles = a.prefix[r + 1] - before, per = a.prefix[a.rows + 1];
   const int64_t head = (int64_t)r * a.heads + h;
   if (tiles == 0) {
-    for (int d = tid; d < a.dim; d += kJoinThreads) store_scalar(a.out, a.out_dtype, head * a.dim + d, 0.f);
+    for (int d = tid; d < a.dim; d += THREADS) store_scalar(a.out, a.out_dtype, head * a.dim + d, 0.f);
     if (a.lse && tid == 0) a.lse[head] = -INFINITY;
     return;
   }
-  const int64_t per = tiles_per_worker(a, (int64_t)a.prefix[a.rows] * per_row);
-  const int64_t s = (int64_t)a.prefix[r] * per_row + (int64_t)(kvh * a.groups + grp) * tiles;
-  const int w0 = (int)(s / per), w1 = (int)((s + tiles - 1) / per);
+  const int64_t s = (int64_t)before * per_row + (int64_t)(kvh * a.groups + grp) * tiles;
+  const int w0 = quotient(s, per), w1 = quotient(s + tiles - 1, per);
   if (w0 == w1) return;
   const int count = w1 - w0 + 1;
-  // the first of them may have had another row before this one
-  auto part = [&](int i) { return partial(a, w0 + i, i == 0 && (int64_t)w0 * per < s ? 1 : 0); };
-  const int64_t st = (int64_t)a.part_rows * a.dim + 2 * row;
-  float m = -INFINITY;
-  for (int i = tid; i < count; i += kJoinThreads) m = fmaxf(m, part(i)[st]);
+  const bool late = (int64_t)w0 * per < s;  // the first of them had another row before this one
+  const int x = tid & (lanes - 1), y = tid / lanes, across = THREADS / lanes;
+  const bool in = 4 * x < a.dim;
+  Part sum = {-INFINITY, 0.f, {0, 0, 0, 0}};
+  for (int i = y; i < count; i += 4 * across) {
+    Part p[4];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  if ((tid & 63) == 0) sh_m[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3]));
-  const float ref = m == -INFINITY ? 0.f : m;
-  // threads: `lanes` of a piece's row (four dims each) by `across` pieces
-  const int lanes = a.dim / 4, across = kJoinThreads / lanes, x = tid % lanes, y = tid / lanes;
-  f32x4_t o = {0, 0, 0, 0};
-  float l = 0.f;
-  if (y < across)
-    for (int i = y; i < count; i += across) {
-      const float* p = part(i);
-      const float f = __builtin_amdgcn_exp2f(p[st] - ref);
-      const f32x4_t v = *(const f32x4_t*)(p + (int64_t)row * a.dim + 4 * x);
-      l += f * p[st + 1];
-      o += f * v;
+    for (int k = 0; k < 4; ++k) {
+      const int w = i + k * across;
+      const bool ok = w < count;
+      const float* at = partial(a, w0 + (ok ? w : 0), (ok ? w : 0) == 0 && late ? 1 : 0);
+      const float* st = at + (int64_t)a.part_rows * a.dim + 2 * row;
+      p[k].m = ok ? st[0] : -INFINITY;
+      p[k].l = ok ? st[1] : 0.f;
+      p[k].o = ok && in ? *(const f32x4_t*)(at + (int64_t)row * a.dim + 4 * x) : f32x4_t{0, 0, 0, 0};
     }
-  *(f32x4_t*)(sh + 4 * tid) = o;
-  sh_l[tid] = l;
-  __syncthreads();
-  if (y) return;
-  for (int i = 1; i < across; ++i) {
-    o += *(const f32x4_t*)(sh + 4 * (i * lanes + x));
-    l += sh_l[i * lanes + x];
-  }
-  const float f = (a.v_scale ? a.v_scale[kvh] : 1.f) / l;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) store_scalar(a.out, a.out_dtype, head * a.dim + 4 * x + c, o[c] * f);
-  if (a.lse && x == 0) a.lse[head] = (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+    for (int k = 0; k < 4; ++k) add(sum, p[k]);
+  }
+  for (int d = lanes; d < 64; d *= 2) {
+    Part q;
+    q.m = __shfl_xor(sum.m, d);
+    q.l = __shfl_xor(sum.l, d);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) q.o[c] = __shfl_xor(sum.o[c], d);
+    add(sum, q);
+  }
+  sh[tid >> 6][tid & 63] = sum;
+  __syncthreads();
+  if (y || !in) return;
+  for (int w = 1; w < WAVES; ++w) add(sum, sh[w][x]);
+  const float f = (a.v_scale ? a.v_scale[kvh] : 1.f) / sum.l;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) store_scalar(a.out, a.out_dtype, head * a.dim + 4 * x + c, sum.o[c] * f);
+  if (a.lse && x == 0) a.lse[head] = (sum.m + __builtin_amdgcn_logf(sum.l)) * 0.69314718055994531f;
 }
 
 // Workgroups of the launch: as many as the device holds at once.
@@ -89,8 +101,9 @@ AttnKern& kern(const mlxr_paged_cache* c, int q_dtype) {
   return f16 ? kern_f16(c->head_dim, p8) : kern_bf16(c->head_dim, p8);
 }
 
-constexpr size_t kPrefixBytes = (MLXR_PAGED_MAX_ROWS + 1 + 3) / 4 * 4 * sizeof(int32_t);
+constexpr size_t kPrefixBytes = (MLXR_PAGED_MAX_ROWS + 2 + 3) / 4 * 4 * sizeof(int32_t);
 constexpr int kMaxGridPerCu = 4;
+constexpr int kJoinMany = 512;
 
 size_t workspace(const mlxr_paged_cache* c, int heads) {
   const int group = heads / c->kv_heads, part_rows = group < kHeads ? group : kHeads;
@@ -171,7 +184,11 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   void* args[] = {&a};
   e = hipLaunchKernel(k.fn, dim3(grid), dim3(64 * kWaves), args, (size_t)(rows + 1) * 4, (hipStream_t)stream);
   if (e == hipSuccess) {
-    join_kernel<<<rows * heads, kJoinThreads, 0, (hipStream_t)stream>>>(a);
+    // few heads of all: long rows, in many pieces each
+    int lanes = 2;
+    while (4 * lanes < a.dim) lanes *= 2;
+    if (rows * heads >= kJoinMany) join_kernel<256><<<rows * heads, 256, 0, (hipStream_t)stream>>>(a, lanes);
+    else join_kernel<1024><<<rows * heads, 1024, 0, (hipStream_t)stream>>>(a, lanes);
     e = hipGetLastError();
   }
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_attention launch: %s", hipGetErrorString(e));

@@ -26,7 +26,7 @@ extern "C" {
  * (largest value 448). */
 enum { MLXR_E4M3 = 3 };
 
-/* Rows (requests) of one call. */
+/* Rows (requests) of one call of mlxr_page_resize. */
 enum { MLXR_PAGED_MAX_ROWS = 4096 };
 
 typedef struct mlxr_paged_cache {
@@ -88,7 +88,9 @@ int mlxr_paged_append(const mlxr_paged_cache* cache, int tokens, const void* k_d
  * most 256; keys' and values' strides and addresses are multiples of 16 bytes, the pages and tokens
  * of a store at most 2^31 elements apart.  Sums, maxima and
  * the output before its rounding are fp32. */
-int mlxr_paged_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int heads, size_t* bytes);
+/* Workspace bytes of a call (0: none is needed, workspace_dev may be NULL). */
+int mlxr_paged_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int heads, int table_width,
+                                        size_t* bytes);
 int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int heads, const void* q_dev, int q_dtype,
                          int64_t q_row_stride, int64_t q_head_stride, const int32_t* table_dev, int64_t table_stride,
                          int table_width, const int32_t* lens_dev, float scale, int window, void* out_dev, int out_dtype,

@@ -14,11 +14,12 @@
 // large as the output's own.  A second product costs matrix cycles that the kernel, bound by
 // memory, has to spare.
 //
-// The work is cut evenly: the tiles (32 tokens) of all rows and kv heads, in one sequence, are
-// dealt to the wavefronts of the launch in equal contiguous runs.  A run that covers a row's
-// whole (row, kv head) writes the output; others leave (m, sum, unnormalized o) in the workspace,
-// at most two per wavefront, for the join kernel.  Lengths are read on the device, nothing of the
-// launch depends on them.
+// Short rows: a workgroup for each (row, kv head), merged in LDS (attn_rows_kernel).  Long ones are cut
+// evenly (attn_kernel): the tiles (32 tokens) of all rows and kv heads, in one sequence, are dealt to the
+// wavefronts of a launch that fills the device, in equal contiguous runs.  A run that covers a whole (row,
+// kv head) writes the output; others leave (m, sum, unnormalized o) in the workspace, at most two for
+// a wavefront, and a second launch joins them.  Lengths are read on the device; the host chooses by the longest
+// row that the table can hold.
 #pragma once
 #include "mfma16.h"
 #include "paged_internal.h"
@@ -29,6 +30,7 @@ namespace paged {
 constexpr int kTile = 32;     // tokens
 constexpr int kWaves = 4;     // of a workgroup
 constexpr int kHeads = 16;    // columns of the products
+constexpr int kMaxCutRows = 4096;  // rows of a cut launch: their tiles are summed up in LDS
 
 struct AttnArgs {
   const uint8_t *k, *v;  // element addresses in bytes
@@ -343,6 +345,27 @@ struct Attn {
     for (int c = 0; c < NC; ++c) o[c] *= alpha;
   }
 
+  // This lane's sums to LDS, and those of another wavefront of the same row and heads added to its own.
+  static constexpr int PARK = 4 * NC + 2;  // floats of a lane
+  __device__ __forceinline__ void park(float* to) const {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[(4 * c + i) * 64 + lane] = o[c][i];
+    to[4 * NC * 64 + lane] = m;
+    to[(4 * NC + 1) * 64 + lane] = l;
+  }
+  __device__ __forceinline__ void merge(const float* from) {
+    const float m2 = from[4 * NC * 64 + lane], m_new = fmaxf(m, m2), ref = m_new == -INFINITY ? 0.f : m_new;
+    const float f = __builtin_amdgcn_exp2f(m - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
+    m = m_new;
+    l = l * f + from[(4 * NC + 1) * 64 + lane] * f2;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[c][i] = o[c][i] * f + from[(4 * c + i) * 64 + lane] * f2;
+  }
+
   // First of the VE neighbouring dims that this lane holds of row i of the accumulators of half x.
   __device__ __forceinline__ int out_dim(int x, int i) const { return x * 128 + VE * (4 * g + i); }
 
@@ -450,8 +473,49 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_kernel(At
   }
 }
 
+// One launch for short rows: a workgroup for each (row, kv head, 16 heads), its wavefronts take equal runs of
+// tiles and are merged in LDS.  Four wavefronts: of eight, half as many workgroups fit a CU (64 rows of
+// 32 kv heads, up to 1024 tokens: 101 us, four 95).
+template <bool F16, bool F8, int DT, bool DIM, bool P8>
+__global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_rows_kernel(AttnArgs a) {
+  constexpr int WAVES = kWaves;
+  using T = Attn<F16, F8, DT, DIM, P8>;
+  __shared__ float sh[WAVES / 2][T::PARK * 64];
+  // heads above 16 of a kv head: their workgroups read the same keys and values, and follow each other on one of
+  // the eight XCDs (workgroup i runs on XCD i % 8)
+  int unit = blockIdx.x, grp = 0;
+  if (a.groups > 1) {
+    const int n = 8 * a.groups, at = unit % n;
+    grp = at >> 3;
+    unit = unit / n * 8 + (at & 7);
+    if (unit >= a.rows * a.kv_heads) return;
+  }
+  const int r = unit / a.kv_heads, kvh = unit - r * a.kv_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Span s = span_of(a, r);
+  if (s.tiles == 0) {
+    const int h0 = kvh * a.group + grp * kHeads, n = min(kHeads, a.group - grp * kHeads);
+    const int64_t head = (int64_t)r * a.heads + h0;
+    for (int d = threadIdx.x; d < n * a.dim; d += 64 * WAVES) store_scalar(a.out, a.out_dtype, head * a.dim + d, 0.f);
+    if (a.lse && (int)threadIdx.x < n) a.lse[head + threadIdx.x] = -INFINITY;
+    return;
+  }
+  T t(a);
+  t.start(r, kvh, grp);
+  const int per = (s.tiles + WAVES - 1) / WAVES, first = wave * per, count = min(per, s.tiles - first);
+  if (count > 0) t.run(s, first, count);
+#pragma unroll
+  for (int half = WAVES / 2; half; half /= 2) {
+    if (wave >= half && wave < 2 * half) t.park(sh[wave - half]);
+    __syncthreads();
+    if (wave < half) t.merge(sh[wave]);
+    __syncthreads();
+  }
+  if (wave == 0) t.finish(r, kvh, grp, nullptr);
+}
+
 struct AttnKern {
-  const void* fn;
+  const void *fn, *rows_fn;
   std::atomic<int> residents[64];  // workgroups of a CU, by device; 0: not asked yet
 };
 // The kernel for head_dim at a page size; F16/F8 as above.
@@ -462,8 +526,11 @@ AttnKern& kern_f16_e4m3(int dim, bool p8);
 
 template <bool F16, bool F8>
 AttnKern& kern_of(int dim, bool p8) {
-#define MLXR_ATTN(DT, DIM, P8) \
-  { static AttnKern k{(const void*)attn_kernel<F16, F8, DT, DIM, P8>, {}}; return k; }
+#define MLXR_ATTN(DT, DIM, P8)                                                                                              \
+  {                                                                                                                        \
+    static AttnKern k{(const void*)attn_kernel<F16, F8, DT, DIM, P8>, (const void*)attn_rows_kernel<F16, F8, DT, DIM, P8>, {}}; \
+    return k;                                                                                                              \
+  }
   if (dim == 64 && p8) MLXR_ATTN(64, true, true)
   if (dim == 128 && p8) MLXR_ATTN(128, true, true)
   if (dim == 256 && p8) MLXR_ATTN(256, true, true)

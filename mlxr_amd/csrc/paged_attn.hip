@@ -1,5 +1,7 @@
 // Decode attention over a paged cache: the C entry, and the join of the pieces that the kernel
 // (paged_attn.h) leaves of rows dealt to several wavefronts.
+#include <algorithm>
+
 #include "paged_attn.h"
 
 namespace mlxr {
@@ -78,8 +80,50 @@ __global__ __launch_bounds__(THREADS) void join_kernel(AttnArgs a, int lanes) {
   if (a.lse && x == 0) a.lse[head] = (sum.m + __builtin_amdgcn_logf(sum.l)) * 0.69314718055994531f;
 }
 
-// Workgroups of the launch: as many as the device holds at once.
-int grid_of(AttnKern& k, int rows, hipError_t* e) {
+AttnKern& kern(const mlxr_paged_cache* c, int q_dtype) {
+  const bool f16 = q_dtype == MLXR_F16, p8 = c->page_size % 8 == 0;
+  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, p8) : kern_bf16_e4m3(c->head_dim, p8);
+  return f16 ? kern_f16(c->head_dim, p8) : kern_bf16(c->head_dim, p8);
+}
+
+constexpr int kGridPerCu = 4;  // most workgroups of a CU that grid_of gives
+constexpr int kJoinMany = 512;
+constexpr int kMaxHeads = 1 << 24;  // rows times heads: the launch's workgroups stay countable
+
+// How a call runs: short rows in one launch without a workspace.
+struct Plan {
+  int group, groups, part_rows;
+  bool one;
+  size_t bytes;  // of the workspace
+};
+constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 3) / 4 * 4 * sizeof(int32_t); }
+// most: tokens of the longest row that the table can hold.  A workgroup alone gets about 38 GB/s, so few rows have
+// to be cut unless they are short; many rows fill the device uncut, until the longest keeps it waiting.
+// Measured, us, uncut and cut (which also takes the host 4 us more): 8 kv heads of 128 in bf16, one row of up to
+// 512 tokens (256 KiB a head) 10 and 9.4, of 1024 15 and 10.3; 16 ragged rows of up to 1024 21 and 19.5; 64 of up
+// to 1024 37 and 45, 2048 (1 MiB) 68 and 69, 4096 130 and 97; in e4m3 with 64 heads, 64 of up to 2048 40 and 55,
+// 4096 74 and 74; 4 kv heads of 64, one row of up to 1024 10.9 and 9.3, 64 of up to 2048 21 and 29, 4096 39 and 39.
+Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int64_t most) {
+  Plan p;
+  p.group = heads / c->kv_heads;
+  p.groups = (p.group + kHeads - 1) / kHeads;
+  p.part_rows = p.group < kHeads ? p.group : kHeads;
+  const int64_t units = (int64_t)rows * c->kv_heads * p.groups;
+  const int64_t bytes = 2 * most * c->head_dim * (c->dtype == MLXR_E4M3 ? 1 : 2);
+  p.one = bytes <= 256 << 10 || (bytes <= 1 << 20 && units >= 256) || rows > kMaxCutRows ||
+          (most / kTile + 1) * rows > INT32_MAX;  // what a cut launch counts in 32 bits
+  p.bytes = p.one ? 0 : prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * kWaves * 2 *
+                                                 partial_floats(p.part_rows, c->head_dim) * sizeof(float);
+  return p;
+}
+// Tokens that a row may hold and, with a window, attend to.
+int64_t longest(const mlxr_paged_cache* c, int width, int window) {
+  const int64_t most = (int64_t)width * c->page_size;
+  return window > 0 && window < most ? window : most;
+}
+
+// Workgroups of a cut launch: as many as the device holds at once.
+int grid_of(AttnKern& k, hipError_t* e) {
   int dev = 0;
   *e = hipGetDevice(&dev);
   if (*e != hipSuccess) return 0;
@@ -88,34 +132,21 @@ int grid_of(AttnKern& k, int rows, hipError_t* e) {
   if (!occ) {
     *e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k.fn, 64 * kWaves, 0);
     if (*e != hipSuccess) return 0;
-    if (occ < 1) occ = 1;
-    if (occ > 4) occ = 4;
+    occ = std::max(1, std::min(occ, kGridPerCu));
     k.residents[d].store(occ, std::memory_order_release);
   }
   return occ * device_cu_count();
 }
 
-AttnKern& kern(const mlxr_paged_cache* c, int q_dtype) {
-  const bool f16 = q_dtype == MLXR_F16, p8 = c->page_size % 8 == 0;
-  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, p8) : kern_bf16_e4m3(c->head_dim, p8);
-  return f16 ? kern_f16(c->head_dim, p8) : kern_bf16(c->head_dim, p8);
-}
-
-constexpr size_t kPrefixBytes = (MLXR_PAGED_MAX_ROWS + 2 + 3) / 4 * 4 * sizeof(int32_t);
-constexpr int kMaxGridPerCu = 4;
-constexpr int kJoinMany = 512;
-
-size_t workspace(const mlxr_paged_cache* c, int heads) {
-  const int group = heads / c->kv_heads, part_rows = group < kHeads ? group : kHeads;
-  return kPrefixBytes + (size_t)device_cu_count() * kMaxGridPerCu * kWaves * 2 * partial_floats(part_rows, c->head_dim) * sizeof(float);
-}
-
-int check_attn(const mlxr_paged_cache* c, int rows, int heads) {
+int check_attn(const mlxr_paged_cache* c, int rows, int heads, int width) {
   if (const int rc = check_cache(c)) return rc;
-  if (rows < 0 || heads <= 0) return set_error(MLXR_E_INVALID, "paged_attention: bad sizes");
-  if (rows > MLXR_PAGED_MAX_ROWS)
-    return set_error(MLXR_E_SHAPE, "paged_attention: at most %d rows", MLXR_PAGED_MAX_ROWS);
+  if (rows < 0 || heads <= 0 || width <= 0) return set_error(MLXR_E_INVALID, "paged_attention: bad sizes");
   if (heads % c->kv_heads) return set_error(MLXR_E_SHAPE, "heads must be a multiple of kv_heads");
+  for (int i = 0; i < 3; i += 2)
+    if (c->k_stride[i] > UINT32_MAX / 2 || c->v_stride[i] > UINT32_MAX / 2)
+      return set_error(MLXR_E_SHAPE, "paged_attention: pages and tokens must lie less than 4 GiB apart");
+  if ((int64_t)width * c->page_size > INT32_MAX) return set_error(MLXR_E_SHAPE, "paged_attention: the table covers too many tokens");
+  if ((int64_t)rows * heads > kMaxHeads) return set_error(MLXR_E_SHAPE, "paged_attention: at most %d rows times heads", kMaxHeads);
   return MLXR_OK;
 }
 
@@ -126,10 +157,11 @@ int check_attn(const mlxr_paged_cache* c, int rows, int heads) {
 using namespace mlxr;
 using namespace mlxr::paged;
 
-extern "C" int mlxr_paged_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int heads, size_t* bytes) {
+extern "C" int mlxr_paged_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int heads, int table_width,
+                                                   size_t* bytes) {
   if (!bytes) return set_error(MLXR_E_INVALID, "null bytes");
-  if (const int rc = check_attn(cache, rows, heads)) return rc;
-  *bytes = workspace(cache, heads);
+  if (const int rc = check_attn(cache, rows, heads, table_width)) return rc;
+  *bytes = rows ? plan_of(cache, rows, heads, longest(cache, table_width, 0)).bytes : 0;
   return MLXR_OK;
 }
 
@@ -138,7 +170,7 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
                                     int64_t table_stride, int table_width, const int32_t* lens_dev, float scale,
                                     int window, void* out_dev, int out_dtype, float* lse_dev, void* workspace_dev,
                                     size_t workspace_bytes, void* stream) {
-  if (const int rc = check_attn(cache, rows, heads)) return rc;
+  if (const int rc = check_attn(cache, rows, heads, table_width)) return rc;
   if (q_dtype != MLXR_F16 && q_dtype != MLXR_BF16) return set_error(MLXR_E_INVALID, "invalid query dtype %d", q_dtype);
   if (cache->dtype != MLXR_E4M3 && cache->dtype != q_dtype)
     return set_error(MLXR_E_INVALID, "queries must have the cache's type");
@@ -146,22 +178,12 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
     return set_error(MLXR_E_INVALID, "invalid output dtype %d", out_dtype);
   if (window < 0) return set_error(MLXR_E_INVALID, "paged_attention: window must not be negative");
   if (rows == 0) return MLXR_OK;
-  if (!q_dev || !table_dev || !lens_dev || !out_dev || !workspace_dev) return set_error(MLXR_E_INVALID, "null buffer");
-  if (table_width <= 0) return set_error(MLXR_E_INVALID, "paged_attention: table_width must be positive");
-  if (q_row_stride % 8 || q_head_stride % 8 || ((uintptr_t)q_dev & 15) || ((uintptr_t)out_dev & 15) || ((uintptr_t)workspace_dev & 15))
-    return set_error(MLXR_E_SHAPE, "paged_attention: query rows, output and workspace must start at multiples of 16 bytes");
-  const int64_t most = (int64_t)table_width * cache->page_size;
-  if (most > INT32_MAX || (most / kTile + 1) * rows > INT32_MAX || (int64_t)rows * heads > INT32_MAX)
-    return set_error(MLXR_E_SHAPE, "paged_attention: the table covers too many tokens");
-  for (int i = 0; i < 3; i += 2)
-    if (cache->k_stride[i] > UINT32_MAX / 2 || cache->v_stride[i] > UINT32_MAX / 2)
-      return set_error(MLXR_E_SHAPE, "paged_attention: pages and tokens must lie less than 4 GiB apart");
-  if (workspace_bytes < workspace(cache, heads))
+  if (!q_dev || !table_dev || !lens_dev || !out_dev) return set_error(MLXR_E_INVALID, "null buffer");
+  if (q_row_stride % 8 || q_head_stride % 8 || ((uintptr_t)q_dev & 15) || ((uintptr_t)workspace_dev & 15))
+    return set_error(MLXR_E_SHAPE, "paged_attention: query rows and the workspace must start at multiples of 16 bytes");
+  const Plan p = plan_of(cache, rows, heads, longest(cache, table_width, window));
+  if (workspace_bytes < p.bytes || (p.bytes && !workspace_dev))
     return set_error(MLXR_E_INVALID, "paged_attention: the workspace is smaller than mlxr_paged_attention_workspace_size");
-  AttnKern& k = kern(cache, q_dtype);
-  hipError_t e = hipSuccess;
-  const int grid = grid_of(k, rows, &e);
-  if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_attention: %s", hipGetErrorString(e));
   const int es = cache->dtype == MLXR_E4M3 ? 1 : 2;
   AttnArgs a;
   a.k = (const uint8_t*)cache->k_dev, a.v = (const uint8_t*)cache->v_dev;
@@ -172,24 +194,34 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   a.q = (const uint16_t*)q_dev, a.q_row = q_row_stride, a.q_head = q_head_stride;
   a.table = table_dev, a.table_stride = table_stride, a.lens = lens_dev;
   a.out = out_dev, a.lse = lse_dev;
-  a.prefix = (int32_t*)workspace_dev, a.ws = (float*)((uint8_t*)workspace_dev + kPrefixBytes);
-  a.rows = rows, a.heads = heads, a.kv_heads = cache->kv_heads, a.group = heads / cache->kv_heads;
-  a.groups = (a.group + kHeads - 1) / kHeads;
-  a.part_rows = a.group < kHeads ? a.group : kHeads;
+  a.rows = rows, a.heads = heads, a.kv_heads = cache->kv_heads;
+  a.group = p.group, a.groups = p.groups, a.part_rows = p.part_rows;
   a.dim = cache->head_dim, a.page = cache->page_size, a.pages = cache->num_pages, a.width = table_width;
   a.page_shift = a.page > 1 ? 32 - __builtin_clz(a.page - 1) : 0;
   a.page_mul = (uint32_t)((((1ull << a.page_shift) - a.page) << 32) / a.page + 1);
-  a.window = window, a.out_dtype = out_dtype, a.workers = grid * kWaves;
+  a.window = window, a.out_dtype = out_dtype;
   a.scale = scale * 1.44269504088896341f;
+  const hipStream_t st = (hipStream_t)stream;
+  AttnKern& k = kern(cache, q_dtype);
   void* args[] = {&a};
-  e = hipLaunchKernel(k.fn, dim3(grid), dim3(64 * kWaves), args, (size_t)(rows + 1) * 4, (hipStream_t)stream);
-  if (e == hipSuccess) {
-    // few heads of all: long rows, in many pieces each
-    int lanes = 2;
-    while (4 * lanes < a.dim) lanes *= 2;
-    if (rows * heads >= kJoinMany) join_kernel<256><<<rows * heads, 256, 0, (hipStream_t)stream>>>(a, lanes);
-    else join_kernel<1024><<<rows * heads, 1024, 0, (hipStream_t)stream>>>(a, lanes);
-    e = hipGetLastError();
+  hipError_t e = hipSuccess;
+  if (p.one) {
+    const int units = rows * a.kv_heads, grid = a.groups > 1 ? (units + 7) / 8 * 8 * a.groups : units;
+    e = hipLaunchKernel(k.rows_fn, dim3(grid), dim3(64 * kWaves), args, 0, st);
+  } else {
+    const int grid = grid_of(k, &e);
+    if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_attention: %s", hipGetErrorString(e));
+    a.workers = grid * kWaves;
+    a.prefix = (int32_t*)workspace_dev, a.ws = (float*)((uint8_t*)workspace_dev + prefix_bytes(rows));
+    e = hipLaunchKernel(k.fn, dim3(grid), dim3(64 * kWaves), args, (size_t)(rows + 1) * 4, st);
+    if (e == hipSuccess) {
+      // few heads of all: long rows, in many pieces each
+      int lanes = 2;
+      while (4 * lanes < a.dim) lanes *= 2;
+      if (rows * heads >= kJoinMany) join_kernel<256><<<rows * heads, 256, 0, st>>>(a, lanes);
+      else join_kernel<1024><<<rows * heads, 1024, 0, st>>>(a, lanes);
+      e = hipGetLastError();
+    }
   }
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_attention launch: %s", hipGetErrorString(e));
   return MLXR_OK;

@@ -38,7 +38,7 @@ _pack_cache = struct.Struct("@4P6q5i4x").pack
 _SIGS = {
     "mlxr_page_resize": (_I, [_I] * 3 + [_P, _I64, _I] + [_P] * 9 + [_I, _P, _P]),
     "mlxr_paged_append": (_I, [_P, _I, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _P]),
-    "mlxr_paged_attention_workspace_size": (_I, [_P, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
+    "mlxr_paged_attention_workspace_size": (_I, [_P, _I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
     "mlxr_paged_attention": (_I, [_P, _I, _I, _P, _I, _I64, _I64, _P, _I64, _I, _P, ctypes.c_float, _I, _P, _I, _P, _P,
                                   ctypes.c_size_t, _P]),
 }
@@ -170,20 +170,6 @@ def paged_append(k, v, k_store, v_store, slots, k_scale=None, v_scale=None, stre
                                        _stream(stream, d.index)))
 
 
-_ws_bytes = {}
-
-
-def _attention_workspace(lib, c, device, rows, heads, kv_heads, dim):
-    """Workspace bytes of a call; they depend on the device and the heads alone."""
-    key = (device, heads, kv_heads, dim)
-    got = _ws_bytes.get(key)
-    if got is None:
-        n = ctypes.c_size_t()
-        qgemm._check(lib.mlxr_paged_attention_workspace_size(c, rows, heads, ctypes.byref(n)))
-        got = _ws_bytes[key] = n.value
-    return got
-
-
 def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_scale=None, v_scale=None, out=None,
                     out_dtype=None, return_lse=False, stream=None):
     """Attention of one new token per row, q [rows, heads, head_dim], over the row's cached tokens
@@ -192,7 +178,7 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
     (0: all).  Rows of length 0 give zeros.  Returns out [rows, heads, head_dim] (q's dtype or
     ``out_dtype``), with ``return_lse`` also the log of the softmax's sum, float32 [rows, heads]."""
     lib = _lib()
-    c, _, (_, kv_heads, _, dim) = _cache(k_store, v_store, k_scale, v_scale)
+    c, _, (_, _, _, dim) = _cache(k_store, v_store, k_scale, v_scale)
     d, shape = k_store.device, q.shape
     if len(shape) != 3 or shape[2] != dim:
         raise QGemmError(-3, "queries must be [rows, heads, head_dim]")
@@ -211,12 +197,14 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
     odt = _code(_x_codes, out.dtype, "out")
     q = _rows16(q, stream)
     lse = _on(stream, _torch.empty, (rows, heads), dtype=_torch.float32, device=d) if return_lse else None
-    nb = _attention_workspace(lib, c, d.index, rows, heads, kv_heads, dim)
-    ws = _on(stream, _torch.empty, nb, dtype=_torch.uint8, device=d)
+    nb = ctypes.c_size_t()
+    qgemm._check(lib.mlxr_paged_attention_workspace_size(c, rows, heads, width, ctypes.byref(nb)))
+    nb = nb.value
+    ws = _on(stream, _torch.empty, nb, dtype=_torch.uint8, device=d) if nb else None
     qs = q.stride()
     qgemm._check(lib.mlxr_paged_attention(c, rows, heads, q.data_ptr(), dt, qs[0], qs[1], pt, table.stride()[0], width, pl,
                                           dim ** -0.5 if scale is None else scale, window, out.data_ptr(), odt,
-                                          lse.data_ptr() if return_lse else None, ws.data_ptr(), nb, _stream(stream, d.index)))
+                                          lse.data_ptr() if return_lse else None, ws.data_ptr() if nb else None, nb, _stream(stream, d.index)))
     return (out, lse) if return_lse else out
 
 

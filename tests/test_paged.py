@@ -36,7 +36,7 @@ def test_cache_refusals(change, code, text):
     assert L.mlxr_paged_append(ctypes.byref(c), 1, P(64), 1024, 128, P(64), 1024, 128, mx.BF16, P(64), None) == code
     assert text in L.mlxr_qgemm_last_error().decode()
     n = ctypes.c_size_t()
-    assert L.mlxr_paged_attention_workspace_size(ctypes.byref(c), 1, 8, ctypes.byref(n)) == code
+    assert L.mlxr_paged_attention_workspace_size(ctypes.byref(c), 1, 8, 4, ctypes.byref(n)) == code
 
 
 def test_append_refusals():
@@ -61,18 +61,21 @@ def test_attention_refusals():
         return L.mlxr_paged_attention(ctypes.byref(c), rows, heads, P(q), qdt, qr, qh, P(table), width, width, P(lens), 0.1,
                                       window, P(out), odt, None, P(ws), nb, None)
     assert call(rows=-1) == -1 and call(heads=0) == -1 and call(rows=0) == 0
-    assert call(rows=4097) == -3 and call(heads=33) == -3
+    assert call(rows=1 << 24) == -3 and call(heads=33) == -3
     assert call(qdt=mx.F32) == -1 and call(qdt=mx.F16) == -1 and call(odt=3) == -1 and call(window=-1) == -1
-    for name in ("q", "table", "lens", "out", "ws"):
+    for name in ("q", "table", "lens", "out"):
         assert call(**{name: 0}) == -1, name
-    assert call(width=0) == -1
+    assert call(width=0) == -1 and call(width=100, ws=0) == -1
     assert call(q=72) == -3 and call(qr=4095) == -3 and call(qh=4) == -3 and call(ws=72) == -3
     assert call(width=1 << 30) == -3
-    assert call(rows=4096, width=1 << 26) == -3
-    assert call(nb=16) == -1 and "workspace" in L.mlxr_qgemm_last_error().decode()
+    assert call(c=_cache(k0=1 << 31)) == -3 and call(c=_cache(v2=1 << 31)) == -3
+    assert call(width=100, nb=16) == -1 and "workspace" in L.mlxr_qgemm_last_error().decode()
     n = ctypes.c_size_t()
     c = _cache()
-    assert L.mlxr_paged_attention_workspace_size(ctypes.byref(c), 1, 32, None) == -1
+    assert L.mlxr_paged_attention_workspace_size(ctypes.byref(c), 1, 32, 4, None) == -1
+    assert L.mlxr_paged_attention_workspace_size(ctypes.byref(c), 1, 32, 0, ctypes.byref(n)) == -1
+    assert L.mlxr_paged_attention_workspace_size(ctypes.byref(c), 1, 32, 4, ctypes.byref(n)) == 0 and n.value == 0
+    assert L.mlxr_paged_attention_workspace_size(ctypes.byref(c), 1, 32, 400, ctypes.byref(n)) == 0 and n.value > 0
 
 
 def test_resize_refusals():

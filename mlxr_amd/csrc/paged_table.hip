@@ -15,10 +15,11 @@ struct ResizeArgs {
   const int32_t *lens, *want, *free_count;
   int32_t* free;
   int32_t *lens_out, *count_out, *starts, *slots, *positions, *refused;
-  int rows, page, pages, width, tokens;
+  int rows, page, pages, width, tokens, run;  // run: neighbouring tokens of a thread
+  uint32_t page_mul, page_shift;  // n / page = (mulhi(n, page_mul) + n) >> page_shift for n < 2^31
 };
 
-constexpr int kResizeThreads = 1024;
+constexpr int kResizeThreads = 256;
 
 struct Sum3 {
   int a, b, c;
@@ -56,7 +57,10 @@ __device__ __forceinline__ int row_of(const int* first, int n, int k) {
   return lo;
 }
 
-__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((unsigned)tokens + page - 1) / (unsigned)page); }
+__device__ __forceinline__ int page_of(const ResizeArgs& a, int pos) {
+  return (int)((__umulhi((uint32_t)pos, a.page_mul) + (uint32_t)pos) >> a.page_shift);
+}
+__device__ __forceinline__ int pages_of(const ResizeArgs& a, int tokens) { return page_of(a, tokens + a.page - 1); }
 
 // With P(n) = ceil(n / page): row r takes need = P(want) - P(lens) pages or gives back as many, and the
 // exclusive sums of both over the rows say which place of the stack each page goes to or comes
@@ -64,107 +68,107 @@ __device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((u
 // at c1 - 1 - (N_r + i), c1 = count + all that is given back.  Every output element follows from
 // the sums alone (a page taken from a place at or above `count` is read from the table of the row
 // that gives it back), so nothing in the launch waits for anything else in it: each workgroup
-// makes the sums for itself and fills its share of the outputs.
+// makes the sums for itself and fills its share of the outputs.  What bounds it is latency: lengths,
+// two sums, table or stack, outputs, one after the other.
 __global__ __launch_bounds__(kResizeThreads) void resize_kernel(ResizeArgs a) {
-  extern __shared__ int sh[];
-  int* first_need = sh;               // N_r
-  int* first_give = sh + a.rows;      // G_r
-  int* first_new = sh + 2 * a.rows;   // new tokens before row r
+  extern __shared__ int sh[];  // of each row: N_r, G_r, new tokens before it, P(lens), lens, want (-1: refused)
+  int *first_need = sh, *first_give = sh + a.rows, *first_new = sh + 2 * a.rows, *held = sh + 3 * a.rows,
+      *have = sh + 4 * a.rows, *want = sh + 5 * a.rows;
   __shared__ int part[3 * (kResizeThreads / 64)];
-  const int tid = threadIdx.x, nt = blockDim.x, page = a.page;
-  const int most = a.width * page;
+  __shared__ int most_taken;
+  const int tid = threadIdx.x, nt = kResizeThreads, most = a.width * a.page;
   const int per = (a.rows + nt - 1) / nt, r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
-  auto have_of = [&](int r) { return min(max(a.lens[r], 0), most); };
-
+  if (tid == 0) most_taken = 0;
+  const int count = min(max(a.free_count[0], 0), a.pages);
+  for (int r = tid; r < a.rows; r += nt) {
+    const int w = a.want[r], h = min(max(a.lens[r], 0), most);
+    have[r] = h;
+    want[r] = w < 0 || w > most ? -1 : w;
+    held[r] = pages_of(a, h);
+  }
+  __syncthreads();
+  auto change = [&](int r) { return want[r] < 0 ? 0 : pages_of(a, want[r]) - held[r]; };
   Sum3 mine = {0, 0, 0}, total;
   for (int r = r0; r < r1; ++r) {
-    const int have = have_of(r), want = a.want[r];
-    if (want < 0 || want > most) continue;
-    const int d = pages_of(want, page) - pages_of(have, page);
+    const int d = change(r);
     mine.a += max(d, 0);
     mine.b += max(-d, 0);
   }
   Sum3 before = block_scan(mine, &total, part);
-  const int count = min(max(a.free_count[0], 0), a.pages);
-  const int given = total.b;
-  const int stack = min(count + given, a.pages);
-  int taken = 0, refused = 0;
+  const int given = total.b, stack = min(count + given, a.pages);
+  int taken = 0;
   mine = {0, 0, 0};
   for (int r = r0; r < r1; ++r) {
-    const int have = have_of(r), want = a.want[r];
+    const int d = change(r);
     first_need[r] = before.a;
     first_give[r] = before.b;
-    bool ok = want >= 0 && want <= most;
-    if (ok) {
-      const int d = pages_of(want, page) - pages_of(have, page);
-      if (d > 0) {
-        before.a += d;
-        ok = before.a <= stack;
-        if (ok) taken = before.a;
-      } else {
-        before.b -= d;
-      }
+    before.a += max(d, 0);
+    before.b += max(-d, 0);
+    if (d > 0) {
+      // the sums grow with r: the rows that get pages are a prefix of those that ask
+      if (before.a <= stack) taken = before.a;
+      else want[r] = -1;
     }
-    if (!ok) ++refused;
-    const int len = ok ? want : have;
-    mine.c += max(len - have, 0);
-    if (blockIdx.x == 0) a.lens_out[r] = len;
+    if (want[r] < 0) mine.b += 1;
+    else mine.c += max(want[r] - have[r], 0);
   }
-  mine.b = refused;
-  // the sums grow with r: the rows that get pages are a prefix of those that ask
-  before = block_scan(mine, &total, part);
-  const int new_tokens = total.c, all_refused = total.b;
-  __shared__ int most_taken;
-  if (tid == 0) most_taken = 0;
-  __syncthreads();
   if (taken) atomicMax(&most_taken, taken);
-  int at = before.c;
+  before = block_scan(mine, &total, part);
+  const int new_tokens = total.c;
   for (int r = r0; r < r1; ++r) {
-    first_new[r] = at;
-    if (blockIdx.x == 0) a.starts[r] = at;
-    const int have = have_of(r), want = a.want[r];
-    bool ok = want >= 0 && want <= most;
-    if (ok) {
-      const int d = pages_of(want, page) - pages_of(have, page);
-      ok = d <= 0 || first_need[r] + d <= stack;
-    }
-    at += ok ? max(want - have, 0) : 0;
+    first_new[r] = before.c;
+    before.c += want[r] < 0 ? 0 : max(want[r] - have[r], 0);
   }
   __syncthreads();
   const int all_taken = most_taken;
-  if (blockIdx.x == 0 && tid == 0) {
-    a.starts[a.rows] = new_tokens;
-    a.count_out[0] = stack - all_taken;
-    a.refused[0] = all_refused;
+  if (blockIdx.x == 0) {
+    for (int r = tid; r < a.rows; r += nt) {
+      a.starts[r] = first_new[r];
+      a.lens_out[r] = want[r] < 0 ? have[r] : want[r];
+    }
+    if (tid == 0) {
+      a.starts[a.rows] = new_tokens;
+      a.count_out[0] = stack - all_taken;
+      a.refused[0] = total.b;
+    }
   }
 
   const int gid = blockIdx.x * nt + tid, gn = gridDim.x * nt;
   auto given_page = [&](int k) {  // the k-th page given back
     const int r = row_of(first_give, a.rows, k);
-    return a.table[r * a.stride + pages_of(a.want[r], page) + (k - first_give[r])];
+    return a.table[r * a.stride + pages_of(a, want[r]) + (k - first_give[r])];
   };
   auto taken_page = [&](int k) {  // the k-th page taken
     const int p = stack - 1 - k;
     return p < count ? a.free[p] : given_page(p - count);
   };
-  for (int k = gid; k < all_taken; k += gn) {
+  for (int t = gid * a.run; t < a.tokens; t += gn * a.run) {
+    int r = -1, j = -1, id = -1;
+    for (int at = t; at < min(t + a.run, a.tokens); ++at) {
+      int slot = -1, pos = -1;
+      if (at < new_tokens) {
+        if (r < 0 || (r + 1 < a.rows && first_new[r + 1] <= at)) {
+          r = row_of(first_new, a.rows, at);
+          j = -1;
+        }
+        pos = have[r] + (at - first_new[r]);
+        const int page = page_of(a, pos);
+        if (page != j) {
+          j = page;
+          id = j < held[r] ? a.table[r * a.stride + j] : taken_page(first_need[r] + j - held[r]);
+        }
+        slot = id < 0 || id >= a.pages ? -1 : id * a.page + (pos - j * a.page);
+      }
+      a.slots[at] = slot;
+      a.positions[at] = pos;
+    }
+  }
+  // from the far end of the launch, so that these are other workgroups than the next loop's
+  for (int k = gn - 1 - gid; k < all_taken; k += gn) {
     const int r = row_of(first_need, a.rows, k);
-    a.table[r * a.stride + pages_of(have_of(r), page) + (k - first_need[r])] = taken_page(k);
+    a.table[r * a.stride + held[r] + (k - first_need[r])] = taken_page(k);
   }
   for (int k = gid; k < given && count + k < a.pages; k += gn) a.free[count + k] = given_page(k);
-  for (int t = gid; t < a.tokens; t += gn) {
-    int slot = -1, pos = -1;
-    if (t < new_tokens) {
-      const int r = row_of(first_new, a.rows, t);
-      const int have = have_of(r), held = pages_of(have, page);
-      pos = have + (t - first_new[r]);
-      const int j = (int)((unsigned)pos / (unsigned)page);
-      const int id = j < held ? a.table[r * a.stride + j] : taken_page(first_need[r] + j - held);
-      slot = id < 0 || id >= a.pages ? -1 : id * page + (pos - j * page);
-    }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
-  }
 }
 
 struct AppendSide {
@@ -290,10 +294,23 @@ extern "C" int mlxr_page_resize(int rows, int page_size, int num_pages, int32_t*
   if (lens_out_dev == lens_dev || free_count_out_dev == free_count_dev)
     return set_error(MLXR_E_INVALID, "page_resize: outputs must not be the inputs");
   ResizeArgs a{table_dev, table_stride, lens_dev, want_dev, free_count_dev, free_dev, lens_out_dev, free_count_out_dev,
-               starts_dev, slots_dev, positions_dev, refused_dev, rows, page_size, num_pages, table_width, tokens};
-  const int grid = tokens <= 4096 ? 1 : tokens >= 128 * 4096 ? 128 : (tokens + 4095) / 4096;
-  resize_kernel<<<grid, kResizeThreads, (size_t)rows * 12, (hipStream_t)stream>>>(a);
-  const hipError_t e = hipGetLastError();
+               starts_dev, slots_dev, positions_dev, refused_dev, rows, page_size, num_pages, table_width, tokens, 1, 0, 0};
+  a.page_shift = page_size > 1 ? 32 - __builtin_clz(page_size - 1) : 0;
+  a.page_mul = (uint32_t)((((1ull << a.page_shift) - page_size) << 32) / page_size + 1);
+  // one token for each thread up to 64 workgroups; a prompt's neighbours, mostly of one page, share the search
+  constexpr int kTokens = kResizeThreads * 64;
+  if (tokens > kTokens) a.run = 4;
+  const int64_t groups = ((int64_t)tokens + kResizeThreads * a.run - 1) / (kResizeThreads * a.run);
+  const int grid = groups < 1 ? 1 : groups > 1024 ? 1024 : (int)groups;
+  const size_t lds = (size_t)rows * 6 * sizeof(int);
+  hipError_t e = hipSuccess;
+  if (lds > 48 << 10)
+    e = hipFuncSetAttribute((const void*)resize_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            MLXR_PAGED_MAX_ROWS * 6 * (int)sizeof(int));
+  if (e == hipSuccess) {
+    resize_kernel<<<grid, kResizeThreads, lds, (hipStream_t)stream>>>(a);
+    e = hipGetLastError();
+  }
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "page_resize launch: %s", hipGetErrorString(e));
   return MLXR_OK;
 }

@@ -48,7 +48,7 @@ struct AttnArgs {
   int32_t* prefix;  // [rows + 1] tiles before each row, then tiles of a wavefront, for the join
   int rows, heads, kv_heads, group, groups;  // groups: of 16 heads, of a kv head
   int dim, page, pages, width, window, out_dtype;
-  uint32_t page_mul, page_shift;  // n / page = (mulhi(n, page_mul) + n) >> page_shift for n < 2^31
+  Divisor by_page;
   int part_rows, workers;
   float scale;  // times log2(e)
 };
@@ -143,9 +143,7 @@ struct Attn {
     else return *p;
   }
   // Index of a position's page among its row's.
-  __device__ __forceinline__ int page_of(int pos) const {
-    return (int)((__umulhi((uint32_t)pos, a.page_mul) + (uint32_t)pos) >> a.page_shift);
-  }
+  __device__ __forceinline__ int page_of(int pos) const { return a.by_page.quotient(pos); }
   // Table entry of a position of the row (of the row's last token, past it).
   __device__ __forceinline__ int entry_of(int pos, const Span& s) const { return trow[page_of(min(pos, s.len - 1))]; }
   // Byte offset of a position in a store whose page is `id` (page 0 for one outside the cache: read, not used).

@@ -185,7 +185,7 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   if (workspace_bytes < p.bytes || (p.bytes && !workspace_dev))
     return set_error(MLXR_E_INVALID, "paged_attention: the workspace is smaller than mlxr_paged_attention_workspace_size");
   const int es = cache->dtype == MLXR_E4M3 ? 1 : 2;
-  AttnArgs a;
+  AttnArgs a{};
   a.k = (const uint8_t*)cache->k_dev, a.v = (const uint8_t*)cache->v_dev;
   a.k_scale = cache->k_scale_dev, a.v_scale = cache->v_scale_dev;
   a.k_head = cache->k_stride[1] * es, a.v_head = cache->v_stride[1] * es;
@@ -197,8 +197,7 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   a.rows = rows, a.heads = heads, a.kv_heads = cache->kv_heads;
   a.group = p.group, a.groups = p.groups, a.part_rows = p.part_rows;
   a.dim = cache->head_dim, a.page = cache->page_size, a.pages = cache->num_pages, a.width = table_width;
-  a.page_shift = a.page > 1 ? 32 - __builtin_clz(a.page - 1) : 0;
-  a.page_mul = (uint32_t)((((1ull << a.page_shift) - a.page) << 32) / a.page + 1);
+  a.by_page = Divisor(a.page);
   a.window = window, a.out_dtype = out_dtype;
   a.scale = scale * 1.44269504088896341f;
   const hipStream_t st = (hipStream_t)stream;

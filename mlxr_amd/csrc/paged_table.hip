@@ -16,7 +16,7 @@ struct ResizeArgs {
   int32_t* free;
   int32_t *lens_out, *count_out, *starts, *slots, *positions, *refused;
   int rows, page, pages, width, tokens, run;  // run: neighbouring tokens of a thread
-  uint32_t page_mul, page_shift;  // n / page = (mulhi(n, page_mul) + n) >> page_shift for n < 2^31
+  Divisor by_page;
 };
 
 constexpr int kResizeThreads = 256;
@@ -57,10 +57,7 @@ __device__ __forceinline__ int row_of(const int* first, int n, int k) {
   return lo;
 }
 
-__device__ __forceinline__ int page_of(const ResizeArgs& a, int pos) {
-  return (int)((__umulhi((uint32_t)pos, a.page_mul) + (uint32_t)pos) >> a.page_shift);
-}
-__device__ __forceinline__ int pages_of(const ResizeArgs& a, int tokens) { return page_of(a, tokens + a.page - 1); }
+__device__ __forceinline__ int pages_of(const ResizeArgs& a, int tokens) { return a.by_page.quotient(tokens + a.page - 1); }
 
 // With P(n) = ceil(n / page): row r takes need = P(want) - P(lens) pages or gives back as many, and the
 // exclusive sums of both over the rows say which place of the stack each page goes to or comes
@@ -152,7 +149,7 @@ __global__ __launch_bounds__(kResizeThreads) void resize_kernel(ResizeArgs a) {
           j = -1;
         }
         pos = have[r] + (at - first_new[r]);
-        const int page = page_of(a, pos);
+        const int page = a.by_page.quotient(pos);
         if (page != j) {
           j = page;
           id = j < held[r] ? a.table[r * a.stride + j] : taken_page(first_need[r] + j - held[r]);
@@ -181,36 +178,18 @@ struct AppendSide {
 struct AppendArgs {
   AppendSide side[2];  // keys, values
   const int32_t* slots;
-  int tokens, heads, dim8, page;
-  int64_t slots_end;
+  int items, slots_end;
+  Divisor by_token, by_head, by_page;  // items of a token, of a head; tokens of a page
 };
 
-// One thread moves eight elements of one head's row of one token: 16 bytes of a 16-bit input, and
-// 16 or 8 bytes of the store.
-template <int XT, int CT>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
-  const AppendSide& s = a.side[blockIdx.y];
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per = a.heads * a.dim8;
-  if (i >= (int64_t)a.tokens * per) return;
-  const int t = (int)(i / per), e = (int)(i - (int64_t)t * per), h = e / a.dim8, c = e - h * a.dim8;
-  const int slot = a.slots[t];
-  if (slot < 0 || slot >= a.slots_end) return;
-  const int64_t from = (int64_t)t * s.token + (int64_t)h * s.head + 8 * c;
-  const int pg = slot / a.page;
-  const int64_t to = (int64_t)pg * s.s_page + (int64_t)h * s.s_head + (int64_t)(slot - pg * a.page) * s.s_token + 8 * c;
-  if constexpr (XT == CT) {
-    if (!s.scale) {  // same type: the bits
-      *(uint4*)(s.store + 2 * to) = *(const uint4*)((const uint16_t*)s.x + from);
-      return;
-    }
-  }
-  float v[8];
+// Eight elements at p as floats.
+template <int XT>
+__device__ __forceinline__ void load8(const void* x, int64_t at, float* v) {
   if constexpr (XT == DT_F32) {
-    const float4 lo = *(const float4*)((const float*)s.x + from), hi = *(const float4*)((const float*)s.x + from + 4);
+    const float4 lo = *(const float4*)((const float*)x + at), hi = *(const float4*)((const float*)x + at + 4);
     v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
   } else {
-    const uint4 b = *(const uint4*)((const uint16_t*)s.x + from);
+    const uint4 b = *(const uint4*)((const uint16_t*)x + at);
     const uint32_t w[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -218,32 +197,60 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       v[k] = XT == DT_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
     }
   }
-  if (s.scale) {
-    const float d = s.scale[h];
+}
+__device__ __forceinline__ uint32_t e4m3x4(const float* v) {
+  float c[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] /= d;
-  }
-  if constexpr (CT == MLXR_E4M3) {
+  for (int k = 0; k < 4; ++k) c[k] = v[k] > 448.f ? 448.f : v[k] < -448.f ? -448.f : v[k];  // NaN stays
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
+}
+
+// One thread moves 16 bytes of a store, for the keys and the values: 8 or 16 elements of one head's row of one
+// token.  Bound by memory for a prompt and by the launch for a decode batch.
+template <int XT, int CT>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+  constexpr int N = CT == MLXR_E4M3 ? 16 : 8;
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.items) return;
+  const int t = a.by_token.quotient(i), e = i - t * (int)a.by_token.d, h = a.by_head.quotient(e), c = e - h * (int)a.by_head.d;
+  const int slot = a.slots[t];
+  if (slot < 0 || slot >= a.slots_end) return;
+  const int pg = a.by_page.quotient(slot);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = v[k] > 448.f ? 448.f : v[k] < -448.f ? -448.f : v[k];  // NaN stays
-    uint2 o;
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
-    o.x = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
-    o.y = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], w, true);
-    *(uint2*)(s.store + to) = o;
-  } else {
-    uint32_t o[4];
+  for (int k = 0; k < 2; ++k) {
+    const AppendSide& s = a.side[k];
+    const int64_t from = (int64_t)t * s.token + (int64_t)h * s.head + N * c;
+    const int64_t to = (int64_t)pg * s.s_page + (int64_t)h * s.s_head + (int64_t)(slot - pg * (int)a.by_page.d) * s.s_token + N * c;
+    if constexpr (XT == CT) {
+      if (!s.scale) {  // same type: the bits
+        *(uint4*)(s.store + 2 * to) = *(const uint4*)((const uint16_t*)s.x + from);
+        continue;
+      }
+    }
+    float v[N];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      o[k] = CT == DT_BF16 ? pack_bf16x2(v[2 * k], v[2 * k + 1])
-                           : (f32_to_f16_bits(v[2 * k]) | ((uint32_t)f32_to_f16_bits(v[2 * k + 1]) << 16));
-    *(uint4*)(s.store + 2 * to) = make_uint4(o[0], o[1], o[2], o[3]);
+    for (int n = 0; n < N; n += 8) load8<XT>(s.x, from + n, v + n);
+    if (s.scale) {
+      const float d = s.scale[h];
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] /= d;
+    }
+    if constexpr (CT == MLXR_E4M3) {
+      *(uint4*)(s.store + to) = make_uint4(e4m3x4(v), e4m3x4(v + 4), e4m3x4(v + 8), e4m3x4(v + 12));
+    } else {
+      uint32_t o[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        o[n] = CT == DT_BF16 ? pack_bf16x2(v[2 * n], v[2 * n + 1])
+                             : (f32_to_f16_bits(v[2 * n]) | ((uint32_t)f32_to_f16_bits(v[2 * n + 1]) << 16));
+      *(uint4*)(s.store + 2 * to) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
   }
 }
 
 template <int XT>
-void launch_append(const AppendArgs& a, int ct, dim3 grid, hipStream_t s) {
+void launch_append(const AppendArgs& a, int ct, unsigned grid, hipStream_t s) {
   if (ct == MLXR_F16) append_kernel<XT, DT_F16><<<grid, 256, 0, s>>>(a);
   else if (ct == MLXR_BF16) append_kernel<XT, DT_BF16><<<grid, 256, 0, s>>>(a);
   else append_kernel<XT, MLXR_E4M3><<<grid, 256, 0, s>>>(a);
@@ -294,9 +301,7 @@ extern "C" int mlxr_page_resize(int rows, int page_size, int num_pages, int32_t*
   if (lens_out_dev == lens_dev || free_count_out_dev == free_count_dev)
     return set_error(MLXR_E_INVALID, "page_resize: outputs must not be the inputs");
   ResizeArgs a{table_dev, table_stride, lens_dev, want_dev, free_count_dev, free_dev, lens_out_dev, free_count_out_dev,
-               starts_dev, slots_dev, positions_dev, refused_dev, rows, page_size, num_pages, table_width, tokens, 1, 0, 0};
-  a.page_shift = page_size > 1 ? 32 - __builtin_clz(page_size - 1) : 0;
-  a.page_mul = (uint32_t)((((1ull << a.page_shift) - page_size) << 32) / page_size + 1);
+               starts_dev, slots_dev, positions_dev, refused_dev, rows, page_size, num_pages, table_width, tokens, 1, Divisor(page_size)};
   // one token for each thread up to 64 workgroups; a prompt's neighbours, mostly of one page, share the search
   constexpr int kTokens = kResizeThreads * 64;
   if (tokens > kTokens) a.run = 4;
@@ -328,15 +333,17 @@ extern "C" int mlxr_paged_append(const mlxr_paged_cache* cache, int tokens, cons
   if (k_token_stride % unit || k_head_stride % unit || v_token_stride % unit || v_head_stride % unit ||
       (((uintptr_t)k_dev | (uintptr_t)v_dev) & 15))
     return set_error(MLXR_E_SHAPE, "paged_append: rows must start at multiples of 16 bytes");
+  const int of_head = cache->head_dim / (cache->dtype == MLXR_E4M3 ? 16 : 8);
+  const int64_t items = (int64_t)tokens * cache->kv_heads * of_head;
+  if ((int64_t)cache->kv_heads * of_head > INT32_MAX || items > INT32_MAX - 255)
+    return set_error(MLXR_E_SHAPE, "paged_append: too many elements");
   AppendArgs a{{{k_dev, k_token_stride, k_head_stride, (uint8_t*)cache->k_dev, cache->k_stride[0], cache->k_stride[1],
                  cache->k_stride[2], cache->k_scale_dev},
                 {v_dev, v_token_stride, v_head_stride, (uint8_t*)cache->v_dev, cache->v_stride[0], cache->v_stride[1],
                  cache->v_stride[2], cache->v_scale_dev}},
-               slots_dev, tokens, cache->kv_heads, cache->head_dim / 8, cache->page_size,
-               (int64_t)cache->num_pages * cache->page_size};
-  const int64_t blocks = ((int64_t)tokens * a.heads * a.dim8 + 255) / 256;
-  if (blocks > INT32_MAX) return set_error(MLXR_E_SHAPE, "paged_append: too many elements");
-  const dim3 grid((unsigned)blocks, 2);
+               slots_dev, (int)items, cache->num_pages * cache->page_size,
+               Divisor(of_head * cache->kv_heads), Divisor(of_head), Divisor(cache->page_size)};
+  const unsigned grid = (unsigned)((items + 255) / 256);
   const hipStream_t s = (hipStream_t)stream;
   if (x_dtype == MLXR_F32) launch_append<DT_F32>(a, cache->dtype, grid, s);
   else if (x_dtype == MLXR_F16) launch_append<DT_F16>(a, cache->dtype, grid, s);

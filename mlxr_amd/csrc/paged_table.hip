@@ -182,22 +182,22 @@ struct AppendArgs {
   Divisor by_token, by_head, by_page;  // items of a token, of a head; tokens of a page
 };
 
-// Eight elements at p as floats.
+// Eight elements of a row as they lie in memory, and as floats.
 template <int XT>
-__device__ __forceinline__ void load8(const void* x, int64_t at, float* v) {
-  if constexpr (XT == DT_F32) {
-    const float4 lo = *(const float4*)((const float*)x + at), hi = *(const float4*)((const float*)x + at + 4);
-    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-  } else {
-    const uint4 b = *(const uint4*)((const uint16_t*)x + at);
-    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t u = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
-      v[k] = XT == DT_BF16 ? bf16_bits_to_f32(u) : f16_bits_to_f32(u);
-    }
+struct Eight {
+  uint4 w[XT == DT_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* x, int64_t at) {
+    if constexpr (XT == DT_F32) w[0] = ((const uint4*)((const float*)x + at))[0], w[1] = ((const uint4*)((const float*)x + at))[1];
+    else w[0] = *(const uint4*)((const uint16_t*)x + at);
   }
-}
+  __device__ __forceinline__ float get(int k) const {
+    const uint4& q = w[XT == DT_F32 ? k >> 2 : 0];
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (XT == DT_F32) return __builtin_bit_cast(float, u[k & 3]);
+    const uint32_t h = (u[k >> 1] >> (16 * (k & 1))) & 0xffffu;
+    return XT == DT_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+  }
+};
 __device__ __forceinline__ uint32_t e4m3x4(const float* v) {
   float c[4];
 #pragma unroll
@@ -214,23 +214,27 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= a.items) return;
   const int t = a.by_token.quotient(i), e = i - t * (int)a.by_token.d, h = a.by_head.quotient(e), c = e - h * (int)a.by_head.d;
+  Eight<XT> x[2][N / 8];  // on their way together with the slot
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int n = 0; n < N / 8; ++n) x[k][n].load(a.side[k].x, (int64_t)t * a.side[k].token + (int64_t)h * a.side[k].head + N * c + 8 * n);
   const int slot = a.slots[t];
   if (slot < 0 || slot >= a.slots_end) return;
   const int pg = a.by_page.quotient(slot);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const AppendSide& s = a.side[k];
-    const int64_t from = (int64_t)t * s.token + (int64_t)h * s.head + N * c;
     const int64_t to = (int64_t)pg * s.s_page + (int64_t)h * s.s_head + (int64_t)(slot - pg * (int)a.by_page.d) * s.s_token + N * c;
     if constexpr (XT == CT) {
       if (!s.scale) {  // same type: the bits
-        *(uint4*)(s.store + 2 * to) = *(const uint4*)((const uint16_t*)s.x + from);
+        *(uint4*)(s.store + 2 * to) = x[k][0].w[0];
         continue;
       }
     }
     float v[N];
 #pragma unroll
-    for (int n = 0; n < N; n += 8) load8<XT>(s.x, from + n, v + n);
+    for (int n = 0; n < N; ++n) v[n] = x[k][n / 8].get(n % 8);
     if (s.scale) {
       const float d = s.scale[h];
 #pragma unroll

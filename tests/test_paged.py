@@ -280,6 +280,28 @@ def test_append_rounds_every_e4m3_value_and_middle(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["bf16", "f16", "f8"])
+def test_append_divides_as_division_does(cuda, cache):
+    """Quotients over the whole range of fp32, infinite and NaN ones, scales of zero, subnormal and infinite."""
+    import torch
+    g = torch.Generator().manual_seed(7)
+    scales = torch.cat([torch.tensor([0.0, -0.0, 1e-44, 1e-38, 3e38, float("inf"), float("nan"), -0.3, 1.0, 3.0]),
+                        (torch.rand(54, generator=g) * 2 - 1) * 2.0 ** torch.randint(-126, 127, (54,), generator=g)])
+    x = (torch.rand(40, 64, 64, generator=g) * 2 - 1) * 2.0 ** torch.randint(-140, 127, (40, 64, 64), generator=g)
+    x[1] = torch.rand(64, 64, generator=g) * scales[:, None] * 3
+    x[0, :, :6] = torch.tensor([0.0, -0.0, float("inf"), float("-inf"), float("nan"), 3.4e38])
+    store = torch.zeros((1, 64, 40, 64), dtype=_dt(cache), device=cuda)
+    slots = torch.arange(40, dtype=torch.int32, device=cuda)
+    s = scales.to(cuda)
+    mx.paged_append(x.to(cuda), x.to(cuda), store, torch.empty_like(store), slots, s, s)
+    q = x / scales[None, :, None]
+    want = (q.clamp(-448, 448) if cache == "f8" else q).to(_dt(cache)).float()
+    got = store[0].permute(1, 0, 2).float().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(0.0, 1e39, -1e39), want.nan_to_num(0.0, 1e39, -1e39))
+
+
+@pytest.mark.gpu
 def test_append_takes_slices_of_a_fused_projection(cuda):
     import torch
     heads, dim, n, page, pages = 4, 64, 9, 16, 3
@@ -433,7 +455,27 @@ def test_attention_split_over_the_length(cuda, lens, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f8")])
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 128, 16), (33, 1, 64, 8), (40, 2, 80, 5), (4, 4, 256, 32)])
+def test_attention_cut_and_uncut(cuda, dtype, cache, heads, kv, dim, page):
+    """The same rows behind a table that holds little more than they need and one that could hold 40000 tokens."""
+    import torch
+    lens = [0, 1, 33, 150, 64]
+    (k, v), table, (keys, values) = _fill(cuda, lens, kv, dim, page, cache, False, 11)
+    wide = torch.full((len(lens), 40000 // page), -5, dtype=torch.int32, device=cuda)
+    wide[:, :table.shape[1]] = table
+    q = torch.randn(len(lens), heads, dim, device=cuda).to(_dt(dtype))
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    ref, ref_lse = _attend64(q, keys, values, lens, 0, dim ** -0.5)
+    for t in (table, wide):
+        got, lse = mx.paged_attention(q, k, v, t, lt, out_dtype=torch.float32, return_lse=True)
+        _check(got, ref, values, lens, "f32")
+        assert (lse[0] == -math.inf).all() and float((lse[1:].double().cpu() - ref_lse[1:]).abs().max()) < 1e-3
+
+
+@pytest.mark.gpu
 def test_attention_of_many_rows(cuda):
+    _run(cuda, [(i * 5) % 40 for i in range(5000)], 2, 1, 64, 16, "bf16", "bf16")
     _run(cuda, [(i * 7) % 50 for i in range(2500)], 4, 2, 64, 8, "bf16", "bf16")
 
 

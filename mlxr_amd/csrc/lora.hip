@@ -21,13 +21,14 @@ namespace mlxr {
 namespace {
 
 constexpr int kItems = 4;      // projections of one launch
-constexpr int kThreads = 256;  // of expand, and of shrink over 64-token tiles
+constexpr int kThreads = 256;  // of expand
 constexpr int kWaves = kThreads / 64;
-constexpr int kShrinkWide = 512;  // threads of shrink over 16-token tiles
+constexpr int kShrinkThreads = 512;
 constexpr int kInline = kThreads;  // tokens
-// Groups of 16 tokens in a tile of the sorted tokens: the accumulators of a wavefront, sub * rank / 16 of
-// four registers, and what the wavefronts of a workgroup add up in LDS, stay at 16.
+// Groups of 16 tokens in a tile of the sorted tokens, for which expand reads its columns of B once; and those
+// that a workgroup of shrink takes of it.
 constexpr int sub_of(int rank_groups) { return rank_groups > 4 ? 2 : 4; }
+constexpr int shrink_sub(int rank_groups, int sub) { return sub == 1 || rank_groups > 4 ? 1 : 2; }
 constexpr int rank_groups_of(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 constexpr int kMaxSplits = 8;  // of K
 constexpr int kPlanThreads = 1024;
@@ -156,33 +157,39 @@ __device__ __forceinline__ int tile_tokens(const LoraArgs& a, int index, int* ad
   }
 }
 
-// h of one tile over one chunk of K: the wavefronts take turns over it in steps of 64 and add up in LDS.
-// RT: groups of 16 ranks; SUB: of 16 tokens.  A lane reads 32 neighbouring bytes of a row of x or A,
-// the four lane groups 128: which k an operand's place stands for is free, alike for both.
+// h of SS groups of 16 tokens of a tile over one chunk of K: the wavefronts take turns over it in steps of 64
+// and add up in LDS.  RT: groups of 16 ranks; SUB: of 16 tokens in a tile.  A lane reads 32 neighbouring
+// bytes of a row of x or A, the four lane groups 128: which k an operand's place stands for is free, alike
+// for both.
 template <bool F16, int RT, int SUB, bool INLINE>
-__global__ __launch_bounds__(SUB == 1 ? kShrinkWide : kThreads) void shrink_kernel(LoraArgs a) {
-  constexpr int kWaves = (SUB == 1 ? kShrinkWide : kThreads) / 64;
-  __shared__ int token[16 * SUB];
-  __shared__ f32x4_t sh[kWaves - 1][SUB * RT][64];
+__global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
+  constexpr int kWaves = kShrinkThreads / 64, SS = shrink_sub(RT, SUB);
+  __shared__ int tokens[16 * SUB];
+  __shared__ f32x4_t sh[kWaves - 1][SS * RT][64];
   int adapter = 0;
-  const int count = tile_tokens<INLINE, kWaves>(a, blockIdx.x, &adapter, token);
-  if (count == 0 || adapter == a.adapters) return;
+  const int all = tile_tokens<INLINE, kWaves>(a, blockIdx.x / (SUB / SS), &adapter, tokens);
+  const int sub = blockIdx.x % (SUB / SS) * SS * 16, count = min(all - sub, 16 * SS);
+  if (count <= 0 || adapter == a.adapters) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int split = blockIdx.y, item = blockIdx.z, rank = rank_of(a, adapter);
   const int k_end = min((split + 1) * a.chunk, a.K);
   const uint16_t* A = (const uint16_t*)a.item[item].a_dev + (int64_t)adapter * a.rank * a.K + (int64_t)col * a.K;
-  const uint16_t* x[SUB];
+  int token[SS];
+  const uint16_t* x[SS];
 #pragma unroll
-  for (int s = 0; s < SUB; ++s) x[s] = a.x + (int64_t)token[16 * s + col < count ? 16 * s + col : 0] * a.x_stride;
-  f32x4_t acc[SUB][RT] = {};
-  u32x4_t xf[SUB][2], af[RT][2];
+  for (int s = 0; s < SS; ++s) {
+    token[s] = tokens[sub + (16 * s + col < count ? 16 * s + col : 0)];
+    x[s] = a.x + (int64_t)token[s] * a.x_stride;
+  }
+  f32x4_t acc[SS][RT] = {};
+  u32x4_t xf[SS][2], af[RT][2];
   auto load = [&](int k) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int kk = k + 16 * g + 8 * e;
       const bool in = kk < k_end;
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) xf[s][e] = in ? *(const u32x4_t*)(x[s] + kk) : u32x4_t{0, 0, 0, 0};
+      for (int s = 0; s < SS; ++s) xf[s][e] = in ? *(const u32x4_t*)(x[s] + kk) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int r = 0; r < RT; ++r)
         af[r][e] = in && 16 * r + col < rank ? *(const u32x4_t*)(A + (int64_t)(16 * r) * a.K + kk) : u32x4_t{0, 0, 0, 0};
@@ -191,11 +198,11 @@ __global__ __launch_bounds__(SUB == 1 ? kShrinkWide : kThreads) void shrink_kern
   int k = split * a.chunk + wave * 64;
   load(k);
   while (k < k_end) {
-    u32x4_t xc[SUB][2], ac[RT][2];
+    u32x4_t xc[SS][2], ac[RT][2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) xc[s][e] = xf[s][e];
+      for (int s = 0; s < SS; ++s) xc[s][e] = xf[s][e];
 #pragma unroll
       for (int r = 0; r < RT; ++r) ac[r][e] = af[r][e];
     }
@@ -204,21 +211,21 @@ __global__ __launch_bounds__(SUB == 1 ? kShrinkWide : kThreads) void shrink_kern
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int s = 0; s < SUB; ++s)
+      for (int s = 0; s < SS; ++s)
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[s][r] = mfma16<F16>(ac[r][e], xc[s][e], acc[s][r]);
   }
   if (wave)
 #pragma unroll
-    for (int s = 0; s < SUB; ++s)
+    for (int s = 0; s < SS; ++s)
 #pragma unroll
       for (int r = 0; r < RT; ++r) sh[wave - 1][s * RT + r][lane] = acc[s][r];
   __syncthreads();
   if (wave) return;
 #pragma unroll
-  for (int s = 0; s < SUB; ++s) {
+  for (int s = 0; s < SS; ++s) {
     if (16 * s + col >= count) continue;
-    float* h = a.h + (((int64_t)item * a.splits + split) * a.tokens + token[16 * s + col]) * a.rank + 4 * g;
+    float* h = a.h + (((int64_t)item * a.splits + split) * a.tokens + token[s]) * a.rank + 4 * g;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       f32x4_t v = acc[s][r];
@@ -229,49 +236,53 @@ __global__ __launch_bounds__(SUB == 1 ? kShrinkWide : kThreads) void shrink_kern
   }
 }
 
-// 16 neighbouring columns n .. of a token's row of y, as they lie in memory (YT: the type); rows start at
-// multiples of 16 bytes where vec.
+// Columns n .. n + 7 and n + 32 .. n + 39 of a token's row of y, as they lie in memory (YT: the type); rows start
+// at multiples of 16 bytes where vec.
 template <int YT>
 struct Cols {
-  static constexpr int W = YT == DT_F32 ? 4 : 2;
+  static constexpr int W = YT == DT_F32 ? 4 : 2, S = YT == DT_F32 ? 4 : 2;  // 16-byte words; bytes of an element
   u32x4_t w[W];
+  // byte offset of word c
+  static __device__ __forceinline__ int64_t at(int64_t row, int n, int c) {
+    return (row + n) * S + (YT == DT_F32 ? (c >> 1) * 128 + (c & 1) * 16 : c * 64);
+  }
   __device__ __forceinline__ void load(const mlxr_lora_item& it, int64_t row, int n, bool vec) {
-    if (!vec || n + 16 > it.N) return;
-    const u32x4_t* y = (const u32x4_t*)((const uint8_t*)it.y_dev + (row + n) * (YT == DT_F32 ? 4 : 2));
+    if (!vec || n + 40 > it.N) return;
 #pragma unroll
-    for (int c = 0; c < W; ++c) w[c] = y[c];
+    for (int c = 0; c < W; ++c) w[c] = *(const u32x4_t*)((const uint8_t*)it.y_dev + at(row, n, c));
   }
   // out = y + v * back
   __device__ __forceinline__ void store(const mlxr_lora_item& it, int64_t row, int n, bool vec, const f32x4_t* v, float back) {
-    if (vec && n + 16 <= it.N) {
-      u32x4_t* o = (u32x4_t*)((uint8_t*)it.out_dev + (row + n) * (YT == DT_F32 ? 4 : 2));
+    if (vec && n + 40 <= it.N) {
 #pragma unroll
       for (int c = 0; c < W; ++c) {
+        u32x4_t p;
         if constexpr (YT == DT_F32) {
-          o[c] = __builtin_bit_cast(u32x4_t, __builtin_bit_cast(f32x4_t, w[c]) + v[c] * back);
+          p = __builtin_bit_cast(u32x4_t, __builtin_bit_cast(f32x4_t, w[c]) + v[c] * back);
         } else {
           constexpr bool F = YT == DT_F16;
-          u32x4_t p;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             p[e] = pack2<F>(unpack<F>(w[c][e], 0) + v[2 * c + (e >> 1)][2 * (e & 1)] * back,
                             unpack<F>(w[c][e], 1) + v[2 * c + (e >> 1)][2 * (e & 1) + 1] * back);
-          o[c] = p;
         }
+        *(u32x4_t*)((uint8_t*)it.out_dev + at(row, n, c)) = p;
       }
       return;
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (n + 4 * c + i < it.N)
-          store_scalar(it.out_dev, YT, row + n + 4 * c + i, load_scalar(it.y_dev, YT, row + n + 4 * c + i) + v[c][i] * back);
+      for (int i = 0; i < 4; ++i) {
+        const int col = n + 32 * (c >> 1) + 4 * (c & 1) + i;
+        if (col < it.N) store_scalar(it.out_dev, YT, row + col, load_scalar(it.y_dev, YT, row + col) + v[c][i] * back);
+      }
   }
 };
 
 // One tile and `columns` columns of an item, in steps of 64 for each wavefront.  Row 4 g + i of the c-th
-// product of a step is column 16 g + 4 c + i, so a lane ends with 16 neighbouring columns of its token.  h enters
+// product of a step is column 32 (c / 2) + 8 g + 4 (c % 2) + i: a lane ends with 8 neighbouring columns of its
+// token, twice, and the four lane groups with 64 bytes in a row, whole requests of a store.  h enters
 // as the sum of two 16-bit parts: rounded to one it would lose what the fp32 sums kept.
 template <bool F16, int RT, int SUB, bool INLINE>
 __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
@@ -301,7 +312,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
     for (int k = 0; k < KT; ++k)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int n = n0 + 16 * (col >> 2) + 4 * c + (col & 3), at = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g, left = rank - at;
+        const int n = n0 + 32 * (c >> 1) + 8 * (col >> 2) + 4 * (c & 1) + (col & 3), at = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g, left = rank - at;
         next[k][c] = n < it.N && left > 0 ? *(const u32x4_t*)(B + (int64_t)n * a.rank + at) : u32x4_t{0, 0, 0, 0};
         if (left < 8)
 #pragma unroll
@@ -366,7 +377,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) bf[k][c] = next[k][c];
       Cols<YT> y;
-      const int n = n0 + 16 * g;
+      const int n = n0 + 8 * g;
       auto row_of = [&](int s) { return (int64_t)token[16 * s + col] * it.N; };
       if (col < count) y.load(it, row_of(0), n, vec);
       if (n0 + kWaves * 64 < end) load_b(n0 + kWaves * 64);
@@ -415,8 +426,11 @@ Layout layout_of(int count, int tokens, int K, int adapters, int rank) {
   l.tiles = tokens <= kInline ? tokens : std::min(tokens, tokens / tm + buckets);
   // enough workgroups for the device; a wavefront takes two steps of K or more
   l.live = std::min(tokens, tokens / tm + buckets);
-  const long want = 512 / ((long)l.live * items) + 1;
-  const int most = std::min(kMaxSplits, (K + 511) / 512);
+  const bool sorted = tokens > kInline;
+  const int group = sorted ? 16 * shrink_sub(rank_groups_of(rank), 2) : 16;
+  const long want = 512 / ((long)std::min(tokens, tokens / group + buckets) * items) + 1;
+  // expand reads h as often as it has columns / 512, so of many tokens few parts
+  const int most = std::min(sorted ? 4 : kMaxSplits, (K + 511) / 512);
   int splits = (int)(want < most ? want : most);
   l.chunk = ((K + splits - 1) / splits + 63) / 64 * 64;
   l.splits = (K + l.chunk - 1) / l.chunk;
@@ -433,7 +447,7 @@ template <bool F16, int RT, int SUB, bool INLINE>
 void launch(const LoraArgs& a, int tiles, hipStream_t s) {
   int wide = 0;
   for (int i = 0; i < a.count; ++i) wide = wide > a.item[i].N ? wide : a.item[i].N;
-  shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles, a.splits, a.count), SUB == 1 ? kShrinkWide : kThreads, 0, s>>>(a);
+  shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles * (SUB / shrink_sub(RT, SUB)), a.splits, a.count), kShrinkThreads, 0, s>>>(a);
   expand_kernel<F16, RT, SUB, INLINE><<<dim3((wide + a.columns - 1) / a.columns, tiles, a.count), kThreads, 0, s>>>(a);
 }
 template <bool F16, int RT>

@@ -30,7 +30,9 @@ constexpr int kInline = kThreads;  // tokens
 constexpr int sub_of(int rank_groups) { return rank_groups > 4 ? 2 : 4; }
 constexpr int shrink_sub(int rank_groups, int sub) { return sub == 1 || rank_groups > 4 ? 1 : 2; }
 constexpr int rank_groups_of(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
-constexpr int kMaxSplits = 8;  // of K
+// Most splits of K.  Expand reads h for each of its workgroups, so of many tokens few parts (2048 tokens, rank
+// 32: shrink and expand 14 + 65 us with four, 21 + 63 with one).
+constexpr int max_splits(bool few_tokens) { return few_tokens ? 8 : 4; }
 constexpr int kPlanThreads = 1024;
 constexpr int kExpandGroups = 2048;  // workgroups of expand: eight for each CU
 
@@ -120,33 +122,57 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
 }
 
 // Tile `index`: its adapter (a.adapters: none), its tokens in token[0 .. count).  count 0: there is no such
-// tile.  INLINE: tile t exists if token t is the 1st, 17th, 33rd .. of its adapter, and holds it and the next 15.
+// tile.  INLINE: every workgroup ranks the tokens among those of their adapter; tiles start at the tokens of rank 0,
+// 16, 32 .., in the order of these tokens.  Its dynamic LDS holds a counter for each adapter.
 template <bool INLINE, int WAVES>
 __device__ __forceinline__ int tile_tokens(const LoraArgs& a, int index, int* adapter, int* token) {
   const int tid = threadIdx.x;
   if constexpr (INLINE) {
-    __shared__ uint64_t same[WAVES];
-    const int lane = tid & 63, wave = tid >> 6;
-    auto bucket = [&](int id) { return id >= 0 && id < a.adapters ? id : a.adapters; };
-    const int mine = bucket(a.ids[index]);
-    const bool eq = tid < a.tokens && bucket(a.ids[min(tid, a.tokens - 1)]) == mine;
-    const uint64_t vote = __ballot(eq);
-    if (lane == 0) same[wave] = vote;
+    extern __shared__ int seen[];
+    __shared__ uint64_t starts[WAVES];
+    __shared__ int chosen[2];
+    const int lane = tid & 63, wave = tid >> 6, waves = (a.tokens + 63) >> 6;
+    const uint64_t below = (1ull << lane) - 1;
+    int b = -1;
+    if (tid < a.tokens) {
+      b = a.ids[tid];
+      b = b >= 0 && b < a.adapters ? b : a.adapters;
+    }
+    for (int i = tid; i <= a.adapters; i += 64 * WAVES) seen[i] = 0;
+    uint64_t peers = __ballot(b >= 0);  // lanes of the same adapter, bit by bit of its number
+    for (int bit = 1; bit <= a.adapters; bit *= 2) {
+      const uint64_t set = __ballot((b & bit) != 0);
+      peers &= b & bit ? set : ~set;
+    }
     __syncthreads();
-    int before = 0, at = 0, all = 0;  // of the adapter: tokens before `index`, before this thread's, all
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const uint64_t v = same[w];
-      const int n = __popcll(v);
-      before += w < (index >> 6) ? n : w == (index >> 6) ? __popcll(v & ((1ull << (index & 63)) - 1)) : 0;
-      at += w < wave ? n : w == wave ? __popcll(v & ((1ull << lane) - 1)) : 0;
+    int rank = -1;
+    for (int w = 0; w < waves; ++w) {
+      if (wave == w && b >= 0) {
+        const int before = seen[b];
+        rank = before + __popcll(peers & below);
+        if ((peers & below) == 0) seen[b] = before + __popcll(peers);
+      }
+      __syncthreads();
+    }
+    const bool start = b >= 0 && (rank & 15) == 0;
+    const uint64_t vote = __ballot(start);
+    if (lane == 0) starts[wave] = vote;
+    __syncthreads();
+    int at = 0, all = 0;  // starts before this token, all
+    for (int w = 0; w < waves; ++w) {
+      const int n = __popcll(starts[w]);
+      at += w < wave ? n : w == wave ? __popcll(vote & below) : 0;
       all += n;
     }
-    if (before & 15) return 0;
-    if (eq && at >= before && at < before + 16) token[at - before] = tid;
-    *adapter = mine;
+    if (index >= all) return 0;
+    if (start && at == index) chosen[0] = b, chosen[1] = rank;
     __syncthreads();
-    return min(16, all - before);
+    const int first = chosen[1];
+    *adapter = chosen[0];
+    if (b == chosen[0] && rank >= first && rank < first + 16) token[rank - first] = tid;
+    const int count = min(16, seen[chosen[0]] - first);
+    __syncthreads();
+    return count;
   } else {
     if (index >= a.counts[1]) return 0;
     const Tile t = a.tiles[index];
@@ -236,57 +262,60 @@ __global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
   }
 }
 
-// Columns n .. n + 7 and n + 32 .. n + 39 of a token's row of y, as they lie in memory (YT: the type); rows start
-// at multiples of 16 bytes where vec.
-template <int YT>
+// CT neighbouring columns of a token's row of y, as they lie in memory (YT: the type); rows start at multiples of
+// 16 bytes where vec.
+template <int YT, int CT>
 struct Cols {
-  static constexpr int W = YT == DT_F32 ? 4 : 2, S = YT == DT_F32 ? 4 : 2;  // 16-byte words; bytes of an element
-  u32x4_t w[W];
-  // byte offset of word c
-  static __device__ __forceinline__ int64_t at(int64_t row, int n, int c) {
-    return (row + n) * S + (YT == DT_F32 ? (c >> 1) * 128 + (c & 1) * 16 : c * 64);
-  }
-  __device__ __forceinline__ void load(const mlxr_lora_item& it, int64_t row, int n, bool vec) {
-    if (!vec || n + 40 > it.N) return;
+  static constexpr int S = YT == DT_F32 ? 4 : 2, W = CT * S / 4;  // bytes of an element; words
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const mlxr_lora_item& it, int64_t at, bool in) {
+    if (!in) return;
+    const uint8_t* p = (const uint8_t*)it.y_dev + at * S;
+    if constexpr (W == 2) {
+      const u32x2_t v = *(const u32x2_t*)p;
+      w[0] = v.x, w[1] = v.y;
+    } else {
 #pragma unroll
-    for (int c = 0; c < W; ++c) w[c] = *(const u32x4_t*)((const uint8_t*)it.y_dev + at(row, n, c));
-  }
-  // out = y + v * back
-  __device__ __forceinline__ void store(const mlxr_lora_item& it, int64_t row, int n, bool vec, const f32x4_t* v, float back) {
-    if (vec && n + 40 <= it.N) {
-#pragma unroll
-      for (int c = 0; c < W; ++c) {
-        u32x4_t p;
-        if constexpr (YT == DT_F32) {
-          p = __builtin_bit_cast(u32x4_t, __builtin_bit_cast(f32x4_t, w[c]) + v[c] * back);
-        } else {
-          constexpr bool F = YT == DT_F16;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            p[e] = pack2<F>(unpack<F>(w[c][e], 0) + v[2 * c + (e >> 1)][2 * (e & 1)] * back,
-                            unpack<F>(w[c][e], 1) + v[2 * c + (e >> 1)][2 * (e & 1) + 1] * back);
-        }
-        *(u32x4_t*)((uint8_t*)it.out_dev + at(row, n, c)) = p;
+      for (int k = 0; k < W; k += 4) {
+        const u32x4_t v = *(const u32x4_t*)(p + 4 * k);
+        w[k] = v.x, w[k + 1] = v.y, w[k + 2] = v.z, w[k + 3] = v.w;
       }
+    }
+  }
+  // out = y + v * back; left: columns that the row has from here on
+  __device__ __forceinline__ void store(const mlxr_lora_item& it, int64_t at, bool in, int left, const float* v, float back) {
+    if (in) {
+      uint32_t o[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        if constexpr (YT == DT_F32) o[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, w[k]) + v[k] * back);
+        else o[k] = pack2<YT == DT_F16>(unpack<YT == DT_F16>(w[k], 0) + v[2 * k] * back, unpack<YT == DT_F16>(w[k], 1) + v[2 * k + 1] * back);
+      }
+      uint8_t* p = (uint8_t*)it.out_dev + at * S;
+      if constexpr (W == 2) *(u32x2_t*)p = u32x2_t{o[0], o[1]};
+      else
+#pragma unroll
+        for (int k = 0; k < W; k += 4) *(u32x4_t*)(p + 4 * k) = u32x4_t{o[k], o[k + 1], o[k + 2], o[k + 3]};
       return;
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int col = n + 32 * (c >> 1) + 4 * (c & 1) + i;
-        if (col < it.N) store_scalar(it.out_dev, YT, row + col, load_scalar(it.y_dev, YT, row + col) + v[c][i] * back);
-      }
+    for (int c = 0; c < CT; ++c)
+      if (c < left) store_scalar(it.out_dev, YT, at + c, load_scalar(it.y_dev, YT, at + c) + v[c] * back);
   }
 };
 
-// One tile and `columns` columns of an item, in steps of 64 for each wavefront.  Row 4 g + i of the c-th
-// product of a step is column 32 (c / 2) + 8 g + 4 (c % 2) + i: a lane ends with 8 neighbouring columns of its
-// token, twice, and the four lane groups with 64 bytes in a row, whole requests of a store.  h enters
-// as the sum of two 16-bit parts: rounded to one it would lose what the fp32 sums kept.
+// Columns of a wavefront's step: 64 for few tokens (more workgroups), 128 for many: 256 bytes of a row in one
+// store of 16-bit outputs (2048 tokens, two projections of 14336: 62 -> 55 us).
+// In units of 16.
+constexpr int columns_of(int sub) { return sub == 1 ? 4 : 8; }
+
+// One tile and `columns` columns of an item, in steps of 16 CT for each wavefront.  Tokens are the rows of the
+// products; column n of the c-th is column CT n + c, so a lane ends with CT neighbouring columns of four
+// tokens, and 16 lanes with a stretch of a row.  h enters as the sum of two 16-bit parts: rounded to one it would
+// lose what the fp32 sums kept.
 template <bool F16, int RT, int SUB, bool INLINE>
 __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
-  constexpr int R = 16 * RT, KT = RT == 1 ? 1 : RT / 2;
+  constexpr int R = 16 * RT, KT = RT == 1 ? 1 : RT / 2, CT = columns_of(SUB);
   constexpr int ROW = 2 * R + 8;  // of LDS: R high parts, R low parts; padded against bank conflicts
   __shared__ int token[16 * SUB];
   __shared__ float back[16 * SUB];
@@ -301,18 +330,18 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
   if (none && it.out_dev == it.y_dev) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   const int rank = none ? 0 : rank_of(a, adapter);
-  // operands of B for 64 columns, on their way while h is summed up or the columns before are computed; RT 1
+  // operands of B for a step, on their way while h is summed up or the columns before are computed; RT 1
   // multiplies the high and the low parts in one step, ranks 8 (g & 1) ..
   const uint16_t* B = (const uint16_t*)it.b_dev + (int64_t)(none ? 0 : adapter) * it.N * a.rank;
   const int end = min(begin + a.columns, it.N);
-  int n0 = begin + wave * 64;
-  u32x4_t next[KT][4];
+  int n0 = begin + wave * 16 * CT;
+  u32x4_t next[KT][CT];
   auto load_b = [&](int n0) {
 #pragma unroll
     for (int k = 0; k < KT; ++k)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int n = n0 + 32 * (c >> 1) + 8 * (col >> 2) + 4 * (c & 1) + (col & 3), at = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g, left = rank - at;
+      for (int c = 0; c < CT; ++c) {
+        const int n = n0 + CT * col + c, at = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g, left = rank - at;
         next[k][c] = n < it.N && left > 0 ? *(const u32x4_t*)(B + (int64_t)n * a.rank + at) : u32x4_t{0, 0, 0, 0};
         if (left < 8)
 #pragma unroll
@@ -329,13 +358,14 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
       if (t < count && at < rank) {
         const float* p = a.h + ((int64_t)blockIdx.z * a.splits * a.tokens + token[t]) * a.rank + at;
         const int64_t step = (int64_t)a.tokens * a.rank;
-        f32x4_t in[kMaxSplits][2];
+        constexpr int kMost = max_splits(INLINE);
+        f32x4_t in[kMost][2];
 #pragma unroll
-        for (int s = 0; s < kMaxSplits; ++s)
+        for (int s = 0; s < kMost; ++s)
 #pragma unroll
           for (int e = 0; e < 2; ++e) in[s][e] = s < a.splits ? *(const f32x4_t*)(p + s * step + 4 * e) : f32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < kMaxSplits; ++s)
+        for (int s = 0; s < kMost; ++s)
 #pragma unroll
           for (int e = 0; e < 2; ++e) v[e] += in[s][e];
       }
@@ -370,23 +400,31 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
   const bool vec = (it.N * (it.y_dtype == DT_F32 ? 4 : 2)) % 16 == 0 && (((uintptr_t)it.y_dev | (uintptr_t)it.out_dev) & 15) == 0;
   auto columns = [&](auto yt) {
     constexpr int YT = decltype(yt)::value;
-    for (; n0 < end; n0 += kWaves * 64) {
-      u32x4_t bf[KT][4];
+    constexpr bool AHEAD = SUB > 1 && YT != DT_F32;  // y of the next 16 tokens on its way: fp32 has no registers for it
+    for (; n0 < end; n0 += kWaves * 16 * CT) {
+      u32x4_t bf[KT][CT];
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) bf[k][c] = next[k][c];
-      Cols<YT> y;
-      const int n = n0 + 8 * g;
-      auto row_of = [&](int s) { return (int64_t)token[16 * s + col] * it.N; };
-      if (col < count) y.load(it, row_of(0), n, vec);
-      if (n0 + kWaves * 64 < end) load_b(n0 + kWaves * 64);
+        for (int c = 0; c < CT; ++c) bf[k][c] = next[k][c];
+      const int n = n0 + CT * col, left = it.N - n;
+      const bool in = vec && left >= CT;
+      Cols<YT, CT> y[4];
+      auto load_y = [&](Cols<YT, CT>(&to)[4], int s) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * s + 4 * g + i;
+          to[i].load(it, (int64_t)token[t < count ? t : 0] * it.N + n, in && t < count);
+        }
+      };
+      load_y(y, 0);
+      if (n0 + kWaves * 16 * CT < end) load_b(n0 + kWaves * 16 * CT);
 #pragma unroll 1
       for (int s = 0; s < SUB; ++s) {
         if (16 * s >= count) break;
-        Cols<YT> y_next;
-        if (SUB > 1 && 16 * (s + 1) + col < count) y_next.load(it, row_of(s + 1), n, vec);
-        f32x4_t acc[4] = {};
+        Cols<YT, CT> y_next[4];
+        if (AHEAD && 16 * (s + 1) < count) load_y(y_next, s + 1);
+        f32x4_t acc[CT] = {};
         if (!none) {
           const uint16_t* h = hs + (16 * s + col) * ROW;
 #pragma unroll
@@ -394,19 +432,32 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
             if constexpr (RT == 1) {
               const u32x4_t f = *(const u32x4_t*)(h + 8 * g);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) acc[c] = mfma16<F16>(bf[k][c], f, acc[c]);
+              for (int c = 0; c < CT; ++c) acc[c] = mfma16<F16>(f, bf[k][c], acc[c]);
             } else {
               const u32x4_t hi = *(const u32x4_t*)(h + 32 * k + 8 * g), lo = *(const u32x4_t*)(h + R + 32 * k + 8 * g);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                acc[c] = mfma16<F16>(bf[k][c], lo, acc[c]);
-                acc[c] = mfma16<F16>(bf[k][c], hi, acc[c]);
+              for (int c = 0; c < CT; ++c) {
+                acc[c] = mfma16<F16>(lo, bf[k][c], acc[c]);
+                acc[c] = mfma16<F16>(hi, bf[k][c], acc[c]);
               }
             }
           }
         }
-        if (16 * s + col < count) y.store(it, row_of(s), n, vec, acc, F16 && !none ? back[16 * s + col] : 1.f);
-        if constexpr (SUB > 1) y = y_next;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * s + 4 * g + i;
+          if (t >= count || left <= 0) continue;
+          float v[CT];
+#pragma unroll
+          for (int c = 0; c < CT; ++c) v[c] = acc[c][i];
+          y[i].store(it, (int64_t)token[t] * it.N + n, in, left, v, F16 && !none ? back[t] : 1.f);
+        }
+        if constexpr (AHEAD) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = y_next[i];
+        } else if (16 * (s + 1) < count) {
+          load_y(y, s + 1);
+        }
       }
     }
   };
@@ -416,21 +467,19 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
 }
 
 struct Layout {
-  int tiles, live, splits, chunk;  // workgroups for tiles, tiles as far as known; splits of K
+  int tiles, splits, chunk;  // most tiles that the call may have; splits of K
   size_t order, counts, tile, h, bytes;
 };
 Layout layout_of(int count, int tokens, int K, int adapters, int rank) {
   Layout l;
   const int items = count < kItems ? count : kItems, tm = tokens <= kInline ? 16 : 16 * sub_of(rank_groups_of(rank));
   const int buckets = tokens < adapters + 1 ? tokens : adapters + 1;
-  l.tiles = tokens <= kInline ? tokens : std::min(tokens, tokens / tm + buckets);
+  l.tiles = std::min(tokens, tokens / tm + buckets);
   // enough workgroups for the device; a wavefront takes two steps of K or more
-  l.live = std::min(tokens, tokens / tm + buckets);
   const bool sorted = tokens > kInline;
   const int group = sorted ? 16 * shrink_sub(rank_groups_of(rank), 2) : 16;
   const long want = 512 / ((long)std::min(tokens, tokens / group + buckets) * items) + 1;
-  // expand reads h as often as it has columns / 512, so of many tokens few parts
-  const int most = std::min(sorted ? 4 : kMaxSplits, (K + 511) / 512);
+  const int most = std::min(max_splits(!sorted), (K + 511) / 512);
   int splits = (int)(want < most ? want : most);
   l.chunk = ((K + splits - 1) / splits + 63) / 64 * 64;
   l.splits = (K + l.chunk - 1) / l.chunk;
@@ -447,8 +496,9 @@ template <bool F16, int RT, int SUB, bool INLINE>
 void launch(const LoraArgs& a, int tiles, hipStream_t s) {
   int wide = 0;
   for (int i = 0; i < a.count; ++i) wide = wide > a.item[i].N ? wide : a.item[i].N;
-  shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles * (SUB / shrink_sub(RT, SUB)), a.splits, a.count), kShrinkThreads, 0, s>>>(a);
-  expand_kernel<F16, RT, SUB, INLINE><<<dim3((wide + a.columns - 1) / a.columns, tiles, a.count), kThreads, 0, s>>>(a);
+  const size_t lds = INLINE ? (size_t)(a.adapters + 1) * sizeof(int) : 0;
+  shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles * (SUB / shrink_sub(RT, SUB)), a.splits, a.count), kShrinkThreads, lds, s>>>(a);
+  expand_kernel<F16, RT, SUB, INLINE><<<dim3((wide + a.columns - 1) / a.columns, tiles, a.count), kThreads, lds, s>>>(a);
 }
 template <bool F16, int RT>
 void launch_tokens(const LoraArgs& a, int tiles, hipStream_t s) {
@@ -522,8 +572,9 @@ extern "C" int mlxr_lora_apply(int count, const mlxr_lora_item* items, int token
   // workgroup does first (its tile, h) is paid less often
   long wide = 0;
   for (int i = 0; i < count; ++i) wide += items[i].N;
-  const long steps = (wide / count + 255) / 256 * std::min(count, kItems) * l.live / kExpandGroups;
-  a.columns = 64 * kWaves * (int)std::max(1L, std::min(16L, steps));
+  const int step = 16 * columns_of(tokens <= kInline ? 1 : 2) * kWaves;
+  const long steps = (wide / count + step - 1) / step * std::min(count, kItems) * l.tiles / kExpandGroups;
+  a.columns = step * (int)std::max(1L, std::min(16L, steps));
   for (int i = 0; i < count; i += kItems) {
     a.count = count - i < kItems ? count - i : kItems;
     for (int j = 0; j < a.count; ++j) a.item[j] = items[i + j];

@@ -73,22 +73,26 @@ def lora_apply(x, ids, a, b, y, scales=None, ranks=None, outs=None, stream=None)
         xs = x.stride()
         if xs[0] % 8:
             raise QGemmError(-3, "lora: K must be a multiple of 8")
-    if outs is None:
-        outs = [_on(stream, torch.empty_like, t, memory_format=torch.contiguous_format) for t in y]
+    given = outs is not None
+    if not given:
+        make = torch.empty_like
+        outs = [make(t) for t in y] if stream is None else [_on(stream, make, t) for t in y]
     items = b""
+    codes = paged._x_codes
     for i in range(n):
         A, B, t, o = a[i], b[i], y[i], outs[i]
+        bs, ts = B.shape, t.shape
         if A.shape != shape or shape[2] != K:
             raise QGemmError(-3, f"a[{i}] must be [{adapters}, {rank}, {K}]")
-        N = B.shape[1] if B.dim() == 3 else 0
-        if B.shape != (adapters, N, rank):
+        if len(bs) != 3 or bs[0] != adapters or bs[2] != rank:
             raise QGemmError(-3, f"b[{i}] must be [{adapters}, N, {rank}]")
-        if A.dtype != xt or B.dtype != xt or A.device != d or B.device != d or not A.is_contiguous() or not B.is_contiguous():
+        N = bs[1]
+        if A.dtype is not xt or B.dtype is not xt or A.device != d or B.device != d or not A.is_contiguous() or not B.is_contiguous():
             raise QGemmError(-1, f"a[{i}] and b[{i}] must be contiguous, of x's dtype and device")
-        if t.shape != (tokens, N) or o.shape != t.shape or t.dtype != o.dtype or t.device != d or o.device != d or \
-                not t.is_contiguous() or not o.is_contiguous():
+        if len(ts) != 2 or ts[0] != tokens or ts[1] != N or t.device != d or not t.is_contiguous() or \
+                given and (o.shape != ts or o.dtype is not t.dtype or o.device != d or not o.is_contiguous()):
             raise QGemmError(-1, f"y[{i}] and its output must be contiguous [{tokens}, {N}] tensors of one dtype on {d}")
-        items += _pack_item(A.data_ptr(), B.data_ptr(), t.data_ptr(), o.data_ptr(), N, _code(paged._x_codes, t.dtype, "y"))
+        items += _pack_item(A.data_ptr(), B.data_ptr(), t.data_ptr(), o.data_ptr(), N, _code(codes, t.dtype, "y"))
     nb = ctypes.c_size_t()
     qgemm._check(lib.mlxr_lora_workspace_size(n, tokens, K, adapters, rank, ctypes.byref(nb)))
     nb = nb.value

@@ -30,8 +30,9 @@ typedef struct mlxr_lora_item {
   int N, y_dtype;    /* of y and out: MLXR_F32 / MLXR_F16 / MLXR_BF16 */
 } mlxr_lora_item;
 
-/* Workspace bytes of mlxr_lora_apply. */
-int mlxr_lora_workspace_size(int count, int tokens, int K, int adapters, int rank, size_t* bytes);
+/* Workspace bytes of mlxr_lora_apply (0: none is needed, workspace_dev may be NULL).  Only the items' N are read. */
+int mlxr_lora_workspace_size(int count, const mlxr_lora_item* items, int tokens, int K, int adapters, int rank,
+                             size_t* bytes);
 
 /* x_dev [tokens, K] of x_dtype (MLXR_F16 / MLXR_BF16), row stride x_stride elements; K and x_stride
  * multiples of 8, rank a multiple of 8 up to MLXR_LORA_MAX_RANK; x, A and B at multiples of 16 bytes.

@@ -24,10 +24,11 @@ constexpr int kItems = 4;      // projections of one launch
 constexpr int kThreads = 256;  // of expand
 constexpr int kWaves = kThreads / 64;
 constexpr int kShrinkThreads = 512;
+constexpr int kFusedThreads = 512;
 constexpr int kInline = kThreads;  // tokens
 // Groups of 16 tokens in a tile of the sorted tokens, for which expand reads its columns of B once; and those
 // that a workgroup of shrink takes of it.
-constexpr int sub_of(int rank_groups) { return rank_groups > 4 ? 2 : 4; }
+constexpr int kSub = 4;
 constexpr int shrink_sub(int rank_groups, int sub) { return sub == 1 || rank_groups > 4 ? 1 : 2; }
 constexpr int rank_groups_of(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 // Most splits of K.  Expand reads h for each of its workgroups, so of many tokens few parts (2048 tokens, rank
@@ -78,7 +79,7 @@ __device__ __forceinline__ int wave_add(int* counter, int b) {
 // Tokens sorted by adapter, and the tiles; the last bucket holds the tokens without one.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   extern __shared__ int sh[];
-  const int TM = 16 * sub_of(rank_groups_of(a.rank)), nb = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int TM = 16 * kSub, nb = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int *count = sh, *next = sh + nb;
   __shared__ int part[2 * kPlanThreads / 64];
   for (int b = tid; b < nb; b += kPlanThreads) count[b] = 0;
@@ -304,39 +305,68 @@ struct Cols {
   }
 };
 
-// Columns of a wavefront's step: 64 for few tokens (more workgroups), 128 for many: 256 bytes of a row in one
-// store of 16-bit outputs (2048 tokens, two projections of 14336: 62 -> 55 us).
-// In units of 16.
-constexpr int columns_of(int sub) { return sub == 1 ? 4 : 8; }
+// Columns of a wavefront's step, in units of 16: 64 for few tokens (more workgroups), 128 for many: 256 bytes of a
+// row in one store of 16-bit outputs (2048 tokens, two projections of 14336, rank 32: 62 -> 55 us); not where B's
+// operands then leave few wavefronts on a SIMD (rank 64: 128 us, 111).
+constexpr int columns_of(int sub, int rank_groups) { return sub == 1 || rank_groups > 2 ? 4 : 8; }
 
-// One tile and `columns` columns of an item, in steps of 16 CT for each wavefront.  Tokens are the rows of the
-// products; column n of the c-th is column CT n + c, so a lane ends with CT neighbouring columns of four
-// tokens, and 16 lanes with a stretch of a row.  h enters as the sum of two 16-bit parts: rounded to one it would
-// lose what the fp32 sums kept.
-template <bool F16, int RT, int SUB, bool INLINE>
-__global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
-  constexpr int R = 16 * RT, KT = RT == 1 ? 1 : RT / 2, CT = columns_of(SUB);
-  constexpr int ROW = 2 * R + 8;  // of LDS: R high parts, R low parts; padded against bank conflicts
-  __shared__ int token[16 * SUB];
-  __shared__ float back[16 * SUB];
-  __shared__ __attribute__((aligned(16))) uint16_t hs[16 * SUB * ROW];
-  const mlxr_lora_item& it = a.item[blockIdx.z];
-  const int begin = blockIdx.x * a.columns;
-  if (begin >= it.N) return;
-  int adapter = 0;
-  const int count = tile_tokens<INLINE, kWaves>(a, blockIdx.y, &adapter, token);
-  if (count == 0) return;
-  const bool none = adapter == a.adapters;
-  if (none && it.out_dev == it.y_dev) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int rank = none ? 0 : rank_of(a, adapter);
-  // operands of B for a step, on their way while h is summed up or the columns before are computed; RT 1
-  // multiplies the high and the low parts in one step, ranks 8 (g & 1) ..
-  const uint16_t* B = (const uint16_t*)it.b_dev + (int64_t)(none ? 0 : adapter) * it.N * a.rank;
-  const int end = min(begin + a.columns, it.N);
-  int n0 = begin + wave * 16 * CT;
-  u32x4_t next[KT][CT];
-  auto load_b = [&](int n0) {
+// 8 ranks at .. of token t of a tile into LDS as high and low 16-bit parts: rounded to one part h would lose what the
+// fp32 sums kept.  In f16, whose range h may leave, relative to a power of two that brings the token's largest to
+// [1/2, 1), the reciprocal in back[t]; the 2 RT threads of a token are neighbours.
+template <bool F16, int RT>
+__device__ __forceinline__ void split_h(f32x4_t (&v)[2], float scale, int t, int at, uint16_t* row, float* back) {
+  constexpr int R = 16 * RT;
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    v[e] *= scale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[e][i]));
+  }
+  if constexpr (F16) {
+#pragma unroll
+    for (int d = 1; d < 2 * RT; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+    if (at == 0) back[t] = __builtin_amdgcn_ldexpf(1.f, e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = __builtin_amdgcn_ldexpf(v[i >> 2][i & 3], -e);
+  }
+  u32x4_t hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float v0 = v[e >> 1][2 * (e & 1)], v1 = v[e >> 1][2 * (e & 1) + 1];
+    hi[e] = pack2<F16>(v0, v1);
+    const float d0 = v0 - unpack<F16>(hi[e], 0), d1 = v1 - unpack<F16>(hi[e], 1);
+    lo[e] = pack2<F16>(d0 == d0 ? d0 : 0.f, d1 == d1 ? d1 : 0.f);  // an infinite h stays infinite
+  }
+  *(u32x4_t*)(row + at) = hi;
+  *(u32x4_t*)(row + R + at) = lo;
+}
+// Elements of such a row: R high parts, R low parts; padded against bank conflicts.
+constexpr int h_row(int rt) { return 32 * rt + 8; }
+
+// The second product of a tile: columns [n0, end) of an item in steps of 16 CT for each of WAVES wavefronts.
+// Tokens are the rows of the products; column n of the c-th is column CT n + c of the step, so a lane ends
+// with CT neighbouring columns of four tokens, and 16 lanes with a stretch of a row.
+template <bool F16, int RT, int SUB, int WAVES>
+struct Expand {
+  static constexpr int R = 16 * RT, KT = RT == 1 ? 1 : RT / 2, CT = columns_of(SUB, RT), STEP = WAVES * 16 * CT;
+  const LoraArgs& a;
+  const mlxr_lora_item& it;
+  const uint16_t* B;
+  int rank, n0, end, col, g;
+  u32x4_t next[KT][CT];  // operands of B for a step, on their way while h or the columns before are computed
+
+  __device__ __forceinline__ Expand(const LoraArgs& a_, const mlxr_lora_item& it_, int adapter, int rank_, int begin)
+      : a(a_), it(it_), B((const uint16_t*)it_.b_dev + (int64_t)adapter * it_.N * a_.rank), rank(rank_) {
+    const int lane = threadIdx.x & 63;
+    col = lane & 15, g = lane >> 4;
+    n0 = begin + (threadIdx.x >> 6) * 16 * CT;
+    end = min(begin + a.columns, it.N);
+    load_b(n0);
+  }
+  // RT 1 multiplies the high and the low parts in one product, ranks 8 (g & 1) ..
+  __device__ __forceinline__ void load_b(int n0) {
 #pragma unroll
     for (int k = 0; k < KT; ++k)
 #pragma unroll
@@ -347,61 +377,13 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) next[k][c][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
       }
-  };
-  load_b(n0);
-  if (!none) {
-    const float scale = a.scales ? a.scales[adapter] : 1.f;
-    // 8 ranks of a token for each thread, a token's threads side by side
-    for (int u = threadIdx.x; u < 16 * SUB * 2 * RT; u += kThreads) {
-      const int t = u / (2 * RT), at = 8 * (u % (2 * RT));
-      f32x4_t v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-      if (t < count && at < rank) {
-        const float* p = a.h + ((int64_t)blockIdx.z * a.splits * a.tokens + token[t]) * a.rank + at;
-        const int64_t step = (int64_t)a.tokens * a.rank;
-        constexpr int kMost = max_splits(INLINE);
-        f32x4_t in[kMost][2];
-#pragma unroll
-        for (int s = 0; s < kMost; ++s)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) in[s][e] = s < a.splits ? *(const f32x4_t*)(p + s * step + 4 * e) : f32x4_t{0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < kMost; ++s)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) v[e] += in[s][e];
-      }
-      float top = 0.f;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        v[e] *= scale;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[e][i]));
-      }
-      if constexpr (F16) {  // h may lie outside f16: a power of two brings the token's largest to [1/2, 1)
-#pragma unroll
-        for (int d = 1; d < 2 * RT; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-        const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-        if (at == 0) back[t] = __builtin_amdgcn_ldexpf(1.f, e);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = __builtin_amdgcn_ldexpf(v[i >> 2][i & 3], -e);
-      }
-      u32x4_t hi, lo;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v0 = v[e >> 1][2 * (e & 1)], v1 = v[e >> 1][2 * (e & 1) + 1];
-        hi[e] = pack2<F16>(v0, v1);
-        const float d0 = v0 - unpack<F16>(hi[e], 0), d1 = v1 - unpack<F16>(hi[e], 1);
-        lo[e] = pack2<F16>(d0 == d0 ? d0 : 0.f, d1 == d1 ? d1 : 0.f);  // an infinite h stays infinite
-      }
-      *(u32x4_t*)(hs + t * ROW + at) = hi;
-      *(u32x4_t*)(hs + t * ROW + R + at) = lo;
-    }
-    __syncthreads();
   }
-  const bool vec = (it.N * (it.y_dtype == DT_F32 ? 4 : 2)) % 16 == 0 && (((uintptr_t)it.y_dev | (uintptr_t)it.out_dev) & 15) == 0;
-  auto columns = [&](auto yt) {
-    constexpr int YT = decltype(yt)::value;
+  // hs: the tile's rows of h; none: the tokens have no adapter
+  template <int YT>
+  __device__ __forceinline__ void columns(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
     constexpr bool AHEAD = SUB > 1 && YT != DT_F32;  // y of the next 16 tokens on its way: fp32 has no registers for it
-    for (; n0 < end; n0 += kWaves * 16 * CT) {
+    const bool vec = it.N * Cols<YT, CT>::S % 16 == 0 && (((uintptr_t)it.y_dev | (uintptr_t)it.out_dev) & 15) == 0;
+    for (; n0 < end; n0 += STEP) {
       u32x4_t bf[KT][CT];
 #pragma unroll
       for (int k = 0; k < KT; ++k)
@@ -418,7 +400,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
         }
       };
       load_y(y, 0);
-      if (n0 + kWaves * 16 * CT < end) load_b(n0 + kWaves * 16 * CT);
+      if (n0 + STEP < end) load_b(n0 + STEP);
 #pragma unroll 1
       for (int s = 0; s < SUB; ++s) {
         if (16 * s >= count) break;
@@ -426,7 +408,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
         if (AHEAD && 16 * (s + 1) < count) load_y(y_next, s + 1);
         f32x4_t acc[CT] = {};
         if (!none) {
-          const uint16_t* h = hs + (16 * s + col) * ROW;
+          const uint16_t* h = hs + (16 * s + col) * h_row(RT);
 #pragma unroll
           for (int k = 0; k < KT; ++k) {
             if constexpr (RT == 1) {
@@ -460,29 +442,154 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
         }
       }
     }
-  };
-  if (it.y_dtype == DT_BF16) columns(std::integral_constant<int, DT_BF16>());
-  else if (it.y_dtype == DT_F16) columns(std::integral_constant<int, DT_F16>());
-  else columns(std::integral_constant<int, DT_F32>());
+  }
+  __device__ __forceinline__ void run(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
+    if (it.y_dtype == DT_BF16) columns<DT_BF16>(token, count, none, hs, back);
+    else if (it.y_dtype == DT_F16) columns<DT_F16>(token, count, none, hs, back);
+    else columns<DT_F32>(token, count, none, hs, back);
+  }
+};
+
+// One tile and a.columns columns of an item, h from the workspace.
+template <bool F16, int RT, int SUB, bool INLINE>
+__global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
+  constexpr int kMost = max_splits(INLINE);
+  __shared__ int token[16 * SUB];
+  __shared__ float back[16 * SUB];
+  __shared__ __attribute__((aligned(16))) uint16_t hs[16 * SUB * h_row(RT)];
+  const mlxr_lora_item& it = a.item[blockIdx.z];
+  const int begin = blockIdx.x * a.columns;
+  if (begin >= it.N) return;
+  int adapter = 0;
+  const int count = tile_tokens<INLINE, kWaves>(a, blockIdx.y, &adapter, token);
+  if (count == 0) return;
+  const bool none = adapter == a.adapters;
+  if (none && it.out_dev == it.y_dev) return;
+  const int rank = none ? 0 : rank_of(a, adapter);
+  Expand<F16, RT, SUB, kWaves> e(a, it, none ? 0 : adapter, rank, begin);
+  if (!none) {
+    const float scale = a.scales ? a.scales[adapter] : 1.f;
+    for (int u = threadIdx.x; u < 16 * SUB * 2 * RT; u += kThreads) {
+      const int t = u / (2 * RT), at = 8 * (u % (2 * RT));
+      f32x4_t v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      if (t < count && at < rank) {
+        const float* p = a.h + ((int64_t)blockIdx.z * a.splits * a.tokens + token[t]) * a.rank + at;
+        const int64_t step = (int64_t)a.tokens * a.rank;
+        f32x4_t in[kMost][2];
+#pragma unroll
+        for (int s = 0; s < kMost; ++s)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) in[s][k] = s < a.splits ? *(const f32x4_t*)(p + s * step + 4 * k) : f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < kMost; ++s)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) v[k] += in[s][k];
+      }
+      split_h<F16, RT>(v, scale, t, at, hs + t * h_row(RT), back);
+    }
+    __syncthreads();
+  }
+  e.run(token, count, none, hs, back);
+}
+
+// Both products of one tile and a.columns columns of an item: every workgroup of a tile computes its h for itself.
+// For few tokens and small A, where that costs less than a launch, and no workspace.
+template <bool F16, int RT>
+__global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
+  constexpr int WAVES = kFusedThreads / 64, U = 4;  // steps of 64 k on their way at once
+  __shared__ int token[16];
+  __shared__ float back[16];
+  __shared__ __attribute__((aligned(16))) uint16_t hs[16 * h_row(RT)];
+  __shared__ f32x4_t sh[WAVES][RT][64];
+  const mlxr_lora_item& it = a.item[blockIdx.z];
+  const int begin = blockIdx.x * a.columns;
+  if (begin >= it.N) return;
+  int adapter = 0;
+  const int count = tile_tokens<true, WAVES>(a, blockIdx.y, &adapter, token);
+  if (count == 0) return;
+  const bool none = adapter == a.adapters;
+  if (none && it.out_dev == it.y_dev) return;
+  const int rank = none ? 0 : rank_of(a, adapter);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  Expand<F16, RT, 1, WAVES> e(a, it, none ? 0 : adapter, rank, begin);
+  if (!none) {
+    const uint16_t* A = (const uint16_t*)it.a_dev + (int64_t)adapter * a.rank * a.K + (int64_t)col * a.K;
+    const uint16_t* x = a.x + (int64_t)token[col < count ? col : 0] * a.x_stride;
+    f32x4_t acc[RT] = {};
+    for (int k0 = wave * 64; k0 < a.K; k0 += WAVES * U * 64) {
+      u32x4_t xf[U][2], af[U][RT][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int kk = k0 + u * WAVES * 64 + 16 * g + 8 * h;
+          const bool in = kk < a.K;
+          xf[u][h] = in ? *(const u32x4_t*)(x + kk) : u32x4_t{0, 0, 0, 0};
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            af[u][r][h] = in && 16 * r + col < rank ? *(const u32x4_t*)(A + (int64_t)(16 * r) * a.K + kk) : u32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) acc[r] = mfma16<F16>(af[u][r][h], xf[u][h], acc[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) sh[wave][r][lane] = acc[r];
+    __syncthreads();
+    if (threadIdx.x < 32 * RT) {
+      const int t = threadIdx.x / (2 * RT), part = threadIdx.x % (2 * RT);
+      f32x4_t v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v[k] += sh[w][part >> 1][(2 * (part & 1) + k) * 16 + t];
+      split_h<F16, RT>(v, a.scales ? a.scales[adapter] : 1.f, t, 8 * part, hs + t * h_row(RT), back);
+    }
+    __syncthreads();
+  }
+  e.run(token, count, none, hs, back);
 }
 
 struct Layout {
-  int tiles, splits, chunk;  // most tiles that the call may have; splits of K
+  bool fused;
+  int tiles, splits, chunk, columns;  // most tiles that the call may have; splits of K; columns of a workgroup
   size_t order, counts, tile, h, bytes;
 };
-Layout layout_of(int count, int tokens, int K, int adapters, int rank) {
-  Layout l;
-  const int items = count < kItems ? count : kItems, tm = tokens <= kInline ? 16 : 16 * sub_of(rank_groups_of(rank));
-  const int buckets = tokens < adapters + 1 ? tokens : adapters + 1;
+Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int adapters, int rank) {
+  Layout l{};
+  const int items = count < kItems ? count : kItems, tm = tokens <= kInline ? 16 : 16 * kSub;
+  const int buckets = std::min(tokens, adapters + 1), groups = rank_groups_of(rank);
   l.tiles = std::min(tokens, tokens / tm + buckets);
+  long wide = 0, fused_groups = 0;
+  for (int i = 0; i < count; ++i) {
+    wide += item[i].N;
+    fused_groups += ((long)item[i].N + kFusedThreads - 1) / kFusedThreads;  // 64 columns a wavefront
+  }
+  // One launch where each workgroup's reading of A (at most 128 KiB) is short beside a launch and all of it together
+  // at most 16 MiB.  Measured, us, one launch and two (the host needs 4 more for two): rank 16, K 2048, three
+  // projections of 2560 together, 1 token 6.5 and 8.1, 64 tokens 9.3 and 11.4; rank 16, K 4096, 6144, 4 tokens
+  // 10.3 and 9.8, 16 tokens (24 MiB) 16.9 and 12.4; rank 16, K 8192, 10240, 1 token 12.8 and 8.7.
+  l.fused = tokens <= kInline && groups <= 2 && (long)rank * K <= 1 << 16 && fused_groups * l.tiles * rank * K <= 1 << 23;
+  if (l.fused) {
+    l.columns = kFusedThreads;
+    return l;
+  }
   // enough workgroups for the device; a wavefront takes two steps of K or more
   const bool sorted = tokens > kInline;
-  const int group = sorted ? 16 * shrink_sub(rank_groups_of(rank), 2) : 16;
+  const int group = sorted ? 16 * shrink_sub(groups, kSub) : 16;
   const long want = 512 / ((long)std::min(tokens, tokens / group + buckets) * items) + 1;
   const int most = std::min(max_splits(!sorted), (K + 511) / 512);
   int splits = (int)(want < most ? want : most);
   l.chunk = ((K + splits - 1) / splits + 63) / 64 * 64;
   l.splits = (K + l.chunk - 1) / l.chunk;
+  // columns of a workgroup of expand: several steps where that leaves enough workgroups, so that what a
+  // workgroup does first (its tile, h) is paid less often
+  const int step = 16 * columns_of(sorted ? kSub : 1, groups) * kWaves;
+  const long steps = (wide / count + step - 1) / step * items * l.tiles / kExpandGroups;
+  l.columns = step * (int)std::max(1L, std::min(16L, steps));
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   l.order = 0;
   l.counts = up((size_t)tokens * 4);
@@ -492,29 +599,40 @@ Layout layout_of(int count, int tokens, int K, int adapters, int rank) {
   return l;
 }
 
+int widest(const LoraArgs& a) {
+  int n = 0;
+  for (int i = 0; i < a.count; ++i) n = std::max(n, a.item[i].N);
+  return n;
+}
 template <bool F16, int RT, int SUB, bool INLINE>
 void launch(const LoraArgs& a, int tiles, hipStream_t s) {
-  int wide = 0;
-  for (int i = 0; i < a.count; ++i) wide = wide > a.item[i].N ? wide : a.item[i].N;
+  const int wide = widest(a);
   const size_t lds = INLINE ? (size_t)(a.adapters + 1) * sizeof(int) : 0;
   shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles * (SUB / shrink_sub(RT, SUB)), a.splits, a.count), kShrinkThreads, lds, s>>>(a);
   expand_kernel<F16, RT, SUB, INLINE><<<dim3((wide + a.columns - 1) / a.columns, tiles, a.count), kThreads, lds, s>>>(a);
 }
 template <bool F16, int RT>
-void launch_tokens(const LoraArgs& a, int tiles, hipStream_t s) {
+void launch_tokens(const LoraArgs& a, const Layout& l, hipStream_t s) {
+  const int tiles = l.tiles;
+  if constexpr (RT <= 2)
+    if (l.fused) {
+      fused_kernel<F16, RT><<<dim3((widest(a) + a.columns - 1) / a.columns, tiles, a.count), kFusedThreads,
+                              (size_t)(a.adapters + 1) * sizeof(int), s>>>(a);
+      return;
+    }
   if (a.tokens <= kInline) launch<F16, RT, 1, true>(a, tiles, s);
-  else launch<F16, RT, sub_of(RT), false>(a, tiles, s);
+  else launch<F16, RT, kSub, false>(a, tiles, s);
 }
 template <bool F16>
-void launch_rank(const LoraArgs& a, int tiles, hipStream_t s) {
+void launch_rank(const LoraArgs& a, const Layout& l, hipStream_t s) {
   const int n = rank_groups_of(a.rank);
-  if (n == 1) launch_tokens<F16, 1>(a, tiles, s);
-  else if (n == 2) launch_tokens<F16, 2>(a, tiles, s);
-  else if (n == 4) launch_tokens<F16, 4>(a, tiles, s);
-  else launch_tokens<F16, 8>(a, tiles, s);
+  if (n == 1) launch_tokens<F16, 1>(a, l, s);
+  else if (n == 2) launch_tokens<F16, 2>(a, l, s);
+  else if (n == 4) launch_tokens<F16, 4>(a, l, s);
+  else launch_tokens<F16, 8>(a, l, s);
 }
 
-int check_lora(int count, int tokens, int K, int adapters, int rank) {
+int check_lora(int count, const mlxr_lora_item* items, int tokens, int K, int adapters, int rank) {
   if (count < 0 || tokens < 0 || K <= 0 || adapters <= 0 || rank <= 0) return set_error(MLXR_E_INVALID, "lora: bad sizes");
   if (adapters > MLXR_LORA_MAX_ADAPTERS)
     return set_error(MLXR_E_SHAPE, "lora: at most %d adapters", MLXR_LORA_MAX_ADAPTERS);
@@ -522,6 +640,9 @@ int check_lora(int count, int tokens, int K, int adapters, int rank) {
     return set_error(MLXR_E_SHAPE, "lora: rank must be a multiple of 8 and at most %d", MLXR_LORA_MAX_RANK);
   if (K % 8) return set_error(MLXR_E_SHAPE, "lora: K must be a multiple of 8");
   if (tokens > MLXR_LORA_MAX_TOKENS) return set_error(MLXR_E_SHAPE, "lora: at most %d tokens", MLXR_LORA_MAX_TOKENS);
+  if (count && !items) return set_error(MLXR_E_INVALID, "null items");
+  for (int i = 0; i < count; ++i)
+    if (items[i].N <= 0) return set_error(MLXR_E_INVALID, "lora: N must be positive");
   return MLXR_OK;
 }
 
@@ -531,10 +652,11 @@ int check_lora(int count, int tokens, int K, int adapters, int rank) {
 
 using namespace mlxr;
 
-extern "C" int mlxr_lora_workspace_size(int count, int tokens, int K, int adapters, int rank, size_t* bytes) {
+extern "C" int mlxr_lora_workspace_size(int count, const mlxr_lora_item* items, int tokens, int K, int adapters, int rank,
+                                        size_t* bytes) {
   if (!bytes) return set_error(MLXR_E_INVALID, "null bytes");
-  if (const int rc = check_lora(count, tokens, K, adapters, rank)) return rc;
-  *bytes = count && tokens ? layout_of(count, tokens, K, adapters, rank).bytes : 0;
+  if (const int rc = check_lora(count, items, tokens, K, adapters, rank)) return rc;
+  *bytes = count && tokens ? layout_of(count, items, tokens, K, adapters, rank).bytes : 0;
   return MLXR_OK;
 }
 
@@ -542,45 +664,38 @@ extern "C" int mlxr_lora_apply(int count, const mlxr_lora_item* items, int token
                                const void* x_dev, int x_dtype, int64_t x_stride, const int32_t* ids_dev,
                                const float* scales_dev, const int32_t* ranks_dev, void* workspace_dev,
                                size_t workspace_bytes, void* stream) {
-  if (const int rc = check_lora(count, tokens, K, adapters, rank)) return rc;
+  if (const int rc = check_lora(count, items, tokens, K, adapters, rank)) return rc;
   if (x_dtype != MLXR_F16 && x_dtype != MLXR_BF16) return set_error(MLXR_E_INVALID, "invalid activation dtype %d", x_dtype);
   if (count == 0 || tokens == 0) return MLXR_OK;
-  if (!items || !x_dev || !ids_dev || !workspace_dev) return set_error(MLXR_E_INVALID, "null buffer");
+  if (!x_dev || !ids_dev) return set_error(MLXR_E_INVALID, "null buffer");
   if (x_stride % 8 || ((uintptr_t)x_dev & 15) || ((uintptr_t)workspace_dev & 15))
     return set_error(MLXR_E_SHAPE, "lora: rows of x and the workspace must start at multiples of 16 bytes");
   for (int i = 0; i < count; ++i) {
     const mlxr_lora_item& t = items[i];
     if (!t.a_dev || !t.b_dev || !t.y_dev || !t.out_dev) return set_error(MLXR_E_INVALID, "null buffer");
-    if (t.N <= 0) return set_error(MLXR_E_INVALID, "lora: N must be positive");
     if (t.y_dtype != MLXR_F32 && t.y_dtype != MLXR_F16 && t.y_dtype != MLXR_BF16)
       return set_error(MLXR_E_INVALID, "invalid output dtype %d", t.y_dtype);
     if (((uintptr_t)t.a_dev | (uintptr_t)t.b_dev) & 15)
       return set_error(MLXR_E_SHAPE, "lora: A and B must start at multiples of 16 bytes");
   }
-  const Layout l = layout_of(count, tokens, K, adapters, rank);
-  if (workspace_bytes < l.bytes)
+  const Layout l = layout_of(count, items, tokens, K, adapters, rank);
+  if (workspace_bytes < l.bytes || (l.bytes && !workspace_dev))
     return set_error(MLXR_E_INVALID, "lora: the workspace is smaller than mlxr_lora_workspace_size");
   const hipStream_t s = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)workspace_dev;
-  LoraArgs a;
+  LoraArgs a{};
   a.x = (const uint16_t*)x_dev, a.x_stride = x_stride;
   a.ids = ids_dev, a.ranks = ranks_dev, a.scales = scales_dev;
   a.order = (int32_t*)(ws + l.order), a.counts = (int32_t*)(ws + l.counts), a.tiles = (Tile*)(ws + l.tile);
   a.h = (float*)(ws + l.h);
   a.tokens = tokens, a.K = K, a.adapters = adapters, a.rank = rank, a.splits = l.splits, a.chunk = l.chunk;
-  // columns of a workgroup of expand: several steps where that leaves enough workgroups, so that what a
-  // workgroup does first (its tile, h) is paid less often
-  long wide = 0;
-  for (int i = 0; i < count; ++i) wide += items[i].N;
-  const int step = 16 * columns_of(tokens <= kInline ? 1 : 2) * kWaves;
-  const long steps = (wide / count + step - 1) / step * std::min(count, kItems) * l.tiles / kExpandGroups;
-  a.columns = step * (int)std::max(1L, std::min(16L, steps));
+  a.columns = l.columns;
   for (int i = 0; i < count; i += kItems) {
     a.count = count - i < kItems ? count - i : kItems;
     for (int j = 0; j < a.count; ++j) a.item[j] = items[i + j];
     if (i == 0 && tokens > kInline) plan_kernel<<<1, kPlanThreads, (size_t)(adapters + 1) * 8, s>>>(a);
-    if (x_dtype == MLXR_F16) launch_rank<true>(a, l.tiles, s);
-    else launch_rank<false>(a, l.tiles, s);
+    if (x_dtype == MLXR_F16) launch_rank<true>(a, l, s);
+    else launch_rank<false>(a, l, s);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "lora launch: %s", hipGetErrorString(e));

@@ -23,7 +23,7 @@ class Item(ctypes.Structure):
 _pack_item = struct.Struct("@4P2i").pack  # the same as bytes
 
 _SIGS = {
-    "mlxr_lora_workspace_size": (_I, [_I] * 5 + [ctypes.POINTER(ctypes.c_size_t)]),
+    "mlxr_lora_workspace_size": (_I, [_I, _P] + [_I] * 4 + [ctypes.POINTER(ctypes.c_size_t)]),
     "mlxr_lora_apply": (_I, [_I, _P] + [_I] * 4 + [_P, _I, ctypes.c_int64, _P, _P, _P, _P, ctypes.c_size_t, _P]),
 }
 _bound = None
@@ -94,10 +94,10 @@ def lora_apply(x, ids, a, b, y, scales=None, ranks=None, outs=None, stream=None)
             raise QGemmError(-1, f"y[{i}] and its output must be contiguous [{tokens}, {N}] tensors of one dtype on {d}")
         items += _pack_item(A.data_ptr(), B.data_ptr(), t.data_ptr(), o.data_ptr(), N, _code(codes, t.dtype, "y"))
     nb = ctypes.c_size_t()
-    qgemm._check(lib.mlxr_lora_workspace_size(n, tokens, K, adapters, rank, ctypes.byref(nb)))
+    qgemm._check(lib.mlxr_lora_workspace_size(n, items, tokens, K, adapters, rank, ctypes.byref(nb)))
     nb = nb.value
-    ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=d)
-    qgemm._check(lib.mlxr_lora_apply(n, items, tokens, K, adapters, rank, x.data_ptr(), dt, xs[0], pi, ps, pr, ws.data_ptr(), nb,
+    ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=d) if nb else None
+    qgemm._check(lib.mlxr_lora_apply(n, items, tokens, K, adapters, rank, x.data_ptr(), dt, xs[0], pi, ps, pr, ws.data_ptr() if nb else None, nb,
                                      _stream(stream, d.index)))
     return outs
 

@@ -23,15 +23,22 @@ def test_refusals():
     assert call(adapters=4097) == -3 and call(rank=12) == -3 and call(rank=136) == -3 and call(K=252) == -3
     assert call(tokens=(1 << 24) + 1) == -3
     assert call(dt=mx.F32) == -1 and call(dt=3) == -1
-    for name in ("x", "ids", "ws", "a", "b", "y", "out"):
-        assert call(**{name: 0 if name in ("x", "ids", "ws") else None}) == -1, name
+    for name in ("x", "ids", "a", "b", "y", "out"):
+        assert call(**{name: 0 if name in ("x", "ids") else None}) == -1, name
+    assert call(tokens=300, ws=0) == -1
     assert call(xs=252) == -3 and call(x=72) == -3 and call(ws=72) == -3 and call(a=72) == -3 and call(b=72) == -3
     assert call(N=0) == -1 and call(ydt=3) == -1
-    assert call(nb=16) == -1 and "workspace" in L.mlxr_qgemm_last_error().decode()
+    assert call(tokens=300, nb=16) == -1 and "workspace" in L.mlxr_qgemm_last_error().decode()
     n = ctypes.c_size_t()
-    assert L.mlxr_lora_workspace_size(1, 4, 256, 3, 16, None) == -1
-    assert L.mlxr_lora_workspace_size(1, 4, 256, 3, 17, ctypes.byref(n)) == -3
-    assert L.mlxr_lora_workspace_size(0, 4, 256, 3, 16, ctypes.byref(n)) == 0 and n.value == 0
+    item = (lora.Item * 1)(lora.Item(None, None, None, None, 32, mx.BF16))
+    bad = (lora.Item * 1)(lora.Item(None, None, None, None, 0, mx.BF16))
+
+    def size(count=1, items=item, tokens=4, rank=16, out=ctypes.byref(n)):
+        return L.mlxr_lora_workspace_size(count, items, tokens, 256, 3, rank, out)
+    assert size(out=None) == -1 and size(rank=17) == -3 and size(items=None) == -1 and size(items=bad) == -1
+    assert size(count=0) == 0 and n.value == 0
+    assert size() == 0 and n.value == 0  # one launch
+    assert size(tokens=300) == 0 and n.value > 0
 
 
 def test_wrapper_refusals():
@@ -119,6 +126,7 @@ def _run(cuda, tokens, K, adapters, rank, widths, dtype="bf16", ydt=None, seed=0
     (1, 8, 1, 8, [1]), (1, 4096, 3, 16, [64]), (2, 264, 2, 8, [65, 3]), (8, 2048, 16, 16, [2048, 256, 256]),
     (15, 520, 4, 24, [100]), (16, 1024, 1, 32, [257]), (17, 1024, 2, 40, [130, 64, 7, 12, 33]), (61, 2048, 24, 64, [500, 500]),
     (100, 1000, 5, 128, [300]), (333, 256, 300, 8, [72]), (700, 512, 6, 16, [640]), (2048, 256, 3, 32, [96, 1024]),
+    (200, 4096, 20, 16, [2048]), (3, 8192, 4, 32, [1000, 24]), (64, 4096, 3, 8, [14336]), (257, 2048, 2, 120, [520]),
 ])
 def test_lora(cuda, dtype, tokens, K, adapters, rank, widths):
     _run(cuda, tokens, K, adapters, rank, widths, dtype, seed=tokens)

@@ -49,7 +49,7 @@ struct AttnArgs {
   int rows, heads, kv_heads, group, groups;  // groups: of 16 heads, of a kv head
   int dim, page, pages, width, window, out_dtype;
   Divisor by_page;
-  int part_rows, workers;
+  int part_rows, workers, near;
   float scale;  // times log2(e)
 };
 
@@ -479,13 +479,13 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_rows_kern
   constexpr int WAVES = kWaves;
   using T = Attn<F16, F8, DT, DIM, P8>;
   __shared__ float sh[WAVES / 2][T::PARK * 64];
-  // heads above 16 of a kv head: their workgroups read the same keys and values, and follow each other on one of
-  // the eight XCDs (workgroup i runs on XCD i % 8)
+  // Workgroup i runs on XCD i % 8, each with its own L2.  Those that read the same lines follow each other on
+  // one: the groups of 16 heads of a kv head, and a.near kv heads whose rows share lines.
   int unit = blockIdx.x, grp = 0;
-  if (a.groups > 1) {
-    const int n = 8 * a.groups, at = unit % n;
-    grp = at >> 3;
-    unit = unit / n * 8 + (at & 7);
+  if (const int n = a.near * a.groups; n > 1) {
+    const int set = unit / (8 * n), at = unit - set * 8 * n, k = at >> 3;
+    grp = k % a.groups;
+    unit = (set * 8 + (at & 7)) * a.near + k / a.groups;
     if (unit >= a.rows * a.kv_heads) return;
   }
   const int r = unit / a.kv_heads, kvh = unit - r * a.kv_heads;

@@ -205,7 +205,12 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   void* args[] = {&a};
   hipError_t e = hipSuccess;
   if (p.one) {
-    const int units = rows * a.kv_heads, grid = a.groups > 1 ? (units + 7) / 8 * 8 * a.groups : units;
+    // neighbouring kv heads share lines where a token's heads lie side by side and are no whole lines
+    a.near = 1;
+    if (a.k_head % 128 || a.v_head % 128)
+      while (a.near < 8 && a.kv_heads % (2 * a.near) == 0) a.near *= 2;
+    const int n = a.near * a.groups, units = rows * a.kv_heads;
+    const int grid = n > 1 ? (units / a.near + 7) / 8 * 8 * n : units;
     e = hipLaunchKernel(k.rows_fn, dim3(grid), dim3(64 * kWaves), args, 0, st);
   } else {
     const int grid = grid_of(k, &e);

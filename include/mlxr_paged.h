@@ -80,7 +80,8 @@ int mlxr_paged_append(const mlxr_paged_cache* cache, int tokens, const void* k_d
  *   table_dev      [rows, table_width] int32, row stride table_stride
  *   lens_dev       [rows] int32; a row of length 0 (or less) gives zeros.  Lengths past
  *                  table_width * page_size are taken as that
- *   out_dev        [rows, heads, head_dim] contiguous, out_dtype MLXR_F32 / MLXR_F16 / MLXR_BF16
+ *   out_dev        [rows, heads, head_dim] contiguous, at a multiple of 16 bytes, out_dtype MLXR_F32 / MLXR_F16 /
+ *                  MLXR_BF16
  *   lse_dev        [rows, heads] fp32 or NULL: natural logarithm of the softmax's sum, -inf for
  *                  an empty row
  * Tokens of pages whose table entry lies outside the cache are left out.  What lies in the cache

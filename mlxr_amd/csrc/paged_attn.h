@@ -85,6 +85,43 @@ __device__ __forceinline__ uint32_t widen(uint32_t w) {
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, H));
 }
 
+// N (1, 2, 4) words at a multiple of 4 N bytes.
+template <int N>
+struct Words {
+  uint32_t w[N];
+};
+template <int N, bool NT>
+__device__ __forceinline__ Words<N> load_words(const void* p) {
+  Words<N> r;
+  if constexpr (N == 1) {
+    r.w[0] = NT ? __builtin_nontemporal_load((const uint32_t*)p) : *(const uint32_t*)p;
+  } else {
+    typedef __attribute__((ext_vector_type(N))) uint32_t V;
+    const V v = NT ? __builtin_nontemporal_load((const V*)p) : *(const V*)p;
+#pragma unroll
+    for (int k = 0; k < N; ++k) r.w[k] = v[k];
+  }
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void store_words(void* p, const Words<N>& v) {
+  __builtin_memcpy(__builtin_assume_aligned(p, 4 * N), &v, 4 * N);
+}
+// N (4, 8) neighbouring values from element i, a multiple of N, of an output on.
+template <int N>
+__device__ __forceinline__ void store_values(void* out, int dtype, int64_t i, const float* v) {
+  if (dtype == DT_F32) {
+#pragma unroll
+    for (int c = 0; c < N; c += 4) *(f32x4_t*)((float*)out + i + c) = f32x4_t{v[c], v[c + 1], v[c + 2], v[c + 3]};
+  } else {
+    Words<N / 2> w;
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k)
+      w.w[k] = dtype == DT_F16 ? pack2<true>(v[2 * k], v[2 * k + 1]) : pack2<false>(v[2 * k], v[2 * k + 1]);
+    store_words<N / 2>((uint16_t*)out + i, w);
+  }
+}
+
 // F16: the products' type (else bf16).  F8: the cache is e4m3.  DT: 64, 128 or 256, at least dim (DIM:
 // equal).  P8: page_size % 8 == 0.
 template <bool F16, bool F8, int DT, bool DIM, bool P8>
@@ -96,6 +133,7 @@ struct Attn {
   // p times 2^14 in f16: weights down to 2^-28 of the largest stay normal numbers (bf16 has the range)
   static constexpr float SHIFT = F16 ? 14.f : 0.f;
   static constexpr float UNSHIFT = F16 ? 0x1p-14f : 1.f;
+  static constexpr bool NT = DIM && DT * (F8 ? 1 : 2) % 128 == 0;  // past the caches
   static constexpr int KL = F8 ? KS / 2 : KS;      // 16-byte loads of a key row by a lane
 
   const AttnArgs& a;
@@ -139,7 +177,7 @@ struct Attn {
   // of 80 in [token, head] order 53 -> 66 us).
   template <class T>
   static __device__ __forceinline__ T stream_load(const T* p) {
-    if constexpr (DIM && DT * (F8 ? 1 : 2) >= 128) return __builtin_nontemporal_load(p);
+    if constexpr (NT) return __builtin_nontemporal_load(p);
     else return *p;
   }
   // Index of a position's page among its row's.
@@ -184,6 +222,11 @@ struct Attn {
     return live;
   }
 
+  // First of the VE neighbouring dims of row m of the second product's operand, half x; rows past the head's dims
+  // repeat the first, their sums are not stored.
+  __device__ __forceinline__ bool has_row(int x, int m) const { return DIM || x * 128 + VE * m < a.dim; }
+  __device__ __forceinline__ int dims_of(int x, int m) const { return has_row(x, m) ? x * 128 + VE * m : 0; }
+
   // The loads of a tile are unconditional, from an address within the stores for whatever does not count, so
   // that they stay in flight over the branches: what they bring for tokens that do not count is left out later.
   // more: false where there is no further tile; all lanes then read the first page's first rows again.
@@ -211,18 +254,9 @@ struct Attn {
                             : vh + (more ? offset(n.id[P8 ? 0 : j], t0 + 8 * g + j, a.v_page, a.v_token) : 0);
 #pragma unroll
       for (int x = 0; x < VH; ++x) {
-        int d = x * 128 + VE * col;
-        if (!DIM && d >= a.dim) d = 0;  // its sums are not stored
-        const uint8_t* at = p + d * (F8 ? 1 : 2);
-        if constexpr (W == 4) {
-          const u32x4_t w = stream_load((const u32x4_t*)at);
-          vr[x][j][0] = w.x, vr[x][j][1] = w.y, vr[x][j][2] = w.z, vr[x][j][3] = w.w;
-        } else if constexpr (W == 2) {
-          const u32x2_t w = stream_load((const u32x2_t*)at);
-          vr[x][j][0] = w.x, vr[x][j][1] = w.y;
-        } else {
-          vr[x][j][0] = stream_load((const uint32_t*)at);
-        }
+        const Words<W> w = load_words<W, NT>(p + dims_of(x, col) * (F8 ? 1 : 2));
+#pragma unroll
+        for (int k = 0; k < W; ++k) vr[x][j][k] = w.w[k];
       }
     }
   }
@@ -364,8 +398,6 @@ struct Attn {
       for (int i = 0; i < 4; ++i) o[c][i] = o[c][i] * f + from[(4 * c + i) * 64 + lane] * f2;
   }
 
-  // First of the VE neighbouring dims that this lane holds of row i of the accumulators of half x.
-  __device__ __forceinline__ int out_dim(int x, int i) const { return x * 128 + VE * (4 * g + i); }
 
   __device__ __forceinline__ void finish(int r, int kvh, int grp, float* part) {
     l += __shfl_xor(l, 16);
@@ -378,11 +410,10 @@ struct Attn {
       for (int x = 0; x < VH; ++x)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int d = out_dim(x, i);
-          if (DIM || d < a.dim)
+          float v[VE];
 #pragma unroll
-            for (int c = 0; c < VE; c += 4)
-              *(f32x4_t*)(row + d + c) = f32x4_t{o[x * VE + c][i], o[x * VE + c + 1][i], o[x * VE + c + 2][i], o[x * VE + c + 3][i]} * UNSHIFT;
+          for (int c = 0; c < VE; ++c) v[c] = o[x * VE + c][i] * UNSHIFT;
+          if (has_row(x, 4 * g + i)) store_values<VE>(row, DT_F32, dims_of(x, 4 * g + i), v);
         }
       if (g == 0) {
         float* st = part + (int64_t)a.part_rows * a.dim + 2 * col;
@@ -397,10 +428,10 @@ struct Attn {
     for (int x = 0; x < VH; ++x)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int d = out_dim(x, i);
-        if (DIM || d < a.dim)
+        float v[VE];
 #pragma unroll
-          for (int c = 0; c < VE; ++c) store_scalar(a.out, a.out_dtype, head * a.dim + d + c, o[x * VE + c][i] * f);
+        for (int c = 0; c < VE; ++c) v[c] = o[x * VE + c][i] * f;
+        if (has_row(x, 4 * g + i)) store_values<VE>(a.out, a.out_dtype, head * a.dim + dims_of(x, 4 * g + i), v);
       }
     if (a.lse && g == 0) a.lse[head] = (m + __builtin_amdgcn_logf(l * UNSHIFT)) * 0.69314718055994531f;
   }

@@ -75,8 +75,9 @@ __global__ __launch_bounds__(THREADS) void join_kernel(AttnArgs a, int lanes) {
   if (y || !in) return;
   for (int w = 1; w < WAVES; ++w) add(sum, sh[w][x]);
   const float f = (a.v_scale ? a.v_scale[kvh] : 1.f) / sum.l;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) store_scalar(a.out, a.out_dtype, head * a.dim + 4 * x + c, sum.o[c] * f);
+  const f32x4_t v = sum.o * f;
+  const float each[4] = {v[0], v[1], v[2], v[3]};
+  store_values<4>(a.out, a.out_dtype, head * a.dim + 4 * x, each);
   if (a.lse && x == 0) a.lse[head] = (sum.m + __builtin_amdgcn_logf(sum.l)) * 0.69314718055994531f;
 }
 
@@ -179,8 +180,8 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   if (window < 0) return set_error(MLXR_E_INVALID, "paged_attention: window must not be negative");
   if (rows == 0) return MLXR_OK;
   if (!q_dev || !table_dev || !lens_dev || !out_dev) return set_error(MLXR_E_INVALID, "null buffer");
-  if (q_row_stride % 8 || q_head_stride % 8 || ((uintptr_t)q_dev & 15) || ((uintptr_t)workspace_dev & 15))
-    return set_error(MLXR_E_SHAPE, "paged_attention: query rows and the workspace must start at multiples of 16 bytes");
+  if (q_row_stride % 8 || q_head_stride % 8 || (((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15))
+    return set_error(MLXR_E_SHAPE, "paged_attention: query rows, output and workspace must start at multiples of 16 bytes");
   const Plan p = plan_of(cache, rows, heads, longest(cache, table_width, window));
   if (workspace_bytes < p.bytes || (p.bytes && !workspace_dev))
     return set_error(MLXR_E_INVALID, "paged_attention: the workspace is smaller than mlxr_paged_attention_workspace_size");

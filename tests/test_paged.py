@@ -66,7 +66,7 @@ def test_attention_refusals():
     for name in ("q", "table", "lens", "out"):
         assert call(**{name: 0}) == -1, name
     assert call(width=0) == -1 and call(width=100, ws=0) == -1
-    assert call(q=72) == -3 and call(qr=4095) == -3 and call(qh=4) == -3 and call(ws=72) == -3
+    assert call(q=72) == -3 and call(out=72) == -3 and call(qr=4095) == -3 and call(qh=4) == -3 and call(ws=72) == -3
     assert call(width=1 << 30) == -3
     assert call(c=_cache(k0=1 << 31)) == -3 and call(c=_cache(v2=1 << 31)) == -3
     assert call(width=100, nb=16) == -1 and "workspace" in L.mlxr_qgemm_last_error().decode()
@@ -429,7 +429,7 @@ def test_attention(cuda, dtype, cache, heads, kv, dim, page, token_major):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dim", [8, 24, 40, 56, 72, 104, 120, 136, 248])
+@pytest.mark.parametrize("dim", [8, 24, 40, 56, 72, 80, 88, 96, 104, 120, 136, 248])
 def test_attention_dims_of_eight(cuda, dim):
     _run(cuda, [1, 40, 333, 0], 6, 2, dim, 16, "bf16", "bf16", seed=dim)
 

@@ -63,9 +63,15 @@ class Linear:
             raise QGemmError(-3, "Bias shape must be [N]")
         self.bias = bias
 
-    def forward(self, x, stream=None):
+    def forward(self, x, stream=None, lora=None, adapter_ids=None):
+        """x W^T (+ b); with ``lora`` (a LoraBank of this layer's shape) and ``adapter_ids`` [tokens] (int32,
+        -1: none) also each token's own adapter (lora_apply)."""
         if self.weight is None:
             raise QGemmError(-1, "Linear: weight not loaded")
+        if (lora is None) != (adapter_ids is None):
+            raise QGemmError(-1, "Linear: lora and adapter_ids go together")
+        if lora is not None and (lora.N, lora.K) != (self.out_features, self.in_features):
+            raise QGemmError(-3, "adapters do not match [out_features, in_features]")
         if self.has_bias and self.bias is None:
             raise QGemmError(-1, "Linear: bias not set")
         if x.dim() < 1 or x.shape[-1] != self.in_features:
@@ -77,6 +83,8 @@ class Linear:
         x2 = x.reshape(M, self.in_features)
         y = qgemm.q_gemm_dequant(x2, self.weight, M, self.out_features, self.in_features, self.weight.qtype,
                                  bias=self.bias, stream=stream)
+        if lora is not None:
+            y = lora.apply(x2, adapter_ids, y, out=y, stream=stream)
         return y.reshape(*lead, self.out_features)
 
     __call__ = forward

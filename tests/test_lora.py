@@ -214,3 +214,25 @@ def test_lora_bank(cuda):
             A, B, s = parts[i]
             ref = ref + s * (x[t].double() @ A.t() @ B.t())
         assert float((got[t].double().cpu() - ref).abs().max()) < 1e-3
+
+
+@pytest.mark.gpu
+def test_linear_with_adapters(cuda):
+    """Linear(x, lora, ids) is its projection plus each token's adapter; without them nothing changes."""
+    import torch
+    K, N = 512, 384
+    lin = mx.Linear(K, N, bias=True).load_weight(mx.synth_gguf(mx.QuantType.Q4_K, N, K, 3), mx.QuantType.Q4_K, device=cuda)
+    lin.set_bias(torch.linspace(-1, 1, N, device=cuda))
+    bank = mx.LoraBank(2, 8, N, K, device=cuda)
+    bank.load(0, torch.randn(8, K) / 20, torch.randn(N, 8)).load(1, torch.randn(3, K) / 20, torch.randn(N, 3), 2.0)
+    x = torch.randn(2, 5, K, device=cuda).to(torch.bfloat16)
+    ids = torch.tensor([0, 1, -1, 1, 0, 0, -1, 1, 1, 0], dtype=torch.int32, device=cuda)
+    y = lin(x)
+    got = lin(x, lora=bank, adapter_ids=ids)
+    want = mx.lora_apply(x.view(10, K), ids, [bank.a], [bank.b], [y.view(10, N)], bank.scales, bank.ranks)[0]
+    assert got.shape == (2, 5, N) and torch.equal(got.view(10, N), want) and not torch.equal(got, y)
+    assert torch.equal(got.view(10, N)[[2, 6]], y.view(10, N)[[2, 6]])
+    with pytest.raises(mx.QGemmError, match="together"):
+        lin(x, lora=bank)
+    with pytest.raises(mx.QGemmError, match="do not match"):
+        lin(x, lora=mx.LoraBank(2, 8, N, 256, device=cuda), adapter_ids=ids)

@@ -6,7 +6,8 @@
  *
  * for each of `count` projections that read the same x (q/k/v, gate/up); y is the shared
  * projection's output (mlxr_qgemm_run and its kin).  Tokens of any adapters may follow each
- * other in any order; a token without one (ids[t] outside [0, adapters)) keeps y[t].
+ * other in any order; a token without one (ids[t] outside [0, adapters)) keeps y[t].  An output may
+ * be its y and must not overlap anything else that the call reads.
  */
 #ifndef MLXR_LORA_H
 #define MLXR_LORA_H

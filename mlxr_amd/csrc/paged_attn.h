@@ -10,8 +10,8 @@
 // 8 b + 4 hh + i, so the scores that a lane holds (heads across lanes, rows 4 g .. 4 g + 3 for lane
 // group g) are those of tokens 8 g .. 8 g + 7, which is what the second product wants in that lane
 // as its operand: P never leaves the registers, and the softmax's factors are one value per lane.
-// P is split in two 16-bit parts, hi + lo: with one part its rounding (2^-9 in bf16) would be as
-// large as the output's own.  A second product costs matrix cycles that the kernel, bound by
+// P is split in two 16-bit parts, hi + lo (together 2^-16 in bf16): with one part its rounding
+// would be as large as the output's own.  A second product costs matrix cycles that the kernel, bound by
 // memory, has to spare.
 //
 // Short rows: a workgroup for each (row, kv head), merged in LDS (attn_rows_kernel).  Long ones are cut
@@ -321,6 +321,21 @@ struct Attn {
     }
   }
 
+  // Two weights as the sum of two 16-bit parts, neither of them negative nor, beside a weight above 0, the second 0:
+  // an infinite value then gives an infinite output as a weight in one piece does, not NaN.  (The least
+  // second part, 2^-126 or 2^-38 of the largest weight, is far below the rounding of the sums.)
+  static __device__ __forceinline__ void split2(float p0, float p1, uint32_t* hi, uint32_t* lo) {
+    if constexpr (F16) {
+      *hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+      *lo = pack2<true>(fmaxf(p0 - unpack<true>(*hi, 0), 0x1p-24f), fmaxf(p1 - unpack<true>(*hi, 1), 0x1p-24f));
+    } else {
+      const uint32_t b0 = __builtin_bit_cast(uint32_t, p0), b1 = __builtin_bit_cast(uint32_t, p1);
+      *hi = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+      *lo = pack2<false>(fmaxf(p0 - __builtin_bit_cast(float, b0 & 0xffff0000u), 0x1p-126f),
+                         fmaxf(p1 - __builtin_bit_cast(float, b1 & 0xffff0000u), 0x1p-126f));
+    }
+  }
+
   // Zeros for the values of tokens that do not count: their weight is 0, their bits may be NaN.
   __device__ __forceinline__ void drop(uint32_t live) {
 #pragma unroll
@@ -369,8 +384,10 @@ struct Attn {
     for (int k = 0; k < 4; ++k) {
       const float p0 = __builtin_amdgcn_exp2f(x[2 * k] + off), p1 = __builtin_amdgcn_exp2f(x[2 * k + 1] + off);
       sum += p0 + p1;
-      (*hi)[k] = pack2<F16>(p0, p1);
-      (*lo)[k] = pack2<F16>(p0 - unpack<F16>((*hi)[k], 0), p1 - unpack<F16>((*hi)[k], 1));
+      uint32_t h, r;
+      split2(p0, p1, &h, &r);
+      (*hi)[k] = h;
+      (*lo)[k] = r;
     }
     l = l * alpha + sum;
 #pragma unroll

@@ -146,7 +146,7 @@ int check_attn(const mlxr_paged_cache* c, int rows, int heads, int width) {
   for (int i = 0; i < 3; i += 2)
     if (c->k_stride[i] > UINT32_MAX / 2 || c->v_stride[i] > UINT32_MAX / 2)
       return set_error(MLXR_E_SHAPE, "paged_attention: pages and tokens must lie less than 4 GiB apart");
-  if ((int64_t)width * c->page_size > INT32_MAX) return set_error(MLXR_E_SHAPE, "paged_attention: the table covers too many tokens");
+  if ((int64_t)width * c->page_size > INT32_MAX - 1024) return set_error(MLXR_E_SHAPE, "paged_attention: the table covers too many tokens");
   if ((int64_t)rows * heads > kMaxHeads) return set_error(MLXR_E_SHAPE, "paged_attention: at most %d rows times heads", kMaxHeads);
   return MLXR_OK;
 }

@@ -298,7 +298,7 @@ extern "C" int mlxr_page_resize(int rows, int page_size, int num_pages, int32_t*
     return set_error(MLXR_E_INVALID, "null buffer");
   if (rows > MLXR_PAGED_MAX_ROWS)
     return set_error(MLXR_E_SHAPE, "page_resize: at most %d rows", MLXR_PAGED_MAX_ROWS);
-  if (table_stride < table_width) return set_error(MLXR_E_SHAPE, "page_resize: table rows overlap");
+  if (rows > 1 && table_stride < table_width) return set_error(MLXR_E_SHAPE, "page_resize: table rows overlap");
   if ((int64_t)num_pages * page_size > INT32_MAX ||
       (__int128)(rows ? rows : 1) * table_width * page_size > INT32_MAX)
     return set_error(MLXR_E_SHAPE, "page_resize: a pool and a table cover at most %d tokens", INT32_MAX);

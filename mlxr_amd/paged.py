@@ -106,6 +106,8 @@ def _cache(k, v, k_scale, v_scale):
     if ks[3] != 1 or vs[3] != 1:
         raise QGemmError(-3, "the last dimension of a store must be contiguous")
     pages, heads, page, dim = shape
+    if pages == 1 or heads == 1 or page == 1:  # strides of single places mean nothing
+        ks, vs = ([s if n > 1 else 0 for s, n in zip(t, shape)] for t in (ks, vs))
     code = _code(_cache_codes, k.dtype, "the cache")
     return _pack_cache(k.data_ptr(), v.data_ptr(), _per_head(k_scale, heads, "k_scale", d) if k_scale is not None else 0,
                        _per_head(v_scale, heads, "v_scale", d) if v_scale is not None else 0, ks[0], ks[1], ks[2], vs[0], vs[1],
@@ -115,7 +117,7 @@ def _cache(k, v, k_scale, v_scale):
 def _rows16(t, stream):
     """t [n, heads, dim] with rows that start at multiples of 16 bytes: t itself, or a copy."""
     s, size = t.stride(), t.element_size()
-    if s[2] == 1 and s[0] * size % 16 == 0 and s[1] * size % 16 == 0 and s[0] >= 0 and t.data_ptr() % 16 == 0:
+    if (s[2] == 1 or t.shape[2] == 1) and s[0] * size % 16 == 0 and s[1] * size % 16 == 0 and s[0] >= 0 and t.data_ptr() % 16 == 0:
         return t
     return _on(stream, t.clone, memory_format=_torch.contiguous_format)
 
@@ -137,8 +139,8 @@ def page_resize(table, lens, want, free, free_count, page_size, tokens, stream=N
     rows, width = table.shape
     if not table.is_cuda or lens.shape != (rows,) or want.shape != (rows,) or free_count.shape != (1,):
         raise QGemmError(-3, "page_resize: lens and want must be [rows], free_count [1], on the table's GPU")
-    if tokens < 0:
-        raise QGemmError(-1, "page_resize: tokens must not be negative")
+    if not 0 <= tokens < 1 << 31 or not 0 < page_size < 1 << 31:
+        raise QGemmError(-1, "page_resize: tokens must not be negative and page_size must be positive")
     buf = _on(stream, _torch.empty, 2 * (rows + tokens) + 3, dtype=_torch.int32, device=d)
     p0 = buf.data_ptr()
     p1 = p0 + 4 * rows
@@ -174,7 +176,8 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
                     out_dtype=None, return_lse=False, stream=None):
     """Attention of one new token per row, q [rows, heads, head_dim], over the row's cached tokens
     (mlxr_paged_attention): ``lens`` [rows] counts them, the new one included, ``table`` [rows, width]
-    names their pages.  ``scale`` defaults to head_dim ** -0.5; ``window`` keeps the last tokens only
+    names their pages; how the work is split goes by what the table could hold, so pass ``table[:, :n]``
+    where no row needs more than n pages.  ``scale`` defaults to head_dim ** -0.5; ``window`` keeps the last tokens only
     (0: all).  Rows of length 0 give zeros.  Returns out [rows, heads, head_dim] (q's dtype or
     ``out_dtype``), with ``return_lse`` also the log of the softmax's sum, float32 [rows, heads]."""
     lib = _lib()
@@ -189,6 +192,8 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
     width = table.shape[1]
     if table.shape[0] != rows or lens.shape[0] != rows:
         raise QGemmError(-3, "table and lens must have one row per query")
+    if not 0 <= window < 1 << 31:
+        raise QGemmError(-1, "paged_attention: window must not be negative")
     dt = _code(_x_codes, q.dtype, "queries")
     if out is None:
         out = _on(stream, _torch.empty, shape, dtype=out_dtype or q.dtype, device=d)

@@ -527,6 +527,45 @@ def test_attention_infinite_scores(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("width", [5, 400])
+def test_attention_infinite_values(cuda, dtype, width):
+    """An infinite value makes its dimension of the output infinite, not NaN; NaN values make it NaN; the other
+    dimensions and rows stay as they are."""
+    import torch
+    n, dim = 70, 64
+    k = torch.randn((10, 1, 16, dim), device=cuda).to(_dt(dtype))
+    v = torch.randn((10, 1, 16, dim), device=cuda).to(_dt(dtype))
+    q = torch.randn((2, 3, dim), device=cuda).to(_dt(dtype))
+    table = torch.full((2, width), -1, dtype=torch.int32, device=cuda)
+    table[:, :5] = torch.arange(10, dtype=torch.int32, device=cuda).view(2, 5)
+    lens = torch.tensor([n, n], dtype=torch.int32, device=cuda)
+    plain = mx.paged_attention(q, k, v, table, lens, out_dtype=torch.float32)
+    v[1, 0, 3, 5], v[2, 0, 0, 7], v[0, 0, 9, 8] = float("inf"), float("-inf"), float("nan")
+    got = mx.paged_attention(q, k, v, table, lens, out_dtype=torch.float32)
+    assert (got[0, :, 5] == float("inf")).all() and (got[0, :, 7] == float("-inf")).all() and torch.isnan(got[0, :, 8]).all()
+    got[0, :, [5, 7, 8]] = plain[0, :, [5, 7, 8]]
+    assert torch.equal(got, plain)
+
+
+@pytest.mark.gpu
+def test_single_places_have_any_stride(cuda):
+    """Stores of one page, one head or one token, whose strides torch may have set to anything."""
+    import torch
+    q = torch.randn(1, 2, 64, device=cuda).to(torch.bfloat16)
+    one = torch.ones(1, dtype=torch.int32, device=cuda)
+    zero = torch.zeros(1, dtype=torch.int32, device=cuda)
+    for shape in ((1, 1, 16, 64), (3, 1, 8, 64), (4, 2, 1, 64), (1, 1, 1, 64)):
+        k, v = torch.randn(2, *shape, device=cuda).to(torch.bfloat16)
+        odd = [torch.as_strided(t, shape, [s if n > 1 else 3 for s, n in zip(t.stride(), shape)]) for t in (k, v)]
+        mx.paged_append(q[:, :shape[1]], q[:, :shape[1]], *odd, zero)
+        assert torch.equal(k[0, :, 0], q[0, :shape[1]])
+        table = torch.as_strided(zero, (1, 1), (0, 1))
+        a = mx.paged_attention(q, *odd, table, one)
+        assert torch.equal(a, mx.paged_attention(q, k, v, table, one))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("page", [16, 6])
 def test_attention_leaves_pages_outside_the_cache_out(cuda, page):
     import torch

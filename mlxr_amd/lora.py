@@ -8,7 +8,7 @@ import ctypes
 import struct
 
 from . import paged, qgemm
-from .paged import _code, _i32, _on, _stream
+from .paged import _code, _on, _stream, _vector
 from .qgemm import QGemmError
 
 MAX_ADAPTERS, MAX_RANK = 4096, 128
@@ -47,24 +47,20 @@ def lora_apply(x, ids, a, b, y, scales=None, ranks=None, outs=None, stream=None)
     a[i] [adapters, rank, K] and b[i] [adapters, N_i, rank] have x's dtype (float16 / bfloat16), one
     rank (a multiple of 8, up to 128) for all; ``ranks`` [adapters] (int32) says how much of it each
     adapter uses.  ``scales`` [adapters] float32.  outs[i] may be y[i].  Returns the outputs."""
-    lib, d, n, torch = _lib(), x.device, len(a), paged._torch
-    if x.dim() != 2 or not x.is_cuda:
+    lib, index, n, torch = _lib(), x.get_device(), len(a), paged._torch
+    if x.dim() != 2 or index < 0:
         raise QGemmError(-3, "Input shape must be [tokens, K] on a GPU")
     tokens, K = x.shape
     if len(b) != n or len(y) != n or (outs is not None and len(outs) != n):
         raise QGemmError(-1, "one A, one B, one y (and one output) per projection")
-    pi = _i32(ids, "ids", d)
-    if ids.shape[0] != tokens:
-        raise QGemmError(-3, "ids must be [tokens]")
+    pi = _vector(ids, tokens, "ids", index)
     if n == 0:
         return []
     if a[0].dim() != 3:
         raise QGemmError(-3, "a[0] must be [adapters, rank, K]")
     adapters, rank, _ = shape = a[0].shape
-    ps = paged._per_head(scales, adapters, "scales", d) if scales is not None else None
-    pr = _i32(ranks, "ranks", d) if ranks is not None else None
-    if ranks is not None and ranks.shape[0] != adapters:
-        raise QGemmError(-3, f"ranks must be [{adapters}]")
+    ps = None if scales is None else _vector(scales, adapters, "scales", index, paged._float32)
+    pr = None if ranks is None else _vector(ranks, adapters, "ranks", index)
     xt = x.dtype
     dt = _code(paged._x_codes, xt, "x")
     xs = x.stride()
@@ -87,18 +83,18 @@ def lora_apply(x, ids, a, b, y, scales=None, ranks=None, outs=None, stream=None)
         if len(bs) != 3 or bs[0] != adapters or bs[2] != rank:
             raise QGemmError(-3, f"b[{i}] must be [{adapters}, N, {rank}]")
         N = bs[1]
-        if A.dtype is not xt or B.dtype is not xt or A.device != d or B.device != d or not A.is_contiguous() or not B.is_contiguous():
+        if A.dtype is not xt or B.dtype is not xt or A.get_device() != index or B.get_device() != index or not A.is_contiguous() or not B.is_contiguous():
             raise QGemmError(-1, f"a[{i}] and b[{i}] must be contiguous, of x's dtype and device")
-        if len(ts) != 2 or ts[0] != tokens or ts[1] != N or t.device != d or not t.is_contiguous() or \
-                given and (o.shape != ts or o.dtype is not t.dtype or o.device != d or not o.is_contiguous()):
-            raise QGemmError(-1, f"y[{i}] and its output must be contiguous [{tokens}, {N}] tensors of one dtype on {d}")
+        if len(ts) != 2 or ts[0] != tokens or ts[1] != N or t.get_device() != index or not t.is_contiguous() or \
+                given and (o.shape != ts or o.dtype is not t.dtype or o.get_device() != index or not o.is_contiguous()):
+            raise QGemmError(-1, f"y[{i}] and its output must be contiguous [{tokens}, {N}] tensors of one dtype on GPU {index}")
         items += _pack_item(A.data_ptr(), B.data_ptr(), t.data_ptr(), o.data_ptr(), N, _code(codes, t.dtype, "y"))
     nb = ctypes.c_size_t()
     qgemm._check(lib.mlxr_lora_workspace_size(n, items, tokens, K, adapters, rank, ctypes.byref(nb)))
     nb = nb.value
-    ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=d) if nb else None
+    ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=x.device) if nb else None
     qgemm._check(lib.mlxr_lora_apply(n, items, tokens, K, adapters, rank, x.data_ptr(), dt, xs[0], pi, ps, pr, ws.data_ptr() if nb else None, nb,
-                                     _stream(stream, d.index)))
+                                     _stream(stream, index)))
     return outs
 
 

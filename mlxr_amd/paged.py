@@ -44,20 +44,20 @@ _SIGS = {
 }
 
 _bound = None
-_torch = None
+_torch = _int32 = _float32 = None
 _x_codes, _cache_codes = {}, {}
 
 
 def _lib():
     """The library with this module's entries declared."""
-    global _bound, _torch
+    global _bound, _torch, _int32, _float32
     if _bound is None:
         l = qgemm.lib()
         for name, (res, args) in _SIGS.items():
             f = getattr(l, name)
             f.restype, f.argtypes = res, args
         import torch
-        _torch = torch
+        _torch, _int32, _float32 = torch, torch.int32, torch.float32
         _x_codes.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
         _cache_codes.update({torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3})
         _bound = l
@@ -84,24 +84,28 @@ def _on(stream, make, *args, **kw):
         return make(*args, **kw)
 
 
-def _i32(t, what, device, dims=1):
-    if t.dtype != _torch.int32 or t.dim() != dims or t.device != device or (t.stride()[-1] != 1 and t.shape[-1] > 1):
-        raise QGemmError(-1, f"{what} must be a{' contiguous' if dims == 1 else ''} {dims}-dimensional int32 tensor on {device}")
+def _vector(t, n, what, index, dtype=None):
+    """Address of a contiguous [n] tensor of int32 (or dtype) on GPU `index`."""
+    dtype = dtype or _int32
+    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != index or not t.is_contiguous():
+        raise QGemmError(-1 if t.dtype is not dtype or t.get_device() != index or t.dim() != 1 else -3,
+                         f"{what} must be a contiguous {str(dtype)[6:]} [{n}] tensor on GPU {index}")
     return t.data_ptr()
 
 
-def _per_head(t, heads, what, device):
-    if t.dtype != _torch.float32 or t.shape != (heads,) or not t.is_contiguous() or t.device != device:
-        raise QGemmError(-1, f"{what} must be a contiguous float32 [{heads}] tensor on {device}")
+def _table(t, index):
+    """Address of a page table [rows, width] on GPU `index`."""
+    if t.dtype is not _int32 or t.dim() != 2 or t.get_device() != index or (t.stride()[1] != 1 and t.shape[1] > 1):
+        raise QGemmError(-1, f"table must be a 2-dimensional int32 tensor with contiguous rows on GPU {index}")
     return t.data_ptr()
 
 
 def _cache(k, v, k_scale, v_scale):
-    """mlxr_paged_cache of two stores, its dtype code and the stores' shape."""
-    shape, ks, vs, d = k.shape, k.stride(), v.stride(), k.device
+    """mlxr_paged_cache of two stores, their heads, head_dim and GPU."""
+    shape, ks, vs, index = k.shape, k.stride(), v.stride(), k.get_device()
     if len(shape) != 4 or v.shape != shape:
         raise QGemmError(-3, "key and value stores must be [num_pages, kv_heads, page_size, head_dim] of one shape")
-    if v.dtype != k.dtype or v.device != d or not k.is_cuda:
+    if v.dtype is not k.dtype or v.get_device() != index or index < 0:
         raise QGemmError(-1, "key and value stores must have one dtype and be on one GPU")
     if ks[3] != 1 or vs[3] != 1:
         raise QGemmError(-3, "the last dimension of a store must be contiguous")
@@ -109,9 +113,10 @@ def _cache(k, v, k_scale, v_scale):
     if pages == 1 or heads == 1 or page == 1:  # strides of single places mean nothing
         ks, vs = ([s if n > 1 else 0 for s, n in zip(t, shape)] for t in (ks, vs))
     code = _code(_cache_codes, k.dtype, "the cache")
-    return _pack_cache(k.data_ptr(), v.data_ptr(), _per_head(k_scale, heads, "k_scale", d) if k_scale is not None else 0,
-                       _per_head(v_scale, heads, "v_scale", d) if v_scale is not None else 0, ks[0], ks[1], ks[2], vs[0], vs[1],
-                       vs[2], code, pages, page, heads, dim), code, shape
+    return _pack_cache(k.data_ptr(), v.data_ptr(),
+                       0 if k_scale is None else _vector(k_scale, heads, "k_scale", index, _float32),
+                       0 if v_scale is None else _vector(v_scale, heads, "v_scale", index, _float32), ks[0], ks[1], ks[2], vs[0],
+                       vs[1], vs[2], code, pages, page, heads, dim), heads, dim, index
 
 
 def _rows16(t, stream):
@@ -133,43 +138,44 @@ def page_resize(table, lens, want, free, free_count, page_size, tokens, stream=N
     ``free`` [num_pages] is the pool's stack of free pages, its first ``free_count`` [1] entries; both
     it and the table are changed in place.  ``tokens``: places for the new tokens' slots.  All
     tensors int32.  Returns ``Resized``; nothing is copied to the host."""
-    lib, d = _lib(), table.device
-    pt, pl, pw = _i32(table, "table", d, 2), _i32(lens, "lens", d), _i32(want, "want", d)
-    pf, pc = _i32(free, "free", d), _i32(free_count, "free_count", d)
-    rows, width = table.shape
-    if not table.is_cuda or lens.shape != (rows,) or want.shape != (rows,) or free_count.shape != (1,):
-        raise QGemmError(-3, "page_resize: lens and want must be [rows], free_count [1], on the table's GPU")
+    lib, index, shape = _lib(), table.get_device(), table.shape
+    if index < 0:
+        raise QGemmError(-1, "page_resize: table must be on a GPU")
+    pt = _table(table, index)
+    rows, width = shape
+    pl, pw = _vector(lens, rows, "lens", index), _vector(want, rows, "want", index)
+    pages = free.shape[0]
+    pf, pc = _vector(free, pages, "free", index), _vector(free_count, 1, "free_count", index)
     if not 0 <= tokens < 1 << 31 or not 0 < page_size < 1 << 31:
         raise QGemmError(-1, "page_resize: tokens must not be negative and page_size must be positive")
-    buf = _on(stream, _torch.empty, 2 * (rows + tokens) + 3, dtype=_torch.int32, device=d)
+    buf = _on(stream, _torch.empty, 2 * (rows + tokens) + 3, dtype=_int32, device=table.device)
     p0 = buf.data_ptr()
     p1 = p0 + 4 * rows
     p2 = p1 + 4
     p3 = p2 + 4 * (rows + 1)
     p4 = p3 + 4 * tokens
-    qgemm._check(lib.mlxr_page_resize(rows, page_size, free.shape[0], pt, table.stride()[0], width, pl, pw, pf, pc, p0, p1, p2,
-                                      p3, p4, tokens, p4 + 4 * tokens, _stream(stream, d.index)))
-    return Resized._make(buf.split((rows, 1, rows + 1, tokens, tokens, 1)))
+    qgemm._check(lib.mlxr_page_resize(rows, page_size, pages, pt, table.stride()[0], width, pl, pw, pf, pc, p0, p1, p2,
+                                      p3, p4, tokens, p4 + 4 * tokens, _stream(stream, index)))
+    return Resized._make(buf.unsafe_split_with_sizes((rows, 1, rows + 1, tokens, tokens, 1)))
 
 
 def paged_append(k, v, k_store, v_store, slots, k_scale=None, v_scale=None, stream=None):
     """Writes keys and values [tokens, kv_heads, head_dim] into the slots [tokens] (int32; tokens whose
     slot is -1 are left out) of the stores, divided by their head's scale (mlxr_paged_append)."""
     lib = _lib()
-    c, _, (_, heads, _, dim) = _cache(k_store, v_store, k_scale, v_scale)
-    d, shape = k_store.device, k.shape
+    c, heads, dim, index = _cache(k_store, v_store, k_scale, v_scale)
+    shape = k.shape
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim or v.shape != shape:
         raise QGemmError(-3, "keys and values must be [tokens, kv_heads, head_dim]")
-    if k.device != d or v.device != d or v.dtype != k.dtype:
+    if k.get_device() != index or v.get_device() != index or v.dtype is not k.dtype:
         raise QGemmError(-1, "keys and values must have one dtype and be on the cache's GPU")
-    n, ps = shape[0], _i32(slots, "slots", d)
-    if slots.shape != (n,):
-        raise QGemmError(-3, "slots must be [tokens]")
+    n = shape[0]
+    ps = _vector(slots, n, "slots", index)
     dt = _code(_x_codes, k.dtype, "keys")
     k, v = _rows16(k, stream), _rows16(v, stream)
     ks, vs = k.stride(), v.stride()
     qgemm._check(lib.mlxr_paged_append(c, n, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, ps,
-                                       _stream(stream, d.index)))
+                                       _stream(stream, index)))
 
 
 def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_scale=None, v_scale=None, out=None,
@@ -181,35 +187,38 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
     (0: all).  Rows of length 0 give zeros.  Returns out [rows, heads, head_dim] (q's dtype or
     ``out_dtype``), with ``return_lse`` also the log of the softmax's sum, float32 [rows, heads]."""
     lib = _lib()
-    c, _, (_, _, _, dim) = _cache(k_store, v_store, k_scale, v_scale)
-    d, shape = k_store.device, q.shape
+    c, _, dim, index = _cache(k_store, v_store, k_scale, v_scale)
+    shape = q.shape
     if len(shape) != 3 or shape[2] != dim:
         raise QGemmError(-3, "queries must be [rows, heads, head_dim]")
-    if q.device != d:
+    if q.get_device() != index:
         raise QGemmError(-1, "queries must be on the cache's GPU")
     rows, heads, _ = shape
-    pt, pl = _i32(table, "table", d, 2), _i32(lens, "lens", d)
-    width = table.shape[1]
-    if table.shape[0] != rows or lens.shape[0] != rows:
-        raise QGemmError(-3, "table and lens must have one row per query")
+    pt, (table_rows, width) = _table(table, index), table.shape
+    if table_rows != rows:
+        raise QGemmError(-3, "table must have one row per query")
+    pl = _vector(lens, rows, "lens", index)
     if not 0 <= window < 1 << 31:
         raise QGemmError(-1, "paged_attention: window must not be negative")
     dt = _code(_x_codes, q.dtype, "queries")
     if out is None:
-        out = _on(stream, _torch.empty, shape, dtype=out_dtype or q.dtype, device=d)
-    elif out.shape != shape or not out.is_contiguous() or out.device != d:
-        raise QGemmError(-1, f"out must be a contiguous [{rows}, {heads}, {dim}] tensor on {d}")
+        if out_dtype is None and q.is_contiguous():
+            out = _on(stream, _torch.empty_like, q)
+        else:
+            out = _on(stream, _torch.empty, shape, dtype=out_dtype or q.dtype, device=q.device)
+    elif out.shape != shape or not out.is_contiguous() or out.get_device() != index:
+        raise QGemmError(-1, f"out must be a contiguous [{rows}, {heads}, {dim}] tensor on GPU {index}")
     odt = _code(_x_codes, out.dtype, "out")
     q = _rows16(q, stream)
-    lse = _on(stream, _torch.empty, (rows, heads), dtype=_torch.float32, device=d) if return_lse else None
+    lse = _on(stream, _torch.empty, (rows, heads), dtype=_float32, device=q.device) if return_lse else None
     nb = ctypes.c_size_t()
     qgemm._check(lib.mlxr_paged_attention_workspace_size(c, rows, heads, width, ctypes.byref(nb)))
     nb = nb.value
-    ws = _on(stream, _torch.empty, nb, dtype=_torch.uint8, device=d) if nb else None
+    ws = _on(stream, _torch.empty, nb, dtype=_torch.uint8, device=q.device) if nb else None
     qs = q.stride()
     qgemm._check(lib.mlxr_paged_attention(c, rows, heads, q.data_ptr(), dt, qs[0], qs[1], pt, table.stride()[0], width, pl,
                                           dim ** -0.5 if scale is None else scale, window, out.data_ptr(), odt,
-                                          lse.data_ptr() if return_lse else None, ws.data_ptr() if nb else None, nb, _stream(stream, d.index)))
+                                          lse.data_ptr() if return_lse else None, ws.data_ptr() if nb else None, nb, _stream(stream, index)))
     return (out, lse) if return_lse else out
 
 

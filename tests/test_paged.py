@@ -97,9 +97,7 @@ def test_wrapper_refusals():
     import torch
     t = torch.zeros((2, 3), dtype=torch.int32)
     one = torch.zeros(1, dtype=torch.int32)
-    with pytest.raises(mx.QGemmError, match="int32"):
-        mx.page_resize(t.long(), one, one, one, one, 16, 1)
-    with pytest.raises(mx.QGemmError, match="on the table's GPU"):
+    with pytest.raises(mx.QGemmError, match="on a GPU"):
         mx.page_resize(t, one, one, one, one, 16, 1)
     k = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
     q = torch.zeros((2, 8, 64), dtype=torch.bfloat16)
@@ -722,3 +720,45 @@ def test_paged_cache_class(cuda):
             _check(got, ref, values, want, "f32")
         assert c.lens.tolist() == want and n == sum(max(0, w - b) for w, b in zip(want, before))
         assert int(c.free_count) == 12 - sum(-(-w // page) for w in want)
+
+
+@pytest.mark.gpu
+def test_wrapper_refusals_on_the_gpu(cuda):
+    import torch
+    i32 = dict(dtype=torch.int32, device=cuda)
+    t, two, one = torch.zeros((2, 3), **i32), torch.zeros(2, **i32), torch.ones(1, **i32)
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16, device=cuda)
+    q = torch.zeros((2, 8, 64), dtype=torch.bfloat16, device=cuda)
+
+    def refused(match, code, call, *args, **kw):
+        with pytest.raises(mx.QGemmError, match=match) as e:
+            call(*args, **kw)
+        assert e.value.code == code
+    refused("table must", -1, mx.page_resize, t.long(), two, two, one, one, 16, 1)
+    refused("table must", -1, mx.page_resize, t.t(), two, two, one, one, 16, 1)
+    refused("lens must", -3, mx.page_resize, t, one, two, one, one, 16, 1)
+    refused("want must", -1, mx.page_resize, t, two, two.float(), one, one, 16, 1)
+    refused("want must", -1, mx.page_resize, t, two, two.cpu(), one, one, 16, 1)
+    refused("free_count must", -3, mx.page_resize, t, two, two, one, two, 16, 1)
+    refused("tokens must not", -1, mx.page_resize, t, two, two, one, one, 16, -1)
+    refused("page_size must", -1, mx.page_resize, t, two, two, one, one, 0, 1)
+    refused("queries must be", -3, mx.paged_attention, q[..., :32], k, k, t, two)
+    refused("on the cache's GPU", -1, mx.paged_attention, q.cpu(), k, k, t, two)
+    refused("must have the cache's type", -1, mx.paged_attention, q.half(), k, k, t, two)
+    refused("unsupported dtype", -1, mx.paged_attention, q, k.float(), k.float(), t, two)
+    refused("one row per query", -3, mx.paged_attention, q, k, k, t[:1], two)
+    refused("lens must", -3, mx.paged_attention, q, k, k, t, one)
+    refused("multiple of kv_heads", -3, mx.paged_attention, q[:, :7], k, k, t, two)
+    refused("window must not", -1, mx.paged_attention, q, k, k, t, two, window=-1)
+    refused("window must not", -1, mx.paged_attention, q, k, k, t, two, window=1 << 32)
+    refused("out must be", -1, mx.paged_attention, q, k, k, t, two, out=q[:1])
+    refused("k_scale must", -3, mx.paged_attention, q, k, k, t, two, k_scale=torch.ones(3, device=cuda))
+    refused("last dimension", -3, mx.paged_attention, q, k.transpose(2, 3), k.transpose(2, 3), t, two)
+    refused("keys and values must be", -3, mx.paged_append, q, q, k, k, two)
+    refused("one dtype", -1, mx.paged_append, q[:, :2], q[:, :2].float(), k, k, two)
+    refused("slots must", -3, mx.paged_append, q[:, :2], q[:, :2], k, k, one)
+    odd = torch.zeros(4 * 2 * 16 * 64 + 1, dtype=torch.bfloat16, device=cuda)[1:].view(4, 2, 16, 64)
+    refused("multiples of 16 bytes", -1, mx.paged_attention, q, odd, odd, t, two)
+    empty = mx.paged_attention(q[:0], k, k, t[:0], two[:0])
+    assert empty.shape == (0, 8, 64)
+    mx.paged_append(q[:0, :2], q[:0, :2], k, k, two[:0])

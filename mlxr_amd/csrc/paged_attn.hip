@@ -112,7 +112,7 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int64_t most) {
   const int64_t units = (int64_t)rows * c->kv_heads * p.groups;
   const int64_t bytes = 2 * most * c->head_dim * (c->dtype == MLXR_E4M3 ? 1 : 2);
   p.one = bytes <= 256 << 10 || (bytes <= 1 << 20 && units >= 256) || rows > kMaxCutRows ||
-          (most / kTile + 1) * rows > INT32_MAX;  // what a cut launch counts in 32 bits
+          (most / kTile + 1) * rows > INT32_MAX || (most / kTile + 1) * units / 64 > INT32_MAX;  // what a cut launch counts in 32 bits
   p.bytes = p.one ? 0 : prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * kWaves * 2 *
                                                  partial_floats(p.part_rows, c->head_dim) * sizeof(float);
   return p;

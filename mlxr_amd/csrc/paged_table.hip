@@ -57,7 +57,7 @@ __device__ __forceinline__ int row_of(const int* first, int n, int k) {
   return lo;
 }
 
-__device__ __forceinline__ int pages_of(const ResizeArgs& a, int tokens) { return a.by_page.quotient(tokens + a.page - 1); }
+__device__ __forceinline__ int pages_of(const ResizeArgs& a, int tokens) { return tokens ? a.by_page.quotient(tokens - 1) + 1 : 0; }
 
 // With P(n) = ceil(n / page): row r takes need = P(want) - P(lens) pages or gives back as many, and the
 // exclusive sums of both over the rows say which place of the stack each page goes to or comes
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kResizeThreads) void resize_kernel(ResizeArgs a) {
     mine.b += max(-d, 0);
   }
   Sum3 before = block_scan(mine, &total, part);
-  const int given = total.b, stack = min(count + given, a.pages);
+  const int given = total.b, stack = count + min(given, a.pages - count);
   int taken = 0;
   mine = {0, 0, 0};
   for (int r = r0; r < r1; ++r) {
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kResizeThreads) void resize_kernel(ResizeArgs a) {
     }
   }
 
-  const int gid = blockIdx.x * nt + tid, gn = gridDim.x * nt;
+  const uint32_t gid = blockIdx.x * nt + tid, gn = gridDim.x * nt;
   auto given_page = [&](int k) {  // the k-th page given back
     const int r = row_of(first_give, a.rows, k);
     return a.table[r * a.stride + pages_of(a, want[r]) + (k - first_give[r])];
@@ -139,9 +139,10 @@ __global__ __launch_bounds__(kResizeThreads) void resize_kernel(ResizeArgs a) {
     const int p = stack - 1 - k;
     return p < count ? a.free[p] : given_page(p - count);
   };
-  for (int t = gid * a.run; t < a.tokens; t += gn * a.run) {
+  const uint32_t tokens = a.tokens;
+  for (uint32_t t = gid * a.run; t < tokens; t += gn * a.run) {
     int r = -1, j = -1, id = -1;
-    for (int at = t; at < min(t + a.run, a.tokens); ++at) {
+    for (int at = (int)t, end = (int)min(t + a.run, tokens); at < end; ++at) {
       int slot = -1, pos = -1;
       if (at < new_tokens) {
         if (r < 0 || (r + 1 < a.rows && first_new[r + 1] <= at)) {
@@ -161,11 +162,11 @@ __global__ __launch_bounds__(kResizeThreads) void resize_kernel(ResizeArgs a) {
     }
   }
   // from the far end of the launch, so that these are other workgroups than the next loop's
-  for (int k = gn - 1 - gid; k < all_taken; k += gn) {
+  for (uint32_t k = gn - 1 - gid; k < (uint32_t)all_taken; k += gn) {
     const int r = row_of(first_need, a.rows, k);
     a.table[r * a.stride + held[r] + (k - first_need[r])] = taken_page(k);
   }
-  for (int k = gid; k < given && count + k < a.pages; k += gn) a.free[count + k] = given_page(k);
+  for (uint32_t k = gid; k < (uint32_t)(stack - count); k += gn) a.free[count + k] = given_page((int)k);
 }
 
 struct AppendSide {

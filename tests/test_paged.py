@@ -195,6 +195,27 @@ def test_resize_equals_the_definition(cuda, rows, width, page, pages, tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page,pages,width", [(2 ** 31 - 1, 1, 1), (2 ** 30, 1, 1), (1, 2000, 2000)])
+def test_resize_at_the_ends_of_the_page_sizes(cuda, page, pages, width):
+    """A page of all the tokens that 32 bits count, and pages of one token."""
+    import torch
+    most = width * page
+    table = torch.full((1, width), -1, dtype=torch.int32, device=cuda)
+    free = torch.arange(pages, dtype=torch.int32, device=cuda)
+
+    def i32(*v):
+        return torch.tensor(v, dtype=torch.int32, device=cuda)
+    r = mx.page_resize(table, i32(0), i32(most), free, i32(pages), page, 3)
+    assert r.lens.tolist() == [most] and r.free_count.tolist() == [0] and r.refused.tolist() == [0]
+    assert r.starts.tolist() == [0, most] and r.positions.tolist() == [0, 1, 2]
+    assert r.slots.tolist() == ([0, 1, 2] if page > 1 else [pages - 1, pages - 2, pages - 3])
+    r = mx.page_resize(table, r.lens, i32(1), free, r.free_count, page, 3)
+    assert r.lens.tolist() == [1] and r.free_count.tolist() == [pages - 1] and r.slots.tolist() == [-1] * 3
+    r = mx.page_resize(table, r.lens, i32(0), free, r.free_count, page, 0)
+    assert r.lens.tolist() == [0] and sorted(free.tolist()) == list(range(pages)) and r.free_count.tolist() == [pages]
+
+
+@pytest.mark.gpu
 def test_resize_of_no_rows(cuda):
     import torch
     i32 = dict(dtype=torch.int32, device=cuda)

@@ -21,7 +21,7 @@
 extern "C" {
 #endif
 
-enum { MLXR_LORA_MAX_ADAPTERS = 4096, MLXR_LORA_MAX_RANK = 128, MLXR_LORA_MAX_TOKENS = 1 << 20 };
+enum { MLXR_LORA_MAX_ADAPTERS = 4096, MLXR_LORA_MAX_RANK = 128, MLXR_LORA_MAX_TOKENS = 1 << 20, MLXR_LORA_MAX_SIZE = 1 << 28 };
 
 typedef struct mlxr_lora_item {
   const void* a_dev; /* [adapters, rank, K] of x's type, contiguous */
@@ -36,7 +36,7 @@ int mlxr_lora_workspace_size(int count, const mlxr_lora_item* items, int tokens,
                              size_t* bytes);
 
 /* x_dev [tokens, K] of x_dtype (MLXR_F16 / MLXR_BF16), row stride x_stride elements; K and x_stride
- * multiples of 8, rank a multiple of 8 up to MLXR_LORA_MAX_RANK; x, A and B at multiples of 16 bytes.
+ * multiples of 8, K and N up to MLXR_LORA_MAX_SIZE, rank a multiple of 8 up to MLXR_LORA_MAX_RANK; x, A and B at multiples of 16 bytes.
  *   ids_dev     [tokens] int32
  *   scales_dev  [adapters] fp32 or NULL (1)
  *   ranks_dev   [adapters] int32 or NULL (rank): rank of each adapter, up to `rank`; what A and B hold

@@ -5,8 +5,8 @@
 // Tokens of one adapter are brought together in tiles, the columns of the matrix instructions; the
 // adapter's rows of A and B are their other operand, read once for a tile.  The first launch
 // computes h, K split over workgroups (fp32 partial sums in the workspace); the second adds the
-// partial sums up, multiplies with B and adds y.  Up to kInline tokens, each workgroup finds its
-// tile among the ids by itself; above, a launch before sorts the tokens.
+// partial sums up, multiplies with B and adds y.  Up to kInline tokens, each workgroup of the first
+// finds its tile among the ids by itself; above, a launch before sorts the tokens.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,14 +31,14 @@ constexpr int kInline = kThreads;  // tokens
 constexpr int kSub = 4;
 constexpr int shrink_sub(int rank_groups, int sub) { return sub == 1 || rank_groups > 4 ? 1 : 2; }
 constexpr int rank_groups_of(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
-// Most splits of K.  Expand reads h for each of its workgroups, so of many tokens few parts (2048 tokens, rank
-// 32: shrink and expand 14 + 65 us with four, 21 + 63 with one).
-constexpr int max_splits(bool few_tokens) { return few_tokens ? 8 : 4; }
+constexpr int kSplits = 8;  // most splits of K
 constexpr int kPlanThreads = 1024;
-constexpr int kExpandGroups = 2048;  // workgroups of expand: eight for each CU
+constexpr int kExpandGroups = 1536;  // workgroups of expand: six for each CU
 
-struct Tile {
-  int adapter, first, count;  // tokens order[first .. first + count)
+// A tile's adapter (number `adapters`: none), its rank and scale; `count` tokens, order[16 SUB index ..] (0: no tile).
+struct __attribute__((aligned(16))) Tile {
+  int adapter, count, rank;
+  float scale;
 };
 struct LoraArgs {
   mlxr_lora_item item[kItems];
@@ -46,15 +46,15 @@ struct LoraArgs {
   int64_t x_stride;
   const int32_t *ids, *ranks;
   const float* scales;
-  int32_t* order;   // [tokens]
-  int32_t* counts;  // tiles with an adapter, all tiles
+  int32_t* order;  // a tile's tokens, in places of its own
   Tile* tiles;
   float* h;  // [count][splits][tokens][rank]
-  int count, tokens, K, adapters, rank, splits, chunk, columns;
+  int count, tokens, K, adapters, rank, splits, chunk, columns, most_tiles;
 };
 
-__device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
-  return a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank;
+__device__ __forceinline__ Tile tile_of(const LoraArgs& a, int adapter, int count) {
+  if (adapter == a.adapters) return {adapter, count, 0, 0.f};
+  return {adapter, count, a.ranks ? min(max(a.ranks[adapter], 0), a.rank) : a.rank, a.scales ? a.scales[adapter] : 1.f};
 }
 
 // counter[b] + 1 for each active lane with its own b; returns a place of its own, as atomicAdd would.
@@ -76,112 +76,123 @@ __device__ __forceinline__ int wave_add(int* counter, int b) {
   return at;
 }
 
-// Tokens sorted by adapter, and the tiles; the last bucket holds the tokens without one.
+// Tokens sorted by adapter, in tiles; the last bucket holds the tokens without one.
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   extern __shared__ int sh[];
-  const int TM = 16 * kSub, nb = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int TM = 16 * kSub, AHEAD = 4;  // ids of a thread on their way at once
+  const int nb = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int *count = sh, *next = sh + nb;
-  __shared__ int part[2 * kPlanThreads / 64];
+  __shared__ int part[kPlanThreads / 64];
   for (int b = tid; b < nb; b += kPlanThreads) count[b] = 0;
   __syncthreads();
-  auto bucket = [&](int t) {
-    const int id = a.ids[t];
-    return id >= 0 && id < a.adapters ? id : a.adapters;
+  auto each = [&](auto&& f) {
+    for (int t0 = tid; t0 < a.tokens; t0 += AHEAD * kPlanThreads) {
+      int id[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) id[k] = a.ids[min(t0 + k * kPlanThreads, a.tokens - 1)];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (const int t = t0 + k * kPlanThreads; t < a.tokens) f(t, id[k] >= 0 && id[k] < a.adapters ? id[k] : a.adapters);
+    }
   };
   // one atomic for the lanes of a wavefront that share a bucket: neighbouring tokens often do
-  for (int t = tid; t < a.tokens; t += kPlanThreads) {
-    const int b = bucket(t);
-    wave_add(count, b);
-  }
+  each([&](int, int b) { wave_add(count, b); });
   __syncthreads();
   const int per = (nb + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, nb), b1 = min(b0 + per, nb);
-  int n = 0, m = 0;
-  for (int b = b0; b < b1; ++b) n += count[b], m += (count[b] + TM - 1) / TM;
-  int sn = n, sm = m;
+  int m = 0;
+  for (int b = b0; b < b1; ++b) m += (count[b] + TM - 1) / TM;
+  int sum = m;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
-    const int u = __shfl_up(sn, d), v = __shfl_up(sm, d);
-    if (lane >= d) sn += u, sm += v;
+    const int v = __shfl_up(sum, d);
+    if (lane >= d) sum += v;
   }
-  if (lane == 63) part[2 * wave] = sn, part[2 * wave + 1] = sm;
+  if (lane == 63) part[wave] = sum;
   __syncthreads();
-  int at = sn - n, tile = sm - m;
-  for (int w = 0; w < wave; ++w) at += part[2 * w], tile += part[2 * w + 1];
+  int tile = sum - m, all = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wave) tile += part[w];
+    all += part[w];
+  }
   for (int b = b0; b < b1; ++b) {
     const int c = count[b];
-    next[b] = at;
-    if (b == a.adapters) {
-      a.counts[0] = tile;
-      a.counts[1] = tile + (c + TM - 1) / TM;
+    next[b] = tile * TM;
+    Tile t = tile_of(a, b, 0);
+    for (int i = 0; i < c; i += TM) {
+      t.count = min(TM, c - i);
+      a.tiles[tile++] = t;
     }
-    for (int i = 0; i < c; i += TM) a.tiles[tile++] = {b, at + i, min(TM, c - i)};
-    at += c;
   }
+  for (int i = all + tid; i < a.most_tiles; i += kPlanThreads) a.tiles[i] = {0, 0, 0, 0.f};
   __syncthreads();
   // which place of its adapter a token gets depends on the order of the atomics; no value does
-  for (int t = tid; t < a.tokens; t += kPlanThreads) a.order[wave_add(next, bucket(t))] = t;
+  each([&](int t, int b) { a.order[wave_add(next, b)] = t; });
 }
 
-// Tile `index`: its adapter (a.adapters: none), its tokens in token[0 .. count).  count 0: there is no such
-// tile.  INLINE: every workgroup ranks the tokens among those of their adapter; tiles start at the tokens of rank 0,
-// 16, 32 .., in the order of these tokens.  Its dynamic LDS holds a counter for each adapter.
-template <bool INLINE, int WAVES>
-__device__ __forceinline__ int tile_tokens(const LoraArgs& a, int index, int* adapter, int* token) {
+// Tile `index` as planned, its tokens in token[0 .. count).
+template <int SUB>
+__device__ __forceinline__ Tile planned_tile(const LoraArgs& a, int index, int* token) {
+  const Tile t = a.tiles[index];
+  if (threadIdx.x < 16 * SUB) token[threadIdx.x] = a.order[index * 16 * SUB + threadIdx.x];
+  __syncthreads();
+  return t;
+}
+
+// Up to kInline tokens, without a plan: every workgroup ranks the tokens among those of their adapter; tiles start at
+// the tokens of rank 0, 16, 32 .., in the order of these tokens.  The dynamic LDS holds a counter for each adapter.
+template <int WAVES>
+__device__ __forceinline__ Tile found_tile(const LoraArgs& a, int index, int* token) {
   const int tid = threadIdx.x;
-  if constexpr (INLINE) {
-    extern __shared__ int seen[];
-    __shared__ uint64_t starts[WAVES];
-    __shared__ int chosen[2];
-    const int lane = tid & 63, wave = tid >> 6, waves = (a.tokens + 63) >> 6;
-    const uint64_t below = (1ull << lane) - 1;
-    int b = -1;
-    if (tid < a.tokens) {
-      b = a.ids[tid];
-      b = b >= 0 && b < a.adapters ? b : a.adapters;
-    }
-    for (int i = tid; i <= a.adapters; i += 64 * WAVES) seen[i] = 0;
-    uint64_t peers = __ballot(b >= 0);  // lanes of the same adapter, bit by bit of its number
-    for (int bit = 1; bit <= a.adapters; bit *= 2) {
-      const uint64_t set = __ballot((b & bit) != 0);
-      peers &= b & bit ? set : ~set;
-    }
-    __syncthreads();
-    int rank = -1;
-    for (int w = 0; w < waves; ++w) {
-      if (wave == w && b >= 0) {
-        const int before = seen[b];
-        rank = before + __popcll(peers & below);
-        if ((peers & below) == 0) seen[b] = before + __popcll(peers);
-      }
-      __syncthreads();
-    }
-    const bool start = b >= 0 && (rank & 15) == 0;
-    const uint64_t vote = __ballot(start);
-    if (lane == 0) starts[wave] = vote;
-    __syncthreads();
-    int at = 0, all = 0;  // starts before this token, all
-    for (int w = 0; w < waves; ++w) {
-      const int n = __popcll(starts[w]);
-      at += w < wave ? n : w == wave ? __popcll(vote & below) : 0;
-      all += n;
-    }
-    if (index >= all) return 0;
-    if (start && at == index) chosen[0] = b, chosen[1] = rank;
-    __syncthreads();
-    const int first = chosen[1];
-    *adapter = chosen[0];
-    if (b == chosen[0] && rank >= first && rank < first + 16) token[rank - first] = tid;
-    const int count = min(16, seen[chosen[0]] - first);
-    __syncthreads();
-    return count;
-  } else {
-    if (index >= a.counts[1]) return 0;
-    const Tile t = a.tiles[index];
-    if (tid < t.count) token[tid] = a.order[t.first + tid];
-    *adapter = t.adapter;
-    __syncthreads();
-    return t.count;
+  extern __shared__ int seen[];
+  __shared__ uint64_t starts[WAVES];
+  __shared__ Tile chosen;
+  __shared__ int chosen_rank;
+  const int lane = tid & 63, wave = tid >> 6, waves = (a.tokens + 63) >> 6;
+  const uint64_t below = (1ull << lane) - 1;
+  int b = -1;
+  Tile mine = {0, 0, 0, 0.f};
+  if (tid < a.tokens) {
+    b = a.ids[tid];
+    b = b >= 0 && b < a.adapters ? b : a.adapters;
+    mine = tile_of(a, b, 0);  // on its way while the tokens are ranked
   }
+  for (int i = tid; i <= a.adapters; i += 64 * WAVES) seen[i] = 0;
+  uint64_t peers = __ballot(b >= 0);  // lanes of the same adapter, bit by bit of its number
+  for (int bit = 1; bit <= a.adapters; bit *= 2) {
+    const uint64_t set = __ballot((b & bit) != 0);
+    peers &= b & bit ? set : ~set;
+  }
+  __syncthreads();
+  int rank = -1;
+  for (int w = 0; w < waves; ++w) {
+    if (wave == w && b >= 0) {
+      const int before = seen[b];
+      rank = before + __popcll(peers & below);
+      if ((peers & below) == 0) seen[b] = before + __popcll(peers);
+    }
+    __syncthreads();
+  }
+  const bool start = b >= 0 && (rank & 15) == 0;
+  const uint64_t vote = __ballot(start);
+  if (lane == 0) starts[wave] = vote;
+  __syncthreads();
+  int at = 0, all = 0;  // starts before this token, all
+  for (int w = 0; w < waves; ++w) {
+    const int n = __popcll(starts[w]);
+    at += w < wave ? n : w == wave ? __popcll(vote & below) : 0;
+    all += n;
+  }
+  if (index >= all) return {0, 0, 0, 0.f};
+  if (start && at == index) {
+    mine.count = min(16, seen[b] - rank);
+    chosen = mine, chosen_rank = rank;
+  }
+  __syncthreads();
+  const Tile t = chosen;
+  const int first = chosen_rank;
+  if (b == t.adapter && rank >= first && rank < first + 16) token[rank - first] = tid;
+  __syncthreads();
+  return t;
 }
 
 // h of SS groups of 16 tokens of a tile over one chunk of K: the wavefronts take turns over it in steps of 64
@@ -193,14 +204,22 @@ __global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
   constexpr int kWaves = kShrinkThreads / 64, SS = shrink_sub(RT, SUB);
   __shared__ int tokens[16 * SUB];
   __shared__ f32x4_t sh[kWaves - 1][SS * RT][64];
-  int adapter = 0;
-  const int all = tile_tokens<INLINE, kWaves>(a, blockIdx.x / (SUB / SS), &adapter, tokens);
-  const int sub = blockIdx.x % (SUB / SS) * SS * 16, count = min(all - sub, 16 * SS);
+  Tile tile;
+  if constexpr (INLINE) {
+    tile = found_tile<kWaves>(a, blockIdx.x, tokens);
+    if (blockIdx.y == 0 && blockIdx.z == 0) {  // for expand
+      if (threadIdx.x == 0) a.tiles[blockIdx.x] = tile;
+      if ((int)threadIdx.x < tile.count) a.order[blockIdx.x * 16 + threadIdx.x] = tokens[threadIdx.x];
+    }
+  } else {
+    tile = planned_tile<SUB>(a, blockIdx.x / (SUB / SS), tokens);
+  }
+  const int sub = blockIdx.x % (SUB / SS) * SS * 16, count = min(tile.count - sub, 16 * SS), adapter = tile.adapter;
   if (count <= 0 || adapter == a.adapters) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int split = blockIdx.y, item = blockIdx.z, rank = rank_of(a, adapter);
+  const int split = blockIdx.y, item = blockIdx.z, rank = tile.rank;
   const int k_end = min((split + 1) * a.chunk, a.K);
-  const uint16_t* A = (const uint16_t*)a.item[item].a_dev + (int64_t)adapter * a.rank * a.K + (int64_t)col * a.K;
+  const uint16_t* A = (const uint16_t*)a.item[item].a_dev + (int64_t)adapter * a.rank * a.K;
   int token[SS];
   const uint16_t* x[SS];
 #pragma unroll
@@ -209,38 +228,49 @@ __global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
     x[s] = a.x + (int64_t)token[s] * a.x_stride;
   }
   f32x4_t acc[SS][RT] = {};
-  u32x4_t xf[SS][2], af[RT][2];
-  auto load = [&](int k) {
+  // Two steps are on their way.  The loads are unconditional: ranks that the adapter has not read its first (their
+  // sums are not kept), places past the chunk its last.
+  u32x4_t xf[2][SS][2], af[2][RT][2];
+  auto load = [&](int b, int k) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int kk = k + 16 * g + 8 * e;
-      const bool in = kk < k_end;
+      const int kk = min(k + 16 * g + 8 * e, k_end - 8);
 #pragma unroll
-      for (int s = 0; s < SS; ++s) xf[s][e] = in ? *(const u32x4_t*)(x[s] + kk) : u32x4_t{0, 0, 0, 0};
+      for (int s = 0; s < SS; ++s) xf[b][s][e] = *(const u32x4_t*)(x[s] + kk);
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
-        af[r][e] = in && 16 * r + col < rank ? *(const u32x4_t*)(A + (int64_t)(16 * r) * a.K + kk) : u32x4_t{0, 0, 0, 0};
+      for (int r = 0; r < RT; ++r) af[b][r][e] = *(const u32x4_t*)(A + (int64_t)(16 * r + col < rank ? 16 * r + col : 0) * a.K + kk);
     }
   };
-  int k = split * a.chunk + wave * 64;
-  load(k);
-  while (k < k_end) {
-    u32x4_t xc[SS][2], ac[RT][2];
+  auto add = [&](int b, int k) {
+    if (k + 64 > k_end)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2; ++e) {
+        const bool in = k + 16 * g + 8 * e < k_end;
 #pragma unroll
-      for (int s = 0; s < SS; ++s) xc[s][e] = xf[s][e];
+        for (int s = 0; s < SS; ++s) xf[b][s][e] = in ? xf[b][s][e] : u32x4_t{0, 0, 0, 0};
 #pragma unroll
-      for (int r = 0; r < RT; ++r) ac[r][e] = af[r][e];
-    }
-    k += kWaves * 64;
-    load(k);  // nothing past k_end is read
+        for (int r = 0; r < RT; ++r) af[b][r][e] = in ? af[b][r][e] : u32x4_t{0, 0, 0, 0};
+      }
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int s = 0; s < SS; ++s)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) acc[s][r] = mfma16<F16>(ac[r][e], xc[s][e], acc[s][r]);
+        for (int r = 0; r < RT; ++r) acc[s][r] = mfma16<F16>(af[b][r][e], xf[b][s][e], acc[s][r]);
+  };
+  constexpr int S = kWaves * 64;
+  int k = split * a.chunk + wave * 64;
+  if (k < k_end) {
+    load(0, k);
+    load(1, k + S);
+    for (; k + 2 * S < k_end; k += 2 * S) {
+      add(0, k);
+      load(0, k + 2 * S);
+      add(1, k + S);
+      load(1, k + 3 * S);
+    }
+    add(0, k);
+    if (k + S < k_end) add(1, k + S);
   }
   if (wave)
 #pragma unroll
@@ -258,61 +288,67 @@ __global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
       f32x4_t v = acc[s][r];
 #pragma unroll
       for (int w = 0; w < kWaves - 1; ++w) v += sh[w][s * RT + r][lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = 16 * r + 4 * g + i < rank ? v[i] : 0.f;
       if (16 * r + 4 * g < a.rank) *(f32x4_t*)(h + 16 * r) = v;
     }
   }
 }
 
-// CT neighbouring columns of a token's row of y, as they lie in memory (YT: the type); rows start at multiples of
-// 16 bytes where vec.
+// CT neighbouring columns of a token's row of y, as they lie in memory (YT: the type).
 template <int YT, int CT>
 struct Cols {
   static constexpr int S = YT == DT_F32 ? 4 : 2, W = CT * S / 4;  // bytes of an element; words
   uint32_t w[W];
-  __device__ __forceinline__ void load(const mlxr_lora_item& it, int64_t at, bool in) {
-    if (!in) return;
-    const uint8_t* p = (const uint8_t*)it.y_dev + at * S;
-    if constexpr (W == 2) {
+  // other: 16 bytes that are read, and not used, where `in` is false: the load is unconditional
+  __device__ __forceinline__ void load(const mlxr_lora_item& it, int64_t at, bool in, const void* other) {
+    const uint8_t* p = in ? (const uint8_t*)it.y_dev + at * S : (const uint8_t*)other;
+    if constexpr (W == 1) {
+      w[0] = *(const uint32_t*)p;
+    } else if constexpr (W == 2) {
       const u32x2_t v = *(const u32x2_t*)p;
       w[0] = v.x, w[1] = v.y;
     } else {
 #pragma unroll
       for (int k = 0; k < W; k += 4) {
-        const u32x4_t v = *(const u32x4_t*)(p + 4 * k);
+        const u32x4_t v = *(const u32x4_t*)(p + (in ? 4 * k : 0));
         w[k] = v.x, w[k + 1] = v.y, w[k + 2] = v.z, w[k + 3] = v.w;
       }
     }
   }
-  // out = y + v * back; left: columns that the row has from here on
-  __device__ __forceinline__ void store(const mlxr_lora_item& it, int64_t at, bool in, int left, const float* v, float back) {
-    if (in) {
-      uint32_t o[W];
+  // out = y + v * back
+  __device__ __forceinline__ void store(const mlxr_lora_item& it, int64_t at, const float* v, float back) {
+    uint32_t o[W];
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        if constexpr (YT == DT_F32) o[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, w[k]) + v[k] * back);
-        else o[k] = pack2<YT == DT_F16>(unpack<YT == DT_F16>(w[k], 0) + v[2 * k] * back, unpack<YT == DT_F16>(w[k], 1) + v[2 * k + 1] * back);
-      }
-      uint8_t* p = (uint8_t*)it.out_dev + at * S;
-      if constexpr (W == 2) *(u32x2_t*)p = u32x2_t{o[0], o[1]};
-      else
-#pragma unroll
-        for (int k = 0; k < W; k += 4) *(u32x4_t*)(p + 4 * k) = u32x4_t{o[k], o[k + 1], o[k + 2], o[k + 3]};
-      return;
+    for (int k = 0; k < W; ++k) {
+      if constexpr (YT == DT_F32) o[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, w[k]) + v[k] * back);
+      else o[k] = pack2<YT == DT_F16>(unpack<YT == DT_F16>(w[k], 0) + v[2 * k] * back, unpack<YT == DT_F16>(w[k], 1) + v[2 * k + 1] * back);
     }
+    uint8_t* p = (uint8_t*)it.out_dev + at * S;
+    if constexpr (W == 1) *(uint32_t*)p = o[0];
+    else if constexpr (W == 2) *(u32x2_t*)p = u32x2_t{o[0], o[1]};
+    else
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
-      if (c < left) store_scalar(it.out_dev, YT, at + c, load_scalar(it.y_dev, YT, at + c) + v[c] * back);
+      for (int k = 0; k < W; k += 4) *(u32x4_t*)(p + 4 * k) = u32x4_t{o[k], o[k + 1], o[k + 2], o[k + 3]};
   }
 };
 
 // Columns of a wavefront's step, in units of 16: 64 for few tokens (more workgroups), 128 for many: 256 bytes of a
-// row in one store of 16-bit outputs (2048 tokens, two projections of 14336, rank 32: 62 -> 55 us); not where B's
-// operands then leave few wavefronts on a SIMD (rank 64: 128 us, 111).
-constexpr int columns_of(int sub, int rank_groups) { return sub == 1 || rank_groups > 2 ? 4 : 8; }
+// row in one store of 16-bit outputs (2048 tokens, two projections of 14336, rank 32: 62 -> 55 us); fewer where B's
+// operands leave few wavefronts on a SIMD (us, with more and with fewer: 2048 tokens of rank 64 128 and 111; rank 128,
+// 64 tokens of 16 adapters, K 4096, two projections of 14336: 64 columns 61, 32 49).
+constexpr int columns_of(int sub, int rank_groups) { return rank_groups == 8 ? 2 : sub == 1 || rank_groups == 4 ? 4 : 8; }
+
+// The bits of x that bf16 has, in the upper half; NaN (whose upper bits may be those of an infinity) quieted.
+__device__ __forceinline__ uint32_t cut_bf16(float x) {
+  return (__builtin_bit_cast(uint32_t, x) | (x != x ? 0x400000u : 0u)) & 0xffff0000u;
+}
 
 // 8 ranks at .. of token t of a tile into LDS as high and low 16-bit parts: rounded to one part h would lose what the
-// fp32 sums kept.  In f16, whose range h may leave, relative to a power of two that brings the token's largest to
-// [1/2, 1), the reciprocal in back[t]; the 2 RT threads of a token are neighbours.
+// fp32 sums kept.  The high part is cut, not rounded, and the low one never 0 beside it nor of the other sign, so that
+// an infinite element of B gives an infinity as h in one piece does, not NaN (the least low part is 2^-24 of the token's
+// largest, or 2^-126).  In f16, whose range h may leave, relative to a power of two that brings the token's
+// largest to [1/2, 1), the reciprocal in back[t]; the 2 RT threads of a token are neighbours.
 template <bool F16, int RT>
 __device__ __forceinline__ void split_h(f32x4_t (&v)[2], float scale, int t, int at, uint16_t* row, float* back) {
   constexpr int R = 16 * RT;
@@ -331,13 +367,17 @@ __device__ __forceinline__ void split_h(f32x4_t (&v)[2], float scale, int t, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = __builtin_amdgcn_ldexpf(v[i >> 2][i & 3], -e);
   }
+  auto low = [](float x, float high) {
+    if (!(fabsf(x) < INFINITY) || x == 0.f) return 0.f;  // an infinite h stays infinite, NaN stays NaN
+    return copysignf(fmaxf(fabsf(x - high), F16 ? 0x1p-24f : 0x1p-126f), x);
+  };
   u32x4_t hi, lo;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float v0 = v[e >> 1][2 * (e & 1)], v1 = v[e >> 1][2 * (e & 1) + 1];
-    hi[e] = pack2<F16>(v0, v1);
-    const float d0 = v0 - unpack<F16>(hi[e], 0), d1 = v1 - unpack<F16>(hi[e], 1);
-    lo[e] = pack2<F16>(d0 == d0 ? d0 : 0.f, d1 == d1 ? d1 : 0.f);  // an infinite h stays infinite
+    if constexpr (F16) hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v0, v1));
+    else hi[e] = cut_bf16(v0) >> 16 | cut_bf16(v1);
+    lo[e] = pack2<F16>(low(v0, unpack<F16>(hi[e], 0)), low(v1, unpack<F16>(hi[e], 1)));
   }
   *(u32x4_t*)(row + at) = hi;
   *(u32x4_t*)(row + R + at) = lo;
@@ -354,35 +394,36 @@ struct Expand {
   const LoraArgs& a;
   const mlxr_lora_item& it;
   const uint16_t* B;
-  int rank, n0, end, col, g;
+  int rank, ld, n0, end, col, g;
   u32x4_t next[KT][CT];  // operands of B for a step, on their way while h or the columns before are computed
 
-  __device__ __forceinline__ Expand(const LoraArgs& a_, const mlxr_lora_item& it_, int adapter, int rank_, int begin)
-      : a(a_), it(it_), B((const uint16_t*)it_.b_dev + (int64_t)adapter * it_.N * a_.rank), rank(rank_) {
+  __device__ __forceinline__ Expand(const LoraArgs& a_, const mlxr_lora_item& it_, const Tile& t, int begin)
+      : a(a_), it(it_), B((const uint16_t*)it_.b_dev + (t.adapter == a_.adapters ? 0 : (int64_t)t.adapter * it_.N * a_.rank)),
+        rank(t.rank), ld(t.rank ? a_.rank : 0) {
     const int lane = threadIdx.x & 63;
     col = lane & 15, g = lane >> 4;
     n0 = begin + (threadIdx.x >> 6) * 16 * CT;
     end = min(begin + a.columns, it.N);
-    load_b(n0);
+    load_b(n0, n0 < end);
   }
-  // RT 1 multiplies the high and the low parts in one product, ranks 8 (g & 1) ..
-  __device__ __forceinline__ void load_b(int n0) {
+  // RT 1 multiplies the high and the low parts in one product, ranks 8 (g & 1) ..  The loads are unconditional, so that
+  // they stay in flight: what a column or rank that is not there gets lies in a row that is read anyway.
+  __device__ __forceinline__ void load_b(int n0, bool more) {
+    const int ld = more ? this->ld : 0;
 #pragma unroll
     for (int k = 0; k < KT; ++k)
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        const int n = n0 + CT * col + c, at = RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g, left = rank - at;
-        next[k][c] = n < it.N && left > 0 ? *(const u32x4_t*)(B + (int64_t)n * a.rank + at) : u32x4_t{0, 0, 0, 0};
-        if (left < 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) next[k][c][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
+        const int n = min(n0 + CT * col + c, it.N - 1), at = rank_at(k);
+        next[k][c] = *(const u32x4_t*)(B + (int64_t)n * ld + (at < rank ? at : 0));
       }
   }
-  // hs: the tile's rows of h; none: the tokens have no adapter
-  template <int YT>
+  __device__ __forceinline__ int rank_at(int k) const { return RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g; }
+  // hs: the tile's rows of h; none: the tokens have no adapter.  VEC: rows of y and out start at multiples of 16
+  // bytes and are whole groups of CT columns.
+  template <int YT, bool VEC>
   __device__ __forceinline__ void columns(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
-    constexpr bool AHEAD = SUB > 1 && YT != DT_F32;  // y of the next 16 tokens on its way: fp32 has no registers for it
-    const bool vec = it.N * Cols<YT, CT>::S % 16 == 0 && (((uintptr_t)it.y_dev | (uintptr_t)it.out_dev) & 15) == 0;
+    constexpr bool AHEAD = VEC && SUB > 1 && YT != DT_F32;  // y of the next 16 tokens on its way: fp32 has no registers for it
     for (; n0 < end; n0 += STEP) {
       u32x4_t bf[KT][CT];
 #pragma unroll
@@ -390,20 +431,32 @@ struct Expand {
 #pragma unroll
         for (int c = 0; c < CT; ++c) bf[k][c] = next[k][c];
       const int n = n0 + CT * col, left = it.N - n;
-      const bool in = vec && left >= CT;
       Cols<YT, CT> y[4];
       auto load_y = [&](Cols<YT, CT>(&to)[4], int s) {
+        if constexpr (VEC)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 16 * s + 4 * g + i;
-          to[i].load(it, (int64_t)token[t < count ? t : 0] * it.N + n, in && t < count);
-        }
+          for (int i = 0; i < 4; ++i) {
+            const int t = 16 * s + 4 * g + i;
+            to[i].load(it, (int64_t)token[t < count ? t : 0] * it.N + n, left > 0 && t < count, B);
+          }
       };
       load_y(y, 0);
-      if (n0 + STEP < end) load_b(n0 + STEP);
+      asm volatile("" ::: "memory");  // the loads stay in this order: what waits for y would wait for those before it too
+      load_b(n0 + STEP, n0 + STEP < end);
+      if (rank < R)  // nothing of ranks that the adapter has not
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+          const int past = rank - rank_at(k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t mask = past >= 2 * e + 2 ? ~0u : past > 2 * e ? 0xffffu : 0u;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) bf[k][c][e] &= mask;
+          }
+        }
 #pragma unroll 1
       for (int s = 0; s < SUB; ++s) {
-        if (16 * s >= count) break;
+        if (SUB > 1 && 16 * s >= count) break;
         Cols<YT, CT> y_next[4];
         if (AHEAD && 16 * (s + 1) < count) load_y(y_next, s + 1);
         f32x4_t acc[CT] = {};
@@ -429,10 +482,18 @@ struct Expand {
         for (int i = 0; i < 4; ++i) {
           const int t = 16 * s + 4 * g + i;
           if (t >= count || left <= 0) continue;
-          float v[CT];
+          const int64_t at = (int64_t)token[t] * it.N + n;
+          const float f = F16 && !none ? back[t] : 1.f;
+          if constexpr (VEC) {
+            float v[CT];
 #pragma unroll
-          for (int c = 0; c < CT; ++c) v[c] = acc[c][i];
-          y[i].store(it, (int64_t)token[t] * it.N + n, in, left, v, F16 && !none ? back[t] : 1.f);
+            for (int c = 0; c < CT; ++c) v[c] = acc[c][i];
+            y[i].store(it, at, v, f);
+          } else {
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+              if (c < left) store_scalar(it.out_dev, YT, at + c, load_scalar(it.y_dev, YT, at + c) + acc[c][i] * f);
+          }
         }
         if constexpr (AHEAD) {
 #pragma unroll
@@ -443,6 +504,12 @@ struct Expand {
       }
     }
   }
+  template <int YT>
+  __device__ __forceinline__ void columns(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
+    const bool vec = it.N % CT == 0 && it.N * (YT == DT_F32 ? 4 : 2) % 16 == 0 && (((uintptr_t)it.y_dev | (uintptr_t)it.out_dev) & 15) == 0;
+    if (vec) columns<YT, true>(token, count, none, hs, back);
+    else columns<YT, false>(token, count, none, hs, back);
+  }
   __device__ __forceinline__ void run(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
     if (it.y_dtype == DT_BF16) columns<DT_BF16>(token, count, none, hs, back);
     else if (it.y_dtype == DT_F16) columns<DT_F16>(token, count, none, hs, back);
@@ -451,41 +518,38 @@ struct Expand {
 };
 
 // One tile and a.columns columns of an item, h from the workspace.
-template <bool F16, int RT, int SUB, bool INLINE>
-__global__ __launch_bounds__(kThreads) void expand_kernel(LoraArgs a) {
-  constexpr int kMost = max_splits(INLINE);
+template <bool F16, int RT, int SUB>
+__global__ __launch_bounds__(kThreads, RT <= 4 && SUB == 1 ? 3 : 1) void expand_kernel(LoraArgs a) {
   __shared__ int token[16 * SUB];
   __shared__ float back[16 * SUB];
   __shared__ __attribute__((aligned(16))) uint16_t hs[16 * SUB * h_row(RT)];
   const mlxr_lora_item& it = a.item[blockIdx.z];
   const int begin = blockIdx.x * a.columns;
   if (begin >= it.N) return;
-  int adapter = 0;
-  const int count = tile_tokens<INLINE, kWaves>(a, blockIdx.y, &adapter, token);
+  const Tile tile = planned_tile<SUB>(a, blockIdx.y, token);
+  const int count = tile.count, rank = tile.rank;
   if (count == 0) return;
-  const bool none = adapter == a.adapters;
+  const bool none = tile.adapter == a.adapters;
   if (none && it.out_dev == it.y_dev) return;
-  const int rank = none ? 0 : rank_of(a, adapter);
-  Expand<F16, RT, SUB, kWaves> e(a, it, none ? 0 : adapter, rank, begin);
+  Expand<F16, RT, SUB, kWaves> e(a, it, tile, begin);
   if (!none) {
-    const float scale = a.scales ? a.scales[adapter] : 1.f;
     for (int u = threadIdx.x; u < 16 * SUB * 2 * RT; u += kThreads) {
       const int t = u / (2 * RT), at = 8 * (u % (2 * RT));
       f32x4_t v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
       if (t < count && at < rank) {
         const float* p = a.h + ((int64_t)blockIdx.z * a.splits * a.tokens + token[t]) * a.rank + at;
         const int64_t step = (int64_t)a.tokens * a.rank;
-        f32x4_t in[kMost][2];
+        f32x4_t in[kSplits][2];
 #pragma unroll
-        for (int s = 0; s < kMost; ++s)
+        for (int s = 0; s < kSplits; ++s)
 #pragma unroll
           for (int k = 0; k < 2; ++k) in[s][k] = s < a.splits ? *(const f32x4_t*)(p + s * step + 4 * k) : f32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < kMost; ++s)
+        for (int s = 0; s < kSplits; ++s)
 #pragma unroll
           for (int k = 0; k < 2; ++k) v[k] += in[s][k];
       }
-      split_h<F16, RT>(v, scale, t, at, hs + t * h_row(RT), back);
+      split_h<F16, RT>(v, tile.scale, t, at, hs + t * h_row(RT), back);
     }
     __syncthreads();
   }
@@ -504,16 +568,15 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
   const mlxr_lora_item& it = a.item[blockIdx.z];
   const int begin = blockIdx.x * a.columns;
   if (begin >= it.N) return;
-  int adapter = 0;
-  const int count = tile_tokens<true, WAVES>(a, blockIdx.y, &adapter, token);
+  const Tile tile = found_tile<WAVES>(a, blockIdx.y, token);
+  const int count = tile.count, rank = tile.rank;
   if (count == 0) return;
-  const bool none = adapter == a.adapters;
+  const bool none = tile.adapter == a.adapters;
   if (none && it.out_dev == it.y_dev) return;
-  const int rank = none ? 0 : rank_of(a, adapter);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  Expand<F16, RT, 1, WAVES> e(a, it, none ? 0 : adapter, rank, begin);
+  Expand<F16, RT, 1, WAVES> e(a, it, tile, begin);
   if (!none) {
-    const uint16_t* A = (const uint16_t*)it.a_dev + (int64_t)adapter * a.rank * a.K + (int64_t)col * a.K;
+    const uint16_t* A = (const uint16_t*)it.a_dev + (int64_t)tile.adapter * a.rank * a.K + (int64_t)col * a.K;
     const uint16_t* x = a.x + (int64_t)token[col < count ? col : 0] * a.x_stride;
     f32x4_t acc[RT] = {};
     for (int k0 = wave * 64; k0 < a.K; k0 += WAVES * U * 64) {
@@ -546,7 +609,7 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
       for (int w = 0; w < WAVES; ++w)
 #pragma unroll
         for (int k = 0; k < 2; ++k) v[k] += sh[w][part >> 1][(2 * (part & 1) + k) * 16 + t];
-      split_h<F16, RT>(v, a.scales ? a.scales[adapter] : 1.f, t, 8 * part, hs + t * h_row(RT), back);
+      split_h<F16, RT>(v, tile.scale, t, 8 * part, hs + t * h_row(RT), back);
     }
     __syncthreads();
   }
@@ -556,7 +619,7 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
 struct Layout {
   bool fused;
   int tiles, splits, chunk, columns;  // most tiles that the call may have; splits of K; columns of a workgroup
-  size_t order, counts, tile, h, bytes;
+  size_t order, tile, h, bytes;
 };
 Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int adapters, int rank) {
   Layout l{};
@@ -577,13 +640,17 @@ Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int a
     l.columns = kFusedThreads;
     return l;
   }
-  // enough workgroups for the device; a wavefront takes two steps of K or more
   const bool sorted = tokens > kInline;
   const int group = sorted ? 16 * shrink_sub(groups, kSub) : 16;
-  const long want = 512 / ((long)std::min(tokens, tokens / group + buckets) * items) + 1;
-  const int most = std::min(max_splits(!sorted), (K + 511) / 512);
+  // As many splits as the device holds workgroups of shrink at once (two on a CU up to rank 32, else one; a quarter more
+  // for sorted tokens, whose adapters' last tiles are partly empty), in chunks of whole steps of the workgroup, two at least.
+  // us, at once / twice that / half: 64 tokens of 16 adapters of rank 128, K 8192, three projections of 10240 together
+  // 62 / 65 / -; 16 tokens of rank 64 there 27 / 28 / -; rank 64, K 28672, 8192, 33 / - / 46; 2048 tokens of 6
+  // adapters of rank 32, K 4096, two of 14336, 66 / 66 / 71.
+  const long want = std::max(1L, 256L * (groups <= 2 ? 2 : 1) * (sorted ? 5 : 4) / 4 / ((long)std::min(tokens, tokens / group + buckets) * items));
+  const int most = std::min(kSplits, (K + 1023) / 1024);
   int splits = (int)(want < most ? want : most);
-  l.chunk = ((K + splits - 1) / splits + 63) / 64 * 64;
+  l.chunk = ((K + splits - 1) / splits + kShrinkThreads - 1) / kShrinkThreads * kShrinkThreads;
   l.splits = (K + l.chunk - 1) / l.chunk;
   // columns of a workgroup of expand: several steps where that leaves enough workgroups, so that what a
   // workgroup does first (its tile, h) is paid less often
@@ -592,8 +659,7 @@ Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int a
   l.columns = step * (int)std::max(1L, std::min(16L, steps));
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   l.order = 0;
-  l.counts = up((size_t)tokens * 4);
-  l.tile = l.counts + 256;
+  l.tile = up((size_t)l.tiles * tm * 4);
   l.h = l.tile + up((size_t)l.tiles * sizeof(Tile));
   l.bytes = l.h + (size_t)items * l.splits * tokens * rank * 4;
   return l;
@@ -609,7 +675,7 @@ void launch(const LoraArgs& a, int tiles, hipStream_t s) {
   const int wide = widest(a);
   const size_t lds = INLINE ? (size_t)(a.adapters + 1) * sizeof(int) : 0;
   shrink_kernel<F16, RT, SUB, INLINE><<<dim3(tiles * (SUB / shrink_sub(RT, SUB)), a.splits, a.count), kShrinkThreads, lds, s>>>(a);
-  expand_kernel<F16, RT, SUB, INLINE><<<dim3((wide + a.columns - 1) / a.columns, tiles, a.count), kThreads, lds, s>>>(a);
+  expand_kernel<F16, RT, SUB><<<dim3((wide + a.columns - 1) / a.columns, tiles, a.count), kThreads, 0, s>>>(a);
 }
 template <bool F16, int RT>
 void launch_tokens(const LoraArgs& a, const Layout& l, hipStream_t s) {
@@ -638,11 +704,13 @@ int check_lora(int count, const mlxr_lora_item* items, int tokens, int K, int ad
     return set_error(MLXR_E_SHAPE, "lora: at most %d adapters", MLXR_LORA_MAX_ADAPTERS);
   if (rank % 8 || rank > MLXR_LORA_MAX_RANK)
     return set_error(MLXR_E_SHAPE, "lora: rank must be a multiple of 8 and at most %d", MLXR_LORA_MAX_RANK);
+  if (K > MLXR_LORA_MAX_SIZE) return set_error(MLXR_E_SHAPE, "lora: K must be at most %d", MLXR_LORA_MAX_SIZE);
   if (K % 8) return set_error(MLXR_E_SHAPE, "lora: K must be a multiple of 8");
   if (tokens > MLXR_LORA_MAX_TOKENS) return set_error(MLXR_E_SHAPE, "lora: at most %d tokens", MLXR_LORA_MAX_TOKENS);
   if (count && !items) return set_error(MLXR_E_INVALID, "null items");
   for (int i = 0; i < count; ++i)
-    if (items[i].N <= 0) return set_error(MLXR_E_INVALID, "lora: N must be positive");
+    if (items[i].N <= 0 || items[i].N > MLXR_LORA_MAX_SIZE)
+      return set_error(MLXR_E_INVALID, "lora: N must be positive and at most %d", MLXR_LORA_MAX_SIZE);
   return MLXR_OK;
 }
 
@@ -686,10 +754,10 @@ extern "C" int mlxr_lora_apply(int count, const mlxr_lora_item* items, int token
   LoraArgs a{};
   a.x = (const uint16_t*)x_dev, a.x_stride = x_stride;
   a.ids = ids_dev, a.ranks = ranks_dev, a.scales = scales_dev;
-  a.order = (int32_t*)(ws + l.order), a.counts = (int32_t*)(ws + l.counts), a.tiles = (Tile*)(ws + l.tile);
+  a.order = (int32_t*)(ws + l.order), a.tiles = (Tile*)(ws + l.tile);
   a.h = (float*)(ws + l.h);
   a.tokens = tokens, a.K = K, a.adapters = adapters, a.rank = rank, a.splits = l.splits, a.chunk = l.chunk;
-  a.columns = l.columns;
+  a.columns = l.columns, a.most_tiles = l.tiles;
   for (int i = 0; i < count; i += kItems) {
     a.count = count - i < kItems ? count - i : kItems;
     for (int j = 0; j < a.count; ++j) a.item[j] = items[i + j];

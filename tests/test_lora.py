@@ -1,5 +1,6 @@
 """Low-rank adapters beside shared projections (lora_apply) against the formula in float64."""
 import ctypes
+import math
 
 import pytest
 
@@ -39,6 +40,13 @@ def test_refusals():
     assert size(count=0) == 0 and n.value == 0
     assert size() == 0 and n.value == 0  # one launch
     assert size(tokens=300) == 0 and n.value > 0
+
+
+def test_sizes_that_indexes_would_not_hold_are_refused():
+    L = lora._lib()
+    for N, K in ((32, (1 << 28) + 8), ((1 << 28) + 1, 256)):
+        item = (lora.Item * 1)(lora.Item(64, 64, 64, 64, N, mx.BF16))
+        assert L.mlxr_lora_apply(1, item, 4, K, 3, 16, P(64), mx.BF16, K, P(64), None, None, P(64), 1 << 40, None) in (-1, -3)
 
 
 def test_wrapper_refusals():
@@ -193,6 +201,34 @@ def test_lora_in_place_strided_and_on_another_stream(cuda):
     assert all(torch.equal(g, w) for g, w in zip(mine, want))
     with pytest.raises(mx.QGemmError, match="x's dtype"):
         mx.lora_apply(dev(x), ids, [t.half() for t in a], b, y, scales, ranks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,K,rank", [(3, 64, 8), (20, 2048, 64), (300, 256, 32)])
+def test_infinite_b_gives_infinity(cuda, dtype, tokens, K, rank):
+    """An infinite element of B: an infinite output of h's sign, whatever h's bits past 16 (0 among them), not NaN."""
+    import torch
+    x, ids, a, b, y, scales, ranks = _make(cuda, tokens, K, 3, rank, [40], dtype, dtype, 5)
+    ids = torch.arange(tokens, dtype=torch.int32) % 3
+    a, b = [t.nan_to_num(0.0) for t in a], [t.nan_to_num(0.0) for t in b]
+    x[::2] = x[::2].round()  # every other token: h is a small multiple of a power of two, its low part 0
+    a[0] = (a[0] * 16).round() / 4
+    ranks[:], scales[:] = rank, 0.5
+    for i in range(3):
+        b[0][i, 7 + i, i], b[0][i, 20, 3] = math.inf, -math.inf
+    got = mx.lora_apply(x.to(cuda), ids.to(cuda), [a[0].to(cuda)], [b[0].to(cuda)], [y[0].to(cuda)], scales.to(cuda),
+                        ranks.to(cuda))[0].double().cpu()
+    for t in range(tokens):
+        i = int(ids[t])
+        h = a[0][i].double() @ x[t].double()
+        for n, r, sign in ((7 + i, i, 1.0), (20, 3, -1.0)):
+            if abs(float(h[r])) > 1e-3:
+                assert float(got[t, n]) == math.copysign(math.inf, sign * float(h[r])), (t, n)
+            elif float(h[r]) == 0:
+                assert math.isnan(float(got[t, n]))
+        rest = [n for n in range(40) if n not in (7 + i, 20)]
+        assert torch.isfinite(got[t, rest]).all()
 
 
 @pytest.mark.gpu

@@ -122,14 +122,14 @@ __device__ __forceinline__ void store_values(void* out, int dtype, int64_t i, co
   }
 }
 
-// F16: the products' type (else bf16).  F8: the cache is e4m3.  DT: 64, 128 or 256, at least dim (DIM:
-// equal).  P8: page_size % 8 == 0.
+// F16: the products' type (else bf16).  F8: the cache is e4m3.  DT: 64, 96, 128 or 256, at least dim (DIM:
+// equal; 96: above 64, not for e4m3; 128: above that).  P8: page_size % 8 == 0.
 template <bool F16, bool F8, int DT, bool DIM, bool P8>
 struct Attn {
   static constexpr int KS = DT / 32;               // steps of the first product
   static constexpr int VE = DT == 64 ? 4 : 8;      // neighbouring values of a token that a lane loads
-  static constexpr int VH = DT / (16 * VE);        // times that
-  static constexpr int NC = DT / 16;               // accumulators
+  static constexpr int VH = DT == 256 ? 2 : 1;     // times that
+  static constexpr int NC = VH * VE;               // accumulators
   // p times 2^14 in f16: weights down to 2^-28 of the largest stay normal numbers (bf16 has the range)
   static constexpr float SHIFT = F16 ? 14.f : 0.f;
   static constexpr float UNSHIFT = F16 ? 0x1p-14f : 1.f;
@@ -148,6 +148,9 @@ struct Attn {
 
   __device__ Attn(const AttnArgs& a_) : a(a_), lane(threadIdx.x & 63), col(lane & 15), g(lane >> 4) {}
 
+  // Whether all lanes' part of load j of a key's row lies within the head's dims.
+  static constexpr bool whole(int j) { return DIM || ((DT == 96 || DT == 128) && j < KL - 1); }
+
   // First element of the k-th operand of step j that lane group g holds, as in the keys' loads.
   __device__ __forceinline__ int dim_of(int j) const {
     return F8 ? (j >> 1) * 64 + g * 16 + (j & 1) * 8 : j * 32 + g * 8;
@@ -160,7 +163,7 @@ struct Attn {
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
       const int d = dim_of(j);
-      q[j] = ok && (DIM || d < a.dim) ? *(const u32x4_t*)(p + d) : u32x4_t{0, 0, 0, 0};
+      q[j] = ok && (whole(F8 ? j >> 1 : j) || d < a.dim) ? *(const u32x4_t*)(p + d) : u32x4_t{0, 0, 0, 0};
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) o[c] = f32x4_t{0, 0, 0, 0};
@@ -240,7 +243,7 @@ struct Attn {
 #pragma unroll
       for (int j = 0; j < KL; ++j) {
         int d = F8 ? j * 64 + g * 16 : j * 32 + g * 8;
-        if (!DIM && d >= a.dim) d = 0;
+        if (!whole(j) && d >= a.dim) d = 0;
         kr[hh][j] = stream_load((const u32x4_t*)(p + d * (F8 ? 1 : 2)));
       }
     }
@@ -357,7 +360,7 @@ struct Attn {
           const uint32_t w0 = kf[2 * (j & 1)], w1 = kf[2 * (j & 1) + 1];
           kf = u32x4_t{widen<F16, false>(w0), widen<F16, true>(w0), widen<F16, false>(w1), widen<F16, true>(w1)};
         }
-        if (!DIM && dim_of(j) >= a.dim) kf = u32x4_t{0, 0, 0, 0};
+        if (!whole(F8 ? j >> 1 : j) && dim_of(j) >= a.dim) kf = u32x4_t{0, 0, 0, 0};
         s[hh] = mfma16<F16>(kf, q[j], s[hh]);
       }
     }
@@ -582,10 +585,14 @@ AttnKern& kern_of(int dim, bool p8) {
   if (dim == 256 && p8) MLXR_ATTN(256, true, true)
   if (p8) {
     if (dim < 64) MLXR_ATTN(64, false, true)
+    if constexpr (!F8)
+      if (dim <= 96) MLXR_ATTN(96, false, true)
     if (dim < 128) MLXR_ATTN(128, false, true)
     MLXR_ATTN(256, false, true)
   }
   if (dim <= 64) MLXR_ATTN(64, false, false)
+  if constexpr (!F8)
+    if (dim <= 96) MLXR_ATTN(96, false, false)
   if (dim <= 128) MLXR_ATTN(128, false, false)
   MLXR_ATTN(256, false, false)
 #undef MLXR_ATTN

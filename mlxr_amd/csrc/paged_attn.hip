@@ -95,7 +95,7 @@ constexpr int kMaxHeads = 1 << 24;  // rows times heads: the launch's workgroups
 struct Plan {
   int group, groups, part_rows;
   bool one;
-  size_t bytes;  // of the workspace
+  size_t lds, bytes;  // LDS that one launch asks for beside its own; bytes of the workspace
 };
 constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 3) / 4 * 4 * sizeof(int32_t); }
 // most: tokens of the longest row that the table can hold.  A workgroup alone gets about 38 GB/s, so few rows have
@@ -113,6 +113,12 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int64_t most) {
   const int64_t bytes = 2 * most * c->head_dim * (c->dtype == MLXR_E4M3 ? 1 : 2);
   p.one = bytes <= 256 << 10 || (bytes <= 1 << 20 && units >= 256) || rows > kMaxCutRows ||
           (most / kTile + 1) * rows > INT32_MAX || (most / kTile + 1) * units / 64 > INT32_MAX;  // what a cut launch counts in 32 bits
+  // Rows of more than 256 KiB: two workgroups of a CU, not the three or four that its registers hold, by LDS that they do
+  // not use.  Later workgroups then start where rows turn out short, and lines that heads share stay in the L2.  us, three
+  // or four and two: 32 kv heads of 80 in [token, head] order, 1024 tokens, 17 rows 57 and 43, 48 rows 112 and 104; 32 of
+  // 128, up to 1024, 17 rows 38 and 36, 200 rows 259 and 264; 4 of 64, up to 2048, 200 rows 56 and 48; below: 32 of 80,
+  // 256 tokens, 100 rows 40 and 47; 8 of 128, up to 300, 200 rows 30 and 33.  (Above 128 dims one is resident.)
+  p.lds = bytes > 256 << 10 && c->head_dim <= 128 ? 46 << 10 : 0;
   p.bytes = p.one ? 0 : prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * kWaves * 2 *
                                                  partial_floats(p.part_rows, c->head_dim) * sizeof(float);
   return p;
@@ -212,7 +218,7 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
       while (a.near < 8 && a.kv_heads % (2 * a.near) == 0) a.near *= 2;
     const int n = a.near * a.groups, units = rows * a.kv_heads;
     const int grid = n > 1 ? (units / a.near + 7) / 8 * 8 * n : units;
-    e = hipLaunchKernel(k.rows_fn, dim3(grid), dim3(64 * kWaves), args, 0, st);
+    e = hipLaunchKernel(k.rows_fn, dim3(grid), dim3(64 * kWaves), args, p.lds, st);
   } else {
     const int grid = grid_of(k, &e);
     if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_attention: %s", hipGetErrorString(e));

@@ -124,7 +124,8 @@ __device__ __forceinline__ void store_values(void* out, int dtype, int64_t i, co
 
 // F16: the products' type (else bf16).  F8: the cache is e4m3.  DT: 64, 96, 128 or 256, at least dim (DIM:
 // equal; 96: above 64, not for e4m3; 128: above that).  P8: page_size % 8 == 0.
-template <bool F16, bool F8, int DT, bool DIM, bool P8>
+// LK: keys through LDS (load_k).
+template <bool F16, bool F8, int DT, bool DIM, bool P8, bool LK>
 struct Attn {
   static constexpr int KS = DT / 32;               // steps of the first product
   static constexpr int VE = DT == 64 ? 4 : 8;      // neighbouring values of a token that a lane loads
@@ -134,19 +135,22 @@ struct Attn {
   static constexpr float SHIFT = F16 ? 14.f : 0.f;
   static constexpr float UNSHIFT = F16 ? 0x1p-14f : 1.f;
   static constexpr bool NT = DIM && DT * (F8 ? 1 : 2) % 128 == 0;  // past the caches
-  static constexpr int KL = F8 ? KS / 2 : KS;      // 16-byte loads of a key row by a lane
+  static constexpr int KL = F8 ? KS / 2 : KS;      // 16-byte parts of a key row in a lane's operands
+  // Keys through LDS: parts of a row, tokens of a load, loads of a tile.
+  static constexpr int CH = F8 ? DT / 16 : DT == 96 ? 16 : DT / 8, TPL = 64 / CH, NL = LK ? kTile / TPL : 2 * KL;
 
   const AttnArgs& a;
   const int lane, col, g;
   u32x4_t q[KS];
-  u32x4_t kr[2][KL];
+  u32x4_t kr[NL];
+  u32x4_t* keys;  // [32 tokens][CH] of this wavefront
   uint32_t vr[VH][8][F8 ? VE / 4 : VE / 2];
   f32x4_t o[NC];
   float m, l, sc;
   const uint8_t *kh, *vh;
   const int32_t* trow;
 
-  __device__ Attn(const AttnArgs& a_) : a(a_), lane(threadIdx.x & 63), col(lane & 15), g(lane >> 4) {}
+  __device__ Attn(const AttnArgs& a_, u32x4_t* keys_) : a(a_), lane(threadIdx.x & 63), col(lane & 15), g(lane >> 4), keys(keys_) {}
 
   // Whether all lanes' part of load j of a key's row lies within the head's dims.
   static constexpr bool whole(int j) { return DIM || ((DT == 96 || DT == 128) && j < KL - 1); }
@@ -233,20 +237,63 @@ struct Attn {
   // The loads of a tile are unconditional, from an address within the stores for whatever does not count, so
   // that they stay in flight over the branches: what they bring for tokens that do not count is left out later.
   // more: false where there is no further tile; all lanes then read the first page's first rows again.
+  //
+  // Keys: an operand's lanes are 16 tokens at a time, so that a load of it is 16 pieces of 64 bytes.  LK: loads of whole
+  // rows side by side instead, brought into operand order through LDS; blocks of eight tokens lie side by side, their
+  // offsets come from the lane groups by readlane.  us, straight and through LDS: 64 rows of 32 kv heads of 128, up to 1024
+  // tokens, 93 and 82; of 32 of 80, window 1024, 137 and 121; 8 of 128, up to 8192, 172 and 168; but a row of 4 kv heads
+  // of 64, 700 tokens, 7.3 and 8.6: nothing hides the way through LDS there.
   __device__ __forceinline__ void load_k(const Ids& n, int t0, bool more) {
-    const uint8_t* block = nullptr;
-    if constexpr (P8) block = kh + (more ? offset(__shfl(n.id[0], (col & 12) * 4), t0 + key_token(0), a.k_page, a.k_token) : 0);
+    if constexpr (LK) {
+      const int c = lane % CH, tk = lane / CH;
+      const uint64_t at = (uint64_t)a.k_token * (tk & 7) + (DIM || c * (F8 ? 16 : 8) < a.dim ? c : 0) * 16;
+      const uint64_t mine = more ? offset(n.id[0], t0 + 8 * g, a.k_page, a.k_token) : 0;  // of the block of eight tokens g
+      const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
 #pragma unroll
-    for (int hh = 0; hh < 2; ++hh) {
-      const uint8_t* p = P8 ? block + (uint64_t)a.k_token * (4 * hh)
-                            : kh + (more ? offset(n.id[P8 ? 0 : 8 + hh], t0 + key_token(hh), a.k_page, a.k_token) : 0);
+      for (int i = 0; i < NL; ++i) {
+        const int from = 16 * (i * TPL / 8);
+        uint64_t row;
+        if constexpr (TPL > 8)
+          row = (uint64_t)(uint32_t)__shfl((int)hi, from + 2 * (tk & 8)) << 32 | (uint32_t)__shfl((int)lo, from + 2 * (tk & 8));
+        else
+          row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, from) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)lo, from);
+        kr[i] = stream_load((const u32x4_t*)(kh + row + (uint64_t)a.k_token * (i * TPL & 7) + at));
+      }
+    } else {
+      const uint8_t* block = nullptr;
+      if constexpr (P8) block = kh + (more ? offset(__shfl(n.id[0], (col & 12) * 4), t0 + key_token(0), a.k_page, a.k_token) : 0);
 #pragma unroll
-      for (int j = 0; j < KL; ++j) {
-        int d = F8 ? j * 64 + g * 16 : j * 32 + g * 8;
-        if (!whole(j) && d >= a.dim) d = 0;
-        kr[hh][j] = stream_load((const u32x4_t*)(p + d * (F8 ? 1 : 2)));
+      for (int hh = 0; hh < 2; ++hh) {
+        const uint8_t* p = P8 ? block + (uint64_t)a.k_token * (4 * hh)
+                              : kh + (more ? offset(n.id[P8 ? 0 : 8 + hh], t0 + key_token(hh), a.k_page, a.k_token) : 0);
+#pragma unroll
+        for (int j = 0; j < KL; ++j) {
+          int d = F8 ? j * 64 + g * 16 : j * 32 + g * 8;
+          if (!whole(j) && d >= a.dim) d = 0;
+          kr[hh * KL + j] = stream_load((const u32x4_t*)(p + d * (F8 ? 1 : 2)));
+        }
       }
     }
+  }
+  // Place of part c of a token's key: 8 lanes that read or write at once, and so 128 bytes, lie in different banks.
+  static __device__ __forceinline__ int place(int token, int c) {
+    const int swap = CH == 4 ? (token >> 1 & 1) | (token >> 2 & 2) : (token & 3) | (token >> 1 & 4);
+    return token * CH + (c ^ swap);
+  }
+  __device__ __forceinline__ void store_k() {
+    if constexpr (LK) {
+      const int c = lane % CH, tk = lane / CH;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) keys[place(i * TPL + tk, c)] = kr[i];
+      // a wavefront's accesses to LDS are in order: only the compiler has to keep them so
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+  }
+  __device__ __forceinline__ u32x4_t key_part(int hh, int j) const {
+    if constexpr (LK) return keys[place(key_token(hh), 4 * j + g)];
+    else return kr[hh * KL + j];
   }
   __device__ __forceinline__ void load_v(const Ids& n, int t0, bool more) {
     constexpr int W = F8 ? VE / 4 : VE / 2;
@@ -307,6 +354,7 @@ struct Attn {
       ids = next;
       next = ids_of(t1 + kTile, s);
       f32x4_t x[2];
+      store_k();
       scores(x);
       load_k(ids, t1, more);
       const bool full = __ballot(live != 0xff) == 0;
@@ -355,7 +403,7 @@ struct Attn {
       s[hh] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < KS; ++j) {
-        u32x4_t kf = kr[hh][F8 ? j >> 1 : j];
+        u32x4_t kf = key_part(hh, F8 ? j >> 1 : j);
         if constexpr (F8) {
           const uint32_t w0 = kf[2 * (j & 1)], w1 = kf[2 * (j & 1) + 1];
           kf = u32x4_t{widen<F16, false>(w0), widen<F16, true>(w0), widen<F16, false>(w1), widen<F16, true>(w1)};
@@ -500,7 +548,10 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_kernel(At
     else hi = mid;
   }
   int r = __builtin_amdgcn_readfirstlane(lo);
-  Attn<F16, F8, DT, DIM, P8> t(a);
+  constexpr bool LK = P8 && DT < 256;  // above, a workgroup's keys would be 64 KiB
+  using T = Attn<F16, F8, DT, DIM, P8, LK>;
+  __shared__ u32x4_t keys[LK ? kWaves : 1][LK ? kTile * T::CH : 1];
+  T t(a, keys[LK ? wave : 0]);
   int slot = 0;
   while (pos < end) {
     const Span s = span_of(a, r);
@@ -525,11 +576,16 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_kernel(At
 // One launch for short rows: a workgroup for each (row, kv head, 16 heads), its wavefronts take equal runs of
 // tiles and are merged in LDS.  Four wavefronts: of eight, half as many workgroups fit a CU (64 rows of
 // 32 kv heads, up to 1024 tokens: 101 us, four 95).
-template <bool F16, bool F8, int DT, bool DIM, bool P8>
+template <class T, bool LK>
+union RowsLds {
+  float park[kWaves / 2][T::PARK * 64];
+  u32x4_t keys[LK ? kWaves : 1][LK ? kTile * T::CH : 1];
+};
+template <bool F16, bool F8, int DT, bool DIM, bool P8, bool LK>
 __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_rows_kernel(AttnArgs a) {
   constexpr int WAVES = kWaves;
-  using T = Attn<F16, F8, DT, DIM, P8>;
-  __shared__ float sh[WAVES / 2][T::PARK * 64];
+  using T = Attn<F16, F8, DT, DIM, P8, LK>;
+  __shared__ RowsLds<T, LK> sh;
   // Workgroup i runs on XCD i % 8, each with its own L2.  Those that read the same lines follow each other on
   // one: the groups of 16 heads of a kv head, and a.near kv heads whose rows share lines.
   int unit = blockIdx.x, grp = 0;
@@ -549,22 +605,24 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_rows_kern
     if (a.lse && (int)threadIdx.x < n) a.lse[head + threadIdx.x] = -INFINITY;
     return;
   }
-  T t(a);
+  T t(a, sh.keys[LK ? wave : 0]);
   t.start(r, kvh, grp);
   const int per = (s.tiles + WAVES - 1) / WAVES, first = wave * per, count = min(per, s.tiles - first);
   if (count > 0) t.run(s, first, count);
+  if constexpr (LK) __syncthreads();
 #pragma unroll
   for (int half = WAVES / 2; half; half /= 2) {
-    if (wave >= half && wave < 2 * half) t.park(sh[wave - half]);
+    if (wave >= half && wave < 2 * half) t.park(sh.park[wave - half]);
     __syncthreads();
-    if (wave < half) t.merge(sh[wave]);
+    if (wave < half) t.merge(sh.park[wave]);
     __syncthreads();
   }
   if (wave == 0) t.finish(r, kvh, grp, nullptr);
 }
 
 struct AttnKern {
-  const void *fn, *rows_fn;
+  const void *fn, *rows_fn[2];  // rows_fn[1]: keys through LDS
+  int rows_lds[2];
   std::atomic<int> residents[64];  // workgroups of a CU, by device; 0: not asked yet
 };
 // The kernel for head_dim at a page size; F16/F8 as above.
@@ -577,7 +635,13 @@ template <bool F16, bool F8>
 AttnKern& kern_of(int dim, bool p8) {
 #define MLXR_ATTN(DT, DIM, P8)                                                                                              \
   {                                                                                                                        \
-    static AttnKern k{(const void*)attn_kernel<F16, F8, DT, DIM, P8>, (const void*)attn_rows_kernel<F16, F8, DT, DIM, P8>, {}}; \
+    constexpr bool LK = P8 && DT < 256;                                                                                    \
+    static AttnKern k{(const void*)attn_kernel<F16, F8, DT, DIM, P8>,                                                      \
+                      {(const void*)attn_rows_kernel<F16, F8, DT, DIM, P8, false>,                                         \
+                       (const void*)attn_rows_kernel<F16, F8, DT, DIM, P8, LK>},                                           \
+                      {(int)sizeof(RowsLds<Attn<F16, F8, DT, DIM, P8, false>, false>),                                     \
+                       (int)sizeof(RowsLds<Attn<F16, F8, DT, DIM, P8, LK>, LK>)},                                          \
+                      {}};                                                                                                 \
     return k;                                                                                                              \
   }
   if (dim == 64 && p8) MLXR_ATTN(64, true, true)

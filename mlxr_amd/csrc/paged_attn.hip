@@ -94,8 +94,8 @@ constexpr int kMaxHeads = 1 << 24;  // rows times heads: the launch's workgroups
 // How a call runs: short rows in one launch without a workspace.
 struct Plan {
   int group, groups, part_rows;
-  bool one;
-  size_t lds, bytes;  // LDS that one launch asks for beside its own; bytes of the workspace
+  bool one, two_of_cu, keys_in_lds;  // of one launch
+  size_t bytes;                      // of the workspace
 };
 constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 3) / 4 * 4 * sizeof(int32_t); }
 // most: tokens of the longest row that the table can hold.  A workgroup alone gets about 38 GB/s, so few rows have
@@ -118,7 +118,8 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int64_t most) {
   // or four and two: 32 kv heads of 80 in [token, head] order, 1024 tokens, 17 rows 57 and 43, 48 rows 112 and 104; 32 of
   // 128, up to 1024, 17 rows 38 and 36, 200 rows 259 and 264; 4 of 64, up to 2048, 200 rows 56 and 48; below: 32 of 80,
   // 256 tokens, 100 rows 40 and 47; 8 of 128, up to 300, 200 rows 30 and 33.  (Above 128 dims one is resident.)
-  p.lds = bytes > 256 << 10 && c->head_dim <= 128 ? 46 << 10 : 0;
+  p.two_of_cu = bytes > 256 << 10 && c->head_dim <= 128;
+  p.keys_in_lds = units >= device_cu_count();  // fewer: latency counts (load_k)
   p.bytes = p.one ? 0 : prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * kWaves * 2 *
                                                  partial_floats(p.part_rows, c->head_dim) * sizeof(float);
   return p;
@@ -218,7 +219,8 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
       while (a.near < 8 && a.kv_heads % (2 * a.near) == 0) a.near *= 2;
     const int n = a.near * a.groups, units = rows * a.kv_heads;
     const int grid = n > 1 ? (units / a.near + 7) / 8 * 8 * n : units;
-    e = hipLaunchKernel(k.rows_fn, dim3(grid), dim3(64 * kWaves), args, p.lds, st);
+    const int own = k.rows_lds[p.keys_in_lds], lds = p.two_of_cu ? (56 << 10) - own : 0;  // of 160 KiB
+    e = hipLaunchKernel(k.rows_fn[p.keys_in_lds], dim3(grid), dim3(64 * kWaves), args, lds, st);
   } else {
     const int grid = grid_of(k, &e);
     if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_attention: %s", hipGetErrorString(e));

@@ -98,21 +98,24 @@ struct Plan {
   size_t bytes;                      // of the workspace
 };
 constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 3) / 4 * 4 * sizeof(int32_t); }
-// most: tokens of the longest row that the table can hold.  A workgroup alone gets about 38 GB/s, so few rows have
+// By the longest row that the table can hold, or the window; a window never needs more workspace.  A workgroup alone gets about 38 GB/s, so few rows have
 // to be cut unless they are short; many rows fill the device uncut, until the longest keeps it waiting.
-// Measured, us, uncut and cut (which also takes the host 4 us more): 8 kv heads of 128 in bf16, one row of up to
-// 512 tokens (256 KiB a head) 10 and 9.4, of 1024 15 and 10.3; 16 ragged rows of up to 1024 21 and 19.5; 64 of up
-// to 1024 37 and 45, 2048 (1 MiB) 68 and 69, 4096 130 and 97; in e4m3 with 64 heads, 64 of up to 2048 40 and 55,
-// 4096 74 and 74; 4 kv heads of 64, one row of up to 1024 10.9 and 9.3, 64 of up to 2048 21 and 29, 4096 39 and 39.
-Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int64_t most) {
+// Measured, us, uncut and cut (which also takes the host 4 us more), rows up to the longest, ragged unless one; 8 kv heads of
+// 128 in bf16, up to 512 tokens (256 KiB a head): one row 9.5 and 9.5, 64 rows 18 and 24; 1024: 15 and 11, 4 rows 18 and
+// 12, 16 19 and 17, 64 30 and 37; 2048 (1 MiB): 32 rows 30 and 35, 64 55 and 58; 4096 (2 MiB): 64 rows 103 and 95, 128
+// 171 and 176; 8192: 128 rows 335 and 319.  32 of 128, 4096: 16 rows 102 and 103, 64 315 and 342; 8192: 64 rows 627 and
+// 624.  In e4m3, 2048 (512 KiB): 16 rows 22 and 23, 64 33 and 46; 8192: 128 rows 186 and 192.  4 of 64, 2048: one row
+// 18 and 10, 64 20 and 26; 8192: 64 rows 63 and 54.
+Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int width, int window) {
   Plan p;
+  const int64_t held = (int64_t)width * c->page_size, most = window > 0 && window < held ? window : held;
   p.group = heads / c->kv_heads;
   p.groups = (p.group + kHeads - 1) / kHeads;
   p.part_rows = p.group < kHeads ? p.group : kHeads;
   const int64_t units = (int64_t)rows * c->kv_heads * p.groups;
   const int64_t bytes = 2 * most * c->head_dim * (c->dtype == MLXR_E4M3 ? 1 : 2);
-  p.one = bytes <= 256 << 10 || (bytes <= 1 << 20 && units >= 256) || rows > kMaxCutRows ||
-          (most / kTile + 1) * rows > INT32_MAX || (most / kTile + 1) * units / 64 > INT32_MAX;  // what a cut launch counts in 32 bits
+  p.one = bytes <= 256 << 10 || (bytes <= 1 << 20 && units >= 256) || (bytes <= 2 << 20 && units >= 1024) || rows > kMaxCutRows ||
+          (held / kTile + 1) * rows > INT32_MAX || (held / kTile + 1) * units / 64 > INT32_MAX;  // what a cut launch counts in 32 bits
   // Rows of more than 256 KiB: two workgroups of a CU, not the three or four that its registers hold, by LDS that they do
   // not use.  Later workgroups then start where rows turn out short, and lines that heads share stay in the L2.  us, three
   // or four and two: 32 kv heads of 80 in [token, head] order, 1024 tokens, 17 rows 57 and 43, 48 rows 112 and 104; 32 of
@@ -124,12 +127,6 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int64_t most) {
                                                  partial_floats(p.part_rows, c->head_dim) * sizeof(float);
   return p;
 }
-// Tokens that a row may hold and, with a window, attend to.
-int64_t longest(const mlxr_paged_cache* c, int width, int window) {
-  const int64_t most = (int64_t)width * c->page_size;
-  return window > 0 && window < most ? window : most;
-}
-
 // Workgroups of a cut launch: as many as the device holds at once.
 int grid_of(AttnKern& k, hipError_t* e) {
   int dev = 0;
@@ -169,7 +166,7 @@ extern "C" int mlxr_paged_attention_workspace_size(const mlxr_paged_cache* cache
                                                    size_t* bytes) {
   if (!bytes) return set_error(MLXR_E_INVALID, "null bytes");
   if (const int rc = check_attn(cache, rows, heads, table_width)) return rc;
-  *bytes = rows ? plan_of(cache, rows, heads, longest(cache, table_width, 0)).bytes : 0;
+  *bytes = rows ? plan_of(cache, rows, heads, table_width, 0).bytes : 0;
   return MLXR_OK;
 }
 
@@ -189,7 +186,7 @@ extern "C" int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int
   if (!q_dev || !table_dev || !lens_dev || !out_dev) return set_error(MLXR_E_INVALID, "null buffer");
   if (q_row_stride % 8 || q_head_stride % 8 || (((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15))
     return set_error(MLXR_E_SHAPE, "paged_attention: query rows, output and workspace must start at multiples of 16 bytes");
-  const Plan p = plan_of(cache, rows, heads, longest(cache, table_width, window));
+  const Plan p = plan_of(cache, rows, heads, table_width, window);
   if (workspace_bytes < p.bytes || (p.bytes && !workspace_dev))
     return set_error(MLXR_E_INVALID, "paged_attention: the workspace is smaller than mlxr_paged_attention_workspace_size");
   const int es = cache->dtype == MLXR_E4M3 ? 1 : 2;

@@ -391,45 +391,68 @@ constexpr int h_row(int rt) { return 32 * rt + 8; }
 template <bool F16, int RT, int SUB, int WAVES>
 struct Expand {
   static constexpr int R = 16 * RT, KT = RT == 1 ? 1 : RT / 2, CT = columns_of(SUB, RT), STEP = WAVES * 16 * CT;
+  static constexpr int C = R / 8, NB = 16 * CT * C / 64;  // 16-byte parts of a column's row of B; loads of a step
   const LoraArgs& a;
   const mlxr_lora_item& it;
   const uint16_t* B;
   int rank, ld, n0, end, col, g;
-  u32x4_t next[KT][CT];  // operands of B for a step, on their way while h or the columns before are computed
+  // B of a step, on its way while h or the columns before are computed, and its place in LDS: loads of rows side by
+  // side, brought into operand order there (an operand's own load would be 16 pieces of 64 bytes).
+  u32x4_t next[NB];
+  u32x4_t* rows;
 
-  __device__ __forceinline__ Expand(const LoraArgs& a_, const mlxr_lora_item& it_, const Tile& t, int begin)
+  __device__ __forceinline__ Expand(const LoraArgs& a_, const mlxr_lora_item& it_, const Tile& t, int begin, u32x4_t* lds)
       : a(a_), it(it_), B((const uint16_t*)it_.b_dev + (t.adapter == a_.adapters ? 0 : (int64_t)t.adapter * it_.N * a_.rank)),
         rank(t.rank), ld(t.rank ? a_.rank : 0) {
     const int lane = threadIdx.x & 63;
     col = lane & 15, g = lane >> 4;
     n0 = begin + (threadIdx.x >> 6) * 16 * CT;
+    rows = lds + (threadIdx.x >> 6) * NB * 64;
     end = min(begin + a.columns, it.N);
     load_b(n0, n0 < end);
   }
-  // RT 1 multiplies the high and the low parts in one product, ranks 8 (g & 1) ..  The loads are unconditional, so that
-  // they stay in flight: what a column or rank that is not there gets lies in a row that is read anyway.
+  // The loads are unconditional, so that they stay in flight: what a column or rank that is not there gets lies in a row
+  // that is read anyway.
   __device__ __forceinline__ void load_b(int n0, bool more) {
     const int ld = more ? this->ld : 0;
 #pragma unroll
-    for (int k = 0; k < KT; ++k)
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        const int n = min(n0 + CT * col + c, it.N - 1), at = rank_at(k);
-        next[k][c] = *(const u32x4_t*)(B + (int64_t)n * ld + (at < rank ? at : 0));
-      }
+    for (int i = 0; i < NB; ++i) {
+      const int at = i * 64 + (threadIdx.x & 63), part = at % C;
+      next[i] = *(const u32x4_t*)(B + (int64_t)min(n0 + at / C, it.N - 1) * ld + (8 * part < rank ? 8 * part : 0));
+    }
   }
+  // Place of part `part` of column n of a step: 8 lanes that read or write at once, and so 128 bytes, lie in different banks.
+  static __device__ __forceinline__ int place(int n, int part) { return (n * C + part) ^ (n / CT & 7); }
+  __device__ __forceinline__ void store_b() {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int at = i * 64 + (threadIdx.x & 63);
+      rows[place(at / C, at % C)] = next[i];
+    }
+    // a wavefront's accesses to LDS are in order: only the compiler has to keep them so
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  // RT 1 multiplies the high and the low parts in one product, ranks 8 (g & 1) ..
   __device__ __forceinline__ int rank_at(int k) const { return RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g; }
+  // Operand c of the ranks k, without what the adapter has not.
+  __device__ __forceinline__ u32x4_t operand(int k, int c) const {
+    u32x4_t b = rows[place(CT * col + c, rank_at(k) / 8)];
+    if (rank < R) {
+      const int left = rank - rank_at(k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] &= left >= 2 * e + 2 ? ~0u : left > 2 * e ? 0xffffu : 0u;
+    }
+    return b;
+  }
   // hs: the tile's rows of h; none: the tokens have no adapter.  VEC: rows of y and out start at multiples of 16
   // bytes and are whole groups of CT columns.
   template <int YT, bool VEC>
   __device__ __forceinline__ void columns(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
     constexpr bool AHEAD = VEC && SUB > 1 && YT != DT_F32;  // y of the next 16 tokens on its way: fp32 has no registers for it
     for (; n0 < end; n0 += STEP) {
-      u32x4_t bf[KT][CT];
-#pragma unroll
-      for (int k = 0; k < KT; ++k)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) bf[k][c] = next[k][c];
+      store_b();
       const int n = n0 + CT * col, left = it.N - n;
       Cols<YT, CT> y[4];
       auto load_y = [&](Cols<YT, CT>(&to)[4], int s) {
@@ -443,17 +466,12 @@ struct Expand {
       load_y(y, 0);
       asm volatile("" ::: "memory");  // the loads stay in this order: what waits for y would wait for those before it too
       load_b(n0 + STEP, n0 + STEP < end);
-      if (rank < R)  // nothing of ranks that the adapter has not
+      u32x4_t bf[SUB > 1 ? KT : 1][SUB > 1 ? CT : 1];  // read once for all tokens
+      if constexpr (SUB > 1)
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-          const int past = rank - rank_at(k);
+        for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t mask = past >= 2 * e + 2 ? ~0u : past > 2 * e ? 0xffffu : 0u;
-#pragma unroll
-            for (int c = 0; c < CT; ++c) bf[k][c][e] &= mask;
-          }
-        }
+          for (int c = 0; c < CT; ++c) bf[k][c] = operand(k, c);
 #pragma unroll 1
       for (int s = 0; s < SUB; ++s) {
         if (SUB > 1 && 16 * s >= count) break;
@@ -467,13 +485,21 @@ struct Expand {
             if constexpr (RT == 1) {
               const u32x4_t f = *(const u32x4_t*)(h + 8 * g);
 #pragma unroll
-              for (int c = 0; c < CT; ++c) acc[c] = mfma16<F16>(f, bf[k][c], acc[c]);
+              for (int c = 0; c < CT; ++c) {
+                u32x4_t b;
+                if constexpr (SUB > 1) b = bf[k][c];
+                else b = operand(k, c);
+                acc[c] = mfma16<F16>(f, b, acc[c]);
+              }
             } else {
               const u32x4_t hi = *(const u32x4_t*)(h + 32 * k + 8 * g), lo = *(const u32x4_t*)(h + R + 32 * k + 8 * g);
 #pragma unroll
               for (int c = 0; c < CT; ++c) {
-                acc[c] = mfma16<F16>(lo, bf[k][c], acc[c]);
-                acc[c] = mfma16<F16>(hi, bf[k][c], acc[c]);
+                u32x4_t b;
+                if constexpr (SUB > 1) b = bf[k][c];
+                else b = operand(k, c);
+                acc[c] = mfma16<F16>(lo, b, acc[c]);
+                acc[c] = mfma16<F16>(hi, b, acc[c]);
               }
             }
           }
@@ -531,7 +557,9 @@ __global__ __launch_bounds__(kThreads, RT <= 4 && SUB == 1 ? 3 : 1) void expand_
   if (count == 0) return;
   const bool none = tile.adapter == a.adapters;
   if (none && it.out_dev == it.y_dev) return;
-  Expand<F16, RT, SUB, kWaves> e(a, it, tile, begin);
+  using E = Expand<F16, RT, SUB, kWaves>;
+  __shared__ u32x4_t rows[kWaves * E::NB * 64];
+  E e(a, it, tile, begin, rows);
   if (!none) {
     for (int u = threadIdx.x; u < 16 * SUB * 2 * RT; u += kThreads) {
       const int t = u / (2 * RT), at = 8 * (u % (2 * RT));
@@ -574,7 +602,9 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
   const bool none = tile.adapter == a.adapters;
   if (none && it.out_dev == it.y_dev) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  Expand<F16, RT, 1, WAVES> e(a, it, tile, begin);
+  using E = Expand<F16, RT, 1, WAVES>;
+  __shared__ u32x4_t rows[WAVES * E::NB * 64];
+  E e(a, it, tile, begin, rows);
   if (!none) {
     const uint16_t* A = (const uint16_t*)it.a_dev + (int64_t)tile.adapter * a.rank * a.K + (int64_t)col * a.K;
     const uint16_t* x = a.x + (int64_t)token[col < count ? col : 0] * a.x_stride;

@@ -195,15 +195,33 @@ __device__ __forceinline__ Tile found_tile(const LoraArgs& a, int index, int* to
   return t;
 }
 
+// 16 rows of x or A by 64 k: a lane loads 16 bytes of rows lane / 8 and 8 + lane / 8, part lane % 8 of the 128, so that
+// rows are read whole; turn makes operands of them by way of 2 KiB of LDS that the wavefront has for itself.  Which k an
+// operand's place stands for is free, alike for x and A.  (An operand's own load would be 16 pieces.)
+__device__ __forceinline__ void turn(u32x4_t (&v)[2], u32x4_t* buf) {
+  const int lane = threadIdx.x & 63, row = lane >> 3, part = lane & 7, col = lane & 15, g = lane >> 4;
+  // 8 lanes that read or write at once, and so 128 bytes, lie in different banks
+  buf[row * 8 + (part ^ row)] = v[0];
+  buf[(row + 8) * 8 + (part ^ row)] = v[1];
+  // a wavefront's accesses to LDS are in order: only the compiler has to keep them so
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  v[0] = buf[col * 8 + (g ^ (col & 7))];
+  v[1] = buf[col * 8 + ((4 + g) ^ (col & 7))];
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // h of SS groups of 16 tokens of a tile over one chunk of K: the wavefronts take turns over it in steps of 64
-// and add up in LDS.  RT: groups of 16 ranks; SUB: of 16 tokens in a tile.  A lane reads 32 neighbouring
-// bytes of a row of x or A, the four lane groups 128: which k an operand's place stands for is free, alike
-// for both.
+// and add up in LDS.  RT: groups of 16 ranks; SUB: of 16 tokens in a tile.
 template <bool F16, int RT, int SUB, bool INLINE>
-__global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kShrinkThreads, RT == 4 && SUB == 1 ? 2 : 1) void shrink_kernel(LoraArgs a) {
   constexpr int kWaves = kShrinkThreads / 64, SS = shrink_sub(RT, SUB);
   __shared__ int tokens[16 * SUB];
   __shared__ f32x4_t sh[kWaves - 1][SS * RT][64];
+  __shared__ u32x4_t turns[kWaves][128];
   Tile tile;
   if constexpr (INLINE) {
     tile = found_tile<kWaves>(a, blockIdx.x, tokens);
@@ -215,48 +233,61 @@ __global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
     tile = planned_tile<SUB>(a, blockIdx.x / (SUB / SS), tokens);
   }
   const int sub = blockIdx.x % (SUB / SS) * SS * 16, count = min(tile.count - sub, 16 * SS), adapter = tile.adapter;
-  if (count <= 0 || adapter == a.adapters) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int split = blockIdx.y, item = blockIdx.z, rank = tile.rank;
+  if (count <= 0 || tile.rank == 0) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int split = blockIdx.y, item = blockIdx.z, rank = __builtin_amdgcn_readfirstlane(tile.rank);
   const int k_end = min((split + 1) * a.chunk, a.K);
+  const int row = lane >> 3, at = 8 * (lane & 7);
   const uint16_t* A = (const uint16_t*)a.item[item].a_dev + (int64_t)adapter * a.rank * a.K;
-  int token[SS];
-  const uint16_t* x[SS];
+  const uint16_t* x[SS][2];
 #pragma unroll
-  for (int s = 0; s < SS; ++s) {
-    token[s] = tokens[sub + (16 * s + col < count ? 16 * s + col : 0)];
-    x[s] = a.x + (int64_t)token[s] * a.x_stride;
-  }
+  for (int s = 0; s < SS; ++s)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = 16 * s + 8 * i + row;
+      x[s][i] = a.x + (int64_t)tokens[sub + (t < count ? t : 0)] * a.x_stride;
+    }
   f32x4_t acc[SS][RT] = {};
-  // Two steps are on their way.  The loads are unconditional: ranks that the adapter has not read its first (their
+  // Two steps are on their way.  The loads are unconditional: ranks that the adapter has not read its last (their
   // sums are not kept), places past the chunk its last.
+  const int last = (rank - 1) & ~7, last_row = min(row, rank - 1 - last);
   u32x4_t xf[2][SS][2], af[2][RT][2];
   auto load = [&](int b, int k) {
+    const int kk = min(k + at, k_end - 8);
+    int64_t whole = (int64_t)row * a.K + kk, part = (int64_t)last_row * a.K + kk;
+    asm("" : "+v"(whole), "+v"(part));  // or each row's address is kept over the loop, in two registers
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int kk = min(k + 16 * g + 8 * e, k_end - 8);
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int s = 0; s < SS; ++s) xf[b][s][e] = *(const u32x4_t*)(x[s] + kk);
+      for (int s = 0; s < SS; ++s) xf[b][s][i] = *(const u32x4_t*)(x[s][i] + kk);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) af[b][r][e] = *(const u32x4_t*)(A + (int64_t)(16 * r + col < rank ? 16 * r + col : 0) * a.K + kk);
+      for (int r = 0; r < RT; ++r) {
+        const int n = min(16 * r + 8 * i, last);
+        af[b][r][i] = *(const u32x4_t*)(A + (int64_t)n * a.K + (n < last ? whole : part));
+      }
     }
   };
   auto add = [&](int b, int k) {
-    if (k + 64 > k_end)
+    if (k + 64 > k_end) {
+      const bool in = k + at < k_end;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const bool in = k + 16 * g + 8 * e < k_end;
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int s = 0; s < SS; ++s) xf[b][s][e] = in ? xf[b][s][e] : u32x4_t{0, 0, 0, 0};
+        for (int s = 0; s < SS; ++s) xf[b][s][i] = in ? xf[b][s][i] : u32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int r = 0; r < RT; ++r) af[b][r][e] = in ? af[b][r][e] : u32x4_t{0, 0, 0, 0};
+        for (int r = 0; r < RT; ++r) af[b][r][i] = in ? af[b][r][i] : u32x4_t{0, 0, 0, 0};
       }
+    }
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int s = 0; s < SS; ++s) turn(xf[b][s], turns[wave]);
 #pragma unroll
-      for (int s = 0; s < SS; ++s)
+    for (int r = 0; r < RT; ++r) {
+      turn(af[b][r], turns[wave]);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) acc[s][r] = mfma16<F16>(af[b][r][e], xf[b][s][e], acc[s][r]);
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int s = 0; s < SS; ++s) acc[s][r] = mfma16<F16>(af[b][r][e], xf[b][s][e], acc[s][r]);
+    }
   };
   constexpr int S = kWaves * 64;
   int k = split * a.chunk + wave * 64;
@@ -268,6 +299,7 @@ __global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
       load(0, k + 2 * S);
       add(1, k + S);
       load(1, k + 3 * S);
+      asm volatile("" ::: "memory");  // the loads stay at the loop's end, not shared with those before it
     }
     add(0, k);
     if (k + S < k_end) add(1, k + S);
@@ -282,7 +314,7 @@ __global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
 #pragma unroll
   for (int s = 0; s < SS; ++s) {
     if (16 * s + col >= count) continue;
-    float* h = a.h + (((int64_t)item * a.splits + split) * a.tokens + token[s]) * a.rank + 4 * g;
+    float* h = a.h + (((int64_t)item * a.splits + split) * a.tokens + tokens[sub + 16 * s + col]) * a.rank + 4 * g;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       f32x4_t v = acc[s][r];

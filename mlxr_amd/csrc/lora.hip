@@ -217,7 +217,7 @@ __device__ __forceinline__ void turn(u32x4_t (&v)[2], u32x4_t* buf) {
 // h of SS groups of 16 tokens of a tile over one chunk of K: the wavefronts take turns over it in steps of 64
 // and add up in LDS.  RT: groups of 16 ranks; SUB: of 16 tokens in a tile.
 template <bool F16, int RT, int SUB, bool INLINE>
-__global__ __launch_bounds__(kShrinkThreads, RT == 4 && SUB == 1 ? 2 : 1) void shrink_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
   constexpr int kWaves = kShrinkThreads / 64, SS = shrink_sub(RT, SUB);
   __shared__ int tokens[16 * SUB];
   __shared__ f32x4_t sh[kWaves - 1][SS * RT][64];
@@ -633,33 +633,41 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
   if (count == 0) return;
   const bool none = tile.adapter == a.adapters;
   if (none && it.out_dev == it.y_dev) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   using E = Expand<F16, RT, 1, WAVES>;
   __shared__ u32x4_t rows[WAVES * E::NB * 64];
   E e(a, it, tile, begin, rows);
   if (!none) {
-    const uint16_t* A = (const uint16_t*)it.a_dev + (int64_t)tile.adapter * a.rank * a.K + (int64_t)col * a.K;
-    const uint16_t* x = a.x + (int64_t)token[col < count ? col : 0] * a.x_stride;
+    const int row = lane >> 3, at = 8 * (lane & 7);
+    const uint16_t* A = (const uint16_t*)it.a_dev + (int64_t)tile.adapter * a.rank * a.K;
+    const uint16_t* x[2] = {a.x + (int64_t)token[row < count ? row : 0] * a.x_stride,
+                            a.x + (int64_t)token[row + 8 < count ? row + 8 : 0] * a.x_stride};
     f32x4_t acc[RT] = {};
     for (int k0 = wave * 64; k0 < a.K; k0 += WAVES * U * 64) {
       u32x4_t xf[U][2], af[U][RT][2];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int kk = k0 + u * WAVES * 64 + 16 * g + 8 * h;
+        for (int i = 0; i < 2; ++i) {
+          const int kk = k0 + u * WAVES * 64 + at;
           const bool in = kk < a.K;
-          xf[u][h] = in ? *(const u32x4_t*)(x + kk) : u32x4_t{0, 0, 0, 0};
+          xf[u][i] = in ? *(const u32x4_t*)(x[i] + kk) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
-          for (int r = 0; r < RT; ++r)
-            af[u][r][h] = in && 16 * r + col < rank ? *(const u32x4_t*)(A + (int64_t)(16 * r) * a.K + kk) : u32x4_t{0, 0, 0, 0};
+          for (int r = 0; r < RT; ++r) {
+            const int n = 16 * r + 8 * i + row;
+            af[u][r][i] = in && n < rank ? *(const u32x4_t*)(A + (int64_t)n * a.K + kk) : u32x4_t{0, 0, 0, 0};
+          }
         }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        turn(xf[u], rows + wave * E::NB * 64);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int r = 0; r < RT; ++r) {
+          turn(af[u][r], rows + wave * E::NB * 64);
 #pragma unroll
-          for (int r = 0; r < RT; ++r) acc[r] = mfma16<F16>(af[u][r][h], xf[u][h], acc[r]);
+          for (int e = 0; e < 2; ++e) acc[r] = mfma16<F16>(af[u][r][e], xf[u][e], acc[r]);
+        }
+      }
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r) sh[wave][r][lane] = acc[r];

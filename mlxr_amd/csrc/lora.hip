@@ -7,6 +7,13 @@
 // computes h, K split over workgroups (fp32 partial sums in the workspace); the second adds the
 // partial sums up, multiplies with B and adds y.  Up to kInline tokens, each workgroup of the first
 // finds its tile among the ids by itself; above, a launch before sorts the tokens.
+//
+// Bound by the bytes of A, B and y.  A load of a matrix operand as it lies in its lanes is 16 pieces of 16 bytes for
+// each 16 lanes, which the address path serves at a quarter of what whole rows get: x, A and B are loaded by rows and
+// turned in LDS (64 tokens of rank 128 of 16 adapters: K 28672, N 8192 57 -> 47 us, K 4096, two of 14336 49 -> 39).
+// Measured: 61 tokens of 24 adapters of rank 64, K 8192, two of 28672 (194 MB) shrink 13 us, expand 37 (4.1 TB/s); 2048
+// tokens of 6 adapters of rank 32, K 4096, two of 14336 (259 MB) plan 6, shrink 10, expand 48 (5.0 TB/s); 8 tokens of 16
+// adapters of rank 16, K 4096, 6144 together, one launch 9.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -33,7 +40,9 @@ constexpr int shrink_sub(int rank_groups, int sub) { return sub == 1 || rank_gro
 constexpr int rank_groups_of(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 constexpr int kSplits = 8;  // most splits of K
 constexpr int kPlanThreads = 1024;
-constexpr int kExpandGroups = 1536;  // workgroups of expand: six for each CU
+// Workgroups of expand: six for each CU (61 tokens of rank 64 as above with 1024, 1536, 2048: 55, 50, 52 us; 2000 tokens
+// of 8 adapters of rank 64 164, 151, 149).
+constexpr int kExpandGroups = 1536;
 
 // A tile's adapter (number `adapters`: none), its rank and scale; `count` tokens, order[16 SUB index ..] (0: no tile).
 struct __attribute__((aligned(16))) Tile {
@@ -366,9 +375,9 @@ struct Cols {
 };
 
 // Columns of a wavefront's step, in units of 16: 64 for few tokens (more workgroups), 128 for many: 256 bytes of a
-// row in one store of 16-bit outputs (2048 tokens, two projections of 14336, rank 32: 62 -> 55 us); fewer where B's
-// operands leave few wavefronts on a SIMD (us, with more and with fewer: 2048 tokens of rank 64 128 and 111; rank 128,
-// 64 tokens of 16 adapters, K 4096, two projections of 14336: 64 columns 61, 32 49).
+// row in one store of 16-bit outputs; fewer where B leaves few wavefronts on a SIMD.  us: 2048 tokens of rank 32, two
+// projections of 14336, 64 and 128 columns 71 and 64; 2000 of rank 64 32, 64 and 128 columns 97, 85 and 94; 64 tokens of
+// rank 64, two of 28672, 32 and 64 columns 46 and 42; of rank 128, two of 14336, 39 and 45.
 constexpr int columns_of(int sub, int rank_groups) { return rank_groups == 8 ? 2 : sub == 1 || rank_groups == 4 ? 4 : 8; }
 
 // The bits of x that bf16 has, in the upper half; NaN (whose upper bits may be those of an infinity) quieted.
@@ -635,6 +644,7 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
   if (none && it.out_dev == it.y_dev) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   using E = Expand<F16, RT, 1, WAVES>;
+  static_assert(E::NB >= 2, "turn's room");
   __shared__ u32x4_t rows[WAVES * E::NB * 64];
   E e(a, it, tile, begin, rows);
   if (!none) {
@@ -703,8 +713,8 @@ Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int a
   }
   // One launch where each workgroup's reading of A (at most 128 KiB) is short beside a launch and all of it together
   // at most 16 MiB.  Measured, us, one launch and two (the host needs 4 more for two): rank 16, K 2048, three
-  // projections of 2560 together, 1 token 6.5 and 8.1, 64 tokens 9.3 and 11.4; rank 16, K 4096, 6144, 4 tokens
-  // 10.3 and 9.8, 16 tokens (24 MiB) 16.9 and 12.4; rank 16, K 8192, 10240, 1 token 12.8 and 8.7.
+  // projections of 2560 together, 1 token 5.8 and 7.6, 64 tokens 7.8 and 9.0; rank 16, K 4096, 6144, 4 tokens
+  // 8.7 and 8.6, 16 tokens (24 MiB) 12.3 and 9.9; rank 16, K 8192, 10240, 1 token 8.4 and 7.8; K 14336, 4096, 11.3 and 8.1.
   l.fused = tokens <= kInline && groups <= 2 && (long)rank * K <= 1 << 16 && fused_groups * l.tiles * rank * K <= 1 << 23;
   if (l.fused) {
     l.columns = kFusedThreads;
@@ -714,9 +724,8 @@ Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int a
   const int group = sorted ? 16 * shrink_sub(groups, kSub) : 16;
   // As many splits as the device holds workgroups of shrink at once (two on a CU up to rank 32, else one; a quarter more
   // for sorted tokens, whose adapters' last tiles are partly empty), in chunks of whole steps of the workgroup, two at least.
-  // us, at once / twice that / half: 64 tokens of 16 adapters of rank 128, K 8192, three projections of 10240 together
-  // 62 / 65 / -; 16 tokens of rank 64 there 27 / 28 / -; rank 64, K 28672, 8192, 33 / - / 46; 2048 tokens of 6
-  // adapters of rank 32, K 4096, two of 14336, 66 / 66 / 71.
+  // us, at once, twice that, half: 64 tokens of 16 adapters of rank 128, K 8192, three projections of 10240 together 43,
+  // 46, 51; 16 tokens of rank 64 there 23, 26, 27; 64 of rank 128, K 28672, 8192, 47, 45, 52; 2000 of rank 64 there 67, 73, 85.
   const long want = std::max(1L, 256L * (groups <= 2 ? 2 : 1) * (sorted ? 5 : 4) / 4 / ((long)std::min(tokens, tokens / group + buckets) * items));
   const int most = std::min(kSplits, (K + 1023) / 1024);
   int splits = (int)(want < most ? want : most);

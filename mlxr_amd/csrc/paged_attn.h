@@ -20,6 +20,11 @@
 // kv head) writes the output; others leave (m, sum, unnormalized o) in the workspace, at most two for
 // a wavefront, and a second launch joins them.  Lengths are read on the device; the host chooses by the longest
 // row that the table can hold.
+//
+// Bound by memory: 64 rows of 8 kv heads of 128 in bf16, up to 8192 tokens (961 MB), 156 us and 6 of the join, 6.1 TB/s;
+// one row of 120001 tokens (492 MB) 80 and 6; 32 rows of an e4m3 cache, up to 16384 tokens (547 MB), 92 and 6; 17 rows of 32
+// heads of 80, window 1024, in one launch 38 (158 MB; lines that heads share).  One row of 4 kv heads of 64, 700
+// tokens, 7.4: latency.
 #pragma once
 #include "mfma16.h"
 #include "paged_internal.h"
@@ -179,9 +184,9 @@ struct Attn {
     trow = a.table + (int64_t)r * a.table_stride;
   }
 
-  // Keys and values are read once: past the caches (64 rows of Llama-3-8B heads 180 -> 170 us), unless a row
-  // of a head is not whole 128-byte lines and so shares them with rows that other wavefronts read (32 heads
-  // of 80 in [token, head] order 53 -> 66 us).
+  // Keys and values are read once: past the caches (64 rows of 8 kv heads of 128, up to 8192 tokens, 187 -> 167 us), unless
+  // a row of a head is not whole 128-byte lines and so shares them with rows that other wavefronts read (33 rows of 32
+  // heads of 80 in [token, head] order, window 1024, 69 -> 75 us).
   template <class T>
   static __device__ __forceinline__ T stream_load(const T* p) {
     if constexpr (NT) return __builtin_nontemporal_load(p);
@@ -575,7 +580,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_kernel(At
 
 // One launch for short rows: a workgroup for each (row, kv head, 16 heads), its wavefronts take equal runs of
 // tiles and are merged in LDS.  Four wavefronts: of eight, half as many workgroups fit a CU (64 rows of
-// 32 kv heads, up to 1024 tokens: 101 us, four 95).
+// 32 kv heads, up to 1024 tokens, keys not by way of LDS: 101 us, four 95).
 template <class T, bool LK>
 union RowsLds {
   float park[kWaves / 2][T::PARK * 64];

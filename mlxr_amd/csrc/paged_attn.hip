@@ -103,7 +103,7 @@ constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 3) / 4 * 4 
 // Measured, us, uncut and cut (which also takes the host 4 us more), rows up to the longest, ragged unless one; 8 kv heads of
 // 128 in bf16, up to 512 tokens (256 KiB a head): one row 9.5 and 9.5, 64 rows 18 and 24; 1024: 15 and 11, 4 rows 18 and
 // 12, 16 19 and 17, 64 30 and 37; 2048 (1 MiB): 32 rows 30 and 35, 64 55 and 58; 4096 (2 MiB): 64 rows 103 and 95, 128
-// 171 and 176; 8192: 128 rows 335 and 319.  32 of 128, 4096: 16 rows 102 and 103, 64 315 and 342; 8192: 64 rows 627 and
+// 171 and 176; 8192: 128 rows 335 and 319.  32 of 128, 4096: 33 rows 197 and 176, 64 315 and 342; 8192: 64 rows 627 and
 // 624.  In e4m3, 2048 (512 KiB): 16 rows 22 and 23, 64 33 and 46; 8192: 128 rows 186 and 192.  4 of 64, 2048: one row
 // 18 and 10, 64 20 and 26; 8192: 64 rows 63 and 54.
 Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int width, int window) {
@@ -114,12 +114,12 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int width, int wind
   p.part_rows = p.group < kHeads ? p.group : kHeads;
   const int64_t units = (int64_t)rows * c->kv_heads * p.groups;
   const int64_t bytes = 2 * most * c->head_dim * (c->dtype == MLXR_E4M3 ? 1 : 2);
-  p.one = bytes <= 256 << 10 || (bytes <= 1 << 20 && units >= 256) || (bytes <= 2 << 20 && units >= 1024) || rows > kMaxCutRows ||
+  p.one = bytes <= 256 << 10 || (bytes <= 1 << 20 && units >= 256) || (bytes <= 2 << 20 && units >= 2048) || rows > kMaxCutRows ||
           (held / kTile + 1) * rows > INT32_MAX || (held / kTile + 1) * units / 64 > INT32_MAX;  // what a cut launch counts in 32 bits
   // Rows of more than 256 KiB: two workgroups of a CU, not the three or four that its registers hold, by LDS that they do
   // not use.  Later workgroups then start where rows turn out short, and lines that heads share stay in the L2.  us, three
   // or four and two: 32 kv heads of 80 in [token, head] order, 1024 tokens, 17 rows 57 and 43, 48 rows 112 and 104; 32 of
-  // 128, up to 1024, 17 rows 38 and 36, 200 rows 259 and 264; 4 of 64, up to 2048, 200 rows 56 and 48; below: 32 of 80,
+  // 128, up to 1024, 17 rows 38 and 36, 200 rows 259 and 262; 4 of 64, up to 2048, 200 rows 56 and 48; below: 32 of 80,
   // 256 tokens, 100 rows 40 and 47; 8 of 128, up to 300, 200 rows 30 and 33.  (Above 128 dims one is resident.)
   p.two_of_cu = bytes > 256 << 10 && c->head_dim <= 128;
   p.keys_in_lds = units >= device_cu_count();  // fewer: latency counts (load_k)

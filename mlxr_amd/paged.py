@@ -253,6 +253,9 @@ class PagedKVCache:
     def append(self, layer, k, v, slots, stream=None):
         paged_append(k, v, self.k[layer], self.v[layer], slots, self.k_scale, self.v_scale, stream=stream)
 
-    def attend(self, layer, q, **options):
-        return paged_attention(q, self.k[layer], self.v[layer], self.table, self.lens, k_scale=self.k_scale,
+    def attend(self, layer, q, longest=None, **options):
+        """paged_attention over the rows of a layer.  ``longest``: no row holds more tokens (None: not known), which
+        the split of the work goes by; tokens past it would be left out."""
+        table = self.table if longest is None else self.table[:, :max(1, -(-longest // self.page_size))]
+        return paged_attention(q, self.k[layer], self.v[layer], table, self.lens, k_scale=self.k_scale,
                                v_scale=self.v_scale, **options)

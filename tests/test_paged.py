@@ -744,6 +744,23 @@ def test_paged_cache_class(cuda):
 
 
 @pytest.mark.gpu
+def test_attend_with_a_bound_on_the_lengths(cuda):
+    """A bound that holds changes the split, not the result; what lies past one that does not is left out."""
+    import torch
+    c = mx.PagedKVCache(1, 600, 8, 2, 64, 2, 2400, device=cuda)
+    r = c.resize(torch.tensor([37, 5], dtype=torch.int32, device=cuda), 64)
+    torch.manual_seed(2)
+    k, v = torch.randn(2, 64, 2, 64, device=cuda).to(torch.bfloat16)
+    c.append(0, k, v, r.slots)
+    q = torch.randn(2, 4, 64, device=cuda).to(torch.bfloat16)
+    keys, values = ([t[:37].double().cpu(), t[37:42].double().cpu()] for t in (k, v))
+    for longest, lens in ((None, [37, 5]), (37, [37, 5]), (40, [37, 5]), (16, [16, 5]), (0, [8, 5])):
+        got = c.attend(0, q, longest=longest, out_dtype=torch.float32)
+        ref, _ = _attend64(q, [t[:n] for t, n in zip(keys, lens)], [t[:n] for t, n in zip(values, lens)], lens, 0, 0.125)
+        _check(got, ref, [t[:n] for t, n in zip(values, lens)], lens, "f32")
+
+
+@pytest.mark.gpu
 def test_wrapper_refusals_on_the_gpu(cuda):
     import torch
     i32 = dict(dtype=torch.int32, device=cuda)

@@ -92,13 +92,23 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   const int nb = a.adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int *count = sh, *next = sh + nb;
   __shared__ int part[kPlanThreads / 64];
+  const int per = (nb + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, nb), b1 = min(b0 + per, nb);
+  auto load = [&](int (&id)[AHEAD], int t0) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) id[k] = a.ids[min(t0 + k * kPlanThreads, a.tokens - 1)];
+  };
+  int first[AHEAD];
+  load(first, tid);
+  const Tile mine = tile_of(a, min(b0, a.adapters), 0);  // on its way while the tokens are counted
   for (int b = tid; b < nb; b += kPlanThreads) count[b] = 0;
   __syncthreads();
   auto each = [&](auto&& f) {
     for (int t0 = tid; t0 < a.tokens; t0 += AHEAD * kPlanThreads) {
       int id[AHEAD];
+      if (t0 == tid)
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) id[k] = a.ids[min(t0 + k * kPlanThreads, a.tokens - 1)];
+        for (int k = 0; k < AHEAD; ++k) id[k] = first[k];
+      else load(id, t0);
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)
         if (const int t = t0 + k * kPlanThreads; t < a.tokens) f(t, id[k] >= 0 && id[k] < a.adapters ? id[k] : a.adapters);
@@ -107,7 +117,6 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   // one atomic for the lanes of a wavefront that share a bucket: neighbouring tokens often do
   each([&](int, int b) { wave_add(count, b); });
   __syncthreads();
-  const int per = (nb + kPlanThreads - 1) / kPlanThreads, b0 = min(tid * per, nb), b1 = min(b0 + per, nb);
   int m = 0;
   for (int b = b0; b < b1; ++b) m += (count[b] + TM - 1) / TM;
   int sum = m;
@@ -126,7 +135,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(LoraArgs a) {
   for (int b = b0; b < b1; ++b) {
     const int c = count[b];
     next[b] = tile * TM;
-    Tile t = tile_of(a, b, 0);
+    Tile t = b == b0 ? mine : tile_of(a, b, 0);
     for (int i = 0; i < c; i += TM) {
       t.count = min(TM, c - i);
       a.tiles[tile++] = t;

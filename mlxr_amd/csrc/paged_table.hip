@@ -201,16 +201,42 @@ struct Eight {
   }
 };
 __device__ __forceinline__ uint32_t e4m3x4(const float* v) {
-  float c[4];
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+}
+template <int N>
+__device__ __forceinline__ float largest(const float (&v)[N]) {
+  float top = 0.f;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) c[k] = v[k] > 448.f ? 448.f : v[k] < -448.f ? -448.f : v[k];  // NaN stays
-  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
+  for (int n = 0; n < N; ++n) top = fmaxf(top, fabsf(v[n]));
+  return top;
+}
+
+// v / d rounded as division does, for what becomes e4m3: a reciprocal for all of them and two corrections each, the last
+// of which is exact (Markstein's theorem: q within an ulp, r the rounded reciprocal, the residue exact).  That holds
+// where nothing overflows or comes near the smallest numbers; quotients below 2^-10 become 0 whatever their bits, of v's
+// sign.  (4099 tokens as below: 10.5 us with divisions and every value clamped, 8.3 now, 6.1 without scales.)
+template <int N>
+__device__ __forceinline__ void divide(float (&v)[N], float d) {
+  const float r = 1.f / d;
+  float q[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) q[n] = v[n] * r;
+  if (largest(q) < 0x1p80f && fabsf(d) > 0x1p-40f && fabsf(d) < 0x1p40f) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float q1 = __builtin_fmaf(__builtin_fmaf(-q[n], d, v[n]), r, q[n]);
+      v[n] = copysignf(__builtin_fmaf(__builtin_fmaf(-q1, d, v[n]), r, q1), q[n]);
+    }
+  } else {
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] /= d;
+  }
 }
 
 // One thread moves 16 bytes of a store, for the keys and the values: 8 or 16 elements of one head's row of one
 // token.  Bound by memory for a prompt (4099 tokens
-// of 8 heads of 128, bf16 to e4m3 with scales, 25 MB, 10.5 us) and by the launch for a decode batch (64 tokens 2.5 us).
+// of 8 heads of 128, bf16 to e4m3 with scales, 25 MB, 8.3 us) and by the launch for a decode batch (64 tokens 2.5 us).
 template <int XT, int CT>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   constexpr int N = CT == MLXR_E4M3 ? 16 : 8;
@@ -240,10 +266,17 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     for (int n = 0; n < N; ++n) v[n] = x[k][n / 8].get(n % 8);
     if (s.scale) {
       const float d = s.scale[h];
+      if constexpr (CT == MLXR_E4M3) {
+        divide(v, d);
+      } else {
 #pragma unroll
-      for (int n = 0; n < N; ++n) v[n] /= d;
+        for (int n = 0; n < N; ++n) v[n] /= d;
+      }
     }
     if constexpr (CT == MLXR_E4M3) {
+      if (largest(v) > 448.f)
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = v[n] > 448.f ? 448.f : v[n] < -448.f ? -448.f : v[n];  // NaN stays
       *(uint4*)(s.store + to) = make_uint4(e4m3x4(v), e4m3x4(v + 4), e4m3x4(v + 8), e4m3x4(v + 12));
     } else {
       uint32_t o[4];

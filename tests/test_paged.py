@@ -321,6 +321,28 @@ def test_append_divides_as_division_does(cuda, cache):
 
 
 @pytest.mark.gpu
+def test_append_of_every_bf16_value_divided_to_e4m3(cuda):
+    """All 65536 values by scales of ordinary size, those among them whose multiples lie next to middles of e4m3 values; zeros
+    keep their sign."""
+    import torch
+    g = torch.Generator().manual_seed(8)
+    near = [(2 ** 20 * m + e) * 2.0 ** (k - 23) for m in range(9, 16) for e in (-3, -1, 1, 2) for k in (-6, 5)]
+    scales = torch.tensor((near + [1.0, -0.125, 3.0, 448.0])[:60] + [2.0 ** -39, 2.0 ** 39, 2.0 ** -41, 2.0 ** 41])
+    assert scales.shape == (64,)
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)[torch.randperm(65536, generator=g)]
+    x = x.view(1024, 1, 64).expand(1024, 64, 64)
+    store = torch.zeros((32, 64, 32, 64), dtype=torch.float8_e4m3fn, device=cuda)
+    slots = torch.arange(1024, dtype=torch.int32, device=cuda)
+    s = scales.to(cuda)
+    mx.paged_append(x.to(cuda), x.to(cuda), store, torch.empty_like(store), slots, s, s)
+    want = (x.float() / scales[None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    got = store.permute(0, 2, 1, 3).reshape(1024, 64, 64).cpu()
+    nan = torch.isnan(want.float())
+    assert torch.equal(torch.isnan(got.float()), nan)
+    assert torch.equal(got.view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
+
+
+@pytest.mark.gpu
 def test_append_takes_slices_of_a_fused_projection(cuda):
     import torch
     heads, dim, n, page, pages = 4, 64, 9, 16, 3

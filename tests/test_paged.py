@@ -515,6 +515,17 @@ def test_attention_cut_and_uncut(cuda, dtype, cache, heads, kv, dim, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f8"), ("f16", "f8")])
+@pytest.mark.parametrize("heads,dim,page,window", [(16, 16, 8, 0), (32, 48, 16, 0), (16, 64, 16, 0), (32, 64, 40, 37), (16, 80, 16, 0),
+                                                   (16, 96, 8, 300), (32, 112, 32, 0), (48, 128, 16, 0), (16, 128, 64, 100), (16, 256, 16, 0),
+                                                   (16, 80, 6, 0)])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_attention_that_fills_the_device(cuda, dtype, cache, heads, dim, page, window, token_major):
+    """As many kv heads of all rows as there are CUs: keys go through LDS where pages allow it."""
+    _run(cuda, LENS, heads, 16, dim, page, dtype, cache, window=window, token_major=token_major, seed=heads + dim + page)
+
+
+@pytest.mark.gpu
 def test_attention_of_many_rows(cuda):
     _run(cuda, [(i * 5) % 40 for i in range(5000)], 2, 1, 64, 16, "bf16", "bf16")
     _run(cuda, [(i * 7) % 50 for i in range(2500)], 4, 2, 64, 8, "bf16", "bf16")

@@ -345,7 +345,8 @@ __global__ __launch_bounds__(kShrinkThreads) void shrink_kernel(LoraArgs a) {
   }
 }
 
-// CT neighbouring columns of a token's row of y, as they lie in memory (YT: the type).
+// CT neighbouring columns of a token's row of y, as they lie in memory (YT: the type), in accesses of up to 16 bytes at
+// any element: rows of odd widths start anywhere.
 template <int YT, int CT>
 struct Cols {
   static constexpr int S = YT == DT_F32 ? 4 : 2, W = CT * S / 4;  // bytes of an element; words
@@ -353,17 +354,11 @@ struct Cols {
   // other: 16 bytes that are read, and not used, where `in` is false: the load is unconditional
   __device__ __forceinline__ void load(const mlxr_lora_item& it, int64_t at, bool in, const void* other) {
     const uint8_t* p = in ? (const uint8_t*)it.y_dev + at * S : (const uint8_t*)other;
-    if constexpr (W == 1) {
-      w[0] = *(const uint32_t*)p;
-    } else if constexpr (W == 2) {
-      const u32x2_t v = *(const u32x2_t*)p;
-      w[0] = v.x, w[1] = v.y;
+    if constexpr (W <= 4) {
+      __builtin_memcpy(w, p, 4 * W);
     } else {
 #pragma unroll
-      for (int k = 0; k < W; k += 4) {
-        const u32x4_t v = *(const u32x4_t*)(p + (in ? 4 * k : 0));
-        w[k] = v.x, w[k + 1] = v.y, w[k + 2] = v.z, w[k + 3] = v.w;
-      }
+      for (int k = 0; k < W; k += 4) __builtin_memcpy(w + k, p + (in ? 4 * k : 0), 16);
     }
   }
   // out = y + v * back
@@ -375,11 +370,8 @@ struct Cols {
       else o[k] = pack2<YT == DT_F16>(unpack<YT == DT_F16>(w[k], 0) + v[2 * k] * back, unpack<YT == DT_F16>(w[k], 1) + v[2 * k + 1] * back);
     }
     uint8_t* p = (uint8_t*)it.out_dev + at * S;
-    if constexpr (W == 1) *(uint32_t*)p = o[0];
-    else if constexpr (W == 2) *(u32x2_t*)p = u32x2_t{o[0], o[1]};
-    else
 #pragma unroll
-      for (int k = 0; k < W; k += 4) *(u32x4_t*)(p + 4 * k) = u32x4_t{o[k], o[k + 1], o[k + 2], o[k + 3]};
+    for (int k = 0; k < W; k += 4) __builtin_memcpy(p + 4 * k, o + k, W < 4 ? 4 * W : 16);
   }
 };
 
@@ -496,22 +488,32 @@ struct Expand {
     }
     return b;
   }
-  // hs: the tile's rows of h; none: the tokens have no adapter.  VEC: rows of y and out start at multiples of 16
-  // bytes and are whole groups of CT columns.
+  // The steps before n0 = stop.  hs: the tile's rows of h; none: the tokens have no adapter.  VEC: these steps hold no
+  // part of a group of CT columns.
   template <int YT, bool VEC>
-  __device__ __forceinline__ void columns(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
+  __device__ __forceinline__ void columns(int stop, const int* token, int count, bool none, const uint16_t* hs, const float* back) {
     constexpr bool AHEAD = VEC && SUB > 1 && YT != DT_F32;  // y of the next 16 tokens on its way: fp32 has no registers for it
-    for (; n0 < end; n0 += STEP) {
+    for (; n0 < stop; n0 += STEP) {
       store_b();
       const int n = n0 + CT * col, left = it.N - n;
       Cols<YT, CT> y[4];
+      uint32_t bits[VEC ? 1 : 4][VEC ? 1 : CT];  // of single elements of y
       auto load_y = [&](Cols<YT, CT>(&to)[4], int s) {
-        if constexpr (VEC)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int t = 16 * s + 4 * g + i;
-            to[i].load(it, (int64_t)token[t < count ? t : 0] * it.N + n, left > 0 && t < count, B);
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * s + 4 * g + i;
+          const int64_t at = (int64_t)token[t < count ? t : 0] * it.N + n;
+          if constexpr (VEC) {
+            to[i].load(it, at, left > 0 && t < count, B);
+          } else {
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+              bits[i][c] = 0;
+              if (t < count && c < left)
+                bits[i][c] = YT == DT_F32 ? ((const uint32_t*)it.y_dev)[at + c] : ((const uint16_t*)it.y_dev)[at + c];
+            }
           }
+        }
       };
       load_y(y, 0);
       asm volatile("" ::: "memory");  // the loads stay in this order: what waits for y would wait for those before it too
@@ -568,7 +570,11 @@ struct Expand {
           } else {
 #pragma unroll
             for (int c = 0; c < CT; ++c)
-              if (c < left) store_scalar(it.out_dev, YT, at + c, load_scalar(it.y_dev, YT, at + c) + acc[c][i] * f);
+              if (c < left) {
+                const uint32_t b = bits[i][c];
+                const float y0 = YT == DT_F32 ? __builtin_bit_cast(float, b) : unpack<YT == DT_F16>(b, 0);
+                store_scalar(it.out_dev, YT, at + c, y0 + acc[c][i] * f);
+              }
           }
         }
         if constexpr (AHEAD) {
@@ -582,9 +588,9 @@ struct Expand {
   }
   template <int YT>
   __device__ __forceinline__ void columns(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
-    const bool vec = it.N % CT == 0 && it.N * (YT == DT_F32 ? 4 : 2) % 16 == 0 && (((uintptr_t)it.y_dev | (uintptr_t)it.out_dev) & 15) == 0;
-    if (vec) columns<YT, true>(token, count, none, hs, back);
-    else columns<YT, false>(token, count, none, hs, back);
+    // a row's last columns, where they are fewer than CT, one by one with the others of their step
+    columns<YT, true>(it.N % CT ? min(end, it.N - 16 * CT + 1) : end, token, count, none, hs, back);
+    if (it.N % CT) columns<YT, false>(end, token, count, none, hs, back);
   }
   __device__ __forceinline__ void run(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
     if (it.y_dtype == DT_BF16) columns<DT_BF16>(token, count, none, hs, back);

@@ -553,7 +553,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void attn_kernel(At
     else hi = mid;
   }
   int r = __builtin_amdgcn_readfirstlane(lo);
-  constexpr bool LK = P8 && DT < 256;  // above, a workgroup's keys would be 64 KiB
+  constexpr bool LK = P8;
   using T = Attn<F16, F8, DT, DIM, P8, LK>;
   __shared__ u32x4_t keys[LK ? kWaves : 1][LK ? kTile * T::CH : 1];
   T t(a, keys[LK ? wave : 0]);
@@ -640,7 +640,7 @@ template <bool F16, bool F8>
 AttnKern& kern_of(int dim, bool p8) {
 #define MLXR_ATTN(DT, DIM, P8)                                                                                              \
   {                                                                                                                        \
-    constexpr bool LK = P8 && DT < 256;                                                                                    \
+    constexpr bool LK = P8;                                                                                    \
     static AttnKern k{(const void*)attn_kernel<F16, F8, DT, DIM, P8>,                                                      \
                       {(const void*)attn_rows_kernel<F16, F8, DT, DIM, P8, false>,                                         \
                        (const void*)attn_rows_kernel<F16, F8, DT, DIM, P8, LK>},                                           \

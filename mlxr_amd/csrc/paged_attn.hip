@@ -122,7 +122,10 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int heads, int width, int wind
   // 128, up to 1024, 17 rows 38 and 36, 200 rows 259 and 262; 4 of 64, up to 2048, 200 rows 56 and 48; below: 32 of 80,
   // 256 tokens, 100 rows 40 and 47; 8 of 128, up to 300, 200 rows 30 and 33.  (Above 128 dims one is resident.)
   p.two_of_cu = bytes > 256 << 10 && c->head_dim <= 128;
-  p.keys_in_lds = units >= device_cu_count();  // fewer: latency counts (load_k)
+  // Where latency does not count (load_k): a workgroup for each CU, two tiles for a wavefront.  us, straight and through
+  // LDS, 128 rows of 8 kv heads of 128 in bf16, up to 34 tokens 10.1 and 11.2, 100 13.1 and 13.7, 200 17.2 and 16.9, 1000 55
+  // and 47; of 256, 100 37.3 and 37.1, 400 65 and 57, 1000 119 and 94; in e4m3 of 128, 200 14.7 and 14.7, 1000 33 and 29.
+  p.keys_in_lds = units >= device_cu_count() && most >= 2 * kWaves * kTile;
   p.bytes = p.one ? 0 : prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * kWaves * 2 *
                                                  partial_floats(p.part_rows, c->head_dim) * sizeof(float);
   return p;

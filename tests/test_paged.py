@@ -777,6 +777,22 @@ def test_paged_cache_class(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [128, 256])
+def test_attention_of_as_many_rows_as_are_cut(cuda, dim):
+    """4096 rows of a table that could hold long ones: their tiles are summed up beside the keys in LDS; 4097 rows are not cut."""
+    import torch
+    lens = [(i * 11) % 70 for i in range(4097)]
+    (k, v), table, (keys, values) = _fill(cuda, lens, 1, dim, 16, "bf16", False, 3, 1.0)
+    wide = torch.nn.functional.pad(table, (0, 300), value=-1)
+    q = torch.randn(4097, 2, dim, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).to(cuda)
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    ref, _ = _attend64(q, keys, values, lens, 0, dim ** -0.5)
+    for n in (4096, 4097):
+        got = mx.paged_attention(q[:n], k, v, wide[:n], lt[:n], out_dtype=torch.float32)
+        _check(got, ref[:n], values[:n], lens[:n], "f32")
+
+
+@pytest.mark.gpu
 def test_attend_with_a_bound_on_the_lengths(cuda):
     """A bound that holds changes the split, not the result; what lies past one that does not is left out."""
     import torch

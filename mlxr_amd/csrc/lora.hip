@@ -17,7 +17,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "../../include/mlxr_lora.h"
 #include "mfma16.h"
@@ -734,7 +733,8 @@ Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int a
   // for sorted tokens, whose adapters' last tiles are partly empty), in chunks of whole steps of the workgroup, two at least.
   // us, at once, twice that, half: 64 tokens of 16 adapters of rank 128, K 8192, three projections of 10240 together 43,
   // 46, 51; 16 tokens of rank 64 there 23, 26, 27; 64 of rank 128, K 28672, 8192, 47, 45, 52; 2000 of rank 64 there 67, 73, 85.
-  const long want = std::max(1L, 256L * (groups <= 2 ? 2 : 1) * (sorted ? 5 : 4) / 4 / ((long)std::min(tokens, tokens / group + buckets) * items));
+  const long places = 256L * (groups <= 2 ? 2 : 1) * (sorted ? 5 : 4) / 4;
+  const long want = std::max(1L, places / ((long)std::min(tokens, tokens / group + buckets) * items));
   const int most = std::min(kSplits, (K + 1023) / 1024);
   int splits = (int)(want < most ? want : most);
   l.chunk = ((K + splits - 1) / splits + kShrinkThreads - 1) / kShrinkThreads * kShrinkThreads;

@@ -98,8 +98,9 @@ struct Plan {
   size_t bytes;                      // of the workspace
 };
 constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 3) / 4 * 4 * sizeof(int32_t); }
-// By the longest row that the table can hold, or the window; a window never needs more workspace.  A workgroup alone gets about 38 GB/s, so few rows have
-// to be cut unless they are short; many rows fill the device uncut, until the longest keeps it waiting.
+// By the longest row that the table can hold, or the window; a window never needs more workspace.  A workgroup alone
+// gets about 38 GB/s, so few rows have to be cut unless they are short; many rows fill the device uncut, until the longest
+// keeps it waiting.
 // Measured, us, uncut and cut (which also takes the host 4 us more), rows up to the longest, ragged unless one; 8 kv heads of
 // 128 in bf16, up to 512 tokens (256 KiB a head): one row 9.5 and 9.5, 64 rows 18 and 24; 1024: 15 and 11, 4 rows 18 and
 // 12, 16 19 and 17, 64 30 and 37; 2048 (1 MiB): 32 rows 30 and 35, 64 55 and 58; 4096 (2 MiB): 64 rows 103 and 95, 128

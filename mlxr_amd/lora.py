@@ -83,7 +83,8 @@ def lora_apply(x, ids, a, b, y, scales=None, ranks=None, outs=None, stream=None)
         if len(bs) != 3 or bs[0] != adapters or bs[2] != rank:
             raise QGemmError(-3, f"b[{i}] must be [{adapters}, N, {rank}]")
         N = bs[1]
-        if A.dtype is not xt or B.dtype is not xt or A.get_device() != index or B.get_device() != index or not A.is_contiguous() or not B.is_contiguous():
+        if A.dtype is not xt or B.dtype is not xt or A.get_device() != index or B.get_device() != index or \
+                not A.is_contiguous() or not B.is_contiguous():
             raise QGemmError(-1, f"a[{i}] and b[{i}] must be contiguous, of x's dtype and device")
         if len(ts) != 2 or ts[0] != tokens or ts[1] != N or t.get_device() != index or not t.is_contiguous() or \
                 given and (o.shape != ts or o.dtype is not t.dtype or o.get_device() != index or not o.is_contiguous()):
@@ -93,8 +94,8 @@ def lora_apply(x, ids, a, b, y, scales=None, ranks=None, outs=None, stream=None)
     qgemm._check(lib.mlxr_lora_workspace_size(n, items, tokens, K, adapters, rank, ctypes.byref(nb)))
     nb = nb.value
     ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=x.device) if nb else None
-    qgemm._check(lib.mlxr_lora_apply(n, items, tokens, K, adapters, rank, x.data_ptr(), dt, xs[0], pi, ps, pr, ws.data_ptr() if nb else None, nb,
-                                     _stream(stream, index)))
+    qgemm._check(lib.mlxr_lora_apply(n, items, tokens, K, adapters, rank, x.data_ptr(), dt, xs[0], pi, ps, pr,
+                                     ws.data_ptr() if nb else None, nb, _stream(stream, index)))
     return outs
 
 

@@ -218,7 +218,8 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
     qs = q.stride()
     qgemm._check(lib.mlxr_paged_attention(c, rows, heads, q.data_ptr(), dt, qs[0], qs[1], pt, table.stride()[0], width, pl,
                                           dim ** -0.5 if scale is None else scale, window, out.data_ptr(), odt,
-                                          lse.data_ptr() if return_lse else None, ws.data_ptr() if nb else None, nb, _stream(stream, index)))
+                                          lse.data_ptr() if return_lse else None, ws.data_ptr() if nb else None, nb,
+                                          _stream(stream, index)))
     return (out, lse) if return_lse else out
 
 

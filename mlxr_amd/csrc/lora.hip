@@ -205,6 +205,14 @@ __device__ __forceinline__ Tile found_tile(const LoraArgs& a, int index, int* to
   return t;
 }
 
+// Stands between accesses of a wavefront to LDS by which one lane sees or replaces what another wrote or read.  The hardware
+// keeps a wavefront's accesses in order; only the compiler has to be told, which sees one lane's addresses.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // 16 rows of x or A by 64 k: a lane loads 16 bytes of rows lane / 8 and 8 + lane / 8, part lane % 8 of the 128, so that
 // rows are read whole; turn makes operands of them by way of 2 KiB of LDS that the wavefront has for itself.  Which k an
 // operand's place stands for is free, alike for x and A.  (An operand's own load would be 16 pieces.)
@@ -213,15 +221,10 @@ __device__ __forceinline__ void turn(u32x4_t (&v)[2], u32x4_t* buf) {
   // 8 lanes that read or write at once, and so 128 bytes, lie in different banks
   buf[row * 8 + (part ^ row)] = v[0];
   buf[(row + 8) * 8 + (part ^ row)] = v[1];
-  // a wavefront's accesses to LDS are in order: only the compiler has to keep them so
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  wave_sync();
   v[0] = buf[col * 8 + (g ^ (col & 7))];
   v[1] = buf[col * 8 + ((4 + g) ^ (col & 7))];
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  wave_sync();
 }
 
 // h of SS groups of 16 tokens of a tile over one chunk of K: the wavefronts take turns over it in steps of 64
@@ -458,15 +461,13 @@ struct Expand {
   // Place of part `part` of column n of a step: 8 lanes that read or write at once, and so 128 bytes, lie in different banks.
   static __device__ __forceinline__ int place(int n, int part) { return (n * C + part) ^ (n / CT & 7); }
   __device__ __forceinline__ void store_b() {
+    wave_sync();  // other lanes' reads of the step before
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int at = i * 64 + (threadIdx.x & 63);
       rows[place(at / C, at % C)] = next[i];
     }
-    // a wavefront's accesses to LDS are in order: only the compiler has to keep them so
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_sync();
   }
   // RT 1 multiplies the high and the low parts in one product, ranks 8 (g & 1) ..
   __device__ __forceinline__ int rank_at(int k) const { return RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g; }

@@ -141,6 +141,18 @@ def test_lora(cuda, dtype, tokens, K, adapters, rank, widths):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,ydt", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32")])
+@pytest.mark.parametrize("tokens,K,adapters,rank,N", [
+    (256, 4352, 1, 16, 43693), (256, 2560, 1, 32, 43776), (256, 128, 1, 64, 43693), (256, 128, 1, 128, 21851),
+    (300, 64, 60, 16, 24208), (300, 64, 60, 16, 24203), (300, 64, 60, 64, 12107), (300, 64, 60, 128, 6101)])
+def test_lora_of_wide_projections(cuda, dtype, ydt, tokens, K, adapters, rank, N):
+    """Two to four steps of columns to a workgroup of the second product, for each of its forms: rows of B of the step
+    after on their way, their place in LDS used again, widths that end inside a lane's columns."""
+    ids = [(7 * t) % (adapters + 1) - 1 if t < 120 else adapters - 1 for t in range(tokens)]
+    _run(cuda, tokens, K, adapters, rank, [N], dtype, ydt, seed=rank, ids=ids)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("ydt", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_lora_output_types(cuda, dtype, ydt):

@@ -10,9 +10,9 @@
 // 8 b + 4 hh + i, so the scores that a lane holds (heads across lanes, rows 4 g .. 4 g + 3 for lane
 // group g) are those of tokens 8 g .. 8 g + 7, which is what the second product wants in that lane
 // as its operand: P never leaves the registers, and the softmax's factors are one value per lane.
-// P is split in two 16-bit parts, hi + lo (together 2^-16 in bf16): with one part its rounding
-// would be as large as the output's own.  A second product costs matrix cycles that the kernel, bound by
-// memory, has to spare.
+// P is split in 16-bit parts that add up to it: three in bf16 (all bits of fp32), two in f16 (22 bits), which an e4m3
+// cache's values, exact in either type, take too.  More products cost matrix cycles that the kernel, bound by memory, has to
+// spare.
 //
 // Short rows: a workgroup for each (row, kv head), merged in LDS (attn_rows_kernel).  Long ones are cut
 // evenly (attn_kernel): the tiles (32 tokens) of all rows and kv heads, in one sequence, are dealt to the
@@ -127,7 +127,7 @@ __device__ __forceinline__ void store_values(void* out, int dtype, int64_t i, co
   }
 }
 
-// F16: the products' type (else bf16).  F8: the cache is e4m3.  DT: 64, 96, 128 or 256, at least dim (DIM:
+// F16: the type of the queries' product (else bf16).  F8: the cache is e4m3.  DT: 64, 96, 128 or 256, at least dim (DIM:
 // equal; 96: above 64, not for e4m3; 128: above that).  P8: page_size % 8 == 0.
 // LK: keys through LDS (load_k).
 template <bool F16, bool F8, int DT, bool DIM, bool P8, bool LK>
@@ -136,9 +136,11 @@ struct Attn {
   static constexpr int VE = DT == 64 ? 4 : 8;      // neighbouring values of a token that a lane loads
   static constexpr int VH = DT == 256 ? 2 : 1;     // times that
   static constexpr int NC = VH * VE;               // accumulators
+  static constexpr bool P16 = F16 || F8;           // the second product's type, f16 or else bf16
+  static constexpr int PARTS = P16 ? 2 : 3;        // of P
   // p times 2^14 in f16: weights down to 2^-28 of the largest stay normal numbers (bf16 has the range)
-  static constexpr float SHIFT = F16 ? 14.f : 0.f;
-  static constexpr float UNSHIFT = F16 ? 0x1p-14f : 1.f;
+  static constexpr float SHIFT = P16 ? 14.f : 0.f;
+  static constexpr float UNSHIFT = P16 ? 0x1p-14f : 1.f;
   static constexpr bool NT = DIM && DT * (F8 ? 1 : 2) % 128 == 0;  // past the caches
   static constexpr int KL = F8 ? KS / 2 : KS;      // 16-byte parts of a key row in a lane's operands
   // Keys through LDS: parts of a row, tokens of a load, loads of a tile.
@@ -319,11 +321,11 @@ struct Attn {
   // Word w (dims 2 w, 2 w + 1 of the lane's VE) of token j, as a pair of 16-bit floats.
   template <int W>
   __device__ __forceinline__ uint32_t v_word(int x, int j) const {
-    if constexpr (F8) return widen<F16, (W & 1) != 0>(vr[x][j][W >> 1]);
+    if constexpr (F8) return widen<P16, (W & 1) != 0>(vr[x][j][W >> 1]);
     else return vr[x][j][W];
   }
   template <int W>
-  __device__ __forceinline__ void add_v(int x, u32x4_t hi, u32x4_t lo) {
+  __device__ __forceinline__ void add_v(int x, const u32x4_t (&p)[PARTS]) {
     if constexpr (W < VE / 2) {
       uint32_t w[8];
 #pragma unroll
@@ -334,10 +336,10 @@ struct Attn {
 #pragma unroll
         for (int k = 0; k < 4; ++k) f[k] = __builtin_amdgcn_perm(w[2 * k + 1], w[2 * k], odd ? 0x07060302u : 0x05040100u);
         const int c = x * VE + 2 * W + odd;
-        o[c] = mfma16<F16>(f, lo, o[c]);
-        o[c] = mfma16<F16>(f, hi, o[c]);
+#pragma unroll
+        for (int k = PARTS - 1; k >= 0; --k) o[c] = mfma16<P16>(f, p[k], o[c]);
       }
-      add_v<W + 1>(x, hi, lo);
+      add_v<W + 1>(x, p);
     }
   }
 
@@ -363,11 +365,11 @@ struct Attn {
       scores(x);
       load_k(ids, t1, more);
       const bool full = __ballot(live != 0xff) == 0;
-      u32x4_t hi, lo;
-      weights(x, live, full, &hi, &lo);
+      u32x4_t p[PARTS];
+      weights(x, live, full, p);
       if (!full) drop(live);
 #pragma unroll
-      for (int xh = 0; xh < VH; ++xh) add_v<0>(xh, hi, lo);
+      for (int xh = 0; xh < VH; ++xh) add_v<0>(xh, p);
       load_v(ids, t1, more);
       asm volatile("" ::: "memory");  // the loads stay here, or what waits for the keys would wait for the values too
       if (!more) break;
@@ -377,18 +379,22 @@ struct Attn {
     }
   }
 
-  // Two weights as the sum of two 16-bit parts, neither of them negative nor, beside a weight above 0, the second 0:
-  // an infinite value then gives an infinite output as a weight in one piece does, not NaN.  (The least
-  // second part, 2^-126 or 2^-38 of the largest weight, is far below the rounding of the sums.)
-  static __device__ __forceinline__ void split2(float p0, float p1, uint32_t* hi, uint32_t* lo) {
-    if constexpr (F16) {
-      *hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-      *lo = pack2<true>(fmaxf(p0 - unpack<true>(*hi, 0), 0x1p-24f), fmaxf(p1 - unpack<true>(*hi, 1), 0x1p-24f));
+  // Pair k of two weights in parts, neither of them negative nor, beside a weight above 0, a later one 0: an infinite value
+  // then gives an infinite output as a weight in one piece does, not NaN.  (The least later part, 2^-126 or 2^-38 of the
+  // largest weight, is far below the rounding of the sums.)
+  static __device__ __forceinline__ void split2(float p0, float p1, u32x4_t (&p)[PARTS], int k) {
+    if constexpr (P16) {
+      const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+      p[0][k] = hi;
+      p[1][k] = pack2<true>(fmaxf(p0 - unpack<true>(hi, 0), 0x1p-24f), fmaxf(p1 - unpack<true>(hi, 1), 0x1p-24f));
     } else {
-      const uint32_t b0 = __builtin_bit_cast(uint32_t, p0), b1 = __builtin_bit_cast(uint32_t, p1);
-      *hi = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-      *lo = pack2<false>(fmaxf(p0 - __builtin_bit_cast(float, b0 & 0xffff0000u), 0x1p-126f),
-                         fmaxf(p1 - __builtin_bit_cast(float, b1 & 0xffff0000u), 0x1p-126f));
+#pragma unroll
+      for (int n = 0; n < PARTS; ++n) {  // each the upper half of what is left; the last holds all of it
+        const uint32_t b0 = __builtin_bit_cast(uint32_t, p0), b1 = __builtin_bit_cast(uint32_t, p1);
+        p[n][k] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+        p0 = fmaxf(p0 - __builtin_bit_cast(float, b0 & 0xffff0000u), 0x1p-126f);
+        p1 = fmaxf(p1 - __builtin_bit_cast(float, b1 & 0xffff0000u), 0x1p-126f);
+      }
     }
   }
 
@@ -419,7 +425,7 @@ struct Attn {
     }
   }
 
-  __device__ __forceinline__ void weights(const f32x4_t (&s)[2], uint32_t live, bool full, u32x4_t* hi, u32x4_t* lo) {
+  __device__ __forceinline__ void weights(const f32x4_t (&s)[2], uint32_t live, bool full, u32x4_t (&p)[PARTS]) {
     float x[8], top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * sc;
@@ -440,10 +446,7 @@ struct Attn {
     for (int k = 0; k < 4; ++k) {
       const float p0 = __builtin_amdgcn_exp2f(x[2 * k] + off), p1 = __builtin_amdgcn_exp2f(x[2 * k + 1] + off);
       sum += p0 + p1;
-      uint32_t h, r;
-      split2(p0, p1, &h, &r);
-      (*hi)[k] = h;
-      (*lo)[k] = r;
+      split2(p0, p1, p, k);
     }
     l = l * alpha + sum;
 #pragma unroll

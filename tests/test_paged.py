@@ -557,6 +557,34 @@ def test_attention_of_one_large_and_many_tiny_weights(cuda, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f8"), ("f16", "f8")])
+@pytest.mark.parametrize("dim", [64, 80, 96, 128, 256])
+@pytest.mark.parametrize("pages", [0, 2500])
+def test_attention_weights_have_the_bits_of_fp32(cuda, dtype, cache, dim, pages):
+    """Value t is 1 in dim t and 0 elsewhere, so an output element is one weight: off by 2^-19 of itself at most.
+    Scores lie in [-1, 1], so that in units of log2 (below 1.5, with f16's shift of 14 below 16) the scale, the score
+    and the two sums of the exponent are off by 2 * 2^-24 * 1.5 + 2 * 2^-21, times ln 2; the exponential, its parts, the sum of
+    dim weights, two rescalings and the division by 2^-23, 2^-22, 2^-22, 2^-22 and 2^-22: 2^-19 in all."""
+    import torch
+    g = torch.Generator().manual_seed(dim)
+    page, heads = 16, 4
+    held = -(-dim // page)
+    s = (torch.randint(-128, 129, (dim,), generator=g) / 128.0).to(_dt(cache))
+    k, v = torch.zeros(2, held * page, dim)
+    k[:dim, 0] = s.float()
+    v[torch.arange(dim), torch.arange(dim)] = 1.0
+    k, v = (t.view(held, 1, page, dim).to(_dt(cache)).to(cuda) for t in (k, v))
+    q = torch.zeros(1, heads, dim)
+    q[0, :, 0] = torch.tensor([1.0, 0.5, -1.0, 0.75])
+    table = torch.full((1, max(held, pages)), -1, dtype=torch.int32, device=cuda)
+    table[0, :held] = torch.arange(held, dtype=torch.int32, device=cuda)
+    got = mx.paged_attention(q.to(_dt(dtype)).to(cuda), k, v, table, torch.tensor([dim], dtype=torch.int32, device=cuda), scale=1.0,
+                             out_dtype=torch.float32)[0].double().cpu()
+    ref = torch.softmax(q[0, :, :1].double() * s.double()[None, :], 1)
+    assert float(((got - ref).abs() / ref).max()) <= 2.0 ** -19
+
+
+@pytest.mark.gpu
 def test_attention_infinite_scores(cuda):
     """Scores of -inf have no weight, wherever they lie; a row of nothing else, or with +inf, is NaN as by
     the formula; other rows are not touched."""

@@ -84,11 +84,12 @@ int mlxr_paged_append(const mlxr_paged_cache* cache, int tokens, const void* k_d
  *                  MLXR_BF16
  *   lse_dev        [rows, heads] fp32 or NULL: natural logarithm of the softmax's sum, -inf for
  *                  an empty row
- * Tokens of pages whose table entry lies outside the cache are left out.  What lies in the cache
- * past a row's tokens is not used, whatever its bits.  head_dim: a multiple of 8 (e4m3: 16), at
- * most 256; keys' and values' strides and addresses are multiples of 16 bytes, the pages and tokens
- * of a store at most 2^31 elements apart.  Sums, maxima and
- * the output before its rounding are fp32; weights enter their products with the values with 24 bits (bf16 caches) or 22. */
+ * Tokens of pages whose table entry lies outside the cache are left out; a row with no others is an empty
+ * row, as one of length 0.  What lies in the cache past a row's tokens is not used, whatever its
+ * bits.  head_dim: a multiple of 8 (e4m3: 16), at most 256; keys' and values' strides and addresses
+ * are multiples of 16 bytes, the pages and tokens of a store at most 2^31 elements apart.  Sums,
+ * maxima and the output before its rounding are fp32; weights enter their products with the values
+ * with 24 bits (bf16 caches) or 22. */
 /* Workspace bytes of a call (0: none is needed, workspace_dev may be NULL). */
 int mlxr_paged_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int heads, int table_width,
                                         size_t* bytes);

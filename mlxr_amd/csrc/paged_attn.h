@@ -26,6 +26,8 @@
 // heads of 80, window 1024, in one launch 38 (158 MB; lines that heads share).  One row of 4 kv heads of 64, 700
 // tokens, 7.4: latency.
 #pragma once
+#include <cfloat>
+
 #include "mfma16.h"
 #include "paged_internal.h"
 
@@ -77,6 +79,11 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, int r) {
 __host__ __device__ constexpr int partial_floats(int part_rows, int dim) { return part_rows * dim + (2 * part_rows + 3) / 4 * 4; }
 __device__ __forceinline__ float* partial(const AttnArgs& a, int w, int slot) {
   return a.ws + ((int64_t)w * 2 + slot) * partial_floats(a.part_rows, a.dim);
+}
+// What makes an average of a row's weighted values.  A row none of whose tokens counts (m is -inf) gets zeros; one whose
+// scores are all -inf (its weights, and so l, are 0) NaN, by the formula.
+__device__ __forceinline__ float average_factor(const AttnArgs& a, int kvh, float m, float l) {
+  return m == -INFINITY ? 0.f : l == 0.f ? NAN : (a.v_scale ? a.v_scale[kvh] : 1.f) / l;
 }
 // n / d, d > 0; most calls stay within 32 bits, whose division takes a tenth of the instructions.
 __device__ __forceinline__ int quotient(int64_t n, int d) {
@@ -356,6 +363,7 @@ struct Attn {
     __builtin_amdgcn_sched_barrier(0);  // the order of the loop's loads, which its waits count
     load_v(ids, t0, true);
     uint32_t live = live_of(ids, t0, s);
+    uint64_t any = 0;
     while (true) {
       const bool more = t0 != last;
       ids = next;
@@ -365,6 +373,7 @@ struct Attn {
       scores(x);
       load_k(ids, t1, more);
       const bool full = __ballot(live != 0xff) == 0;
+      any |= __ballot(live != 0);
       u32x4_t p[PARTS];
       weights(x, live, full, p);
       if (!full) drop(live);
@@ -377,6 +386,7 @@ struct Attn {
       t0 = t1;
       t1 += kTile;
     }
+    if (any) m = fmaxf(m, -FLT_MAX);  // a token counts, whatever its score (average_factor)
   }
 
   // Pair k of two weights in parts, neither of them negative nor, beside a weight above 0, a later one 0: an infinite value
@@ -499,7 +509,7 @@ struct Attn {
       return;
     }
     const int64_t head = (int64_t)r * a.heads + kvh * a.group + h;
-    const float f = (a.v_scale ? a.v_scale[kvh] : 1.f) / l;
+    const float f = average_factor(a, kvh, m, l);
 #pragma unroll
     for (int x = 0; x < VH; ++x)
 #pragma unroll

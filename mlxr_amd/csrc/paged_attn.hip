@@ -23,7 +23,7 @@ __device__ __forceinline__ void add(Part& a, const Part& b) {
 }
 
 // One workgroup per (row, head): o = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w over the wavefronts w
-// that had a piece of the row, M the maximum of their m.  Rows without tokens get zeros; rows that one
+// that had a piece of the row, M the maximum of their m (-inf: no token counted).  Rows without tokens get zeros; rows that one
 // wavefront covered are done.  Threads: four dims each (LANES, a power of two that covers head_dim), several
 // pieces side by side, four of them on their way at once.
 template <int THREADS>
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(AttnArgs a, int lanes) {
   __syncthreads();
   if (y || !in) return;
   for (int w = 1; w < WAVES; ++w) add(sum, sh[w][x]);
-  const float f = (a.v_scale ? a.v_scale[kvh] : 1.f) / sum.l;
+  const float f = average_factor(a, kvh, sum.m, sum.l);
   const f32x4_t v = sum.o * f;
   const float each[4] = {v[0], v[1], v[2], v[3]};
   store_values<4>(a.out, a.out_dtype, head * a.dim + 4 * x, each);

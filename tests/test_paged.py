@@ -664,6 +664,35 @@ def test_attention_leaves_pages_outside_the_cache_out(cuda, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["bf16", "f8"])
+@pytest.mark.parametrize("heads,kv,dim,page", [(4, 2, 64, 16), (20, 1, 128, 8), (4, 2, 80, 6), (2, 2, 256, 16)])
+@pytest.mark.parametrize("width", [0, 40000])
+@pytest.mark.parametrize("window", [0, 33])
+def test_attention_rows_without_a_page_in_the_cache(cuda, cache, heads, kv, dim, page, width, window):
+    """Rows that have a length, but none of whose tokens (none of whose window) lies in the cache, are empty: zeros, -inf."""
+    import torch
+    lens = [100, 3 * page, 700, 650, 90, 1]
+    (k, v), table, (keys, values) = _fill(cuda, lens, kv, dim, page, cache, False, 21)
+    table = torch.nn.functional.pad(table, (0, max(0, width // page - table.shape[1])), value=-1)
+    table[1, :3] = torch.tensor([-1, k.shape[0], 1 << 30], dtype=torch.int32, device=cuda)  # none
+    table[3, :] = -5  # none of many
+    table[2, (lens[2] - 33) // page:] = -1  # none of the window's
+    kept = (lens[2] - 33) // page * page
+    empty = [1, 3] + ([2] if window else [])
+    q = torch.randn(len(lens), heads, dim, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(cuda)
+    vs = torch.full((kv,), 2.0, device=cuda) if cache == "f8" else None
+    got, lse = mx.paged_attention(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device=cuda), window=window,
+                                  v_scale=vs, out_dtype=torch.float32, return_lse=True)
+    assert not got[empty].any() and (lse[empty] == -math.inf).all()
+    if not window:  # what is left of row 2
+        keys[2], values[2], lens[2] = keys[2][:kept], values[2][:kept], kept
+    rest = [r for r in range(len(lens)) if r not in empty]
+    ref, ref_lse = _attend64(q[rest], [keys[r] for r in rest], [values[r] for r in rest], [lens[r] for r in rest], window, dim ** -0.5, vs=vs)
+    _check(got[rest], ref, [values[r] for r in rest], [lens[r] for r in rest], "f32", vs)
+    assert float((lse[rest].double().cpu() - ref_lse).abs().max()) < 1e-3
+
+
+@pytest.mark.gpu
 def test_attention_lengths_past_the_table_and_negative(cuda):
     import torch
     (k, v), table, (keys, values) = _fill(cuda, [64, 64, 5], 2, 64, 16, "bf16", False, 4)

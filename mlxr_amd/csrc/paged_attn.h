@@ -97,6 +97,12 @@ __device__ __forceinline__ uint32_t widen(uint32_t w) {
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, H));
 }
 
+// The larger of the 16-bit halves: of floats that are not negative, the larger float.
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
+  typedef __attribute__((ext_vector_type(2))) uint16_t V;
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b)));
+}
+
 // N (1, 2, 4) words at a multiple of 4 N bytes.
 template <int N>
 struct Words {
@@ -154,7 +160,8 @@ struct Attn {
   static constexpr int CH = F8 ? DT / 16 : DT == 96 ? 16 : DT / 8, TPL = 64 / CH, NL = LK ? kTile / TPL : 2 * KL;
 
   const AttnArgs& a;
-  const int lane, col, g;
+  const int lane, col;
+  int g;
   u32x4_t q[KS];
   u32x4_t kr[NL];
   u32x4_t* keys;  // [32 tokens][CH] of this wavefront
@@ -365,6 +372,9 @@ struct Attn {
     uint32_t live = live_of(ids, t0, s);
     uint64_t any = 0;
     while (true) {
+      // Between 96 and 128 dims what follows from g is computed again for each tile: kept over the loop, it would cost a
+      // third workgroup's registers (128 rows of 8 kv heads of 112, up to 200 tokens, 15.4 us and 14.4; other sizes lose 1 to 4 %).
+      if constexpr (DT == 128 && !DIM && !LK && P8) asm("" : "+v"(g));
       const bool more = t0 != last;
       ids = next;
       next = ids_of(t1 + kTile, s);
@@ -389,21 +399,23 @@ struct Attn {
     if (any) m = fmaxf(m, -FLT_MAX);  // a token counts, whatever its score (average_factor)
   }
 
-  // Pair k of two weights in parts, neither of them negative nor, beside a weight above 0, a later one 0: an infinite value
-  // then gives an infinite output as a weight in one piece does, not NaN.  (The least later part, 2^-126 or 2^-38 of the
-  // largest weight, is far below the rounding of the sums.)
+  // Pair k of two weights in parts, none of them negative nor a later one 0: an infinite value then gives an infinite output
+  // as a weight in one piece does, not NaN.  (The least later part, 2^-126 or 2^-38 of the largest weight, is far below the
+  // rounding of the sums.)
   static __device__ __forceinline__ void split2(float p0, float p1, u32x4_t (&p)[PARTS], int k) {
+    auto floor2 = [](uint32_t w) { return pair_max(w, P16 ? 0x00010001u : 0x00800080u); };
     if constexpr (P16) {
       const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
       p[0][k] = hi;
-      p[1][k] = pack2<true>(fmaxf(p0 - unpack<true>(hi, 0), 0x1p-24f), fmaxf(p1 - unpack<true>(hi, 1), 0x1p-24f));
+      p[1][k] = floor2(pack2<true>(p0 - unpack<true>(hi, 0), p1 - unpack<true>(hi, 1)));
     } else {
 #pragma unroll
       for (int n = 0; n < PARTS; ++n) {  // each the upper half of what is left; the last holds all of it
         const uint32_t b0 = __builtin_bit_cast(uint32_t, p0), b1 = __builtin_bit_cast(uint32_t, p1);
-        p[n][k] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-        p0 = fmaxf(p0 - __builtin_bit_cast(float, b0 & 0xffff0000u), 0x1p-126f);
-        p1 = fmaxf(p1 - __builtin_bit_cast(float, b1 & 0xffff0000u), 0x1p-126f);
+        const uint32_t w = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+        p[n][k] = n ? floor2(w) : w;
+        p0 -= __builtin_bit_cast(float, b0 & 0xffff0000u);
+        p1 -= __builtin_bit_cast(float, b1 & 0xffff0000u);
       }
     }
   }

@@ -697,6 +697,8 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
       for (int w = 0; w < WAVES; ++w)
 #pragma unroll
         for (int k = 0; k < 2; ++k) v[k] += sh[w][part >> 1][(2 * (part & 1) + k) * 16 + t];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = 8 * part + i < rank ? v[i >> 2][i & 3] : 0.f;  // an infinite x gave NaN there
       split_h<F16, RT>(v, tile.scale, t, 8 * part, hs + t * h_row(RT), back);
     }
     __syncthreads();

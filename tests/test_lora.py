@@ -244,6 +244,33 @@ def test_infinite_b_gives_infinity(cuda, dtype, tokens, K, rank):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,rank", [(3, 8), (20, 64), (300, 32), (300, 8), (20, 24)])
+@pytest.mark.parametrize("short", [0, 3])
+def test_infinite_sums_of_the_first_product(cuda, dtype, tokens, rank, short):
+    """An infinite element of x: infinite outputs, and NaN where B is 0; NaN in x: NaN; the tokens beside them stay as
+    they are; also where the adapter uses less than the bank's rank, or that is no multiple of 16."""
+    import torch
+    g = torch.Generator().manual_seed(rank)
+    x = torch.rand(tokens, 64, generator=g) + 0.5
+    a, b = torch.rand(1, rank, 64, generator=g) + 0.5, torch.rand(1, 40, rank, generator=g) + 0.5
+    b[0, 7, 1] = 0.0
+    ranks = torch.tensor([rank - short], dtype=torch.int32, device=cuda)
+    ids = torch.zeros(tokens, dtype=torch.int32, device=cuda)
+    dev = lambda t: t.to(_dt(dtype)).to(cuda)  # noqa: E731
+
+    def run():
+        return mx.lora_apply(dev(x), ids, [dev(a)], [dev(b)], [torch.zeros(tokens, 40, device=cuda)], ranks=ranks)[0].cpu()
+    plain = run()
+    assert torch.isfinite(plain).all()
+    x[1, 9], x[2, 9] = math.inf, math.nan
+    got = run()
+    assert torch.isnan(got[1, 7]) and (got[1, [n for n in range(40) if n != 7]] == math.inf).all() and torch.isnan(got[2]).all()
+    rest = [t for t in range(tokens) if t not in (1, 2)]
+    assert torch.equal(got[rest], plain[rest])
+
+
+@pytest.mark.gpu
 def test_lora_bank(cuda):
     import torch
     bank = mx.LoraBank(3, 20, 96, 256, device=cuda)

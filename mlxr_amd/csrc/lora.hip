@@ -383,26 +383,42 @@ __device__ __forceinline__ uint32_t cut_bf16(float x) {
 
 // 8 ranks at .. of token t of a tile into LDS as high and low 16-bit parts: rounded to one part h would lose what the
 // fp32 sums kept.  The high part is cut, not rounded, and the low one never 0 beside it nor of the other sign, so that
-// an infinite element of B gives an infinity as h in one piece does, not NaN (the least low part is 2^-24 of the token's
-// largest, or 2^-126).  In f16, whose range h may leave, relative to a power of two that brings the token's
-// largest to [1/2, 1), the reciprocal in back[t]; the 2 RT threads of a token are neighbours.
+// an infinite element of B gives an infinity as h in one piece does, not NaN.
+// In bf16 the least low part is 2^-126.  In f16 the parts are relative to a power of two that brings the token's largest to
+// [2^14, 2^15), the reciprocal in back[t]: off by 2^-22 of every rank above 2^-16 of the largest, 2^-20 at 2^-18 of it.  A
+// token with one below that (not 0), an infinite one or NaN, or a largest that leaves no room for the power of two has back[t]
+// = 0 and its ranks in fp32 in place of the parts (Expand::wide_tokens); of ranks that are alike one in 2^17 lies so low by
+// chance.  The 2 RT threads of a token are neighbours.
 template <bool F16, int RT>
 __device__ __forceinline__ void split_h(f32x4_t (&v)[2], float scale, int t, int at, uint16_t* row, float* back) {
   constexpr int R = 16 * RT;
-  float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    v[e] *= scale;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[e][i]));
-  }
+  for (int e = 0; e < 2; ++e) v[e] *= scale;
   if constexpr (F16) {
+    constexpr uint32_t kInf = 0x7f800000, kOct = 1 << 23;
+    uint32_t top = 0, least = ~0u;  // bits of the largest, of the least that is not 0 less 1
 #pragma unroll
-    for (int d = 1; d < 2 * RT; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-    if (at == 0) back[t] = __builtin_amdgcn_ldexpf(1.f, e);
+    for (int i = 0; i < 8; ++i) {
+      const float f = v[i >> 2][i & 3];  // of a vector's element itself, the compiler's bit cast takes the first's bits
+      const uint32_t x = __builtin_bit_cast(uint32_t, f) & 0x7fffffff;
+      top = max(top, x);
+      least = min(least, x - 1);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = __builtin_amdgcn_ldexpf(v[i >> 2][i & 3], -e);
+    for (int d = 1; d < 2 * RT; d *= 2) {
+      top = max(top, (uint32_t)__shfl_xor((int)top, d));
+      least = min(least, (uint32_t)__shfl_xor((int)least, d));
+    }
+    const bool wide = top && (top >= kInf || top < 27 * kOct || least + 1 < top - 18 * kOct);  // below 2^-100; 2^-18 apart
+    const int e = top && !wide ? 141 - (int)(top >> 23) : 0;
+    if (at == 0) back[t] = wide ? 0.f : __builtin_amdgcn_ldexpf(1.f, -e);
+    if (wide) {
+      *(f32x4_t*)(row + 2 * at) = v[0];
+      *(f32x4_t*)(row + 2 * at + 8) = v[1];
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = __builtin_amdgcn_ldexpf(v[i >> 2][i & 3], e);
   }
   auto low = [](float x, float high) {
     if (!(fabsf(x) < INFINITY) || x == 0.f) return 0.f;  // an infinite h stays infinite, NaN stays NaN
@@ -437,6 +453,7 @@ struct Expand {
   // side, brought into operand order there (an operand's own load would be 16 pieces of 64 bytes).
   u32x4_t next[NB];
   u32x4_t* rows;
+  bool wide = false;  // a token of this lane's is left to wide_tokens
 
   __device__ __forceinline__ Expand(const LoraArgs& a_, const mlxr_lora_item& it_, const Tile& t, int begin, u32x4_t* lds)
       : a(a_), it(it_), B((const uint16_t*)it_.b_dev + (t.adapter == a_.adapters ? 0 : (int64_t)t.adapter * it_.N * a_.rank)),
@@ -552,9 +569,13 @@ struct Expand {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = 16 * s + 4 * g + i;
-          if (t >= count || left <= 0) continue;
-          const int64_t at = (int64_t)token[t] * it.N + n;
           const float f = F16 && !none ? back[t] : 1.f;
+          if (t >= count || left <= 0) continue;
+          if (f == 0.f) {
+            wide = true;
+            continue;
+          }
+          const int64_t at = (int64_t)token[t] * it.N + n;
           if constexpr (VEC) {
             float v[CT];
 #pragma unroll
@@ -585,10 +606,37 @@ struct Expand {
     columns<YT, true>(it.N % CT ? min(end, it.N - 16 * CT + 1) : end, token, count, none, hs, back);
     if (it.N % CT) columns<YT, false>(end, token, count, none, hs, back);
   }
-  __device__ __forceinline__ void run(const int* token, int count, bool none, const uint16_t* hs, const float* back) {
+  // The wavefront's columns of the tokens whose ranks are in fp32 (split_h), a column a lane: few, or none.
+  __device__ __forceinline__ void wide_tokens(int begin, const int* token, int count, const uint16_t* hs, const float* back) {
+    static_assert(16 * SUB <= 64, "a token for each lane");
+    const int lane = threadIdx.x & 63, first = begin + (threadIdx.x >> 6) * 16 * CT;
+    for (uint64_t which = __ballot(lane < count && back[min(lane, count - 1)] == 0.f); which; which &= which - 1) {
+      const int t = __builtin_ctzll(which);
+      const float* h = (const float*)(hs + t * h_row(RT));
+      for (int at = lane; first + at / (16 * CT) * STEP < end; at += 64) {
+        const int n = first + at / (16 * CT) * STEP + at % (16 * CT);
+        if (n >= end) continue;
+        const int64_t to = (int64_t)token[t] * it.N + n;
+        float sum = load_scalar(it.y_dev, it.y_dtype, to);
+        constexpr int U = C < 4 ? C : 4;  // loads on their way at once
+        for (int r0 = 0; r0 < rank; r0 += 8 * U) {
+          u32x4_t b[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) b[u] = *(const u32x4_t*)(B + (int64_t)n * ld + (r0 + 8 * u < rank ? r0 + 8 * u : 0));
+#pragma unroll
+          for (int i = 0; i < 8 * U; ++i)
+            if (r0 + i < rank) sum = __builtin_fmaf(h[r0 + i], unpack<true>(b[i / 8][i % 8 / 2], i % 2), sum);
+        }
+        store_scalar(it.out_dev, it.y_dtype, to, sum);
+      }
+    }
+  }
+  __device__ __forceinline__ void run(int begin, const int* token, int count, bool none, const uint16_t* hs, const float* back) {
     if (it.y_dtype == DT_BF16) columns<DT_BF16>(token, count, none, hs, back);
     else if (it.y_dtype == DT_F16) columns<DT_F16>(token, count, none, hs, back);
     else columns<DT_F32>(token, count, none, hs, back);
+    if constexpr (F16)
+      if (__ballot(wide)) wide_tokens(begin, token, count, hs, back);
   }
 };
 
@@ -630,7 +678,7 @@ __global__ __launch_bounds__(kThreads, RT <= 4 && SUB == 1 ? 3 : 1) void expand_
     }
     __syncthreads();
   }
-  e.run(token, count, none, hs, back);
+  e.run(begin, token, count, none, hs, back);
 }
 
 // Both products of one tile and a.columns columns of an item: every workgroup of a tile computes its h for itself.
@@ -703,7 +751,7 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
     }
     __syncthreads();
   }
-  e.run(token, count, none, hs, back);
+  e.run(begin, token, count, none, hs, back);
 }
 
 struct Layout {

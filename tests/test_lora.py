@@ -270,6 +270,45 @@ def test_infinite_sums_of_the_first_product(cuda, dtype, tokens, rank, short):
     assert torch.equal(got[rest], plain[rest])
 
 
+def _one_hot(adapters, N, rank):
+    """B whose row j picks rank j, row rank + j the difference of ranks j and j + 1."""
+    import torch
+    b = torch.zeros(adapters, N, rank)
+    b[:, :rank] = torch.eye(rank)
+    b[:, rank:2 * rank - 1] = torch.eye(rank)[:-1] - torch.eye(rank)[1:]
+    return b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16"])
+@pytest.mark.parametrize("tokens,K,rank", [(5, 64, 16), (33, 64, 32), (20, 64, 64), (20, 64, 128), (100, 8192, 16), (300, 64, 8), (300, 64, 16),
+                                           (300, 64, 32), (300, 64, 64), (300, 64, 128)])
+def test_lora_ranks_of_a_token_far_apart(cuda, dtype, tokens, K, rank):
+    """x . A^T of 2^16 in one rank and 2^-22 in another of the same token: each is held relative to itself (2^-20), not to
+    the largest; among tokens of the same adapter whose ranks are alike, and whose results they do not touch."""
+    import torch
+    g = torch.Generator().manual_seed(rank + K)
+    x = torch.randint(1, 8, (tokens, K), generator=g)
+    a = torch.randint(-7, 8, (2, rank, K), generator=g).double()
+    a[:, :, K // 2:] *= 2.0 ** (10 - 2.0 * (torch.arange(rank) % 17))[None, :, None]
+    alike = torch.rand(tokens, generator=g) < 0.6
+    x[alike, K // 2:], x[~alike, :K // 2] = 0, 0
+    N = 2 * rank
+    ids = torch.randint(-1, 2, (tokens,), generator=g).to(torch.int32)
+    dev = lambda t: t.to(_dt(dtype)).to(cuda)  # noqa: E731
+    b, y = dev(_one_hot(2, N, rank)), torch.zeros(tokens, N, device=cuda)
+    scales = torch.tensor([1.0, 3.0], device=cuda)
+    got = mx.lora_apply(dev(x), ids.to(cuda), [dev(a)], [b], [y], scales)[0]
+    i = ids.clamp(min=0).long()
+    h = torch.einsum("tk,trk->tr", x.double(), a[i]) * ((ids >= 0) * torch.where(i > 0, 3.0, 1.0))[:, None]
+    assert ((got[:, :rank].double().cpu() - h).abs() <= 2.0 ** -20 * h.abs()).all()
+    step = (h[:, :-1] - h[:, 1:]).abs(), h[:, :-1].abs() + h[:, 1:].abs()
+    assert ((got[:, rank:2 * rank - 1].double().cpu().abs() - step[0]).abs() <= 2.0 ** -20 * step[1]).all()
+    x[~alike] = 0
+    again = mx.lora_apply(dev(x), ids.to(cuda), [dev(a)], [b], [y], scales)[0]
+    assert torch.equal(again[alike.to(cuda)], got[alike.to(cuda)])
+
+
 @pytest.mark.gpu
 def test_lora_bank(cuda):
     import torch

@@ -41,7 +41,8 @@ int mlxr_lora_workspace_size(int count, const mlxr_lora_item* items, int tokens,
  *   scales_dev  [adapters] fp32 or NULL (1)
  *   ranks_dev   [adapters] int32 or NULL (rank): rank of each adapter, up to `rank`; what A and B hold
  *               past an adapter's rank is not used, whatever its bits
- * Sums are fp32; x . A^T is not rounded between the products, out is rounded once. */
+ * Sums are fp32, out is rounded once.  x . A^T enters the second product with all its bits (bf16), or to 2^-20 of each of its
+ * elements (f16). */
 int mlxr_lora_apply(int count, const mlxr_lora_item* items, int tokens, int K, int adapters, int rank, const void* x_dev,
                     int x_dtype, int64_t x_stride, const int32_t* ids_dev, const float* scales_dev,
                     const int32_t* ranks_dev, void* workspace_dev, size_t workspace_bytes, void* stream);

@@ -381,14 +381,18 @@ __device__ __forceinline__ uint32_t cut_bf16(float x) {
   return (__builtin_bit_cast(uint32_t, x) | (x != x ? 0x400000u : 0u)) & 0xffff0000u;
 }
 
-// 8 ranks at .. of token t of a tile into LDS as high and low 16-bit parts: rounded to one part h would lose what the
-// fp32 sums kept.  The high part is cut, not rounded, and the low one never 0 beside it nor of the other sign, so that
-// an infinite element of B gives an infinity as h in one piece does, not NaN.
-// In bf16 the least low part is 2^-126.  In f16 the parts are relative to a power of two that brings the token's largest to
-// [2^14, 2^15), the reciprocal in back[t]: off by 2^-22 of every rank above 2^-16 of the largest, 2^-20 at 2^-18 of it.  A
-// token with one below that (not 0), an infinite one or NaN, or a largest that leaves no room for the power of two has back[t]
-// = 0 and its ranks in fp32 in place of the parts (Expand::wide_tokens); of ranks that are alike one in 2^17 lies so low by
-// chance.  The 2 RT threads of a token are neighbours.
+// 16-bit parts of h that add up to it: rounded to one part h would lose what the fp32 sums kept.
+constexpr int h_parts(bool f16) { return f16 ? 2 : 3; }
+// Elements of a token's row of them: R of each part; padded against bank conflicts.
+constexpr int h_row(bool f16, int rt) { return 16 * rt * h_parts(f16) + 8; }
+
+// 8 ranks at .. of token t of a tile into LDS in parts.  A part is cut, not rounded, and those after it never 0 beside it nor
+// of the other sign, so that an infinite element of B gives an infinity as h in one piece does, not NaN.
+// bf16: three parts, all bits of fp32 (the least later part is 2^-125).  f16: two, relative to a power of two that brings
+// the token's largest to [2^14, 2^15), the reciprocal in back[t]: off by 2^-22 of every rank above 2^-16 of the largest, 2^-20
+// at 2^-18 of it.  A token with one below that (not 0), an infinite one or NaN, or a largest that leaves no room for the power
+// of two has back[t] = 0 and its ranks in fp32 in place of the parts (Expand::wide_tokens); of ranks that are alike one in 2^17
+// lies so low by chance.  The 2 RT threads of a token are neighbours.
 template <bool F16, int RT>
 __device__ __forceinline__ void split_h(f32x4_t (&v)[2], float scale, int t, int at, uint16_t* row, float* back) {
   constexpr int R = 16 * RT;
@@ -420,23 +424,33 @@ __device__ __forceinline__ void split_h(f32x4_t (&v)[2], float scale, int t, int
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = __builtin_amdgcn_ldexpf(v[i >> 2][i & 3], e);
   }
-  auto low = [](float x, float high) {
-    if (!(fabsf(x) < INFINITY) || x == 0.f) return 0.f;  // an infinite h stays infinite, NaN stays NaN
-    return copysignf(fmaxf(fabsf(x - high), F16 ? 0x1p-24f : 0x1p-126f), x);
+  constexpr float LEAST = F16 ? 0x1p-24f : 0x1p-125f;
+  auto rest = [](float x, float part) {  // of an infinite x: finite, of its sign
+    return x == 0.f ? 0.f : copysignf(fmaxf(fabsf(x - part), LEAST), x);
   };
   u32x4_t hi, lo;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float v0 = v[e >> 1][2 * (e & 1)], v1 = v[e >> 1][2 * (e & 1) + 1];
+    float v0 = v[e >> 1][2 * (e & 1)], v1 = v[e >> 1][2 * (e & 1) + 1];
     if constexpr (F16) hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(v0, v1));
     else hi[e] = cut_bf16(v0) >> 16 | cut_bf16(v1);
-    lo[e] = pack2<F16>(low(v0, unpack<F16>(hi[e], 0)), low(v1, unpack<F16>(hi[e], 1)));
+    v0 = rest(v0, unpack<F16>(hi[e], 0)), v1 = rest(v1, unpack<F16>(hi[e], 1));
+    if constexpr (F16) {
+      lo[e] = pack2<true>(v0, v1);
+    } else {
+      lo[e] = cut_bf16(v0) >> 16 | cut_bf16(v1);
+      v[e >> 1][2 * (e & 1)] = rest(v0, unpack<false>(lo[e], 0)), v[e >> 1][2 * (e & 1) + 1] = rest(v1, unpack<false>(lo[e], 1));
+    }
   }
   *(u32x4_t*)(row + at) = hi;
   *(u32x4_t*)(row + R + at) = lo;
+  if constexpr (!F16) {
+    constexpr float SHARE = RT == 1 ? 0.5f : 1.f;  // RT 1 multiplies it twice
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lo[e] = cut_bf16(v[e >> 1][2 * (e & 1)] * SHARE) >> 16 | cut_bf16(v[e >> 1][2 * (e & 1) + 1] * SHARE);
+    *(u32x4_t*)(row + 2 * R + at) = lo;
+  }
 }
-// Elements of such a row: R high parts, R low parts; padded against bank conflicts.
-constexpr int h_row(int rt) { return 32 * rt + 8; }
 
 // The second product of a tile: columns [n0, end) of an item in steps of 16 CT for each of WAVES wavefronts.
 // Tokens are the rows of the products; column n of the c-th is column CT n + c of the step, so a lane ends
@@ -445,6 +459,9 @@ template <bool F16, int RT, int SUB, int WAVES>
 struct Expand {
   static constexpr int R = 16 * RT, KT = RT == 1 ? 1 : RT / 2, CT = columns_of(SUB, RT), STEP = WAVES * 16 * CT;
   static constexpr int C = R / 8, NB = 16 * CT * C / 64;  // 16-byte parts of a column's row of B; loads of a step
+  // Turns in which a step's B goes through LDS.  A tile of 64 tokens of rank 128 in bf16 has 49 KiB of h: beside 32
+  // KiB of B a CU would hold one workgroup, beside 16 it holds two (2000 tokens, two projections of 14336, 212 us and 158).
+  static constexpr int TURNS = !F16 && RT == 8 && SUB > 1 ? 2 : 1, CTT = CT / TURNS, NBT = NB / TURNS, ROWS = NBT * 64;
   const LoraArgs& a;
   const mlxr_lora_item& it;
   const uint16_t* B;
@@ -461,7 +478,7 @@ struct Expand {
     const int lane = threadIdx.x & 63;
     col = lane & 15, g = lane >> 4;
     n0 = begin + (threadIdx.x >> 6) * 16 * CT;
-    rows = lds + (threadIdx.x >> 6) * NB * 64;
+    rows = lds + (threadIdx.x >> 6) * ROWS;
     end = min(begin + a.columns, it.N);
     load_b(n0, n0 < end);
   }
@@ -471,26 +488,27 @@ struct Expand {
     const int ld = more ? this->ld : 0;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int at = i * 64 + (threadIdx.x & 63), part = at % C;
-      next[i] = *(const u32x4_t*)(B + (int64_t)min(n0 + at / C, it.N - 1) * ld + (8 * part < rank ? 8 * part : 0));
+      const int at = i % NBT * 64 + (threadIdx.x & 63), part = at % C, n = at / C;
+      const int column = n / CTT * CT + i / NBT * CTT + n % CTT;
+      next[i] = *(const u32x4_t*)(B + (int64_t)min(n0 + column, it.N - 1) * ld + (8 * part < rank ? 8 * part : 0));
     }
   }
-  // Place of part `part` of column n of a step: 8 lanes that read or write at once, and so 128 bytes, lie in different banks.
-  static __device__ __forceinline__ int place(int n, int part) { return (n * C + part) ^ (n / CT & 7); }
-  __device__ __forceinline__ void store_b() {
-    wave_sync();  // other lanes' reads of the step before
+  // Place of part `part` of column n of a turn: 8 lanes that read or write at once, and so 128 bytes, lie in different banks.
+  static __device__ __forceinline__ int place(int n, int part) { return (n * C + part) ^ (n / CTT & 7); }
+  __device__ __forceinline__ void store_b(int turn) {
+    wave_sync();  // other lanes' reads of the turn before
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
+    for (int i = 0; i < NBT; ++i) {
       const int at = i * 64 + (threadIdx.x & 63);
-      rows[place(at / C, at % C)] = next[i];
+      rows[place(at / C, at % C)] = next[turn * NBT + i];
     }
     wave_sync();
   }
-  // RT 1 multiplies the high and the low parts in one product, ranks 8 (g & 1) ..
+  // RT 1 multiplies the first two parts in one product, ranks 8 (g & 1) .., and in bf16 half of the third twice in another.
   __device__ __forceinline__ int rank_at(int k) const { return RT == 1 ? 8 * (g & 1) : 32 * k + 8 * g; }
   // Operand c of the ranks k, without what the adapter has not.
   __device__ __forceinline__ u32x4_t operand(int k, int c) const {
-    u32x4_t b = rows[place(CT * col + c, rank_at(k) / 8)];
+    u32x4_t b = rows[place(CTT * col + c % CTT, rank_at(k) / 8)];
     if (rank < R) {
       const int left = rank - rank_at(k);
 #pragma unroll
@@ -504,7 +522,16 @@ struct Expand {
   __device__ __forceinline__ void columns(int stop, const int* token, int count, bool none, const uint16_t* hs, const float* back) {
     constexpr bool AHEAD = VEC && SUB > 1 && YT != DT_F32;  // y of the next 16 tokens on its way: fp32 has no registers for it
     for (; n0 < stop; n0 += STEP) {
-      store_b();
+      u32x4_t bf[SUB > 1 ? KT : 1][SUB > 1 ? CT : 1];  // read once for all tokens
+#pragma unroll
+      for (int turn = 0; turn < TURNS; ++turn) {
+        store_b(turn);
+        if constexpr (TURNS > 1)
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int c = turn * CTT; c < (turn + 1) * CTT; ++c) bf[k][c] = operand(k, c);
+      }
       const int n = n0 + CT * col, left = it.N - n;
       Cols<YT, CT> y[4];
       uint32_t bits[VEC ? 1 : 4][VEC ? 1 : CT];  // of single elements of y
@@ -528,8 +555,7 @@ struct Expand {
       load_y(y, 0);
       asm volatile("" ::: "memory");  // the loads stay in this order: what waits for y would wait for those before it too
       load_b(n0 + STEP, n0 + STEP < end);
-      u32x4_t bf[SUB > 1 ? KT : 1][SUB > 1 ? CT : 1];  // read once for all tokens
-      if constexpr (SUB > 1)
+      if constexpr (SUB > 1 && TURNS == 1)
 #pragma unroll
         for (int k = 0; k < KT; ++k)
 #pragma unroll
@@ -541,28 +567,21 @@ struct Expand {
         if (AHEAD && 16 * (s + 1) < count) load_y(y_next, s + 1);
         f32x4_t acc[CT] = {};
         if (!none) {
-          const uint16_t* h = hs + (16 * s + col) * h_row(RT);
+          const uint16_t* h = hs + (16 * s + col) * h_row(F16, RT);
 #pragma unroll
           for (int k = 0; k < KT; ++k) {
-            if constexpr (RT == 1) {
-              const u32x4_t f = *(const u32x4_t*)(h + 8 * g);
+            constexpr int PARTS = RT == 1 ? h_parts(F16) - 1 : h_parts(F16);  // operands
+            u32x4_t f[PARTS];
 #pragma unroll
-              for (int c = 0; c < CT; ++c) {
-                u32x4_t b;
-                if constexpr (SUB > 1) b = bf[k][c];
-                else b = operand(k, c);
-                acc[c] = mfma16<F16>(f, b, acc[c]);
-              }
-            } else {
-              const u32x4_t hi = *(const u32x4_t*)(h + 32 * k + 8 * g), lo = *(const u32x4_t*)(h + R + 32 * k + 8 * g);
+            for (int p = 0; p < PARTS; ++p)
+              f[p] = *(const u32x4_t*)(h + (RT == 1 ? p ? 2 * R + rank_at(0) : 8 * g : p * R + 32 * k + 8 * g));
 #pragma unroll
-              for (int c = 0; c < CT; ++c) {
-                u32x4_t b;
-                if constexpr (SUB > 1) b = bf[k][c];
-                else b = operand(k, c);
-                acc[c] = mfma16<F16>(lo, b, acc[c]);
-                acc[c] = mfma16<F16>(hi, b, acc[c]);
-              }
+            for (int c = 0; c < CT; ++c) {
+              u32x4_t b;
+              if constexpr (SUB > 1) b = bf[k][c];
+              else b = operand(k, c);
+#pragma unroll
+              for (int p = PARTS - 1; p >= 0; --p) acc[c] = mfma16<F16>(f[p], b, acc[c]);
             }
           }
         }
@@ -612,20 +631,22 @@ struct Expand {
     const int lane = threadIdx.x & 63, first = begin + (threadIdx.x >> 6) * 16 * CT;
     for (uint64_t which = __ballot(lane < count && back[min(lane, count - 1)] == 0.f); which; which &= which - 1) {
       const int t = __builtin_ctzll(which);
-      const float* h = (const float*)(hs + t * h_row(RT));
+      const float* h = (const float*)(hs + t * h_row(F16, RT));
       for (int at = lane; first + at / (16 * CT) * STEP < end; at += 64) {
         const int n = first + at / (16 * CT) * STEP + at % (16 * CT);
         if (n >= end) continue;
         const int64_t to = (int64_t)token[t] * it.N + n;
+        u32x4_t b[C];  // all on their way at once
+#pragma unroll
+        for (int p = 0; p < C; ++p) b[p] = *(const u32x4_t*)(B + (int64_t)n * ld + (8 * p < rank ? 8 * p : 0));
         float sum = load_scalar(it.y_dev, it.y_dtype, to);
-        constexpr int U = C < 4 ? C : 4;  // loads on their way at once
-        for (int r0 = 0; r0 < rank; r0 += 8 * U) {
-          u32x4_t b[U];
 #pragma unroll
-          for (int u = 0; u < U; ++u) b[u] = *(const u32x4_t*)(B + (int64_t)n * ld + (r0 + 8 * u < rank ? r0 + 8 * u : 0));
+        for (int p = 0; p < C; ++p) {
+          if (8 * p >= rank) break;
+          const f32x4_t lower = *(const f32x4_t*)(h + 8 * p), upper = *(const f32x4_t*)(h + 8 * p + 4);
 #pragma unroll
-          for (int i = 0; i < 8 * U; ++i)
-            if (r0 + i < rank) sum = __builtin_fmaf(h[r0 + i], unpack<true>(b[i / 8][i % 8 / 2], i % 2), sum);
+          for (int i = 0; i < 8; ++i)
+            if (8 * p + i < rank) sum = __builtin_fmaf(i < 4 ? lower[i & 3] : upper[i & 3], unpack<true>(b[p][i / 2], i % 2), sum);
         }
         store_scalar(it.out_dev, it.y_dtype, to, sum);
       }
@@ -642,10 +663,10 @@ struct Expand {
 
 // One tile and a.columns columns of an item, h from the workspace.
 template <bool F16, int RT, int SUB>
-__global__ __launch_bounds__(kThreads, RT <= 4 && SUB == 1 ? 3 : 1) void expand_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kThreads, RT <= 4 && SUB == 1 ? 3 : 2) void expand_kernel(LoraArgs a) {
   __shared__ int token[16 * SUB];
   __shared__ float back[16 * SUB];
-  __shared__ __attribute__((aligned(16))) uint16_t hs[16 * SUB * h_row(RT)];
+  __shared__ __attribute__((aligned(16))) uint16_t hs[16 * SUB * h_row(F16, RT)];
   const mlxr_lora_item& it = a.item[blockIdx.z];
   const int begin = blockIdx.x * a.columns;
   if (begin >= it.N) return;
@@ -655,7 +676,7 @@ __global__ __launch_bounds__(kThreads, RT <= 4 && SUB == 1 ? 3 : 1) void expand_
   const bool none = tile.adapter == a.adapters;
   if (none && it.out_dev == it.y_dev) return;
   using E = Expand<F16, RT, SUB, kWaves>;
-  __shared__ u32x4_t rows[kWaves * E::NB * 64];
+  __shared__ u32x4_t rows[kWaves * E::ROWS];
   E e(a, it, tile, begin, rows);
   if (!none) {
     for (int u = threadIdx.x; u < 16 * SUB * 2 * RT; u += kThreads) {
@@ -674,7 +695,7 @@ __global__ __launch_bounds__(kThreads, RT <= 4 && SUB == 1 ? 3 : 1) void expand_
 #pragma unroll
           for (int k = 0; k < 2; ++k) v[k] += in[s][k];
       }
-      split_h<F16, RT>(v, tile.scale, t, at, hs + t * h_row(RT), back);
+      split_h<F16, RT>(v, tile.scale, t, at, hs + t * h_row(F16, RT), back);
     }
     __syncthreads();
   }
@@ -688,7 +709,7 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
   constexpr int WAVES = kFusedThreads / 64, U = 4;  // steps of 64 k on their way at once
   __shared__ int token[16];
   __shared__ float back[16];
-  __shared__ __attribute__((aligned(16))) uint16_t hs[16 * h_row(RT)];
+  __shared__ __attribute__((aligned(16))) uint16_t hs[16 * h_row(F16, RT)];
   __shared__ f32x4_t sh[WAVES][RT][64];
   const mlxr_lora_item& it = a.item[blockIdx.z];
   const int begin = blockIdx.x * a.columns;
@@ -700,8 +721,8 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
   if (none && it.out_dev == it.y_dev) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   using E = Expand<F16, RT, 1, WAVES>;
-  static_assert(E::NB >= 2, "turn's room");
-  __shared__ u32x4_t rows[WAVES * E::NB * 64];
+  static_assert(E::ROWS >= 128, "turn's room");
+  __shared__ u32x4_t rows[WAVES * E::ROWS];
   E e(a, it, tile, begin, rows);
   if (!none) {
     const int row = lane >> 3, at = 8 * (lane & 7);
@@ -726,10 +747,10 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
         }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        turn(xf[u], rows + wave * E::NB * 64);
+        turn(xf[u], rows + wave * E::ROWS);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          turn(af[u][r], rows + wave * E::NB * 64);
+          turn(af[u][r], rows + wave * E::ROWS);
 #pragma unroll
           for (int e = 0; e < 2; ++e) acc[r] = mfma16<F16>(af[u][r][e], xf[u][e], acc[r]);
         }
@@ -747,7 +768,7 @@ __global__ __launch_bounds__(kFusedThreads) void fused_kernel(LoraArgs a) {
         for (int k = 0; k < 2; ++k) v[k] += sh[w][part >> 1][(2 * (part & 1) + k) * 16 + t];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = 8 * part + i < rank ? v[i >> 2][i & 3] : 0.f;  // an infinite x gave NaN there
-      split_h<F16, RT>(v, tile.scale, t, 8 * part, hs + t * h_row(RT), back);
+      split_h<F16, RT>(v, tile.scale, t, 8 * part, hs + t * h_row(F16, RT), back);
     }
     __syncthreads();
   }

@@ -280,7 +280,32 @@ def _one_hot(adapters, N, rank):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", ["f16"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,K,rank", [(5, 64, 8), (5, 64, 16), (33, 64, 32), (20, 64, 64), (20, 64, 128), (100, 8192, 16), (100, 4096, 32),
+                                           (300, 64, 8), (300, 64, 16), (300, 64, 32), (300, 64, 64), (300, 64, 128)])
+def test_lora_keeps_the_sums_of_the_first_product(cuda, dtype, tokens, K, rank):
+    """x and A are integers of up to 8 bits, so x . A^T has up to 22 and is exact in fp32; B shows it, and differences of its
+    ranks.  What the second product takes of it is off by 2^-22 of each rank at most (f16; bf16 holds it all), the fp32 sum of
+    two by 2^-24 of them."""
+    import torch
+    g = torch.Generator().manual_seed(rank + K)
+    top = 255 if K == 64 else 15
+    x, a = torch.randint(top // 2, top + 1, (tokens, K), generator=g), torch.randint(top // 2, top + 1, (3, rank, K), generator=g)
+    a *= torch.randint(0, 2, (3, rank, 1), generator=g) * 2 - 1
+    N = 2 * rank + 3
+    ids = torch.randint(-1, 3, (tokens,), generator=g).to(torch.int32)
+    dev = lambda t: t.to(_dt(dtype)).to(cuda)  # noqa: E731
+    got = mx.lora_apply(dev(x), ids.to(cuda), [dev(a)], [dev(_one_hot(3, N, rank))], [torch.zeros(tokens, N, device=cuda)])[0].double().cpu()
+    h = torch.einsum("tk,trk->tr", x.double(), a.double()[ids.clamp(min=0).long()]) * (ids >= 0)[:, None]
+    assert float(h.abs().max()) < 1 << 24
+    ref, size = torch.zeros(2, tokens, N, dtype=torch.float64)
+    ref[:, :rank], size[:, :rank] = h, h.abs()
+    ref[:, rank:2 * rank - 1], size[:, rank:2 * rank - 1] = h[:, :-1] - h[:, 1:], h[:, :-1].abs() + h[:, 1:].abs()
+    assert ((got - ref).abs() <= 2.0 ** -21 * size).all(), float(((got - ref).abs() / size.clamp(min=1)).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("tokens,K,rank", [(5, 64, 16), (33, 64, 32), (20, 64, 64), (20, 64, 128), (100, 8192, 16), (300, 64, 8), (300, 64, 16),
                                            (300, 64, 32), (300, 64, 64), (300, 64, 128)])
 def test_lora_ranks_of_a_token_far_apart(cuda, dtype, tokens, K, rank):
@@ -307,6 +332,30 @@ def test_lora_ranks_of_a_token_far_apart(cuda, dtype, tokens, K, rank):
     x[~alike] = 0
     again = mx.lora_apply(dev(x), ids.to(cuda), [dev(a)], [b], [y], scales)[0]
     assert torch.equal(again[alike.to(cuda)], got[alike.to(cuda)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,rank", [(3, 8), (20, 64), (300, 32)])
+def test_infinite_b_beside_infinite_sums(cuda, dtype, tokens, rank):
+    """The product of an infinite x . A^T and an infinite element of B is infinite."""
+    import torch
+    g = torch.Generator().manual_seed(rank)
+    x = torch.rand(tokens, 64, generator=g) + 0.5
+    a, b = torch.rand(1, rank, 64, generator=g) + 0.5, torch.rand(1, 40, rank, generator=g) + 0.5
+    b[0, 6, 1], b[0, 7, 1] = math.inf, 0.0
+    ids = torch.zeros(tokens, dtype=torch.int32, device=cuda)
+    dev = lambda t: t.to(_dt(dtype)).to(cuda)  # noqa: E731
+
+    def run():
+        return mx.lora_apply(dev(x), ids, [dev(a)], [dev(b)], [torch.zeros(tokens, 40, device=cuda)])[0].cpu()
+    plain = run()
+    assert (plain[:, 6] == math.inf).all() and torch.isfinite(plain[:, 7:]).all()
+    x[1, 9], x[2, 9] = math.inf, math.nan
+    got = run()
+    assert torch.isnan(got[1, 7]) and (got[1, [n for n in range(40) if n != 7]] == math.inf).all() and torch.isnan(got[2]).all()
+    rest = [t for t in range(tokens) if t not in (1, 2)]
+    assert torch.equal(got[rest], plain[rest])
 
 
 @pytest.mark.gpu

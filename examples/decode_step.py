@@ -84,15 +84,18 @@ def rotate(x, positions):
     return torch.cat([a * c - b * s, b * c + a * s], -1).to(x.dtype)
 
 
+def new_tokens(grown):
+    """Slot and position [rows] of each row's new token, -1 for a row without one: a free row, and one that was refused
+    (its place in the list is the next row's).  What such a row computes is written nowhere and read by nobody."""
+    first, has = grown.starts[:-1].long(), grown.starts[1:] > grown.starts[:-1]
+    at = first.clamp(max=len(grown.slots) - 1)
+    return torch.where(has, grown.slots[at], -1), torch.where(has, grown.positions[at], -1)
+
+
 def step(model, cache, tokens, want, ids):
     """One token for each row: tokens, the lengths after it (0: the row is free) and the adapters [rows], on
-    the device.  Returns the logits [rows, VOCAB]."""
-    grown = cache.resize(want, ROWS)
-    # a free row has no new token: what it computes is written nowhere and read by nobody
-    has = want > 0
-    at = grown.starts[:-1].long().clamp(max=ROWS - 1)
-    slots = torch.where(has, grown.slots[at], -1)
-    positions = torch.where(has, grown.positions[at], -1)
+    the device.  Returns the logits [rows, VOCAB]; those of a row whose length is not the wanted one mean nothing."""
+    slots, positions = new_tokens(cache.resize(want, ROWS))
     x = model.embed[tokens]
     for i, lay in enumerate(model.layers):
         h = norm(x)
@@ -109,37 +112,44 @@ def step(model, cache, tokens, want, ids):
     return model.head(norm(x))
 
 
-def serve(model, requests, steps):
+def serve(model, requests, steps, pages=PAGES):
     """requests: [(prompt tokens, tokens to generate, adapter)].  Returns each one's generated tokens and the
-    logits that chose them, and the cache as it is left."""
+    logits that chose them, and the cache as it is left.  Where the pool has no page for a row's next token the
+    row waits; where no row can go on, the one that came last gives its pages back and starts again later.  A request that
+    the tables or the pool cannot hold is not served at all."""
     dev = model.device
-    cache = mx.PagedKVCache(LAYERS, PAGES, PAGE, KV, DIM, ROWS, LONGEST, device=dev)
-    waiting, rows = list(range(len(requests))), [None] * ROWS
-    fed, want = [0] * ROWS, [0] * ROWS
+    cache = mx.PagedKVCache(LAYERS, pages, PAGE, KV, DIM, ROWS, LONGEST, device=dev)
+    held = lambda q: len(requests[q][0]) + requests[q][1] - 1  # noqa: E731  (the last token is not fed)
+    waiting = [q for q in range(len(requests)) if held(q) <= min(LONGEST, pages * PAGE)]
+    rows, lens = [None] * ROWS, [0] * ROWS  # the request in each, the tokens of it in the cache
     out = [([], []) for _ in requests]
+    came = []  # requests in rows, in the order in which they came
     for _ in range(steps):
-        for r in range(ROWS):
-            if rows[r] is not None and len(out[rows[r]][0]) == requests[rows[r]][1]:
-                rows[r], fed[r] = None, 0  # done: length 0 in this step, its pages go back
-            elif rows[r] is None and want[r] == 0 and waiting:
+        # a row that a request left has length 0 in this step (its pages go back) and is taken in the next
+        for r, q in enumerate(rows):
+            if q is not None and len(out[q][0]) == requests[q][1]:
+                came.remove(q)
+                rows[r] = None
+            elif q is None and lens[r] == 0 and waiting:
                 rows[r] = waiting.pop(0)
+                came.append(rows[r])
         want, tokens, ids = [0] * ROWS, [0] * ROWS, [-1] * ROWS
         for r, q in enumerate(rows):
-            if q is None:
-                continue
-            prompt, _, ids[r] = requests[q]
-            tokens[r] = (prompt + out[q][0])[fed[r]]
-            fed[r] += 1
-            want[r] = fed[r]
+            if q is not None:
+                prompt, _, ids[r] = requests[q]
+                tokens[r], want[r] = (prompt + out[q][0])[lens[r]], lens[r] + 1
         as_dev = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
         logits = step(model, cache, as_dev(tokens).long(), as_dev(want), as_dev(ids))
-        best = logits.argmax(-1).tolist()
+        best, lens = logits.argmax(-1).tolist(), cache.lens.tolist()
         for r, q in enumerate(rows):
-            if q is not None and fed[r] >= len(requests[q][0]):
+            if q is not None and lens[r] == want[r] == len(requests[q][0]) + len(out[q][0]):
                 out[q][0].append(best[r])
                 out[q][1].append(logits[r].float())
         if not any(want) and not waiting:
             break
+        if any(want) and not any(w and n == w for w, n in zip(want, lens)):
+            waiting.insert(0, came.pop())  # it will feed its prompt and what it has generated again
+            rows[rows.index(waiting[0])] = None
     return out, cache
 
 

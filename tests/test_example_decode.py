@@ -55,6 +55,38 @@ def _dense(ex, model, sequence, adapter):
     return norm(x) @ w(model.head).t()
 
 
+def test_a_refused_row_has_no_new_token():
+    """Its place in the list of slots is that of the next row that has one."""
+    import torch
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    # four rows: refused, one token, free, one token at the end of the list
+    grown = mx.Resized(i32(16, 6, 0, 40), i32(0), i32(0, 0, 1, 1, 2), i32(85, 39, -1, -1), i32(5, 39, -1, -1), i32(1))
+    slots, positions = _example().new_tokens(grown)
+    assert slots.tolist() == [-1, 85, -1, 39] and positions.tolist() == [-1, 5, -1, 39]
+    # the last row refused: its place lies past the list
+    grown = mx.Resized(i32(1, 1, 1, 16), i32(0), i32(0, 1, 2, 3, 3), i32(0, 16, 32, -1), i32(0, 0, 0, -1), i32(1))
+    slots, positions = _example().new_tokens(grown)
+    assert slots.tolist() == [0, 16, 32, -1] and positions.tolist() == [0, 0, 0, -1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", [3, 5])
+def test_requests_wait_for_pages(cuda, pages):
+    """A pool too small for the requests that come together: rows wait, the last gives its pages back and starts again;
+    every request that fits the pool alone gets the dense model's logits (bound as below), one that does not gets none."""
+    ex = _example()
+    model = ex.Model(cuda)
+    requests = ex.REQUESTS + [([4] * (pages * ex.PAGE), 2, 0)]
+    out, cache = ex.serve(model, requests, 400, pages)
+    assert out.pop() == ([], [])
+    for (prompt, n, adapter), (tokens, logits) in zip(ex.REQUESTS, out):
+        assert len(tokens) == n and len(logits) == n
+        ref = _dense(ex, model, prompt + tokens[:-1], adapter)[len(prompt) - 1:]
+        for got, want in zip(logits, ref):
+            assert float((got.double().cpu() - want).norm() / want.norm()) < 0.04
+    assert cache.lens.tolist() == [0] * ex.ROWS and sorted(cache.free.tolist()) == list(range(pages))
+
+
 @pytest.mark.gpu
 def test_served_requests_match_a_dense_model(cuda):
     """bf16 activations are rounded about thirty times on the way through the layers (2^-9 rms each, half of them on

@@ -227,7 +227,9 @@ class PagedKVCache:
     """Key and value stores of ``layers`` layers over one pool of pages, and the requests' page tables.
 
     Row r of the tables is a request; ``resize`` brings the requests to new lengths (0 frees a
-    row), ``append`` and ``attend`` work on one layer with the slots and tables that it left."""
+    row), ``append`` and ``attend`` work on one layer with the slots and tables that it left.  All state
+    (``table``, ``lens``, ``free``, ``free_count``) stays in the same memory, so that a captured step goes on
+    from where the last one left it."""
 
     def __init__(self, layers, num_pages, page_size, kv_heads, head_dim, rows, max_tokens, dtype=None, device="cuda",
                  k_scale=None, v_scale=None):
@@ -248,7 +250,7 @@ class PagedKVCache:
     def resize(self, want, tokens, stream=None):
         """Requests to ``want`` [rows] tokens; returns ``Resized`` (slots of up to ``tokens`` new tokens)."""
         r = page_resize(self.table, self.lens, want, self.free, self.free_count, self.page_size, tokens, stream=stream)
-        self.lens, self.free_count = r.lens, r.free_count
+        _on(stream, _torch._foreach_copy_, [self.lens, self.free_count], [r.lens, r.free_count])  # one launch
         return r
 
     def append(self, layer, k, v, slots, stream=None):

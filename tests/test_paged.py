@@ -805,6 +805,39 @@ def test_cache_step_in_a_graph(cuda):
 
 
 @pytest.mark.gpu
+def test_paged_cache_class_in_a_graph(cuda):
+    """A step through the class's methods, captured once: every replay goes on from where the one before it left the rows."""
+    import torch
+    heads, kv, dim, page, rows, steps = 4, 2, 64, 16, 3, 40
+    torch.manual_seed(3)
+    inputs = torch.randn(steps, rows, heads + 2 * kv, dim, device=cuda).to(torch.bfloat16)
+
+    def step(c, x):
+        r = c.resize(c.lens + 1, rows)
+        c.append(0, x[:, heads:heads + kv], x[:, heads + kv:], r.slots)
+        return c.attend(0, x[:, :heads]), r
+    eager = mx.PagedKVCache(1, 20, page, kv, dim, rows, 100, device=cuda)
+    want = [(out.clone(), r.slots.tolist(), r.positions.tolist()) for out, r in (step(eager, x) for x in inputs)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(mx.PagedKVCache(1, 20, page, kv, dim, rows, 100, device=cuda), inputs[0])
+    torch.cuda.current_stream().wait_stream(side)
+    c, x = mx.PagedKVCache(1, 20, page, kv, dim, rows, 100, device=cuda), inputs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, r = step(c, x)
+    for i in range(steps):
+        x.copy_(inputs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert r.positions.tolist() == [i] * rows == want[i][2], i
+        assert r.slots.tolist() == want[i][1] and torch.equal(out, want[i][0]), i
+        assert c.lens.tolist() == [i + 1] * rows
+    assert int(c.free_count) == int(eager.free_count) and c.table.tolist() == eager.table.tolist()
+
+
+@pytest.mark.gpu
 def test_paged_cache_class(cuda):
     import torch
     rows, kv, heads, dim, page = 3, 2, 4, 64, 8

@@ -42,6 +42,19 @@ def test_refusals():
     assert size(tokens=300) == 0 and n.value > 0
 
 
+def test_limits():
+    """The largest sizes the workspace of which is told, and those just past them."""
+    L, n = lora._lib(), ctypes.c_size_t()
+    item = (lora.Item * 1)(lora.Item(None, None, None, None, 32, mx.BF16))
+
+    def size(tokens=300, K=256, adapters=3, rank=16):
+        return L.mlxr_lora_workspace_size(1, item, tokens, K, adapters, rank, ctypes.byref(n))
+    assert size(tokens=1 << 20) == 0 and size(tokens=(1 << 20) + 1) == -3
+    assert size(adapters=4096) == 0 and size(adapters=4097) == -3
+    assert size(rank=128) == 0 and size(rank=136) == -3
+    assert size(K=1 << 28) == 0 and size(K=(1 << 28) + 8) == -3
+
+
 def test_sizes_that_indexes_would_not_hold_are_refused():
     L = lora._lib()
     for N, K in ((32, (1 << 28) + 8), ((1 << 28) + 1, 256)):
@@ -158,6 +171,29 @@ def test_lora_of_wide_projections(cuda, dtype, ydt, tokens, K, adapters, rank, N
 def test_lora_output_types(cuda, dtype, ydt):
     _run(cuda, 37, 512, 4, 16, [130, 64], dtype, ydt)
 
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ydt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,K,rank", [(40, 512, 64), (40, 512, 128), (100, 4608, 16), (64, 2560, 32), (300, 128, 8), (300, 128, 32),
+                                           (300, 128, 64), (300, 128, 128)])
+def test_lora_output_types_of_two_launches(cuda, dtype, ydt, tokens, K, rank):
+    """Every kernel of the second product, at widths whose rows start at any element and end inside a lane's columns."""
+    _run(cuda, tokens, K, 4, rank, [640, 131, 1025], dtype, ydt, seed=rank)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,K,rank", [(9, 256, 16), (40, 512, 64), (300, 128, 32)])
+def test_lora_of_outputs_of_different_types(cuda, tokens, K, rank):
+    import torch
+    x, ids, a, b, y, scales, ranks = _make(cuda, tokens, K, 5, rank, [96, 72, 130, 40, 33], "bf16", "f32", 4)
+    types = ["f32", "bf16", "f16", "bf16", "f32"]
+    y = [t.to(_dt(name)) for t, name in zip(y, types)]
+    got = mx.lora_apply(x.to(cuda), ids.to(cuda), [t.to(cuda) for t in a], [t.to(cuda) for t in b], [t.to(cuda) for t in y],
+                        scales.to(cuda), ranks.to(cuda))
+    for o, A, B, t, name in zip(got, a, b, y, types):
+        assert o.dtype is _dt(name)
+        _check(o, x, ids, A, B, t, scales, ranks, name)
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("ids", [[-1] * 40, [2] * 40, [3, 4, -5, 1 << 30] * 10, list(range(40)), [0] * 16 + [1] * 24, [0] * 17 + [-1] * 23])
@@ -399,3 +435,35 @@ def test_linear_with_adapters(cuda):
         lin(x, lora=bank)
     with pytest.raises(mx.QGemmError, match="do not match"):
         lin(x, lora=mx.LoraBank(2, 8, N, 256, device=cuda), adapter_ids=ids)
+
+
+@pytest.mark.gpu
+def test_concurrent_calls_from_host_threads(cuda):
+    """Four host threads, each with a stream of its own, make calls of every kernel at once: the results of the same
+    calls made alone, bit for bit."""
+    import threading
+    import torch
+    cases = []
+    for tokens, K, rank, dtype in ((9, 256, 16, "bf16"), (40, 512, 64, "f16"), (300, 128, 32, "bf16"), (300, 128, 128, "f16")):
+        x, ids, a, b, y, scales, ranks = _make(cuda, tokens, K, 5, rank, [96, 1030], dtype, dtype, rank)
+        dev = lambda v: [t.to(cuda) for t in v]  # noqa: E731
+        cases.append((x.to(cuda), ids.to(cuda), dev(a), dev(b), dev(y), scales.to(cuda), ranks.to(cuda)))
+    want = [mx.lora_apply(*c) for c in cases]
+    torch.cuda.synchronize()
+    errors = []
+
+    def thread(t):
+        torch.cuda.set_device(cuda)
+        stream = torch.cuda.Stream()
+        for rep in range(20):
+            i = (t + rep) % len(cases)
+            got = mx.lora_apply(*cases[i], stream=stream)
+            stream.synchronize()
+            if not all(torch.equal(g, w) for g, w in zip(got, want[i])):
+                errors.append((t, i))
+    threads = [threading.Thread(target=thread, args=(t,)) for t in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors, errors

@@ -483,6 +483,27 @@ def test_attention_window(cuda, window, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f8")])
+@pytest.mark.parametrize("heads,kv,dim,page", [(8, 2, 128, 16), (33, 1, 128, 8), (4, 4, 256, 6), (6, 2, 80, 16)])
+@pytest.mark.parametrize("window", [1100, 2049, 4000])
+def test_attention_window_of_cut_rows(cuda, dtype, cache, heads, kv, dim, page, window):
+    """Windows of more than 256 KiB a head of few rows: the rows are cut, and what is in the window is joined; rows shorter
+    than it, and empty ones, among them.  Then the same rows behind a table that could hold many more."""
+    import torch
+    lens = [5000, 0, 700, 3001, 1, window, window + 1]
+    g = torch.Generator().manual_seed(window)
+    (k, v), table, (keys, values) = _fill(cuda, lens, kv, dim, page, cache, page == 8, window + dim)
+    q = torch.randn(len(lens), heads, dim, generator=g).to(_dt(dtype)).to(cuda)
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    ref, ref_lse = _attend64(q, keys, values, lens, window, dim ** -0.5)
+    for t in (table, torch.nn.functional.pad(table, (0, 30000 // page), value=-1)):
+        got, lse = mx.paged_attention(q, k, v, t, lt, window=window, out_dtype=torch.float32, return_lse=True)
+        _check(got, ref, values, lens, "f32")
+        assert (lse[1] == -math.inf).all()
+        held = [r for r, n in enumerate(lens) if n]
+        assert float((lse[held].double().cpu() - ref_lse[held]).abs().max()) < 1e-3
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
 def test_attention_output_types(cuda, out):
     _run(cuda, [5, 0, 700], 8, 2, 128, 16, "bf16", "bf16", out=out)
@@ -939,3 +960,49 @@ def test_wrapper_refusals_on_the_gpu(cuda):
     empty = mx.paged_attention(q[:0], k, k, t[:0], two[:0])
     assert empty.shape == (0, 8, 64)
     mx.paged_append(q[:0, :2], q[:0, :2], k, k, two[:0])
+
+
+@pytest.mark.gpu
+def test_concurrent_calls_from_host_threads(cuda):
+    """Four host threads, each with a stream of its own, make calls of every operator of the cache at once: the
+    results of the same calls made alone, bit for bit."""
+    import threading
+    import torch
+    lens = [3000, 0, 33, 1200]
+    cases = []
+    for cache, dim, page in (("bf16", 128, 16), ("f8", 64, 16), ("bf16", 256, 6)):
+        (k, v), table, _ = _fill(cuda, lens, 2, dim, page, cache, False, dim)
+        cases.append((k, v, table, torch.randn(4, 8, dim, device=cuda).to(torch.bfloat16)))
+    lt = torch.tensor(lens, dtype=torch.int32, device=cuda)
+
+    def work(stream):
+        """Attention of the given stores, then resizes, writes and attention of a cache of the thread's own."""
+        got = [mx.paged_attention(q, k, v, t, lt, stream=stream) for k, v, t, q in cases]
+        got += [mx.paged_attention(q, k, v, t[:, :5], lt, window=40, stream=stream) for k, v, t, q in cases]
+        with torch.cuda.stream(stream):
+            c = mx.PagedKVCache(1, 60, 16, 2, 128, 4, 400, device=cuda)
+            rows = torch.arange(128 * 2 * 128, device=cuda).view(128, 2, 128).remainder(63).sub(31).to(torch.bfloat16)
+        for n in (1, 17, 90, 3):
+            with torch.cuda.stream(stream):
+                want = torch.arange(4, dtype=torch.int32, device=cuda) * n
+            r = c.resize(want, 128, stream=stream)
+            c.append(0, rows, rows, r.slots, stream=stream)
+            got += [c.attend(0, cases[0][3], stream=stream), r.slots, r.positions, r.lens]
+        stream.synchronize()
+        return got
+    want = work(torch.cuda.Stream())
+    errors = []
+
+    def thread():
+        torch.cuda.set_device(cuda)
+        stream = torch.cuda.Stream()
+        for _ in range(5):
+            if not all(torch.equal(a, b) for a, b in zip(work(stream), want)):
+                errors.append("mismatch")
+    threads = [threading.Thread(target=thread) for _ in range(4)]
+    torch.cuda.synchronize()
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors

@@ -39,9 +39,9 @@ constexpr int shrink_sub(int rank_groups, int sub) { return sub == 1 || rank_gro
 constexpr int rank_groups_of(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 constexpr int kSplits = 8;  // most splits of K
 constexpr int kPlanThreads = 1024;
-// Workgroups of expand: six for each CU (61 tokens of rank 64 as above with 1024, 1536, 2048: 55, 50, 52 us; 2000 tokens
+// Workgroups of expand for each CU (61 tokens of rank 64 as above with four, six, eight: 55, 50, 52 us; 2000 tokens
 // of 8 adapters of rank 64 164, 151, 149).
-constexpr int kExpandGroups = 1536;
+constexpr int kExpandPerCu = 6;
 
 // A tile's adapter (number `adapters`: none), its rank and scale; `count` tokens, order[16 SUB index ..] (0: no tile).
 struct __attribute__((aligned(16))) Tile {
@@ -805,7 +805,7 @@ Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int a
   // for sorted tokens, whose adapters' last tiles are partly empty), in chunks of whole steps of the workgroup, two at least.
   // us, at once, twice that, half: 64 tokens of 16 adapters of rank 128, K 8192, three projections of 10240 together 43,
   // 46, 51; 16 tokens of rank 64 there 23, 26, 27; 64 of rank 128, K 28672, 8192, 47, 45, 52; 2000 of rank 64 there 67, 73, 85.
-  const long places = 256L * (groups <= 2 ? 2 : 1) * (sorted ? 5 : 4) / 4;
+  const long places = (long)device_cu_count() * (groups <= 2 ? 2 : 1) * (sorted ? 5 : 4) / 4;
   const long want = std::max(1L, places / ((long)std::min(tokens, tokens / group + buckets) * items));
   const int most = std::min(kSplits, (K + 1023) / 1024);
   int splits = (int)(want < most ? want : most);
@@ -814,7 +814,7 @@ Layout layout_of(int count, const mlxr_lora_item* item, int tokens, int K, int a
   // columns of a workgroup of expand: several steps where that leaves enough workgroups, so that what a
   // workgroup does first (its tile, h) is paid less often
   const int step = 16 * columns_of(sorted ? kSub : 1, groups) * kWaves;
-  const long steps = (wide / count + step - 1) / step * items * l.tiles / kExpandGroups;
+  const long steps = (wide / count + step - 1) / step * items * l.tiles / (kExpandPerCu * device_cu_count());
   l.columns = step * (int)std::max(1L, std::min(16L, steps));
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   l.order = 0;

@@ -53,9 +53,13 @@ typedef struct mlxr_paged_cache {
  *   slots_dev, positions_dev  [tokens] int32: slot and position of each new token (rows in order,
  *                  a row's tokens in order), -1 past the last; new tokens past `tokens` are not listed
  *   refused_dev    [1]: rows refused, that is left as they were: want[r] is negative or needs more than
- *                  table_width pages, or the pool has too few pages for it after the rows before it
+ *                  table_width pages, or the pool has too few pages for it and the rows before it that ask for
+ *                  any.  So rows that need pages are served as a prefix: after the first that the pool cannot
+ *                  serve, every later one that needs a page is refused too, also where pages are left for it
+ *                  (rows that need none are not); put those first that should not wait
  * lens_out_dev and free_count_out_dev must not overlap lens_dev and free_count_dev.  lens outside
- * [0, table_width * page_size] are taken as the nearest of these.  One launch, no workspace. */
+ * [0, table_width * page_size] are taken as the nearest of these.  num_pages * page_size and
+ * rows * table_width * page_size are at most 2^31 - 1.  One launch, no workspace. */
 int mlxr_page_resize(int rows, int page_size, int num_pages, int32_t* table_dev, int64_t table_stride, int table_width,
                      const int32_t* lens_dev, const int32_t* want_dev, int32_t* free_dev, const int32_t* free_count_dev,
                      int32_t* lens_out_dev, int32_t* free_count_out_dev, int32_t* starts_dev, int32_t* slots_dev,
@@ -87,7 +91,8 @@ int mlxr_paged_append(const mlxr_paged_cache* cache, int tokens, const void* k_d
  * Tokens of pages whose table entry lies outside the cache are left out; a row with no others is an empty
  * row, as one of length 0.  What lies in the cache past a row's tokens is not used, whatever its
  * bits.  head_dim: a multiple of 8 (e4m3: 16), at most 256; keys' and values' strides and addresses
- * are multiples of 16 bytes, the pages and tokens of a store at most 2^31 elements apart.  Sums,
+ * are multiples of 16 bytes, the pages and tokens of a store less than 2^31 elements apart;
+ * rows * heads is at most 2^24 - 64, the table covers less than 2^31 - 1024 tokens.  Sums,
  * maxima and the output before its rounding are fp32; weights enter their products with the values
  * with 24 bits (bf16 caches) or 22. */
 /* Workspace bytes of a call (0: none is needed, workspace_dev may be NULL). */

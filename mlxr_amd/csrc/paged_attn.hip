@@ -89,7 +89,7 @@ AttnKern& kern(const mlxr_paged_cache* c, int q_dtype) {
 
 constexpr int kGridPerCu = 4;  // most workgroups of a CU that grid_of gives
 constexpr int kJoinMany = 512;
-constexpr int kMaxHeads = 1 << 24;  // rows times heads: the launch's workgroups stay countable
+constexpr int kMaxHeads = (1 << 24) - 64;  // rows times heads: a launch has fewer than 2^32 threads
 
 // How a call runs: short rows in one launch without a workspace.
 struct Plan {

@@ -136,8 +136,8 @@ def page_resize(table, lens, want, free, free_count, page_size, tokens, stream=N
     """Brings the rows of ``table`` [rows, width] from ``lens`` to ``want`` tokens (mlxr_page_resize).
 
     ``free`` [num_pages] is the pool's stack of free pages, its first ``free_count`` [1] entries; both
-    it and the table are changed in place.  ``tokens``: places for the new tokens' slots.  All
-    tensors int32.  Returns ``Resized``; nothing is copied to the host."""
+    it and the table are changed in place.  ``tokens``: places for the new tokens' slots.  Where the pool has too few
+    pages for a row, it and all later rows that need any are refused.  All tensors int32.  Returns ``Resized``; nothing is copied to the host."""
     lib, index, shape = _lib(), table.get_device(), table.shape
     if index < 0:
         raise QGemmError(-1, "page_resize: table must be on a GPU")
@@ -248,7 +248,9 @@ class PagedKVCache:
         self.free_count = torch.full((1,), num_pages, **i32)
 
     def resize(self, want, tokens, stream=None):
-        """Requests to ``want`` [rows] tokens; returns ``Resized`` (slots of up to ``tokens`` new tokens)."""
+        """Requests to ``want`` [rows] tokens; returns ``Resized`` (slots of up to ``tokens`` new tokens).  Rows that
+        need pages are served in their order until the pool has too few for one; it and all later ones that need any are
+        refused: they keep their lengths and have no new token (``starts`` of the next row is theirs)."""
         r = page_resize(self.table, self.lens, want, self.free, self.free_count, self.page_size, tokens, stream=stream)
         _on(stream, _torch._foreach_copy_, [self.lens, self.free_count], [r.lens, r.free_count])  # one launch
         return r

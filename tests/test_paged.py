@@ -78,6 +78,18 @@ def test_attention_refusals():
     assert L.mlxr_paged_attention_workspace_size(ctypes.byref(c), 1, 32, 400, ctypes.byref(n)) == 0 and n.value > 0
 
 
+def test_attention_limits():
+    """Just within the limits, and just past them."""
+    L, n = paged._lib(), ctypes.c_size_t()
+
+    def size(rows=1, heads=8, width=4, **change):
+        return L.mlxr_paged_attention_workspace_size(ctypes.byref(_cache(**change)), rows, heads, width, ctypes.byref(n))
+    assert size(rows=(1 << 21) - 8) == 0 and size(rows=(1 << 21) - 7) == -3
+    assert size(heads=(1 << 24) - 64) == 0 and size(heads=(1 << 24) - 56) == -3
+    assert size(k0=(1 << 31) - 8) == 0 and size(k0=1 << 31) == -3 and size(v2=(1 << 31) - 8) == 0 and size(v2=1 << 31) == -3
+    assert size(width=(1 << 27) - 65) == 0 and size(width=(1 << 27) - 63) == -3
+
+
 def test_resize_refusals():
     L = paged._lib()
 

@@ -11,9 +11,9 @@
 // Bound by the bytes of A, B and y.  A load of a matrix operand as it lies in its lanes is 16 pieces of 16 bytes for
 // each 16 lanes, which the address path serves at a quarter of what whole rows get: x, A and B are loaded by rows and
 // turned in LDS (64 tokens of rank 128 of 16 adapters: K 28672, N 8192 57 -> 47 us, K 4096, two of 14336 49 -> 39).
-// Measured: 61 tokens of 24 adapters of rank 64, K 8192, two of 28672 (194 MB) shrink 13 us, expand 37 (4.1 TB/s); 2048
-// tokens of 6 adapters of rank 32, K 4096, two of 14336 (259 MB) plan 5, shrink 10, expand 48 (5.0 TB/s); 8 tokens of 16
-// adapters of rank 16, K 4096, 6144 together, one launch 9.
+// Measured, in a graph on the same tensors: 61 tokens of 24 adapters of rank 64, K 8192, two of 28672 (194 MB) 40 us; 2048 tokens
+// of 6 adapters of rank 32, K 4096, two of 14336 (259 MB) 59 (plan 5, shrink 9, expand 44 by their own); 8 tokens of 16 adapters
+// of rank 16, K 4096, 6144 together, one launch 8.3.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

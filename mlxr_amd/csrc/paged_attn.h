@@ -21,10 +21,10 @@
 // a wavefront, and a second launch joins them.  Lengths are read on the device; the host chooses by the longest
 // row that the table can hold.
 //
-// Bound by memory: 64 rows of 8 kv heads of 128 in bf16, up to 8192 tokens (961 MB), 156 us and 6 of the join, 6.1 TB/s;
-// one row of 120001 tokens (492 MB) 80 and 6; 32 rows of an e4m3 cache, up to 16384 tokens (547 MB), 98 and 7; 17 rows of 32
-// heads of 80, window 1024, in one launch 38 (158 MB; lines that heads share).  One row of 4 kv heads of 64, 700
-// tokens, 7.4: latency.
+// Bound by memory: 64 rows of 8 kv heads of 128 in bf16, up to 8192 tokens (961 MB), 158 us and 7 of the join, 6.1 TB/s;
+// one row of 120001 tokens (492 MB) 78 and 6; 32 rows of an e4m3 cache, up to 16384 tokens (547 MB), 100 and 7; 17 rows of 32
+// heads of 80, window 1024, in one launch 33 (158 MB; lines that heads share).  One row of 4 kv heads of 64, 700
+// tokens, 7.6: latency.
 #pragma once
 #include <cfloat>
 

@@ -438,6 +438,41 @@ def test_linear_with_adapters(cuda):
 
 
 @pytest.mark.gpu
+def test_mlp_taken_apart_for_adapters(cuda):
+    """Gate and up with adapters, gating, down with adapters; tokens without one get what the layer gives them, within the
+    bf16 rounding of gate and up (2^-8 each, about 2^-8 of the output's norm together as they are independent; bound 2^-6)."""
+    import torch
+    K, inter, tokens = 512, 768, 6
+    torch.manual_seed(6)
+    mlp = mx.MLP(K, inter)
+    banks = {}
+    for i, (name, n, k) in enumerate((("gate", inter, K), ("up", inter, K), ("down", K, inter))):
+        getattr(mlp, name + "_proj").load_weight(mx.synth_gguf(mx.QuantType.Q4_K, n, k, 60 + i), mx.QuantType.Q4_K, device=cuda)
+        banks[name] = mx.LoraBank(2, 8, n, k, device=cuda)
+        for j in range(2):
+            banks[name].load(j, torch.randn(8, k) * k ** -0.5, torch.randn(n, 8) * 0.2, 1.0 + j)
+    gate, up, down = banks["gate"], banks["up"], banks["down"]
+    x = torch.randn(tokens, K).to(torch.bfloat16).to(cuda)
+    ids = torch.tensor([0, 1, -1, 1, -1, 0], dtype=torch.int32, device=cuda)
+    g, u = mx.q_gemm_dequant_grouped(x, [mlp.gate_proj.weight, mlp.up_proj.weight])
+    mx.lora_apply(x, ids, [gate.a, up.a], [gate.b, up.b], [g, u], gate.scales, gate.ranks, outs=[g, u])
+    got = mlp.down_proj(mx.swiglu(g, u, out=g), lora=down, adapter_ids=ids).double().cpu()
+
+    def project(h, name, i):
+        out = h @ mx.dequantize(getattr(mlp, name + "_proj").weight).double().cpu().t()
+        bank = banks[name]
+        if i >= 0:
+            out = out + float(bank.scales[i]) * (h @ bank.a[i].double().cpu().t() @ bank.b[i].double().cpu().t())
+        return out
+    for t, i in enumerate(ids.tolist()):
+        h = x[t].double().cpu()
+        ref = project(torch.nn.functional.silu(project(h, "gate", i)) * project(h, "up", i), "down", i)
+        assert float((got[t] - ref).norm() / ref.norm()) < 2.0 ** -6
+    plain = mlp(x).double().cpu()
+    none = [t for t, i in enumerate(ids.tolist()) if i < 0]
+    assert float((got[none] - plain[none]).norm() / plain[none].norm()) < 2.0 ** -6
+
+@pytest.mark.gpu
 def test_concurrent_calls_from_host_threads(cuda):
     """Four host threads, each with a stream of its own, make calls of every kernel at once: the results of the same
     calls made alone, bit for bit."""

@@ -213,6 +213,12 @@ def test_lora_of_many_adapters(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,rank", [(40, 16), (40, 32), (256, 64), (256, 128), (260, 128)])
+def test_lora_of_the_most_adapters(cuda, tokens, rank):
+    """A counter for each of 4096 adapters beside the LDS of every kernel; tokens that share adapters and that do not."""
+    _run(cuda, tokens, 64, 4096, rank, [24], seed=rank, ids=[(t * 1237) % 4097 - 1 if t % 3 else 4095 for t in range(tokens)])
+
+@pytest.mark.gpu
 def test_lora_f16_products_outside_its_range(cuda):
     """x . A^T far above 65504 and far below 2^-24 in f16: the products between are held in fp32."""
     import torch

@@ -1,6 +1,6 @@
 /*
  * mlxr_paged.h -- C ABI of the paged key-value cache: page tables and slot maps built on the
- * device, writes of new keys and values, and decode attention over the cache
+ * device, writes of new keys and values, decode attention over the cache, and tokens moved within it
  * (libmlxr_qgemm.so; conventions, element types and status codes of mlxr_qgemm.h).
  *
  * A cache holds pages of page_size tokens.  Row r of a batch (a request) owns the pages
@@ -102,6 +102,33 @@ int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int heads, con
                          int64_t q_row_stride, int64_t q_head_stride, const int32_t* table_dev, int64_t table_stride,
                          int table_width, const int32_t* lens_dev, float scale, int window, void* out_dev, int out_dtype,
                          float* lse_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* Tokens moved from slots to slots, bit for bit, in `layers` layers whose stores lie k_layer_stride and
+ * v_layer_stride elements apart (the cache describes the first; its scales are not used).
+ *
+ * mlxr_paged_accept keeps the accepted path of each row's drafted tokens: the last n = starts[r + 1] - starts[r] of
+ * its lens[r] tokens are the nodes of a tree, at positions c .. c + n - 1, c = lens[r] - n.  Node path[r][j] moves to
+ * position c + j, for j < counts[r]; the row then has lens_out[r] = c + the number of nodes kept.
+ *   path_dev       [rows, depth] int32, row stride path_stride: ascending.  An entry that is not above the one before it,
+ *                  or no node of the row, ends its path
+ *   counts_dev     [rows] int32 (negative: 0; past depth: depth)
+ *   lens_out_dev   [rows] int32; not lens_dev
+ * mlxr_page_resize to lens_out then gives back the pages that the other nodes were in.  Tokens of pages outside the
+ * cache are not moved.  No page in two places of the table.  rows up to MLXR_PAGED_MAX_ROWS. */
+int mlxr_paged_accept(const mlxr_paged_cache* cache, int layers, int64_t k_layer_stride, int64_t v_layer_stride,
+                      int rows, const int32_t* table_dev, int64_t table_stride, int table_width, const int32_t* lens_dev,
+                      const int32_t* starts_dev, const int32_t* path_dev, int64_t path_stride, int depth,
+                      const int32_t* counts_dev, int32_t* lens_out_dev, void* stream);
+/* Slots src[i] to slots dst[i]; pairs with a slot outside the cache are left out.  No slot twice in dst, none of dst in
+ * src.  Up to 2^27 tokens. */
+int mlxr_paged_copy(const mlxr_paged_cache* cache, int layers, int64_t k_layer_stride, int64_t v_layer_stride, int tokens,
+                    const int32_t* src_dev, const int32_t* dst_dev, void* stream);
+/* The new tokens of a mlxr_page_resize (its starts, slots and positions) filled from other rows: those of row r with the
+ * tokens at the same positions of row sources[r] (outside [0, rows) or r itself: left out).  Up to 2^27 tokens. */
+int mlxr_paged_fork(const mlxr_paged_cache* cache, int layers, int64_t k_layer_stride, int64_t v_layer_stride, int rows,
+                    const int32_t* table_dev, int64_t table_stride, int table_width, const int32_t* sources_dev,
+                    const int32_t* starts_dev, const int32_t* slots_dev, const int32_t* positions_dev, int tokens,
+                    void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,7 +5,8 @@ The functions take torch tensors as device memory (include/mlxr_paged.h has the 
 - ``page_resize`` brings the requests of a batch to new lengths: pages go back to the pool, pages
   are taken from it, and the slots of the new tokens are listed;
 - ``paged_append`` writes keys and values into those slots;
-- ``paged_attention`` attends with one new token per request over its cached tokens.
+- ``paged_attention`` attends with one new token per request over its cached tokens;
+- ``paged_accept``, ``paged_copy`` and ``paged_fork`` move tokens within the cache, in all layers at once.
 
 ``PagedKVCache`` holds the stores of several layers with the pool and the tables they share.
 A store is ``[num_pages, kv_heads, page_size, head_dim]`` in any memory order whose last
@@ -41,6 +42,9 @@ _SIGS = {
     "mlxr_paged_attention_workspace_size": (_I, [_P, _I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
     "mlxr_paged_attention": (_I, [_P, _I, _I, _P, _I, _I64, _I64, _P, _I64, _I, _P, ctypes.c_float, _I, _P, _I, _P, _P,
                                   ctypes.c_size_t, _P]),
+    "mlxr_paged_accept": (_I, [_P, _I, _I64, _I64, _I, _P, _I64, _I, _P, _P, _P, _I64, _I, _P, _P, _P]),
+    "mlxr_paged_copy": (_I, [_P, _I, _I64, _I64, _I, _P, _P, _P]),
+    "mlxr_paged_fork": (_I, [_P, _I, _I64, _I64, _I, _P, _I64, _I, _P, _P, _P, _P, _I, _P]),
 }
 
 _bound = None
@@ -223,6 +227,58 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
     return (out, lse) if return_lse else out
 
 
+def _layers(k, v):
+    """mlxr_paged_cache of the first of a model's layers' stores [layers, pages, heads, page, dim] (or of one layer's), the
+    layers, their strides and the GPU."""
+    if k.dim() == 4 and v.dim() == 4:
+        k, v = k[None], v[None]
+    if k.dim() != 5 or v.shape != k.shape or k.shape[0] == 0:
+        raise QGemmError(-3, "key and value stores must be [layers, num_pages, kv_heads, page_size, head_dim] of one shape")
+    c, _, _, index = _cache(k[0], v[0], None, None)
+    return c, k.shape[0], k.stride(0), v.stride(0), index
+
+
+def paged_accept(k_store, v_store, table, lens, starts, path, counts, stream=None):
+    """Keeps the accepted path of each row's drafted tokens (mlxr_paged_accept): the last starts[r + 1] - starts[r] of its
+    ``lens`` [rows] tokens are the nodes of a tree; nodes ``path`` [rows, depth] (ascending), the first ``counts`` [rows] of
+    them, move together behind the row's other tokens in every layer of the stores [layers, num_pages, kv_heads, page_size,
+    head_dim].  All int32.  Returns the new lengths [rows]; ``page_resize`` to them gives the other nodes' pages back."""
+    lib = _lib()
+    c, layers, kl, vl, index = _layers(k_store, v_store)
+    pt, (rows, width) = _table(table, index), table.shape
+    pl, ps, pc = _vector(lens, rows, "lens", index), _vector(starts, rows + 1, "starts", index), _vector(counts, rows, "counts", index)
+    if path.dim() != 2 or path.shape[0] != rows:
+        raise QGemmError(-3, "path must have one row per request")
+    if path.dtype is not _int32 or path.get_device() != index or (path.shape[1] > 1 and path.stride()[1] != 1):
+        raise QGemmError(-1, f"path must be an int32 tensor with contiguous rows on GPU {index}")
+    out = _on(stream, _torch.empty, rows, dtype=_int32, device=table.device)
+    qgemm._check(lib.mlxr_paged_accept(c, layers, kl, vl, rows, pt, table.stride()[0], width, pl, ps, path.data_ptr(),
+                                       path.stride()[0], path.shape[1], pc, out.data_ptr(), _stream(stream, index)))
+    return out
+
+
+def paged_copy(k_store, v_store, src, dst, stream=None):
+    """Copies the tokens in slots ``src`` to slots ``dst`` [tokens] (int32; -1: left out), bit for bit, in every layer of the
+    stores (mlxr_paged_copy).  No slot may be twice in dst, or in both."""
+    lib = _lib()
+    c, layers, kl, vl, index = _layers(k_store, v_store)
+    n = src.shape[0] if src.dim() else 0
+    qgemm._check(lib.mlxr_paged_copy(c, layers, kl, vl, n, _vector(src, n, "src", index), _vector(dst, n, "dst", index),
+                                     _stream(stream, index)))
+
+
+def paged_fork(k_store, v_store, table, sources, grown, stream=None):
+    """Fills the new tokens of a ``page_resize`` (``grown``) with those at the same positions of rows ``sources`` [rows]
+    (int32; -1: not filled), in every layer (mlxr_paged_fork)."""
+    lib = _lib()
+    c, layers, kl, vl, index = _layers(k_store, v_store)
+    pt, (rows, width) = _table(table, index), table.shape
+    n = grown.slots.shape[0]
+    qgemm._check(lib.mlxr_paged_fork(c, layers, kl, vl, rows, pt, table.stride()[0], width, _vector(sources, rows, "sources", index),
+                                     _vector(grown.starts, rows + 1, "starts", index), _vector(grown.slots, n, "slots", index),
+                                     _vector(grown.positions, n, "positions", index), n, _stream(stream, index)))
+
+
 class PagedKVCache:
     """Key and value stores of ``layers`` layers over one pool of pages, and the requests' page tables.
 
@@ -264,3 +320,21 @@ class PagedKVCache:
         table = self.table if longest is None else self.table[:, :max(1, -(-longest // self.page_size))]
         return paged_attention(q, self.k[layer], self.v[layer], table, self.lens, k_scale=self.k_scale,
                                v_scale=self.v_scale, **options)
+
+    def accept(self, grown, path, counts, stream=None):
+        """After a pass over drafted tokens (``grown``: what the ``resize`` that made room for them gave): each row keeps
+        the nodes of its accepted path, which become its last tokens, and gives back the pages of the others
+        (paged_accept, page_resize).  Returns ``Resized``."""
+        lens = paged_accept(self.k, self.v, self.table, self.lens, grown.starts, path, counts, stream=stream)
+        return self.resize(lens, 0, stream=stream)
+
+    def fork(self, sources, tokens, stream=None):
+        """Rows whose ``sources`` [rows] (int32) names another row become copies of it; rows with -1 stay.  ``tokens``: at
+        least as many as are copied in all.  A row that becomes a copy must be empty (resize it to 0 before).  Returns
+        ``Resized``; rows for which the pool had no pages are refused as by ``resize``."""
+        def wanted():
+            at = sources.clamp(min=0).long()
+            return _torch.where(sources >= 0, self.lens[at], self.lens)
+        grown = self.resize(_on(stream, wanted), tokens, stream=stream)
+        paged_fork(self.k, self.v, self.table, sources, grown, stream=stream)
+        return grown

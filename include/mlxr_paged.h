@@ -103,6 +103,39 @@ int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int heads, con
                          int table_width, const int32_t* lens_dev, float scale, int window, void* out_dev, int out_dtype,
                          float* lse_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
 
+/* Attention of drafted tokens: the last n = starts[r + 1] - starts[r] of row r's lens[r] cached tokens are the nodes of a
+ * tree (their keys and values are in the cache, written as any tokens'), queries starts[r] .. starts[r] + n - 1 are theirs.
+ * Node i sees the row's tokens before the nodes, and node j where bit j % 64 of mask[token][j / 64] is set, its own
+ * included; without a mask nodes 0 .. i (a chain: the next part of a prompt).
+ *   q_dev          [tokens, heads, head_dim] of q_dtype (as mlxr_paged_attention), strides in elements, multiples of 16
+ *                  bytes; queries from starts[rows] on are padding
+ *   starts_dev     [rows + 1] int32, ascending from 0 (mlxr_page_resize gives them)
+ *   mask_dev       [tokens, words] of 64 bits, or NULL; nodes from 64 * words on are seen by none
+ *   out_dev        [tokens, heads, head_dim] contiguous; padding and nodes that see nothing are zeros
+ *   lse_dev        [tokens, heads] fp32 or NULL: as mlxr_paged_attention
+ * Tokens of pages outside the cache are left out, and nodes before a row's first token (n > lens[r]).  What a node does not
+ * see does not reach it, whatever its bits.  rows up to MLXR_PAGED_MAX_ROWS, tokens * heads up to 2^26; head_dim, strides and
+ * the rest as mlxr_paged_attention, without its limits on the distance of pages.  Sums, maxima and the output before
+ * its rounding are fp32; weights enter their products with the values with 22 bits (f16, e4m3), 24 (bf16 with fp32
+ * outputs) or 16 (bf16 with 16-bit outputs). */
+enum { MLXR_TREE_MAX_WORDS = 64 };
+int mlxr_paged_tree_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int tokens, int heads, int table_width,
+                                             int q_dtype, int out_dtype, size_t* bytes);
+int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows, int tokens, int heads, const void* q_dev, int q_dtype,
+                              int64_t q_token_stride, int64_t q_head_stride, const int32_t* table_dev, int64_t table_stride,
+                              int table_width, const int32_t* lens_dev, const int32_t* starts_dev, const int64_t* mask_dev,
+                              int words, float scale, void* out_dev, int out_dtype, float* lse_dev, void* workspace_dev,
+                              size_t workspace_bytes, void* stream);
+/* Masks of trees: bit j of mask[token] for each node j of the token's row on its way to the root, itself included.
+ *   parents_dev    [tokens] int32: index of a node's parent among its row's nodes, before its own; anything else: a root
+ *   positions_dev  [tokens] int32 or NULL: places of the tokens in their rows (mlxr_page_resize's positions; NULL: the
+ *                  nodes' indices), from which positions_out gets those in the text, place - index + depth (for rotary
+ *                  embeddings; siblings share one)
+ *   mask_dev       [tokens, words]; padding sees nothing
+ *   positions_out_dev  [tokens] int32 or NULL; -1 for padding */
+int mlxr_tree_mask(int rows, int tokens, const int32_t* starts_dev, const int32_t* parents_dev, const int32_t* positions_dev,
+                   int words, int64_t* mask_dev, int32_t* positions_out_dev, void* stream);
+
 /* Tokens moved from slots to slots, bit for bit, in `layers` layers whose stores lie k_layer_stride and
  * v_layer_stride elements apart (the cache describes the first; its scales are not used).
  *

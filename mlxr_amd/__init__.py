@@ -6,6 +6,6 @@ from .qgemm import (F16, F32, BF16, PATH_AUTO, PATH_GEMV, PATH_MFMA, PackedWeigh
                     workspace_size, auto_path)
 from .layers import MLP, Linear, swiglu  # noqa: E402,F401
 from .paged import (PagedKVCache, Resized, page_resize, paged_accept, paged_append, paged_attention,  # noqa: E402,F401
-                    paged_copy, paged_fork)
+                    paged_copy, paged_fork, paged_tree_attention, tree_mask)
 from .lora import LoraBank, lora_apply  # noqa: E402,F401
 from .fp8 import (Fp8Rows, Fp8Weight, fp8_matmul, quantize_fp8, quantize_fp8_weight, rms_norm)  # noqa: E402,F401

@@ -1,0 +1,256 @@
+// Attention of drafted tokens over a paged cache: the C entries, the join of the pieces that the kernel (paged_tree.h)
+// leaves of cut rows, and the masks of trees.
+#include <algorithm>
+
+#include "paged_tree.h"
+
+namespace mlxr {
+namespace tree {
+namespace {
+
+// One token's head for each `lanes` threads, four dims a thread: o = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w over the
+// workgroups w that had a piece of its columns, M the maximum of their m (-inf: no token counted).  Rows without
+// tokens get zeros; columns that one workgroup covered are done.
+__global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
+  const int tid = threadIdx.x, x = tid & (lanes - 1);
+  const int64_t at = (int64_t)blockIdx.x * (kThreads / lanes) + tid / lanes;  // token * heads + head
+  if (at >= (int64_t)a.tokens * a.heads) return;
+  const int token = (int)(at / a.heads), h = (int)(at - (int64_t)token * a.heads);
+  if (token >= a.starts[a.rows]) return;
+  int lo = 0, hi = a.rows;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.starts[mid] <= token) lo = mid;
+    else hi = mid;
+  }
+  const Row row = row_of(a, lo);
+  const int node = token - row.start;
+  if (node < 0 || node >= row.n) return;
+  const bool in = 4 * x < a.dim;
+  float o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.f;
+  const int kvh = a.by_group.quotient(h);
+  if (row.tiles) {
+    const int64_t c = (int64_t)node * a.group + (h - kvh * a.group);
+    const int block = (int)(c / a.qb), i = (int)(c - (int64_t)block * a.qb);
+    const int64_t per = a.prefix[a.rows + 1], s = a.prefix[lo] + ((int64_t)kvh * row.blocks + block) * row.tiles;
+    const int64_t w0 = s / per, w1 = (s + row.tiles - 1) / per;
+    if (w0 == w1) return;
+    constexpr int N = 4;  // pieces on their way at once
+    for (int64_t w = w0; w <= w1; w += N) {
+      float pm[N], pl[N];
+      f32x4_t po[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const bool ok = w + k <= w1;
+        const int64_t v = ok ? w + k : w;
+        const float* sums = a.ws + (v * 2 + (v * per < s ? 1 : 0)) * partial_floats(a.qb, a.dim);  // after another in its run
+        pm[k] = ok ? sums[(int64_t)a.qb * a.dim + 2 * i] : -INFINITY;
+        pl[k] = ok ? sums[(int64_t)a.qb * a.dim + 2 * i + 1] : 0.f;
+        po[k] = ok && in ? *(const f32x4_t*)(sums + (int64_t)i * a.dim + 4 * x) : f32x4_t{0, 0, 0, 0};
+      }
+      float top = m;
+#pragma unroll
+      for (int k = 0; k < N; ++k) top = fmaxf(top, pm[k]);
+      const float ref = top == -INFINITY ? 0.f : top, f0 = __builtin_amdgcn_exp2f(m - ref);
+      m = top;
+      l *= f0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= f0;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const float f = __builtin_amdgcn_exp2f(pm[k] - ref);
+        l += pl[k] * f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += po[k][e] * f;
+      }
+    }
+  }
+  const float f = m == -INFINITY ? 0.f : l == 0.f ? NAN : (a.v_scale ? a.v_scale[kvh] : 1.f) / l;
+  const float v[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
+  if (in) store_values<4>(a.out, a.out_dtype, at * a.dim + 4 * x, v);
+  if (a.lse && x == 0) a.lse[at] = (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
+}
+
+// A token's ancestors: one thread walks from each node to its root, by the parents of the row in LDS where they fit.
+struct MaskArgs {
+  const int32_t *starts, *parents, *positions;
+  uint64_t* mask;
+  int32_t* out;
+  int rows, tokens, words;
+};
+constexpr int kMaskNodes = 4096;  // of a row in LDS
+__global__ __launch_bounds__(kThreads) void mask_kernel(MaskArgs a) {
+  __shared__ int sh[kMaskNodes];
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const int s0 = r < a.rows ? min(max(a.starts[r], 0), a.tokens) : min(max(a.starts[a.rows], 0), a.tokens);
+  if (r == a.rows) {  // padding: nothing is seen
+    for (int t = s0 + tid; t < a.tokens; t += kThreads) {
+      for (int w = 0; w < a.words; ++w) a.mask[(int64_t)t * a.words + w] = 0;
+      if (a.out) a.out[t] = -1;
+    }
+    return;
+  }
+  const int n = min(max(a.starts[r + 1], s0), a.tokens) - s0;
+  for (int i = tid; i < min(n, kMaskNodes); i += kThreads) sh[i] = a.parents[s0 + i];
+  __syncthreads();
+  for (int i = tid; i < n; i += kThreads) {
+    int at = i, depth = 0;
+    for (int w = i >> 6; w >= 0; --w) {
+      uint64_t bits = 0;
+      while (at >= 0 && at >> 6 == w) {  // parents come before their children: the words are met from the last on
+        bits |= 1ull << (at & 63);
+        const int p = at < kMaskNodes ? sh[at] : a.parents[s0 + at];
+        at = p < at ? p : -1;
+        ++depth;
+      }
+      if (w < a.words) a.mask[(int64_t)(s0 + i) * a.words + w] = bits;
+    }
+    for (int w = (i >> 6) + 1; w < a.words; ++w) a.mask[(int64_t)(s0 + i) * a.words + w] = 0;
+    if (a.out) {
+      const int p = a.positions ? a.positions[s0 + i] : i;
+      a.out[s0 + i] = p < 0 ? -1 : p - i + depth - 1;
+    }
+  }
+}
+
+TreeKern kern(const mlxr_paged_cache* c, int q_dtype, int columns, bool three) {
+  const bool f16 = q_dtype == MLXR_F16;
+  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, columns, three) : kern_bf16_e4m3(c->head_dim, columns, three);
+  return f16 ? kern_f16(c->head_dim, columns, three) : kern_bf16(c->head_dim, columns, three);
+}
+
+constexpr int kMaxHeads = 1 << 26;  // tokens times heads: a launch has fewer than 2^32 threads
+constexpr int kGridPerCu = 4;
+
+// How a call runs.
+struct Plan {
+  TreeKern k;
+  bool cut;
+  int64_t units;  // at most: (row, kv head, QB columns)
+  size_t bytes;   // of the workspace
+};
+constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 1) / 2 * 2 * sizeof(int64_t); }
+Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int width, int q_dtype, int out_dtype) {
+  Plan p;
+  const int group = heads / c->kv_heads;
+  const int64_t columns = ((int64_t)tokens * group + rows - 1) / rows;
+  p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), out_dtype == MLXR_F32);
+  p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
+  const int64_t held = (int64_t)width * c->page_size, tiles = (held + p.k.tok - 1) / p.k.tok;
+  p.cut = tiles > 4 && p.units < 8 * device_cu_count();
+  p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
+  return p;
+}
+
+int check_tree(const mlxr_paged_cache* c, int rows, int tokens, int heads, int width) {
+  if (const int rc = check_cache(c)) return rc;
+  if (rows < 0 || tokens < 0 || heads <= 0 || width <= 0) return set_error(MLXR_E_INVALID, "paged_tree_attention: bad sizes");
+  if (heads % c->kv_heads) return set_error(MLXR_E_SHAPE, "heads must be a multiple of kv_heads");
+  if (rows > kMaxRows) return set_error(MLXR_E_SHAPE, "paged_tree_attention: at most %d rows", kMaxRows);
+  if ((int64_t)width * c->page_size > INT32_MAX - 1024) return set_error(MLXR_E_SHAPE, "paged_tree_attention: the table covers too many tokens");
+  if ((int64_t)tokens * heads > kMaxHeads) return set_error(MLXR_E_SHAPE, "paged_tree_attention: at most %d tokens times heads", kMaxHeads);
+  return MLXR_OK;
+}
+int check_types(const mlxr_paged_cache* c, int q_dtype, int out_dtype) {
+  if (q_dtype != MLXR_F16 && q_dtype != MLXR_BF16) return set_error(MLXR_E_INVALID, "invalid query dtype %d", q_dtype);
+  if (c->dtype != MLXR_E4M3 && c->dtype != q_dtype) return set_error(MLXR_E_INVALID, "queries must have the cache's type");
+  if (out_dtype != MLXR_F32 && out_dtype != MLXR_F16 && out_dtype != MLXR_BF16)
+    return set_error(MLXR_E_INVALID, "invalid output dtype %d", out_dtype);
+  return MLXR_OK;
+}
+
+}  // namespace
+}  // namespace tree
+}  // namespace mlxr
+
+using namespace mlxr;
+using namespace mlxr::tree;
+
+extern "C" int mlxr_tree_mask(int rows, int tokens, const int32_t* starts_dev, const int32_t* parents_dev,
+                              const int32_t* positions_dev, int words, int64_t* mask_dev, int32_t* positions_out_dev, void* stream) {
+  if (rows < 0 || tokens < 0 || words <= 0) return set_error(MLXR_E_INVALID, "tree_mask: bad sizes");
+  if (rows > kMaxRows || words > MLXR_TREE_MAX_WORDS)
+    return set_error(MLXR_E_SHAPE, "tree_mask: at most %d rows and %d words", kMaxRows, MLXR_TREE_MAX_WORDS);
+  if (tokens == 0) return MLXR_OK;
+  if (!starts_dev || !parents_dev || !mask_dev) return set_error(MLXR_E_INVALID, "null buffer");
+  MaskArgs a{starts_dev, parents_dev, positions_dev, (uint64_t*)mask_dev, positions_out_dev, rows, tokens, words};
+  mask_kernel<<<(unsigned)(rows + 1), kThreads, 0, (hipStream_t)stream>>>(a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return set_error(MLXR_E_HIP, "tree_mask launch: %s", hipGetErrorString(e));
+  return MLXR_OK;
+}
+
+extern "C" int mlxr_paged_tree_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int tokens, int heads,
+                                                        int table_width, int q_dtype, int out_dtype, size_t* bytes) {
+  if (!bytes) return set_error(MLXR_E_INVALID, "null bytes");
+  if (const int rc = check_tree(cache, rows, tokens, heads, table_width)) return rc;
+  if (const int rc = check_types(cache, q_dtype, out_dtype)) return rc;
+  *bytes = rows && tokens ? plan_of(cache, rows, tokens, heads, table_width, q_dtype, out_dtype).bytes : 0;
+  return MLXR_OK;
+}
+
+extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows, int tokens, int heads, const void* q_dev,
+                                         int q_dtype, int64_t q_token_stride, int64_t q_head_stride, const int32_t* table_dev,
+                                         int64_t table_stride, int table_width, const int32_t* lens_dev, const int32_t* starts_dev,
+                                         const int64_t* mask_dev, int words, float scale, void* out_dev, int out_dtype,
+                                         float* lse_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+  if (const int rc = check_tree(cache, rows, tokens, heads, table_width)) return rc;
+  if (const int rc = check_types(cache, q_dtype, out_dtype)) return rc;
+  if (mask_dev && (words <= 0 || words > MLXR_TREE_MAX_WORDS))
+    return set_error(MLXR_E_SHAPE, "paged_tree_attention: a mask has 1 to %d words", MLXR_TREE_MAX_WORDS);
+  if (tokens == 0) return MLXR_OK;
+  if (rows == 0) return set_error(MLXR_E_INVALID, "paged_tree_attention: tokens without rows");
+  if (!q_dev || !table_dev || !lens_dev || !starts_dev || !out_dev) return set_error(MLXR_E_INVALID, "null buffer");
+  if (q_token_stride % 8 || q_head_stride % 8 || (((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15))
+    return set_error(MLXR_E_SHAPE, "paged_tree_attention: query rows, output and workspace must start at multiples of 16 bytes");
+  const Plan p = plan_of(cache, rows, tokens, heads, table_width, q_dtype, out_dtype);
+  if (workspace_bytes < p.bytes || (p.bytes && !workspace_dev))
+    return set_error(MLXR_E_INVALID, "paged_tree_attention: the workspace is smaller than mlxr_paged_tree_attention_workspace_size");
+  const int es = cache->dtype == MLXR_E4M3 ? 1 : 2;
+  Args a{};
+  a.k = (const uint8_t*)cache->k_dev, a.v = (const uint8_t*)cache->v_dev;
+  a.k_scale = cache->k_scale_dev, a.v_scale = cache->v_scale_dev;
+  a.k_page = cache->k_stride[0] * es, a.k_head = cache->k_stride[1] * es, a.k_token = cache->k_stride[2] * es;
+  a.v_page = cache->v_stride[0] * es, a.v_head = cache->v_stride[1] * es, a.v_token = cache->v_stride[2] * es;
+  a.q = (const uint16_t*)q_dev, a.q_token = q_token_stride, a.q_head = q_head_stride;
+  a.table = table_dev, a.table_stride = table_stride, a.lens = lens_dev, a.starts = starts_dev;
+  a.mask = (const uint64_t*)mask_dev, a.words = words;
+  a.out = out_dev, a.lse = lse_dev, a.out_dtype = out_dtype;
+  a.rows = rows, a.tokens = tokens, a.heads = heads, a.kv_heads = cache->kv_heads, a.group = heads / cache->kv_heads;
+  a.dim = cache->head_dim, a.page = cache->page_size, a.pages = cache->num_pages, a.width = table_width;
+  a.qb = p.k.qb, a.tok = p.k.tok;
+  a.by_page = Divisor(a.page), a.by_group = Divisor(a.group);
+  a.scale = scale * 1.44269504088896341f;
+  const hipStream_t st = (hipStream_t)stream;
+  // LDS: two tiles, the rows' prefix and four sums; the limit is raised to all that a workgroup may use, once on each device
+  const int lds = p.k.lds + (rows + 1 + 4) * (int)sizeof(int64_t), most = (int)device_lds_limit();
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention: %s", hipGetErrorString(e));
+  std::atomic<int>& residents = p.k.residents[dev & 63];
+  int occ = residents.load(std::memory_order_acquire);
+  if (!occ) {
+    e = hipFuncSetAttribute(p.k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == hipSuccess) e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, p.k.fn, kThreads, p.k.lds + 1024);
+    if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention: %s", hipGetErrorString(e));
+    occ = std::max(1, std::min(occ, kGridPerCu));
+    residents.store(occ, std::memory_order_release);
+  }
+  int64_t grid = p.units;
+  if (p.cut) {
+    grid = (int64_t)occ * device_cu_count();
+    a.workers = (int)grid;
+    a.prefix = (int64_t*)workspace_dev, a.ws = (float*)((uint8_t*)workspace_dev + prefix_bytes(rows));
+  }
+  void* args[] = {&a};
+  e = hipLaunchKernel(p.k.fn, dim3((unsigned)grid), dim3(kThreads), args, (size_t)lds, st);
+  if (e == hipSuccess && p.cut) {
+    int lanes = 2;
+    while (4 * lanes < a.dim) lanes *= 2;
+    const int64_t of = kThreads / lanes;
+    join_kernel<<<(unsigned)(((int64_t)tokens * heads + of - 1) / of), kThreads, 0, st>>>(a, lanes);
+    e = hipGetLastError();
+  }
+  if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention launch: %s", hipGetErrorString(e));
+  return MLXR_OK;
+}

@@ -1,0 +1,8 @@
+// Attention of drafted tokens instantiated for one pair of query and cache types (paged_tree.h).
+#include "paged_tree.h"
+
+namespace mlxr {
+namespace tree {
+TreeKern kern_f16(int dim, int columns, bool) { return kern_of<true, false, 2>(dim, columns); }
+}  // namespace tree
+}  // namespace mlxr

@@ -6,6 +6,7 @@ The functions take torch tensors as device memory (include/mlxr_paged.h has the 
   are taken from it, and the slots of the new tokens are listed;
 - ``paged_append`` writes keys and values into those slots;
 - ``paged_attention`` attends with one new token per request over its cached tokens;
+- ``paged_tree_attention`` attends with many drafted tokens per request, a tree (``tree_mask``) or a chain of them;
 - ``paged_accept``, ``paged_copy`` and ``paged_fork`` move tokens within the cache, in all layers at once.
 
 ``PagedKVCache`` holds the stores of several layers with the pool and the tables they share.
@@ -42,6 +43,10 @@ _SIGS = {
     "mlxr_paged_attention_workspace_size": (_I, [_P, _I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
     "mlxr_paged_attention": (_I, [_P, _I, _I, _P, _I, _I64, _I64, _P, _I64, _I, _P, ctypes.c_float, _I, _P, _I, _P, _P,
                                   ctypes.c_size_t, _P]),
+    "mlxr_paged_tree_attention_workspace_size": (_I, [_P] + [_I] * 6 + [ctypes.POINTER(ctypes.c_size_t)]),
+    "mlxr_paged_tree_attention": (_I, [_P] + [_I] * 3 + [_P, _I, _I64, _I64, _P, _I64, _I, _P, _P, _P, _I, ctypes.c_float, _P, _I,
+                                                         _P, _P, ctypes.c_size_t, _P]),
+    "mlxr_tree_mask": (_I, [_I, _I, _P, _P, _P, _I, _P, _P, _P]),
     "mlxr_paged_accept": (_I, [_P, _I, _I64, _I64, _I, _P, _I64, _I, _P, _P, _P, _I64, _I, _P, _P, _P]),
     "mlxr_paged_copy": (_I, [_P, _I, _I64, _I64, _I, _P, _P, _P]),
     "mlxr_paged_fork": (_I, [_P, _I, _I64, _I64, _I, _P, _I64, _I, _P, _P, _P, _P, _I, _P]),
@@ -227,6 +232,69 @@ def paged_attention(q, k_store, v_store, table, lens, scale=None, window=0, k_sc
     return (out, lse) if return_lse else out
 
 
+def tree_mask(parents, starts, words, positions=None, stream=None):
+    """Masks of drafted trees for ``paged_tree_attention`` (mlxr_tree_mask): ``parents`` [tokens] (int32) is the index of each
+    node's parent among its row's nodes (before its own; -1: a root), ``starts`` [rows + 1] the rows' first nodes.  Returns the
+    mask [tokens, words] (int64) and the nodes' positions [tokens] in the text: with ``positions`` (page_resize's) those
+    of the roots' plus their depth, else the depth."""
+    lib, index = _lib(), parents.get_device()
+    if index < 0 or parents.dim() != 1 or starts.dim() != 1 or starts.shape[0] < 1:
+        raise QGemmError(-3, "tree_mask: parents [tokens] and starts [rows + 1] must be on a GPU")
+    n, rows = parents.shape[0], starts.shape[0] - 1
+    pp, ps = _vector(parents, n, "parents", index), _vector(starts, rows + 1, "starts", index)
+    px = None if positions is None else _vector(positions, n, "positions", index)
+    mask = _on(stream, _torch.empty, (n, words if words > 0 else 1), dtype=_torch.int64, device=parents.device)
+    out = _on(stream, _torch.empty, n, dtype=_int32, device=parents.device)
+    qgemm._check(lib.mlxr_tree_mask(rows, n, ps, pp, px, words, mask.data_ptr(), out.data_ptr(), _stream(stream, index)))
+    return mask, out
+
+
+def paged_tree_attention(q, k_store, v_store, table, lens, starts, mask=None, scale=None, k_scale=None, v_scale=None, out=None,
+                         out_dtype=None, return_lse=False, stream=None):
+    """Attention of drafted tokens, q [tokens, heads, head_dim], over their rows' cached tokens (mlxr_paged_tree_attention).
+
+    Row r's queries are starts[r] .. starts[r + 1] - 1 (``starts`` [rows + 1] as page_resize gives them; later queries are
+    padding), its nodes the last as many of its ``lens`` [rows] cached tokens.  A node sees the tokens before them and
+    the nodes whose bits its ``mask`` [tokens, words] (int64; bit j % 64 of word j / 64) has; without a mask itself
+    and the nodes before it.  Returns out [tokens, heads, head_dim] (q's dtype or ``out_dtype``; zeros for padding and for
+    nodes that see nothing), with ``return_lse`` also the log of the softmax's sum, float32 [tokens, heads]."""
+    lib = _lib()
+    c, _, dim, index = _cache(k_store, v_store, k_scale, v_scale)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != dim:
+        raise QGemmError(-3, "queries must be [tokens, heads, head_dim]")
+    if q.get_device() != index:
+        raise QGemmError(-1, "queries must be on the cache's GPU")
+    tokens, heads, _ = shape
+    pt, (rows, width) = _table(table, index), table.shape
+    pl, ps = _vector(lens, rows, "lens", index), _vector(starts, rows + 1, "starts", index)
+    pm, words = None, 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] != tokens:
+            raise QGemmError(-3, "mask must be [tokens, words]")
+        if mask.dtype is not _torch.int64 or mask.get_device() != index or not mask.is_contiguous():
+            raise QGemmError(-1, f"mask must be a contiguous int64 tensor on GPU {index}")
+        pm, words = mask.data_ptr(), mask.shape[1]
+    dt = _code(_x_codes, q.dtype, "queries")
+    if out is None:
+        out = _on(stream, _torch.empty, shape, dtype=out_dtype or q.dtype, device=q.device)
+    elif out.shape != shape or not out.is_contiguous() or out.get_device() != index:
+        raise QGemmError(-1, f"out must be a contiguous [{tokens}, {heads}, {dim}] tensor on GPU {index}")
+    odt = _code(_x_codes, out.dtype, "out")
+    q = _rows16(q, stream)
+    lse = _on(stream, _torch.empty, (tokens, heads), dtype=_float32, device=q.device) if return_lse else None
+    nb = ctypes.c_size_t()
+    qgemm._check(lib.mlxr_paged_tree_attention_workspace_size(c, rows, tokens, heads, width, dt, odt, ctypes.byref(nb)))
+    nb = nb.value
+    ws = _on(stream, _torch.empty, nb, dtype=_torch.uint8, device=q.device) if nb else None
+    qs = q.stride()
+    qgemm._check(lib.mlxr_paged_tree_attention(c, rows, tokens, heads, q.data_ptr(), dt, qs[0], qs[1], pt, table.stride()[0], width,
+                                               pl, ps, pm, words, dim ** -0.5 if scale is None else scale, out.data_ptr(), odt,
+                                               lse.data_ptr() if return_lse else None, ws.data_ptr() if nb else None, nb,
+                                               _stream(stream, index)))
+    return (out, lse) if return_lse else out
+
+
 def _layers(k, v):
     """mlxr_paged_cache of the first of a model's layers' stores [layers, pages, heads, page, dim] (or of one layer's), the
     layers, their strides and the GPU."""
@@ -320,6 +388,13 @@ class PagedKVCache:
         table = self.table if longest is None else self.table[:, :max(1, -(-longest // self.page_size))]
         return paged_attention(q, self.k[layer], self.v[layer], table, self.lens, k_scale=self.k_scale,
                                v_scale=self.v_scale, **options)
+
+    def attend_tree(self, layer, q, starts, mask=None, longest=None, **options):
+        """paged_tree_attention of a layer's drafted tokens, which are the last of their rows (``starts`` as the ``resize`` that made
+        room for them gave).  ``longest``: as for ``attend``."""
+        table = self.table if longest is None else self.table[:, :max(1, -(-longest // self.page_size))]
+        return paged_tree_attention(q, self.k[layer], self.v[layer], table, self.lens, starts, mask, k_scale=self.k_scale,
+                                    v_scale=self.v_scale, **options)
 
     def accept(self, grown, path, counts, stream=None):
         """After a pass over drafted tokens (``grown``: what the ``resize`` that made room for them gave): each row keeps

@@ -1,0 +1,435 @@
+"""Attention of drafted tokens over a paged cache, and masks of trees, against plain float64 forms."""
+import ctypes
+import math
+import random
+
+import pytest
+
+import mlxr_amd as mx
+from mlxr_amd import paged
+
+P = ctypes.c_void_p
+
+
+def _cache(**kw):
+    c = dict(k_dev=64, v_dev=128, k_scale_dev=None, v_scale_dev=None, k0=2048 * 8, k1=2048, k2=128, v0=2048 * 8, v1=2048,
+             v2=128, dtype=mx.BF16, num_pages=10, page_size=16, kv_heads=8, head_dim=128)
+    c.update(kw)
+    return paged.Cache(**c)
+
+
+# ------------------------------------------------------------------------------ refusals (no GPU)
+
+def test_refusals():
+    L, n = paged._lib(), ctypes.c_size_t()
+
+    def call(c=None, rows=2, tokens=6, heads=32, q=64, qdt=mx.BF16, qt=4096, qh=128, table=64, width=4, lens=64, starts=64, mask=64,
+             words=1, out=64, odt=mx.BF16, ws=64, nb=1 << 40):
+        return L.mlxr_paged_tree_attention(ctypes.byref(c or _cache()), rows, tokens, heads, P(q), qdt, qt, qh, P(table), width, width,
+                                           P(lens), P(starts), P(mask), words, 0.1, P(out), odt, None, P(ws), nb, None)
+    assert call(rows=-1) == -1 and call(tokens=-1) == -1 and call(heads=0) == -1 and call(width=0) == -1 and call(tokens=0) == 0
+    assert call(rows=0) == -1 and call(rows=4097) == -3 and call(heads=33) == -3 and call(tokens=1 << 22) == -3
+    assert call(width=1 << 27) == -3 and call(c=_cache(head_dim=12)) == -3
+    assert call(qdt=mx.F32) == -1 and call(qdt=mx.F16) == -1 and call(odt=3) == -1
+    assert call(words=0) == -3 and call(words=65) == -3
+    for name in ("q", "table", "lens", "starts", "out"):
+        assert call(**{name: 0}) == -1, name
+    assert call(q=72) == -3 and call(out=72) == -3 and call(qt=4095) == -3 and call(qh=4) == -3 and call(ws=72) == -3
+    assert call(width=100, ws=0) == -1 and call(width=100, nb=16) == -1
+
+    def size(rows=2, tokens=6, heads=32, width=4, qdt=mx.BF16, odt=mx.BF16):
+        return L.mlxr_paged_tree_attention_workspace_size(ctypes.byref(_cache()), rows, tokens, heads, width, qdt, odt, ctypes.byref(n))
+    assert size() == 0 and n.value == 0 and size(width=400) == 0 and n.value > 0 and size(tokens=0) == 0 and n.value == 0
+    assert size(qdt=mx.F16) == -1 and size(odt=3) == -1 and size(width=0) == -1
+    assert L.mlxr_paged_tree_attention_workspace_size(ctypes.byref(_cache()), 1, 1, 8, 4, mx.BF16, mx.BF16, None) == -1
+
+    def mask(rows=2, tokens=6, starts=64, parents=64, words=1, out=64):
+        return L.mlxr_tree_mask(rows, tokens, P(starts), P(parents), None, words, P(out), None, None)
+    assert mask(rows=-1) == -1 and mask(tokens=-1) == -1 and mask(words=0) == -1 and mask(words=65) == -3 and mask(rows=4097) == -3
+    assert mask(tokens=0) == 0 and mask(starts=0) == -1 and mask(parents=0) == -1 and mask(out=0) == -1
+
+
+def test_wrapper_refusals():
+    import torch
+    k, t = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16), torch.zeros((2, 3), dtype=torch.int32)
+    one = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(mx.QGemmError, match="on one GPU"):
+        mx.paged_tree_attention(torch.zeros((2, 8, 64), dtype=torch.bfloat16), k, k, t, one, one)
+    with pytest.raises(mx.QGemmError, match="on a GPU"):
+        mx.tree_mask(one, one, 1)
+
+
+# ------------------------------------------------------------------------------ the kernels
+
+def _dt(name):
+    import torch
+    return {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32, "f8": torch.float8_e4m3fn}[name]
+
+
+def _i32(v):
+    import torch
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _words(rows_of_bits, words):
+    """[tokens, words] int64 of Python integers of bits."""
+    import torch
+    got = []
+    for b in rows_of_bits:
+        w = [b >> 64 * i & (1 << 64) - 1 for i in range(words)]
+        got.append([v - (1 << 64) if v >> 63 else v for v in w])
+    return torch.tensor(got, dtype=torch.int64, device="cuda").view(len(rows_of_bits), words)
+
+
+def _tree(n, rng):
+    """Parents and bits of a random tree."""
+    parents = [rng.randrange(-1, i) if i else -1 for i in range(n)]
+    bits = []
+    for i, p in enumerate(parents):
+        bits.append((bits[p] if p >= 0 else 0) | 1 << i)
+    return parents, bits
+
+
+class Batch:
+    """Rows with a context and drafts each, their cache and queries."""
+
+    def __init__(self, context, drafts, heads, kv, dim, page, dtype, cache, token_major=False, seed=0, pad=2, spread=1.0, extra=0):
+        import torch
+        self.g = torch.Generator(device="cuda").manual_seed(seed)
+        self.context, self.drafts, self.lens = context, drafts, [a + b for a, b in zip(context, drafts)]
+        self.heads, self.kv, self.dim, self.page, self.cache = heads, kv, dim, page, cache
+        held = [-(-n // page) for n in self.lens]
+        pages = sum(held) + 2
+        order = random.Random(seed).sample(range(pages), pages)
+        self.table = torch.full((len(context), max(held + [1]) + extra), -1, dtype=torch.int32)
+        for r, n in enumerate(held):
+            for i in range(n):
+                self.table[r, i] = order.pop()
+        shape = (pages, page, kv, dim) if token_major else (pages, kv, page, dim)
+        big = 40.0 if cache == "f8" else 1.0
+        self.k, self.v = ((torch.randn(shape, device="cuda", generator=self.g) * big * spread).clamp(-440, 440).to(_dt(cache))
+                          for _ in range(2))
+        if token_major:
+            self.k, self.v = self.k.transpose(1, 2), self.v.transpose(1, 2)
+        self.ks = self.vs = None
+        if cache == "f8":
+            self.ks, self.vs = ((0.5 + torch.rand(kv, device="cuda", generator=self.g)) / 40 for _ in range(2))
+        self.starts = [0]
+        for n in drafts:
+            self.starts.append(self.starts[-1] + n)
+        self.tokens = self.starts[-1] + pad
+        self.q = (torch.randn((self.tokens, heads, dim), device="cuda", generator=self.g) * 2).to(_dt(dtype))
+
+    def call(self, bits=None, words=1, **kw):
+        mask = None if bits is None else _words(bits + [0] * (self.tokens - len(bits)), words)
+        return mx.paged_tree_attention(self.q, self.k, self.v, self.table.cuda(), _i32(self.lens), _i32(self.starts), mask,
+                                       k_scale=self.ks, v_scale=self.vs, **kw)
+
+    def sees(self, r, bits, words):
+        """[drafts, len] of what the nodes of row r see."""
+        import torch
+        n, c = self.drafts[r], self.context[r]
+        got = torch.zeros((n, c + n), dtype=torch.bool)
+        got[:, :c] = True
+        for i in range(n):
+            for j in range(n):
+                got[i, c + j] = j <= i if bits is None else bool(j < 64 * words and bits[self.starts[r] + i] >> j & 1)
+        return got.cuda()
+
+    def values(self, store, scale, r):
+        """[len, kv, dim] of a row's keys or values (64 bits)."""
+        import torch
+        n = self.lens[r]
+        at = torch.arange(n)
+        t = self.table[r, at // self.page].long().cuda()
+        x = store.view(torch.uint8)[t, :, (at % self.page).cuda()].view(store.dtype) if self.cache == "f8" else store[t, :, (at % self.page).cuda()]
+        x = x.double()
+        return x if scale is None else x * scale.double()[None, :, None]
+
+    def check(self, got, lse, bits=None, words=1, scale=None, odt="f32", dtype="bf16"):
+        import torch
+        got, group = got.double(), self.heads // self.kv
+        scale = self.dim ** -0.5 if scale is None else scale
+        half = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}[odt]
+        parts = 2.0 ** -15 if dtype == "bf16" and self.cache == "bf16" and odt != "f32" else 2.0 ** -21
+        assert not got[self.starts[-1]:].any()
+        assert (lse[self.starts[-1]:] == -math.inf).all()
+        for r, n in enumerate(self.drafts):
+            if n == 0:
+                continue
+            a = self.starts[r]
+            sees = self.sees(r, bits, words)
+            k, v = self.values(self.k, self.ks, r), self.values(self.v, self.vs, r)
+            q = self.q[a:a + n].double().view(n, self.kv, group, self.dim)
+            s = torch.stack([q[:, h].reshape(n * group, self.dim) @ k[:, h].t() for h in range(self.kv)]).view(self.kv, n, group, -1) * scale
+            size = torch.stack([q[:, h].reshape(n * group, self.dim).abs() @ k[:, h].abs().t() for h in range(self.kv)])
+            size = size.view(self.kv, n, group, -1).masked_fill(~sees[None, :, None], 0.0).amax(-1) * abs(scale)  # [kv, n, group]
+            s = s.masked_fill(~sees[None, :, None], -math.inf)
+            ref = torch.softmax(s, -1).nan_to_num(0.0)
+            ref = torch.stack([ref[h].reshape(n * group, -1) @ v[:, h] for h in range(self.kv)]).view(self.kv, n, group, self.dim)
+            top = torch.stack([v[:, h].abs().amax() for h in range(self.kv)]).view(-1, 1, 1, 1)
+            # a score is off by 2^-24 of the sum of its magnitudes for each product and five more roundings, its weight by that
+            # much relative, the exponential (2^-22) and its parts; sums of weights add one rounding for each 32 tokens and wavefront
+            own = (self.dim + 8) * 2.0 ** -24 * size + 2.0 ** -21 + parts + (self.lens[r] / 16 + 64) * 2.0 ** -24
+            tol = 2 * own[..., None] * top + half * ref.abs() + (2.0 ** -25 if odt == "f16" else 0)
+            have = got[a:a + n].view(n, self.kv, group, self.dim).permute(1, 0, 2, 3)
+            off = (have - ref).abs() / tol
+            assert off.max().item() <= 1, (r, off.max().item())
+            want = torch.logsumexp(s, -1)
+            have = lse[a:a + n].double().view(n, self.kv, group).permute(1, 0, 2)
+            none = want == -math.inf
+            assert torch.equal(have == -math.inf, none)
+            off = (have - want).abs() / (own + 2.0 ** -21 * want.abs())
+            assert off[~none].numel() == 0 or off[~none].max().item() <= 1
+
+
+CASES = [("bf16", "bf16", 8, 2, 128, 16, False), ("f16", "f16", 32, 4, 64, 16, False), ("bf16", "f8", 16, 2, 128, 32, False),
+         ("f16", "f8", 8, 8, 64, 7, True), ("bf16", "bf16", 7, 1, 256, 5, True), ("f16", "f16", 4, 4, 80, 64, True),
+         ("bf16", "bf16", 6, 3, 8, 1, False), ("bf16", "f8", 10, 2, 112, 16, True), ("f16", "f8", 4, 2, 256, 16, False),
+         ("bf16", "bf16", 40, 1, 96, 24, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache,heads,kv,dim,page,token_major", CASES)
+@pytest.mark.parametrize("nodes", [1, 3, 9, 30, 70, 150])
+def test_trees(dtype, cache, heads, kv, dim, page, token_major, nodes):
+    rng = random.Random(nodes * 31 + dim)
+    drafts = [nodes, rng.randrange(1, nodes + 1), 0, nodes, 1, rng.randrange(1, nodes + 1)]
+    context = [rng.randrange(0, 300), 0, 5, 64 * rng.randrange(1, 4) - nodes % 64, 777, 128]
+    b = Batch(context, drafts, heads, kv, dim, page, dtype, cache, token_major, seed=nodes)
+    words = -(-nodes // 64)
+    bits = []
+    for n in drafts:
+        bits += _tree(n, rng)[1]
+    b.check(*b.call(bits, words, out_dtype=_dt("f32"), return_lse=True), bits, words, dtype=dtype)
+    got, lse = b.call(bits, words, return_lse=True)
+    b.check(got, lse, bits, words, odt=dtype, dtype=dtype)
+    b.check(*b.call(out_dtype=_dt("f32"), return_lse=True), dtype=dtype)  # a chain
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache,heads,kv,dim", [("bf16", "bf16", 32, 8, 128), ("f16", "f16", 8, 1, 64), ("bf16", "f8", 16, 2, 128),
+                                                     ("f16", "f16", 6, 2, 256), ("bf16", "bf16", 64, 2, 128)])
+@pytest.mark.parametrize("drafts", [[3], [5, 12], [40], [100, 7, 64]])
+def test_long_rows_are_cut(dtype, cache, heads, kv, dim, drafts):
+    rng = random.Random(len(drafts))
+    context = [rng.randrange(2500, 5000) for _ in drafts]
+    if len(context) > 1:
+        context[1] = 3
+    b = Batch(context, drafts, heads, kv, dim, 16, dtype, cache, seed=3, pad=0 if len(drafts) == 1 else 3)
+    words, bits = 2, []
+    for n in drafts:
+        bits += _tree(n, rng)[1]
+    b.check(*b.call(bits, words, out_dtype=_dt("f32"), return_lse=True), bits, words, dtype=dtype)
+    b.check(*b.call(out_dtype=_dt("f32"), return_lse=True), dtype=dtype)
+    # the same bits again, and on another stream
+    import torch
+    want = b.call(bits, words)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = b.call(bits, words, stream=side)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(b.call(bits, words), want)
+
+
+@pytest.mark.gpu
+def test_many_rows_and_long_chains():
+    rng = random.Random(8)
+    rows = 600
+    b = Batch([rng.randrange(0, 90) for _ in range(rows)], [rng.randrange(0, 5) for _ in range(rows)], 8, 2, 64, 16, "bf16", "bf16", seed=4)
+    b.check(*b.call(out_dtype=_dt("f32"), return_lse=True))
+    b = Batch([0, 1000], [700, 300], 8, 2, 128, 16, "bf16", "bf16", seed=5)
+    b.check(*b.call(out_dtype=_dt("f32"), return_lse=True))
+    b = Batch([0], [1500], 4, 4, 64, 64, "f16", "f16", seed=5)
+    b.check(*b.call(out_dtype=_dt("f32"), return_lse=True), dtype="f16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [0, 200])  # one launch; cut
+@pytest.mark.parametrize("dtype,heads,kv,dim", [("bf16", 8, 2, 128), ("f16", 16, 1, 64), ("bf16", 2, 2, 256)])
+def test_masks_of_any_shape(dtype, heads, kv, dim, extra):
+    """Masks that are no trees: nothing, one far node, everything, later nodes; without context nothing leaves zeros."""
+    rng = random.Random(dim)
+    drafts, context = [9, 70, 5], [0, 0, 40]
+    b = Batch(context, drafts, heads, kv, dim, 16, dtype, dtype, seed=6, extra=extra)
+    bits = []
+    for n in drafts:
+        bits += [0, 1 << (n - 1), (1 << n) - 1] + [rng.getrandbits(n) for _ in range(n - 3)]
+    bits = [v | rng.getrandbits(60) << 70 for v in bits]  # bits past the row's nodes mean nothing
+    got, lse = b.call(bits, 3, out_dtype=_dt("f32"), return_lse=True)
+    b.check(got, lse, bits, 3, dtype=dtype)
+    assert not got[0].any() and not got[9].any() and got[79].any()
+    got, lse = b.call(bits, 1, out_dtype=_dt("f32"), return_lse=True)  # nodes from 64 on are seen by none
+    b.check(got, lse, bits, 1, dtype=dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [0, 200])
+@pytest.mark.parametrize("dtype,cache,heads,kv,dim", [("bf16", "bf16", 8, 2, 128), ("f16", "f16", 32, 1, 64), ("bf16", "f8", 8, 2, 128)])
+def test_what_is_not_seen_does_not_count(dtype, cache, heads, kv, dim, extra):
+    """NaN and infinities in a node reach those that see it and no others; those behind the row's tokens reach nobody."""
+    import torch
+    b = Batch([37, 100], [20, 33], heads, kv, dim, 16, dtype, cache, seed=7, extra=extra)
+    rng = random.Random(1)
+    bits = []
+    for n in b.drafts:
+        bits += _tree(n, rng)[1]
+    want, lse = b.call(bits, 1, return_lse=True)
+    bad = math.nan if cache == "f8" else math.inf
+    for r, node, value in ((0, 4, math.nan), (1, 9, bad)):
+        at = b.context[r] + node
+        pg, t = int(b.table[r, at // 16]), at % 16
+        keep = b.v[pg, 0, t].clone()
+        b.v[pg, 0, t, dim // 2 + 1] = value
+        got = b.call(bits, 1)
+        group, a = heads // kv, b.starts[r]
+        for i in range(b.drafts[r]):
+            sees = bits[a + i] >> node & 1
+            cell = got[a + i, :group, dim // 2 + 1]
+            if sees:
+                assert (cell == math.inf).all() if value == math.inf else torch.isnan(cell).all()
+                got[a + i, :group, dim // 2 + 1] = want[a + i, :group, dim // 2 + 1]
+        assert torch.equal(got, want)
+        b.v[pg, 0, t] = keep
+        keep = b.k[pg, 0, t].clone()
+        b.k[pg, 0, t] = math.nan
+        got = b.call(bits, 1)
+        for i in range(b.drafts[r]):
+            if bits[a + i] >> node & 1:
+                got[a + i, :group] = want[a + i, :group]
+        assert torch.equal(got, want)
+        b.k[pg, 0, t] = keep
+    # behind the last token, and in pages of nobody
+    used = {int(p) for p in b.table.flatten() if p >= 0}
+    for pg in set(range(b.k.shape[0])) - used:
+        b.k[pg], b.v[pg] = math.nan, math.nan
+    for r, n in enumerate(b.lens):
+        if n % 16:
+            pg = int(b.table[r, n // 16])
+            b.k[pg, :, n % 16:], b.v[pg, :, n % 16:] = math.nan, math.nan
+    got, l2 = b.call(bits, 1, return_lse=True)
+    assert torch.equal(got, want) and torch.equal(l2, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [0, 200])
+def test_bad_pages_lengths_and_starts(extra):
+    """Tokens of pages outside the cache are left out; a row whose tokens all are, or that has none, gives zeros; lengths past
+    the table are taken as the table's; a row of more nodes than tokens has nodes before its first token."""
+    import torch
+    b = Batch([40, 30, 20, 64], [4, 5, 6, 7], 8, 2, 128, 16, "bf16", "bf16", seed=9, extra=extra)
+    bits = [(1 << 7) - 1] * b.starts[-1]
+    table = b.table.clone()
+    b.table[0, 1], b.table[1, :] = b.k.shape[0], -1
+    got, lse = b.call(bits, 1, out_dtype=_dt("f32"), return_lse=True)
+    assert not got[4:9].any() and (lse[4:9] == -math.inf).all()
+    # row 0 without positions 16 .. 31: as if its row were two pages
+    c = Batch([24], [4], 8, 2, 128, 16, "bf16", "bf16", seed=9)
+    c.k, c.v, c.q = b.k, b.v, b.q[:6]
+    c.table = torch.cat([table[:1, :1], table[:1, 2:3]], 1)
+    want = c.call([15] * 4, 1, out_dtype=_dt("f32"))
+    assert (got[:4] - want[:4]).abs().max().item() < 1e-5
+    b.table = table
+    b.lens = [-3, 0, 4, 1 << 30]
+    got, lse = b.call(bits, 1, out_dtype=_dt("f32"), return_lse=True)
+    assert not got[:9].any() and (lse[:9] == -math.inf).all()
+    assert torch.isfinite(got).all() and got[9:15].any()  # nodes 2 .. 5 at positions 0 .. 3
+    c = Batch([0], [4], 8, 2, 128, 16, "bf16", "bf16", seed=9)
+    c.k, c.v, c.table, c.q = b.k, b.v, table[2:3], torch.cat([b.q[9:15]])
+    c.starts, c.tokens, c.drafts = [0, 4], 6, [4]
+    want = c.call([15] * 4, 1, out_dtype=_dt("f32"))
+    assert (got[9:13] - want[:4]).abs().max().item() < 1e-5
+
+
+@pytest.mark.gpu
+def test_strides_and_outputs():
+    import torch
+    b = Batch([100, 9], [5, 12], 8, 2, 64, 16, "bf16", "bf16", seed=10)
+    bits = [(1 << 12) - 1] * 17
+    want = b.call(bits, 1)
+    wide = torch.zeros((b.tokens, 3, 8, 72), dtype=torch.bfloat16, device="cuda")
+    wide[:, 1, :, :64] = b.q
+    b.q = wide[:, 1, :, :64]
+    assert torch.equal(b.call(bits, 1), want)
+    odd = torch.zeros((b.tokens, 8, 65), dtype=torch.bfloat16, device="cuda")
+    odd[..., 1:] = b.q
+    b.q = odd[..., 1:]
+    assert torch.equal(b.call(bits, 1), want)
+    out = torch.full((b.tokens + 1, 8, 64), 3.0, dtype=torch.float16, device="cuda")
+    assert b.call(bits, 1, out=out[:-1]).data_ptr() == out.data_ptr() and (out[-1] == 3).all()
+    assert torch.allclose(out[:-1].float(), want.float(), atol=2e-2)
+    table = torch.full((2, 300), 7, dtype=torch.int32)
+    table[:, 5:5 + b.table.shape[1]] = b.table
+    b.table = table[:, 5:5 + b.table.shape[1]]
+    assert torch.equal(b.call(bits, 1), want)
+
+
+@pytest.mark.gpu
+def test_past_four_gigabytes():
+    """Pages, heads and tokens far apart: offsets past 32 bits."""
+    import torch
+    room = torch.empty(9 << 30, dtype=torch.uint8, device="cuda").view(torch.bfloat16)
+    k = room.as_strided((2, 2, 16, 64), (1 << 31, 1 << 30, 64, 1))
+    v = room.as_strided((2, 2, 16, 64), (1 << 31, 1 << 30, 64, 1), 4096)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k.copy_(torch.randn(k.shape, device="cuda", generator=g)), v.copy_(torch.randn(v.shape, device="cuda", generator=g))
+    q = torch.randn((6, 4, 64), device="cuda", generator=g).bfloat16()
+    table, lens, starts = _i32([[1, 0]]), _i32([30]), _i32([0, 6])
+    assert torch.equal(mx.paged_tree_attention(q, k, v, table, lens, starts),
+                       mx.paged_tree_attention(q, k.contiguous(), v.contiguous(), table, lens, starts))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [8, 300])
+def test_in_a_graph(width):
+    """A captured call follows lengths, starts and masks that change between replays."""
+    import torch
+    b = Batch([90, 17], [6, 9], 8, 2, 128, 16, "bf16", "bf16", seed=11, extra=width - 7)
+    table, lens, starts = b.table.cuda(), _i32(b.lens), _i32(b.starts)
+    mask = _words([(1 << 9) - 1] * b.tokens, 1)
+
+    def call():
+        return mx.paged_tree_attention(b.q, b.k, b.v, table, lens, starts, mask)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for ln, st, bits in ((b.lens, b.starts, 511), ([50, 26], [0, 3, 12], 7), ([96, 3], [0, 15, 15], 0x7fff), ([0, 26], [0, 0, 0], 1)):
+        lens.copy_(_i32(ln)), starts.copy_(_i32(st)), mask.copy_(_words([bits] * b.tokens, 1))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = held.clone()
+        assert torch.equal(got, call())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nodes,words", [(1, 1), (5, 1), (64, 1), (65, 2), (130, 1), (300, 5), (5000, 3)])
+def test_tree_masks(nodes, words):
+    rng = random.Random(nodes)
+    drafts = [nodes, 0, rng.randrange(1, nodes + 1), 1]
+    parents, bits, depth = [], [], []
+    for n in drafts:
+        p, b = _tree(n, rng) if n < 1000 else ([i - 1 if i % 3 else max(i - 3000, -1) for i in range(n)], None)
+        if b is None:
+            b = []
+            for i, x in enumerate(p):
+                b.append((b[x] if x >= 0 else 0) | 1 << i)
+        d = []
+        for i, x in enumerate(p):
+            d.append(d[x] + 1 if x >= 0 else 0)
+        if n > 3:
+            i = n - 1  # no parent before it: a root
+            p[i], b[i], d[i] = n + 5, 1 << i, 0
+        parents, bits, depth = parents + p, bits + b, depth + d
+    starts = [0]
+    for n in drafts:
+        starts.append(starts[-1] + n)
+    at = [j + 10 * r for r, n in enumerate(drafts) for j in range(n)]
+    pad = [0, 1]
+    mask, pos = mx.tree_mask(_i32(parents + pad), _i32(starts), words, positions=_i32(at + [-1, -1]))
+    low = [v & (1 << 64 * words) - 1 for v in bits]
+    assert mask.tolist() == _words(low + [0, 0], words).tolist()
+    want = [10 * r + depth[starts[r] + j] for r, n in enumerate(drafts) for j in range(n)]
+    assert pos.tolist() == want + [-1, -1]
+    assert mx.tree_mask(_i32(parents + pad), _i32(starts), words)[1].tolist() == depth + [-1, -1]

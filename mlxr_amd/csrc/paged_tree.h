@@ -10,11 +10,12 @@
 // Which token an element of the second product's 32 is, is free: lane group g's eight are tokens 4 g .. 4 g + 3 of two
 // neighbouring 16 x 16 tiles of S^T, as the first product leaves them.  P enters in 16-bit parts: f16 (and the values of an
 // e4m3 cache, exact in f16) two parts, 22 bits; bf16 three, 24 bits, for fp32 outputs, two, 16 bits, for 16-bit outputs, whose
-// own half step (2^-9, 2^-12) is far larger than what that leaves out of each weight (2^-17).
+// own half step (2^-9, 2^-12) is far larger than what that leaves out of each weight (2^-17); an e4m3 cache with
+// bf16 outputs one, which leaves out 2^-12 of a weight, an eighth of the output's half step.  (Matrix instructions bound
+// wide trees, and each part is half as many as the first product takes.)
 //
 // A tile of TOK tokens goes memory -> registers -> LDS, one tile ahead: while tile t is multiplied, t + 1 is on its way to
-// registers; it is written to the other half of LDS before the tile's one barrier.  Four wavefronts are WQ groups of
-// columns times WT groups of the tile's tokens (merged at the end), by the columns that a row has on average.
+// registers; it is written to the other half of LDS before the tile's one barrier.
 //
 // The tiles of all (row, kv head, QB columns) are dealt to the workgroups of a launch that fills the device in equal
 // contiguous runs; a run that covers all of its columns' tiles writes the output, others leave (m, sum, unnormalized o) in
@@ -22,6 +23,7 @@
 // (row, kv head, QB columns).
 #pragma once
 #include <cfloat>
+#include <type_traits>
 
 #include "paged_attn.h"
 
@@ -32,8 +34,9 @@ using paged::load_words;
 using paged::store_values;
 using paged::widen;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = 4;
 constexpr int kMaxRows = MLXR_PAGED_MAX_ROWS;
+constexpr int kStart = 2;  // tiles that the start and the end of a row's columns are counted for
 
 struct Args {
   const uint8_t *k, *v;  // element addresses in bytes
@@ -78,20 +81,28 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
 // Floats of a cut run's partial sums: QB rows of dim, then m and sum of each.
 __host__ __device__ constexpr int partial_floats(int qb, int dim) { return qb * dim + 2 * qb; }
 
-// The 64 bits from bit `at` on of what node i sees: 1s before its row's drafts (at < 0), the mask's words, then 0s.
-__device__ __forceinline__ uint64_t mask_word(const Args& a, const uint64_t* mask, int w) {
-  return w < 0 ? ~0ull : w < a.words ? mask[w] : 0ull;
-}
-__device__ __forceinline__ uint64_t seen(const Args& a, int token, int i, int at) {
-  if (!a.mask) {
-    const int more = i - at;  // the last bit that counts
-    return more < 0 ? 0ull : more >= 63 ? ~0ull : (2ull << more) - 1;
+// What a node sees of its row's nodes: 64 bits from bit `at` on, 1s before the nodes (at < 0).  The first two words stay in
+// registers; no mask: bits 0 .. i.
+struct Seen {
+  uint64_t w[2];
+  __device__ __forceinline__ void start(const Args& a, int token) {
+    const uint64_t* mask = a.mask + (int64_t)token * a.words;
+    w[0] = a.mask ? mask[0] : 0;
+    w[1] = a.mask && a.words > 1 ? mask[1] : 0;
   }
-  const uint64_t* m = a.mask + (int64_t)token * a.words;
-  const int w = at >> 6, s = at & 63;
-  const uint64_t lo = mask_word(a, m, w);
-  return s ? lo >> s | mask_word(a, m, w + 1) << (64 - s) : lo;
-}
+  __device__ __forceinline__ uint64_t word(const Args& a, int token, int k) const {
+    return k < 0 ? ~0ull : k < 2 ? (k ? w[1] : w[0]) : k < a.words ? a.mask[(int64_t)token * a.words + k] : 0ull;
+  }
+  __device__ __forceinline__ uint64_t bits(const Args& a, int token, int i, int at) const {
+    if (!a.mask) {
+      const int more = i - at;  // the last bit that counts
+      return more < 0 ? 0ull : more >= 63 ? ~0ull : (2ull << more) - 1;
+    }
+    const int k = at >> 6, s = at & 63;
+    const uint64_t lo = word(a, token, k);
+    return s ? lo >> s | word(a, token, k + 1) << (64 - s) : lo;
+  }
+};
 
 // Two weights in PARTS 16-bit parts that add up to them (the last rounded), none negative nor a later one 0: an infinite
 // value then gives an infinite output as a weight in one piece does, not NaN.
@@ -99,10 +110,15 @@ template <bool P16, int PARTS>
 __device__ __forceinline__ void split_parts(float p0, float p1, uint32_t (&out)[PARTS]) {
   auto floor2 = [](uint32_t w) { return paged::pair_max(w, P16 ? 0x00010001u : 0x00800080u); };
   if constexpr (P16) {
-    static_assert(PARTS == 2, "f16: two parts");
-    const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-    out[0] = hi;
-    out[1] = floor2(pack2<true>(p0 - unpack<true>(hi, 0), p1 - unpack<true>(hi, 1)));
+    if constexpr (PARTS == 1) {
+      typedef __attribute__((ext_vector_type(2))) float f32x2;
+      typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+      out[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{p0, p1}), f16x2));
+    } else {
+      const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+      out[0] = hi;
+      out[1] = floor2(pack2<true>(p0 - unpack<true>(hi, 0), p1 - unpack<true>(hi, 1)));
+    }
   } else {
 #pragma unroll
     for (int n = 0; n < PARTS - 1; ++n) {  // each the upper half of what is left
@@ -123,52 +139,65 @@ __device__ __forceinline__ bool odd_half(uint32_t h) {
   return (h & E) == E;
 }
 template <bool F16>
+__device__ __forceinline__ bool odd_word(uint32_t w) {
+  return odd_half<F16>(w) || odd_half<F16>(w >> 16);
+}
+template <bool F16>
 __device__ __forceinline__ uint32_t clean2(uint32_t w) {
   if (odd_half<F16>(w)) w &= 0xffff0000u;
   if (odd_half<F16>(w >> 16)) w &= 0x0000ffffu;
   return w;
 }
 
-template <bool F16, bool F8, int DT, int WQ, int WT, int CW, int PARTS>
+// DT: 64, 128 or 256, at least head_dim.  CW: columns of a wavefront, by 16.  TOK: tokens of a tile (32, 64).  OCC: workgroups
+// that a CU's registers and LDS hold.
+template <bool F16, bool F8, int DT, int CW, int TOK, int OCC, int PARTS>
 struct Kern {
   static constexpr bool P16 = F16 || F8;                      // the second product's type, f16 or else bf16
-  static constexpr int TPW = WT == 1 && DT < 256 ? 64 : 32;   // tokens of a tile and wavefront
-  static constexpr int TOK = TPW * WT, QB = 16 * CW * WQ;
-  static constexpr int NT = TPW / 16, KT = TPW / 32, KS = DT / 32, ND = DT / 16;
+  static constexpr int QB = 16 * CW * kWaves;
+  static constexpr int NT = TOK / 16, KT = TOK / 32, KS = DT / 32, ND = DT / 16;
   static constexpr int CH = DT / 8;                           // 16-byte pieces of a row in LDS
   static constexpr int CG = F8 ? DT / 16 : DT / 8;            // and in memory
-  static constexpr int NL = TOK * CG / kThreads;              // loads of a thread, tile and store
-  static constexpr int SETS = (TOK + 63) / 64;
+  static constexpr int R = kThreads / TOK;                    // threads that bring a token's key and value to LDS
+  static constexpr int LR = R == 4 ? 2 : 3;
+  static constexpr int NL = CG / R > 0 ? CG / R : 1;          // loads of a thread, tile and store
   static constexpr int STORE = TOK * DT * 2;                  // bytes of a tile's keys or values in LDS
-  static constexpr int PARK = (4 * ND + 2) * CW * 256;        // bytes of a wavefront's sums
-  static constexpr int LDS = 4 * STORE > (WT > 1 ? WQ * WT / 2 * PARK : 0) ? 4 * STORE : WQ * WT / 2 * PARK;
-  static constexpr float SHIFT = P16 ? 14.f : 0.f;            // f16: weights down to 2^-28 stay normal numbers
-  static constexpr float UNSHIFT = P16 ? 0x1p-14f : 1.f;
+  static constexpr int LDS = 4 * STORE;
+  // The reference that weights are relative to follows the maximum only when that is 2^SLACK above it: weights are at most
+  // 2^(SHIFT + SLACK), below f16's largest number, and down to 2^-22 of that they stay normal ones.
+  static constexpr float SHIFT = P16 ? 8.f : 0.f, SLACK = 7.f;
+  static constexpr float UNSHIFT = P16 ? 0x1p-8f : 1.f;
 
-  // Place of 16-byte piece c of token t's key: the 16 rows of an operand's read lie in different banks.
+  // Places in LDS: 16-byte piece c of token t's key, 16 dims (32 bytes) p of its value.  What 16 lanes access at once lies in
+  // different banks: 16 tokens' piece of an operand's read, four tokens' dims of the transposing read (eight for two lane
+  // groups), and R pieces of 16 / R tokens of a write.
   static __device__ __forceinline__ int key_place(int t, int c) {
-    return t * DT * 2 + (CH >= 16 ? c ^ (t & 15) : c ^ (t >> 1 & 7)) * 16;
+    constexpr int N = CH >= 16 ? 4 : 3;  // bits of a piece's place within 256 bytes of banks; shorter rows are two to those
+    const int u = CH >= 16 ? t : t >> 1;
+    return t * DT * 2 + (c ^ ((u & ((1 << (N - LR)) - 1)) << LR | (u >> (N - LR) & (R - 1)))) * 16;
   }
-  // Place of 16 dims (32 bytes) p of token t's value: the four tokens of two lane groups' transposing read likewise.
   static __device__ __forceinline__ int value_place(int t, int p) {
-    return t * DT * 2 + (ND >= 8 ? p ^ (t & 7) : p ^ (t >> 1 & 3)) * 32;
+    const int swap = ND < 8 ? (t & 2) | (t >> 2 & 1) : R == 8 ? (t & 1) << 2 | (t >> 1 & 3) : (t & 3) << 1 | (t >> 2 & 1);
+    return t * DT * 2 + (p ^ swap) * 32;
   }
 };
 
-template <bool F16, bool F8, int DT, int WQ, int WT, int CW, int PARTS>
-__global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void tree_kernel(Args a) {
-  using T = Kern<F16, F8, DT, WQ, WT, CW, PARTS>;
-  constexpr int NT = T::NT, KT = T::KT, KS = T::KS, ND = T::ND, NL = T::NL, CG = T::CG, TOK = T::TOK;
+template <bool F16, bool F8, int DT, int CW, int TOK, int OCC, int PARTS>
+__global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
+  using T = Kern<F16, F8, DT, CW, TOK, OCC, PARTS>;
+  constexpr int NT = T::NT, KT = T::KT, KS = T::KS, ND = T::ND, NL = T::NL;
   constexpr bool P16 = T::P16;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wq = wave / WT, wt = wave - wq * WT, g = lane >> 4, col = lane & 15;
+  const int g = lane >> 4, col = lane & 15;
 
   // ---- this workgroup's run of tiles
   int64_t* pre = (int64_t*)(lds + T::LDS);  // [rows + 1] before each row: tiles, or (not cut) blocks of columns
   int64_t* part = pre + a.rows + 1;         // [4]
+  int* flag = (int*)(part + 4);             // [2][4] of the tiles' wavefronts
   const bool cut = a.ws != nullptr;
-  auto weight = [&](const Row& w) { return (int64_t)a.kv_heads * w.blocks * (cut ? w.tiles : 1); };
+  // a unit of the deal: kStart places, then its tiles
+  auto weight = [&](const Row& w) { return (int64_t)a.kv_heads * w.blocks * (!cut ? 1 : w.tiles ? w.tiles + kStart : 0); };
   {
     const int per_thread = (a.rows + kThreads - 1) / kThreads;
     const int r0 = min(tid * per_thread, a.rows), r1 = min(r0 + per_thread, a.rows);
@@ -230,34 +259,45 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void tree_kernel(Args 
       continue;
     }
     const int64_t in_row = pos - pre[r];
-    const int unit = (int)(cut ? in_row / row.tiles : in_row);
-    const int first = cut ? (int)(in_row - (int64_t)unit * row.tiles) : 0;
-    const int count = cut ? (int)min((int64_t)(row.tiles - first), end - pos) : row.tiles;
+    const int span = row.tiles + kStart, unit = (int)(cut ? in_row / span : in_row), from = (int)(in_row - (int64_t)unit * span);
+    const int places = cut ? (int)min((int64_t)(span - from), end - pos) : 0;  // of this run
+    const int first = cut ? max(from - kStart, 0) : 0, count = cut ? max(from + places - kStart, 0) - first : row.tiles;
+    if (cut && count == 0) {  // the run ends within a unit's first places
+      pos += places;
+      continue;
+    }
     const int kvh = unit / row.blocks, block = unit - kvh * row.blocks;
     const int32_t* trow = a.table + (int64_t)r * a.table_stride;
     const uint8_t *kh = a.k + (int64_t)kvh * a.k_head, *vh = a.v + (int64_t)kvh * a.v_head;
-    const float sc = a.scale * (a.k_scale ? a.k_scale[kvh] : 1.f);
+    // scores times sc, which is made positive by the queries' sign (and never 0: -inf stays -inf)
+    const float signed_sc = a.scale * (a.k_scale ? a.k_scale[kvh] : 1.f);
+    const float sc = fabsf(signed_sc) < FLT_MIN ? FLT_MIN : fabsf(signed_sc);
+    const uint32_t flip = signed_sc < 0.f ? 0x80008000u : 0u;
 
-    // columns of this wavefront: (node, head) pairs
-    int node[CW], head[CW];
-    bool has[CW];
+    // columns of this wavefront: (node, head) pairs; those past the row's last are node 0's with queries of 0
+    const int columns = row.n * a.group, first_column = block * T::QB + wave * CW * 16 + col;
+    const bool idle = block * T::QB + wave * CW * 16 >= columns;  // the wavefront only brings tiles
+    int node[CW];
+    Seen sees[CW];
     u32x4_t q[CW][KS];
 #pragma unroll
     for (int j = 0; j < CW; ++j) {
-      const int c = block * T::QB + (wq * CW + j) * 16 + col;
-      has[j] = c < row.n * a.group;
-      node[j] = has[j] ? a.by_group.quotient(c) : 0;
-      head[j] = kvh * a.group + (has[j] ? c - node[j] * a.group : 0);
-      const uint16_t* p = a.q + (int64_t)(row.start + node[j]) * a.q_token + (int64_t)head[j] * a.q_head;
+      const int c = first_column + 16 * j;
+      const bool has = c < columns;
+      node[j] = has ? a.by_group.quotient(c) : 0;
+      sees[j].start(a, row.start + node[j]);
+      const uint16_t* p = a.q + (int64_t)(row.start + node[j]) * a.q_token + (int64_t)(kvh * a.group + (has ? c - node[j] * a.group : 0)) * a.q_head;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int d = 32 * s + 8 * g;
-        q[j][s] = has[j] && d < a.dim ? *(const u32x4_t*)(p + d) : u32x4_t{0, 0, 0, 0};
+        q[j][s] = has && d < a.dim ? *(const u32x4_t*)(p + d) : u32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < 4; ++n) q[j][s][n] ^= flip;
       }
     }
     f32x4_t o[ND][CW];
-    float m[CW], l[CW];
-    bool counts[CW];  // some token of the column counts
+    float m[CW], l[CW];  // what weights are relative to, and their sum
+    bool counts[CW];     // some token of the column counts
 #pragma unroll
     for (int j = 0; j < CW; ++j) {
       m[j] = -INFINITY, l[j] = 0.f, counts[j] = false;
@@ -265,195 +305,202 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void tree_kernel(Args 
       for (int d = 0; d < ND; ++d) o[d][j] = f32x4_t{0, 0, 0, 0};
     }
 
-    // ---- a tile's way to LDS
+    // ---- a tile's way to LDS: R threads for a token, each every R-th piece of its key and value
+    const int rt = tid / T::R, rp = tid % T::R;  // this thread's token and first piece
     u32x4_t kr[NL], vr[NL];
-    int id[T::SETS];     // page of token `lane` (+ 64) of the tile, or -1
-    uint64_t live[T::SETS], next_live[T::SETS];
+    int id, seen_id;           // pages of this thread's token, and of token `lane`
+    bool ok;                   // this thread's token counts
+    uint64_t live, next_live;  // tokens of the tile that count
     auto pages_of = [&](int t0) {
-#pragma unroll
-      for (int s = 0; s < T::SETS; ++s) {
-        const int t = t0 + 64 * s + lane;
-        const int e = trow[a.by_page.quotient(min(t, row.len - 1))];
-        id[s] = t < row.len && 64 * s + lane < TOK && (uint32_t)e < (uint32_t)a.pages ? e : -1;
-      }
+      const int t = t0 + rt, u = t0 + (lane & (TOK - 1));
+      id = trow[a.by_page.quotient(min(t, row.len - 1))];
+      seen_id = trow[a.by_page.quotient(min(u, row.len - 1))];
     };
     auto load = [&](int t0) {  // unconditional loads: of page 0 where a token does not count
-#pragma unroll
-      for (int s = 0; s < T::SETS; ++s) next_live[s] = __ballot(id[s] >= 0);
+      const int t = t0 + rt, u = t0 + (lane & (TOK - 1)), in = t - a.by_page.quotient(t) * a.page;
+      next_live = __ballot(u < row.len && (uint32_t)seen_id < (uint32_t)a.pages);
+      ok = t < row.len && (uint32_t)id < (uint32_t)a.pages;
+      const uint8_t* kp = kh + (ok ? id * a.k_page + in * a.k_token : 0);
+      const uint8_t* vp = vh + (ok ? id * a.v_page + in * a.v_token : 0);
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int at = i * kThreads + tid, t = at / CG, c = at - t * CG;
-        const int pg = __shfl(id[(i * kThreads / CG) >> 6], t & 63);
-        const int p = t0 + t, in = p - a.by_page.quotient(p) * a.page;
-        const bool ok = pg >= 0;
-        const int64_t piece = c * (F8 ? 16 : 8) < a.dim ? 16 * c : 0;
-        kr[i] = *(const u32x4_t*)(kh + (ok ? pg * a.k_page + in * a.k_token : 0) + piece);
-        vr[i] = *(const u32x4_t*)(vh + (ok ? pg * a.v_page + in * a.v_token : 0) + piece);
+        const int c = rp + T::R * i, piece = c * (F8 ? 16 : 8) < a.dim ? 16 * c : 0;
+        kr[i] = *(const u32x4_t*)(kp + piece);
+        vr[i] = *(const u32x4_t*)(vp + piece);
       }
     };
-    auto store = [&](int half) {
+    // Whether a value of the tile is infinite or NaN (asked of tiles that hold nodes).
+    auto store = [&](int half, bool nodes) {
+      bool odd = false;
       uint8_t *ks = lds + half * 2 * T::STORE, *vs = ks + T::STORE;
+      if (__ballot(!ok))  // zeros for values of tokens that do not count: their bits may be NaN, their weight is 0
+#pragma unroll
+        for (int i = 0; i < NL; ++i) vr[i] = ok ? vr[i] : u32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int at = i * kThreads + tid, t = at / CG, c = at - t * CG;
-        // zeros for values of tokens that do not count (their bits may be NaN, their weight is 0) and past the head's dims
-        const bool in = c * (F8 ? 16 : 8) < a.dim, ok = in && (next_live[(i * kThreads / CG) >> 6] >> (t & 63) & 1);
-        const u32x4_t zero = {0, 0, 0, 0}, kv = in ? kr[i] : zero, vv = ok ? vr[i] : zero;
+        const int c = rp + T::R * i;
+        // keys past the head's dims are zeros (the queries are); what values hold there reaches no output
+        const u32x4_t kv = c * (F8 ? 16 : 8) < a.dim ? kr[i] : u32x4_t{0, 0, 0, 0}, vv = vr[i];
         if constexpr (F8) {
+          u32x4_t wide[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t k0 = kv[2 * h], k1 = kv[2 * h + 1], v0 = vv[2 * h], v1 = vv[2 * h + 1];
-            *(u32x4_t*)(ks + T::key_place(t, 2 * c + h)) = u32x4_t{widen<F16, false>(k0), widen<F16, true>(k0), widen<F16, false>(k1), widen<F16, true>(k1)};
-            *(u32x4_t*)(vs + T::value_place(t, c) + 16 * h) = u32x4_t{widen<P16, false>(v0), widen<P16, true>(v0), widen<P16, false>(v1), widen<P16, true>(v1)};
+            *(u32x4_t*)(ks + T::key_place(rt, 2 * c + h)) = u32x4_t{widen<F16, false>(k0), widen<F16, true>(k0), widen<F16, false>(k1), widen<F16, true>(k1)};
+            wide[h] = u32x4_t{widen<P16, false>(v0), widen<P16, true>(v0), widen<P16, false>(v1), widen<P16, true>(v1)};
+            *(u32x4_t*)(vs + T::value_place(rt, c) + 16 * h) = wide[h];
           }
+          if (nodes)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) odd |= odd_word<P16>(wide[k >> 2][k & 3]);
         } else {
-          *(u32x4_t*)(ks + T::key_place(t, c)) = kv;
-          *(u32x4_t*)(vs + T::value_place(t, c >> 1) + 16 * (c & 1)) = vv;
+          *(u32x4_t*)(ks + T::key_place(rt, c)) = kv;
+          *(u32x4_t*)(vs + T::value_place(rt, c >> 1) + 16 * (c & 1)) = vv;
+          if (nodes)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) odd |= odd_word<P16>(vv[k]);
         }
       }
-#pragma unroll
-      for (int s = 0; s < T::SETS; ++s) live[s] = next_live[s];
+      live = next_live;
+      return odd;
     };
 
     const int base = first * TOK, stop = (first + count) * TOK;
+    // A value that is infinite or NaN counts for the columns that see its token only, but 0 times it would reach all: where
+    // a tile with nodes holds one (odd), the products take 0 for it, and it is added to its columns by hand.
+    bool odd = false;
+    auto join_waves = [&](int half, bool nodes, bool any) {
+      // words of this half are read before the next barrier, and written again only after it
+      if (nodes && lane == 0) flag[4 * half + wave] = 0;
+      if (nodes && any) flag[4 * half + wave] = 1;
+      __syncthreads();
+      odd = nodes && __builtin_amdgcn_readfirstlane(flag[4 * half] | flag[4 * half + 1] | flag[4 * half + 2] | flag[4 * half + 3]);
+    };
     if (count > 0) {  // a row without tokens has no tile
       pages_of(base);
       load(base);
       __syncthreads();  // the run before may still be read
-      store(0);
+      const bool nodes = base + TOK > row.context, any = store(0, nodes);
       if (count > 1) {
         pages_of(base + TOK);
         load(base + TOK);
       }
-      __syncthreads();
+      join_waves(0, nodes, any);
     }
     int half = 0;
     for (int t0 = base; t0 < stop; t0 += TOK) {
       const bool further = t0 + 2 * TOK < stop;
       if (further) pages_of(t0 + 2 * TOK);
-      const uint8_t *ks = lds + half * 2 * T::STORE, *vs = ks + T::STORE;
-      const int mine = wt * T::TPW;  // this wavefront's tokens of the tile
-      f32x4_t s[NT][CW];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int j = 0; j < CW; ++j) s[i][j] = f32x4_t{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const u32x4_t kf = *(const u32x4_t*)(ks + T::key_place(mine + 16 * i + col, 4 * k + g));
-#pragma unroll
-          for (int j = 0; j < CW; ++j) s[i][j] = mfma16<F16>(kf, q[j][k], s[i][j]);
-        }
-      }
-      uint64_t valid = (T::SETS > 1 && mine >= 64 ? live[T::SETS - 1] : live[0]) >> (mine & 63);
-      if constexpr (T::TPW < 64) valid &= (1ull << T::TPW) - 1;
-      constexpr uint64_t ALL = T::TPW < 64 ? (1ull << T::TPW) - 1 : ~0ull;
+      uint8_t *ks = lds + half * 2 * T::STORE, *vs = ks + T::STORE;
+      constexpr uint64_t ALL = TOK < 64 ? (1ull << TOK) - 1 : ~0ull;
+      const uint64_t valid = live & ALL;
       const bool plain = t0 + TOK <= row.context && valid == ALL;
-      // A value that is infinite or NaN counts for the columns that see its token only, but 0 times it would reach all: where
-      // a tile that is not seen by all holds one, the products take 0 for it, and it is added to its columns by hand.
-      bool odd = false;
-      if (!plain) {
+      if (odd) {
+        if (!idle)
+#pragma unroll
+          for (int j = 0; j < CW; ++j) {
+            const uint64_t bits = sees[j].bits(a, row.start + node[j], node[j], t0 - row.context) & valid;
 #pragma unroll 1
-        for (int i = lane; i < T::TPW * T::CH; i += 64) {
-          const u32x4_t w = *(const u32x4_t*)(vs + mine * DT * 2 + 16 * i);
+            for (int t = 0; t < TOK; ++t)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) odd |= odd_half<P16>(w[k]) || odd_half<P16>(w[k] >> 16);
-        }
-        odd = __ballot(odd) != 0;
+              for (int d = 0; d < ND; ++d) {
+                const u32x2_t v = *(const u32x2_t*)(vs + T::value_place(t, d) + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t h = v[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+                  if (odd_half<P16>(h) && (bits >> t & 1)) o[d][j][e] += unpack<P16>(h, 0);
+                }
+              }
+          }
+        __syncthreads();
+#pragma unroll 1
+        for (int i = tid; i < T::STORE / 4; i += kThreads) ((uint32_t*)vs)[i] = clean2<P16>(((uint32_t*)vs)[i]);
+        __syncthreads();
       }
-      u32x4_t p[KT][CW][PARTS];
+      if (!idle) {
+        u32x4_t p[KT][CW][PARTS];
+        f32x4_t s[NT][CW];
 #pragma unroll
-      for (int j = 0; j < CW; ++j) {
-        float v[NT][4], top = -INFINITY;
+        for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
+          for (int i = 0; i < NT; ++i) {
+            const u32x4_t kf = *(const u32x4_t*)(ks + T::key_place(16 * i + col, 4 * k + g));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[i][e] = s[i][j][e] * sc;
-        if (!plain) {
-          const uint64_t bits = (seen(a, row.start + node[j], node[j], t0 + mine - row.context) & valid) >> (4 * g);
-          counts[j] |= bits != 0;
+            for (int j = 0; j < CW; ++j) s[i][j] = mfma16<F16>(kf, q[j][k], k ? s[i][j] : f32x4_t{0, 0, 0, 0});
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < CW; ++j) {
+          if (!plain) {
+            const uint64_t bits = (sees[j].bits(a, row.start + node[j], node[j], t0 - row.context) & valid) >> (4 * g);
+            const uint32_t word[2] = {(uint32_t)bits, (uint32_t)(bits >> 32)};
+            counts[j] |= bits != 0;
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[i][j][e] = word[i >> 1] & (1u << (16 * (i & 1) + e)) ? s[i][j][e] : -INFINITY;
+          } else {
+            counts[j] = true;
+          }
+          float top = -INFINITY;
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = bits >> (16 * i + e) & 1 ? v[i][e] : -INFINITY;
-        } else {
-          counts[j] = true;
-        }
+            for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][j][e]);
+          top = fmaxf(top, __shfl_xor(top, 16));
+          top = fmaxf(top, __shfl_xor(top, 32)) * sc;
+          if (__ballot(top > m[j] + T::SLACK)) {
+            const float m_new = top > m[j] + T::SLACK ? top : m[j];
+            // never 0: an infinite sum stays infinite
+            const float alpha = m_new == m[j] ? 1.f : fmaxf(__builtin_amdgcn_exp2f(m[j] - m_new), FLT_MIN);
+            m[j] = m_new;
+            l[j] *= alpha;
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, v[i][e]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float m_new = fmaxf(m[j], top);
-        const float ref = m_new == -INFINITY ? 0.f : m_new;  // nothing but -inf so far: p = 0, not NaN
-        if (__ballot(m_new != m[j])) {
-          const float alpha = __builtin_amdgcn_exp2f(m[j] - ref);
-          m[j] = m_new;
-          l[j] *= alpha;
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[d][j] *= alpha;
-        }
-        const float off = T::SHIFT - ref;
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float p0 = __builtin_amdgcn_exp2f(v[i][2 * h] + off), p1 = __builtin_amdgcn_exp2f(v[i][2 * h + 1] + off);
-            sum += p0 + p1;
-            uint32_t out[PARTS];
-            split_parts<P16, PARTS>(p0, p1, out);
-#pragma unroll
-            for (int n = 0; n < PARTS; ++n) p[i >> 1][j][n][2 * (i & 1) + h] = out[n];
+            for (int d = 0; d < ND; ++d) o[d][j] *= alpha;
           }
-        l[j] += sum;
-      }
+          const float off = T::SHIFT - (m[j] == -INFINITY ? 0.f : m[j]);  // nothing but -inf so far: weights 0, not NaN
+          float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < KT; ++k)
+          for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          typedef __attribute__((ext_vector_type(4))) short s16x4_t;
-          typedef __attribute__((address_space(3))) s16x4_t* lds_p;
-          u32x2_t v[2];
+            for (int h = 0; h < 2; ++h) {
+              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][2 * h], sc, off));
+              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][2 * h + 1], sc, off));
+              sum += p0 + p1;
+              uint32_t out[PARTS];
+              split_parts<P16, PARTS>(p0, p1, out);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            // rows 4 g .. 4 g + 3 of 16 tokens, eight bytes a lane; the read gives each lane its dim of the four
-            const int t = mine + 32 * k + 16 * h + 4 * g + (col >> 2);
-            v[h] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                   (lds_p)(vs + T::value_place(t, d) + 8 * (col & 3))));
-          }
-          u32x4_t vf = {v[0][0], v[0][1], v[1][0], v[1][1]};
-          if (odd)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) vf[n] = clean2<P16>(vf[n]);
-#pragma unroll
-          for (int j = 0; j < CW; ++j)
-#pragma unroll
-            for (int n = PARTS - 1; n >= 0; --n) o[d][j] = mfma16<P16>(vf, p[k][j][n], o[d][j]);
-        }
-      if (odd) {
-#pragma unroll
-        for (int j = 0; j < CW; ++j) {
-          const uint64_t bits = seen(a, row.start + node[j], node[j], t0 + mine - row.context) & valid;
-#pragma unroll 1
-          for (int t = 0; t < T::TPW; ++t)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-              const u32x2_t v = *(const u32x2_t*)(vs + T::value_place(mine + t, d) + 8 * g);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t h = v[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-                if (odd_half<P16>(h) && (bits >> t & 1)) o[d][j][e] += unpack<P16>(h, 0);
-              }
+              for (int n = 0; n < PARTS; ++n) p[i >> 1][j][n][2 * (i & 1) + h] = out[n];
             }
+          l[j] += sum;
+        }
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+            typedef __attribute__((address_space(3))) s16x4_t* lds_p;
+            u32x4_t vf;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              // rows 4 g .. 4 g + 3 of 16 tokens, eight bytes a lane; the read gives each lane its dim of the four
+              const int t = 32 * k + 16 * h + 4 * g + (col >> 2);
+              const u32x2_t v = __builtin_bit_cast(
+                  u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(vs + T::value_place(t, d) + 8 * (col & 3))));
+              vf[2 * h] = v[0], vf[2 * h + 1] = v[1];
+            }
+#pragma unroll
+            for (int j = 0; j < CW; ++j)
+#pragma unroll
+              for (int n = PARTS - 1; n >= 0; --n) o[d][j] = mfma16<P16>(vf, p[k][j][n], o[d][j]);
+          }
         }
       }
       if (t0 + TOK < stop) {
         half ^= 1;
-        store(half);
+        const bool nodes = t0 + 2 * TOK > row.context, any = store(half, nodes);
         if (further) load(t0 + 2 * TOK);
-        __syncthreads();
+        join_waves(half, nodes, any);
       }
     }
 #pragma unroll
@@ -464,60 +511,25 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void tree_kernel(Args 
       l[j] += __shfl_xor(l[j], 16);
       l[j] += __shfl_xor(l[j], 32);
     }
-    // ---- wavefronts of the same columns
-    if constexpr (WT > 1) {
-      __syncthreads();
-#pragma unroll
-      for (int step = WT / 2; step; step /= 2) {
-        float* at = (float*)lds + (wq * (WT / 2) + (wt < step ? wt : wt - step)) * (T::PARK / 4) + lane;
-        if (wt >= step && wt < 2 * step) {
-#pragma unroll
-          for (int j = 0; j < CW; ++j) {
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) at[((j * ND + d) * 4 + e) * 64] = o[d][j][e];
-            at[(4 * ND * CW + 2 * j) * 64] = m[j];
-            at[(4 * ND * CW + 2 * j + 1) * 64] = l[j];
-          }
-        }
-        __syncthreads();
-        if (wt < step) {
-#pragma unroll
-          for (int j = 0; j < CW; ++j) {
-            const float m2 = at[(4 * ND * CW + 2 * j) * 64], l2 = at[(4 * ND * CW + 2 * j + 1) * 64];
-            const float mx = fmaxf(m[j], m2), ref = mx == -INFINITY ? 0.f : mx;
-            const float f = __builtin_amdgcn_exp2f(m[j] - ref), f2 = __builtin_amdgcn_exp2f(m2 - ref);
-            m[j] = mx;
-            l[j] = l[j] * f + l2 * f2;
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[d][j][e] = o[d][j][e] * f + at[((j * ND + d) * 4 + e) * 64] * f2;
-          }
-        }
-        __syncthreads();
-      }
-    }
     // ---- outputs, or this run's part of them
     const bool whole = first == 0 && count == row.tiles;
-    if (wt == 0) {
-      float* sums = whole ? nullptr : a.ws + ((int64_t)w * 2 + slot) * partial_floats(T::QB, a.dim);
+    {
+      float* part_sums = whole ? nullptr : a.ws + ((int64_t)w * 2 + slot) * partial_floats(T::QB, a.dim);
 #pragma unroll
       for (int j = 0; j < CW; ++j) {
-        if (!has[j]) continue;
-        const int c = (wq * CW + j) * 16 + col;
-        if (sums) {
+        const int column = first_column + 16 * j, c = (wave * CW + j) * 16 + col;
+        if (column >= columns) continue;
+        if (part_sums) {
 #pragma unroll
           for (int d = 0; d < ND; ++d)
-            if (16 * d + 4 * g < a.dim) *(f32x4_t*)(sums + (int64_t)c * a.dim + 16 * d + 4 * g) = o[d][j] * T::UNSHIFT;
+            if (16 * d + 4 * g < a.dim) *(f32x4_t*)(part_sums + (int64_t)c * a.dim + 16 * d + 4 * g) = o[d][j] * T::UNSHIFT;
           if (g == 0) {
-            float* st = sums + (int64_t)T::QB * a.dim + 2 * c;
+            float* st = part_sums + (int64_t)T::QB * a.dim + 2 * c;
             st[0] = m[j];
             st[1] = l[j] * T::UNSHIFT;
           }
         } else {
-          const int64_t at = (int64_t)(row.start + node[j]) * a.heads + head[j];
+          const int64_t at = (int64_t)(row.start + node[j]) * a.heads + kvh * a.group + (column - node[j] * a.group);
           const float f = m[j] == -INFINITY ? 0.f : l[j] == 0.f ? NAN : (a.v_scale ? a.v_scale[kvh] : 1.f) / l[j];
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
@@ -530,7 +542,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void tree_kernel(Args 
     }
     slot = 1;
     if (!cut) return;
-    pos += count;
+    pos += places;
     if (pos >= pre[r + 1]) ++r;
   }
 }
@@ -541,31 +553,23 @@ struct TreeKern {
   std::atomic<int>* residents;  // workgroups of a CU, by device; 0: not asked yet
 };
 
-// The kernel for head_dim and about `columns` columns of a row; three: P in three parts where its type is bf16.
-TreeKern kern_bf16(int dim, int columns, bool three);
-TreeKern kern_f16(int dim, int columns, bool three);
-TreeKern kern_bf16_e4m3(int dim, int columns, bool three);
-TreeKern kern_f16_e4m3(int dim, int columns, bool three);
+// The kernel for head_dim, about `columns` columns of a row and the type of the output.
+TreeKern kern_bf16(int dim, int columns, int out_dtype);
+TreeKern kern_f16(int dim, int columns, int out_dtype);
+TreeKern kern_bf16_e4m3(int dim, int columns, int out_dtype);
+TreeKern kern_f16_e4m3(int dim, int columns, int out_dtype);
 
-template <bool F16, bool F8, int DT, int WQ, int WT, int CW, int PARTS>
+template <bool F16, bool F8, int DT, int CW, int TOK, int OCC, int PARTS>
 TreeKern kern_t() {
-  using T = Kern<F16, F8, DT, WQ, WT, CW, PARTS>;
+  using T = Kern<F16, F8, DT, CW, TOK, OCC, PARTS>;
   static std::atomic<int> residents[64];
-  return TreeKern{(const void*)tree_kernel<F16, F8, DT, WQ, WT, CW, PARTS>, T::QB, T::TOK, T::LDS, residents};
+  return TreeKern{(const void*)tree_kernel<F16, F8, DT, CW, TOK, OCC, PARTS>, T::QB, TOK, T::LDS, residents};
 }
 template <bool F16, bool F8, int PARTS>
 TreeKern kern_of(int dim, int columns) {
-  if (dim > 128) return columns > 32 ? kern_t<F16, F8, 256, 4, 1, 1, PARTS>() : kern_t<F16, F8, 256, 2, 2, 1, PARTS>();
-  if (dim > 64) {
-    if (columns > 64) return kern_t<F16, F8, 128, 4, 1, 2, PARTS>();
-    if (columns > 32) return kern_t<F16, F8, 128, 2, 2, 2, PARTS>();
-    if (columns > 16) return kern_t<F16, F8, 128, 1, 4, 2, PARTS>();
-    return kern_t<F16, F8, 128, 1, 4, 1, PARTS>();
-  }
-  if (columns > 64) return kern_t<F16, F8, 64, 4, 1, 2, PARTS>();
-  if (columns > 32) return kern_t<F16, F8, 64, 2, 2, 2, PARTS>();
-  if (columns > 16) return kern_t<F16, F8, 64, 1, 4, 2, PARTS>();
-  return kern_t<F16, F8, 64, 1, 4, 1, PARTS>();
+  if (dim > 128) return kern_t<F16, F8, 256, 1, 32, 2, PARTS>();
+  if (dim > 64) return columns > 64 ? kern_t<F16, F8, 128, 2, 64, 2, PARTS>() : kern_t<F16, F8, 128, 1, 32, 4, PARTS>();
+  return columns > 64 ? kern_t<F16, F8, 64, 2, 64, 2, PARTS>() : kern_t<F16, F8, 64, 1, 64, 4, PARTS>();
 }
 
 }  // namespace tree

@@ -32,8 +32,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
   if (row.tiles) {
     const int64_t c = (int64_t)node * a.group + (h - kvh * a.group);
     const int block = (int)(c / a.qb), i = (int)(c - (int64_t)block * a.qb);
-    const int64_t per = a.prefix[a.rows + 1], s = a.prefix[lo] + ((int64_t)kvh * row.blocks + block) * row.tiles;
-    const int64_t w0 = s / per, w1 = (s + row.tiles - 1) / per;
+    const int64_t per = a.prefix[a.rows + 1], s = a.prefix[lo] + ((int64_t)kvh * row.blocks + block) * (row.tiles + kStart);
+    const int64_t w0 = (s + kStart) / per, w1 = (s + kStart + row.tiles - 1) / per;
     if (w0 == w1) return;
     constexpr int N = 4;  // pieces on their way at once
     for (int64_t w = w0; w <= w1; w += N) {
@@ -113,10 +113,10 @@ __global__ __launch_bounds__(kThreads) void mask_kernel(MaskArgs a) {
   }
 }
 
-TreeKern kern(const mlxr_paged_cache* c, int q_dtype, int columns, bool three) {
+TreeKern kern(const mlxr_paged_cache* c, int q_dtype, int columns, int out_dtype) {
   const bool f16 = q_dtype == MLXR_F16;
-  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, columns, three) : kern_bf16_e4m3(c->head_dim, columns, three);
-  return f16 ? kern_f16(c->head_dim, columns, three) : kern_bf16(c->head_dim, columns, three);
+  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, columns, out_dtype) : kern_bf16_e4m3(c->head_dim, columns, out_dtype);
+  return f16 ? kern_f16(c->head_dim, columns, out_dtype) : kern_bf16(c->head_dim, columns, out_dtype);
 }
 
 constexpr int kMaxHeads = 1 << 26;  // tokens times heads: a launch has fewer than 2^32 threads
@@ -134,7 +134,7 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   Plan p;
   const int group = heads / c->kv_heads;
   const int64_t columns = ((int64_t)tokens * group + rows - 1) / rows;
-  p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), out_dtype == MLXR_F32);
+  p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), out_dtype);
   p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
   const int64_t held = (int64_t)width * c->page_size, tiles = (held + p.k.tok - 1) / p.k.tok;
   p.cut = tiles > 4 && p.units < 8 * device_cu_count();
@@ -222,8 +222,8 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   a.by_page = Divisor(a.page), a.by_group = Divisor(a.group);
   a.scale = scale * 1.44269504088896341f;
   const hipStream_t st = (hipStream_t)stream;
-  // LDS: two tiles, the rows' prefix and four sums; the limit is raised to all that a workgroup may use, once on each device
-  const int lds = p.k.lds + (rows + 1 + 4) * (int)sizeof(int64_t), most = (int)device_lds_limit();
+  // LDS: two tiles, the rows' prefix, four sums and eight words; the limit is raised to all that a workgroup may use, once on each device
+  const int lds = p.k.lds + (rows + 1 + 8) * (int)sizeof(int64_t), most = (int)device_lds_limit();
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention: %s", hipGetErrorString(e));

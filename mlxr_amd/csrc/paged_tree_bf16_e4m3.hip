@@ -3,6 +3,8 @@
 
 namespace mlxr {
 namespace tree {
-TreeKern kern_bf16_e4m3(int dim, int columns, bool) { return kern_of<false, true, 2>(dim, columns); }
+TreeKern kern_bf16_e4m3(int dim, int columns, int out_dtype) {
+  return out_dtype == MLXR_BF16 ? kern_of<false, true, 1>(dim, columns) : kern_of<false, true, 2>(dim, columns);
+}
 }  // namespace tree
 }  // namespace mlxr

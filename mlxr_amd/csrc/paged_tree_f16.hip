@@ -3,6 +3,8 @@
 
 namespace mlxr {
 namespace tree {
-TreeKern kern_f16(int dim, int columns, bool) { return kern_of<true, false, 2>(dim, columns); }
+TreeKern kern_f16(int dim, int columns, int) {
+  return kern_of<true, false, 2>(dim, columns);
+}
 }  // namespace tree
 }  // namespace mlxr

@@ -3,6 +3,8 @@
 
 namespace mlxr {
 namespace tree {
-TreeKern kern_f16_e4m3(int dim, int columns, bool) { return kern_of<true, true, 2>(dim, columns); }
+TreeKern kern_f16_e4m3(int dim, int columns, int out_dtype) {
+  return out_dtype == MLXR_BF16 ? kern_of<true, true, 1>(dim, columns) : kern_of<true, true, 2>(dim, columns);
+}
 }  // namespace tree
 }  // namespace mlxr

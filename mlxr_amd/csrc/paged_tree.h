@@ -55,6 +55,7 @@ struct Args {
   int64_t* prefix;  // [rows + 1] tiles before each row, then tiles of a workgroup, for the join
   int rows, tokens, heads, kv_heads, group;
   int dim, page, pages, width, out_dtype, qb, tok;
+  int step;  // pages of a tile where they are whole, else 0
   Divisor by_page, by_group;
   int workers;
   float scale;  // times log2(e)
@@ -80,6 +81,11 @@ __device__ __forceinline__ Row row_of(const Args& a, int r) {
 
 // Floats of a cut run's partial sums: QB rows of dim, then m and sum of each.
 __host__ __device__ constexpr int partial_floats(int qb, int dim) { return qb * dim + 2 * qb; }
+
+// n / d, d > 0; most calls stay within 32 bits, whose division takes a tenth of the instructions.
+__device__ __forceinline__ int quotient(int64_t n, int64_t d) {
+  return n < (1ll << 31) && d < (1ll << 31) ? (int)((uint32_t)n / (uint32_t)d) : (int)(n / d);
+}
 
 // What a node sees of its row's nodes: 64 bits from bit `at` on, 1s before the nodes (at < 0).  The first two words stay in
 // registers; no mask: bits 0 .. i.
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
       continue;
     }
     const int64_t in_row = pos - pre[r];
-    const int span = row.tiles + kStart, unit = (int)(cut ? in_row / span : in_row), from = (int)(in_row - (int64_t)unit * span);
+    const int span = row.tiles + kStart, unit = cut ? quotient(in_row, span) : (int)in_row, from = (int)(in_row - (int64_t)unit * span);
     const int places = cut ? (int)min((int64_t)(span - from), end - pos) : 0;  // of this run
     const int first = cut ? max(from - kStart, 0) : 0, count = cut ? max(from + places - kStart, 0) - first : row.tiles;
     if (cut && count == 0) {  // the run ends within a unit's first places
@@ -311,17 +317,33 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
     int id, seen_id;           // pages of this thread's token, and of token `lane`
     bool ok;                   // this thread's token counts
     uint64_t live, next_live;  // tokens of the tile that count
+    // Where a tile is whole pages, a thread's place in its page is the same in every tile, and its page index goes on by
+    // as many.
+    const int lane_t = lane & (TOK - 1), own_page = a.by_page.quotient(rt), lane_page = a.by_page.quotient(lane_t), last_page = a.by_page.quotient(max(row.len - 1, 0));
+    const int own_in = rt - own_page * a.page;
+    const int64_t k_in = own_in * a.k_token, v_in = own_in * a.v_token;
     auto pages_of = [&](int t0) {
-      const int t = t0 + rt, u = t0 + (lane & (TOK - 1));
-      id = trow[a.by_page.quotient(min(t, row.len - 1))];
-      seen_id = trow[a.by_page.quotient(min(u, row.len - 1))];
+      if (a.step) {
+        const int before = t0 / TOK * a.step;
+        id = trow[min(before + own_page, last_page)];
+        seen_id = trow[min(before + lane_page, last_page)];
+      } else {
+        id = trow[a.by_page.quotient(min(t0 + rt, row.len - 1))];
+        seen_id = trow[a.by_page.quotient(min(t0 + lane_t, row.len - 1))];
+      }
     };
     auto load = [&](int t0) {  // unconditional loads: of page 0 where a token does not count
-      const int t = t0 + rt, u = t0 + (lane & (TOK - 1)), in = t - a.by_page.quotient(t) * a.page;
-      next_live = __ballot(u < row.len && (uint32_t)seen_id < (uint32_t)a.pages);
+      const int t = t0 + rt;
+      next_live = __ballot(t0 + lane_t < row.len && (uint32_t)seen_id < (uint32_t)a.pages);
       ok = t < row.len && (uint32_t)id < (uint32_t)a.pages;
-      const uint8_t* kp = kh + (ok ? id * a.k_page + in * a.k_token : 0);
-      const uint8_t* vp = vh + (ok ? id * a.v_page + in * a.v_token : 0);
+      const int64_t pg = ok ? id : 0;
+      const uint8_t *kp = kh + pg * a.k_page, *vp = vh + pg * a.v_page;
+      if (a.step) {
+        kp += k_in, vp += v_in;
+      } else {
+        const int in = ok ? t - a.by_page.quotient(t) * a.page : 0;
+        kp += in * a.k_token, vp += in * a.v_token;
+      }
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int c = rp + T::R * i, piece = c * (F8 ? 16 : 8) < a.dim ? 16 * c : 0;
@@ -336,11 +358,13 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
       if (__ballot(!ok))  // zeros for values of tokens that do not count: their bits may be NaN, their weight is 0
 #pragma unroll
         for (int i = 0; i < NL; ++i) vr[i] = ok ? vr[i] : u32x4_t{0, 0, 0, 0};
+      if (a.dim < DT)  // keys past the head's dims are zeros (the queries are); what values hold there reaches no output
+#pragma unroll
+        for (int i = 0; i < NL; ++i) kr[i] = (rp + T::R * i) * (F8 ? 16 : 8) < a.dim ? kr[i] : u32x4_t{0, 0, 0, 0};
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int c = rp + T::R * i;
-        // keys past the head's dims are zeros (the queries are); what values hold there reaches no output
-        const u32x4_t kv = c * (F8 ? 16 : 8) < a.dim ? kr[i] : u32x4_t{0, 0, 0, 0}, vv = vr[i];
+        const u32x4_t kv = kr[i], vv = vr[i];
         if constexpr (F8) {
           u32x4_t wide[2];
 #pragma unroll
@@ -568,7 +592,7 @@ TreeKern kern_t() {
 template <bool F16, bool F8, int PARTS>
 TreeKern kern_of(int dim, int columns) {
   if (dim > 128) return kern_t<F16, F8, 256, 1, 32, 2, PARTS>();
-  if (dim > 64) return columns > 64 ? kern_t<F16, F8, 128, 2, 64, 2, PARTS>() : kern_t<F16, F8, 128, 1, 32, 4, PARTS>();
+  if (dim > 64) return columns > 64 ? kern_t<F16, F8, 128, 2, 64, 2, PARTS>() : kern_t<F16, F8, 128, 1, 64, 2, PARTS>();
   return columns > 64 ? kern_t<F16, F8, 64, 2, 64, 2, PARTS>() : kern_t<F16, F8, 64, 1, 64, 4, PARTS>();
 }
 

@@ -12,15 +12,19 @@ namespace {
 // workgroups w that had a piece of its columns, M the maximum of their m (-inf: no token counted).  Rows without
 // tokens get zeros; columns that one workgroup covered are done.
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
+  extern __shared__ int starts[];  // [rows + 1]: searched in LDS
   const int tid = threadIdx.x, x = tid & (lanes - 1);
-  const int64_t at = (int64_t)blockIdx.x * (kThreads / lanes) + tid / lanes;  // token * heads + head
+  for (int r = tid; r <= a.rows; r += kThreads) starts[r] = a.starts[r];
+  const int64_t per = a.prefix[a.rows + 1];
+  __syncthreads();
+  const int64_t at = (int64_t)blockIdx.x * (kThreads / lanes) + tid / lanes;  // token * heads + head, below 2^27
   if (at >= (int64_t)a.tokens * a.heads) return;
-  const int token = (int)(at / a.heads), h = (int)(at - (int64_t)token * a.heads);
-  if (token >= a.starts[a.rows]) return;
+  const int token = (int)at / a.heads, h = (int)at - token * a.heads;
+  if (token >= starts[a.rows]) return;
   int lo = 0, hi = a.rows;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (a.starts[mid] <= token) lo = mid;
+    if (starts[mid] <= token) lo = mid;
     else hi = mid;
   }
   const Row row = row_of(a, lo);
@@ -30,13 +34,12 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
   float o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.f;
   const int kvh = a.by_group.quotient(h);
   if (row.tiles) {
-    const int64_t c = (int64_t)node * a.group + (h - kvh * a.group);
-    const int block = (int)(c / a.qb), i = (int)(c - (int64_t)block * a.qb);
-    const int64_t per = a.prefix[a.rows + 1], s = a.prefix[lo] + ((int64_t)kvh * row.blocks + block) * (row.tiles + kStart);
-    const int64_t w0 = (s + kStart) / per, w1 = (s + kStart + row.tiles - 1) / per;
+    const int c = node * a.group + (h - kvh * a.group), block = c / a.qb, i = c - block * a.qb;  // below 2^27
+    const int64_t s = a.prefix[lo] + ((int64_t)kvh * row.blocks + block) * (row.tiles + kStart);
+    const int w0 = quotient(s + kStart, per), w1 = quotient(s + kStart + row.tiles - 1, per);
     if (w0 == w1) return;
     constexpr int N = 4;  // pieces on their way at once
-    for (int64_t w = w0; w <= w1; w += N) {
+    for (int w = w0; w <= w1; w += N) {
       float pm[N], pl[N];
       f32x4_t po[N];
 #pragma unroll
@@ -218,7 +221,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   a.out = out_dev, a.lse = lse_dev, a.out_dtype = out_dtype;
   a.rows = rows, a.tokens = tokens, a.heads = heads, a.kv_heads = cache->kv_heads, a.group = heads / cache->kv_heads;
   a.dim = cache->head_dim, a.page = cache->page_size, a.pages = cache->num_pages, a.width = table_width;
-  a.qb = p.k.qb, a.tok = p.k.tok;
+  a.qb = p.k.qb, a.tok = p.k.tok, a.step = p.k.tok % a.page == 0 ? p.k.tok / a.page : 0;
   a.by_page = Divisor(a.page), a.by_group = Divisor(a.group);
   a.scale = scale * 1.44269504088896341f;
   const hipStream_t st = (hipStream_t)stream;
@@ -248,7 +251,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
     int lanes = 2;
     while (4 * lanes < a.dim) lanes *= 2;
     const int64_t of = kThreads / lanes;
-    join_kernel<<<(unsigned)(((int64_t)tokens * heads + of - 1) / of), kThreads, 0, st>>>(a, lanes);
+    join_kernel<<<(unsigned)(((int64_t)tokens * heads + of - 1) / of), kThreads, (rows + 1) * sizeof(int), st>>>(a, lanes);
     e = hipGetLastError();
   }
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention launch: %s", hipGetErrorString(e));

@@ -50,7 +50,7 @@ int mlxr_quantize_fp8_weight(int N, int K, const void* w_dev, int w_dtype, void*
  *   x_scale_dev    [M, ceil(K / 128)], w_scale_dev [ceil(N / 128), ceil(K / 128)] fp32, contiguous
  *   bias_dev       [N] of bias_dtype (MLXR_F32 / MLXR_F16 / MLXR_BF16) or NULL
  *   y_dev          [M, N] contiguous, of y_dtype
- * Sums are fp32 and y is rounded once.  For 16-bit y and many rows the matrix instruction of 8 bits is used, which adds
+ * Sums are fp32 and y is rounded once.  For 16-bit y and more than 16 rows the matrix instruction of 8 bits may be used, which adds
  * eight neighbouring products (k / 8) at a time and drops what each has below 2^-13 of the largest of them; else
  * products and sums within a block are fp32 too.  M and N up to 2^26, K up to 2^22,
  * M * N up to 2^37. */
@@ -58,6 +58,9 @@ int mlxr_fp8_matmul_workspace_size(int M, int N, int K, int y_dtype, size_t* byt
 int mlxr_fp8_matmul(int M, int N, int K, const void* x_dev, const float* x_scale_dev, const void* w_dev,
                     const float* w_scale_dev, const void* bias_dev, int bias_dtype, void* y_dev, int y_dtype,
                     void* workspace_dev, size_t workspace_bytes, void* stream);
+/* Test hook, process-wide: kernel (0: by shape; 1, 2: of few rows; 3 .. 7: tiles, ascending) and splits of K over workgroups of
+ * every later mlxr_fp8_matmul and its workspace size. */
+int mlxr_fp8_test_force(int kind, int splits);
 
 #ifdef __cplusplus
 }

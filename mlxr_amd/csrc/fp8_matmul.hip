@@ -11,12 +11,13 @@
 // of them (measured; the sums of eight are then added in fp32): of random values 1.5e-5 of the result, a hundredth of half a
 // step of bf16 and a sixteenth of f16's.  That is taken for 16-bit outputs of many rows, where the instruction bounds the
 // kernel.  WIDE: both operands to bf16, which holds them exactly, and four 16 x 16 x 32 instructions, twice the clocks,
-// whose sums keep fp32 (1e-7): fp32 outputs, and calls that memory bounds.
+// whose sums keep fp32 (1e-7): fp32 outputs, and the kernels of few rows, which memory bounds.
 //
 // Both operands lie in memory as rows of K bytes, 128 of them (a line) a block.  They go to LDS by DMA, whole lines at a time,
 // with the 16-byte piece c of row r at place c ^ (r / 2 % 8), so that the 16 rows of an operand's read lie in different banks;
 // rows and pieces past the ends arrive as zeros.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "../../include/mlxr_fp8.h"
@@ -54,11 +55,13 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 template <bool WIDE>
 struct Operand {
   i32x8_t v;
+  Operand() = default;
   __device__ __forceinline__ explicit Operand(const i32x8_t& raw) : v(raw) {}
 };
 template <>
 struct Operand<true> {
   bf16x8_t v[4];
+  Operand() = default;
   __device__ __forceinline__ explicit Operand(const i32x8_t& raw) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -96,6 +99,10 @@ __device__ __forceinline__ void dma(i32x4_t rsrc, uint32_t voff, uint32_t soff, 
     asm volatile("s_mov_b32 m0, %3\n\tbuffer_load_dword %0, %1, %2 offen lds" : : "v"(voff), "s"(rsrc), "s"(soff), "s"(m0v) : "memory", "m0");
 #pragma clang diagnostic pop
 }
+
+// w's scales through the scalar cache: a vector load would be waited for together with the DMA behind it.
+typedef const __attribute__((address_space(4))) float* scalar_p;
+__device__ __forceinline__ scalar_p scalar_pointer(const float* p) { return (scalar_p)(uintptr_t)p; }
 
 __device__ __forceinline__ int place(int r, int c) { return r * 128 + ((c ^ (r >> 1)) & 7) * 16; }
 
@@ -208,7 +215,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(Args a) {
   // the block of w's scales that this wavefront's columns lie in
   static_assert(kK % (BN / WN) == 0, "a wavefront's columns lie in one block of 128");
   const int nb = __builtin_amdgcn_readfirstlane(min((n0 + wn * (BN / WN)) / kK, (a.N - 1) / kK));
-  const float* ws = a.ws + (int64_t)nb * a.blocks;
+  const scalar_p ws = scalar_pointer(a.ws + (int64_t)nb * a.blocks);
   int stage = 0;
   for (int b = b0; b < b1; ++b) {
     vm_wait<(STAGES - 2) * T::DMAS>();
@@ -221,20 +228,28 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(Args a) {
     float f[TM];
 #pragma unroll
     for (int j = 0; j < TM; ++j) f[j] = ts[(wm * TM + j) * 16 + (lane & 15)] * wsc;
-    auto rows_of_w = [&](int i, const Operand<WIDE>(&fx)[TM]) {
-      const Operand<WIDE> fw(operand(tw, (wn * TN + i) * 16, lane));
+    Operand<WIDE> fx[TM], fw[2];
+    f32x4_t p[2][TM];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) fx[j] = Operand<WIDE>(operand(tx, (wm * TM + j) * 16, lane));
+    fw[0] = Operand<WIDE>(operand(tw, wn * TN * 16, lane));
+    // While the matrix unit works on 16 rows of w, the vector unit adds up the 16 before them and the next are read.
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+      if (i + 1 < TN) fw[(i + 1) & 1] = Operand<WIDE>(operand(tw, (wn * TN + i + 1) * 16, lane));
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        const f32x4_t p = mfma128(fw, fx[j]);
+        p[i & 1][j] = mfma128(fw[i & 1], fx[j]);
+        if (i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(p[e], f[j], acc[i][j][e]);
+          for (int e = 0; e < 4; ++e) acc[i - 1][j][e] = __builtin_fmaf(p[(i - 1) & 1][j][e], f[j], acc[i - 1][j][e]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    };
-    static_assert(TM == 4, "operands of x listed below");
-    const Operand<WIDE> fx[TM] = {Operand<WIDE>(operand(tx, wm * TM * 16, lane)), Operand<WIDE>(operand(tx, wm * TM * 16 + 16, lane)),
-                                  Operand<WIDE>(operand(tx, wm * TM * 16 + 32, lane)), Operand<WIDE>(operand(tx, wm * TM * 16 + 48, lane))};
+    }
 #pragma unroll
-    for (int i = 0; i < TN; ++i) rows_of_w(i, fx);
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[TN - 1][j][e] = __builtin_fmaf(p[(TN - 1) & 1][j][e], f[j], acc[TN - 1][j][e]);
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   }
   vm_wait<0>();  // no DMA may still land in LDS
@@ -287,11 +302,12 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(Args a) {
 }
 
 // Few rows of x: the weights are read once, and what bounds the kernel is how many of them are on their way.  A workgroup is
-// 16 NT columns of y; its eight wavefronts take every eighth block of K, each with a ring of its own in LDS that only it
-// waits for, and meet once at the end.
-template <int NT, int MB, int STAGES>
+// 16 NT columns of y; its wavefronts take blocks of K by turns, each with a ring of its own in LDS that only it
+// waits for, and meet once at the end.  Up to 16 rows, four wavefronts with three blocks on their way and two workgroups a CU, so that one
+// starts while another ends: 4096 x 4096 at M = 1 5.7 us, 28672 x 8192 42 (5.6 TB/s), at M = 16 50; eight wavefronts and one
+// workgroup 5.6, 48 and 57.
+template <int NT, int MB, int STAGES, int WAVES>
 struct Skinny {
-  static constexpr int WAVES = 8;
   static constexpr int STAGE = (NT + MB) * 2048 + 256;
   static constexpr int DMAS = 2 * (NT + MB) + 1;
   static constexpr int RING = STAGES * STAGE;
@@ -299,9 +315,9 @@ struct Skinny {
   static constexpr int LDS = WAVES * (RING > PARK ? RING : PARK);
 };
 
-template <int NT, int MB, int STAGES, bool WIDE>
-__global__ __launch_bounds__(512, 1) void skinny_kernel(Args a) {
-  using S = Skinny<NT, MB, STAGES>;
+template <int NT, int MB, int STAGES, int WAVES, bool WIDE>
+__global__ __launch_bounds__(64 * WAVES, 1) void skinny_kernel(Args a) {
+  using S = Skinny<NT, MB, STAGES, WAVES>;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MB, K = a.K;
@@ -331,12 +347,12 @@ __global__ __launch_bounds__(512, 1) void skinny_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < MB; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) issue(wave + 8 * s, s);
-  const float* ws = a.ws + (int64_t)(n0 / kK) * a.blocks;  // 16 NT divides 128
+  for (int s = 0; s < STAGES - 1; ++s) issue(wave + WAVES * s, s);
+  const scalar_p ws = scalar_pointer(a.ws + (int64_t)(n0 / kK) * a.blocks);  // 16 NT divides 128
   int stage = 0;
-  for (int b = wave; b < a.blocks; b += 8) {
+  for (int b = wave; b < a.blocks; b += WAVES) {
     const float wsc = ws[b];
-    issue(b + 8 * (STAGES - 1), stage == 0 ? STAGES - 1 : stage - 1);
+    issue(b + WAVES * (STAGES - 1), stage == 0 ? STAGES - 1 : stage - 1);
     vm_wait<(STAGES - 1) * S::DMAS>();
     const uint8_t* tw = ring + stage * S::STAGE;
     const uint8_t* tx = tw + NT * 2048;
@@ -367,36 +383,73 @@ __global__ __launch_bounds__(512, 1) void skinny_kernel(Args a) {
     for (int j = 0; j < MB; ++j)
       *(f32x4_t*)(all + wave * OUT + (16 * j + (lane & 15)) * COLS + 16 * i + 4 * (lane >> 4)) = acc[i][j];
   __syncthreads();
-  for (int o = tid; o < OUT; o += 512) {
+  for (int o = tid; o < OUT; o += 64 * WAVES) {
     const int m = m0 + o / COLS, n = n0 + o % COLS;
     if (m >= a.M || n >= a.N) continue;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) v += all[w * OUT + o];
+    for (int w = 0; w < WAVES; ++w) v += all[w * OUT + o];
     if (a.bias) v += load_scalar(a.bias, a.bias_dtype, n);
     store_scalar(a.y, a.y_dtype, (int64_t)m * a.N + n, v);
   }
 }
 
+// The kernels: of few rows, and tiles of rows x columns of y.
+enum Kind { AUTO = 0, SKINNY16, SKINNY32, TILE32x64, TILE64x128, TILE128x128, TILE128x256, TILE256x256, KINDS };
+std::atomic<int> g_kind{AUTO}, g_splits{0};  // what tests force
+
 // How a call runs.
 struct Plan {
-  int kind;    // 0: skinny, else tiles of `kind` rows
-  int splits;  // of K
+  Kind kind;
+  int splits;  // of K, over workgroups
   size_t bytes;
 };
+constexpr int kMaxSplits = 16;
+// Up to 16 rows the weights are streamed, above the kernel and split with the shortest time by a model: rounds of
+// workgroups times blocks of K times the time of a block's step, and the reduce (3 us and its fp32 partial sums at 4.5 TB/s).
+// us of a step measured where a workgroup is alone on its CU (two of 64 x 128 fit, which then take 1.5).  us, the best
+// of all kernels and splits and the model's choice: 32 x 14336 x 4096 16.1 and 16.1; 61 x 28672 x 8192 55.4 and 55.4; 64 x 8192
+// x 8192 21.1 and 21.1; 100 x 14336 x 4096 23.4 and 26; 128 x 28672 x 8192 72 and 81; 256 x 8192 x 8192 41 and 48; 512 x 14336 x 4096
+// 51 and 51; 1024 x 4096 x 4096 30 and 30; 2048 x 14336 x 4096 137 and 137; 2048 x 4096 x 4096 44 and 44.  256 x 256
+// and 128 x 256 have no WIDE form (registers).
 Plan plan_of(int M, int N, int K, bool wide) {
-  Plan p{0, 1, 0};
-  if (M <= 32) return p;
   const int blocks = (K + kK - 1) / kK, cus = device_cu_count();
-  auto tiles = [&](int bm, int bn) { return (int64_t)((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
-  p.kind = M <= 64 ? 64 : !wide && tiles(256, 256) >= cus ? 256 : 128;
-  const int64_t t = p.kind == 64 ? tiles(64, 64) : p.kind == 128 ? tiles(128, 128) : tiles(256, 256);
-  if (p.kind != 256 && t < cus) {
-    p.splits = (int)std::min<int64_t>(std::max<int64_t>(1, 2 * cus / t), std::max(1, blocks / 4));
-    const int per = (blocks + p.splits - 1) / p.splits;
-    p.splits = (blocks + per - 1) / per;
-    if (p.splits > 1) p.bytes = (size_t)p.splits * M * N * sizeof(float);
+  Plan p{SKINNY16, 1, 0};
+  struct Tiles {
+    Kind kind;
+    int bm, bn;
+    double step;
+  };
+  static const Tiles tiles[] = {{TILE32x64, 32, 64, 0.48}, {TILE64x128, 64, 128, 0.8}, {TILE128x128, 128, 128, 0.95},
+                                {TILE128x256, 128, 256, 1.5}, {TILE256x256, 256, 256, 2.1}};
+  const int forced = g_kind.load(std::memory_order_relaxed), splits = g_splits.load(std::memory_order_relaxed);
+  if (forced != AUTO) {
+    p.kind = (Kind)forced;
+    if (wide && p.kind > TILE128x128) p.kind = TILE128x128;
+    p.splits = p.kind >= TILE32x64 ? std::max(1, std::min(splits, blocks)) : 1;
+  } else if (M > 16) {
+    double best = 1e30;
+    if (M <= 32) {
+      p.kind = SKINNY32;
+      best = (double)((N + 32 * cus - 1) / (32 * cus)) * (3 + 0.2 * blocks);
+    }
+    for (const Tiles& t : tiles) {
+      if (wide && t.kind > TILE128x128) break;
+      const int64_t n = (int64_t)((M + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+      for (int S = 1; S <= std::min(kMaxSplits, blocks); ++S) {
+        if (S > 1 && n * (S - 1) >= 2 * cus) break;
+        const int per = (blocks + S - 1) / S;
+        if ((blocks + per - 1) / per != S) continue;
+        const bool two = t.kind == TILE64x128 && n * S > cus;
+        const double rounds = (double)((n * S + (two ? 2 : 1) * cus - 1) / ((two ? 2 : 1) * cus));
+        const double us = 2 + rounds * per * (two ? 1.5 : t.step) + (S > 1 ? 3 + 8e-6 / 4.5 * S * M * N : 0);
+        if (us < best) best = us, p.kind = t.kind, p.splits = S;
+      }
+    }
   }
+  const int per = (blocks + p.splits - 1) / p.splits;
+  p.splits = (blocks + per - 1) / per;
+  if (p.splits > 1) p.bytes = (size_t)p.splits * M * N * sizeof(float);
   return p;
 }
 
@@ -422,13 +475,13 @@ hipError_t launch_tiles(Args& a, int splits, hipStream_t s) {
   fn<<<dim3((unsigned)(a.tiles_m * a.tiles_n * splits)), dim3(64 * T::WAVES), T::LDS, s>>>(a);
   return hipGetLastError();
 }
-template <int NT, int MB, int STAGES, bool WIDE>
+template <int NT, int MB, int STAGES, int WAVES, bool WIDE>
 hipError_t launch_skinny(const Args& a, hipStream_t s) {
-  using S = Skinny<NT, MB, STAGES>;
+  using S = Skinny<NT, MB, STAGES, WAVES>;
   static std::atomic<uint64_t> done{0};
-  const auto fn = skinny_kernel<NT, MB, STAGES, WIDE>;
+  const auto fn = skinny_kernel<NT, MB, STAGES, WAVES, WIDE>;
   if (const hipError_t e = allow_lds((const void*)fn, S::LDS, &done); e != hipSuccess) return e;
-  fn<<<dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MB - 1) / (16 * MB))), dim3(512), S::LDS, s>>>(a);
+  fn<<<dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT)), (unsigned)((a.M + 16 * MB - 1) / (16 * MB))), dim3(64 * WAVES), S::LDS, s>>>(a);
   return hipGetLastError();
 }
 
@@ -447,6 +500,12 @@ int check(int M, int N, int K) {
 
 using namespace mlxr;
 using namespace mlxr::fp8;
+
+extern "C" int mlxr_fp8_test_force(int kind, int splits) {
+  if (kind < 0 || kind >= KINDS || splits < 0) return set_error(MLXR_E_INVALID, "fp8_test_force: no such kernel");
+  g_kind.store(kind), g_splits.store(splits);
+  return MLXR_OK;
+}
 
 extern "C" int mlxr_fp8_matmul_workspace_size(int M, int N, int K, int y_dtype, size_t* bytes) {
   if (!bytes) return set_error(MLXR_E_INVALID, "null bytes");
@@ -476,11 +535,15 @@ extern "C" int mlxr_fp8_matmul(int M, int N, int K, const void* x_dev, const flo
   if (p.splits > 1) a.part = (float*)workspace_dev;
   const hipStream_t s = (hipStream_t)stream;
   hipError_t e;
-  if (p.kind == 0) e = M <= 16 ? launch_skinny<1, 1, 4, true>(a, s) : launch_skinny<2, 2, 2, true>(a, s);
-  else if (p.kind == 64) e = launch_tiles<64, 64, 1, 4, 4, true>(a, p.splits, s);
-  else if (p.kind == 256) e = launch_tiles<256, 256, 4, 2, 2, false>(a, p.splits, s);
-  else if (wide) e = launch_tiles<128, 128, 2, 2, 2, true>(a, p.splits, s);
-  else e = launch_tiles<128, 128, 2, 2, 2, false>(a, p.splits, s);
+  switch (p.kind) {
+    case SKINNY16: e = launch_skinny<1, 1, 4, 4, true>(a, s); break;
+    case SKINNY32: e = launch_skinny<2, 2, 2, 8, true>(a, s); break;
+    case TILE32x64: e = wide ? launch_tiles<32, 64, 1, 4, 8, true>(a, p.splits, s) : launch_tiles<32, 64, 1, 4, 8, false>(a, p.splits, s); break;
+    case TILE64x128: e = wide ? launch_tiles<64, 128, 1, 4, 3, true>(a, p.splits, s) : launch_tiles<64, 128, 1, 4, 3, false>(a, p.splits, s); break;
+    case TILE128x256: e = launch_tiles<128, 256, 2, 4, 3, false>(a, p.splits, s); break;
+    case TILE256x256: e = launch_tiles<256, 256, 4, 2, 2, false>(a, p.splits, s); break;
+    default: e = wide ? launch_tiles<128, 128, 2, 2, 2, true>(a, p.splits, s) : launch_tiles<128, 128, 2, 4, 4, false>(a, p.splits, s); break;
+  }
   if (e == hipSuccess && p.splits > 1)
     e = launch_splitk_reduce(a.part, (size_t)M * N, p.splits, bias_dev, bias_dtype, y_dev, y_dtype, M, N, s);
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "fp8_matmul launch: %s", hipGetErrorString(e));

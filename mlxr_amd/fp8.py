@@ -29,6 +29,7 @@ _SIGS = {
     "mlxr_quantize_fp8_weight": (_I, [_I, _I, _P, _I, _P, _P, _P]),
     "mlxr_fp8_matmul_workspace_size": (_I, [_I, _I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
     "mlxr_fp8_matmul": (_I, [_I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, ctypes.c_size_t, _P]),
+    "mlxr_fp8_test_force": (_I, [_I, _I]),
 }
 _bound = None
 

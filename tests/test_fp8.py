@@ -314,6 +314,22 @@ def test_product(m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", range(1, 8))
+@pytest.mark.parametrize("m,n,k,splits", [(1, 5, 16, 1), (33, 300, 528, 1), (260, 517, 1040, 1), (300, 260, 1168, 3), (70, 1000, 2304, 7)])
+def test_product_in_every_kernel(kind, m, n, k, splits):
+    import torch
+    x, w = _activations(m, k, kind), _weights(n, k, kind + 1)
+    L = fp8._lib()
+    assert L.mlxr_fp8_test_force(8, 1) == -1 and L.mlxr_fp8_test_force(-1, 1) == -1
+    assert L.mlxr_fp8_test_force(kind, splits) == 0
+    try:
+        for dtype, bias in ((torch.float32, None), (torch.bfloat16, torch.randn(n, device="cuda", generator=_gen(3)))):
+            _check_product(mx.fp8_matmul(x, w, bias=bias, out_dtype=dtype), x, w, bias, dtype)
+    finally:
+        L.mlxr_fp8_test_force(0, 0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(1, 300, 272), (20, 256, 512), (50, 300, 272), (200, 300, 640), (600, 8192, 256)])
 def test_product_uses_nothing_outside(m, n, k):
     """NaN before and behind the operands, in rows of others and in scales of blocks that do not exist: none is seen.  A NaN

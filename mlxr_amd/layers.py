@@ -4,9 +4,11 @@ Mirror of the C++ classes in include/mlxr_linear.h, which follow the reference's
 core/graph/layers.h:59-94 (Linear: in_features, out_features, bias; forward(x) over
 x [..., in_features] with M = batch * seq, layers.cpp:86-99) and MLP::forward
 (layers.cpp:391-414: down(swish(gate(x)) * up(x))).  Weights are packed GGUF blocks on the
-device; every computation runs in libmlxr_qgemm.so (torch supplies memory and streams).
+device, or 8-bit floats with a scale for each 128 x 128 (Fp8Weight); every computation runs in
+libmlxr_qgemm.so (torch supplies memory and streams).
 """
-from . import qgemm
+from . import fp8, qgemm
+from .fp8 import Fp8Rows, Fp8Weight
 from .qgemm import BF16, F16, F32, PackedWeight, QGemmError
 
 
@@ -27,7 +29,7 @@ def swiglu(gate, up, out=None, stream=None):
 
 
 class Linear:
-    """y = x W^T (+ b) with W [out_features, in_features] held as packed GGUF blocks."""
+    """y = x W^T (+ b) with W [out_features, in_features] held as packed GGUF blocks or as an ``Fp8Weight``."""
 
     def __init__(self, in_features, out_features, bias=False):
         if in_features <= 0 or out_features <= 0:
@@ -37,10 +39,10 @@ class Linear:
         self.bias = None
 
     def load_weight(self, src, quant_type=None, name=None, device="cuda"):
-        """src: GGUF block bytes (numpy/torch uint8) with quant_type, a PackedWeight, or a
+        """src: GGUF block bytes (numpy/torch uint8) with quant_type, a PackedWeight, an Fp8Weight, or a
         GGUFFile with the tensor name."""
         from .gguf import GGUFFile
-        if isinstance(src, PackedWeight):
+        if isinstance(src, (PackedWeight, Fp8Weight)):
             pw = src
         elif isinstance(src, GGUFFile):
             info = src.find_tensor(name)
@@ -65,7 +67,8 @@ class Linear:
 
     def forward(self, x, stream=None, lora=None, adapter_ids=None):
         """x W^T (+ b); with ``lora`` (a LoraBank of this layer's shape) and ``adapter_ids`` [tokens] (int32,
-        -1: none) also each token's own adapter (lora_apply)."""
+        -1: none) also each token's own adapter (lora_apply).  An 8-bit weight also takes x as ``Fp8Rows`` [M, in_features]
+        (rms_norm's), giving bfloat16, without adapters; other x it rounds to 8 bits first."""
         if self.weight is None:
             raise QGemmError(-1, "Linear: weight not loaded")
         if (lora is None) != (adapter_ids is None):
@@ -74,6 +77,11 @@ class Linear:
             raise QGemmError(-3, "adapters do not match [out_features, in_features]")
         if self.has_bias and self.bias is None:
             raise QGemmError(-1, "Linear: bias not set")
+        eight = isinstance(self.weight, Fp8Weight)
+        if isinstance(x, Fp8Rows):
+            if not eight or lora is not None:
+                raise QGemmError(-1, "Linear: rows in 8 bits need an 8-bit weight and take no adapters")
+            return fp8.fp8_matmul(x, self.weight, bias=self.bias, stream=stream)
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise QGemmError(-3, "Input shape must be [..., in_features]")
         lead = x.shape[:-1]
@@ -81,8 +89,11 @@ class Linear:
         for d in lead:
             M *= int(d)
         x2 = x.reshape(M, self.in_features)
-        y = qgemm.q_gemm_dequant(x2, self.weight, M, self.out_features, self.in_features, self.weight.qtype,
-                                 bias=self.bias, stream=stream)
+        if eight:
+            y = fp8.fp8_matmul(x2, self.weight, bias=self.bias, stream=stream)
+        else:
+            y = qgemm.q_gemm_dequant(x2, self.weight, M, self.out_features, self.in_features, self.weight.qtype,
+                                     bias=self.bias, stream=stream)
         if lora is not None:
             y = lora.apply(x2, adapter_ids, y, out=y, stream=stream)
         return y.reshape(*lead, self.out_features)
@@ -93,7 +104,8 @@ class Linear:
 class MLP:
     """down(swish(gate(x)) * up(x)) through mlxr_qgemm_mlp: at M = 1 the whole block is one
     launch; above, the fused gate/up/gating launch and the down projection.  The layer holds
-    the workspace (sync words, h, split-K partials)."""
+    the workspace (sync words, h, split-K partials).  With 8-bit weights (Fp8Weight) x is rounded to 8 bits once
+    for gate and up, or comes as ``Fp8Rows``, and the gated rows once for down."""
 
     def __init__(self, hidden_size, intermediate_size):
         self.hidden_size, self.intermediate_size = hidden_size, intermediate_size
@@ -103,13 +115,16 @@ class MLP:
         self._ws = None
 
     def forward(self, x, stream=None):
-        if x.dim() < 1 or x.shape[-1] != self.hidden_size:
-            raise QGemmError(-3, "Input shape must be [..., hidden_size]")
-        lead = x.shape[:-1]
-        x2 = x.reshape(-1, self.hidden_size)
         gw, uw, dw = self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight
+        rows = isinstance(x, Fp8Rows)
+        if not rows and (x.dim() < 1 or x.shape[-1] != self.hidden_size):
+            raise QGemmError(-3, "Input shape must be [..., hidden_size]")
         if gw is None or uw is None or dw is None:
             raise QGemmError(-1, "MLP: weights not loaded")
+        if rows or isinstance(gw, Fp8Weight) or isinstance(uw, Fp8Weight) or isinstance(dw, Fp8Weight):
+            return self._forward8(x, rows, stream)
+        lead = x.shape[:-1]
+        x2 = x.reshape(-1, self.hidden_size)
         if (gw.qtype, gw.N) == (uw.qtype, uw.N):
             if self._ws is None:
                 self._ws = qgemm.MlpWorkspace(x.device)
@@ -120,5 +135,21 @@ class MLP:
             h = swiglu(g, u, out=g, stream=stream)
             y = self.down_proj.forward(h, stream=stream)
         return y.reshape(*lead, self.hidden_size)
+
+    def _forward8(self, x, rows, stream):
+        """forward where at least one weight is 8-bit, or x is Fp8Rows."""
+        gate, up = self.gate_proj, self.up_proj
+        both = isinstance(gate.weight, Fp8Weight) and isinstance(up.weight, Fp8Weight)
+        if rows and not both:
+            raise QGemmError(-1, "MLP: rows in 8 bits need 8-bit gate and up weights")
+        if both:
+            lead, dtype = ((x.data.shape[0],), None) if rows else (x.shape[:-1], x.dtype)
+            x8 = x if rows else fp8.quantize_fp8(x, stream=stream)
+            g, u = (fp8.fp8_matmul(x8, p.weight, out_dtype=dtype, stream=stream) for p in (gate, up))
+        else:
+            lead, x2 = x.shape[:-1], x.reshape(-1, self.hidden_size)
+            g, u = gate.forward(x2, stream=stream), up.forward(x2, stream=stream)
+        h = swiglu(g, u, out=g, stream=stream)
+        return self.down_proj.forward(h, stream=stream).reshape(*lead, self.hidden_size)
 
     __call__ = forward

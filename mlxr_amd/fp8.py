@@ -45,18 +45,22 @@ def _lib():
     return _bound
 
 
-def _rows(x, what):
-    """x [..., K] as rows [M, K] whose elements lie side by side (x's memory wherever that is possible)."""
-    if x.dim() < 1 or x.get_device() < 0:
+def _rows(x, index, what, stream):
+    """x [..., K] as rows: (x or what takes its place, rows, K, row stride in elements); copied only where no stride says it."""
+    shape = x.shape
+    if not shape or x.get_device() != index or index < 0:
         raise QGemmError(-3, f"{what} must be [..., K] on a GPU")
-    return x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-
-
-def _strided(x, stream):
-    s = x.stride()
-    if (s[1] == 1 or x.shape[1] == 1) and s[0] >= 0:
-        return x
-    return _on(stream, x.clone, memory_format=paged._torch.contiguous_format)
+    k = shape[-1]
+    if k == 0:
+        raise QGemmError(-3, f"{what}: rows must not be empty")
+    if x.is_contiguous():
+        return x, x.numel() // k, k, k
+    x = x.reshape(-1, k) if stream is None else _on(stream, x.reshape, -1, k)
+    st = x.stride()
+    if (st[1] != 1 and k > 1) or st[0] < 0:
+        x = _on(stream, x.clone, memory_format=paged._torch.contiguous_format)
+        st = x.stride()
+    return x, x.shape[0], k, st[0]
 
 
 def _out8(m, k, like, stream):
@@ -71,51 +75,53 @@ def rms_norm(x, weight=None, eps=1e-5, residual=None, quantize=False, out_dtype=
     x and ``residual``: one shape and dtype (float32, float16, bfloat16); ``weight`` [K] of any of them.  Returns the
     normed tensor in x's dtype (or ``out_dtype``), with ``quantize`` as ``Fp8Rows`` of [rows, K]; with a residual
     also the sum s in x's dtype: (normed, sum)."""
-    lib, shape = _lib(), x.shape
-    x2 = _rows(x, "rms_norm: x")
-    index, (m, k) = x2.get_device(), x2.shape
-    dt = _code(paged._x_codes, x.dtype, "x")
-    if k == 0:
-        raise QGemmError(-3, "rms_norm: rows must not be empty")
-    x2 = _strided(x2, stream)
-    r2 = total = None
+    lib = _bound or _lib()
+    torch, codes, index, shape, xt = paged._torch, paged._x_codes, x.get_device(), x.shape, x.dtype
+    x2, m, k, xs = _rows(x, index, "rms_norm: x", stream)
+    dt = codes.get(xt)
+    if dt is None:
+        _code(codes, xt, "x")
+    r2 = total = pr = pt = pw = None
+    rs = wt = 0
     if residual is not None:
-        if residual.shape != shape or residual.dtype is not x.dtype or residual.get_device() != index:
+        if residual.shape != shape or residual.dtype is not xt:
             raise QGemmError(-3, "rms_norm: the residual must have x's shape and dtype and be on its GPU")
-        r2 = _strided(_rows(residual, "rms_norm: residual"), stream)
-        total = _on(stream, paged._torch.empty, shape, dtype=x.dtype, device=x.device)
-    pw, wt = None, 0
+        r2, _, _, rs = _rows(residual, index, "rms_norm: the residual", stream)
+        total = torch.empty_like(x, memory_format=torch.contiguous_format) if stream is None else \
+            _on(stream, torch.empty, shape, dtype=xt, device=x.device)
+        pr, pt = r2.data_ptr(), total.data_ptr()
     if weight is not None:
         if weight.shape != (k,) or weight.get_device() != index or not weight.is_contiguous():
             raise QGemmError(-3, f"rms_norm: weight must be a contiguous [{k}] tensor on GPU {index}")
-        pw, wt = weight.data_ptr(), _code(paged._x_codes, weight.dtype, "weight")
+        pw, wt = weight.data_ptr(), _code(codes, weight.dtype, "weight")
+    ps = None
     if quantize:
         if out_dtype is not None:
             raise QGemmError(-1, "rms_norm: quantize and out_dtype exclude each other")
         out = _out8(m, k, x, stream)
         po, ot, ps = out.data.data_ptr(), E4M3, out.scales.data_ptr()
     else:
-        out = _on(stream, paged._torch.empty, shape, dtype=out_dtype or x.dtype, device=x.device)
-        po, ot, ps = out.data_ptr(), _code(paged._x_codes, out.dtype, "out"), None
-    qgemm._check(lib.mlxr_rms_norm(m, k, x2.data_ptr(), dt, x2.stride()[0], None if r2 is None else r2.data_ptr(),
-                                   0 if r2 is None else r2.stride()[0], pw, wt, eps, None if total is None else total.data_ptr(),
-                                   po, ot, ps, _stream(stream, index)))
+        if stream is None:
+            out = torch.empty_like(x, dtype=out_dtype, memory_format=torch.contiguous_format)
+        else:
+            out = _on(stream, torch.empty, shape, dtype=out_dtype or xt, device=x.device)
+        po, ot = out.data_ptr(), dt if out_dtype is None else _code(codes, out_dtype, "out")
+    rc = lib.mlxr_rms_norm(m, k, x2.data_ptr(), dt, xs, pr, rs, pw, wt, eps, pt, po, ot, ps, _stream(stream, index))
+    if rc:
+        qgemm._check(rc)
     return out if total is None else (out, total)
 
 
 def quantize_fp8(x, stream=None):
     """Rows x [..., K] in 8 bits, with a scale max|x| / 448 for each 128 elements (mlxr_quantize_fp8): ``Fp8Rows`` of
     [rows, K]."""
-    lib = _lib()
-    x2 = _rows(x, "quantize_fp8: x")
-    m, k = x2.shape
+    lib, index = _bound or _lib(), x.get_device()
     dt = _code(paged._x_codes, x.dtype, "x")
-    if k == 0:
-        raise QGemmError(-3, "quantize_fp8: rows must not be empty")
-    x2 = _strided(x2, stream)
+    x2, m, k, xs = _rows(x, index, "quantize_fp8: x", stream)
     out = _out8(m, k, x, stream)
-    qgemm._check(lib.mlxr_quantize_fp8(m, k, x2.data_ptr(), dt, x2.stride()[0], out.data.data_ptr(), out.scales.data_ptr(),
-                                       _stream(stream, x2.get_device())))
+    rc = lib.mlxr_quantize_fp8(m, k, x2.data_ptr(), dt, xs, out[0].data_ptr(), out[1].data_ptr(), _stream(stream, index))
+    if rc:
+        qgemm._check(rc)
     return out
 
 
@@ -160,7 +166,7 @@ def fp8_matmul(x, w, bias=None, out=None, out_dtype=None, stream=None):
 
     x: ``Fp8Rows`` [M, K], or [..., K] in float16, bfloat16 or float32, which is rounded by ``quantize_fp8`` first.  Returns
     [M, N] ([..., N]) in x's dtype (of ``Fp8Rows`` bfloat16), ``out_dtype``, or in ``out``."""
-    lib, torch = _lib(), paged._torch
+    lib, torch = _bound or _lib(), paged._torch
     if not isinstance(w, Fp8Weight):
         raise QGemmError(-1, "fp8_matmul: w must be an Fp8Weight")
     n, k, index = w.N, w.K, w.data.get_device()
@@ -198,6 +204,8 @@ def fp8_matmul(x, w, bias=None, out=None, out_dtype=None, stream=None):
     qgemm._check(lib.mlxr_fp8_matmul_workspace_size(m, n, k, yt, ctypes.byref(nb)))
     nb = nb.value
     ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=data.device) if nb else None
-    qgemm._check(lib.mlxr_fp8_matmul(m, n, k, data.data_ptr(), scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), pb, bt,
-                                     out.data_ptr(), yt, ws.data_ptr() if nb else None, nb, _stream(stream, index)))
+    rc = lib.mlxr_fp8_matmul(m, n, k, data.data_ptr(), scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), pb, bt,
+                             out.data_ptr(), yt, ws.data_ptr() if nb else None, nb, _stream(stream, index))
+    if rc:
+        qgemm._check(rc)
     return out

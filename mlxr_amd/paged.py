@@ -298,12 +298,21 @@ def paged_tree_attention(q, k_store, v_store, table, lens, starts, mask=None, sc
 def _layers(k, v):
     """mlxr_paged_cache of the first of a model's layers' stores [layers, pages, heads, page, dim] (or of one layer's), the
     layers, their strides and the GPU."""
-    if k.dim() == 4 and v.dim() == 4:
-        k, v = k[None], v[None]
-    if k.dim() != 5 or v.shape != k.shape or k.shape[0] == 0:
+    shape, ks, vs, index = k.shape, k.stride(), v.stride(), k.get_device()
+    if len(shape) == 4:
+        shape, ks, vs = (1, *shape), (0, *ks), (0, *vs)
+    if len(shape) != 5 or v.shape != k.shape or shape[0] == 0:
         raise QGemmError(-3, "key and value stores must be [layers, num_pages, kv_heads, page_size, head_dim] of one shape")
-    c, _, _, index = _cache(k[0], v[0], None, None)
-    return c, k.shape[0], k.stride(0), v.stride(0), index
+    if v.dtype is not k.dtype or v.get_device() != index or index < 0:
+        raise QGemmError(-1, "key and value stores must have one dtype and be on one GPU")
+    layers, pages, heads, page, dim = shape
+    if (ks[4] != 1 or vs[4] != 1) and dim > 1:
+        raise QGemmError(-3, "the last dimension of a store must be contiguous")
+    if pages == 1 or heads == 1 or page == 1:  # strides of single places mean nothing
+        ks, vs = ([s if n > 1 else 0 for s, n in zip(t, shape)] for t in (ks, vs))
+    code = _code(_cache_codes, k.dtype, "the cache")
+    return _pack_cache(k.data_ptr(), v.data_ptr(), 0, 0, ks[1], ks[2], ks[3], vs[1], vs[2], vs[3], code, pages, page, heads,
+                       dim), layers, ks[0], vs[0], index
 
 
 def paged_accept(k_store, v_store, table, lens, starts, path, counts, stream=None):

@@ -167,6 +167,7 @@ struct Kern {
   static constexpr int R = kThreads / TOK;                    // threads that bring a token's key and value to LDS
   static constexpr int LR = R == 4 ? 2 : 3;
   static constexpr int NL = CG / R > 0 ? CG / R : 1;          // loads of a thread, tile and store
+  static constexpr int AHEAD = F8 || CW == 1 ? 3 : 2;         // steps that reads of LDS go before their products
   static constexpr int STORE = TOK * DT * 2;                  // bytes of a tile's keys or values in LDS
   static constexpr int LDS = 4 * STORE;
   // The reference that weights are relative to follows the maximum only when that is 2^SLACK above it: weights are at most
@@ -196,6 +197,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15;
+
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
 
   // ---- this workgroup's run of tiles
   int64_t* pre = (int64_t*)(lds + T::LDS);  // [rows + 1] before each row: tiles, or (not cut) blocks of columns
@@ -442,17 +445,29 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
         __syncthreads();
       }
       if (!idle) {
+        // Reads of LDS go AHEAD steps before the products that take them, in the order written (sched_barrier): left to
+        // itself the compiler saves registers and waits for each read.
+        constexpr int AHEAD = T::AHEAD;
         u32x4_t p[KT][CW][PARTS];
         f32x4_t s[NT][CW];
+        {
+          constexpr int N = KS * NT;
+          u32x4_t kf[AHEAD + 1];
+          // of tokens 16 i + col, piece 4 k + g: its place is token col's, with 4 k in the exclusive or, 16 i rows further
+          const uint32_t at = lds_at + half * 2 * T::STORE + T::key_place(col, g);
+          auto key = [&](int n) { return *(const __attribute__((address_space(3))) u32x4_t*)(uintptr_t)((at ^ (n / NT * 64)) + n % NT * 16 * DT * 2); };
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+          for (int n = 0; n < AHEAD; ++n) kf[n] = key(n);
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            const u32x4_t kf = *(const u32x4_t*)(ks + T::key_place(16 * i + col, 4 * k + g));
+          for (int n = 0; n < N; ++n) {
+            if (n + AHEAD < N) kf[(n + AHEAD) % (AHEAD + 1)] = key(n + AHEAD);
+            const int k = n / NT, i = n % NT;
 #pragma unroll
-            for (int j = 0; j < CW; ++j) s[i][j] = mfma16<F16>(kf, q[j][k], k ? s[i][j] : f32x4_t{0, 0, 0, 0});
+            for (int j = 0; j < CW; ++j) s[i][j] = mfma16<F16>(kf[n % (AHEAD + 1)], q[j][k], k ? s[i][j] : f32x4_t{0, 0, 0, 0});
+            __builtin_amdgcn_sched_barrier(0);
           }
-        __builtin_amdgcn_sched_barrier(0);
+        }
+        float off[CW];
 #pragma unroll
         for (int j = 0; j < CW; ++j) {
           if (!plain) {
@@ -482,42 +497,54 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d][j] *= alpha;
           }
-          const float off = T::SHIFT - (m[j] == -INFINITY ? 0.f : m[j]);  // nothing but -inf so far: weights 0, not NaN
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][2 * h], sc, off));
-              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][2 * h + 1], sc, off));
-              sum += p0 + p1;
-              uint32_t out[PARTS];
-              split_parts<P16, PARTS>(p0, p1, out);
-#pragma unroll
-              for (int n = 0; n < PARTS; ++n) p[i >> 1][j][n][2 * (i & 1) + h] = out[n];
-            }
-          l[j] += sum;
+          off[j] = T::SHIFT - (m[j] == -INFINITY ? 0.f : m[j]);  // nothing but -inf so far: weights 0, not NaN
         }
+        // Weights of pair u of 32 tokens k: two of a lane's eight, of a column.  Those of the next 32 tokens are made between the
+        // products of these.
+        auto weights = [&](int k, int u) {
+          const int j = u % CW, i = 2 * k + u / CW / 2, h = u / CW % 2;
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][2 * h], sc, off[j]));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][2 * h + 1], sc, off[j]));
+          l[j] += p0 + p1;
+          uint32_t out[PARTS];
+          split_parts<P16, PARTS>(p0, p1, out);
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
+          for (int n = 0; n < PARTS; ++n) p[k][j][n][2 * (i & 1) + h] = out[n];
+        };
+        constexpr int N = KT * ND, PAIRS = 4 * CW;
+        // Of 16 tokens, lane group g's four: rows 4 g .. 4 g + 3, eight bytes a lane; the transposing read gives each lane its dim of the
+        // four.  Dims d are in the exclusive or of the first row's place, later tokens rows further.
+        const uint32_t at = lds_at + (half * 2 + 1) * T::STORE + T::value_place(4 * g + (col >> 2), 0) + 8 * (col & 3);
+        auto value = [&](int n) {  // dims n % ND of 32 tokens n / ND
+          typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+          typedef __attribute__((address_space(3))) s16x4_t* lds_p;
+          u32x4_t vf;
 #pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            typedef __attribute__((ext_vector_type(4))) short s16x4_t;
-            typedef __attribute__((address_space(3))) s16x4_t* lds_p;
-            u32x4_t vf;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              // rows 4 g .. 4 g + 3 of 16 tokens, eight bytes a lane; the read gives each lane its dim of the four
-              const int t = 32 * k + 16 * h + 4 * g + (col >> 2);
-              const u32x2_t v = __builtin_bit_cast(
-                  u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(vs + T::value_place(t, d) + 8 * (col & 3))));
-              vf[2 * h] = v[0], vf[2 * h + 1] = v[1];
-            }
-#pragma unroll
-            for (int j = 0; j < CW; ++j)
-#pragma unroll
-              for (int n = PARTS - 1; n >= 0; --n) o[d][j] = mfma16<P16>(vf, p[k][j][n], o[d][j]);
+          for (int h = 0; h < 2; ++h) {
+            const u32x2_t v = __builtin_bit_cast(
+                u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(uintptr_t)((at ^ (n % ND * 32)) + (32 * (n / ND) + 16 * h) * DT * 2)));
+            vf[2 * h] = v[0], vf[2 * h + 1] = v[1];
           }
+          return vf;
+        };
+        u32x4_t vf[AHEAD + 1];
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) vf[n] = value(n);
+#pragma unroll
+        for (int u = 0; u < PAIRS; ++u) weights(0, u);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (n + AHEAD < N) vf[(n + AHEAD) % (AHEAD + 1)] = value(n + AHEAD);
+          const int k = n / ND, d = n % ND;
+#pragma unroll
+          for (int j = 0; j < CW; ++j)
+#pragma unroll
+            for (int part = PARTS - 1; part >= 0; --part) o[d][j] = mfma16<P16>(vf[n % (AHEAD + 1)], p[k][j][part], o[d][j]);
+          if (k + 1 < KT)
+#pragma unroll
+            for (int u = d * PAIRS / ND; u < (d + 1) * PAIRS / ND; ++u) weights(k + 1, u);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (t0 + TOK < stop) {

@@ -136,7 +136,8 @@ constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 1) / 2 * 2 
 Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int width, int q_dtype, int out_dtype) {
   Plan p;
   const int group = heads / c->kv_heads;
-  const int64_t columns = ((int64_t)tokens * group + rows - 1) / rows;
+  // on average, padding included; an eighth more than a block of columns is still taken as one
+  const int64_t columns = (int64_t)tokens * group / rows * 8 / 9;
   p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), out_dtype);
   p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
   const int64_t held = (int64_t)width * c->page_size, tiles = (held + p.k.tok - 1) / p.k.tok;

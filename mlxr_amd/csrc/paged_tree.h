@@ -181,7 +181,11 @@ struct Kern {
   static __device__ __forceinline__ int key_place(int t, int c) {
     constexpr int N = CH >= 16 ? 4 : 3;  // bits of a piece's place within 256 bytes of banks; shorter rows are two to those
     const int u = CH >= 16 ? t : t >> 1;
-    return t * DT * 2 + (c ^ ((u & ((1 << (N - LR)) - 1)) << LR | (u >> (N - LR) & (R - 1)))) * 16;
+    int swap;
+    if constexpr (!F8) swap = (u & ((1 << (N - LR)) - 1)) << LR | (u >> (N - LR) & (R - 1));
+    else if constexpr (N - LR == 1) swap = u & ((1 << N) - 1);  // e4m3: of the two pieces that one widens to, every other at once
+    else swap = (u & 1) | (u >> 2 & 3) << 1 | (u >> 1 & 1) << 3;
+    return t * DT * 2 + (c ^ swap) * 16;
   }
   static __device__ __forceinline__ int value_place(int t, int p) {
     const int swap = ND < 8 ? (t & 2) | (t >> 2 & 1) : R == 8 ? (t & 1) << 2 | (t >> 1 & 3) : (t & 3) << 1 | (t >> 2 & 1);

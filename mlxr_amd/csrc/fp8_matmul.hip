@@ -406,10 +406,11 @@ struct Plan {
 };
 constexpr int kMaxSplits = 16;
 // Up to 16 rows the weights are streamed, above the kernel and split with the shortest time by a model: rounds of
-// workgroups times blocks of K times the time of a block's step, and the reduce (3 us and its fp32 partial sums at 4.5 TB/s).
+// workgroups times blocks of K times the time of a block's step, no less than the weights at the rate at which a kernel
+// streams them (TB/s), and the reduce (3 us and its fp32 partial sums at 4.5 TB/s).
 // us of a step measured where a workgroup is alone on its CU (two of 64 x 128 fit, which then take 1.5).  us, the best
 // of all kernels and splits and the model's choice: 32 x 14336 x 4096 16.1 and 16.1; 61 x 28672 x 8192 55.4 and 55.4; 64 x 8192
-// x 8192 21.1 and 21.1; 100 x 14336 x 4096 23.4 and 26; 128 x 28672 x 8192 72 and 81; 256 x 8192 x 8192 41 and 48; 512 x 14336 x 4096
+// x 8192 21.1 and 21.1; 100 x 14336 x 4096 23 and 23; 128 x 28672 x 8192 72 and 72; 256 x 8192 x 8192 36 and 36; 512 x 14336 x 4096
 // 51 and 51; 1024 x 4096 x 4096 30 and 30; 2048 x 14336 x 4096 137 and 137; 2048 x 4096 x 4096 44 and 44.  256 x 256
 // and 128 x 256 have no WIDE form (registers).
 Plan plan_of(int M, int N, int K, bool wide) {
@@ -418,10 +419,10 @@ Plan plan_of(int M, int N, int K, bool wide) {
   struct Tiles {
     Kind kind;
     int bm, bn;
-    double step;
+    double step, rate;
   };
-  static const Tiles tiles[] = {{TILE32x64, 32, 64, 0.48}, {TILE64x128, 64, 128, 0.8}, {TILE128x128, 128, 128, 0.95},
-                                {TILE128x256, 128, 256, 1.5}, {TILE256x256, 256, 256, 2.1}};
+  static const Tiles tiles[] = {{TILE32x64, 32, 64, 0.48, 4.5}, {TILE64x128, 64, 128, 0.8, 4.4}, {TILE128x128, 128, 128, 0.95, 2.9},
+                                {TILE128x256, 128, 256, 1.5, 4}, {TILE256x256, 256, 256, 2.1, 4}};
   const int forced = g_kind.load(std::memory_order_relaxed), splits = g_splits.load(std::memory_order_relaxed);
   if (forced != AUTO) {
     p.kind = (Kind)forced;
@@ -442,7 +443,7 @@ Plan plan_of(int M, int N, int K, bool wide) {
         if ((blocks + per - 1) / per != S) continue;
         const bool two = t.kind == TILE64x128 && n * S > cus;
         const double rounds = (double)((n * S + (two ? 2 : 1) * cus - 1) / ((two ? 2 : 1) * cus));
-        const double us = 2 + rounds * per * (two ? 1.5 : t.step) + (S > 1 ? 3 + 8e-6 / 4.5 * S * M * N : 0);
+        const double us = 2 + std::max(rounds * per * (two ? 1.5 : t.step), 1e-6 / t.rate * N * K) + (S > 1 ? 3 + 8e-6 / 4.5 * S * M * N : 0);
         if (us < best) best = us, p.kind = t.kind, p.splits = S;
       }
     }

@@ -330,6 +330,30 @@ def test_product_in_every_kernel(kind, m, n, k, splits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", range(0, 8))
+def test_product_knows_every_code(kind):
+    """One-hot rows read single weights off, of every one of the 256 codes (both zeros, the values below the normal ones, NaN)."""
+    import torch
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    w = mx.Fp8Weight(codes.view(256, 1).expand(256, 16).contiguous().view(torch.float8_e4m3fn), torch.full((2, 1), 0.5, device="cuda"))
+    one = torch.zeros((40, 16), device="cuda")
+    one[torch.arange(40), torch.arange(40) % 16] = 1.0
+    x = mx.Fp8Rows(one.to(torch.float8_e4m3fn), torch.full((40, 1), 2.0, device="cuda"))
+    # 0 times NaN is NaN: codes of one are their value in every row
+    want = codes.view(torch.float8_e4m3fn).float().expand(40, 256)
+    L = fp8._lib()
+    assert L.mlxr_fp8_test_force(kind, 1) == 0
+    try:
+        for dtype in (torch.float32, torch.bfloat16, torch.float16):
+            got = mx.fp8_matmul(x, w, out_dtype=dtype).float()
+            assert torch.equal(got.nan_to_num(1e9), want.nan_to_num(1e9)), dtype  # 4 bits fit every output type
+            back = mx.fp8_matmul(mx.Fp8Rows(w.data, torch.ones((256, 1), device="cuda")), mx.Fp8Weight(x.data, torch.ones((1, 1), device="cuda")), out_dtype=dtype)
+            assert torch.equal(back.float().nan_to_num(1e9), want.t().contiguous().nan_to_num(1e9)), dtype
+    finally:
+        L.mlxr_fp8_test_force(0, 0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m,n,k", [(1, 300, 272), (20, 256, 512), (50, 300, 272), (200, 300, 640), (600, 8192, 256)])
 def test_product_uses_nothing_outside(m, n, k):
     """NaN before and behind the operands, in rows of others and in scales of blocks that do not exist: none is seen.  A NaN

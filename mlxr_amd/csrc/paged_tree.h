@@ -34,7 +34,7 @@ using paged::load_words;
 using paged::store_values;
 using paged::widen;
 
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kThreads = 256;  // of the join and the masks
 constexpr int kMaxRows = MLXR_PAGED_MAX_ROWS;
 constexpr int kStart = 2;  // tiles that the start and the end of a row's columns are counted for
 
@@ -155,16 +155,16 @@ __device__ __forceinline__ uint32_t clean2(uint32_t w) {
   return w;
 }
 
-// DT: 64, 128 or 256, at least head_dim.  CW: columns of a wavefront, by 16.  TOK: tokens of a tile (32, 64).  OCC: workgroups
+// DT: 64, 128 or 256, at least head_dim.  W: wavefronts.  CW: columns of a wavefront, by 16.  TOK: tokens of a tile (32, 64).  OCC: workgroups
 // that a CU's registers and LDS hold.
-template <bool F16, bool F8, int DT, int CW, int TOK, int OCC, int PARTS>
+template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC, int PARTS>
 struct Kern {
   static constexpr bool P16 = F16 || F8;                      // the second product's type, f16 or else bf16
-  static constexpr int QB = 16 * CW * kWaves;
+  static constexpr int THREADS = 64 * W, QB = 16 * CW * W;
   static constexpr int NT = TOK / 16, KT = TOK / 32, KS = DT / 32, ND = DT / 16;
   static constexpr int CH = DT / 8;                           // 16-byte pieces of a row in LDS
   static constexpr int CG = F8 ? DT / 16 : DT / 8;            // and in memory
-  static constexpr int R = kThreads / TOK;                    // threads that bring a token's key and value to LDS
+  static constexpr int R = THREADS / TOK;                     // threads that bring a token's key and value to LDS
   static constexpr int LR = R == 4 ? 2 : 3;
   static constexpr int NL = CG / R > 0 ? CG / R : 1;          // loads of a thread, tile and store
   static constexpr int AHEAD = F8 || CW == 1 ? 3 : 2;         // steps that reads of LDS go before their products
@@ -193,10 +193,10 @@ struct Kern {
   }
 };
 
-template <bool F16, bool F8, int DT, int CW, int TOK, int OCC, int PARTS>
-__global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
-  using T = Kern<F16, F8, DT, CW, TOK, OCC, PARTS>;
-  constexpr int NT = T::NT, KT = T::KT, KS = T::KS, ND = T::ND, NL = T::NL;
+template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC, int PARTS>
+__global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
+  using T = Kern<F16, F8, DT, W, CW, TOK, OCC, PARTS>;
+  constexpr int THREADS = T::THREADS, NT = T::NT, KT = T::KT, KS = T::KS, ND = T::ND, NL = T::NL;
   constexpr bool P16 = T::P16;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -206,13 +206,13 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
 
   // ---- this workgroup's run of tiles
   int64_t* pre = (int64_t*)(lds + T::LDS);  // [rows + 1] before each row: tiles, or (not cut) blocks of columns
-  int64_t* part = pre + a.rows + 1;         // [4]
-  int* flag = (int*)(part + 4);             // [2][4] of the tiles' wavefronts
+  int64_t* part = pre + a.rows + 1;         // [W]
+  int* flag = (int*)(part + W);             // [2][W] of the tiles' wavefronts
   const bool cut = a.ws != nullptr;
   // a unit of the deal: kStart places, then its tiles
   auto weight = [&](const Row& w) { return (int64_t)a.kv_heads * w.blocks * (!cut ? 1 : w.tiles ? w.tiles + kStart : 0); };
   {
-    const int per_thread = (a.rows + kThreads - 1) / kThreads;
+    const int per_thread = (a.rows + THREADS - 1) / THREADS;
     const int r0 = min(tid * per_thread, a.rows), r1 = min(r0 + per_thread, a.rows);
     int64_t n = 0;
     for (int r = r0; r < r1; ++r) n += weight(row_of(a, r));
@@ -230,14 +230,14 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
       pre[r] = at;
       at += weight(row_of(a, r));
     }
-    if (tid == kThreads - 1) pre[a.rows] = at;
+    if (tid == THREADS - 1) pre[a.rows] = at;
     __syncthreads();
   }
   // tokens behind the last row's: zeros
   {
     const int from = min(max(a.starts[a.rows], 0), a.tokens);
     const int64_t first = (int64_t)from * a.heads * a.dim, count = (int64_t)(a.tokens - from) * a.heads * a.dim;
-    const int64_t id = (int64_t)blockIdx.x * kThreads + tid, step = (int64_t)gridDim.x * kThreads;
+    const int64_t id = (int64_t)blockIdx.x * THREADS + tid, step = (int64_t)gridDim.x * THREADS;
     for (int64_t i = id; i < count / 8; i += step) {
       const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
       store_values<8>(a.out, a.out_dtype, first + 8 * i, z);
@@ -248,7 +248,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
   const int64_t total = pre[a.rows];
   const int64_t per = cut ? (total + a.workers - 1) / a.workers : 1;
   if (cut && blockIdx.x == 0) {
-    for (int r = tid; r <= a.rows; r += kThreads) a.prefix[r] = pre[r];
+    for (int r = tid; r <= a.rows; r += THREADS) a.prefix[r] = pre[r];
     if (tid == 0) a.prefix[a.rows + 1] = per;
   }
   // workgroup id % 8 is the XCD: each takes neighbouring runs, which read the same keys and values
@@ -402,10 +402,14 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
     bool odd = false;
     auto join_waves = [&](int half, bool nodes, bool any) {
       // words of this half are read before the next barrier, and written again only after it
-      if (nodes && lane == 0) flag[4 * half + wave] = 0;
-      if (nodes && any) flag[4 * half + wave] = 1;
+      if (nodes && lane == 0) flag[W * half + wave] = 0;
+      if (nodes && any) flag[W * half + wave] = 1;
       __syncthreads();
-      odd = nodes && __builtin_amdgcn_readfirstlane(flag[4 * half] | flag[4 * half + 1] | flag[4 * half + 2] | flag[4 * half + 3]);
+      int any_wave = 0;
+      if (nodes)
+#pragma unroll
+        for (int w = 0; w < W; ++w) any_wave |= flag[W * half + w];
+      odd = __builtin_amdgcn_readfirstlane(any_wave);
     };
     if (count > 0) {  // a row without tokens has no tile
       pages_of(base);
@@ -445,7 +449,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
           }
         __syncthreads();
 #pragma unroll 1
-        for (int i = tid; i < T::STORE / 4; i += kThreads) ((uint32_t*)vs)[i] = clean2<P16>(((uint32_t*)vs)[i]);
+        for (int i = tid; i < T::STORE / 4; i += THREADS) ((uint32_t*)vs)[i] = clean2<P16>(((uint32_t*)vs)[i]);
         __syncthreads();
       }
       if (!idle) {
@@ -604,27 +608,34 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_kernel(Args a) {
 
 struct TreeKern {
   const void* fn;
-  int qb, tok, lds;
+  int qb, tok, lds, threads;
   std::atomic<int>* residents;  // workgroups of a CU, by device; 0: not asked yet
 };
 
-// The kernel for head_dim, about `columns` columns of a row and the type of the output.
-TreeKern kern_bf16(int dim, int columns, int out_dtype);
-TreeKern kern_f16(int dim, int columns, int out_dtype);
-TreeKern kern_bf16_e4m3(int dim, int columns, int out_dtype);
-TreeKern kern_f16_e4m3(int dim, int columns, int out_dtype);
+// The kernel for head_dim, about `columns` columns of a row, the longest row that the table holds and the type of the output.
+// Eight wavefronts share a tile where there are columns for them: half as many loads, widenings and LDS writes a column.  us, four
+// and eight: 64 drafts of 8 rows of 16384, e4m3, 365 and 333; of 8192, bf16, 164 and 147; a chain of 513 over 6001 131 and 124; but 64
+// drafts of 64 rows of 64 91 and 101, of 256 135 and 147.  Up to 64 columns, one group of 16 a wavefront: 16 drafts of 32 rows of
+// 8192 (64 columns) 226, two groups 359.
+TreeKern kern_bf16(int dim, int columns, int longest, int out_dtype);
+TreeKern kern_f16(int dim, int columns, int longest, int out_dtype);
+TreeKern kern_bf16_e4m3(int dim, int columns, int longest, int out_dtype);
+TreeKern kern_f16_e4m3(int dim, int columns, int longest, int out_dtype);
 
-template <bool F16, bool F8, int DT, int CW, int TOK, int OCC, int PARTS>
+template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC, int PARTS>
 TreeKern kern_t() {
-  using T = Kern<F16, F8, DT, CW, TOK, OCC, PARTS>;
+  using T = Kern<F16, F8, DT, W, CW, TOK, OCC, PARTS>;
   static std::atomic<int> residents[64];
-  return TreeKern{(const void*)tree_kernel<F16, F8, DT, CW, TOK, OCC, PARTS>, T::QB, TOK, T::LDS, residents};
+  return TreeKern{(const void*)tree_kernel<F16, F8, DT, W, CW, TOK, OCC, PARTS>, T::QB, TOK, T::LDS, T::THREADS, residents};
 }
 template <bool F16, bool F8, int PARTS>
-TreeKern kern_of(int dim, int columns) {
-  if (dim > 128) return kern_t<F16, F8, 256, 1, 32, 2, PARTS>();
-  if (dim > 64) return columns > 64 ? kern_t<F16, F8, 128, 2, 64, 2, PARTS>() : kern_t<F16, F8, 128, 1, 64, 2, PARTS>();
-  return columns > 64 ? kern_t<F16, F8, 64, 2, 64, 2, PARTS>() : kern_t<F16, F8, 64, 1, 64, 4, PARTS>();
+TreeKern kern_of(int dim, int columns, int longest) {
+  if (dim > 128) return kern_t<F16, F8, 256, 4, 1, 32, 2, PARTS>();
+  if (dim > 64) {
+    if (columns > 128 && longest > 512) return kern_t<F16, F8, 128, 8, 2, 64, 1, PARTS>();
+    return columns > 64 ? kern_t<F16, F8, 128, 4, 2, 64, 2, PARTS>() : kern_t<F16, F8, 128, 4, 1, 64, 2, PARTS>();
+  }
+  return columns > 64 ? kern_t<F16, F8, 64, 4, 2, 64, 2, PARTS>() : kern_t<F16, F8, 64, 4, 1, 64, 4, PARTS>();
 }
 
 }  // namespace tree

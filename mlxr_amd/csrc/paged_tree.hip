@@ -116,10 +116,10 @@ __global__ __launch_bounds__(kThreads) void mask_kernel(MaskArgs a) {
   }
 }
 
-TreeKern kern(const mlxr_paged_cache* c, int q_dtype, int columns, int out_dtype) {
+TreeKern kern(const mlxr_paged_cache* c, int q_dtype, int columns, int longest, int out_dtype) {
   const bool f16 = q_dtype == MLXR_F16;
-  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, columns, out_dtype) : kern_bf16_e4m3(c->head_dim, columns, out_dtype);
-  return f16 ? kern_f16(c->head_dim, columns, out_dtype) : kern_bf16(c->head_dim, columns, out_dtype);
+  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, columns, longest, out_dtype) : kern_bf16_e4m3(c->head_dim, columns, longest, out_dtype);
+  return f16 ? kern_f16(c->head_dim, columns, longest, out_dtype) : kern_bf16(c->head_dim, columns, longest, out_dtype);
 }
 
 constexpr int kMaxHeads = 1 << 26;  // tokens times heads: a launch has fewer than 2^32 threads
@@ -138,9 +138,10 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   const int group = heads / c->kv_heads;
   // on average, padding included; an eighth more than a block of columns is still taken as one
   const int64_t columns = (int64_t)tokens * group / rows * 8 / 9;
-  p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), out_dtype);
+  const int64_t held = (int64_t)width * c->page_size;
+  p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), (int)held, out_dtype);
   p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
-  const int64_t held = (int64_t)width * c->page_size, tiles = (held + p.k.tok - 1) / p.k.tok;
+  const int64_t tiles = (held + p.k.tok - 1) / p.k.tok;
   p.cut = tiles > 4 && p.units < 8 * device_cu_count();
   p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
   return p;
@@ -226,8 +227,8 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   a.by_page = Divisor(a.page), a.by_group = Divisor(a.group);
   a.scale = scale * 1.44269504088896341f;
   const hipStream_t st = (hipStream_t)stream;
-  // LDS: two tiles, the rows' prefix, four sums and eight words; the limit is raised to all that a workgroup may use, once on each device
-  const int lds = p.k.lds + (rows + 1 + 8) * (int)sizeof(int64_t), most = (int)device_lds_limit();
+  // LDS: two tiles, the rows' prefix, the wavefronts' sums and words; the limit is raised to all that a workgroup may use, once on each device
+  const int lds = p.k.lds + (rows + 1 + 16) * (int)sizeof(int64_t), most = (int)device_lds_limit();
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention: %s", hipGetErrorString(e));
@@ -235,7 +236,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   int occ = residents.load(std::memory_order_acquire);
   if (!occ) {
     e = hipFuncSetAttribute(p.k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == hipSuccess) e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, p.k.fn, kThreads, p.k.lds + 1024);
+    if (e == hipSuccess) e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, p.k.fn, p.k.threads, p.k.lds + 1024);
     if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention: %s", hipGetErrorString(e));
     occ = std::max(1, std::min(occ, kGridPerCu));
     residents.store(occ, std::memory_order_release);
@@ -247,7 +248,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
     a.prefix = (int64_t*)workspace_dev, a.ws = (float*)((uint8_t*)workspace_dev + prefix_bytes(rows));
   }
   void* args[] = {&a};
-  e = hipLaunchKernel(p.k.fn, dim3((unsigned)grid), dim3(kThreads), args, (size_t)lds, st);
+  e = hipLaunchKernel(p.k.fn, dim3((unsigned)grid), dim3(p.k.threads), args, (size_t)lds, st);
   if (e == hipSuccess && p.cut) {
     int lanes = 2;
     while (4 * lanes < a.dim) lanes *= 2;

@@ -58,6 +58,12 @@ int mlxr_fp8_matmul_workspace_size(int M, int N, int K, int y_dtype, size_t* byt
 int mlxr_fp8_matmul(int M, int N, int K, const void* x_dev, const float* x_scale_dev, const void* w_dev,
                     const float* w_scale_dev, const void* bias_dev, int bias_dtype, void* y_dev, int y_dtype,
                     void* workspace_dev, size_t workspace_bytes, void* stream);
+/* The same of rows in 16 or 32 bits: x_dev [M, K] of x_dtype (MLXR_F32 / MLXR_F16 / MLXR_BF16), row stride x_stride elements, is
+ * rounded by mlxr_quantize_fp8 into the workspace (at a multiple of 16 bytes, always needed) first. */
+int mlxr_fp8_linear_workspace_size(int M, int N, int K, int y_dtype, size_t* bytes);
+int mlxr_fp8_linear(int M, int N, int K, const void* x_dev, int x_dtype, int64_t x_stride, const void* w_dev,
+                    const float* w_scale_dev, const void* bias_dev, int bias_dtype, void* y_dev, int y_dtype,
+                    void* workspace_dev, size_t workspace_bytes, void* stream);
 /* Test hook, process-wide: kernel (0: by shape; 1, 2: of few rows; 3 .. 7: tiles, ascending) and splits of K over workgroups of
  * every later mlxr_fp8_matmul and its workspace size. */
 int mlxr_fp8_test_force(int kind, int splits);

@@ -550,3 +550,36 @@ extern "C" int mlxr_fp8_matmul(int M, int N, int K, const void* x_dev, const flo
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "fp8_matmul launch: %s", hipGetErrorString(e));
   return MLXR_OK;
 }
+
+namespace {
+// Rows in 8 bits, their scales, the product's own workspace, each at a multiple of 256 bytes.
+size_t padded(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+size_t row_bytes(int M, int K) { return padded((size_t)M * K); }
+size_t scale_bytes(int M, int K) { return padded((size_t)M * ((K + kK - 1) / kK) * sizeof(float)); }
+}  // namespace
+
+extern "C" int mlxr_fp8_linear_workspace_size(int M, int N, int K, int y_dtype, size_t* bytes) {
+  if (const int rc = mlxr_fp8_matmul_workspace_size(M, N, K, y_dtype, bytes)) return rc;
+  if (M) *bytes += row_bytes(M, K) + scale_bytes(M, K);
+  return MLXR_OK;
+}
+
+extern "C" int mlxr_fp8_linear(int M, int N, int K, const void* x_dev, int x_dtype, int64_t x_stride, const void* w_dev,
+                               const float* w_scale_dev, const void* bias_dev, int bias_dtype, void* y_dev, int y_dtype,
+                               void* workspace_dev, size_t workspace_bytes, void* stream) {
+  size_t need;
+  if (const int rc = mlxr_fp8_linear_workspace_size(M, N, K, y_dtype, &need)) return rc;
+  if (bias_dev && !float_type(bias_dtype)) return set_error(MLXR_E_INVALID, "fp8_linear: invalid dtype");
+  if (M == 0) return MLXR_OK;
+  if (!x_dev || !w_dev || !w_scale_dev || !y_dev) return set_error(MLXR_E_INVALID, "null buffer");
+  if (((uintptr_t)w_dev | (uintptr_t)y_dev | (uintptr_t)workspace_dev) & 15)
+    return set_error(MLXR_E_SHAPE, "fp8_linear: w, y and workspace must lie at multiples of 16 bytes");
+  if (workspace_bytes < need || !workspace_dev)
+    return set_error(MLXR_E_INVALID, "fp8_linear: the workspace is smaller than mlxr_fp8_linear_workspace_size");
+  uint8_t* rows = (uint8_t*)workspace_dev;
+  float* scales = (float*)(rows + row_bytes(M, K));
+  uint8_t* rest = (uint8_t*)scales + scale_bytes(M, K);
+  if (const int rc = mlxr_quantize_fp8(M, K, x_dev, x_dtype, x_stride, rows, scales, stream)) return rc;
+  return mlxr_fp8_matmul(M, N, K, rows, scales, w_dev, w_scale_dev, bias_dev, bias_dtype, y_dev, y_dtype, rest,
+                         workspace_bytes - (size_t)(rest - rows), stream);
+}

@@ -29,6 +29,8 @@ _SIGS = {
     "mlxr_quantize_fp8_weight": (_I, [_I, _I, _P, _I, _P, _P, _P]),
     "mlxr_fp8_matmul_workspace_size": (_I, [_I, _I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
     "mlxr_fp8_matmul": (_I, [_I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, ctypes.c_size_t, _P]),
+    "mlxr_fp8_linear_workspace_size": (_I, [_I, _I, _I, _I, ctypes.POINTER(ctypes.c_size_t)]),
+    "mlxr_fp8_linear": (_I, [_I, _I, _I, _P, _I, _I64, _P, _P, _P, _I, _P, _I, _P, ctypes.c_size_t, _P]),
     "mlxr_fp8_test_force": (_I, [_I, _I]),
 }
 _bound = None
@@ -162,50 +164,59 @@ def quantize_fp8_weight(w, stream=None):
 
 
 def fp8_matmul(x, w, bias=None, out=None, out_dtype=None, stream=None):
-    """x W^T (+ bias) with W an ``Fp8Weight`` [N, K] (mlxr_fp8_matmul).
+    """x W^T (+ bias) with W an ``Fp8Weight`` [N, K] (mlxr_fp8_matmul, mlxr_fp8_linear).
 
     x: ``Fp8Rows`` [M, K], or [..., K] in float16, bfloat16 or float32, which is rounded by ``quantize_fp8`` first.  Returns
     [M, N] ([..., N]) in x's dtype (of ``Fp8Rows`` bfloat16), ``out_dtype``, or in ``out``."""
     lib, torch = _bound or _lib(), paged._torch
     if not isinstance(w, Fp8Weight):
         raise QGemmError(-1, "fp8_matmul: w must be an Fp8Weight")
-    n, k, index = w.N, w.K, w.data.get_device()
-    if isinstance(x, Fp8Rows):
-        lead, default = x.data.shape[:-1], torch.bfloat16
+    n, k, wd = w.N, w.K, w.data
+    index = wd.get_device()
+    rows = isinstance(x, Fp8Rows)
+    if rows:
+        data, scales = x
+        lead, dtype = data.shape[:-1], torch.bfloat16
+        if data.dim() != 2 or data.shape[1] != k:
+            raise QGemmError(-3, f"Input shape must be [M, {k}]")
+        m = data.shape[0]
+        if data.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32 or data.get_device() != index or \
+                scales.get_device() != index or scales.shape != (m, -(-k // BLOCK)) or not data.is_contiguous() or \
+                not scales.is_contiguous():
+            raise QGemmError(-1, f"fp8_matmul: rows must be contiguous float8_e4m3fn [M, {k}] with float32 scales "
+                                 f"[M, {-(-k // BLOCK)}] on GPU {index}")
+        if data.data_ptr() % 16:
+            data = _on(stream, data.clone)
     else:
-        if x.dim() < 1 or x.shape[-1] != k:
+        shape, dtype = x.shape, x.dtype
+        if not shape or shape[-1] != k:
             raise QGemmError(-3, f"Input shape must be [..., {k}]")
         if x.get_device() != index:
             raise QGemmError(-1, "fp8_matmul: x must be on the weight's GPU")
-        lead, default = x.shape[:-1], x.dtype
-        x = quantize_fp8(x, stream=stream)
-    data, scales = x
-    if data.dim() != 2 or data.shape[1] != k:
-        raise QGemmError(-3, f"Input shape must be [M, {k}]")
-    m = data.shape[0]
-    if data.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32 or data.get_device() != index or \
-            scales.get_device() != index or scales.shape != (m, -(-k // BLOCK)) or not data.is_contiguous() or \
-            not scales.is_contiguous():
-        raise QGemmError(-1, f"fp8_matmul: rows must be contiguous float8_e4m3fn [M, {k}] with float32 scales "
-                             f"[M, {-(-k // BLOCK)}] on GPU {index}")
-    if data.data_ptr() % 16:
-        data = _on(stream, data.clone)
+        lead, xt = shape[:-1], _code(paged._x_codes, dtype, "x")
+        data, m, _, stride = _rows(x, index, "fp8_matmul: x", stream)
     pb, bt = None, 0
     if bias is not None:
         if bias.shape != (n,) or bias.get_device() != index or not bias.is_contiguous():
             raise QGemmError(-3, "Bias shape must be [N]")
         pb, bt = bias.data_ptr(), _code(paged._x_codes, bias.dtype, "bias")
     if out is None:
-        out = _on(stream, torch.empty, (*lead, n), dtype=out_dtype or default, device=data.device)
+        out = _on(stream, torch.empty, (*lead, n), dtype=out_dtype or dtype, device=wd.device)
     elif out.shape != (*lead, n) or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 16:
         raise QGemmError(-1, f"out must be a contiguous {[*lead, n]} tensor on GPU {index}, at a multiple of 16 bytes")
     yt = _code(paged._x_codes, out.dtype, "out")
-    nb = ctypes.c_size_t()
-    qgemm._check(lib.mlxr_fp8_matmul_workspace_size(m, n, k, yt, ctypes.byref(nb)))
-    nb = nb.value
-    ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=data.device) if nb else None
-    rc = lib.mlxr_fp8_matmul(m, n, k, data.data_ptr(), scales.data_ptr(), w.data.data_ptr(), w.scales.data_ptr(), pb, bt,
-                             out.data_ptr(), yt, ws.data_ptr() if nb else None, nb, _stream(stream, index))
+    size = ctypes.c_size_t()
+    rc = (lib.mlxr_fp8_matmul_workspace_size if rows else lib.mlxr_fp8_linear_workspace_size)(m, n, k, yt, ctypes.byref(size))
+    if rc:
+        qgemm._check(rc)
+    nb = size.value
+    ws = _on(stream, torch.empty, nb, dtype=torch.uint8, device=wd.device) if nb else None
+    rest = (wd.data_ptr(), w.scales.data_ptr(), pb, bt, out.data_ptr(), yt, ws.data_ptr() if nb else None, nb,
+            _stream(stream, index))
+    if rows:
+        rc = lib.mlxr_fp8_matmul(m, n, k, data.data_ptr(), scales.data_ptr(), *rest)
+    else:
+        rc = lib.mlxr_fp8_linear(m, n, k, data.data_ptr(), xt, stride, *rest)
     if rc:
         qgemm._check(rc)
     return out

@@ -407,6 +407,46 @@ def test_product_of_16_bit_rows_streams_and_graphs():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(1, 16, 16), (3, 100, 144), (16, 130, 4096), (7, 300, 400), (33, 5, 128), (100, 64, 28672), (600, 1040, 2048)])
+def test_product_of_rows_in_16_and_32_bits(m, n, k, kind):
+    """The same bits as quantize_fp8 and the product of its rows, values that are not finite included, of rows that lie apart and
+    of their copy; nothing behind or between the rows is seen."""
+    import torch
+    w = _weights(n, k, m)
+    room = torch.full((m + 3, k + 8), math.nan, device="cuda", dtype=_types()[kind])
+    x = room[:m, :k]
+    x.copy_(torch.randn((m, k), device="cuda", generator=_gen(k)) * 3)
+    x[0, :min(k, 128)] = 0
+    x[m // 2, k - 1] = 3e4
+    bias = torch.randn(n, device="cuda", generator=_gen(1))
+    for y in (x, x.contiguous(), x.reshape(1, m, k)):
+        for dtype in (torch.float32, torch.bfloat16):
+            got = mx.fp8_matmul(y, w, bias, out_dtype=dtype)
+            assert torch.equal(got.reshape(m, n), mx.fp8_matmul(mx.quantize_fp8(x), w, bias, out_dtype=dtype))
+    x[m - 1, k // 2] = math.nan
+    x[0, 1] = math.inf
+    got, want = mx.fp8_matmul(x, w), mx.fp8_matmul(mx.quantize_fp8(x), w, out_dtype=x.dtype)
+    assert torch.isnan(got[m - 1]).all() and torch.isnan(got[0]).all()
+    assert torch.equal(got.nan_to_num(1e4), want.nan_to_num(1e4))
+
+
+def test_linear_entry_refuses():
+    L, n = mx.fp8._lib(), ctypes.c_size_t()
+    P = ctypes.c_void_p
+
+    def call(M=2, N=64, K=64, x=64, xt=mx.BF16, w=64, ws=64, bias=0, bt=mx.F32, y=64, yt=mx.BF16, space=64, nb=1 << 20):
+        return L.mlxr_fp8_linear(M, N, K, P(x), xt, 64, P(w), P(ws), P(bias), bt, P(y), yt, P(space), nb, None)
+    assert call(M=-1) == -1 and call(K=0) == -1 and call(K=72) == -3 and call(yt=3) == -1 and call(xt=3) == -1
+    assert call(x=0) == -1 and call(w=0) == -1 and call(ws=0) == -1 and call(y=0) == -1 and call(bias=64, bt=3) == -1
+    assert call(w=72) == -3 and call(y=72) == -3 and call(space=72) == -3 and call(space=0) == -1 and call(nb=100) == -1
+    assert call(M=0, x=0, space=0, nb=0) == 0
+    assert L.mlxr_fp8_linear_workspace_size(2, 64, 64, mx.BF16, None) == -1
+    assert L.mlxr_fp8_linear_workspace_size(0, 64, 64, mx.BF16, ctypes.byref(n)) == 0 and n.value == 0
+    assert L.mlxr_fp8_linear_workspace_size(5, 64, 144, mx.BF16, ctypes.byref(n)) == 0 and n.value == 768 + 256
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n,k", [(64, 16), (128, 128), (300, 400), (1000, 1040)])
 def test_weights_to_eight_bits(n, k):
     import torch

@@ -17,10 +17,15 @@
 // A tile of TOK tokens goes memory -> registers -> LDS, one tile ahead: while tile t is multiplied, t + 1 is on its way to
 // registers; it is written to the other half of LDS before the tile's one barrier.
 //
+// What bounds it: few columns, memory (16 drafts of 32 rows of 8192, 32 heads and 8 kv heads of 128, bf16: 223 us, 4.9 TB/s); many
+// columns, the vector unit's work on each score beside the matrix unit's two products (64 drafts of 8 rows of 16384, 64 heads, e4m3
+// cache: 335 us, 0.82 PFLOP/s; a chain of 513 over 6001 tokens 0.43); a few rows, the launches and the start of each
+// workgroup (8 drafts of one row of 1000 16 us).
+//
 // The tiles of all (row, kv head, QB columns) are dealt to the workgroups of a launch that fills the device in equal
 // contiguous runs; a run that covers all of its columns' tiles writes the output, others leave (m, sum, unnormalized o) in
-// the workspace, at most two a workgroup, and a second launch joins them.  Short rows, or many: a workgroup for each
-// (row, kv head, QB columns).
+// the workspace, at most two a workgroup, and a second launch joins them.  Short rows, or many (plan_of): a workgroup for
+// each (row, kv head, QB columns).
 #pragma once
 #include <cfloat>
 #include <type_traits>
@@ -36,7 +41,7 @@ using paged::widen;
 
 constexpr int kThreads = 256;  // of the join and the masks
 constexpr int kMaxRows = MLXR_PAGED_MAX_ROWS;
-constexpr int kStart = 2;  // tiles that the start and the end of a row's columns are counted for
+constexpr int kStart = 2;  // tiles that the start and the end of a row's columns are counted for in the deal
 
 struct Args {
   const uint8_t *k, *v;  // element addresses in bytes
@@ -166,7 +171,8 @@ struct Kern {
   static constexpr int CG = F8 ? DT / 16 : DT / 8;            // and in memory
   static constexpr int R = THREADS / TOK;                     // threads that bring a token's key and value to LDS
   static constexpr int LR = R == 4 ? 2 : 3;
-  static constexpr int NL = CG / R > 0 ? CG / R : 1;          // loads of a thread, tile and store
+  static_assert(CG % R == 0, "a token's threads share its pieces evenly");
+  static constexpr int NL = CG / R;                           // loads of a thread, tile and store
   static constexpr int AHEAD = F8 || CW == 1 ? 3 : 2;         // steps that reads of LDS go before their products
   static constexpr int STORE = TOK * DT * 2;                  // bytes of a tile's keys or values in LDS
   static constexpr int LDS = 4 * STORE;
@@ -251,12 +257,14 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
     for (int r = tid; r <= a.rows; r += THREADS) a.prefix[r] = pre[r];
     if (tid == 0) a.prefix[a.rows + 1] = per;
   }
-  // workgroup id % 8 is the XCD: each takes neighbouring runs, which read the same keys and values
-  const int nb = (int)gridDim.x, x = (int)blockIdx.x & 7, each = nb >> 3, more = nb & 7;
-  const int w = x * each + min(x, more) + ((int)blockIdx.x >> 3);
+  if (total == 0) return;
+  // workgroup id % 8 is the XCD: each takes neighbouring runs, which read the same keys and values, and as many as any other
+  const int nb = min((int)gridDim.x, quotient(total + per - 1, per));
+  const int x = (int)blockIdx.x & 7, i = (int)blockIdx.x >> 3, each = nb >> 3, more = nb & 7;
+  if (i >= each + (x < more)) return;
+  const int w = x * each + min(x, more) + i;
   int64_t pos = (int64_t)w * per;
   const int64_t end = pos + per < total ? pos + per : total;
-  if (pos >= end) return;
   int lo = 0, hi = a.rows;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -613,10 +621,10 @@ struct TreeKern {
 };
 
 // The kernel for head_dim, about `columns` columns of a row, the longest row that the table holds and the type of the output.
-// Eight wavefronts share a tile where there are columns for them: half as many loads, widenings and LDS writes a column.  us, four
-// and eight: 64 drafts of 8 rows of 16384, e4m3, 365 and 333; of 8192, bf16, 164 and 147; a chain of 513 over 6001 131 and 124; but 64
-// drafts of 64 rows of 64 91 and 101, of 256 135 and 147.  Up to 64 columns, one group of 16 a wavefront: 16 drafts of 32 rows of
-// 8192 (64 columns) 226, two groups 359.
+// Eight wavefronts share a tile where there are columns for them and rows are long: half as many loads, widenings and LDS writes
+// a column, but half as many workgroups.  us, four and eight: 64 drafts of 8 rows of 16384, e4m3, 350 and 335; of 8192, bf16, 167 and
+// 142; of 32 rows of 500 58 and 51; a chain of 513 tokens 55 and 48; but 64 drafts of 8 rows of 256 27 and 34.  Up to 64
+// columns, one group of 16 a wavefront: 16 drafts of 32 rows of 8192 (64 columns) 226, two groups 359.
 TreeKern kern_bf16(int dim, int columns, int longest, int out_dtype);
 TreeKern kern_f16(int dim, int columns, int longest, int out_dtype);
 TreeKern kern_bf16_e4m3(int dim, int columns, int longest, int out_dtype);

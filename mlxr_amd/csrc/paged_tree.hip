@@ -142,7 +142,13 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), (int)held, out_dtype);
   p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
   const int64_t tiles = (held + p.k.tok - 1) / p.k.tok;
-  p.cut = tiles > 4 && p.units < 8 * device_cu_count();
+  // Cut where the longest rows that the table holds are more tiles than 16 for each of a CU's units: what a launch without cuts
+  // leaves idle while its longest unit ends grows with the row, the join with the units.  us, cut and not, 16 drafts a row
+  // of 32 heads and 8 kv heads, rows spread over the lengths: 32 rows (256 units) of up to 500 26 and 24, of 2000 43 and 61, of 8192 123
+  // and 211; 128 rows (1024 units) 56 and 47, 135 and 130, 389 and 457; of one length of 2000 32 rows 73 and 70, 128
+  // rows of 4096 408 and 391.  Up to two tiles: 12.4 and 10.3 for one row of 100.
+  const int64_t units = std::max((int64_t)tokens * group / p.k.qb, (int64_t)rows) * c->kv_heads;  // about
+  p.cut = tiles > 2 && 16 * units < tiles * device_cu_count();
   p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
   return p;
 }

@@ -413,12 +413,15 @@ class PagedKVCache:
         return self.resize(lens, 0, stream=stream)
 
     def fork(self, sources, tokens, stream=None):
-        """Rows whose ``sources`` [rows] (int32) names another row become copies of it; rows with -1 stay.  ``tokens``: at
+        """Rows whose ``sources`` [rows] (int32) names another row become copies of it; rows with -1 (or anything that is no row) stay.  ``tokens``: at
         least as many as are copied in all.  A row that becomes a copy must be empty (resize it to 0 before).  Returns
         ``Resized``; rows for which the pool had no pages are refused as by ``resize``."""
+        rows = self.lens.shape[0]
+        _vector(sources, rows, "sources", self.lens.get_device())
+
         def wanted():
-            at = sources.clamp(min=0).long()
-            return _torch.where(sources >= 0, self.lens[at], self.lens)
+            at = sources.clamp(0, rows - 1)
+            return _torch.where(at == sources, self.lens[at.long()], self.lens)
         grown = self.resize(_on(stream, wanted), tokens, stream=stream)
         paged_fork(self.k, self.v, self.table, sources, grown, stream=stream)
         return grown

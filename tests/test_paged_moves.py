@@ -231,6 +231,12 @@ def test_cache_forks_accepts_and_frees():
 
     append(c.resize(_i32([10, 0, 3, 0, 0]), 20), lambda r, t: 10 * r + t)
     check()
+    c.fork(_i32([0, 5, 2, -7, 1 << 30]), 30)  # itself, and no rows
+    check()
+    with pytest.raises(mx.QGemmError, match="sources"):
+        c.fork(_i32([-1, 0]), 30)
+    with pytest.raises(mx.QGemmError, match="sources"):
+        c.fork(_i32([-1] * 5).long(), 30)
     grown = c.fork(_i32([-1, 0, -1, 0, 2]), 30)
     assert c.lens.tolist() == [10, 10, 3, 10, 3] and grown.refused.item() == 0
     for r, s, n in ((1, 0, 10), (3, 0, 10), (4, 2, 3)):

@@ -245,6 +245,59 @@ def test_many_rows_and_long_chains():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f8"), ("f16", "f8")])
+@pytest.mark.parametrize("extra", [0, 500])  # rows of the table's length, many of its tiles empty
+def test_many_columns_of_long_rows(dtype, cache, extra):
+    """More than 128 columns of rows of more than 512 tokens: masks, a chain, values that are not finite, bad pages."""
+    import torch
+    rng = random.Random(extra)
+    context, drafts = [611, 1300, 0, 64], [40, 65, 130, 0]
+    b = Batch(context, drafts, 16, 2, 128, 16, dtype, cache, seed=12, extra=extra)
+    bits = []
+    for n in drafts:
+        bits += _tree(n, rng)[1]
+    for odt in ("f32", dtype):
+        b.check(*b.call(bits, 3, out_dtype=_dt(odt), return_lse=True), bits, 3, odt=odt, dtype=dtype)
+        b.check(*b.call(out_dtype=_dt(odt), return_lse=True), odt=odt, dtype=dtype)
+    want = b.call(bits, 3)
+    for node in (0, 17, 39):  # of row 0: NaN in a value, then in a key
+        at = b.context[0] + node
+        pg, t = int(b.table[0, at // 16]), at % 16
+        for store in (b.v, b.k):
+            keep = store[pg, 1, t].clone()
+            store[pg, 1, t, 77] = math.nan
+            got = b.call(bits, 3)
+            for i in range(40):
+                if bits[i] >> node & 1:
+                    cell = got[i, 8:, 77] if store is b.v else got[i, 8:]
+                    assert torch.isnan(cell).all()
+                    cell.copy_(want[i, 8:, 77] if store is b.v else want[i, 8:])
+            assert torch.equal(got, want)
+            store[pg, 1, t] = keep
+    b.table[1, :] = -1
+    got = b.call(bits, 3)
+    assert not got[40:105].any()
+    got[40:105] = want[40:105]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_as_many_rows_as_a_call_takes():
+    """MLXR_PAGED_MAX_ROWS rows, and about as many as are cut."""
+    import torch
+    rng = random.Random(1)
+    for rows, dim, extra in ((4096, 256, 0), (1900, 128, 480)):
+        b = Batch([rng.randrange(0, 30) for _ in range(rows)], [r % 3 for r in range(rows)], 2, 1, dim, 16, "bf16", "bf16", seed=13, extra=extra)
+        whole, lse = b.call(out_dtype=_dt("f32"), return_lse=True)
+        some = [0, 1, 2, 1047, rows - 2, rows - 1]
+        c = Batch([1] * 6, [b.drafts[r] for r in some], 2, 1, dim, 16, "bf16", "bf16", seed=13)
+        c.k, c.v, c.table, c.lens, c.context = b.k, b.v, b.table[some], [b.lens[r] for r in some], [b.context[r] for r in some]
+        c.q = torch.cat([b.q[b.starts[r]:b.starts[r + 1]] for r in some] + [b.q[-2:]])
+        c.check(torch.cat([whole[b.starts[r]:b.starts[r + 1]] for r in some] + [whole[-2:]]),
+                torch.cat([lse[b.starts[r]:b.starts[r + 1]] for r in some] + [lse[-2:]]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("extra", [0, 200])  # one launch; cut
 @pytest.mark.parametrize("dtype,heads,kv,dim", [("bf16", 8, 2, 128), ("f16", 16, 1, 64), ("bf16", 2, 2, 256)])
 def test_masks_of_any_shape(dtype, heads, kv, dim, extra):

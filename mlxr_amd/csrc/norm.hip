@@ -278,7 +278,7 @@ void launch_norm(const NormArgs& a, bool wide, hipStream_t s) {
   if (K <= 128) return launch_rows<XT, 16, 1>(a, s);
   if (K <= 256) return launch_rows<XT, 32, 1>(a, s);
   if (K <= 512) return launch_rows<XT, 64, 1>(a, s);
-  if (K <= 1024) return launch_rows<XT, 64, 2>(a, s);
+  if (K <= 1024) return launch_rows<XT, 128, 1>(a, s);
   if (K <= 2048) return launch_rows<XT, 256, 1>(a, s);
   if (K <= 4096) return a.rows >= 4 * device_cu_count() ? launch_rows<XT, 256, 2>(a, s) : launch_rows<XT, 512, 1>(a, s);
   if (K <= 8192) return launch_rows<XT, 1024, 1>(a, s);

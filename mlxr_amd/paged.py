@@ -277,7 +277,7 @@ def paged_tree_attention(q, k_store, v_store, table, lens, starts, mask=None, sc
         pm, words = mask.data_ptr(), mask.shape[1]
     dt = _code(_x_codes, q.dtype, "queries")
     if out is None:
-        out = _on(stream, _torch.empty, shape, dtype=out_dtype or q.dtype, device=q.device)
+        out = _on(stream, _torch.empty_like, q, dtype=out_dtype, memory_format=_torch.contiguous_format)
     elif out.shape != shape or not out.is_contiguous() or out.get_device() != index:
         raise QGemmError(-1, f"out must be a contiguous [{tokens}, {heads}, {dim}] tensor on GPU {index}")
     odt = _code(_x_codes, out.dtype, "out")

@@ -3,7 +3,7 @@
 // copied bit for bit, so one kernel serves every cache type: 16 bytes a lane.
 //
 // Bound by memory: each byte moved is read once and written once.  64 rows of Llama-3-8B's 32 layers (8 heads of 128, bf16),
-// paths of up to 6 of 16 drafted tokens (37 MB read and written): 8 us, 4.6 TB/s; a row of 1501 tokens to three others
+// paths of up to 6 of 16 drafted tokens (37 MB read and written): 10 us, 3.7 TB/s; a row of 1501 tokens to three others
 // (787 MB): 157 us, 5 TB/s.
 #include "mfma16.h"
 #include "paged_internal.h"

@@ -407,11 +407,13 @@ struct Plan {
 constexpr int kMaxSplits = 16;
 // Up to 16 rows the weights are streamed, above the kernel and split with the shortest time by a model: rounds of
 // workgroups times blocks of K times the time of a block's step, no less than the weights at the rate at which a kernel
-// streams them (TB/s), and the reduce (3 us and its fp32 partial sums at 4.5 TB/s).
+// streams them (TB/s), and the reduce (3 us and its fp32 partial sums at 4.5 TB/s).  The kernels of few rows split K over their
+// wavefronts, need no reduce and start quickly: they serve small products of more rows too.
 // us of a step measured where a workgroup is alone on its CU (two of 64 x 128 fit, which then take 1.5).  us, the best
-// of all kernels and splits and the model's choice: 32 x 14336 x 4096 16.1 and 16.1; 61 x 28672 x 8192 55.4 and 55.4; 64 x 8192
-// x 8192 21.1 and 21.1; 100 x 14336 x 4096 23 and 23; 128 x 28672 x 8192 72 and 72; 256 x 8192 x 8192 36 and 36; 512 x 14336 x 4096
-// 51 and 51; 1024 x 4096 x 4096 30 and 30; 2048 x 14336 x 4096 137 and 137; 2048 x 4096 x 4096 44 and 44.  256 x 256
+// of all kernels and splits and the model's choice: 64 x 1024 x 4096 5.1 and 5.2 (of the tiles 8.3); 48 x 4096 x 1024 4.9 and 4.9
+// (6.0); 128 x 1024 x 4096 7.1 and 7.1 (9.5); 32 x 14336 x 4096 16 and 16; 61 x 28672 x 8192 57 and 57; 64 x 8192 x 8192 21 and 21;
+// 128 x 28672 x 8192 76 and 76; 256 x 8192 x 8192 41 and 41; 300 x 1024 x 4096 12.7 and 13.7; 512 x 14336 x 4096 51 and 51;
+// 1024 x 4096 x 4096 29 and 29; 2048 x 14336 x 4096 137 and 137; 2048 x 4096 x 4096 44 and 44.  256 x 256
 // and 128 x 256 have no WIDE form (registers).
 Plan plan_of(int M, int N, int K, bool wide) {
   const int blocks = (K + kK - 1) / kK, cus = device_cu_count();
@@ -421,7 +423,7 @@ Plan plan_of(int M, int N, int K, bool wide) {
     int bm, bn;
     double step, rate;
   };
-  static const Tiles tiles[] = {{TILE32x64, 32, 64, 0.48, 4.5}, {TILE64x128, 64, 128, 0.8, 4.4}, {TILE128x128, 128, 128, 0.95, 2.9},
+  static const Tiles tiles[] = {{TILE32x64, 32, 64, 0.48, 4.5}, {TILE64x128, 64, 128, 0.8, 4.4}, {TILE128x128, 128, 128, 1.1, 2.9},
                                 {TILE128x256, 128, 256, 1.5, 4}, {TILE256x256, 256, 256, 2.1, 4}};
   const int forced = g_kind.load(std::memory_order_relaxed), splits = g_splits.load(std::memory_order_relaxed);
   if (forced != AUTO) {
@@ -430,9 +432,13 @@ Plan plan_of(int M, int N, int K, bool wide) {
     p.splits = p.kind >= TILE32x64 ? std::max(1, std::min(splits, blocks)) : 1;
   } else if (M > 16) {
     double best = 1e30;
-    if (M <= 32) {
-      p.kind = SKINNY32;
-      best = (double)((N + 32 * cus - 1) / (32 * cus)) * (3 + 0.2 * blocks);
+    if (M <= 1024) {
+      const int m16 = (M + 15) / 16, m32 = (M + 31) / 32;  // each reads the weights
+      const int64_t n16 = (int64_t)((N + 15) / 16) * m16, n32 = (int64_t)((N + 31) / 32) * m32;
+      const double step16 = n16 <= cus ? 0.4 + 0.075 * blocks : (double)((n16 + 2 * cus - 1) / (2 * cus)) * (1 + 0.137 * blocks);
+      const double us16 = 1.9 + std::max(step16, 1e-6 / 7 * m16 * N * K);
+      const double us32 = 1.2 + std::max((double)((n32 + cus - 1) / cus) * (2.3 + 0.13 * blocks), 1e-6 / 3.3 * m32 * N * K);
+      p.kind = us16 < us32 ? SKINNY16 : SKINNY32, best = std::min(us16, us32);
     }
     for (const Tiles& t : tiles) {
       if (wide && t.kind > TILE128x128) break;

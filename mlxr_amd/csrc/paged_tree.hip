@@ -1,6 +1,7 @@
 // Attention of drafted tokens over a paged cache: the C entries, the join of the pieces that the kernel (paged_tree.h)
 // leaves of cut rows, and the masks of trees.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_tree.h"
 
@@ -10,7 +11,9 @@ namespace {
 
 // One token's head for each `lanes` threads, four dims a thread: o = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w over the
 // workgroups w that had a piece of its columns, M the maximum of their m (-inf: no token counted).  Rows without
-// tokens get zeros; columns that one workgroup covered are done.
+// tokens get zeros; columns that one workgroup covered are done.  Four pieces are on their way at
+// once, MANY: 16 where there are more.
+template <bool MANY>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
   extern __shared__ int starts[];  // [rows + 1]: searched in LDS
   const int tid = threadIdx.x, x = tid & (lanes - 1);
@@ -38,8 +41,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
     const int64_t s = a.prefix[lo] + ((int64_t)kvh * row.blocks + block) * (row.tiles + kStart);
     const int w0 = quotient(s + kStart, per), w1 = quotient(s + kStart + row.tiles - 1, per);
     if (w0 == w1) return;
-    constexpr int N = 4;  // pieces on their way at once
-    for (int w = w0; w <= w1; w += N) {
+    auto take = [&](int w, auto pieces) {
+      constexpr int N = decltype(pieces)::value;
       float pm[N], pl[N];
       f32x4_t po[N];
 #pragma unroll
@@ -66,7 +69,11 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += po[k][e] * f;
       }
-    }
+    };
+    int w = w0;
+    if constexpr (MANY)
+      for (; w + 3 < w1; w += 16) take(w, std::integral_constant<int, 16>());
+    for (; w <= w1; w += 4) take(w, std::integral_constant<int, 4>());
   }
   const float f = m == -INFINITY ? 0.f : l == 0.f ? NAN : (a.v_scale ? a.v_scale[kvh] : 1.f) / l;
   const float v[4] = {o[0] * f, o[1] * f, o[2] * f, o[3] * f};
@@ -137,18 +144,23 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   Plan p;
   const int group = heads / c->kv_heads;
   // on average, padding included; an eighth more than a block of columns is still taken as one
-  const int64_t columns = (int64_t)tokens * group / rows * 8 / 9;
+  int64_t columns = (int64_t)tokens * group / rows * 8 / 9;
   const int64_t held = (int64_t)width * c->page_size;
+  // Little work (tiles of 16 columns by 64 tokens, for a CU) wants many workgroups rather than few reads of a tile: us, wide kernels
+  // and the one of 64 columns, 64 drafts of 8 rows of 256, 32 heads and 8 kv heads (16) 27 and 17, a chain of 513 (36) 48 and 44, 145 of 8 rows of
+  // up to 1806, 8 heads and 2 (70) 35 and 30; but 64 of 16 rows of up to 500, 64 heads and 8 (144) 36 and 39, of 32 rows of 500, 32
+  // heads and 8 (144) 51 and 63.
+  if ((double)tokens * group / 16 * c->kv_heads * ((held + 63) / 64) < 96.0 * device_cu_count()) columns = std::min<int64_t>(columns, 64);
   p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), (int)held, out_dtype);
   p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
   const int64_t tiles = (held + p.k.tok - 1) / p.k.tok;
-  // Cut where the longest rows that the table holds are more tiles than 16 for each of a CU's units: what a launch without cuts
-  // leaves idle while its longest unit ends grows with the row, the join with the units.  us, cut and not, 16 drafts a row
-  // of 32 heads and 8 kv heads, rows spread over the lengths: 32 rows (256 units) of up to 500 26 and 24, of 2000 43 and 61, of 8192 123
-  // and 211; 128 rows (1024 units) 56 and 47, 135 and 130, 389 and 457; of one length of 2000 32 rows 73 and 70, 128
-  // rows of 4096 408 and 391.  Up to two tiles: 12.4 and 10.3 for one row of 100.
+  // Cut where the longest rows that the table holds are more than 3 tiles and 20 for each of a CU's units: what a launch without cuts
+  // leaves idle while its longest unit ends grows with the row, the pieces and their join with the units.  us, cut and not, 16
+  // drafts a row of 32 heads and 8 kv heads: one row (8 units) of 250 13.1 and 15.5, 8 rows of 250 21.8 and 16.8, of 1000 26 and 34; rows
+  // spread over the lengths, 32 rows (256 units) of up to 500 26 and 24, of 2000 43 and 61, of 8192 123 and 211; 128 rows (1024 units) 56
+  // and 47, 135 and 130, 389 and 457; of one length of 2000 32 rows 73 and 70, 128 rows of 4096 408 and 391.
   const int64_t units = std::max((int64_t)tokens * group / p.k.qb, (int64_t)rows) * c->kv_heads;  // about
-  p.cut = tiles > 2 && 16 * units < tiles * device_cu_count();
+  p.cut = (tiles - 3) * device_cu_count() > 20 * units;
   p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
   return p;
 }
@@ -258,8 +270,11 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   if (e == hipSuccess && p.cut) {
     int lanes = 2;
     while (4 * lanes < a.dim) lanes *= 2;
-    const int64_t of = kThreads / lanes;
-    join_kernel<<<(unsigned)(((int64_t)tokens * heads + of - 1) / of), kThreads, (rows + 1) * sizeof(int), st>>>(a, lanes);
+    const unsigned blocks = (unsigned)(((int64_t)tokens * heads * lanes + kThreads - 1) / kThreads);
+    // A few workgroups wait for memory: more at once, though fewer fit a CU.  us of a call, 4 and 16: 8 drafts of one row of 1000 16.3
+    // and 13.9, 76 of 3 rows of up to 7391, 4 heads of 256 44 and 35; 64 of 8 rows of 8192 142 and 148.
+    const auto join = blocks <= 2 * (unsigned)device_cu_count() ? join_kernel<true> : join_kernel<false>;
+    join<<<blocks, kThreads, (rows + 1) * sizeof(int), st>>>(a, lanes);
     e = hipGetLastError();
   }
   if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention launch: %s", hipGetErrorString(e));

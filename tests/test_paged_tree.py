@@ -282,6 +282,40 @@ def test_many_columns_of_long_rows(dtype, cache, extra):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache,dim", [("bf16", "bf16", 128), ("f16", "f16", 112), ("bf16", "f8", 128), ("f16", "f8", 64), ("bf16", "bf16", 64)])
+@pytest.mark.parametrize("pages,extra", [(30, 0), (36, 0), (36, 700)])  # tiles shared by four and eight wavefronts, cut rows
+def test_many_rows_of_wide_trees(dtype, cache, dim, pages, extra):
+    import torch
+    rng = random.Random(pages)
+    rows = 60
+    drafts = [rng.randrange(56, 65) for _ in range(rows)]
+    context = [rng.randrange(0, 16 * pages - 64) for _ in range(rows)]
+    drafts[7], drafts[30], context[9], context[10] = 0, 1, 0, 16 * pages - drafts[10]
+    b = Batch(context, drafts, 16, 2, dim, 16, dtype, cache, seed=14, extra=extra)
+    bits = []
+    for n in drafts:
+        bits += _tree(n, rng)[1]
+    b.check(*b.call(bits, 1, out_dtype=_dt("f32"), return_lse=True), bits, 1, dtype=dtype)
+    b.check(*b.call(bits, 1, return_lse=True), bits, 1, odt=dtype, dtype=dtype)
+    b.check(*b.call(out_dtype=_dt("f32"), return_lse=True), dtype=dtype)
+    want = b.call(bits, 1)
+    a, c = b.starts[20], b.context[20]
+    for node in (0, 50):
+        pg, t = int(b.table[20, (c + node) // 16]), (c + node) % 16
+        for store in (b.v, b.k):
+            keep = store[pg, 1, t].clone()
+            store[pg, 1, t, 3] = math.nan
+            got = b.call(bits, 1)
+            for i in range(drafts[20]):
+                if bits[a + i] >> node & 1:
+                    cell = got[a + i, 8:, 3] if store is b.v else got[a + i, 8:]
+                    assert torch.isnan(cell).all()
+                    cell.copy_(want[a + i, 8:, 3] if store is b.v else want[a + i, 8:])
+            assert torch.equal(got, want)
+            store[pg, 1, t] = keep
+
+
+@pytest.mark.gpu
 def test_as_many_rows_as_a_call_takes():
     """MLXR_PAGED_MAX_ROWS rows, and about as many as are cut."""
     import torch

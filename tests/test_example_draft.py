@@ -131,3 +131,109 @@ def test_layers_with_8_bit_weights(cuda, shape):
     assert mlp(x).shape == x.shape
     with pytest.raises(mx.QGemmError):
         mlp(x8)
+
+
+@pytest.mark.gpu
+def test_a_captured_pass_follows_its_inputs(cuda):
+    """A whole pass (pages, masks, layers, accepted paths, a fork) captured once and replayed with other lengths, trees, tokens and
+    paths, the program's own calls in between, gives the bits of the same calls made one by one."""
+    import random
+
+    import torch
+    ex = _example()
+    model = ex.Model(cuda)
+    rng = random.Random(5)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    inputs = {"want": i32([0] * ex.ROWS), "tokens": torch.zeros(ex.TOKENS, dtype=torch.int64, device=cuda),
+              "parents": i32([-1] * ex.TOKENS), "path": i32([[-1] * ex.DEPTH] * ex.ROWS), "counts": i32([0] * ex.ROWS),
+              "sources": i32([-1] * ex.ROWS)}
+
+    def one(cache):
+        grown = cache.resize(inputs["want"], ex.TOKENS)
+        logits = ex.step(model, cache, inputs["tokens"], inputs["parents"], grown)
+        kept = cache.accept(grown, inputs["path"], inputs["counts"])
+        forked = cache.fork(inputs["sources"], ex.TOKENS)
+        return grown.starts, logits, kept.lens, forked.refused
+
+    def new():
+        c = mx.PagedKVCache(ex.LAYERS, ex.PAGES, ex.PAGE, ex.KV, ex.DIM, ex.ROWS, ex.LONGEST, device=cuda)
+        c.k.zero_(), c.v.zero_()
+        return c
+    eager, held = new(), new()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one(new())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = one(held)
+    lens = [0] * ex.ROWS
+    for step in range(6):
+        n = [rng.randrange(0, 20) for _ in lens]
+        if step == 3:
+            lens, n[1], n[2] = [lens[0], 0, 0, lens[3]], 0, 0  # rows 1 and 2 end, and become copies
+        want = [a + b for a, b in zip(lens, n)]
+        parents, path, counts = [], [], []
+        for m in n:
+            parents += [rng.randrange(-1, i) if i else -1 for i in range(m)]
+            kept = sorted(rng.sample(range(m), rng.randrange(0, m + 1)))
+            path.append(kept + [-1] * (ex.DEPTH - len(kept))), counts.append(len(kept))
+        inputs["want"].copy_(i32(want)), inputs["path"].copy_(i32(path)), inputs["counts"].copy_(i32(counts))
+        inputs["parents"].copy_(i32(parents + [-1] * (ex.TOKENS - len(parents))))
+        inputs["tokens"].copy_(torch.randint(0, ex.VOCAB, (ex.TOKENS,), device=cuda))
+        inputs["sources"].copy_(i32([-1, 0, 3, -1] if step == 3 else [-1, 9, 2, -5]))
+        want_out = [t.clone() for t in one(eager)]
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want_out, captured):
+            assert torch.equal(a, b), step
+        for t in ("lens", "table", "free_count"):
+            assert torch.equal(getattr(eager, t), getattr(held, t)), (step, t)
+        lens = [a + c for a, c in zip(lens, counts)]
+        if step == 3:
+            lens[1], lens[2] = lens[0], lens[3]
+        assert eager.lens.tolist() == lens
+
+
+@pytest.mark.gpu
+def test_calls_of_several_threads_at_once(cuda):
+    """Each thread's own stream, inputs and outputs; the library keeps nothing between calls that others could see."""
+    import threading
+
+    import torch
+    g = torch.Generator(device=cuda).manual_seed(3)
+    rnd = lambda *s: torch.randn(s, device=cuda, generator=g)  # noqa: E731
+    work = []
+    for i, (m, n, k) in enumerate([(5, 512, 1024), (90, 4096, 2048), (40, 256, 8192)]):
+        w, x, res = mx.quantize_fp8_weight(rnd(n, k)), rnd(m, k).bfloat16(), rnd(m, k).bfloat16()
+        kc, vc = rnd(64 * (i + 1), 2, 16, 128).bfloat16(), rnd(64 * (i + 1), 2, 16, 128).bfloat16()
+        rows = 2 * (i + 1)
+        table = torch.randperm(64 * (i + 1), device=cuda, generator=g).to(torch.int32).view(rows, 32)
+        lens = torch.full((rows,), 400 + 30 * i, dtype=torch.int32, device=cuda)
+        starts = torch.arange(0, 7 * rows + 1, 7, dtype=torch.int32, device=cuda)
+        q = rnd(7 * rows, 8, 128).bfloat16()
+        work.append((w, x, res, kc, vc, table, lens, starts, q))
+
+    def run(job, stream):
+        w, x, res, kc, vc, table, lens, starts, q = job
+        h, total = mx.rms_norm(x, residual=res, quantize=True, stream=stream)
+        return [h.data.view(torch.uint8), h.scales, total, mx.fp8_matmul(h, w, stream=stream), mx.fp8_matmul(x, w, stream=stream),
+                *mx.paged_tree_attention(q, kc, vc, table, lens, starts, return_lse=True, stream=stream)]
+    wants = [run(job, None) for job in work]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def loop(i):
+        stream = torch.cuda.Stream()
+        for _ in range(30):
+            got = run(work[i], stream)
+            stream.synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, wants[i])):
+                wrong.append(i)
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

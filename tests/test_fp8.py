@@ -457,3 +457,18 @@ def test_weights_to_eight_bits(n, k):
     assert torch.equal(q.scales, top / torch.full_like(top, TOP))
     want = (b / q.scales[:, None, :, None]).to(torch.float8_e4m3fn).view(-(-n // BLOCK) * BLOCK, -1)[:n, :k]
     assert torch.equal(q.data.view(torch.uint8), want.contiguous().view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    import torch
+    w = _weights(130, 144, 1)
+    for shape in ((0, 144), (3, 0, 144)):
+        x = torch.zeros(shape, device="cuda", dtype=torch.bfloat16)
+        assert mx.rms_norm(x).shape == shape and mx.rms_norm(x, residual=x)[1].shape == shape
+        q = mx.quantize_fp8(x)
+        assert q.data.shape == (0, 144) and q.scales.shape == (0, 2)
+        assert mx.fp8_matmul(x, w).shape == (*shape[:-1], 130) and mx.fp8_matmul(q, w).shape == (0, 130)
+        assert mx.Linear(144, 130).load_weight(w)(x).shape == (*shape[:-1], 130)
+    strided = torch.zeros((0, 300), device="cuda", dtype=torch.float16)[:, :144]
+    assert mx.fp8_matmul(strided, w, out_dtype=torch.float32).shape == (0, 130)

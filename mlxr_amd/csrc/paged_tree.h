@@ -217,6 +217,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
   const bool cut = a.ws != nullptr;
   // a unit of the deal: kStart places, then its tiles
   auto weight = [&](const Row& w) { return (int64_t)a.kv_heads * w.blocks * (!cut ? 1 : w.tiles ? w.tiles + kStart : 0); };
+  const int behind = min(max(a.starts[a.rows], 0), a.tokens);  // the first token behind the rows
   {
     const int per_thread = (a.rows + THREADS - 1) / THREADS;
     const int r0 = min(tid * per_thread, a.rows), r1 = min(r0 + per_thread, a.rows);
@@ -232,24 +233,23 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
     __syncthreads();
     int64_t at = sum - n;
     for (int w = 0; w < wave; ++w) at += part[w];
+    if (tid == THREADS - 1) pre[a.rows] = at + n;
     for (int r = r0; r < r1; ++r) {
       pre[r] = at;
-      at += weight(row_of(a, r));
+      if (r + 1 < r1) at += weight(row_of(a, r));  // a thread of one row does not ask for it again
     }
-    if (tid == THREADS - 1) pre[a.rows] = at;
     __syncthreads();
   }
   // tokens behind the last row's: zeros
   {
-    const int from = min(max(a.starts[a.rows], 0), a.tokens);
-    const int64_t first = (int64_t)from * a.heads * a.dim, count = (int64_t)(a.tokens - from) * a.heads * a.dim;
+    const int64_t first = (int64_t)behind * a.heads * a.dim, count = (int64_t)(a.tokens - behind) * a.heads * a.dim;
     const int64_t id = (int64_t)blockIdx.x * THREADS + tid, step = (int64_t)gridDim.x * THREADS;
     for (int64_t i = id; i < count / 8; i += step) {
       const float z[8] = {0, 0, 0, 0, 0, 0, 0, 0};
       store_values<8>(a.out, a.out_dtype, first + 8 * i, z);
     }
     if (a.lse)
-      for (int64_t i = id; i < (int64_t)(a.tokens - from) * a.heads; i += step) a.lse[(int64_t)from * a.heads + i] = -INFINITY;
+      for (int64_t i = id; i < (int64_t)(a.tokens - behind) * a.heads; i += step) a.lse[(int64_t)behind * a.heads + i] = -INFINITY;
   }
   const int64_t total = pre[a.rows];
   const int64_t per = cut ? (total + a.workers - 1) / a.workers : 1;

@@ -20,7 +20,7 @@
 // What bounds it: few columns, memory (16 drafts of 32 rows of 8192, 32 heads and 8 kv heads of 128, bf16: 223 us, 4.9 TB/s); many
 // columns, the vector unit's work on each score beside the matrix unit's two products (64 drafts of 8 rows of 16384, 64 heads, e4m3
 // cache: 335 us, 0.82 PFLOP/s; a chain of 513 over 6001 tokens 0.43); a few rows, the launches and the start of each
-// workgroup (8 drafts of one row of 1000 16 us).
+// workgroup (8 drafts of one row of 1000 14 us).
 //
 // The tiles of all (row, kv head, QB columns) are dealt to the workgroups of a launch that fills the device in equal
 // contiguous runs; a run that covers all of its columns' tiles writes the output, others leave (m, sum, unnormalized o) in

@@ -10,6 +10,7 @@
 // Bound by memory for many rows (2048 of 8192, bf16 with the residual, to 8 bits: 118 MB in 24 us, 4.9 TB/s), by the launch and one
 // round trip for few (one row of 4096 2.7 us).
 #include <algorithm>
+#include <type_traits>
 #include <cfloat>
 
 #include "../../include/mlxr_fp8.h"
@@ -35,10 +36,22 @@ struct NormArgs {
 template <int XT>
 struct Row8 {  // eight elements as they lie in memory
   uint4 w[XT == DT_F32 ? 2 : 1];
-  __device__ __forceinline__ void load(const void* p, int64_t at) {
-    const uint4* q = (const uint4*)((const uint8_t*)p + at * (XT == DT_F32 ? 4 : 2));
+  // ANY: at any element's address (the loads are as wide all the same), the row's last n where that is less than eight, then zeros.
+  template <bool ANY>
+  __device__ __forceinline__ void load(const void* p, int64_t at, int n) {
+    typedef std::conditional_t<XT == DT_F32, uint32_t, uint16_t> Element;
+    if constexpr (!ANY) {
+      const uint4* q = (const uint4*)((const uint8_t*)p + at * (XT == DT_F32 ? 4 : 2));
 #pragma unroll
-    for (int i = 0; i < (XT == DT_F32 ? 2 : 1); ++i) w[i] = q[i];
+      for (int i = 0; i < (XT == DT_F32 ? 2 : 1); ++i) w[i] = q[i];
+    } else if (const Element* q = (const Element*)p + at; n >= 8) {
+      __builtin_memcpy(w, q, sizeof w);
+    } else {
+      Element t[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = e < n ? q[e] : (Element)0;
+      __builtin_memcpy(w, t, sizeof w);
+    }
   }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[XT == DT_F32].x, w[XT == DT_F32].y, w[XT == DT_F32].z, w[XT == DT_F32].w};
@@ -47,8 +60,15 @@ struct Row8 {  // eight elements as they lie in memory
       v[k] = XT == DT_F32 ? __builtin_bit_cast(float, u[k]) : unpack<XT == DT_F16>(u[k / 2], k & 1);
   }
 };
-__device__ __forceinline__ void store8(void* p, int dtype, int64_t at, const float (&v)[8]) {
-  if (dtype == DT_F32) {
+template <bool ANY>
+__device__ __forceinline__ void store8(void* p, int dtype, int64_t at, const float (&v)[8], int n) {
+  if (ANY && n < 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) store_scalar(p, dtype, at + e, v[e]);
+  } else if (ANY && dtype == DT_F32) {
+    __builtin_memcpy((float*)p + at, v, sizeof v);
+  } else if (dtype == DT_F32) {
     f32x4_t* o = (f32x4_t*)((float*)p + at);
     o[0] = f32x4_t{v[0], v[1], v[2], v[3]};
     o[1] = f32x4_t{v[4], v[5], v[6], v[7]};
@@ -56,7 +76,8 @@ __device__ __forceinline__ void store8(void* p, int dtype, int64_t at, const flo
     u32x4_t o;
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[k] = dtype == DT_F16 ? pack2<true>(v[2 * k], v[2 * k + 1]) : pack2<false>(v[2 * k], v[2 * k + 1]);
-    *(u32x4_t*)((uint16_t*)p + at) = o;
+    if constexpr (ANY) __builtin_memcpy((uint16_t*)p + at, &o, sizeof o);
+    else *(u32x4_t*)((uint16_t*)p + at) = o;
   }
 }
 
@@ -74,8 +95,8 @@ __device__ __forceinline__ float eight_bits(float (&v)[8], uint2* out) {
 }
 
 // LANES of a row (16 .. 1024, within a wavefront up to 64), CH chunks of eight elements a lane.  A workgroup is one row, or
-// 256 / LANES rows.
-template <int XT, int LANES, int CH, bool EIGHT>
+// 256 / LANES rows.  ANY: rows of any length, stride and address.
+template <int XT, int LANES, int CH, bool EIGHT, bool ANY>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_kernel(NormArgs a) {
   constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES, WAVES = LANES / 64;
   __shared__ float part[LANES > 64 ? THREADS / 64 : 1];
@@ -89,8 +110,8 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_kernel(NormArg
   for (int c = 0; c < CH; ++c) {
     const int k = 8 * (c * LANES + x);
     if (k < a.K) {
-      raw[c].load(a.x, r * a.x_stride + k);
-      if (a.res) res[c].load(a.res, r * a.res_stride + k);
+      raw[c].template load<ANY>(a.x, r * a.x_stride + k, a.K - k);
+      if (a.res) res[c].template load<ANY>(a.res, r * a.res_stride + k, a.K - k);
     }
   }
   float sq = 0.f;
@@ -105,7 +126,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_kernel(NormArg
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[c][e] += u[e];
       }
-      if (a.sum && mine) store8(a.sum, XT, r * a.K + k, v[c]);
+      if (a.sum && mine) store8<ANY>(a.sum, XT, r * a.K + k, v[c], a.K - k);
 #pragma unroll
       for (int e = 0; e < 8; ++e) sq = __builtin_fmaf(v[c][e], v[c][e], sq);
     } else {
@@ -135,15 +156,15 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_kernel(NormArg
         for (int e = 0; e < 8; ++e) w[e] = 1.f;
       } else if (a.weight_dtype == DT_F32) {
         Row8<DT_F32> q;
-        q.load(a.weight, k);
+        q.template load<ANY>(a.weight, k, a.K - k);
         q.get(w);
       } else if (a.weight_dtype == DT_F16) {
         Row8<DT_F16> q;
-        q.load(a.weight, k);
+        q.template load<ANY>(a.weight, k, a.K - k);
         q.get(w);
       } else {
         Row8<DT_BF16> q;
-        q.load(a.weight, k);
+        q.template load<ANY>(a.weight, k, a.K - k);
         q.get(w);
       }
 #pragma unroll
@@ -157,16 +178,25 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_kernel(NormArg
       uint2 q;
       const float scale = eight_bits(v[c], &q);  // all lanes: those past K hold zeros
       if (mine && k < a.K) {
-        *(uint2*)((uint8_t*)a.out + r * a.K + k) = q;
+        uint8_t* o = (uint8_t*)a.out + r * a.K + k;
+        if (!ANY) {
+          *(uint2*)o = q;
+        } else if (a.K - k >= 8) {
+          __builtin_memcpy(o, &q, sizeof q);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < a.K - k) o[e] = (uint8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+        }
         if ((x & 15) == 0) a.scales[r * a.blocks + (k >> 7)] = scale;
       }
     } else if (mine && k < a.K) {
-      store8(a.out, a.out_dtype, r * a.K + k, v[c]);
+      store8<ANY>(a.out, a.out_dtype, r * a.K + k, v[c], a.K - k);
     }
   }
 }
 
-// Rows of any length, stride and address: a workgroup a row, element by element, read twice (a wavefront takes blocks of 128
+// Rows that registers do not hold, of any length, stride and address: a workgroup a row, element by element, read twice (a wavefront takes blocks of 128
 // by turns in the second pass).  s is formed again there, from x and the residual: sum_dev may be either of them, so it is
 // written in that pass, each element by the lane that has just read it.
 template <int XT>
@@ -246,7 +276,7 @@ __global__ __launch_bounds__(256) void weight_kernel(const void* w, int N, int K
   }
 }
 
-template <int XT, int LANES, int CH>
+template <int XT, int LANES, int CH, bool ANY = false>
 void launch_rows(const NormArgs& a, hipStream_t s) {
   constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
   constexpr int MOST = (1 << 20) * ROWS;  // rows of a launch, which has fewer than 2^32 threads
@@ -260,20 +290,28 @@ void launch_rows(const NormArgs& a, hipStream_t s) {
     b.out = (uint8_t*)a.out + r0 * a.K * os;
     if (a.scales) b.scales = a.scales + r0 * a.blocks;
     const unsigned grid = (unsigned)((b.rows + ROWS - 1) / ROWS);
-    if (a.out_dtype == MLXR_E4M3) norm_kernel<XT, LANES, CH, true><<<grid, THREADS, 0, s>>>(b);
-    else norm_kernel<XT, LANES, CH, false><<<grid, THREADS, 0, s>>>(b);
+    if (a.out_dtype == MLXR_E4M3) norm_kernel<XT, LANES, CH, true, ANY><<<grid, THREADS, 0, s>>>(b);
+    else norm_kernel<XT, LANES, CH, false, ANY><<<grid, THREADS, 0, s>>>(b);
   }
 }
 
 // Lanes of a row: as many as take it with one load each, up to 1024, so that all its loads are on their way at once: half as
 // many take 3.3 us for one row of 4096 (2.7), 5.6 for one of 8192 (3.7), 25 for 2048 of 8192 (24).  Many short rows are enough by
 // themselves, and fewer wavefronts meet at a row's sum: 2048 rows of 4096 11.9 and 12.9.
+// Rows that do not lie at multiples of 16 bytes take the same way with a last lane of fewer elements, in four lengths: 2048 rows of
+// 4097 18 us, of 8190 26 (element by element 47 and 88).
 template <int XT>
 void launch_norm(const NormArgs& a, bool wide, hipStream_t s) {
   const int K = a.K;
-  if (!wide || K > 8 * 1024 * 4) {
+  if (K > 8 * 1024 * 4) {
     norm_any_kernel<XT><<<(unsigned)std::min(a.rows, 1 << 20), 256, 0, s>>>(a);
     return;
+  }
+  if (!wide) {
+    if (K <= 512) return launch_rows<XT, 64, 1, true>(a, s);
+    if (K <= 2048) return launch_rows<XT, 256, 1, true>(a, s);
+    if (K <= 8192) return launch_rows<XT, 1024, 1, true>(a, s);
+    return launch_rows<XT, 1024, 4, true>(a, s);
   }
   if (K <= 128) return launch_rows<XT, 16, 1>(a, s);
   if (K <= 256) return launch_rows<XT, 32, 1>(a, s);

@@ -107,7 +107,7 @@ def _norm_own(K, dtype):
 
 SIZES = [(1, 64), (3, 8), (5, 128), (1, 4096), (7, 200), (33, 256), (2, 512), (9, 1000), (4, 1024), (600, 2048), (5, 2560), (513, 4096),
          (520, 5120), (3, 8192), (515, 8192), (4, 9000), (514, 12000), (2, 16384), (3, 20000), (513, 32768), (2, 40000), (3, 77),
-         (2, 1), (5, 129), (3, 4099)]
+         (2, 1), (5, 129), (3, 4099), (600, 501), (5, 2047), (700, 8191), (3, 12345), (2, 32767), (3, 32769)]
 
 
 @pytest.mark.gpu
@@ -201,7 +201,7 @@ def test_norm_strides_shapes_and_streams():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("K", [128, 4096, 4100])
+@pytest.mark.parametrize("K", [128, 4096, 4100, 333, 9001])
 def test_norm_in_place(K):
     """The sum over the residual, the output over x: the C entry allows both."""
     import torch

@@ -268,7 +268,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(Args a) {
   }
   void* out = a.part ? (void*)(a.part + (int64_t)split * a.M * a.N) : a.y;
   const int yt = a.part ? (int)DT_F32 : a.y_dtype;
-  const bool vec = a.N % 4 == 0 && n + 3 < a.N;
+  const bool vec = n + 3 < a.N;  // one store at any element's address
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
 #pragma unroll
@@ -286,9 +286,12 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void tile_kernel(Args a) {
       const int64_t at = (int64_t)m * a.N + n;
       const float o[4] = {v[r][0] + bias[0], v[r][1] + bias[1], v[r][2] + bias[2], v[r][3] + bias[3]};
       if (vec) {
-        if (yt == DT_F32) *(f32x4_t*)((float*)out + at) = f32x4_t{o[0], o[1], o[2], o[3]};
-        else if (yt == DT_BF16) *(uint2*)((uint16_t*)out + at) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
-        else *(uint2*)((uint16_t*)out + at) = make_uint2(pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3]));
+        if (yt == DT_F32) {
+          __builtin_memcpy((float*)out + at, o, 16);
+        } else {
+          const uint2 h = yt == DT_BF16 ? make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])) : make_uint2(pack_f16x2(o[0], o[1]), pack_f16x2(o[2], o[3]));
+          __builtin_memcpy((uint16_t*)out + at, &h, 8);
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)

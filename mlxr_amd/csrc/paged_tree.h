@@ -19,13 +19,16 @@
 //
 // What bounds it: few columns, memory (16 drafts of 32 rows of 8192, 32 heads and 8 kv heads of 128, bf16: 223 us, 4.9 TB/s); many
 // columns, the vector unit's work on each score beside the matrix unit's two products (64 drafts of 8 rows of 16384, 64 heads, e4m3
-// cache: 335 us, 0.82 PFLOP/s; a chain of 513 over 6001 tokens 0.43); a few rows, the launches and the start of each
+// cache: 335 us, 0.82 PFLOP/s; a chain of 513 over 6001 tokens 0.46); a few rows, the launches and the start of each
 // workgroup (8 drafts of one row of 1000 14 us).
 //
 // The tiles of all (row, kv head, QB columns) are dealt to the workgroups of a launch that fills the device in equal
 // contiguous runs; a run that covers all of its columns' tiles writes the output, others leave (m, sum, unnormalized o) in
 // the workspace, at most two a workgroup, and a second launch joins them.  Short rows, or many (plan_of): a workgroup for
 // each (row, kv head, QB columns).
+//
+// A chain's block of columns ends with its last node's token, and what a wavefront's columns all see takes no mask, what they all do
+// not no products: a chain of 513 over 6001 tokens 119 -> 114 us, of 513 without context 44 -> 34.
 #pragma once
 #include <cfloat>
 #include <type_traits>
@@ -285,12 +288,21 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
     const int64_t in_row = pos - pre[r];
     const int span = row.tiles + kStart, unit = cut ? quotient(in_row, span) : (int)in_row, from = (int)(in_row - (int64_t)unit * span);
     const int places = cut ? (int)min((int64_t)(span - from), end - pos) : 0;  // of this run
-    const int first = cut ? max(from - kStart, 0) : 0, count = cut ? max(from + places - kStart, 0) - first : row.tiles;
-    if (cut && count == 0) {  // the run ends within a unit's first places
+    const int first = cut ? max(from - kStart, 0) : 0, dealt = cut ? max(from + places - kStart, 0) - first : row.tiles;
+    if (cut && dealt == 0) {  // the run ends within a unit's first places
       pos += places;
       continue;
     }
-    const int kvh = unit / row.blocks, block = unit - kvh * row.blocks;
+    const int kvh = unit / row.blocks, nth = unit - kvh * row.blocks, block = cut ? nth : row.blocks - 1 - nth;  // a chain's longest first
+    // Tokens below `full` are seen by all columns of the block (of this wavefront), those from `none` on by none.
+    const int columns = row.n * a.group, wave_column = block * T::QB + wave * CW * 16;
+    const bool idle = wave_column >= columns;  // the wavefront only brings tiles
+    auto last_node = [&](int column) { return a.by_group.quotient(min(column, columns) - 1); };
+    const int block_full = row.context + (a.mask ? 0 : a.by_group.quotient(block * T::QB) + 1);
+    const int full = row.context + (a.mask ? 0 : a.by_group.quotient(min(wave_column, columns - 1)) + 1);
+    const int none = a.mask ? INT32_MAX : row.context + last_node(wave_column + CW * 16) + 1;
+    const int block_none = a.mask ? INT32_MAX : max(row.context + last_node((block + 1) * T::QB) + 1, 0);
+    const int count = min(dealt, max((int)(((int64_t)block_none + TOK - 1) / TOK) - first, 0));  // of the tiles dealt, those that are seen
     const int32_t* trow = a.table + (int64_t)r * a.table_stride;
     const uint8_t *kh = a.k + (int64_t)kvh * a.k_head, *vh = a.v + (int64_t)kvh * a.v_head;
     // scores times sc, which is made positive by the queries' sign (and never 0: -inf stays -inf)
@@ -299,8 +311,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
     const uint32_t flip = signed_sc < 0.f ? 0x80008000u : 0u;
 
     // columns of this wavefront: (node, head) pairs; those past the row's last are node 0's with queries of 0
-    const int columns = row.n * a.group, first_column = block * T::QB + wave * CW * 16 + col;
-    const bool idle = block * T::QB + wave * CW * 16 >= columns;  // the wavefront only brings tiles
+    const int first_column = wave_column + col;
     int node[CW];
     Seen sees[CW];
     u32x4_t q[CW][KS];
@@ -426,7 +437,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
       pages_of(base);
       load(base);
       __syncthreads();  // the run before may still be read
-      const bool nodes = base + TOK > row.context, any = store(0, nodes);
+      const bool nodes = base + TOK > block_full, any = store(0, nodes);
       if (count > 1) {
         pages_of(base + TOK);
         load(base + TOK);
@@ -440,7 +451,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
       uint8_t *ks = lds + half * 2 * T::STORE, *vs = ks + T::STORE;
       constexpr uint64_t ALL = TOK < 64 ? (1ull << TOK) - 1 : ~0ull;
       const uint64_t valid = live & ALL;
-      const bool plain = t0 + TOK <= row.context && valid == ALL;
+      const bool plain = t0 + TOK <= full && valid == ALL;
       if (odd) {
         if (!idle)
 #pragma unroll
@@ -463,7 +474,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
         for (int i = tid; i < T::STORE / 4; i += THREADS) ((uint32_t*)vs)[i] = clean2<P16>(((uint32_t*)vs)[i]);
         __syncthreads();
       }
-      if (!idle) {
+      if (!idle && t0 < none) {
         // Reads of LDS go AHEAD steps before the products that take them, in the order written (sched_barrier): left to
         // itself the compiler saves registers and waits for each read.
         constexpr int AHEAD = T::AHEAD;
@@ -568,7 +579,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
       }
       if (t0 + TOK < stop) {
         half ^= 1;
-        const bool nodes = t0 + 2 * TOK > row.context, any = store(half, nodes);
+        const bool nodes = t0 + 2 * TOK > block_full, any = store(half, nodes);
         if (further) load(t0 + 2 * TOK);
         join_waves(half, nodes, any);
       }
@@ -582,7 +593,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
       l[j] += __shfl_xor(l[j], 32);
     }
     // ---- outputs, or this run's part of them
-    const bool whole = first == 0 && count == row.tiles;
+    const bool whole = first == 0 && dealt == row.tiles;
     {
       float* part_sums = whole ? nullptr : a.ws + ((int64_t)w * 2 + slot) * partial_floats(T::QB, a.dim);
 #pragma unroll

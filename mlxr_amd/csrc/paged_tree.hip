@@ -140,7 +140,8 @@ struct Plan {
   size_t bytes;   // of the workspace
 };
 constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 1) / 2 * 2 * sizeof(int64_t); }
-Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int width, int q_dtype, int out_dtype) {
+// chain: no mask; needs no more workspace than with one.
+Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int width, int q_dtype, int out_dtype, bool chain) {
   Plan p;
   const int group = heads / c->kv_heads;
   // on average, padding included; an eighth more than a block of columns is still taken as one
@@ -153,12 +154,15 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   if ((double)tokens * group / 16 * c->kv_heads * ((held + 63) / 64) < 96.0 * device_cu_count()) columns = std::min<int64_t>(columns, 64);
   p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), (int)held, out_dtype);
   p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
-  const int64_t tiles = (held + p.k.tok - 1) / p.k.tok;
+  int64_t tiles = (held + p.k.tok - 1) / p.k.tok;
   // Cut where the longest rows that the table holds are more than 3 tiles and 20 for each of a CU's units: what a launch without cuts
   // leaves idle while its longest unit ends grows with the row, the pieces and their join with the units.  us, cut and not, 16
   // drafts a row of 32 heads and 8 kv heads: one row (8 units) of 250 13.1 and 15.5, 8 rows of 250 21.8 and 16.8, of 1000 26 and 34; rows
   // spread over the lengths, 32 rows (256 units) of up to 500 26 and 24, of 2000 43 and 61, of 8192 123 and 211; 128 rows (1024 units) 56
   // and 47, 135 and 130, 389 and 457; of one length of 2000 32 rows 73 and 70, 128 rows of 4096 408 and 391.
+  // Rows that are mostly a chain have half as many tiles on average, and a cut would deal all of them: a prompt of 4096
+  // (512 units) cut 400, not 223.
+  if (chain && 2 * (int64_t)tokens > rows * held) tiles /= 2;
   const int64_t units = std::max((int64_t)tokens * group / p.k.qb, (int64_t)rows) * c->kv_heads;  // about
   p.cut = (tiles - 3) * device_cu_count() > 20 * units;
   p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
@@ -208,7 +212,7 @@ extern "C" int mlxr_paged_tree_attention_workspace_size(const mlxr_paged_cache* 
   if (!bytes) return set_error(MLXR_E_INVALID, "null bytes");
   if (const int rc = check_tree(cache, rows, tokens, heads, table_width)) return rc;
   if (const int rc = check_types(cache, q_dtype, out_dtype)) return rc;
-  *bytes = rows && tokens ? plan_of(cache, rows, tokens, heads, table_width, q_dtype, out_dtype).bytes : 0;
+  *bytes = rows && tokens ? plan_of(cache, rows, tokens, heads, table_width, q_dtype, out_dtype, false).bytes : 0;
   return MLXR_OK;
 }
 
@@ -226,7 +230,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   if (!q_dev || !table_dev || !lens_dev || !starts_dev || !out_dev) return set_error(MLXR_E_INVALID, "null buffer");
   if (q_token_stride % 8 || q_head_stride % 8 || (((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15))
     return set_error(MLXR_E_SHAPE, "paged_tree_attention: query rows, output and workspace must start at multiples of 16 bytes");
-  const Plan p = plan_of(cache, rows, tokens, heads, table_width, q_dtype, out_dtype);
+  const Plan p = plan_of(cache, rows, tokens, heads, table_width, q_dtype, out_dtype, !mask_dev);
   if (workspace_bytes < p.bytes || (p.bytes && !workspace_dev))
     return set_error(MLXR_E_INVALID, "paged_tree_attention: the workspace is smaller than mlxr_paged_tree_attention_workspace_size");
   const int es = cache->dtype == MLXR_E4M3 ? 1 : 2;

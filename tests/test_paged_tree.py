@@ -399,6 +399,37 @@ def test_what_is_not_seen_does_not_count(dtype, cache, heads, kv, dim, extra):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache,heads,dim", [("bf16", "bf16", 8, 128), ("f16", "f8", 14, 128), ("f16", "f16", 8, 64), ("bf16", "bf16", 4, 256)])
+@pytest.mark.parametrize("nodes,context,extra", [(1100, 0, 0), (700, 437, 0), (700, 70, 900), (65, 300, 100)])
+def test_chains_of_any_length(dtype, cache, heads, dim, nodes, context, extra):
+    """Nodes see themselves and what is before them, to the token: NaN in a node's value or key reaches it and those behind it only; a
+    row of more nodes than tokens has its first nodes before the first token."""
+    import torch
+    b = Batch([context, 5, 0], [nodes, 1, 130], heads, 2, dim, 16, dtype, cache, seed=15, extra=extra)
+    b.check(*b.call(out_dtype=_dt("f32"), return_lse=True), dtype=dtype)
+    want, group = b.call(), heads // 2
+    for node in (0, 1, nodes // 2, nodes // 2 + 63, nodes - 1):
+        if node >= nodes:
+            continue
+        pg, t = int(b.table[0, (context + node) // 16]), (context + node) % 16
+        for store in (b.v, b.k):
+            keep = store[pg, 1, t].clone()
+            store[pg, 1, t, 5] = math.nan
+            got = b.call()
+            assert torch.isnan(got[node:nodes, group:, 5]).all() and not torch.isnan(got[:node]).any()
+            got[node:nodes, group:] = torch.where(torch.isnan(got[node:nodes, group:]), want[node:nodes, group:], got[node:nodes, group:])
+            assert torch.equal(got, want)
+            store[pg, 1, t] = keep
+    b.lens[0] = max(nodes - 30, 1)  # the first nodes are in no cache: they see nothing, the others what is there
+    gone = nodes - b.lens[0]
+    got, lse = b.call(out_dtype=_dt("f32"), return_lse=True)
+    assert not got[:gone].any() and (lse[:gone] == -math.inf).all() and torch.isfinite(lse[gone:nodes]).all()
+    c = Batch([0], [nodes - gone], heads, 2, dim, 16, dtype, cache, seed=15, pad=0)
+    c.k, c.v, c.ks, c.vs, c.table, c.q = b.k, b.v, b.ks, b.vs, b.table[:1], b.q[gone:nodes].contiguous()
+    c.check(got[gone:nodes], lse[gone:nodes], dtype=dtype)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("extra", [0, 200])
 def test_bad_pages_lengths_and_starts(extra):
     """Tokens of pages outside the cache are left out; a row whose tokens all are, or that has none, gives zeros; lengths past

@@ -68,7 +68,7 @@ struct Args {
   int dim, page, pages, width, out_dtype, qb, tok;
   int step;  // pages of a tile where they are whole, else 0
   Divisor by_page, by_group;
-  int workers;
+  int workers, least;  // of a cut launch; a run is at least so many tiles
   float scale;  // times log2(e)
 };
 
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
       for (int64_t i = id; i < (int64_t)(a.tokens - behind) * a.heads; i += step) a.lse[(int64_t)behind * a.heads + i] = -INFINITY;
   }
   const int64_t total = pre[a.rows];
-  const int64_t per = cut ? (total + a.workers - 1) / a.workers : 1;
+  const int64_t per = cut ? max((total + a.workers - 1) / a.workers, (int64_t)a.least) : 1;
   if (cut && blockIdx.x == 0) {
     for (int r = tid; r <= a.rows; r += THREADS) a.prefix[r] = pre[r];
     if (tid == 0) a.prefix[a.rows + 1] = per;

@@ -1,6 +1,7 @@
 // Attention of drafted tokens over a paged cache: the C entries, the join of the pieces that the kernel (paged_tree.h)
 // leaves of cut rows, and the masks of trees.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "paged_tree.h"
@@ -137,6 +138,7 @@ struct Plan {
   TreeKern k;
   bool cut;
   int64_t units;  // at most: (row, kv head, QB columns)
+  int least;      // tiles of a run
   size_t bytes;   // of the workspace
 };
 constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 1) / 2 * 2 * sizeof(int64_t); }
@@ -165,6 +167,10 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   if (chain && 2 * (int64_t)tokens > rows * held) tiles /= 2;
   const int64_t units = std::max((int64_t)tokens * group / p.k.qb, (int64_t)rows) * c->kv_heads;  // about
   p.cut = (tiles - 3) * device_cu_count() > 20 * units;
+  // Few columns of a long row: runs of one tile would leave the join more pieces than it takes at once.  Its time goes with
+  // tiles / run / 16, that of a run with its tiles: least together at about the root.  us, runs of one tile and
+  // these, 4 drafts of one row, 8 heads and 2: of 10893 tokens (3) 32 and 20, of 32000 (6) 46 and 29.
+  p.least = std::max(1, (int)std::sqrt((double)tiles / 13));
   p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
   return p;
 }
@@ -266,7 +272,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   int64_t grid = p.units;
   if (p.cut) {
     grid = (int64_t)occ * device_cu_count();
-    a.workers = (int)grid;
+    a.workers = (int)grid, a.least = p.least;
     a.prefix = (int64_t*)workspace_dev, a.ws = (float*)((uint8_t*)workspace_dev + prefix_bytes(rows));
   }
   void* args[] = {&a};

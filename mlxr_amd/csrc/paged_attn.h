@@ -97,10 +97,15 @@ __device__ __forceinline__ uint32_t widen(uint32_t w) {
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, H));
 }
 
-// The larger of the 16-bit halves: of floats that are not negative, the larger float.
+// The larger and the smaller of the 16-bit halves: of floats that are not negative, the larger and smaller float.
 __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
   typedef __attribute__((ext_vector_type(2))) uint16_t V;
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b)));
+}
+
+__device__ __forceinline__ uint32_t pair_min(uint32_t a, uint32_t b) {
+  typedef __attribute__((ext_vector_type(2))) uint16_t V;
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b)));
 }
 
 // N (1, 2, 4) words at a multiple of 4 N bytes.

@@ -121,11 +121,12 @@ struct Seen {
   }
 };
 
-// Two weights in PARTS 16-bit parts that add up to them (the last rounded), none negative nor a later one 0: an infinite
-// value then gives an infinite output as a weight in one piece does, not NaN.
-template <bool P16, int PARTS>
+// Two weights in PARTS 16-bit parts that add up to them (the last rounded), none negative.  FLOOR, for caches whose values may be
+// infinite: nor a later one 0 where the first is not, so that an infinite value gives an infinite output as a weight in one piece
+// does, not NaN.  Parts of a weight of 0 are all 0: what a column does not see adds nothing to it, whatever its value.
+template <bool P16, int PARTS, bool FLOOR>
 __device__ __forceinline__ void split_parts(float p0, float p1, uint32_t (&out)[PARTS]) {
-  auto floor2 = [](uint32_t w) { return paged::pair_max(w, P16 ? 0x00010001u : 0x00800080u); };
+  auto floor2 = [&](uint32_t w) { return FLOOR ? paged::pair_max(w, paged::pair_min(out[0], P16 ? 0x00010001u : 0x00800080u)) : w; };
   if constexpr (P16) {
     if constexpr (PARTS == 1) {
       typedef __attribute__((ext_vector_type(2))) float f32x2;
@@ -537,7 +538,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][2 * h + 1], sc, off[j]));
           l[j] += p0 + p1;
           uint32_t out[PARTS];
-          split_parts<P16, PARTS>(p0, p1, out);
+          split_parts<P16, PARTS, !F8>(p0, p1, out);  // e4m3 has no infinities
 #pragma unroll
           for (int n = 0; n < PARTS; ++n) p[k][j][n][2 * (i & 1) + h] = out[n];
         };

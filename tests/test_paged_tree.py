@@ -551,3 +551,50 @@ def test_tree_masks(nodes, words):
     want = [10 * r + depth[starts[r] + j] for r, n in enumerate(drafts) for j in range(n)]
     assert pos.tolist() == want + [-1, -1]
     assert mx.tree_mask(_i32(parents + pad), _i32(starts), words)[1].tolist() == depth + [-1, -1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [0, 200])
+@pytest.mark.parametrize("dtype,cache,heads,kv,dim,large", [("bf16", "bf16", 8, 2, 128, 3e38), ("f16", "f16", 8, 2, 128, 65504.0), ("bf16", "f8", 8, 2, 128, 448.0),
+                                                          ("f16", "f16", 64, 2, 64, 65504.0), ("bf16", "bf16", 16, 1, 256, 1e38)])
+def test_large_values_that_are_not_seen_do_not_count(dtype, cache, heads, kv, dim, large, extra):
+    """The largest finite values in nodes: those that do not see them get the bits that zeros there give."""
+    import torch
+    b = Batch([37, 700], [20, 33], heads, kv, dim, 16, dtype, cache, seed=17, extra=extra)
+    rng = random.Random(2)
+    bits = []
+    for n in b.drafts:
+        bits += _tree(n, rng)[1]
+    for mask in (bits, None):  # trees and chains
+        for r, node in ((0, 7), (1, 0), (1, 20)):
+            pg, t = (int(b.table[r, (b.context[r] + node) // 16]), (b.context[r] + node) % 16)
+            keep, a = b.v[pg, :, t].clone(), b.starts[r]
+            got = []
+            for value in (0.0, large):
+                b.v[pg, :, t] = value
+                got.append(b.call(mask, 1, out_dtype=_dt("f32")))
+            b.v[pg, :, t] = keep
+            unseen = [i for i in range(b.starts[-1]) if not a <= i < b.starts[r + 1] or not (bits[i] >> node & 1 if mask else node <= i - a)]
+            assert torch.equal(got[0][unseen], got[1][unseen]) and len(unseen) < b.starts[-1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [0, 500])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (16, 1, 64)])
+def test_tokens_of_no_weight_add_nothing(heads, kv, dim, extra):
+    """Values of one at 4000 tokens whose weights are below 2^-40 of the largest add at most that much to what zeros there give: less
+    than the products keep of a weight (2^-22 of the largest), however many they are."""
+    import torch
+    b = Batch([4000], [5], heads, kv, dim, 16, "f16", "f16", seed=18, extra=extra)
+    b.k.zero_(), b.v.zero_(), b.q.zero_()
+    b.q[..., 0] = 1.0
+    page = b.table[0, 100 // 16]
+    b.k[..., 0] = -40.0
+    b.k[page, :, 100 % 16, 0] = 0.0  # token 100 has all the weight: the others exp(-40) = 2^-57 of it
+    b.v[page, :, 100 % 16, 1] = 1.0
+    want = b.call(scale=1.0, out_dtype=_dt("f32"))
+    assert (want[:5, :, 1] == 1).all()
+    b.v[..., 2] = 1.0
+    b.v[page, :, 100 % 16, 2] = 0.0
+    got = b.call(scale=1.0, out_dtype=_dt("f32"))
+    assert torch.equal(got[..., 1], want[..., 1]) and got[..., 2].abs().max().item() <= 4000 * 2.0 ** -40

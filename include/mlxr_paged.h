@@ -116,8 +116,8 @@ int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int heads, con
  * Tokens of pages outside the cache are left out, and nodes before a row's first token (n > lens[r]).  What a node does not
  * see does not reach it, whatever its bits.  rows up to MLXR_PAGED_MAX_ROWS, tokens * heads up to 2^26; head_dim, strides and
  * the rest as mlxr_paged_attention, without its limits on the distance of pages.  Sums, maxima and the output before
- * its rounding are fp32; weights enter their products with the values with 24 bits (bf16 cache, fp32 outputs), 16 (bf16 cache,
- * 16-bit outputs), 11 (e4m3 cache, bf16 outputs) or else 22. */
+ * its rounding are fp32, whatever the output's type; weights enter their products with the values with 24 bits (bf16 caches) or 22, less
+ * what lies below 2^-32 of the largest. */
 enum { MLXR_TREE_MAX_WORDS = 64 };
 int mlxr_paged_tree_attention_workspace_size(const mlxr_paged_cache* cache, int rows, int tokens, int heads, int table_width,
                                              int q_dtype, int out_dtype, size_t* bytes);

@@ -97,14 +97,14 @@ __device__ __forceinline__ uint32_t widen(uint32_t w) {
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, H));
 }
 
-// The larger and the smaller of the 16-bit halves: of floats that are not negative, the larger and smaller float.
+// The larger of the 16-bit halves: of floats that are not negative, the larger float.
 __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
   typedef __attribute__((ext_vector_type(2))) uint16_t V;
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b)));
 }
-
+// The smaller, of halves that are not negative (with a sign: the compiler makes comparisons and choices of one with 1 without).
 __device__ __forceinline__ uint32_t pair_min(uint32_t a, uint32_t b) {
-  typedef __attribute__((ext_vector_type(2))) uint16_t V;
+  typedef __attribute__((ext_vector_type(2))) int16_t V;
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b)));
 }
 

@@ -8,11 +8,11 @@
 //   S^T[tokens, columns] = K Q^T       K from LDS, Q in registers for the whole row
 //   O^T[dim, columns]   += V^T P^T     V^T by the transposing read of LDS, P from S^T without leaving the registers
 // Which token an element of the second product's 32 is, is free: lane group g's eight are tokens 4 g .. 4 g + 3 of two
-// neighbouring 16 x 16 tiles of S^T, as the first product leaves them.  P enters in 16-bit parts: f16 (and the values of an
-// e4m3 cache, exact in f16) two parts, 22 bits; bf16 three, 24 bits, for fp32 outputs, two, 16 bits, for 16-bit outputs, whose
-// own half step (2^-9, 2^-12) is far larger than what that leaves out of each weight (2^-17); an e4m3 cache with
-// bf16 outputs one, which leaves out 2^-12 of a weight, an eighth of the output's half step.  (Matrix instructions bound
-// wide trees, and each part is half as many as the first product takes.)
+// neighbouring 16 x 16 tiles of S^T, as the first product leaves them.  P enters in 16-bit parts that add up to it, as in decode
+// attention and for every output type: bf16 three, all 24 bits; f16 (and the values of an e4m3 cache, exact in f16) two, 22 bits.
+// A part takes as many matrix instructions as the first product.  us, with a bf16 cache two parts (16 bits) and these: 16 drafts of 16
+// ragged rows of up to 8192 73 and 76, a chain of 513 over 6001 112 and 132; with an e4m3 cache one (11 bits) and these: 64 drafts
+// of 8 ragged rows of up to 16384 153 and 176.  16-bit outputs have the bits of fp32 ones, rounded once.
 //
 // A tile of TOK tokens goes memory -> registers -> LDS, one tile ahead: while tile t is multiplied, t + 1 is on its way to
 // registers; it is written to the other half of LDS before the tile's one barrier.
@@ -121,32 +121,29 @@ struct Seen {
   }
 };
 
-// Two weights in PARTS 16-bit parts that add up to them (the last rounded), none negative.  FLOOR, for caches whose values may be
+// Two weights in 16-bit parts that add up to them (f16: the second rounded), none negative.  FLOOR, for caches whose values may be
 // infinite: nor a later one 0 where the first is not, so that an infinite value gives an infinite output as a weight in one piece
 // does, not NaN.  Parts of a weight of 0 are all 0: what a column does not see adds nothing to it, whatever its value.
-template <bool P16, int PARTS, bool FLOOR>
-__device__ __forceinline__ void split_parts(float p0, float p1, uint32_t (&out)[PARTS]) {
+template <bool P16, bool FLOOR>
+__device__ __forceinline__ void split_parts(float p0, float p1, uint32_t (&out)[P16 ? 2 : 3]) {
   auto floor2 = [&](uint32_t w) { return FLOOR ? paged::pair_max(w, paged::pair_min(out[0], P16 ? 0x00010001u : 0x00800080u)) : w; };
   if constexpr (P16) {
-    if constexpr (PARTS == 1) {
-      typedef __attribute__((ext_vector_type(2))) float f32x2;
-      typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-      out[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{p0, p1}), f16x2));
-    } else {
-      const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-      out[0] = hi;
-      out[1] = floor2(pack2<true>(p0 - unpack<true>(hi, 0), p1 - unpack<true>(hi, 1)));
-    }
+    typedef __attribute__((ext_vector_type(2))) float F;
+    typedef __attribute__((ext_vector_type(2))) _Float16 H;
+    const H hi = __builtin_bit_cast(H, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+    float minus = -1.f;
+    asm("" : "+s"(minus));  // not known to the compiler, which would widen hi and subtract: one instruction takes it as it is
+    out[0] = __builtin_bit_cast(uint32_t, hi);
+    out[1] = floor2(__builtin_bit_cast(uint32_t, __builtin_convertvector((F{__builtin_fmaf(hi[0], minus, p0), __builtin_fmaf(hi[1], minus, p1)}), H)));
   } else {
 #pragma unroll
-    for (int n = 0; n < PARTS - 1; ++n) {  // each the upper half of what is left
+    for (int n = 0; n < 3; ++n) {  // each the upper half of what is left; the last holds all of it
       const uint32_t b0 = __builtin_bit_cast(uint32_t, p0), b1 = __builtin_bit_cast(uint32_t, p1);
       const uint32_t w = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
       out[n] = n ? floor2(w) : w;
       p0 -= __builtin_bit_cast(float, b0 & 0xffff0000u);
       p1 -= __builtin_bit_cast(float, b1 & 0xffff0000u);
     }
-    out[PARTS - 1] = floor2(pack2<false>(p0, p1));
   }
 }
 
@@ -169,9 +166,10 @@ __device__ __forceinline__ uint32_t clean2(uint32_t w) {
 
 // DT: 64, 128 or 256, at least head_dim.  W: wavefronts.  CW: columns of a wavefront, by 16.  TOK: tokens of a tile (32, 64).  OCC: workgroups
 // that a CU's registers and LDS hold.
-template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC, int PARTS>
+template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC>
 struct Kern {
   static constexpr bool P16 = F16 || F8;                      // the second product's type, f16 or else bf16
+  static constexpr int PARTS = P16 ? 2 : 3;                   // of a weight
   static constexpr int THREADS = 64 * W, QB = 16 * CW * W;
   static constexpr int NT = TOK / 16, KT = TOK / 32, KS = DT / 32, ND = DT / 16;
   static constexpr int CH = DT / 8;                           // 16-byte pieces of a row in LDS
@@ -206,10 +204,10 @@ struct Kern {
   }
 };
 
-template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC, int PARTS>
+template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC>
 __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
-  using T = Kern<F16, F8, DT, W, CW, TOK, OCC, PARTS>;
-  constexpr int THREADS = T::THREADS, NT = T::NT, KT = T::KT, KS = T::KS, ND = T::ND, NL = T::NL;
+  using T = Kern<F16, F8, DT, W, CW, TOK, OCC>;
+  constexpr int THREADS = T::THREADS, NT = T::NT, KT = T::KT, KS = T::KS, ND = T::ND, NL = T::NL, PARTS = T::PARTS;
   constexpr bool P16 = T::P16;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -538,7 +536,7 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][2 * h + 1], sc, off[j]));
           l[j] += p0 + p1;
           uint32_t out[PARTS];
-          split_parts<P16, PARTS, !F8>(p0, p1, out);  // e4m3 has no infinities
+          split_parts<P16, !F8>(p0, p1, out);  // e4m3 has no infinities
 #pragma unroll
           for (int n = 0; n < PARTS; ++n) p[k][j][n][2 * (i & 1) + h] = out[n];
         };
@@ -635,30 +633,30 @@ struct TreeKern {
   std::atomic<int>* residents;  // workgroups of a CU, by device; 0: not asked yet
 };
 
-// The kernel for head_dim, about `columns` columns of a row, the longest row that the table holds and the type of the output.
+// The kernel for head_dim, about `columns` columns of a row and the longest row that the table holds.
 // Eight wavefronts share a tile where there are columns for them and rows are long: half as many loads, widenings and LDS writes
 // a column, but half as many workgroups.  us, four and eight: 64 drafts of 8 rows of 16384, e4m3, 350 and 335; of 8192, bf16, 167 and
 // 142; of 32 rows of 500 58 and 51; a chain of 513 tokens 55 and 48; but 64 drafts of 8 rows of 256 27 and 34.  Up to 64
 // columns, one group of 16 a wavefront: 16 drafts of 32 rows of 8192 (64 columns) 226, two groups 359.
-TreeKern kern_bf16(int dim, int columns, int longest, int out_dtype);
-TreeKern kern_f16(int dim, int columns, int longest, int out_dtype);
-TreeKern kern_bf16_e4m3(int dim, int columns, int longest, int out_dtype);
-TreeKern kern_f16_e4m3(int dim, int columns, int longest, int out_dtype);
+TreeKern kern_bf16(int dim, int columns, int longest);
+TreeKern kern_f16(int dim, int columns, int longest);
+TreeKern kern_bf16_e4m3(int dim, int columns, int longest);
+TreeKern kern_f16_e4m3(int dim, int columns, int longest);
 
-template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC, int PARTS>
+template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC>
 TreeKern kern_t() {
-  using T = Kern<F16, F8, DT, W, CW, TOK, OCC, PARTS>;
+  using T = Kern<F16, F8, DT, W, CW, TOK, OCC>;
   static std::atomic<int> residents[64];
-  return TreeKern{(const void*)tree_kernel<F16, F8, DT, W, CW, TOK, OCC, PARTS>, T::QB, TOK, T::LDS, T::THREADS, residents};
+  return TreeKern{(const void*)tree_kernel<F16, F8, DT, W, CW, TOK, OCC>, T::QB, TOK, T::LDS, T::THREADS, residents};
 }
-template <bool F16, bool F8, int PARTS>
+template <bool F16, bool F8>
 TreeKern kern_of(int dim, int columns, int longest) {
-  if (dim > 128) return kern_t<F16, F8, 256, 4, 1, 32, 2, PARTS>();
+  if (dim > 128) return kern_t<F16, F8, 256, 4, 1, 32, 2>();
   if (dim > 64) {
-    if (columns > 128 && longest > 512) return kern_t<F16, F8, 128, 8, 2, 64, 1, PARTS>();
-    return columns > 64 ? kern_t<F16, F8, 128, 4, 2, 64, 2, PARTS>() : kern_t<F16, F8, 128, 4, 1, 64, 2, PARTS>();
+    if (columns > 128 && longest > 512) return kern_t<F16, F8, 128, 8, 2, 64, 1>();
+    return columns > 64 ? kern_t<F16, F8, 128, 4, 2, 64, 2>() : kern_t<F16, F8, 128, 4, 1, 64, 2>();
   }
-  return columns > 64 ? kern_t<F16, F8, 64, 4, 2, 64, 2, PARTS>() : kern_t<F16, F8, 64, 4, 1, 64, 4, PARTS>();
+  return columns > 64 ? kern_t<F16, F8, 64, 4, 2, 64, 2>() : kern_t<F16, F8, 64, 4, 1, 64, 4>();
 }
 
 }  // namespace tree

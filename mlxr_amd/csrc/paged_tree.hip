@@ -124,10 +124,10 @@ __global__ __launch_bounds__(kThreads) void mask_kernel(MaskArgs a) {
   }
 }
 
-TreeKern kern(const mlxr_paged_cache* c, int q_dtype, int columns, int longest, int out_dtype) {
+TreeKern kern(const mlxr_paged_cache* c, int q_dtype, int columns, int longest) {
   const bool f16 = q_dtype == MLXR_F16;
-  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, columns, longest, out_dtype) : kern_bf16_e4m3(c->head_dim, columns, longest, out_dtype);
-  return f16 ? kern_f16(c->head_dim, columns, longest, out_dtype) : kern_bf16(c->head_dim, columns, longest, out_dtype);
+  if (c->dtype == MLXR_E4M3) return f16 ? kern_f16_e4m3(c->head_dim, columns, longest) : kern_bf16_e4m3(c->head_dim, columns, longest);
+  return f16 ? kern_f16(c->head_dim, columns, longest) : kern_bf16(c->head_dim, columns, longest);
 }
 
 constexpr int kMaxHeads = 1 << 26;  // tokens times heads: a launch has fewer than 2^32 threads
@@ -143,7 +143,7 @@ struct Plan {
 };
 constexpr size_t prefix_bytes(int rows) { return (size_t)(rows + 2 + 1) / 2 * 2 * sizeof(int64_t); }
 // chain: no mask; needs no more workspace than with one.
-Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int width, int q_dtype, int out_dtype, bool chain) {
+Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int width, int q_dtype, bool chain) {
   Plan p;
   const int group = heads / c->kv_heads;
   // on average, padding included; an eighth more than a block of columns is still taken as one
@@ -154,7 +154,7 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   // up to 1806, 8 heads and 2 (70) 35 and 30; but 64 of 16 rows of up to 500, 64 heads and 8 (144) 36 and 39, of 32 rows of 500, 32
   // heads and 8 (144) 51 and 63.
   if ((double)tokens * group / 16 * c->kv_heads * ((held + 63) / 64) < 96.0 * device_cu_count()) columns = std::min<int64_t>(columns, 64);
-  p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), (int)held, out_dtype);
+  p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), (int)held);
   p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
   int64_t tiles = (held + p.k.tok - 1) / p.k.tok;
   // Cut where the longest rows that the table holds are more than 3 tiles and 20 for each of a CU's units: what a launch without cuts
@@ -218,7 +218,7 @@ extern "C" int mlxr_paged_tree_attention_workspace_size(const mlxr_paged_cache* 
   if (!bytes) return set_error(MLXR_E_INVALID, "null bytes");
   if (const int rc = check_tree(cache, rows, tokens, heads, table_width)) return rc;
   if (const int rc = check_types(cache, q_dtype, out_dtype)) return rc;
-  *bytes = rows && tokens ? plan_of(cache, rows, tokens, heads, table_width, q_dtype, out_dtype, false).bytes : 0;
+  *bytes = rows && tokens ? plan_of(cache, rows, tokens, heads, table_width, q_dtype, false).bytes : 0;
   return MLXR_OK;
 }
 
@@ -236,7 +236,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   if (!q_dev || !table_dev || !lens_dev || !starts_dev || !out_dev) return set_error(MLXR_E_INVALID, "null buffer");
   if (q_token_stride % 8 || q_head_stride % 8 || (((uintptr_t)q_dev | (uintptr_t)out_dev | (uintptr_t)workspace_dev) & 15))
     return set_error(MLXR_E_SHAPE, "paged_tree_attention: query rows, output and workspace must start at multiples of 16 bytes");
-  const Plan p = plan_of(cache, rows, tokens, heads, table_width, q_dtype, out_dtype, !mask_dev);
+  const Plan p = plan_of(cache, rows, tokens, heads, table_width, q_dtype, !mask_dev);
   if (workspace_bytes < p.bytes || (p.bytes && !workspace_dev))
     return set_error(MLXR_E_INVALID, "paged_tree_attention: the workspace is smaller than mlxr_paged_tree_attention_workspace_size");
   const int es = cache->dtype == MLXR_E4M3 ? 1 : 2;

@@ -3,8 +3,6 @@
 
 namespace mlxr {
 namespace tree {
-TreeKern kern_bf16(int dim, int columns, int longest, int out_dtype) {
-  return out_dtype == MLXR_F32 ? kern_of<false, false, 3>(dim, columns, longest) : kern_of<false, false, 2>(dim, columns, longest);
-}
+TreeKern kern_bf16(int dim, int columns, int longest) { return kern_of<false, false>(dim, columns, longest); }
 }  // namespace tree
 }  // namespace mlxr

@@ -3,8 +3,6 @@
 
 namespace mlxr {
 namespace tree {
-TreeKern kern_bf16_e4m3(int dim, int columns, int longest, int out_dtype) {
-  return out_dtype == MLXR_BF16 ? kern_of<false, true, 1>(dim, columns, longest) : kern_of<false, true, 2>(dim, columns, longest);
-}
+TreeKern kern_bf16_e4m3(int dim, int columns, int longest) { return kern_of<false, true>(dim, columns, longest); }
 }  // namespace tree
 }  // namespace mlxr

@@ -3,8 +3,6 @@
 
 namespace mlxr {
 namespace tree {
-TreeKern kern_f16(int dim, int columns, int longest, int) {
-  return kern_of<true, false, 2>(dim, columns, longest);
-}
+TreeKern kern_f16(int dim, int columns, int longest) { return kern_of<true, false>(dim, columns, longest); }
 }  // namespace tree
 }  // namespace mlxr

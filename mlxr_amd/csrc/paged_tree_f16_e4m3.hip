@@ -3,8 +3,6 @@
 
 namespace mlxr {
 namespace tree {
-TreeKern kern_f16_e4m3(int dim, int columns, int longest, int out_dtype) {
-  return out_dtype == MLXR_BF16 ? kern_of<true, true, 1>(dim, columns, longest) : kern_of<true, true, 2>(dim, columns, longest);
-}
+TreeKern kern_f16_e4m3(int dim, int columns, int longest) { return kern_of<true, true>(dim, columns, longest); }
 }  // namespace tree
 }  // namespace mlxr

@@ -598,3 +598,53 @@ def test_tokens_of_no_weight_add_nothing(heads, kv, dim, extra):
     b.v[page, :, 100 % 16, 2] = 0.0
     got = b.call(scale=1.0, out_dtype=_dt("f32"))
     assert torch.equal(got[..., 1], want[..., 1]) and got[..., 2].abs().max().item() <= 4000 * 2.0 ** -40
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache,heads,kv,dim", [("bf16", "bf16", 32, 8, 128), ("f16", "f16", 8, 1, 64), ("bf16", "f8", 16, 2, 128), ("f16", "f8", 16, 4, 64),
+                                                     ("f16", "f16", 6, 2, 256), ("bf16", "bf16", 16, 1, 112)])
+@pytest.mark.parametrize("drafts,context,extra", [([3], [70], 0), ([9, 40], [100, 64], 0), ([150], [600], 0), ([20, 65], [2000, 64], 300)])
+def test_16_bit_outputs_are_the_32_bit_ones_rounded(dtype, cache, heads, kv, dim, drafts, context, extra):
+    """Nothing within depends on the output's type."""
+    rng = random.Random(dim)
+    b = Batch(context, drafts, heads, kv, dim, 16, dtype, cache, seed=19, extra=extra)
+    bits = []
+    for n in drafts:
+        bits += _tree(n, rng)[1]
+    import torch
+    for mask in (bits, None):
+        got = b.call(mask, 3, out_dtype=_dt("f32"))
+        for odt in ("bf16", "f16"):
+            assert torch.equal(b.call(mask, 3, out_dtype=_dt(odt)), got.to(_dt(odt)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f8"), ("f16", "f8")])
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("nodes,context,extra", [(1, 64, 0), (9, 100, 0), (40, 700, 0), (70, 700, 0), (9, 100, 300), (70, 2000, 300)])
+def test_weights_keep_their_bits(dtype, cache, heads, kv, dim, nodes, context, extra):
+    """Values that are one at one token each read single weights off, relative to token 0's.  Scores are exact (products of a few bits),
+    above -4, and 0 at the first token of each tile, which the weights are relative to.  A weight is off by ln 2 times what its exponent is (2^-23 of 4
+    for the scale times log2(e) in fp32, 2^-22 for the rounding of the sum), the exponential's 2^-23, as is token 0's, 2^-22 for its parts and
+    2^-24 for each of two outputs: 2.5 * 2^-21.  One part less would be off by 2^-12 or 2^-17."""
+    import torch
+    b = Batch([context], [nodes], heads, kv, dim, 16, dtype, cache, seed=20, extra=extra, pad=0)
+    b.ks = b.vs = None
+    t = torch.arange(b.lens[0])
+    page, at, j = b.table[0, t // 16].long().cuda(), (t % 16).cuda(), (t % 32).cuda()
+    keys, values = (torch.zeros((len(t), kv, dim), device="cuda") for _ in range(2))
+    keys[..., 0], keys[..., 1] = -(j // 8)[:, None].float(), -(j % 8)[:, None] / 8
+    values[t[:64], :, t[:64]] = 1.0
+    for store, x in ((b.k, keys), (b.v, values)):
+        whole = torch.zeros(store.shape, device="cuda")
+        whole[page, :, at] = x
+        store.copy_(whole.to(store.dtype))
+    q = 0.5 + torch.arange(nodes * heads, device="cuda").view(nodes, heads) * 37 % 128 / 256
+    b.q.zero_()
+    b.q[..., 0] = b.q[..., 1] = q.to(b.q.dtype)
+    scale = float(torch.tensor(math.log(2.0)))
+    want = torch.exp(-scale * q.double()[..., None] * (torch.arange(64, device="cuda") % 32).double() / 8)
+    for mask in (None, [(1 << nodes) - 1] * nodes):
+        got = b.call(mask, 2, scale=scale, out_dtype=_dt("f32")).double()
+        off = (got[..., :64] / got[..., :1] / want - 1).abs()
+        assert off.max().item() <= 2.5 * 2.0 ** -21, off.max().item() * 2.0 ** 21

@@ -11,7 +11,8 @@ namespace tree {
 namespace {
 
 // One token's head for each `lanes` threads, four dims a thread: o = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w over the
-// workgroups w that had a piece of its columns, M the maximum of their m (-inf: no token counted).  Rows without
+// workgroups w that had a piece of its columns, M the maximum of their m (-inf: no token counted); the factors are never 0, so that
+// an infinite sum stays infinite, as in the kernel (pieces that counted nothing are zeros).  Rows without
 // tokens get zeros; columns that one workgroup covered are done.  Four pieces are on their way at
 // once, MANY: 16 where there are more.
 template <bool MANY>
@@ -58,14 +59,14 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
       float top = m;
 #pragma unroll
       for (int k = 0; k < N; ++k) top = fmaxf(top, pm[k]);
-      const float ref = top == -INFINITY ? 0.f : top, f0 = __builtin_amdgcn_exp2f(m - ref);
+      const float ref = top == -INFINITY ? 0.f : top, f0 = fmaxf(__builtin_amdgcn_exp2f(m - ref), FLT_MIN);
       m = top;
       l *= f0;
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] *= f0;
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float f = __builtin_amdgcn_exp2f(pm[k] - ref);
+        const float f = fmaxf(__builtin_amdgcn_exp2f(pm[k] - ref), FLT_MIN);
         l += pl[k] * f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] += po[k][e] * f;

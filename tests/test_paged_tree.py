@@ -648,3 +648,27 @@ def test_weights_keep_their_bits(dtype, cache, heads, kv, dim, nodes, context, e
         got = b.call(mask, 2, scale=scale, out_dtype=_dt("f32")).double()
         off = (got[..., :64] / got[..., :1] / want - 1).abs()
         assert off.max().item() <= 2.5 * 2.0 ** -21, off.max().item() * 2.0 ** 21
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,extra", [(1, 0), (1, 300), (260, 0), (700, 0)])  # cut differently; a workgroup for each block of columns
+@pytest.mark.parametrize("low", [5, 1500])  # the infinite value's token, at the start and before the middle
+def test_an_infinite_value_counts_however_far_below(dtype, rows, extra, low):
+    """Scores of 0 up to a token with an infinite value, of 400 behind: the output is infinite where the row is one workgroup's and
+    where it is cut between them."""
+    import torch
+    b = Batch([2900] + [4] * (rows - 1), [3] * rows, 4, 1, 128, 16, dtype, dtype, seed=21, extra=extra)
+    t = torch.arange(b.lens[0])
+    page, at = b.table[0, t // 16].long().cuda(), (t % 16).cuda()
+    b.q.zero_()
+    b.q[..., 0] = 20.0
+    b.k[page, :, at] = 0.0
+    high = (t > 1600).cuda()
+    b.k[page[high], :, at[high], 0] = 20.0
+    want = b.call(scale=1.0, out_dtype=_dt("f32"))
+    b.v[page[low], :, at[low], 7] = math.inf
+    got = b.call(scale=1.0, out_dtype=_dt("f32"))
+    assert (got[:3, :, 7] == math.inf).all()
+    got[:3, :, 7] = want[:3, :, 7]
+    assert torch.equal(got, want) and torch.isfinite(want).all()

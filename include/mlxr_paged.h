@@ -109,7 +109,8 @@ int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int heads, con
  * included; without a mask nodes 0 .. i (a chain: the next part of a prompt).
  *   q_dev          [tokens, heads, head_dim] of q_dtype (as mlxr_paged_attention), strides in elements, multiples of 16
  *                  bytes; queries from starts[rows] on are padding
- *   starts_dev     [rows + 1] int32, ascending from 0 (mlxr_page_resize gives them)
+ *   starts_dev     [rows + 1] int32, ascending from 0 (mlxr_page_resize gives them); may go past tokens: nodes from there on
+ *                  count in n but have no query (what is not listed was not written: masks should not name it)
  *   mask_dev       [tokens, words] of 64 bits, or NULL; nodes from 64 * words on are seen by none
  *   out_dev        [tokens, heads, head_dim] contiguous; padding and nodes that see nothing are zeros
  *   lse_dev        [tokens, heads] fp32 or NULL: as mlxr_paged_attention

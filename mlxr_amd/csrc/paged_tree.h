@@ -72,19 +72,20 @@ struct Args {
   float scale;  // times log2(e)
 };
 
-// A row: its drafted tokens are n tokens from `start` on, the last of its len cached ones.
+// A row: its drafted tokens are n tokens from `start` on, the first of those behind its context; starts may go past the listed
+// tokens (page_resize lists no more than it is given places for), its len cached ones hold the others too.
 struct Row {
   int start, n, len, context, blocks, tiles;
 };
 __device__ __forceinline__ Row row_of(const Args& a, int r) {
   Row w;
   const int64_t most = (int64_t)a.width * a.page;
-  const int s0 = min(max(a.starts[r], 0), a.tokens), s1 = min(max(a.starts[r + 1], s0), a.tokens);
-  const int len = a.lens[r];
+  const int u0 = max(a.starts[r], 0), u1 = max(a.starts[r + 1], u0), s0 = min(u0, a.tokens), s1 = min(u1, a.tokens);
+  const int len = max(a.lens[r], 0);
   w.start = s0;
   w.n = s1 - s0;
-  w.context = len - w.n;  // may be negative: the first nodes are then not in the cache
-  w.len = len < 0 ? 0 : len > most ? (int)most : len;
+  w.context = len - (u1 - u0);  // may be negative: the first nodes are then not in the cache
+  w.len = len > most ? (int)most : len;
   w.blocks = (int)(((int64_t)w.n * a.group + a.qb - 1) / a.qb);
   w.tiles = (w.len + a.tok - 1) / a.tok;
   return w;

@@ -672,3 +672,49 @@ def test_an_infinite_value_counts_however_far_below(dtype, rows, extra, low):
     assert (got[:3, :, 7] == math.inf).all()
     got[:3, :, 7] = want[:3, :, 7]
     assert torch.equal(got, want) and torch.isfinite(want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("extra", [0, 300])
+@pytest.mark.parametrize("dtype,cache,heads,kv,dim", [("bf16", "bf16", 8, 2, 128), ("f16", "f16", 16, 1, 64), ("bf16", "f8", 8, 2, 128)])
+@pytest.mark.parametrize("cut", [1, 5, 37, 60])
+def test_starts_past_the_tokens(dtype, cache, heads, kv, dim, cut, extra):
+    """page_resize lists no more tokens than it is given places for, but counts all in starts and lengths: the listed queries of the row
+    where the list ends are its first nodes, and what was not written (NaN here) reaches nobody."""
+    import torch
+    rng = random.Random(cut)
+    whole = Batch([30, 300, 7], [20, 40, 3], heads, kv, dim, 16, dtype, cache, seed=22, extra=extra, pad=0)
+    b = Batch(whole.context, [min(n, max(0, cut - s)) for n, s in zip(whole.drafts, whole.starts)], heads, kv, dim, 16, dtype, cache, seed=22, pad=0)
+    b.k, b.v, b.ks, b.vs, b.table, b.q = whole.k, whole.v, whole.ks, whole.vs, whole.table, whole.q[:cut].contiguous()
+    for r, n in enumerate(b.drafts):
+        for i in range(n, whole.drafts[r]):
+            pg, t = int(b.table[r, (b.context[r] + i) // 16]), (b.context[r] + i) % 16
+            b.k[pg, :, t], b.v[pg, :, t] = math.nan, math.nan
+    bits = []
+    for n in b.drafts:
+        bits += _tree(n, rng)[1]
+    for listed in (bits, None):
+        mask = None if listed is None else _words(listed, 1)
+        got = mx.paged_tree_attention(b.q, b.k, b.v, b.table.cuda(), _i32(whole.lens), _i32(whole.starts), mask, k_scale=b.ks, v_scale=b.vs,
+                                      out_dtype=_dt("f32"), return_lse=True)
+        b.check(*got, listed, 1, dtype=dtype)
+
+
+@pytest.mark.gpu
+def test_a_list_shorter_than_the_drafts():
+    """The same through PagedKVCache.resize: the chain that there is room for gives what it gives alone."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(23)
+    k, v = (torch.randn((12, 2, 64), device="cuda", generator=g).bfloat16() for _ in range(2))
+    q = torch.randn((9, 4, 64), device="cuda", generator=g).bfloat16()
+    got = []
+    for want in (9, 14):  # of the second no more than 9 are listed
+        cache = mx.PagedKVCache(1, 8, 16, 2, 64, 1, 64)
+        cache.k.fill_(math.nan), cache.v.fill_(math.nan)
+        first = cache.resize(_i32([3]), 3)
+        cache.append(0, k[9:], v[9:], first.slots)
+        grown = cache.resize(_i32([3 + want]), 9)
+        cache.append(0, k[:9], v[:9], grown.slots)
+        assert grown.starts.tolist() == [0, want]
+        got.append(cache.attend_tree(0, q, grown.starts))
+    assert torch.isfinite(got[0]).all() and torch.equal(*got)

@@ -115,8 +115,8 @@ int mlxr_paged_attention(const mlxr_paged_cache* cache, int rows, int heads, con
  *   out_dev        [tokens, heads, head_dim] contiguous; padding and nodes that see nothing are zeros
  *   lse_dev        [tokens, heads] fp32 or NULL: as mlxr_paged_attention
  * Tokens of pages outside the cache are left out, and nodes before a row's first token (n > lens[r]).  What a node does not
- * see does not reach it, whatever its bits.  rows up to MLXR_PAGED_MAX_ROWS, tokens * heads up to 2^26; head_dim, strides and
- * the rest as mlxr_paged_attention, without its limits on the distance of pages.  Sums, maxima and the output before
+ * see does not reach it, whatever its bits.  rows up to MLXR_PAGED_MAX_ROWS, rows * kv_heads up to 2^22, tokens * heads
+ * up to 2^26 (less, with head_dim above 128); head_dim, strides and the rest as mlxr_paged_attention, without its limits on the distance of pages.  Sums, maxima and the output before
  * its rounding are fp32, whatever the output's type; weights enter their products with the values with 24 bits (bf16 caches) or 22, less
  * what lies below 2^-32 of the largest. */
 enum { MLXR_TREE_MAX_WORDS = 64 };

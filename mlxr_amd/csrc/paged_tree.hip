@@ -131,7 +131,15 @@ TreeKern kern(const mlxr_paged_cache* c, int q_dtype, int columns, int longest) 
   return f16 ? kern_f16(c->head_dim, columns, longest) : kern_bf16(c->head_dim, columns, longest);
 }
 
-constexpr int kMaxHeads = 1 << 26;  // tokens times heads: a launch has fewer than 2^32 threads
+// A launch has fewer than 2^32 threads: the join at most 64 for each of tokens times heads, the kernel 512 for each 64 of them and
+// for each row's kv heads.
+constexpr int kMaxHeads = 1 << 26, kMaxRowHeads = 1 << 22;
+// Threads of the join that share a token's head.
+int join_lanes(int dim) {
+  int lanes = 2;
+  while (4 * lanes < dim) lanes *= 2;
+  return lanes;
+}
 constexpr int kGridPerCu = 4;
 
 // How a call runs.
@@ -182,7 +190,10 @@ int check_tree(const mlxr_paged_cache* c, int rows, int tokens, int heads, int w
   if (heads % c->kv_heads) return set_error(MLXR_E_SHAPE, "heads must be a multiple of kv_heads");
   if (rows > kMaxRows) return set_error(MLXR_E_SHAPE, "paged_tree_attention: at most %d rows", kMaxRows);
   if ((int64_t)width * c->page_size > INT32_MAX - 1024) return set_error(MLXR_E_SHAPE, "paged_tree_attention: the table covers too many tokens");
-  if ((int64_t)tokens * heads > kMaxHeads) return set_error(MLXR_E_SHAPE, "paged_tree_attention: at most %d tokens times heads", kMaxHeads);
+  if ((int64_t)tokens * heads > kMaxHeads - (join_lanes(c->head_dim) > 32))
+    return set_error(MLXR_E_SHAPE, "paged_tree_attention: at most %d tokens times heads", kMaxHeads - (join_lanes(c->head_dim) > 32));
+  if ((int64_t)rows * c->kv_heads > kMaxRowHeads)
+    return set_error(MLXR_E_SHAPE, "paged_tree_attention: at most %d rows times kv heads", kMaxRowHeads);
   return MLXR_OK;
 }
 int check_types(const mlxr_paged_cache* c, int q_dtype, int out_dtype) {
@@ -279,8 +290,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   void* args[] = {&a};
   e = hipLaunchKernel(p.k.fn, dim3((unsigned)grid), dim3(p.k.threads), args, (size_t)lds, st);
   if (e == hipSuccess && p.cut) {
-    int lanes = 2;
-    while (4 * lanes < a.dim) lanes *= 2;
+    const int lanes = join_lanes(a.dim);
     const unsigned blocks = (unsigned)(((int64_t)tokens * heads * lanes + kThreads - 1) / kThreads);
     // A few workgroups wait for memory: more at once, though fewer fit a CU.  us of a call, 4 and 16: 8 drafts of one row of 1000 16.3
     // and 13.9, 76 of 3 rows of up to 7391, 4 heads of 256 44 and 35; 64 of 8 rows of 8192 142 and 148.

@@ -49,6 +49,22 @@ def test_refusals():
     assert mask(tokens=0) == 0 and mask(starts=0) == -1 and mask(parents=0) == -1 and mask(out=0) == -1
 
 
+def test_launches_too_large_are_refused():
+    """Sizes whose launch would have 2^32 threads or more, and the largest below."""
+    L, n = paged._lib(), ctypes.c_size_t()
+
+    def size(rows, tokens, heads, kv, dim=128, width=4):
+        c = _cache(kv_heads=kv, head_dim=dim)
+        return L.mlxr_paged_tree_attention_workspace_size(ctypes.byref(c), rows, tokens, heads, width, mx.BF16, mx.BF16, ctypes.byref(n))
+    assert size(4096, 4096, 1024, 1024) == 0 and size(1024, 4, 4096, 4096) == 0
+    assert size(4096, 4096, 4096, 4096) == -3 and size(4096, 1, 1025, 1025) == -3 and size(1025, 4, 4096, 4096) == -3
+    assert "kv heads" in L.mlxr_qgemm_last_error().decode()
+    assert size(1, 1 << 23, 8, 8) == 0 and size(1, 1 << 23, 8, 8, dim=136) == -3 and size(1, (1 << 23) - 1, 8, 8, dim=256) == 0
+    c = _cache(kv_heads=4096)
+    assert L.mlxr_paged_tree_attention(ctypes.byref(c), 4096, 1, 4096, P(64), mx.BF16, 4096 * 128, 128, P(64), 4, 4, P(64), P(64), P(64), 1, 0.1,
+                                       P(64), mx.BF16, None, P(64), 1 << 40, None) == -3
+
+
 def test_wrapper_refusals():
     import torch
     k, t = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16), torch.zeros((2, 3), dtype=torch.int32)

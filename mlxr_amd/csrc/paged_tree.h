@@ -630,8 +630,8 @@ __global__ __launch_bounds__(64 * W, OCC) void tree_kernel(Args a) {
 
 struct TreeKern {
   const void* fn;
-  int qb, tok, lds, threads;
-  std::atomic<int>* residents;  // workgroups of a CU, by device; 0: not asked yet
+  int qb, tok, lds, threads, occ;  // occ: workgroups of a CU at most, which the workspace goes by
+  std::atomic<int>* residents;     // workgroups of a CU, by device; 0: not asked yet
 };
 
 // The kernel for head_dim, about `columns` columns of a row and the longest row that the table holds.
@@ -648,7 +648,7 @@ template <bool F16, bool F8, int DT, int W, int CW, int TOK, int OCC>
 TreeKern kern_t() {
   using T = Kern<F16, F8, DT, W, CW, TOK, OCC>;
   static std::atomic<int> residents[64];
-  return TreeKern{(const void*)tree_kernel<F16, F8, DT, W, CW, TOK, OCC>, T::QB, TOK, T::LDS, T::THREADS, residents};
+  return TreeKern{(const void*)tree_kernel<F16, F8, DT, W, CW, TOK, OCC>, T::QB, TOK, T::LDS, T::THREADS, OCC, residents};
 }
 template <bool F16, bool F8>
 TreeKern kern_of(int dim, int columns, int longest) {

@@ -140,7 +140,6 @@ int join_lanes(int dim) {
   while (4 * lanes < dim) lanes *= 2;
   return lanes;
 }
-constexpr int kGridPerCu = 4;
 
 // How a call runs.
 struct Plan {
@@ -180,7 +179,7 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   // tiles / run / 16, that of a run with its tiles: least together at about the root.  us, runs of one tile and
   // these, 4 drafts of one row, 8 heads and 2: of 10893 tokens (3) 32 and 20, of 32000 (6) 46 and 29.
   p.least = std::max(1, (int)std::sqrt((double)tiles / 13));
-  p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * kGridPerCu * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
+  p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * p.k.occ * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
   return p;
 }
 
@@ -278,7 +277,7 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
     e = hipFuncSetAttribute(p.k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == hipSuccess) e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&occ, p.k.fn, p.k.threads, p.k.lds + 1024);
     if (e != hipSuccess) return set_error(MLXR_E_HIP, "paged_tree_attention: %s", hipGetErrorString(e));
-    occ = std::max(1, std::min(occ, kGridPerCu));
+    occ = std::max(1, std::min(occ, p.k.occ));
     residents.store(occ, std::memory_order_release);
   }
   int64_t grid = p.units;

@@ -65,6 +65,15 @@ def test_launches_too_large_are_refused():
                                        P(64), mx.BF16, None, P(64), 1 << 40, None) == -3
 
 
+def test_workspace_holds_what_can_be_written():
+    """Two partial sums (columns x head_dim, and two floats a column) for each workgroup that a CU holds, of 256 CUs, and the rows' tiles."""
+    L, n = paged._lib(), ctypes.c_size_t()
+    for dim, tokens, columns, resident in ((128, 513, 256, 1), (128, 100, 128, 2), (128, 4, 64, 2), (64, 4, 64, 4), (64, 513, 128, 2), (256, 4, 64, 2)):
+        c = _cache(head_dim=dim, kv_heads=8)
+        assert L.mlxr_paged_tree_attention_workspace_size(ctypes.byref(c), 4 if tokens == 100 else 1, tokens, 32, 3000, mx.BF16, mx.BF16, ctypes.byref(n)) == 0
+        assert 0 < n.value <= 256 * resident * 2 * columns * (dim + 2) * 4 + 64, (dim, tokens, n.value)
+
+
 def test_wrapper_refusals():
     import torch
     k, t = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16), torch.zeros((2, 3), dtype=torch.int32)

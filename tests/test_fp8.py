@@ -331,6 +331,44 @@ def test_product_in_every_kernel(kind, m, n, k, splits):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", range(0, 8))
+@pytest.mark.parametrize("m,n,k", [(1, 64, 28672), (17, 100, 400), (61, 257, 2048), (300, 520, 1040), (130, 70, 8192)])
+def test_products_of_small_integers_are_exact(kind, m, n, k):
+    """Products up to 4 and scales that are powers of two: neither the instruction of 8 bits nor sums in fp32 round anything (sums are
+    multiples of 2^-2 below 2^21), so every output is the exact one rounded once.  One product lost or counted twice shows."""
+    import torch
+    g = _gen(m + k)
+    x, w = (torch.randint(-2, 3, (r, k), device="cuda", generator=g).float() for r in (m, n))
+    xs = 2.0 ** torch.randint(-1, 2, (m, -(-k // BLOCK)), device="cuda", generator=g)
+    ws = 2.0 ** torch.randint(-1, 2, (-(-n // BLOCK), -(-k // BLOCK)), device="cuda", generator=g)
+    xq, wq = mx.Fp8Rows(x.to(torch.float8_e4m3fn), xs), mx.Fp8Weight(w.to(torch.float8_e4m3fn), ws)
+    want = _full(xq.data, xs, False) @ _full(wq.data, ws, True).t()
+    L = fp8._lib()
+    for splits in (1, 3):
+        assert L.mlxr_fp8_test_force(kind, splits) == 0
+        try:
+            for dtype in (torch.float32, torch.bfloat16, torch.float16):
+                assert torch.equal(mx.fp8_matmul(xq, wq, out_dtype=dtype), want.to(dtype)), dtype
+        finally:
+            L.mlxr_fp8_test_force(0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(17, 512, 1024), (61, 1024, 8192), (300, 512, 4096), (2048, 2048, 2048), (33, 256, 28672)])
+def test_products_of_16_bit_outputs_as_a_whole(m, n, k):
+    """The norm of the error: half a step of the output, and of the instruction of 8 bits what it drops of the seven smaller of eight
+    products, each a part of 2^-13 of the largest that is evenly spread (2^-13 / sqrt(3) rms) and of either sign: sqrt(7 / 3) 2^-13 of the
+    largest, which of eight products of normal numbers is 2.5 times their size on average, beside their sum, sqrt(8) times it: 1.4 * 2^-13,
+    so 2^-12 is allowed.  A product lost is sqrt(1 / K), 48 * 2^-13 at 28672."""
+    import torch
+    x, w = _activations(m, k, m), _weights(n, k, n)
+    want = _full(x.data, x.scales, False) @ _full(w.data, w.scales, True).t()
+    for dtype in (torch.bfloat16, torch.float16):
+        y = mx.fp8_matmul(x, w, out_dtype=dtype).double()
+        assert ((y - want).norm() / want.norm()).item() <= _half_step(dtype) + 2.0 ** -12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", range(0, 8))
 def test_product_knows_every_code(kind):
     """One-hot rows read single weights off, of every one of the 256 codes (both zeros, the values below the normal ones, NaN)."""
     import torch

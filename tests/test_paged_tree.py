@@ -743,3 +743,21 @@ def test_a_list_shorter_than_the_drafts():
         assert grown.starts.tolist() == [0, want]
         got.append(cache.attend_tree(0, q, grown.starts))
     assert torch.isfinite(got[0]).all() and torch.equal(*got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,cache,heads,kv,dim", [("bf16", "bf16", 8, 2, 128), ("f16", "f16", 16, 2, 64), ("bf16", "f8", 64, 2, 128), ("f16", "f8", 8, 4, 256)])
+@pytest.mark.parametrize("scale", [-0.07, 0.0, -0.0, 0.2, 1e-30])
+@pytest.mark.parametrize("context,extra", [([45, 7], 0), ([2500, 7], 200)])
+def test_scales_of_any_sign(dtype, cache, heads, kv, dim, scale, context, extra):
+    """Negative scales, none at all, and of an e4m3 cache one negative scale among the keys' and one among the values'."""
+    rng = random.Random(3)
+    b = Batch(context, [21, 40], heads, kv, dim, 16, dtype, cache, seed=24, extra=extra)
+    if cache == "f8":
+        b.ks[0] *= -1
+        b.vs[1] *= -1
+    bits = []
+    for n in b.drafts:
+        bits += _tree(n, rng)[1]
+    b.check(*b.call(bits, 1, scale=scale, out_dtype=_dt("f32"), return_lse=True), bits, 1, scale=scale, dtype=dtype)
+    b.check(*b.call(scale=scale, out_dtype=_dt("f32"), return_lse=True), scale=scale, dtype=dtype)

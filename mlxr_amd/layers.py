@@ -69,6 +69,9 @@ class Linear:
         """x W^T (+ b); with ``lora`` (a LoraBank of this layer's shape) and ``adapter_ids`` [tokens] (int32,
         -1: none) also each token's own adapter (lora_apply).  An 8-bit weight also takes x as ``Fp8Rows`` [M, in_features]
         (rms_norm's), giving bfloat16, without adapters; other x it rounds to 8 bits first."""
+        if stream is not None:  # copies of rows that lie apart and intermediate results are that stream's too
+            with qgemm._torch().cuda.stream(stream):
+                return self.forward(x, lora=lora, adapter_ids=adapter_ids)
         if self.weight is None:
             raise QGemmError(-1, "Linear: weight not loaded")
         if (lora is None) != (adapter_ids is None):
@@ -81,7 +84,7 @@ class Linear:
         if isinstance(x, Fp8Rows):
             if not eight or lora is not None:
                 raise QGemmError(-1, "Linear: rows in 8 bits need an 8-bit weight and take no adapters")
-            return fp8.fp8_matmul(x, self.weight, bias=self.bias, stream=stream)
+            return fp8.fp8_matmul(x, self.weight, bias=self.bias)
         if x.dim() < 1 or x.shape[-1] != self.in_features:
             raise QGemmError(-3, "Input shape must be [..., in_features]")
         lead = x.shape[:-1]
@@ -90,12 +93,12 @@ class Linear:
             M *= int(d)
         x2 = x.reshape(M, self.in_features)
         if eight:
-            y = fp8.fp8_matmul(x2, self.weight, bias=self.bias, stream=stream)
+            y = fp8.fp8_matmul(x2, self.weight, bias=self.bias)
         else:
             y = qgemm.q_gemm_dequant(x2, self.weight, M, self.out_features, self.in_features, self.weight.qtype,
-                                     bias=self.bias, stream=stream)
+                                     bias=self.bias)
         if lora is not None:
-            y = lora.apply(x2, adapter_ids, y, out=y, stream=stream)
+            y = lora.apply(x2, adapter_ids, y, out=y)
         return y.reshape(*lead, self.out_features)
 
     __call__ = forward
@@ -115,6 +118,9 @@ class MLP:
         self._ws = None
 
     def forward(self, x, stream=None):
+        if stream is not None:  # as in Linear
+            with qgemm._torch().cuda.stream(stream):
+                return self.forward(x)
         gw, uw, dw = self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight
         rows = isinstance(x, Fp8Rows)
         if not rows and (x.dim() < 1 or x.shape[-1] != self.hidden_size):
@@ -122,21 +128,21 @@ class MLP:
         if gw is None or uw is None or dw is None:
             raise QGemmError(-1, "MLP: weights not loaded")
         if rows or isinstance(gw, Fp8Weight) or isinstance(uw, Fp8Weight) or isinstance(dw, Fp8Weight):
-            return self._forward8(x, rows, stream)
+            return self._forward8(x, rows)
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.hidden_size)
         if (gw.qtype, gw.N) == (uw.qtype, uw.N):
             if self._ws is None:
                 self._ws = qgemm.MlpWorkspace(x.device)
-            y = qgemm.q_gemm_mlp(x2, gw, uw, dw, self._ws, stream=stream)
+            y = qgemm.q_gemm_mlp(x2, gw, uw, dw, self._ws)
         else:
-            g = self.gate_proj.forward(x2, stream=stream)
-            u = self.up_proj.forward(x2, stream=stream)
-            h = swiglu(g, u, out=g, stream=stream)
-            y = self.down_proj.forward(h, stream=stream)
+            g = self.gate_proj.forward(x2)
+            u = self.up_proj.forward(x2)
+            h = swiglu(g, u, out=g)
+            y = self.down_proj.forward(h)
         return y.reshape(*lead, self.hidden_size)
 
-    def _forward8(self, x, rows, stream):
+    def _forward8(self, x, rows):
         """forward where at least one weight is 8-bit, or x is Fp8Rows."""
         gate, up = self.gate_proj, self.up_proj
         both = isinstance(gate.weight, Fp8Weight) and isinstance(up.weight, Fp8Weight)
@@ -144,12 +150,12 @@ class MLP:
             raise QGemmError(-1, "MLP: rows in 8 bits need 8-bit gate and up weights")
         if both:
             lead, dtype = ((x.data.shape[0],), None) if rows else (x.shape[:-1], x.dtype)
-            x8 = x if rows else fp8.quantize_fp8(x, stream=stream)
-            g, u = (fp8.fp8_matmul(x8, p.weight, out_dtype=dtype, stream=stream) for p in (gate, up))
+            x8 = x if rows else fp8.quantize_fp8(x)
+            g, u = (fp8.fp8_matmul(x8, p.weight, out_dtype=dtype) for p in (gate, up))
         else:
             lead, x2 = x.shape[:-1], x.reshape(-1, self.hidden_size)
-            g, u = gate.forward(x2, stream=stream), up.forward(x2, stream=stream)
-        h = swiglu(g, u, out=g, stream=stream)
-        return self.down_proj.forward(h, stream=stream).reshape(*lead, self.hidden_size)
+            g, u = gate.forward(x2), up.forward(x2)
+        h = swiglu(g, u, out=g)
+        return self.down_proj.forward(h).reshape(*lead, self.hidden_size)
 
     __call__ = forward

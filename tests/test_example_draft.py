@@ -134,6 +134,36 @@ def test_layers_with_8_bit_weights(cuda, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["8 bits", "gguf", "8 bits and gguf"])
+def test_layers_work_on_the_given_stream_alone(cuda, kind):
+    """Rows that lie apart are copied, and intermediate results made and freed, on the call's stream: it does not see what the current
+    stream still has to do, nor does that stream's later work take their memory."""
+    import torch
+    g = torch.Generator().manual_seed(2)
+
+    def load(layer, n, k, eight):
+        if eight:
+            return layer.load_weight(mx.quantize_fp8_weight((torch.randn(n, k, generator=g) * k ** -0.5).to(torch.bfloat16).to(cuda)))
+        return layer.load_weight(mx.synth_gguf(mx.QuantType.Q8_0, n, k, n), mx.QuantType.Q8_0, device=cuda)
+    lin, mlp = load(mx.Linear(512, 384), 384, 512, kind != "gguf"), mx.MLP(512, 1024)
+    load(mlp.gate_proj, 1024, 512, kind != "gguf"), load(mlp.up_proj, 1024, 512, kind == "8 bits"), load(mlp.down_proj, 512, 1024, kind == "8 bits")
+    x = torch.randn(70, 2, 512, generator=g).to(torch.bfloat16).to(cuda).transpose(0, 1)
+    big = torch.randn(8192, 8192, device=cuda)
+    want, side = (lin(x), mlp(x)), torch.cuda.Stream()
+    big @ big
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for _ in range(4):
+            big @ big  # some 50 ms of the current stream's
+        got = lin(x, stream=side), mlp(x, stream=side)
+        for n in (70 * 2 * 1024, 70 * 2 * 512, 70 * 2 * 384):  # memory of the sizes that the calls had in between
+            torch.full((n,), 7.0, device=cuda, dtype=torch.bfloat16)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_a_captured_pass_follows_its_inputs(cuda):
     """A whole pass (pages, masks, layers, accepted paths, a fork) captured once and replayed with other lengths, trees, tokens and
     paths, the program's own calls in between, gives the bits of the same calls made one by one."""

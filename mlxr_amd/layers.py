@@ -108,7 +108,8 @@ class MLP:
     """down(swish(gate(x)) * up(x)) through mlxr_qgemm_mlp: at M = 1 the whole block is one
     launch; above, the fused gate/up/gating launch and the down projection.  The layer holds
     the workspace (sync words, h, split-K partials).  With 8-bit weights (Fp8Weight) x is rounded to 8 bits once
-    for gate and up, or comes as ``Fp8Rows``, and the gated rows once for down."""
+    for gate and up, or comes as ``Fp8Rows``, and the gated rows once for down.  Projections built with a bias
+    are run one by one."""
 
     def __init__(self, hidden_size, intermediate_size):
         self.hidden_size, self.intermediate_size = hidden_size, intermediate_size
@@ -131,7 +132,8 @@ class MLP:
             return self._forward8(x, rows)
         lead = x.shape[:-1]
         x2 = x.reshape(-1, self.hidden_size)
-        if (gw.qtype, gw.N) == (uw.qtype, uw.N):
+        biases = self.gate_proj.has_bias or self.up_proj.has_bias or self.down_proj.has_bias
+        if (gw.qtype, gw.N) == (uw.qtype, uw.N) and not biases:
             if self._ws is None:
                 self._ws = qgemm.MlpWorkspace(x.device)
             y = qgemm.q_gemm_mlp(x2, gw, uw, dw, self._ws)
@@ -150,8 +152,10 @@ class MLP:
             raise QGemmError(-1, "MLP: rows in 8 bits need 8-bit gate and up weights")
         if both:
             lead, dtype = ((x.data.shape[0],), None) if rows else (x.shape[:-1], x.dtype)
+            if any(p.has_bias and p.bias is None for p in (gate, up)):
+                raise QGemmError(-1, "MLP: bias not set")
             x8 = x if rows else fp8.quantize_fp8(x)
-            g, u = (fp8.fp8_matmul(x8, p.weight, out_dtype=dtype) for p in (gate, up))
+            g, u = (fp8.fp8_matmul(x8, p.weight, bias=p.bias, out_dtype=dtype) for p in (gate, up))
         else:
             lead, x2 = x.shape[:-1], x.reshape(-1, self.hidden_size)
             g, u = gate.forward(x2), up.forward(x2)

@@ -164,6 +164,35 @@ def test_layers_work_on_the_given_stream_alone(cuda, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("eight", [True, False])
+def test_projections_of_an_mlp_keep_their_biases(cuda, eight):
+    import torch
+    g = torch.Generator().manual_seed(3)
+    mlp, parts = mx.MLP(256, 512), []
+    for name, n, k in (("gate_proj", 512, 256), ("up_proj", 512, 256), ("down_proj", 256, 512)):
+        lin = mx.Linear(k, n, bias=True)
+        if eight:
+            lin.load_weight(mx.quantize_fp8_weight((torch.randn(n, k, generator=g) * k ** -0.5).to(torch.bfloat16).to(cuda)))
+        else:
+            lin.load_weight(mx.synth_gguf(mx.QuantType.Q8_0, n, k, n + len(name)), mx.QuantType.Q8_0, device=cuda)
+        setattr(mlp, name, lin)
+        parts.append(lin)
+    x = torch.randn(9, 256, generator=g).to(torch.bfloat16).to(cuda)
+    with pytest.raises(mx.QGemmError, match="bias not set"):
+        mlp(x)
+    for lin in parts:
+        lin.set_bias(torch.randn(lin.out_features, generator=g).to(cuda))
+    gate, up, down = parts
+    want = down(mx.swiglu(gate(x), up(x)))
+    assert torch.equal(mlp(x), want)
+    if eight:
+        assert torch.equal(mlp(mx.quantize_fp8(x)), want)
+    for lin in parts:
+        lin.bias = torch.zeros_like(lin.bias)
+    assert not torch.equal(mlp(x), want)
+
+
+@pytest.mark.gpu
 def test_a_captured_pass_follows_its_inputs(cuda):
     """A whole pass (pages, masks, layers, accepted paths, a fork) captured once and replayed with other lengths, trees, tokens and
     paths, the program's own calls in between, gives the bits of the same calls made one by one."""

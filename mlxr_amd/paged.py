@@ -23,6 +23,7 @@ from .qgemm import BF16, F16, F32, QGemmError
 
 E4M3 = 3
 MAX_ROWS = 4096
+MAX_WORDS = 64  # of a tree's mask
 
 _I64, _P, _I = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
 
@@ -243,7 +244,7 @@ def tree_mask(parents, starts, words, positions=None, stream=None):
     n, rows = parents.shape[0], starts.shape[0] - 1
     pp, ps = _vector(parents, n, "parents", index), _vector(starts, rows + 1, "starts", index)
     px = None if positions is None else _vector(positions, n, "positions", index)
-    mask = _on(stream, _torch.empty, (n, words if words > 0 else 1), dtype=_torch.int64, device=parents.device)
+    mask = _on(stream, _torch.empty, (n, words if 0 < words <= MAX_WORDS else 1), dtype=_torch.int64, device=parents.device)
     out = _on(stream, _torch.empty, n, dtype=_int32, device=parents.device)
     qgemm._check(lib.mlxr_tree_mask(rows, n, ps, pp, px, words, mask.data_ptr(), out.data_ptr(), _stream(stream, index)))
     return mask, out

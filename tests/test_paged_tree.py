@@ -761,3 +761,11 @@ def test_scales_of_any_sign(dtype, cache, heads, kv, dim, scale, context, extra)
         bits += _tree(n, rng)[1]
     b.check(*b.call(bits, 1, scale=scale, out_dtype=_dt("f32"), return_lse=True), bits, 1, scale=scale, dtype=dtype)
     b.check(*b.call(scale=scale, out_dtype=_dt("f32"), return_lse=True), scale=scale, dtype=dtype)
+
+
+@pytest.mark.gpu
+def test_masks_of_too_many_words_are_refused():
+    """Before memory for them is asked for."""
+    for words in (65, 1 << 30, 0, -1):
+        with pytest.raises(mx.QGemmError):
+            mx.tree_mask(_i32([-1] * 4096), _i32([0, 4096]), words)

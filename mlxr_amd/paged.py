@@ -373,8 +373,9 @@ class PagedKVCache:
         shape = (layers, num_pages, kv_heads, page_size, head_dim)
         dtype = dtype or torch.bfloat16
         self.page_size, self.k_scale, self.v_scale = page_size, k_scale, v_scale
-        self.k = torch.empty(shape, dtype=dtype, device=device)
-        self.v = torch.empty(shape, dtype=dtype, device=device)
+        # zeros: tokens that are counted before they are written (more than `resize` lists) attend to nothing of other owners of the memory
+        self.k = torch.zeros(shape, dtype=dtype, device=device)
+        self.v = torch.zeros(shape, dtype=dtype, device=device)
         i32 = {"dtype": torch.int32, "device": device}
         self.table = torch.full((rows, -(-max_tokens // page_size)), -1, **i32)
         self.lens = torch.zeros(rows, **i32)

@@ -769,3 +769,17 @@ def test_masks_of_too_many_words_are_refused():
     for words in (65, 1 << 30, 0, -1):
         with pytest.raises(mx.QGemmError):
             mx.tree_mask(_i32([-1] * 4096), _i32([0, 4096]), words)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["bf16", "f16", "f8"])
+def test_a_new_cache_holds_nothing_of_the_memorys_last_owner(cache):
+    import torch
+    for _ in range(3):
+        old = [torch.full((2, 60, 2, 16, 128), math.nan, device="cuda").to(_dt(cache)) for _ in range(2)]
+        del old
+        c = mx.PagedKVCache(2, 60, 16, 2, 128, 2, 400, dtype=_dt(cache))
+        assert not c.k.float().any() and not c.v.float().any()
+        c.resize(_i32([40, 7]), 3)
+        q = torch.ones((2, 4, 128), dtype=torch.float16 if cache == "f16" else torch.bfloat16, device="cuda")
+        assert not c.attend(0, q).any()

@@ -17,10 +17,10 @@
 // A tile of TOK tokens goes memory -> registers -> LDS, one tile ahead: while tile t is multiplied, t + 1 is on its way to
 // registers; it is written to the other half of LDS before the tile's one barrier.
 //
-// What bounds it: few columns, memory (16 drafts of 32 rows of 8192, 32 heads and 8 kv heads of 128, bf16: 223 us, 4.9 TB/s); many
+// What bounds it: few columns, memory (16 drafts of 32 rows of 8192, 32 heads and 8 kv heads of 128, bf16: 220 us, 4.9 TB/s); many
 // columns, the vector unit's work on each score beside the matrix unit's two products (64 drafts of 8 rows of 16384, 64 heads, e4m3
-// cache: 335 us, 0.82 PFLOP/s; a chain of 513 over 6001 tokens 0.46); a few rows, the launches and the start of each
-// workgroup (8 drafts of one row of 1000 14 us).
+// cache: 388 us, 0.71 PFLOP/s; a chain of 513 over 6001 tokens 0.39); a few rows, the launches and the start of each
+// workgroup (8 drafts of one row of 1000 14.5 us).
 //
 // The tiles of all (row, kv head, QB columns) are dealt to the workgroups of a launch that fills the device in equal
 // contiguous runs; a run that covers all of its columns' tiles writes the output, others leave (m, sum, unnormalized o) in
@@ -28,7 +28,7 @@
 // each (row, kv head, QB columns).
 //
 // A chain's block of columns ends with its last node's token, and what a wavefront's columns all see takes no mask, what they all do
-// not no products: a chain of 513 over 6001 tokens 119 -> 114 us, of 513 without context 44 -> 34.
+// not no products: a chain of 513 over 6001 tokens 139 -> 136 us, of 513 alone 34 -> 23, of 4096 over 400 609 -> 317.
 #pragma once
 #include <cfloat>
 #include <type_traits>
@@ -45,8 +45,8 @@ using paged::widen;
 constexpr int kThreads = 256;  // of the join and the masks
 constexpr int kMaxRows = MLXR_PAGED_MAX_ROWS;
 // Tiles that the start and the end of a row's columns (queries, outputs or partial sums) are counted for in the deal.  us at 0, 2, 4 and 8:
-// 64 drafts of 8 ragged rows of up to 16384, e4m3, 180, 159, 152 and 155; a chain of 513 over 6001 126, 122, 118 and 122; 16 drafts of 16
-// ragged rows of up to 8192 82, 74, 72 and 74.
+// 64 drafts of 8 ragged rows of up to 16384, e4m3, 206, 184, 179 and 184; a chain of 513 over 6001 138, 135, 136 and 138; 16 drafts of 16
+// ragged rows of up to 8192 85, 77, 75 and 76.
 constexpr int kStart = 4;
 
 struct Args {
@@ -635,10 +635,12 @@ struct TreeKern {
 };
 
 // The kernel for head_dim, about `columns` columns of a row and the longest row that the table holds.
-// Eight wavefronts share a tile where there are columns for them and rows are long: half as many loads, widenings and LDS writes
-// a column, but half as many workgroups.  us, four and eight: 64 drafts of 8 rows of 16384, e4m3, 350 and 335; of 8192, bf16, 167 and
-// 142; of 32 rows of 500 58 and 51; a chain of 513 tokens 55 and 48; but 64 drafts of 8 rows of 256 27 and 34.  Up to 64
-// columns, one group of 16 a wavefront: 16 drafts of 32 rows of 8192 (64 columns) 226, two groups 359.
+// Eight wavefronts of two groups of 16 columns share a tile where there are columns for them and rows are long: a quarter of the loads,
+// widenings and LDS writes a column that four of one group have, but a quarter as many workgroups.  us, four (64 columns) and eight (256): 64
+// drafts of 8 rows of 16384, e4m3, 495 and 387; of 8192, bf16, 182 and 155; of 32 rows of 1000 98 and 81, of 500 59 and 51; a chain of 513
+// over 6001 148 and 135; but 64 drafts of 128 ragged rows of up to 300 100 and 114, of 8 rows of 256 17 and 29.  Four wavefronts of two groups
+// need more than the 256 registers there are and lose at every size between: 32 drafts of 16 ragged rows of up to 8192 (128 columns) 102, with two
+// groups 120; of 64 rows of up to 2048 116 and 147; 64 drafts of 64 rows of up to 500 69 and 87.  Heads of up to 64 dims have registers for two.
 TreeKern kern_bf16(int dim, int columns, int longest);
 TreeKern kern_f16(int dim, int columns, int longest);
 TreeKern kern_bf16_e4m3(int dim, int columns, int longest);
@@ -654,8 +656,7 @@ template <bool F16, bool F8>
 TreeKern kern_of(int dim, int columns, int longest) {
   if (dim > 128) return kern_t<F16, F8, 256, 4, 1, 32, 2>();
   if (dim > 64) {
-    if (columns > 128 && longest > 512) return kern_t<F16, F8, 128, 8, 2, 64, 1>();
-    return columns > 64 ? kern_t<F16, F8, 128, 4, 2, 64, 2>() : kern_t<F16, F8, 128, 4, 1, 64, 2>();
+    return columns > 128 && longest > 512 ? kern_t<F16, F8, 128, 8, 2, 64, 1>() : kern_t<F16, F8, 128, 4, 1, 64, 2>();
   }
   return columns > 64 ? kern_t<F16, F8, 64, 4, 2, 64, 2>() : kern_t<F16, F8, 64, 4, 1, 64, 4>();
 }

@@ -157,27 +157,27 @@ Plan plan_of(const mlxr_paged_cache* c, int rows, int tokens, int heads, int wid
   // on average, padding included; an eighth more than a block of columns is still taken as one
   int64_t columns = (int64_t)tokens * group / rows * 8 / 9;
   const int64_t held = (int64_t)width * c->page_size;
-  // Little work (tiles of 16 columns by 64 tokens, for a CU) wants many workgroups rather than few reads of a tile: us, wide kernels
-  // and the one of 64 columns, 64 drafts of 8 rows of 256, 32 heads and 8 kv heads (16) 27 and 17, a chain of 513 (36) 48 and 44, 145 of 8 rows of
-  // up to 1806, 8 heads and 2 (70) 35 and 30; but 64 of 16 rows of up to 500, 64 heads and 8 (144) 36 and 39, of 32 rows of 500, 32
-  // heads and 8 (144) 51 and 63.
+  // Little work (tiles of 16 columns by 64 tokens, for a CU) wants many workgroups rather than few reads of a tile: us, 256 columns and
+  // 64, a chain of 513 over 600 (72), 32 heads and 8 kv heads, 54 and 41; 64 drafts of one row of 8192 (64) 45 and 41; 145 of 8 rows of up to 1806,
+  // 8 heads and 2 (40) 40 and 31; but 64 drafts of 32 rows of 1000 (256) 81 and 98, of 8 rows of 8192 (512) 155 and 182.  Ragged rows in between lose a
+  // little by it: 64 drafts of 16 rows of up to 2048 (170) 69 and 63.
   if ((double)tokens * group / 16 * c->kv_heads * ((held + 63) / 64) < 96.0 * device_cu_count()) columns = std::min<int64_t>(columns, 64);
   p.k = kern(c, q_dtype, (int)std::min<int64_t>(columns, 1 << 20), (int)held);
   p.units = ((int64_t)tokens * group / p.k.qb + rows) * c->kv_heads;
   int64_t tiles = (held + p.k.tok - 1) / p.k.tok;
   // Cut where the longest rows that the table holds are more than 3 tiles and 20 for each of a CU's units: what a launch without cuts
   // leaves idle while its longest unit ends grows with the row, the pieces and their join with the units.  us, cut and not, 16
-  // drafts a row of 32 heads and 8 kv heads: one row (8 units) of 250 13.1 and 15.5, 8 rows of 250 21.8 and 16.8, of 1000 26 and 34; rows
-  // spread over the lengths, 32 rows (256 units) of up to 500 26 and 24, of 2000 43 and 61, of 8192 123 and 211; 128 rows (1024 units) 56
-  // and 47, 135 and 130, 389 and 457; of one length of 2000 32 rows 73 and 70, 128 rows of 4096 408 and 391.
+  // drafts a row of 32 heads and 8 kv heads: one row (8 units) of 250 13.8 and 15.4, 8 rows of 250 21 and 16, of 1000 27 and 38; rows
+  // spread over the lengths, 32 rows (256 units) of up to 500 29 and 25, of 2000 44 and 66, of 8192 119 and 234; 128 rows (1024 units) 59
+  // and 48, 129 and 137, 383 and 485; of one length of 2000 32 rows 78 and 73, 128 rows of 1000 130 and 117, of 4096 423 and 409.
   // Rows that are mostly a chain have half as many tiles on average, and a cut would deal all of them: a prompt of 4096
-  // (512 units) cut 400, not 223.
+  // (512 units) cut 498, not 276.
   if (chain && 2 * (int64_t)tokens > rows * held) tiles /= 2;
   const int64_t units = std::max((int64_t)tokens * group / p.k.qb, (int64_t)rows) * c->kv_heads;  // about
   p.cut = (tiles - 3) * device_cu_count() > 20 * units;
   // Few columns of a long row: runs of one tile would leave the join more pieces than it takes at once.  Its time goes with
   // tiles / run / 16, that of a run with its tiles: least together at about the root.  us, runs of one tile and
-  // these, 4 drafts of one row, 8 heads and 2: of 10893 tokens (3) 32 and 20, of 32000 (6) 46 and 29.
+  // these, 4 drafts of one row, 8 heads and 2: of 10893 tokens (3) 33 and 22, of 32000 (6) 47 and 32.
   p.least = std::max(1, (int)std::sqrt((double)tiles / 13));
   p.bytes = p.cut ? prefix_bytes(rows) + (size_t)device_cu_count() * p.k.occ * 2 * partial_floats(p.k.qb, c->head_dim) * sizeof(float) : 0;
   return p;
@@ -291,8 +291,8 @@ extern "C" int mlxr_paged_tree_attention(const mlxr_paged_cache* cache, int rows
   if (e == hipSuccess && p.cut) {
     const int lanes = join_lanes(a.dim);
     const unsigned blocks = (unsigned)(((int64_t)tokens * heads * lanes + kThreads - 1) / kThreads);
-    // A few workgroups wait for memory: more at once, though fewer fit a CU.  us of a call, 4 and 16: 8 drafts of one row of 1000 16.3
-    // and 13.9, 76 of 3 rows of up to 7391, 4 heads of 256 44 and 35; 64 of 8 rows of 8192 142 and 148.
+    // A few workgroups wait for memory: more at once, though fewer fit a CU.  us of a call, 4 and 16: 8 drafts of one row of 1000 16.8
+    // and 14.6, 76 of 3 rows of up to 7391, 4 heads of 256 47 and 41; 64 of 8 rows of 8192 156 and 157.
     const auto join = blocks <= 2 * (unsigned)device_cu_count() ? join_kernel<true> : join_kernel<false>;
     join<<<blocks, kThreads, (rows + 1) * sizeof(int), st>>>(a, lanes);
     e = hipGetLastError();

@@ -250,7 +250,8 @@ __global__ __launch_bounds__(256) void norm_any_kernel(NormArgs a) {
   }
 }
 
-// Weights: a workgroup a block of 128 x 128, 64 elements a thread.
+// Weights: a workgroup a block of 128 x 128, 64 elements a thread.  Once for each weight of a model: 28672 x 8192 in bf16 644 us, 1.1 TB/s
+// (two-byte loads).
 template <int XT>
 __global__ __launch_bounds__(256) void weight_kernel(const void* w, int N, int K, int blocks, uint8_t* out, float* scales) {
   __shared__ float part[4];

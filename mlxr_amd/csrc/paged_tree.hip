@@ -83,7 +83,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int lanes) {
   if (a.lse && x == 0) a.lse[at] = (m + __builtin_amdgcn_logf(l)) * 0.69314718055994531f;
 }
 
-// A token's ancestors: one thread walks from each node to its root, by the parents of the row in LDS where they fit.
+// A token's ancestors: one thread walks from each node to its root, by the parents of the row in LDS where they fit.  Bound by the deepest
+// node's walk: 64 rows of 16 nodes 2.7 us, a tree of 4096 209, a chain of 513 82, of 4096 3077 (chains need no mask).
 struct MaskArgs {
   const int32_t *starts, *parents, *positions;
   uint64_t* mask;
